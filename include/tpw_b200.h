@@ -46,7 +46,9 @@ enum tpw_dtype {
     TPW_F32 = 0,
     TPW_F64 = 1,
     TPW_I32 = 2, /* accepted by tpw_cmp_reduce_forward only */
-    TPW_I64 = 3  /* accepted by tpw_cmp_reduce_forward only */
+    TPW_I64 = 3, /* accepted by tpw_cmp_reduce_forward only */
+    TPW_F16 = 4, /* accepted by the attention and rotary entry points only */
+    TPW_BF16 = 5 /* likewise */
 };
 
 /* ---- library ------------------------------------------------------------------------------ */
@@ -581,6 +583,67 @@ TPW_API int tpw_prf_div_backward(int dtype, int mode, const void *grad, const vo
 /* dst[i] = src[i] as float32, exactly; src: bfloat16 (bf16 != 0) or IEEE half.  Both 16-byte aligned.  The reference's own kernels
    compute in the narrow type; the host layer widens on entry instead. */
 TPW_API int tpw_widen(int bf16, const void *src, float *dst, int64_t n, tpw_stream_t stream);
+
+/* ---- attention: the row-normalised exponential kernel on pairwise products, applied to values -------- */
+
+/*
+ * s_ij = scale q_i . k_j for the pairs that are seen, p_ij = exp(s_ij - lse_i), lse_i = log sum_j exp(s_ij),
+ * out_i = sum_j p_ij v_j.  Query i of a sequence with L keys stands at position i + L - Nq.  Key j is seen when
+ * j < L, with `causal` j <= i + L - Nq, with `window` > 0 (causal only) also j > i + L - Nq - window.  A row that sees
+ * nothing has out = 0, lse = -inf and no gradient.  Query head h reads key head h / (Hq / Hk).  Keys and values from L on
+ * are never used, whatever they hold.  No counterpart in the reference.
+ *
+ * Scores, statistics and sums are held in 32 bits (64 for TPW_F64).  With 16-bit inputs the probabilities and the
+ * gradients of the scores are rounded to the inputs' type before they enter a matrix product, as its operands must be.
+ */
+typedef struct tpw_attention {
+    int32_t dtype;            /* TPW_F32, TPW_F64, TPW_F16, TPW_BF16 */
+    int32_t causal;
+    int64_t window;           /* 0: none */
+    int64_t B, Nq, Nk, Hq, Hk, D; /* Hq a multiple of Hk, 1 <= D <= 256 */
+    double scale;             /* positive, finite */
+    const void *q, *k, *v;    /* [B, N, H, D]; strides of batch, token and head in elements, features side by side */
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    const int32_t *key_lengths; /* [B] on the device, clamped to [0, Nk]; NULL: Nk everywhere */
+    void *out;                /* [B, Nq, Hq, D] dense */
+    void *lse;                /* [B, Hq, Nq] dense, float (double for TPW_F64); NULL in the forward: not wanted */
+    /* backward only; q .. lse as the forward had and left them */
+    const void *grad_out;     /* [B, Nq, Hq, D] */
+    int64_t grad_out_stride[3];
+    const void *grad_lse;     /* like lse; NULL: zero */
+    void *grad_q, *grad_k, *grad_v; /* dense, shaped like q, k, v; grad_q NULL: not wanted, grad_k and grad_v both or none */
+} tpw_attention;
+
+/* Scratch (device memory, 16-byte aligned) that the call with these arguments wants; 0: none; -1: refused (tpw_last_error). */
+TPW_API int64_t tpw_attention_scratch_bytes(const tpw_attention *a);
+TPW_API int tpw_attention_forward(const tpw_attention *a, void *scratch, int64_t scratch_bytes, tpw_stream_t stream);
+TPW_API int64_t tpw_attention_backward_scratch_bytes(const tpw_attention *a);
+TPW_API int tpw_attention_backward(const tpw_attention *a, void *scratch, int64_t scratch_bytes, tpw_stream_t stream);
+
+/*
+ * Rotary positions: the first R = 2 * half features of every row of x [B, N, H, D] are turned, pair i of the token at
+ * position t by the angle whose cosine and sine are cos[t, i], sin[t, i]: (a, b) -> (a cos - b sin, a sin + b cos).  The
+ * pairs are (i, half + i), or (2i, 2i + 1) with `interleaved`; features from R on are copied.  `inverse` turns back, which is
+ * the gradient's turn.  Two tensors (queries and keys) go through one launch.  A position outside [0, length) leaves NaN in
+ * the turned features.  No counterpart in the reference.
+ */
+typedef struct tpw_rotary {
+    int32_t dtype;            /* TPW_F32, TPW_F64, TPW_F16, TPW_BF16 */
+    int32_t interleaved, inverse;
+    int64_t B, N, D, half;
+    int64_t H[2];             /* heads of x[0] and x[1]; H[1] = 0: one tensor */
+    const void *x[2];
+    int64_t stride[2][3];     /* batch, token, head */
+    void *out[2];             /* dense */
+    const float *cos, *sin;   /* [length, half] dense */
+    int64_t length;
+    const int64_t *positions; /* [B, N] with the strides below; NULL: 0 .. N-1 */
+    int64_t position_stride[2];
+} tpw_rotary;
+TPW_API int tpw_rotary_apply(const tpw_rotary *a, tpw_stream_t stream);
+/* cos, sin [length, half] = magnitude * cos, sin (t * frequency[i]), t < length; frequency in radians, [half] double on the device. */
+TPW_API int tpw_rotary_table(const double *frequency, double magnitude, float *cos, float *sin, int64_t length, int64_t half,
+                             tpw_stream_t stream);
 
 /* ---- measured issue peaks (roofline denominators for the CUDA-core kernels) -------------------- */
 

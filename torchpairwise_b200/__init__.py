@@ -5,6 +5,7 @@ The module mirrors the reference's Python surface (``torchpairwise/__init__.py``
 CUDA kernels behind the C ABI of ``include/tpw_b200.h``.  CUDA tensors only.
 """
 from ._abi import LIB_PATH, TpwError, device_status, lib, measure_issue_peak
+from .attention_ops import attention, rotary_embedding, rotary_table
 from .cpdist import cdist, pdist
 from .ops import (
     _directed_hausdorff,

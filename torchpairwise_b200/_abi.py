@@ -15,7 +15,7 @@ LIB_PATH = Path(__file__).resolve().parent / "lib" / "libtpw_b200.so"
 
 # enums of include/tpw_b200.h
 TPW_OK = 0
-F32, F64, I32, I64 = 0, 1, 2, 3
+F32, F64, I32, I64, F16, BF16 = 0, 1, 2, 3, 4, 5
 LP_BWD_CDIST, LP_BWD_PPMINKOWSKI, LP_BWD_WMINKOWSKI, LP_BWD_MATMUL = 0, 1, 2, 3
 DOT_LINEAR, DOT_COSINE_SIM, DOT_COSINE_DIST, DOT_ONE_MINUS_SIM, DOT_SQEUCLIDEAN, DOT_EUCLIDEAN = range(6)
 PAIR_CANBERRA, PAIR_ADDITIVE_CHI2 = 0, 1
@@ -91,6 +91,12 @@ SIGNATURES = {
     "tpw_prf_div_forward": (_I, [_I, _I, _P, _P, _P, _L, _P]),
     "tpw_prf_div_backward": (_I, [_I, _I, _P, _P, _P, _P, _P, _L, _P]),
     "tpw_widen": (_I, [_I, _P, _P, _L, _P]),
+    "tpw_attention_scratch_bytes": (_L, [_P]),
+    "tpw_attention_forward": (_I, [_P, _P, _L, _P]),
+    "tpw_attention_backward_scratch_bytes": (_L, [_P]),
+    "tpw_attention_backward": (_I, [_P, _P, _L, _P]),
+    "tpw_rotary_apply": (_I, [_P, _P]),
+    "tpw_rotary_table": (_I, [_P, _D, _P, _P, _L, _L, _P]),
     "tpw_measure_issue_peak": (_I, [_I, POINTER(c_double)]),
 }
 

@@ -13,6 +13,7 @@ from __future__ import annotations
 import argparse
 import concurrent.futures as cf
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -50,12 +51,25 @@ def is_stale() -> bool:
     return any(p.stat().st_mtime > t for p in _deps())
 
 
+def _included(src: Path) -> set[Path]:
+    """The headers that a source includes by a quoted path, directly or through one another."""
+    found: set[Path] = set()
+    todo = [src]
+    while todo:
+        at = todo.pop()
+        for name in re.findall(r'^\s*#include "([^"]+)"', at.read_text(), flags=re.M):
+            path = (at.parent / name).resolve()
+            if path.exists() and path not in found:
+                found.add(path)
+                todo.append(path)
+    return found
+
+
 def _obj_stale(src: Path, obj: Path) -> bool:
     if not obj.exists():
         return True
     t = obj.stat().st_mtime
-    shared = sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h")) + [Path(__file__)]
-    return any(p.stat().st_mtime > t for p in [src, *shared])
+    return any(p.stat().st_mtime > t for p in [src, *_included(src)])
 
 
 def _compile_one(nvcc: str, src: Path, verbose: bool, force: bool) -> tuple[Path, str]:
@@ -96,25 +110,24 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
 
 TORCH_SRC = CSRC / "torch" / "tpw_torch.cpp"
 TORCH_LIB_PATH = LIB_DIR / "libtpw_b200_torch.so"
+# attention and rotary positions: a dispatcher namespace and library of their own
+ATTENTION_SRC = CSRC / "torch" / "tpw_torch_attention.cpp"
+ATTENTION_LIB_PATH = LIB_DIR / "libtpw_b200_attention.so"
 
 
-def build_torch_ops(force: bool = False) -> Path:
-    """Compile the C++ host layer (``csrc/torch/tpw_torch.cpp``: the ``torchpairwise::`` operator
-    registrations on top of the C ABI) with g++ against the installed torch, linked to
-    ``libtpw_b200.so``; returns the path of ``libtpw_b200_torch.so``."""
-    build_library()
-    deps = [TORCH_SRC, *sorted(INCLUDE.glob("*.h")), Path(__file__)]
-    if not force and TORCH_LIB_PATH.exists() and all(p.stat().st_mtime <= TORCH_LIB_PATH.stat().st_mtime for p in deps):
-        return TORCH_LIB_PATH
+def _build_host_layer(src: Path, lib: Path, force: bool) -> Path:
+    deps = [src, *sorted(INCLUDE.glob("*.h")), Path(__file__)]
+    if not force and lib.exists() and all(p.stat().st_mtime <= lib.stat().st_mtime for p in deps):
+        return lib
     import torch
     from torch.utils import cpp_extension as ce
     tdir = Path(torch.__file__).resolve().parent
     cuda_home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     cxx = os.environ.get("CXX", "g++")
-    tmp = TORCH_LIB_PATH.with_suffix(".so.tmp")
+    tmp = lib.with_suffix(".so.tmp")
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *[f"-I{p}" for p in ce.include_paths()], f"-I{cuda_home}/include", f"-I{INCLUDE}",
-           str(TORCH_SRC), "-o", str(tmp),
+           str(src), "-o", str(tmp),
            f"-L{tdir / 'lib'}", "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_cuda", "-lc10_cuda",
            f"-L{LIB_DIR}", "-ltpw_b200", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tdir / 'lib'}",
            # the shared C++ runtime by name: a toolchain whose own libstdc++.so link is broken would otherwise
@@ -124,8 +137,16 @@ def build_torch_ops(force: bool = False) -> Path:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"building the torch host layer failed:\n{r.stdout[-3000:]}\n{r.stderr[-3000:]}")
-    os.replace(tmp, TORCH_LIB_PATH)
-    return TORCH_LIB_PATH
+    os.replace(tmp, lib)
+    return lib
+
+
+def build_torch_ops(force: bool = False) -> Path:
+    """Compile the C++ host layer (``csrc/torch/*.cpp``: the operator registrations on top of the C ABI) with g++
+    against the installed torch, linked to ``libtpw_b200.so``; returns the path of ``libtpw_b200_torch.so``."""
+    build_library()
+    _build_host_layer(ATTENTION_SRC, ATTENTION_LIB_PATH, force)
+    return _build_host_layer(TORCH_SRC, TORCH_LIB_PATH, force)
 
 
 if __name__ == "__main__":

@@ -1,0 +1,106 @@
+// What the attention kernels share: the arguments as a kernel gets them, which pairs are seen, and the entry points of the files.
+#pragma once
+#include "common.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace tpw {
+
+struct AttnParams {
+    const void *q, *k, *v, *dout;
+    long long q_s[3], k_s[3], v_s[3], do_s[3];   // batch, token, head
+    const int *key_lengths;
+    void *out, *lse, *dq, *dk, *dv;
+    const void *dlse;
+    long long B, Nq, Nk, Hq, Hk, D, group;       // group = Hq / Hk
+    long long window;                            // 0: none
+    int causal;
+    double scale;
+    // backward: rows of the pitch Nqp, [B, Hq, Nqp], of what a walk over the queries needs (attention_rows_kernel)
+    void *row_lse, *row_delta;
+    long long Nqp;
+    const unsigned *row_max;                     // 16-bit floats of half precision: largest |dO_i|^2 and |v_j|^2 as float bits
+    int *status;
+};
+
+inline AttnParams attn_params(const tpw_attention &a) {
+    AttnParams P = {};
+    P.q = a.q; P.k = a.k; P.v = a.v; P.dout = a.grad_out;
+    for (int i = 0; i < 3; ++i) {
+        P.q_s[i] = a.q_stride[i];
+        P.k_s[i] = a.k_stride[i];
+        P.v_s[i] = a.v_stride[i];
+        P.do_s[i] = a.grad_out_stride[i];
+    }
+    P.key_lengths = a.key_lengths;
+    P.out = a.out; P.lse = a.lse; P.dq = a.grad_q; P.dk = a.grad_k; P.dv = a.grad_v;
+    P.dlse = a.grad_lse;
+    P.B = a.B; P.Nq = a.Nq; P.Nk = a.Nk; P.Hq = a.Hq; P.Hk = a.Hk; P.D = a.D;
+    P.group = a.Hk > 0 ? a.Hq / a.Hk : 1;
+    P.window = a.window;
+    P.causal = a.causal;
+    P.scale = a.scale;
+    P.Nqp = (a.Nq + 127) / 128 * 128;
+    return P;
+}
+
+// attention_simple.cu: any type, head width and stride, on the CUDA cores
+int attn_simple_forward(int dtype, const AttnParams &P, cudaStream_t s);
+int attn_simple_backward(int dtype, const AttnParams &P, cudaStream_t s);
+// attention_rows.cu: what both gradient walks need of each query row
+long long attn_rows_bytes(int dtype, const AttnParams &P);
+int attn_rows(int dtype, AttnParams &P, void *scratch, bool tensor, cudaStream_t s);
+
+// abi.cu: 16-bit rows of [batch, tokens, heads, features] that lie the given numbers of bytes apart, as boxes of 64 features (128-byte
+// swizzle) by `box_tokens` tokens; what lies beyond the tensor reads as zero
+int make_tensor_map_heads(CUtensorMap *map, const void *base, uint64_t features, uint64_t tokens, uint64_t heads, uint64_t batch,
+                          uint64_t token_pitch, uint64_t head_pitch, uint64_t batch_pitch, uint32_t box_tokens);
+// attention_forward.cu: 16-bit types on the tensor cores
+bool attn_tc_fits(int dtype, const AttnParams &P);
+int attn_tc_forward(int dtype, const AttnParams &P, cudaStream_t s);
+// attention_backward.cu
+bool attn_tc_backward_fits(int dtype, const AttnParams &P);
+int attn_tc_backward(int dtype, const AttnParams &P, cudaStream_t s);
+
+#ifdef __CUDACC__
+namespace {
+
+// The keys [lo, hi) that query i of a sequence sees, and the queries [qlo, qhi) that see key j; off = length - Nq.
+struct Seen {
+    int length, off, nq, window;   // window: 0 none
+    bool causal;
+    __device__ __forceinline__ Seen(const AttnParams &P, long long b) {
+        const int nk = (int)P.Nk;
+        int n = P.key_lengths ? P.key_lengths[b] : nk;
+        length = n < 0 ? 0 : n > nk ? nk : n;
+        nq = (int)P.Nq;
+        off = length - nq;
+        causal = P.causal != 0;
+        window = (int)(P.window < nk ? P.window : 0);   // a window over all keys is none
+    }
+    __device__ __forceinline__ int hi(int i) const {
+        const int h = causal && i + off + 1 < length ? i + off + 1 : length;
+        return h > 0 ? h : 0;
+    }
+    __device__ __forceinline__ int lo(int i) const {
+        const int l = window ? i + off + 1 - window : 0;
+        return l > 0 ? l : 0;
+    }
+    __device__ __forceinline__ int qlo(int j) const {
+        const int l = causal ? j - off : 0;
+        return l > 0 ? l : 0;
+    }
+    __device__ __forceinline__ int qhi(int j) const {
+        const int h = window && j - off + window < nq ? j - off + window : nq;
+        return j < length && h > 0 ? h : 0;
+    }
+};
+
+template <typename T> struct AttnAcc { typedef float type; };
+template <> struct AttnAcc<double> { typedef double type; };
+
+} // namespace
+#endif
+
+} // namespace tpw
