@@ -146,6 +146,23 @@ static int encode_map_3d(CUtensorMap *map, const void *base, int elem_bytes,
     return TPW_OK;
 }
 
+int make_tensor_map_heads(CUtensorMap *map, const void *base, uint64_t features, uint64_t tokens, uint64_t heads, uint64_t batch,
+                          uint64_t token_pitch, uint64_t head_pitch, uint64_t batch_pitch, uint32_t box_tokens) {
+    CUtensorMap first;   // binds the context and resolves the encoder like every other map
+    int e = make_tensor_map_3d_pitched(&first, base, 2, features, tokens, heads, token_pitch, head_pitch, 64, box_tokens);
+    if (e != TPW_OK) return e;
+    if (batch_pitch % 16 != 0) return fail(TPW_ERR_INVALID, "tensor map: pitches are no multiples of 16 bytes");
+    cuuint64_t dims[4] = {features, tokens, heads, batch};
+    cuuint64_t strides[3] = {token_pitch, head_pitch, batch_pitch};
+    cuuint32_t box[4] = {64, box_tokens, 1, 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = resolve_encode_tiled()(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims, strides, box, estr,
+                                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(TPW_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+    return TPW_OK;
+}
+
 // ---- issue-rate microbenchmarks ------------------------------------------------------------------
 template <int KIND>
 __global__ void __launch_bounds__(256) issue_peak_kernel(float *sink, int iters, float seed) {

@@ -27,6 +27,10 @@ int check(const tpw_attention *a, bool backward) {
 
 bool nothing(const tpw_attention &a) { return a.B == 0 || a.Nq == 0 || a.Hq == 0; }
 
+long long split_bytes(const AttnParams &P, const AttnSplits &splits) {
+    return splits.count > 1 ? 4 * splits.count * P.B * P.Hq * P.Nq * (P.D + 1) : 0;
+}
+
 } // namespace
 } // namespace tpw
 
@@ -35,7 +39,9 @@ extern "C" {
 int64_t tpw_attention_scratch_bytes(const tpw_attention *a) {
     tpw::clear_error();
     if (tpw::check(a, false) != TPW_OK) return -1;
-    return 0;
+    if (tpw::nothing(*a)) return 0;
+    const tpw::AttnParams P = tpw::attn_params(*a);
+    return tpw::attn_few_fits(a->dtype, P) ? tpw::split_bytes(P, tpw::attn_few_splits(P)) : 0;
 }
 
 int tpw_attention_forward(const tpw_attention *a, void *scratch, int64_t scratch_bytes, tpw_stream_t stream) {
@@ -43,7 +49,19 @@ int tpw_attention_forward(const tpw_attention *a, void *scratch, int64_t scratch
     const int e = tpw::check(a, false);
     if (e != TPW_OK || tpw::nothing(*a)) return e;
     const tpw::AttnParams P = tpw::attn_params(*a);
-    return tpw::attn_simple_forward(a->dtype, P, static_cast<cudaStream_t>(stream));
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (tpw::attn_few_fits(a->dtype, P)) {
+        tpw::AttnSplits splits = tpw::attn_few_splits(P);
+        const int64_t bytes = tpw::split_bytes(P, splits);
+        TPW_CHECK_ARG(bytes == 0 || (scratch && tpw::aligned16(scratch) && scratch_bytes >= bytes),
+                      "tpw_attention_forward: scratch of %lld bytes, 16-byte aligned, is needed", (long long)bytes);
+        splits.out = static_cast<float *>(scratch);
+        splits.lse = splits.out ? splits.out + splits.count * P.B * P.Hq * P.Nq * P.D : nullptr;
+        const int e = tpw::attn_few_forward(a->dtype, P, splits, s);
+        return e != TPW_OK || splits.count == 1 ? e : tpw::attn_join(a->dtype, P, splits, s);
+    }
+    if (tpw::attn_tc_fits(a->dtype, P)) return tpw::attn_tc_forward(a->dtype, P, s);
+    return tpw::attn_simple_forward(a->dtype, P, s);
 }
 
 int64_t tpw_attention_backward_scratch_bytes(const tpw_attention *a) {
@@ -71,8 +89,10 @@ int tpw_attention_backward(const tpw_attention *a, void *scratch, int64_t scratc
     TPW_CHECK_ARG(scratch && tpw::aligned16(scratch) && scratch_bytes >= tpw::attn_rows_bytes(a->dtype, P),
                   "tpw_attention_backward: scratch of %lld bytes, 16-byte aligned, is needed", tpw::attn_rows_bytes(a->dtype, P));
     if (!P.dq && !P.dk) return TPW_OK;
-    e = tpw::attn_rows(a->dtype, P, scratch, false, s);
+    const bool tensor = tpw::attn_tc_backward_fits(a->dtype, P);
+    e = tpw::attn_rows(a->dtype, P, scratch, tensor, s);
     if (e != TPW_OK) return e;
+    if (tensor) return tpw::attn_tc_backward(a->dtype, P, s);
     return tpw::attn_simple_backward(a->dtype, P, s);
 }
 

@@ -59,6 +59,15 @@ int make_tensor_map_heads(CUtensorMap *map, const void *base, uint64_t features,
 // attention_forward.cu: 16-bit types on the tensor cores
 bool attn_tc_fits(int dtype, const AttnParams &P);
 int attn_tc_forward(int dtype, const AttnParams &P, cudaStream_t s);
+// attention_few.cu: few query rows, the keys cut into ranges that are joined afterwards
+struct AttnSplits {
+    int count = 1, keys = 0;             // ranges and keys of each
+    float *out = nullptr, *lse = nullptr; // [count, B, Hq, Nq, D] outputs and [count, B, Hq, Nq] log-sums of the ranges
+};
+bool attn_few_fits(int dtype, const AttnParams &P);
+AttnSplits attn_few_splits(const AttnParams &P);
+int attn_few_forward(int dtype, const AttnParams &P, const AttnSplits &splits, cudaStream_t s);
+int attn_join(int dtype, const AttnParams &P, const AttnSplits &splits, cudaStream_t s);
 // attention_backward.cu
 bool attn_tc_backward_fits(int dtype, const AttnParams &P);
 int attn_tc_backward(int dtype, const AttnParams &P, cudaStream_t s);

@@ -1,0 +1,580 @@
+// Gradients of attention on the tensor cores (16-bit types, up to 128 features).
+//
+// p_ij = exp(s_ij - lse_i) is formed anew from the forward's lse; ds_ij = p_ij (dO_i . v_j - delta_i).
+//   keys walk    (dk, dv): a CTA holds 128 keys of one key head and walks over the query tiles of every head that shares it.
+//                S^T = K Q^T and dP^T = V dO^T, a key row per thread pair; dV += P^T dO, dK += dS^T Q with P^T and dS^T in tensor memory.
+//   queries walk (dq): a CTA holds 128 queries of one head and walks over the key tiles.  S = Q K^T, dP = dO V^T, dQ += dS K.
+// Every gradient element is summed by one CTA in a fixed order: no atomics, the same bits each time.  That costs S and dP twice, 7 products
+// of 128 x 128 x D per pair of tiles where 5 would do with 32-bit atomics into dq, whose order changes results.
+//
+// Bound by the tensor cores: 4 products (2048 clocks at D = 128) in the keys walk, 3 (1536) in the queries walk, with 16384
+// exponentials (1024 clocks of the special-function units) beside either.  The elementwise work of one half of an
+// iteration runs while the tensor cores do the other half: the keys walk forms P^T(i) during dK(i-1) and dP(i), dS^T(i) during dV(i) and
+// S(i+1); tensor memory is full (S, dP, dV, dK of 128 columns each), so it cannot look further ahead.  The queries walk has room for
+// two dP and gives S back as soon as it is read, so its S and dP are always one tile ahead.
+//
+// Two warpgroups share a tile's 128 rows: each has half of the columns, and writes its half of P or dS over the columns it read.
+#include "attention_tc.cuh"
+
+namespace tpw {
+namespace {
+
+struct BackwardParams {
+    AttnParams a;
+    float scale_log2, scale;
+    int tiles;
+};
+
+// Half precision: probabilities are lifted by 2^12 and gradients of scores by another power of two (attention_rows.cu), both undone in
+// the epilogue; the largest of either is then 2^12 and 2^15.
+template <typename T> struct Lift {
+    static constexpr bool kNeeded = false;
+    static __device__ __forceinline__ float factor(const unsigned *) { return 1.f; }
+};
+template <> struct Lift<__half> {
+    static constexpr bool kNeeded = true;
+    static __device__ __forceinline__ float factor(const unsigned *row_max) {
+        const float most = 2.f * sqrtf(__uint_as_float(row_max[0])) * sqrtf(__uint_as_float(row_max[1])) + __uint_as_float(row_max[2]);
+        if (!(most > 0.f) || !(most < INFINITY)) return 1.f;
+        const float e = floorf(3.f - log2f(most));
+        return exp2f(e < -100.f ? -100.f : e > 100.f ? 100.f : e);
+    }
+};
+
+template <int BLOCKS> struct BackwardSmem {
+    static constexpr int kStages = BLOCKS == 2 ? 2 : 3;
+    static constexpr uint32_t TILE_BYTES = BLOCKS * BLOCK_BYTES;
+    static constexpr uint32_t OFF_RING = 2 * TILE_BYTES;                       // the CTA's own two tiles, then pairs of walked tiles
+    static constexpr uint32_t OFF_ROWS = OFF_RING + kStages * 2 * TILE_BYTES;  // lse, delta of a query tile per stage
+    static constexpr uint32_t OFF_BAR = OFF_ROWS + kStages * 2 * TILE * 4;
+    static constexpr uint32_t OFF_TMEM = OFF_BAR + 8 * (3 * kStages + 10);
+    static constexpr uint32_t ALLOC = OFF_TMEM + 16 + 1024;
+    static_assert(ALLOC <= 232448, "exceeds the dynamic shared memory of one CTA");
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// 64 columns of a thread's row: ds = p (dp - delta) in place of p, times `lift`
+template <bool LIFT>
+__device__ __forceinline__ f32x2 score_gradient(f32x2 p, f32x2 dp, f32x2 minus_delta, f32x2 lift) {
+    f32x2 d = add2(dp, minus_delta);
+    if (LIFT) d = mul2(d, lift);
+    return mul2(p, d);
+}
+
+// rows of an accumulator to global memory, this thread's half of the columns
+template <typename T, int BLOCKS>
+__device__ __forceinline__ void store_half(T *row, uint32_t acc, int half, float by, bool keep, bool valid, int D) {
+#pragma unroll 1
+    for (int g = 0; g < BLOCKS; ++g) {
+        const int col = half * 32 * BLOCKS + 32 * g;
+        uint32_t o[32];
+        tmem_ld32(acc + col, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                w[k] = keep ? Narrow<T>::pack(__uint_as_float(o[e + 2 * k]) * by, __uint_as_float(o[e + 2 * k + 1]) * by) : 0u;
+            if (valid && col + e < D) *reinterpret_cast<uint4 *>(row + col + e) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
+template <typename T, int BLOCKS>
+__global__ void __launch_bounds__(kTcThreads, 1)
+attention_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                     const __grid_constant__ CUtensorMap map_g, const BackwardParams F) {
+    typedef BackwardSmem<BLOCKS> L;
+    typedef Narrow<T> N;
+    const AttnParams &P = F.a;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *q_full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *g_full = q_full + L::kStages, *empty = g_full + L::kStages,
+             *kv_full = empty + L::kStages, *s_full = kv_full + 1, *dp_full = s_full + 1, *p_ready = dp_full + 1, *ds_ready = p_ready + 1,
+             *acc_full = ds_ready + 1, *drained = acc_full + 1;
+    uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(smem + L::OFF_TMEM);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_TMEM + 4);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long heads = P.B * P.Hk;
+    const int row0 = (int)(blockIdx.x / heads) * TILE;   // a causal call's first keys are seen by most queries
+    const long long bh = blockIdx.x % heads;
+    const int hk = (int)(bh % P.Hk), b = (int)(bh / P.Hk);
+    const Seen see(P, b);
+    const int last = (row0 + TILE < see.length ? row0 + TILE : see.length) - 1;
+    const int i_lo = see.qlo(row0), i_hi = last < row0 ? 0 : see.qhi(last);
+    const int begin = i_lo / TILE, per_head = i_hi > i_lo ? (i_hi + TILE - 1) / TILE - begin : 0;
+    const int total = per_head * (int)P.group;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < L::kStages; ++i) { mbar_init(&q_full[i], 1); mbar_init(&g_full[i], 1); mbar_init(&empty[i], 1); }
+        mbar_init(kv_full, 1);
+        mbar_init(s_full, 1);
+        mbar_init(dp_full, 1);
+        mbar_init(p_ready, 8);
+        mbar_init(ds_ready, 8);
+        mbar_init(acc_full, 1);
+        mbar_init(drained, 1);
+        *abort_flag = 0;
+        mbar_init_fence();
+        tma_prefetch_descriptor(&map_q);
+        tma_prefetch_descriptor(&map_k);
+        tma_prefetch_descriptor(&map_v);
+        tma_prefetch_descriptor(&map_g);
+    }
+    if (warp == 9) tmem_alloc(tmem_ptr, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_ptr;
+    auto give_up = [&](int site) {
+        *abort_flag = 1;
+        if (P.status) atomicCAS(P.status, 0, (17 << 16) | site);
+    };
+    auto warp_wait = [&](uint64_t *bar, uint32_t parity, int site) {
+        const bool ok = __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag));
+        if (!ok) give_up(site);
+        return ok;
+    };
+    const uint32_t k_at = smem_u32(smem), v_at = k_at + L::TILE_BYTES, ring = smem_u32(smem + L::OFF_RING);
+    const uint32_t rows_at = smem_u32(smem + L::OFF_ROWS);
+    const uint32_t S = tmem, DP = tmem + TILE, DV = tmem + 2 * TILE, DK = tmem + 3 * TILE;
+
+    if (warp >= 8) registers_down();
+    if (warp == 8) {
+        if (lane == 0 && total > 0) {
+            uint32_t issued = 0;
+            mbar_expect_tx(kv_full, 2 * L::TILE_BYTES);
+            load_tokens<BLOCKS>(k_at, &map_k, kv_full, row0, hk, b);
+            load_tokens<BLOCKS>(v_at, &map_v, kv_full, row0, hk, b);
+            for (int u = 0; u < total; ++u) {
+                const uint32_t st = u % L::kStages;
+                if (u >= L::kStages && !wait_or_abort(&empty[st], parity_of_use(u, L::kStages) ^ 1, abort_flag)) {
+                    give_up(1);
+                    break;
+                }
+                const int h = hk * (int)P.group + u / per_head, i0 = (begin + u % per_head) * TILE;
+                const long long at = (b * P.Hq + h) * P.Nqp + i0;
+                const uint32_t q_at = ring + st * 2 * L::TILE_BYTES, rows = rows_at + st * 2 * TILE * 4;
+                mbar_expect_tx(&q_full[st], L::TILE_BYTES + TILE * 4);
+                load_tokens<BLOCKS>(q_at, &map_q, &q_full[st], i0, h, b);
+                bulk_load(rows, static_cast<const float *>(P.row_lse) + at, TILE * 4, &q_full[st]);
+                mbar_expect_tx(&g_full[st], L::TILE_BYTES + TILE * 4);
+                load_tokens<BLOCKS>(q_at + L::TILE_BYTES, &map_g, &g_full[st], i0, h, b);
+                bulk_load(rows + TILE * 4, static_cast<const float *>(P.row_delta) + at, TILE * 4, &g_full[st]);
+                issued = u + 1;
+            }
+            for (uint32_t u = first_of_last_uses(issued, L::kStages); u < issued; ++u)
+                if (!wait_or_abort(&empty[u % L::kStages], parity_of_use(u, L::kStages), abort_flag)) {
+                    give_up(2);
+                    break;
+                }
+            if (*abort_flag) {   // what was issued arrives before the CTA ends
+                mbar_wait_bounded(kv_full, 0);
+                for (uint32_t u = first_of_last_uses(issued, L::kStages); u < issued; ++u) {
+                    mbar_wait_bounded(&q_full[u % L::kStages], parity_of_use(u, L::kStages));
+                    mbar_wait_bounded(&g_full[u % L::kStages], parity_of_use(u, L::kStages));
+                }
+            }
+        }
+    } else if (warp == 9) {
+        const int steps = (int)(P.D + 15) / 16;
+        const uint32_t idesc_s = instruction(N::kFormat, TILE, false), idesc_d = instruction(N::kFormat, 16 * steps, true);
+        bool ok = total == 0 || warp_wait(kv_full, 0, 3);
+        // S^T or dP^T of use u, once its tile has arrived
+        auto first = [&](uint64_t *arrives, int u, uint32_t d, uint32_t own, uint32_t offset, uint64_t *done, int site) {
+            const uint32_t st = u % L::kStages;
+            if (!warp_wait(&arrives[st], parity_of_use(u, L::kStages), site)) return false;
+            tc_fence_after();
+            if (lane == 0) {
+                product_features(d, own, ring + st * 2 * L::TILE_BYTES + offset, idesc_s, steps);
+                tc_commit<false>(done);
+            }
+            return true;
+        };
+        if (total > 0 && ok) ok = first(q_full, 0, S, k_at, 0, s_full, 4) && first(g_full, 0, DP, v_at, L::TILE_BYTES, dp_full, 5);
+        for (int u = 0; u < total && ok; ++u) {
+            const uint32_t q_at = ring + (u % L::kStages) * 2 * L::TILE_BYTES;
+            if (!(ok = warp_wait(p_ready, u & 1, 6))) break;
+            tc_fence_after();
+            if (lane == 0) product_tokens(DV, S, 64, q_at + L::TILE_BYTES, idesc_d, u > 0);
+            if (u + 1 < total && !(ok = first(q_full, u + 1, S, k_at, 0, s_full, 4))) break;
+            if (!(ok = warp_wait(ds_ready, u & 1, 7))) break;
+            tc_fence_after();
+            if (lane == 0) {
+                product_tokens(DK, DP, 64, q_at, idesc_d, u > 0);
+                tc_commit<false>(&empty[u % L::kStages]);
+            }
+            if (u + 1 < total && !(ok = first(g_full, u + 1, DP, v_at, L::TILE_BYTES, dp_full, 5))) break;
+        }
+        if (ok && total > 0 && lane == 0) tc_commit<false>(acc_full);
+        __syncwarp();
+    } else if (warp < 8) {
+        // ---- a key row and 64 query columns per thread ----
+        registers_up();
+        const int half = warp >> 2, j = row0 + (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t s_at = S + lanes + 64 * half, dp_at = DP + lanes + 64 * half;
+        const int lo = see.qlo(j), hi = see.window ? see.qhi(j) : 0x7fffffff;
+        // query tiles from all_lo on, and below all_hi, are seen by every key of the tile; keys beyond the length are not stored
+        const int all_lo = see.qlo(row0 + TILE - 1), all_hi = see.window ? row0 - see.off + see.window : 0x7fffffff;
+        const float c = F.scale_log2, lift = Lift<T>::factor(P.row_max);
+        const f32x2 c2 = pack2(c, c), lift2 = pack2(lift, lift);
+        bool ok = true;
+        for (int u = 0; u < total; ++u) {
+            const uint32_t st = u % L::kStages;
+            const float *rows = reinterpret_cast<const float *>(smem + L::OFF_ROWS + st * 2 * TILE * 4) + 64 * half;
+            const int i0 = (begin + u % per_head) * TILE;
+            if (!(ok = warp_wait(s_full, u & 1, 8) && warp_wait(&q_full[st], parity_of_use(u, L::kStages), 9))) break;
+            tc_fence_after();
+            uint32_t x[2][32];
+            tmem_ld32(s_at, x[0]);
+            tmem_ld32(s_at + 32, x[1]);
+            tmem_ld_wait();
+            const bool masked = i0 < all_lo || i0 + TILE > all_hi;
+            f32x2 p[32];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+                const float4 minus_lse = *reinterpret_cast<const float4 *>(rows + 2 * e);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t *pair = &x[(e + k) >> 4][2 * ((e + k) & 15)];
+                    const f32x2 z = fma2(pack2(__uint_as_float(pair[0]), __uint_as_float(pair[1])), c2,
+                                         k ? pack2(minus_lse.z, minus_lse.w) : pack2(minus_lse.x, minus_lse.y));
+                    float z0, z1;
+                    unpack2(z, z0, z1);
+                    p[e + k] = pack2(exp2_fast(z0), exp2_fast(z1));
+                }
+            }
+            if (masked) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    const int i = i0 + 64 * half + 2 * e;
+                    float p0, p1;
+                    unpack2(p[e], p0, p1);
+                    p[e] = pack2(i >= lo && i < hi ? p0 : 0.f, i + 1 >= lo && i + 1 < hi ? p1 : 0.f);
+                }
+            }
+            {
+                uint32_t w[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    float p0, p1;
+                    unpack2(p[e], p0, p1);
+                    w[e] = N::pack(p0, p1);
+                }
+                tmem_st32(s_at, w);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_ready);
+            }
+            if (!(ok = warp_wait(dp_full, u & 1, 10) && warp_wait(&g_full[st], parity_of_use(u, L::kStages), 11))) break;
+            tc_fence_after();
+            tmem_ld32(dp_at, x[0]);
+            tmem_ld32(dp_at + 32, x[1]);
+            tmem_ld_wait();
+            uint32_t w[32];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+                const float4 minus_delta = *reinterpret_cast<const float4 *>(rows + TILE + 2 * e);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t *pair = &x[(e + k) >> 4][2 * ((e + k) & 15)];
+                    const f32x2 ds = score_gradient<Lift<T>::kNeeded>(p[e + k], pack2(__uint_as_float(pair[0]), __uint_as_float(pair[1])),
+                                                                     k ? pack2(minus_delta.z, minus_delta.w) : pack2(minus_delta.x, minus_delta.y), lift2);
+                    float d0, d1;
+                    unpack2(ds, d0, d1);
+                    if (masked) {   // 0 times what need not be finite
+                        const int i = i0 + 64 * half + 2 * (e + k);
+                        d0 = i >= lo && i < hi ? d0 : 0.f;
+                        d1 = i + 1 >= lo && i + 1 < hi ? d1 : 0.f;
+                    }
+                    w[e + k] = N::pack(d0, d1);
+                }
+            }
+            tmem_st32(dp_at, w);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ds_ready);
+        }
+        if (ok && total > 0) {
+            ok = warp_wait(acc_full, 0, 12);
+            tc_fence_after();
+        }
+        if (ok) {
+            const bool keep = total > 0 && j < see.length, valid = j < (int)P.Nk;
+            const long long to = ((b * P.Nk + j) * P.Hk + hk) * P.D;
+            const float down = Lift<T>::kNeeded ? 0.000244140625f : 1.f;   // 2^-12
+            store_half<T, BLOCKS>(static_cast<T *>(P.dv) + to, DV + lanes, half, down, keep, valid, (int)P.D);
+            store_half<T, BLOCKS>(static_cast<T *>(P.dk) + to, DK + lanes, half, F.scale * down / lift, keep, valid, (int)P.D);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        if (*abort_flag && lane == 0) {   // the commits behind all MMAs were waited for, or one more is waited for here
+            tc_commit<false>(drained);
+            mbar_wait_bounded(drained, 0);
+        }
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <typename T, int BLOCKS>
+__global__ void __launch_bounds__(kTcThreads, 1)
+attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                    const __grid_constant__ CUtensorMap map_g, const BackwardParams F) {
+    typedef BackwardSmem<BLOCKS> L;
+    typedef Narrow<T> N;
+    const AttnParams &P = F.a;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *empty = full + L::kStages, *own_full = empty + L::kStages, *s_full = own_full + 1,
+             *s_read = s_full + 1, *dp_full = s_read + 1, *ds_ready = dp_full + 2, *acc_full = ds_ready + 1, *drained = acc_full + 1;
+    uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(smem + L::OFF_TMEM);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_TMEM + 4);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long heads = P.B * P.Hq;
+    const int row0 = (F.tiles - 1 - (int)(blockIdx.x / heads)) * TILE;   // a causal call's longest rows first
+    const long long bh = blockIdx.x % heads;
+    const int h = (int)(bh % P.Hq), b = (int)(bh / P.Hq), hk = h / (int)P.group;
+    const Seen see(P, b);
+    const int nq = (int)P.Nq, last = (row0 + TILE < nq ? row0 + TILE : nq) - 1;
+    const int begin = see.lo(row0) / TILE, end = (see.hi(last) + TILE - 1) / TILE;
+    const int total = end > begin ? end - begin : 0;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < L::kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        mbar_init(own_full, 1);
+        mbar_init(s_full, 1);
+        mbar_init(s_read, 8);
+        mbar_init(&dp_full[0], 1);
+        mbar_init(&dp_full[1], 1);
+        mbar_init(ds_ready, 8);
+        mbar_init(acc_full, 1);
+        mbar_init(drained, 1);
+        *abort_flag = 0;
+        mbar_init_fence();
+        tma_prefetch_descriptor(&map_q);
+        tma_prefetch_descriptor(&map_k);
+        tma_prefetch_descriptor(&map_v);
+        tma_prefetch_descriptor(&map_g);
+    }
+    if (warp == 9) tmem_alloc(tmem_ptr, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_ptr;
+    auto give_up = [&](int site) {
+        *abort_flag = 1;
+        if (P.status) atomicCAS(P.status, 0, (18 << 16) | site);
+    };
+    auto warp_wait = [&](uint64_t *bar, uint32_t parity, int site) {
+        const bool ok = __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag));
+        if (!ok) give_up(site);
+        return ok;
+    };
+    const uint32_t q_at = smem_u32(smem), g_at = q_at + L::TILE_BYTES, ring = smem_u32(smem + L::OFF_RING);
+    const uint32_t S = tmem, DP = tmem + TILE, DQ = tmem + 3 * TILE;
+
+    if (warp >= 8) registers_down();
+    if (warp == 8) {
+        if (lane == 0 && total > 0) {
+            uint32_t issued = 0;
+            mbar_expect_tx(own_full, 2 * L::TILE_BYTES);
+            load_tokens<BLOCKS>(q_at, &map_q, own_full, row0, h, b);
+            load_tokens<BLOCKS>(g_at, &map_g, own_full, row0, h, b);
+            for (int u = 0; u < total; ++u) {
+                const uint32_t st = u % L::kStages;
+                if (u >= L::kStages && !wait_or_abort(&empty[st], parity_of_use(u, L::kStages) ^ 1, abort_flag)) {
+                    give_up(1);
+                    break;
+                }
+                mbar_expect_tx(&full[st], 2 * L::TILE_BYTES);
+                load_tokens<BLOCKS>(ring + st * 2 * L::TILE_BYTES, &map_k, &full[st], (begin + u) * TILE, hk, b);
+                load_tokens<BLOCKS>(ring + st * 2 * L::TILE_BYTES + L::TILE_BYTES, &map_v, &full[st], (begin + u) * TILE, hk, b);
+                issued = u + 1;
+            }
+            for (uint32_t u = first_of_last_uses(issued, L::kStages); u < issued; ++u)
+                if (!wait_or_abort(&empty[u % L::kStages], parity_of_use(u, L::kStages), abort_flag)) {
+                    give_up(2);
+                    break;
+                }
+            if (*abort_flag) {   // what was issued arrives before the CTA ends
+                mbar_wait_bounded(own_full, 0);
+                for (uint32_t u = first_of_last_uses(issued, L::kStages); u < issued; ++u) mbar_wait_bounded(&full[u % L::kStages], parity_of_use(u, L::kStages));
+            }
+        }
+    } else if (warp == 9) {
+        const int steps = (int)(P.D + 15) / 16;
+        const uint32_t idesc_s = instruction(N::kFormat, TILE, false), idesc_d = instruction(N::kFormat, 16 * steps, true);
+        bool ok = total == 0 || warp_wait(own_full, 0, 3);
+        auto first = [&](int u) {   // S and dP of key tile u
+            const uint32_t st = u % L::kStages, at = ring + st * 2 * L::TILE_BYTES;
+            if (!warp_wait(&full[st], parity_of_use(u, L::kStages), 4)) return false;
+            tc_fence_after();
+            const int beyond = see.length - (begin + u) * TILE;
+            if (beyond < TILE && (int)P.Nk > see.length) clear_tokens<BLOCKS>(smem + L::OFF_RING + st * 2 * L::TILE_BYTES, beyond, lane);
+            if (lane == 0) {
+                product_features(S, q_at, at, idesc_s, steps);
+                tc_commit<false>(s_full);
+                product_features(DP + (u & 1) * TILE, g_at, at + L::TILE_BYTES, idesc_s, steps);
+                tc_commit<false>(&dp_full[u & 1]);
+            }
+            return true;
+        };
+        if (total > 0 && ok) ok = first(0);
+        for (int u = 0; u < total && ok; ++u) {
+            if (u + 1 < total) {
+                if (!(ok = warp_wait(s_read, u & 1, 5))) break;
+                tc_fence_after();
+                if (!(ok = first(u + 1))) break;
+            }
+            if (!(ok = warp_wait(ds_ready, u & 1, 6))) break;
+            tc_fence_after();
+            if (lane == 0) {
+                product_tokens(DQ, DP + (u & 1) * TILE, 64, ring + (u % L::kStages) * 2 * L::TILE_BYTES, idesc_d, u > 0);
+                tc_commit<false>(&empty[u % L::kStages]);
+            }
+        }
+        if (ok && total > 0 && lane == 0) tc_commit<false>(acc_full);
+        __syncwarp();
+    } else if (warp < 8) {
+        // ---- a query row and 64 key columns per thread ----
+        registers_up();
+        const int half = warp >> 2, i = row0 + (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const int lo = see.lo(i), hi = i < nq ? see.hi(i) : 0;
+        const int all_lo = see.lo(last), all_hi = see.hi(row0);   // seen by every query of the tile
+        const float c = F.scale_log2, lift = Lift<T>::factor(P.row_max);
+        const float lse = static_cast<const float *>(P.row_lse)[bh * P.Nqp + i], delta = static_cast<const float *>(P.row_delta)[bh * P.Nqp + i];
+        const f32x2 c2 = pack2(c, c), lift2 = pack2(lift, lift), minus_lse = pack2(lse, lse), minus_delta = pack2(delta, delta);
+        bool ok = true;
+        for (int u = 0; u < total; ++u) {
+            const int j0 = (begin + u) * TILE;
+            const uint32_t s_at = S + lanes + 64 * half, dp_at = DP + (u & 1) * TILE + lanes + 64 * half;
+            const bool masked = j0 < all_lo || j0 + TILE > all_hi;
+            if (!(ok = warp_wait(s_full, u & 1, 7))) break;
+            tc_fence_after();
+            uint32_t x[2][32];
+            tmem_ld32(s_at, x[0]);
+            tmem_ld32(s_at + 32, x[1]);
+            tmem_ld_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_read);
+            f32x2 p[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+                const uint32_t *pair = &x[e >> 4][2 * (e & 15)];
+                float z0, z1;
+                unpack2(fma2(pack2(__uint_as_float(pair[0]), __uint_as_float(pair[1])), c2, minus_lse), z0, z1);
+                p[e] = pack2(exp2_fast(z0), exp2_fast(z1));
+            }
+            if (!(ok = warp_wait(&dp_full[u & 1], (u >> 1) & 1, 8))) break;
+            tc_fence_after();
+            tmem_ld32(dp_at, x[0]);
+            tmem_ld32(dp_at + 32, x[1]);
+            tmem_ld_wait();
+            uint32_t w[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+                const uint32_t *pair = &x[e >> 4][2 * (e & 15)];
+                float d0, d1;
+                unpack2(score_gradient<Lift<T>::kNeeded>(p[e], pack2(__uint_as_float(pair[0]), __uint_as_float(pair[1])), minus_delta, lift2), d0, d1);
+                if (masked) {
+                    const int j = j0 + 64 * half + 2 * e;
+                    d0 = j >= lo && j < hi ? d0 : 0.f;
+                    d1 = j + 1 >= lo && j + 1 < hi ? d1 : 0.f;
+                }
+                w[e] = N::pack(d0, d1);
+            }
+            tmem_st32(dp_at, w);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ds_ready);
+        }
+        if (ok && total > 0) {
+            ok = warp_wait(acc_full, 0, 9);
+            tc_fence_after();
+        }
+        if (ok) {
+            const float down = Lift<T>::kNeeded ? 0.000244140625f : 1.f;   // 2^-12
+            T *row = static_cast<T *>(P.dq) + ((b * P.Nq + i) * P.Hq + h) * P.D;
+            store_half<T, BLOCKS>(row, DQ + lanes, half, F.scale * down / lift, total > 0, i < nq, (int)P.D);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        if (*abort_flag && lane == 0) {
+            tc_commit<false>(drained);
+            mbar_wait_bounded(drained, 0);
+        }
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <typename T, int BLOCKS> int launch(const AttnParams &P, cudaStream_t s) {
+    typedef BackwardSmem<BLOCKS> L;
+    BackwardParams F = {};
+    F.a = P;
+    F.a.status = device_status_ptr();
+    F.scale = (float)P.scale;
+    F.scale_log2 = (float)(P.scale * 1.4426950408889634074);
+    CUtensorMap q, k, v, g;
+    int e = make_tensor_map_heads(&q, P.q, P.D, P.Nq, P.Hq, P.B, 2 * P.q_s[1], 2 * P.q_s[2], 2 * P.q_s[0], TILE);
+    if (e == TPW_OK) e = make_tensor_map_heads(&k, P.k, P.D, P.Nk, P.Hk, P.B, 2 * P.k_s[1], 2 * P.k_s[2], 2 * P.k_s[0], TILE);
+    if (e == TPW_OK) e = make_tensor_map_heads(&v, P.v, P.D, P.Nk, P.Hk, P.B, 2 * P.v_s[1], 2 * P.v_s[2], 2 * P.v_s[0], TILE);
+    if (e == TPW_OK) e = make_tensor_map_heads(&g, P.dout, P.D, P.Nq, P.Hq, P.B, 2 * P.do_s[1], 2 * P.do_s[2], 2 * P.do_s[0], TILE);
+    if (e != TPW_OK) return e;
+    if (P.dk) {
+        F.tiles = (int)((P.Nk + TILE - 1) / TILE);
+        const long long blocks = F.tiles * P.B * P.Hk;
+        TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
+        auto kern = attention_dkv_kernel<T, BLOCKS>;
+        TPW_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::ALLOC));
+        kern<<<(unsigned)blocks, kTcThreads, L::ALLOC, s>>>(q, k, v, g, F);
+        TPW_LAUNCH_OK("attention_dkv_kernel");
+    }
+    if (P.dq) {
+        F.tiles = (int)((P.Nq + TILE - 1) / TILE);
+        const long long blocks = F.tiles * P.B * P.Hq;
+        TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
+        auto kern = attention_dq_kernel<T, BLOCKS>;
+        TPW_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::ALLOC));
+        kern<<<(unsigned)blocks, kTcThreads, L::ALLOC, s>>>(q, k, v, g, F);
+        TPW_LAUNCH_OK("attention_dq_kernel");
+    }
+    return TPW_OK;
+}
+
+} // namespace
+
+bool attn_tc_backward_fits(int dtype, const AttnParams &P) {
+    if (!attn_tc_fits(dtype, P) || !aligned16(P.dout) || !aligned16(P.dq) || !aligned16(P.dk) || !aligned16(P.dv)) return false;
+    for (int i = 0; i < 3; ++i)
+        if (P.do_s[i] % 8 != 0 || P.do_s[i] <= 0 || P.do_s[i] >= (1LL << 38)) return false;
+    return true;
+}
+
+int attn_tc_backward(int dtype, const AttnParams &P, cudaStream_t s) {
+    if (dtype == TPW_F16) return P.D <= 64 ? launch<__half, 1>(P, s) : launch<__half, 2>(P, s);
+    return P.D <= 64 ? launch<__nv_bfloat16, 1>(P, s) : launch<__nv_bfloat16, 2>(P, s);
+}
+
+} // namespace tpw

@@ -1,0 +1,337 @@
+// Attention forward on the tensor cores (16-bit types, up to 128 features).
+//
+// out_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i) in one pass over the keys with a running reference m_i of every row.
+// A CTA works on 256 queries of one head as two tiles of 128, each with a warpgroup of its own whose thread t owns row t; one more
+// warp issues TMA, one the MMAs.  Tensor memory holds, for each tile, the 128 x 128 scores and the output accumulators.  Per key tile: S = Q K^T
+// (both operands in shared memory), the row's thread reads its 128 scores, forms the probabilities, and writes them, rounded to
+// the inputs' type, over the scores; O += P V takes them from there.  While one tile's threads form probabilities the tensor cores work for the other.
+//
+// Bound: per pair of tiles 4 products of 128 x 128 x D, 2048 tensor-core clocks at D = 128, and 32768 exponentials, 2048 clocks of
+// the four special-function units: both pipes would be full at once.
+//
+// The reference m_i only moves when the maximum exceeds it by more than a factor 2^8 (the accumulators must then be read, scaled and written
+// back); until then probabilities up to 2^8 do no harm in fp32 sums.  Half precision additionally lifts them by 2^6: they
+// stay below 2^14, and lose digits only below 2^-20 of the row's largest.
+#include "attention_tc.cuh"
+
+namespace tpw {
+namespace {
+
+struct ForwardParams {
+    AttnParams a;
+    float scale_log2;
+    int tiles;          // of 256 queries
+};
+
+template <int BLOCKS> struct ForwardSmem {
+    static constexpr int kSlots = BLOCKS == 2 ? 4 : 6;
+    static constexpr uint32_t TILE_BYTES = BLOCKS * BLOCK_BYTES;
+    static constexpr uint32_t OFF_RING = 2 * TILE_BYTES;
+    static constexpr uint32_t OFF_BAR = OFF_RING + kSlots * TILE_BYTES;
+    static constexpr uint32_t OFF_TMEM = OFF_BAR + 8 * (2 * kSlots + 8);
+    static constexpr uint32_t ALLOC = OFF_TMEM + 16 + 1024;
+    static_assert(ALLOC <= 232448, "exceeds the dynamic shared memory of one CTA");
+};
+constexpr float kSlack = 8.f;
+
+template <typename T, int BLOCKS>
+__global__ void __launch_bounds__(kTcThreads, 1)
+attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                         const __grid_constant__ CUtensorMap map_v, const ForwardParams F) {
+    typedef ForwardSmem<BLOCKS> L;
+    typedef Narrow<T> N;
+    const AttnParams &P = F.a;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *empty = full + L::kSlots, *q_full = empty + L::kSlots,
+             *s_full = q_full + 1, *p_full = s_full + 2, *o_full = p_full + 2, *drained = o_full + 2;
+    uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(smem + L::OFF_TMEM);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_TMEM + 4);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long heads = P.B * P.Hq;
+    // a causal call's longest rows first, all heads of them together
+    const int tile = F.tiles - 1 - (int)(blockIdx.x / heads);
+    const long long bh = blockIdx.x % heads;
+    const int h = (int)(bh % P.Hq), b = (int)(bh / P.Hq), hk = h / (int)P.group;
+    const Seen see(P, b);
+    const int nq = (int)P.Nq, row0 = tile * 2 * TILE;
+    // key tiles [t_lo, t_hi) of each query tile, and of both
+    int t_lo[2], t_hi[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const int first = row0 + s * TILE, last = (first + TILE < nq ? first + TILE : nq) - 1;
+        t_lo[s] = see.lo(first) / TILE;
+        t_hi[s] = first < nq ? (see.hi(last) + TILE - 1) / TILE : 0;
+        if (t_hi[s] <= t_lo[s]) t_lo[s] = t_hi[s] = 0;
+    }
+    const bool some0 = t_hi[0] > 0, some1 = t_hi[1] > 0;
+    const int begin = some0 && (!some1 || t_lo[0] < t_lo[1]) ? t_lo[0] : t_lo[1], end = t_hi[0] > t_hi[1] ? t_hi[0] : t_hi[1];
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < L::kSlots; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        mbar_init(q_full, 1);
+        mbar_init(drained, 1);
+        for (int s = 0; s < 2; ++s) { mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
+        *abort_flag = 0;
+        mbar_init_fence();
+        tma_prefetch_descriptor(&map_q);
+        tma_prefetch_descriptor(&map_k);
+        tma_prefetch_descriptor(&map_v);
+    }
+    if (warp == 9) tmem_alloc(tmem_ptr, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_ptr;
+    auto give_up = [&](int site) {
+        *abort_flag = 1;
+        if (P.status) atomicCAS(P.status, 0, (16 << 16) | site);
+    };
+    // a wait of a whole warp, with the same answer in every lane
+    auto warp_wait = [&](uint64_t *bar, uint32_t parity, int site) {
+        const bool ok = __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag));
+        if (!ok) give_up(site);
+        return ok;
+    };
+    const uint32_t ring = smem_u32(smem + L::OFF_RING), q_at = smem_u32(smem);
+    const int uses = 2 * (end - begin);   // of the ring: K and V tiles in turn
+
+    if (warp >= 8) registers_down();
+    if (warp == 8) {
+        if (lane == 0 && uses > 0) {
+            uint32_t issued = 0;
+            mbar_expect_tx(q_full, 2 * L::TILE_BYTES);
+            load_tokens<BLOCKS>(q_at, &map_q, q_full, row0, h, b);
+            load_tokens<BLOCKS>(q_at + L::TILE_BYTES, &map_q, q_full, row0 + TILE, h, b);
+            for (int u = 0; u < uses; ++u) {
+                const uint32_t slot = u % L::kSlots;
+                if (u >= L::kSlots && !wait_or_abort(&empty[slot], parity_of_use(u, L::kSlots) ^ 1, abort_flag)) {
+                    give_up(1);
+                    break;
+                }
+                mbar_expect_tx(&full[slot], L::TILE_BYTES);
+                load_tokens<BLOCKS>(ring + slot * L::TILE_BYTES, u & 1 ? &map_v : &map_k, &full[slot], (begin + u / 2) * TILE, hk, b);
+                issued = u + 1;
+            }
+            // the commits that release the last uses have arrived before the CTA ends
+            for (uint32_t u = first_of_last_uses(issued, L::kSlots); u < issued; ++u)
+                if (!wait_or_abort(&empty[u % L::kSlots], parity_of_use(u, L::kSlots), abort_flag)) {
+                    give_up(2);
+                    break;
+                }
+            if (*abort_flag) {   // what was issued arrives before the CTA ends
+                mbar_wait_bounded(q_full, 0);
+                for (uint32_t u = first_of_last_uses(issued, L::kSlots); u < issued; ++u) mbar_wait_bounded(&full[u % L::kSlots], parity_of_use(u, L::kSlots));
+            }
+        }
+    } else if (warp == 9) {
+        const int steps = (int)(P.D + 15) / 16;
+        const uint32_t idesc_s = instruction(N::kFormat, TILE, false), idesc_o = instruction(N::kFormat, 16 * steps, true);
+        int done[2] = {0, 0};
+        bool ok = uses == 0 || warp_wait(q_full, 0, 3);
+        auto arrived = [&](int u) {
+            if (!warp_wait(&full[u % L::kSlots], parity_of_use(u, L::kSlots), 4)) return false;
+            tc_fence_after();
+            return true;
+        };
+        auto scores = [&](int s, int u) {
+            if (lane == 0) {
+                product_features(tmem + s * TILE, q_at + s * L::TILE_BYTES, ring + (u % L::kSlots) * L::TILE_BYTES, idesc_s, steps);
+                tc_commit<false>(&s_full[s]);
+            }
+        };
+        auto release = [&](int u) {
+            if (lane == 0) tc_commit<false>(&empty[u % L::kSlots]);
+        };
+        if (ok && uses > 0 && (ok = arrived(0))) {
+            for (int s = 0; s < 2; ++s)
+                if (t_lo[s] <= begin && begin < t_hi[s]) scores(s, 0);
+            release(0);
+        }
+        for (int t = begin; t < end && ok; ++t) {
+            const int u = 2 * (t - begin) + 1;   // of V; the next K is u + 1
+            if (!(ok = arrived(u))) break;
+            const int beyond = see.length - t * TILE;
+            if (beyond < TILE && (int)P.Nk > see.length) clear_tokens<BLOCKS>(smem + L::OFF_RING + (u % L::kSlots) * L::TILE_BYTES, beyond, lane);
+            if (t + 1 < end && !(ok = arrived(u + 1))) break;
+            for (int s = 0; s < 2 && ok; ++s) {
+                if (t_lo[s] <= t && t < t_hi[s]) {
+                    if (!(ok = warp_wait(&p_full[s], done[s] & 1, 5))) break;
+                    tc_fence_after();
+                    if (lane == 0) {
+                        product_tokens(tmem + (2 + s) * TILE, tmem + s * TILE, 32, ring + (u % L::kSlots) * L::TILE_BYTES, idesc_o, done[s] > 0);
+                        tc_commit<false>(&o_full[s]);
+                    }
+                    ++done[s];
+                }
+                if (t_lo[s] <= t + 1 && t + 1 < t_hi[s]) scores(s, u + 1);
+            }
+            release(u);
+            if (t + 1 < end) release(u + 1);
+        }
+        __syncwarp();
+    } else if (warp < 8) {
+        // ---- a query row per thread ----
+        registers_up();
+        const int s = warp >> 2, i = row0 + s * TILE + (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + s * TILE, o_at = tmem + lanes + (2 + s) * TILE;
+        const int lo = see.lo(i), hi = i < nq ? see.hi(i) : 0;
+        // tiles in [from, to) are seen whole by every row of this tile
+        const int first = row0 + s * TILE, last = (first + TILE < nq ? first + TILE : nq) - 1;
+        const int all_lo = see.lo(last), all_hi = see.hi(first);
+        const float c = F.scale_log2;
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        int n = 0;
+        for (int t = t_lo[s]; t < t_hi[s]; ++t, ++n) {
+            if (!(ok = warp_wait(&s_full[s], n & 1, 6))) break;
+            tc_fence_after();
+            uint32_t x[4][32];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) tmem_ld32(s_at + 32 * g, x[g]);
+            tmem_ld_wait();
+            const int j0 = t * TILE;
+            if (j0 < all_lo || j0 + TILE > all_hi) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const int j = j0 + 32 * g + e;
+                        if (j < lo || j >= hi) x[g][e] = 0xff800000u;
+                    }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) top = max3(top, __uint_as_float(x[g][e]), __uint_as_float(x[g][e + 1]));
+            const bool moves = m == -INFINITY ? top > -INFINITY : (top - m) * c > kSlack;
+            const bool scales = moves && m != -INFINITY;   // so far only zeros were added otherwise
+            if (__any_sync(0xffffffffu, scales)) {
+                const float by = scales ? exp2_fast((m - top) * c) : 1.f;
+                l *= by;
+                if (!(ok = warp_wait(&o_full[s], (n - 1) & 1, 7))) break;
+                tc_fence_after();
+                for (int g = 0; g < 2 * BLOCKS; ++g) {
+                    uint32_t o[32];
+                    tmem_ld32(o_at + 32 * g, o);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * by);
+                    tmem_st32(o_at + 32 * g, o);
+                }
+            }
+            if (moves) m = top;
+            const float shift = m == -INFINITY ? 0.f : N::kLift - m * c;
+            const f32x2 c2 = pack2(c, c), shift2 = pack2(shift, shift);
+            f32x2 sum = pack2(0.f, 0.f);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                uint32_t p[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    const uint32_t *pair = &x[2 * g + (e >> 4)][2 * (e & 15)];
+                    const f32x2 z = fma2(pack2(__uint_as_float(pair[0]), __uint_as_float(pair[1])), c2, shift2);
+                    float z0, z1;
+                    unpack2(z, z0, z1);
+                    z0 = exp2_fast(z0);
+                    z1 = exp2_fast(z1);
+                    sum = add2(sum, pack2(z0, z1));
+                    p[e] = N::pack(z0, z1);
+                }
+                tmem_st32(s_at + 32 * g, p);
+            }
+            float s0, s1;
+            unpack2(sum, s0, s1);
+            l += s0 + s1;
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[s]);
+        }
+        if (ok && n > 0) {
+            ok = warp_wait(&o_full[s], (n - 1) & 1, 8);
+            tc_fence_after();
+        }
+        if (ok) {
+            const float by = l == 0.f ? 0.f : 1.f / l;
+            if (i < nq && P.lse)
+                static_cast<float *>(P.lse)[bh * P.Nq + i] = l == 0.f ? -INFINITY : (m * c - N::kLift + log2f(l)) * 0.69314718055994531f;
+            T *out = static_cast<T *>(P.out) + ((b * P.Nq + i) * P.Hq + h) * P.D;
+#pragma unroll 1
+            for (int g = 0; g < 2 * BLOCKS; ++g) {
+                uint32_t o[32];
+                if (n > 0) {
+                    tmem_ld32(o_at + 32 * g, o);
+                    tmem_ld_wait();
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float a0 = n > 0 && l != 0.f ? __uint_as_float(o[e + 2 * k]) * by : 0.f, a1 = n > 0 && l != 0.f ? __uint_as_float(o[e + 2 * k + 1]) * by : 0.f;
+                        w[k] = N::pack(a0, a1);
+                    }
+                    const int d = 32 * g + e;
+                    if (i < nq && d < (int)P.D) *reinterpret_cast<uint4 *>(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        // all MMAs are over: the commits behind them were waited for, or, after a wait that gave up, one more is waited for here
+        if (*abort_flag && lane == 0) {
+            tc_commit<false>(drained);
+            mbar_wait_bounded(drained, 0);
+        }
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <typename T, int BLOCKS> int launch(const AttnParams &P, cudaStream_t s) {
+    typedef ForwardSmem<BLOCKS> L;
+    ForwardParams F = {};
+    F.a = P;
+    F.a.status = device_status_ptr();
+    F.scale_log2 = (float)(P.scale * 1.4426950408889634074);
+    F.tiles = (int)((P.Nq + 2 * TILE - 1) / (2 * TILE));
+    CUtensorMap q, k, v;
+    int e = make_tensor_map_heads(&q, P.q, P.D, P.Nq, P.Hq, P.B, 2 * P.q_s[1], 2 * P.q_s[2], 2 * P.q_s[0], TILE);
+    if (e == TPW_OK) e = make_tensor_map_heads(&k, P.k, P.D, P.Nk, P.Hk, P.B, 2 * P.k_s[1], 2 * P.k_s[2], 2 * P.k_s[0], TILE);
+    if (e == TPW_OK) e = make_tensor_map_heads(&v, P.v, P.D, P.Nk, P.Hk, P.B, 2 * P.v_s[1], 2 * P.v_s[2], 2 * P.v_s[0], TILE);
+    if (e != TPW_OK) return e;
+    const long long blocks = F.tiles * P.B * P.Hq;
+    TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
+    auto kern = attention_forward_kernel<T, BLOCKS>;
+    TPW_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::ALLOC));
+    kern<<<(unsigned)blocks, kTcThreads, L::ALLOC, s>>>(q, k, v, F);
+    TPW_LAUNCH_OK("attention_forward_kernel");
+    return TPW_OK;
+}
+
+} // namespace
+
+// Rows must start on 16-byte boundaries (TMA, 16-byte stores), and tensors must not be empty.
+bool attn_tc_fits(int dtype, const AttnParams &P) {
+    if (dtype != TPW_F16 && dtype != TPW_BF16) return false;
+    if (tma_disabled() || P.D % 8 != 0 || P.D > 128 || P.Nk == 0) return false;
+    auto fits = [](const void *p, const long long (&st)[3]) {
+        for (int i = 0; i < 3; ++i)
+            if (st[i] % 8 != 0 || st[i] <= 0 || st[i] >= (1LL << 38)) return false;
+        return aligned16(p);
+    };
+    return fits(P.q, P.q_s) && fits(P.k, P.k_s) && fits(P.v, P.v_s) && aligned16(P.out);
+}
+
+int attn_tc_forward(int dtype, const AttnParams &P, cudaStream_t s) {
+    if (dtype == TPW_F16) return P.D <= 64 ? launch<__half, 1>(P, s) : launch<__half, 2>(P, s);
+    return P.D <= 64 ? launch<__nv_bfloat16, 1>(P, s) : launch<__nv_bfloat16, 2>(P, s);
+}
+
+} // namespace tpw

@@ -1,0 +1,133 @@
+// What the tensor-core attention kernels share: tcgen05 wrappers for 16-bit operands, tiles of [tokens, features] in shared memory
+// and their descriptors, and the exponential.
+//
+// A tile of 128 tokens lies in shared memory as one or two blocks of 64 features (128 tokens x 128 bytes, 128-byte swizzle), 16 KB each,
+// as TMA writes it.  The same bytes serve a product that contracts the features (K-major operand) and one that contracts the tokens
+// (MN-major operand).
+#pragma once
+#include "attention.cuh"
+#include "packed_f32x2.cuh"
+#include "tcgen05.cuh"
+
+namespace tpw {
+namespace {
+
+constexpr int TILE = 128;                  // tokens per tile
+constexpr uint32_t BLOCK_BYTES = 16384;    // 128 tokens x 64 features
+
+template <typename T> struct Narrow;
+template <> struct Narrow<__nv_bfloat16> {
+    static constexpr uint32_t kFormat = 1;   // of the instruction descriptor
+    static constexpr float kLift = 0.f;      // probabilities are formed times 2^kLift: bfloat16 has the exponents of float32
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+};
+template <> struct Narrow<__half> {
+    static constexpr uint32_t kFormat = 0;
+    static constexpr float kLift = 6.f;      // and half precision loses digits below 2^-14: see attention_forward.cu
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+};
+
+// D[tmem] (+)= A[smem] B[smem] and D[tmem] (+)= A[tmem] B[smem]; operands of one 16-bit type, fp32 accumulate, K = 16
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// fp32 accumulators (bits [4,6) = 1), A and B formats in [7,10) and [10,13), bit 16: B is MN-major, N >> 3 in [17,23), M >> 4 in [24,29)
+__device__ __forceinline__ uint32_t instruction(uint32_t format, uint32_t n, bool b_mn) {
+    return (1u << 4) | (format << 7) | (format << 10) | ((b_mn ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24);
+}
+// MN-major 16-bit tile, 128-byte swizzle: groups of eight tokens 1024 bytes apart, blocks of 64 features BLOCK_BYTES apart
+__device__ __forceinline__ uint64_t make_smem_desc_tokens(uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr & 0x3FFFF) >> 4);
+    d |= (uint64_t)(BLOCK_BYTES >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+// start of the k-th 16 features of a K-major tile, in units of 16 bytes
+__device__ __forceinline__ uint64_t feature_step(int k) { return (uint64_t)((k >> 2) * (BLOCK_BYTES >> 4) + (k & 3) * 2); }
+// D (+)= X Y^T over the features; X, Y tiles
+__device__ __forceinline__ void product_features(uint32_t d, uint32_t x, uint32_t y, uint32_t idesc, int steps) {
+    const uint64_t a = make_smem_desc(x), b = make_smem_desc(y);
+    for (int k = 0; k < steps; ++k) mma_ss(d, a + feature_step(k), b + feature_step(k), idesc, k != 0);
+}
+// D (+)= P Y over 128 tokens; P in tensor memory, 16 tokens to 8 columns, its second half `gap` columns behind the first's start
+__device__ __forceinline__ void product_tokens(uint32_t d, uint32_t p, uint32_t gap, uint32_t y, uint32_t idesc, bool accumulate) {
+    const uint64_t b = make_smem_desc_tokens(y);
+#pragma unroll
+    for (int k = 0; k < TILE / 16; ++k)
+        mma_ts(d, p + (k < 4 ? 8 * k : gap + 8 * (k - 4)), b + (uint64_t)k * (2048 >> 4), idesc, accumulate || k != 0);
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+        "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint64_t *bar, int c0, int c1, int c2, int c3) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+        : "memory");
+}
+// tile of 128 tokens, BLOCKS blocks of 64 features
+template <int BLOCKS>
+__device__ __forceinline__ void load_tokens(uint32_t dst, const CUtensorMap *map, uint64_t *bar, int token, int head, int batch) {
+#pragma unroll
+    for (int c = 0; c < BLOCKS; ++c) tma_load_4d(dst + c * BLOCK_BYTES, map, bar, 64 * c, token, head, batch);
+}
+// Tokens [from, 128) of a tile set to zero by one warp, visible to the tensor cores: what lies there belongs to no key, and 0 times it
+// need not be 0.
+template <int BLOCKS> __device__ __forceinline__ void clear_tokens(unsigned char *tile, int from, int lane) {
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    for (int c = 0; c < BLOCKS; ++c)
+        for (int at = from * 8 + lane; at < TILE * 8; at += 32) *reinterpret_cast<uint4 *>(tile + c * BLOCK_BYTES + at * 16) = zero;
+    fence_proxy_async_smem();
+    __syncwarp();
+}
+
+// Registers per thread of a warpgroup.  A block of 384 threads is launched with 168 each, 64512: two warpgroups at 200 and one at 104.
+constexpr int kTcThreads = 384;
+__device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 200;"); }
+__device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 104;"); }
+
+__device__ __forceinline__ float exp2_fast(float x) {   // 2 units of the last place; 0 below 2^-126
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+} // namespace
+} // namespace tpw
