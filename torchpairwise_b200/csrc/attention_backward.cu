@@ -101,7 +101,7 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(smem + L::OFF_TMEM);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_TMEM + 4);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const long long heads = P.B * P.Hk;
     const int row0 = (int)(blockIdx.x / heads) * TILE;   // a causal call's first keys are seen by most queries
     const long long bh = blockIdx.x % heads;
@@ -132,7 +132,7 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_ptr;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
     auto give_up = [&](int site) {
         *abort_flag = 1;
         if (P.status) atomicCAS(P.status, 0, (17 << 16) | site);
@@ -186,16 +186,15 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     } else if (warp == 9) {
         const int steps = (int)(P.D + 15) / 16;
         const uint32_t idesc_s = instruction(N::kFormat, TILE, false), idesc_d = instruction(N::kFormat, 16 * steps, true);
+        const uint32_t leader = elect_lane();
         bool ok = total == 0 || warp_wait(kv_full, 0, 3);
         // S^T or dP^T of use u, once its tile has arrived
         auto first = [&](uint64_t *arrives, int u, uint32_t d, uint32_t own, uint32_t offset, uint64_t *done, int site) {
             const uint32_t st = u % L::kStages;
             if (!warp_wait(&arrives[st], parity_of_use(u, L::kStages), site)) return false;
             tc_fence_after();
-            if (lane == 0) {
-                product_features(d, own, ring + st * 2 * L::TILE_BYTES + offset, idesc_s, steps);
-                tc_commit<false>(done);
-            }
+            product_features<BLOCKS>(leader, d, own, ring + st * 2 * L::TILE_BYTES + offset, idesc_s, steps);
+            commit_by(leader, done);
             return true;
         };
         if (total > 0 && ok) ok = first(q_full, 0, S, k_at, 0, s_full, 4) && first(g_full, 0, DP, v_at, L::TILE_BYTES, dp_full, 5);
@@ -203,17 +202,15 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
             const uint32_t q_at = ring + (u % L::kStages) * 2 * L::TILE_BYTES;
             if (!(ok = warp_wait(p_ready, u & 1, 6))) break;
             tc_fence_after();
-            if (lane == 0) product_tokens(DV, S, 64, q_at + L::TILE_BYTES, idesc_d, u > 0);
+            product_tokens(leader, DV, S, 64, q_at + L::TILE_BYTES, idesc_d, u > 0);
             if (u + 1 < total && !(ok = first(q_full, u + 1, S, k_at, 0, s_full, 4))) break;
             if (!(ok = warp_wait(ds_ready, u & 1, 7))) break;
             tc_fence_after();
-            if (lane == 0) {
-                product_tokens(DK, DP, 64, q_at, idesc_d, u > 0);
-                tc_commit<false>(&empty[u % L::kStages]);
-            }
+            product_tokens(leader, DK, DP, 64, q_at, idesc_d, u > 0);
+            commit_by(leader, &empty[u % L::kStages]);
             if (u + 1 < total && !(ok = first(g_full, u + 1, DP, v_at, L::TILE_BYTES, dp_full, 5))) break;
         }
-        if (ok && total > 0 && lane == 0) tc_commit<false>(acc_full);
+        if (ok && total > 0) commit_by(leader, acc_full);
         __syncwarp();
     } else if (warp < 8) {
         // ---- a key row and 64 query columns per thread ----
@@ -344,7 +341,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(smem + L::OFF_TMEM);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_TMEM + 4);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const long long heads = P.B * P.Hq;
     const int row0 = (F.tiles - 1 - (int)(blockIdx.x / heads)) * TILE;   // a causal call's longest rows first
     const long long bh = blockIdx.x % heads;
@@ -375,7 +372,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_ptr;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
     auto give_up = [&](int site) {
         *abort_flag = 1;
         if (P.status) atomicCAS(P.status, 0, (18 << 16) | site);
@@ -419,6 +416,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     } else if (warp == 9) {
         const int steps = (int)(P.D + 15) / 16;
         const uint32_t idesc_s = instruction(N::kFormat, TILE, false), idesc_d = instruction(N::kFormat, 16 * steps, true);
+        const uint32_t leader = elect_lane();
         bool ok = total == 0 || warp_wait(own_full, 0, 3);
         auto first = [&](int u) {   // S and dP of key tile u
             const uint32_t st = u % L::kStages, at = ring + st * 2 * L::TILE_BYTES;
@@ -426,12 +424,10 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             tc_fence_after();
             const int beyond = see.length - (begin + u) * TILE;
             if (beyond < TILE && (int)P.Nk > see.length) clear_tokens<BLOCKS>(smem + L::OFF_RING + st * 2 * L::TILE_BYTES, beyond, lane);
-            if (lane == 0) {
-                product_features(S, q_at, at, idesc_s, steps);
-                tc_commit<false>(s_full);
-                product_features(DP + (u & 1) * TILE, g_at, at + L::TILE_BYTES, idesc_s, steps);
-                tc_commit<false>(&dp_full[u & 1]);
-            }
+            product_features<BLOCKS>(leader, S, q_at, at, idesc_s, steps);
+            commit_by(leader, s_full);
+            product_features<BLOCKS>(leader, DP + (u & 1) * TILE, g_at, at + L::TILE_BYTES, idesc_s, steps);
+            commit_by(leader, &dp_full[u & 1]);
             return true;
         };
         if (total > 0 && ok) ok = first(0);
@@ -443,12 +439,10 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             }
             if (!(ok = warp_wait(ds_ready, u & 1, 6))) break;
             tc_fence_after();
-            if (lane == 0) {
-                product_tokens(DQ, DP + (u & 1) * TILE, 64, ring + (u % L::kStages) * 2 * L::TILE_BYTES, idesc_d, u > 0);
-                tc_commit<false>(&empty[u % L::kStages]);
-            }
+            product_tokens(leader, DQ, DP + (u & 1) * TILE, 64, ring + (u % L::kStages) * 2 * L::TILE_BYTES, idesc_d, u > 0);
+            commit_by(leader, &empty[u % L::kStages]);
         }
-        if (ok && total > 0 && lane == 0) tc_commit<false>(acc_full);
+        if (ok && total > 0) commit_by(leader, acc_full);
         __syncwarp();
     } else if (warp < 8) {
         // ---- a query row and 64 key columns per thread ----

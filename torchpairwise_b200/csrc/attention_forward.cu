@@ -48,7 +48,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(smem + L::OFF_TMEM);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_TMEM + 4);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const long long heads = P.B * P.Hq;
     // a causal call's longest rows first, all heads of them together
     const int tile = F.tiles - 1 - (int)(blockIdx.x / heads);
@@ -83,7 +83,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_ptr;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
     auto give_up = [&](int site) {
         *abort_flag = 1;
         if (P.status) atomicCAS(P.status, 0, (16 << 16) | site);
@@ -128,6 +128,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     } else if (warp == 9) {
         const int steps = (int)(P.D + 15) / 16;
         const uint32_t idesc_s = instruction(N::kFormat, TILE, false), idesc_o = instruction(N::kFormat, 16 * steps, true);
+        const uint32_t leader = elect_lane();
         int done[2] = {0, 0};
         bool ok = uses == 0 || warp_wait(q_full, 0, 3);
         auto arrived = [&](int u) {
@@ -136,13 +137,11 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             return true;
         };
         auto scores = [&](int s, int u) {
-            if (lane == 0) {
-                product_features(tmem + s * TILE, q_at + s * L::TILE_BYTES, ring + (u % L::kSlots) * L::TILE_BYTES, idesc_s, steps);
-                tc_commit<false>(&s_full[s]);
-            }
+            product_features<BLOCKS>(leader, tmem + s * TILE, q_at + s * L::TILE_BYTES, ring + (u % L::kSlots) * L::TILE_BYTES, idesc_s, steps);
+            commit_by(leader, &s_full[s]);
         };
         auto release = [&](int u) {
-            if (lane == 0) tc_commit<false>(&empty[u % L::kSlots]);
+            commit_by(leader, &empty[u % L::kSlots]);
         };
         if (ok && uses > 0 && (ok = arrived(0))) {
             for (int s = 0; s < 2; ++s)
@@ -159,10 +158,8 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 if (t_lo[s] <= t && t < t_hi[s]) {
                     if (!(ok = warp_wait(&p_full[s], done[s] & 1, 5))) break;
                     tc_fence_after();
-                    if (lane == 0) {
-                        product_tokens(tmem + (2 + s) * TILE, tmem + s * TILE, 32, ring + (u % L::kSlots) * L::TILE_BYTES, idesc_o, done[s] > 0);
-                        tc_commit<false>(&o_full[s]);
-                    }
+                    product_tokens(leader, tmem + (2 + s) * TILE, tmem + s * TILE, 32, ring + (u % L::kSlots) * L::TILE_BYTES, idesc_o, done[s] > 0);
+                    commit_by(leader, &o_full[s]);
                     ++done[s];
                 }
                 if (t_lo[s] <= t + 1 && t + 1 < t_hi[s]) scores(s, u + 1);
@@ -201,11 +198,12 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         if (j < lo || j >= hi) x[g][e] = 0xff800000u;
                     }
             }
-            float top = -INFINITY;
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
+            for (int e = 0; e < 32; e += 2)
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) top = max3(top, __uint_as_float(x[g][e]), __uint_as_float(x[g][e + 1]));
+                for (int g = 0; g < 4; ++g) tops[g] = max3(tops[g], __uint_as_float(x[g][e]), __uint_as_float(x[g][e + 1]));
+            const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
             const bool moves = m == -INFINITY ? top > -INFINITY : (top - m) * c > kSlack;
             const bool scales = moves && m != -INFINITY;   // so far only zeros were added otherwise
             if (__any_sync(0xffffffffu, scales)) {

@@ -35,17 +35,30 @@ template <> struct Narrow<__half> {
     }
 };
 
+// The lane that issues for its warp.  The whole warp runs through the issuing code and the instructions themselves are predicated: their operands
+// then live in uniform registers.  Under a branch on the lane the compiler moves every operand there anew, 80 to 125 clocks per MMA.
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
+}
 // D[tmem] (+)= A[smem] B[smem] and D[tmem] (+)= A[tmem] B[smem]; operands of one 16-bit type, fp32 accumulate, K = 16
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
+        : "memory");
+}
+__device__ __forceinline__ void commit_by(uint32_t leader, uint64_t *bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(leader)
         : "memory");
 }
 // fp32 accumulators (bits [4,6) = 1), A and B formats in [7,10) and [10,13), bit 16: B is MN-major, N >> 3 in [17,23), M >> 4 in [24,29)
@@ -64,17 +77,19 @@ __device__ __forceinline__ uint64_t make_smem_desc_tokens(uint32_t smem_addr) {
 }
 // start of the k-th 16 features of a K-major tile, in units of 16 bytes
 __device__ __forceinline__ uint64_t feature_step(int k) { return (uint64_t)((k >> 2) * (BLOCK_BYTES >> 4) + (k & 3) * 2); }
-// D (+)= X Y^T over the features; X, Y tiles
-__device__ __forceinline__ void product_features(uint32_t d, uint32_t x, uint32_t y, uint32_t idesc, int steps) {
+// D = X Y^T over 16 * steps features, at most 64 * BLOCKS; X, Y tiles
+template <int BLOCKS> __device__ __forceinline__ void product_features(uint32_t leader, uint32_t d, uint32_t x, uint32_t y, uint32_t idesc, int steps) {
     const uint64_t a = make_smem_desc(x), b = make_smem_desc(y);
-    for (int k = 0; k < steps; ++k) mma_ss(d, a + feature_step(k), b + feature_step(k), idesc, k != 0);
+#pragma unroll
+    for (int k = 0; k < 4 * BLOCKS; ++k)
+        if (k < steps) mma_ss(leader, d, a + feature_step(k), b + feature_step(k), idesc, k != 0);
 }
 // D (+)= P Y over 128 tokens; P in tensor memory, 16 tokens to 8 columns, its second half `gap` columns behind the first's start
-__device__ __forceinline__ void product_tokens(uint32_t d, uint32_t p, uint32_t gap, uint32_t y, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void product_tokens(uint32_t leader, uint32_t d, uint32_t p, uint32_t gap, uint32_t y, uint32_t idesc, bool accumulate) {
     const uint64_t b = make_smem_desc_tokens(y);
 #pragma unroll
     for (int k = 0; k < TILE / 16; ++k)
-        mma_ts(d, p + (k < 4 ? 8 * k : gap + 8 * (k - 4)), b + (uint64_t)k * (2048 >> 4), idesc, accumulate || k != 0);
+        mma_ts(leader, d, p + (k < 4 ? 8 * k : gap + 8 * (k - 4)), b + (uint64_t)k * (2048 >> 4), idesc, accumulate || k != 0);
 }
 
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
