@@ -44,10 +44,12 @@ template <> struct Lift<__half> {
 template <int BLOCKS> struct BackwardSmem {
     static constexpr int kStages = BLOCKS == 2 ? 2 : 3;
     static constexpr uint32_t TILE_BYTES = BLOCKS * BLOCK_BYTES;
-    static constexpr uint32_t OFF_RING = 2 * TILE_BYTES;                       // the CTA's own two tiles, then pairs of walked tiles
+    static constexpr uint32_t OFF_RING = 2 * TILE_BYTES;                       // the CTA's own two tiles, then the walked tiles
     static constexpr uint32_t OFF_ROWS = OFF_RING + kStages * 2 * TILE_BYTES;  // lse, delta of a query tile per stage
     static constexpr uint32_t OFF_BAR = OFF_ROWS + kStages * 2 * TILE * 4;
-    static constexpr uint32_t OFF_TMEM = OFF_BAR + 8 * (3 * kStages + 10);
+    static constexpr uint32_t OFF_TMEM = OFF_BAR + 8 * (4 * kStages + 10);
+    // queries walk: a V tile is free again once dP has read it, a K tile only after dQ
+    static constexpr int kKeys = BLOCKS == 2 ? 3 : 4, kValues = 2 * kStages - kKeys;
     static constexpr uint32_t ALLOC = OFF_TMEM + 16 + 1024;
     static_assert(ALLOC <= 232448, "exceeds the dynamic shared memory of one CTA");
 };
@@ -213,100 +215,105 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         if (ok && total > 0) commit_by(leader, acc_full);
         __syncwarp();
     } else if (warp < 8) {
-        // ---- a key row and 64 query columns per thread ----
+        // ---- 32 key rows and 64 query columns per warp ----
+        // Loads of 16 lanes x 256 bits spread them like an mma accumulator: thread 4 g + t has rows g, g + 8, g + 16, g + 24 and of every
+        // eight columns 2 t and 2 t + 1.  It needs 16 of the columns' lse and delta; with a row per thread it would be all 64, 16 bytes
+        // at a time to every lane, 1300 shared-memory wavefronts per tile beside operands that the MMAs read at the full rate.
         registers_up();
-        const int half = warp >> 2, j = row0 + (warp & 3) * 32 + lane;
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const int half = warp >> 2, g = lane >> 2, t = lane & 3;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, upper = 16u << 16;
         const uint32_t s_at = S + lanes + 64 * half, dp_at = DP + lanes + 64 * half;
-        const int lo = see.qlo(j), hi = see.window ? see.qhi(j) : 0x7fffffff;
         // query tiles from all_lo on, and below all_hi, are seen by every key of the tile; keys beyond the length are not stored
         const int all_lo = see.qlo(row0 + TILE - 1), all_hi = see.window ? row0 - see.off + see.window : 0x7fffffff;
         const float c = F.scale_log2, lift = Lift<T>::factor(P.row_max);
         const f32x2 c2 = pack2(c, c), lift2 = pack2(lift, lift);
+        // index 2 i + r of a half's 16 pairs: columns 8 i + 2 t and the next, row g + 8 r (and 16 in the upper half)
+        auto hide = [&](f32x2 (&p)[2][16], int i0) {
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int j = row0 + (warp & 3) * 32 + 16 * hh + 8 * r + g, lo = see.qlo(j), hi = see.window ? see.qhi(j) : 0x7fffffff;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int at = i0 + 64 * half + 8 * i + 2 * t;
+                        float p0, p1;
+                        unpack2(p[hh][2 * i + r], p0, p1);
+                        p[hh][2 * i + r] = pack2(at >= lo && at < hi ? p0 : 0.f, at + 1 >= lo && at + 1 < hi ? p1 : 0.f);
+                    }
+                }
+        };
+        auto hand_over = [&](const f32x2 (&p)[2][16], uint32_t at, uint64_t *bar) {
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                uint32_t w[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float p0, p1;
+                    unpack2(p[hh][e], p0, p1);
+                    w[e] = N::pack(p0, p1);
+                }
+                tmem_st_16x128(at + hh * upper, w);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
         bool ok = true;
         for (int u = 0; u < total; ++u) {
             const uint32_t st = u % L::kStages;
-            const float *rows = reinterpret_cast<const float *>(smem + L::OFF_ROWS + st * 2 * TILE * 4) + 64 * half;
+            const float *rows = reinterpret_cast<const float *>(smem + L::OFF_ROWS + st * 2 * TILE * 4) + 64 * half + 2 * t;
             const int i0 = (begin + u % per_head) * TILE;
             if (!(ok = warp_wait(s_full, u & 1, 8) && warp_wait(&q_full[st], parity_of_use(u, L::kStages), 9))) break;
             tc_fence_after();
             uint32_t x[2][32];
-            tmem_ld32(s_at, x[0]);
-            tmem_ld32(s_at + 32, x[1]);
+            tmem_ld_16x256(s_at, x[0]);
+            tmem_ld_16x256(s_at + upper, x[1]);
             tmem_ld_wait();
             const bool masked = i0 < all_lo || i0 + TILE > all_hi;
-            f32x2 p[32];
+            f32x2 p[2][16];
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-                const float4 minus_lse = *reinterpret_cast<const float4 *>(rows + 2 * e);
+            for (int i = 0; i < 8; ++i) {
+                const f32x2 minus_lse = *reinterpret_cast<const f32x2 *>(rows + 8 * i);
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint32_t *pair = &x[(e + k) >> 4][2 * ((e + k) & 15)];
-                    const f32x2 z = fma2(pack2(__uint_as_float(pair[0]), __uint_as_float(pair[1])), c2,
-                                         k ? pack2(minus_lse.z, minus_lse.w) : pack2(minus_lse.x, minus_lse.y));
-                    float z0, z1;
-                    unpack2(z, z0, z1);
-                    p[e + k] = pack2(exp2_fast(z0), exp2_fast(z1));
-                }
+                for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const uint32_t *pair = &x[hh][4 * i + 2 * r];
+                        float z0, z1;
+                        unpack2(fma2(pack2(__uint_as_float(pair[0]), __uint_as_float(pair[1])), c2, minus_lse), z0, z1);
+                        p[hh][2 * i + r] = pack2(exp2_fast(z0), exp2_fast(z1));
+                    }
             }
-            if (masked) {
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    const int i = i0 + 64 * half + 2 * e;
-                    float p0, p1;
-                    unpack2(p[e], p0, p1);
-                    p[e] = pack2(i >= lo && i < hi ? p0 : 0.f, i + 1 >= lo && i + 1 < hi ? p1 : 0.f);
-                }
-            }
-            {
-                uint32_t w[32];
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    float p0, p1;
-                    unpack2(p[e], p0, p1);
-                    w[e] = N::pack(p0, p1);
-                }
-                tmem_st32(s_at, w);
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_ready);
-            }
+            if (masked) hide(p, i0);
+            hand_over(p, s_at, p_ready);
             if (!(ok = warp_wait(dp_full, u & 1, 10) && warp_wait(&g_full[st], parity_of_use(u, L::kStages), 11))) break;
             tc_fence_after();
-            tmem_ld32(dp_at, x[0]);
-            tmem_ld32(dp_at + 32, x[1]);
+            tmem_ld_16x256(dp_at, x[0]);
+            tmem_ld_16x256(dp_at + upper, x[1]);
             tmem_ld_wait();
-            uint32_t w[32];
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-                const float4 minus_delta = *reinterpret_cast<const float4 *>(rows + TILE + 2 * e);
+            for (int i = 0; i < 8; ++i) {
+                const f32x2 minus_delta = *reinterpret_cast<const f32x2 *>(rows + TILE + 8 * i);
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint32_t *pair = &x[(e + k) >> 4][2 * ((e + k) & 15)];
-                    const f32x2 ds = score_gradient<Lift<T>::kNeeded>(p[e + k], pack2(__uint_as_float(pair[0]), __uint_as_float(pair[1])),
-                                                                     k ? pack2(minus_delta.z, minus_delta.w) : pack2(minus_delta.x, minus_delta.y), lift2);
-                    float d0, d1;
-                    unpack2(ds, d0, d1);
-                    if (masked) {   // 0 times what need not be finite
-                        const int i = i0 + 64 * half + 2 * (e + k);
-                        d0 = i >= lo && i < hi ? d0 : 0.f;
-                        d1 = i + 1 >= lo && i + 1 < hi ? d1 : 0.f;
+                for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const uint32_t *pair = &x[hh][4 * i + 2 * r];
+                        p[hh][2 * i + r] = score_gradient<Lift<T>::kNeeded>(p[hh][2 * i + r], pack2(__uint_as_float(pair[0]), __uint_as_float(pair[1])),
+                                                                           minus_delta, lift2);
                     }
-                    w[e + k] = N::pack(d0, d1);
-                }
             }
-            tmem_st32(dp_at, w);
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(ds_ready);
+            if (masked) hide(p, i0);   // 0 times what need not be finite
+            hand_over(p, dp_at, ds_ready);
         }
         if (ok && total > 0) {
             ok = warp_wait(acc_full, 0, 12);
             tc_fence_after();
         }
         if (ok) {
+            const int j = row0 + (warp & 3) * 32 + lane;
             const bool keep = total > 0 && j < see.length, valid = j < (int)P.Nk;
             const long long to = ((b * P.Nk + j) * P.Hk + hk) * P.D;
             const float down = Lift<T>::kNeeded ? 0.000244140625f : 1.f;   // 2^-12
@@ -336,7 +343,8 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const AttnParams &P = F.a;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *empty = full + L::kStages, *own_full = empty + L::kStages, *s_full = own_full + 1,
+    uint64_t *k_full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *k_empty = k_full + L::kKeys, *v_full = k_empty + L::kKeys,
+             *v_empty = v_full + L::kValues, *own_full = v_empty + L::kValues, *s_full = own_full + 1,
              *s_read = s_full + 1, *dp_full = s_read + 1, *ds_ready = dp_full + 2, *acc_full = ds_ready + 1, *drained = acc_full + 1;
     uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(smem + L::OFF_TMEM);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_TMEM + 4);
@@ -352,7 +360,8 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const int total = end > begin ? end - begin : 0;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < L::kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < L::kKeys; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
+        for (int i = 0; i < L::kValues; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
         mbar_init(own_full, 1);
         mbar_init(s_full, 1);
         mbar_init(s_read, 8);
@@ -382,35 +391,38 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         if (!ok) give_up(site);
         return ok;
     };
-    const uint32_t q_at = smem_u32(smem), g_at = q_at + L::TILE_BYTES, ring = smem_u32(smem + L::OFF_RING);
+    const uint32_t q_at = smem_u32(smem), g_at = q_at + L::TILE_BYTES, keys = smem_u32(smem + L::OFF_RING), values = keys + L::kKeys * L::TILE_BYTES;
     const uint32_t S = tmem, DP = tmem + TILE, DQ = tmem + 3 * TILE;
 
     if (warp >= 8) registers_down();
     if (warp == 8) {
         if (lane == 0 && total > 0) {
-            uint32_t issued = 0;
+            uint32_t issued_k = 0, issued_v = 0;
             mbar_expect_tx(own_full, 2 * L::TILE_BYTES);
             load_tokens<BLOCKS>(q_at, &map_q, own_full, row0, h, b);
             load_tokens<BLOCKS>(g_at, &map_g, own_full, row0, h, b);
             for (int u = 0; u < total; ++u) {
-                const uint32_t st = u % L::kStages;
-                if (u >= L::kStages && !wait_or_abort(&empty[st], parity_of_use(u, L::kStages) ^ 1, abort_flag)) {
+                const uint32_t sk = u % L::kKeys, sv = u % L::kValues;
+                if (u >= L::kKeys && !wait_or_abort(&k_empty[sk], parity_of_use(u, L::kKeys) ^ 1, abort_flag)) {
                     give_up(1);
                     break;
                 }
-                mbar_expect_tx(&full[st], 2 * L::TILE_BYTES);
-                load_tokens<BLOCKS>(ring + st * 2 * L::TILE_BYTES, &map_k, &full[st], (begin + u) * TILE, hk, b);
-                load_tokens<BLOCKS>(ring + st * 2 * L::TILE_BYTES + L::TILE_BYTES, &map_v, &full[st], (begin + u) * TILE, hk, b);
-                issued = u + 1;
-            }
-            for (uint32_t u = first_of_last_uses(issued, L::kStages); u < issued; ++u)
-                if (!wait_or_abort(&empty[u % L::kStages], parity_of_use(u, L::kStages), abort_flag)) {
-                    give_up(2);
+                mbar_expect_tx(&k_full[sk], L::TILE_BYTES);
+                load_tokens<BLOCKS>(keys + sk * L::TILE_BYTES, &map_k, &k_full[sk], (begin + u) * TILE, hk, b);
+                issued_k = u + 1;
+                if (u >= L::kValues && !wait_or_abort(&v_empty[sv], parity_of_use(u, L::kValues) ^ 1, abort_flag)) {
+                    give_up(1);
                     break;
                 }
+                mbar_expect_tx(&v_full[sv], L::TILE_BYTES);
+                load_tokens<BLOCKS>(values + sv * L::TILE_BYTES, &map_v, &v_full[sv], (begin + u) * TILE, hk, b);
+                issued_v = u + 1;
+            }
+            if (!wait_for_releases(k_empty, issued_k, L::kKeys, abort_flag) || !wait_for_releases(v_empty, issued_v, L::kValues, abort_flag)) give_up(2);
             if (*abort_flag) {   // what was issued arrives before the CTA ends
                 mbar_wait_bounded(own_full, 0);
-                for (uint32_t u = first_of_last_uses(issued, L::kStages); u < issued; ++u) mbar_wait_bounded(&full[u % L::kStages], parity_of_use(u, L::kStages));
+                for (uint32_t u = first_of_last_uses(issued_k, L::kKeys); u < issued_k; ++u) mbar_wait_bounded(&k_full[u % L::kKeys], parity_of_use(u, L::kKeys));
+                for (uint32_t u = first_of_last_uses(issued_v, L::kValues); u < issued_v; ++u) mbar_wait_bounded(&v_full[u % L::kValues], parity_of_use(u, L::kValues));
             }
         }
     } else if (warp == 9) {
@@ -419,15 +431,18 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         const uint32_t leader = elect_lane();
         bool ok = total == 0 || warp_wait(own_full, 0, 3);
         auto first = [&](int u) {   // S and dP of key tile u
-            const uint32_t st = u % L::kStages, at = ring + st * 2 * L::TILE_BYTES;
-            if (!warp_wait(&full[st], parity_of_use(u, L::kStages), 4)) return false;
+            const uint32_t sk = u % L::kKeys, sv = u % L::kValues;
+            if (!warp_wait(&k_full[sk], parity_of_use(u, L::kKeys), 4)) return false;
             tc_fence_after();
             const int beyond = see.length - (begin + u) * TILE;
-            if (beyond < TILE && (int)P.Nk > see.length) clear_tokens<BLOCKS>(smem + L::OFF_RING + st * 2 * L::TILE_BYTES, beyond, lane);
-            product_features<BLOCKS>(leader, S, q_at, at, idesc_s, steps);
+            if (beyond < TILE && (int)P.Nk > see.length) clear_tokens<BLOCKS>(smem + L::OFF_RING + sk * L::TILE_BYTES, beyond, lane);
+            product_features<BLOCKS>(leader, S, q_at, keys + sk * L::TILE_BYTES, idesc_s, steps);
             commit_by(leader, s_full);
-            product_features<BLOCKS>(leader, DP + (u & 1) * TILE, g_at, at + L::TILE_BYTES, idesc_s, steps);
+            if (!warp_wait(&v_full[sv], parity_of_use(u, L::kValues), 10)) return false;
+            tc_fence_after();
+            product_features<BLOCKS>(leader, DP + (u & 1) * TILE, g_at, values + sv * L::TILE_BYTES, idesc_s, steps);
             commit_by(leader, &dp_full[u & 1]);
+            commit_by(leader, &v_empty[sv]);
             return true;
         };
         if (total > 0 && ok) ok = first(0);
@@ -439,8 +454,8 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             }
             if (!(ok = warp_wait(ds_ready, u & 1, 6))) break;
             tc_fence_after();
-            product_tokens(leader, DQ, DP + (u & 1) * TILE, 64, ring + (u % L::kStages) * 2 * L::TILE_BYTES, idesc_d, u > 0);
-            commit_by(leader, &empty[u % L::kStages]);
+            product_tokens(leader, DQ, DP + (u & 1) * TILE, 64, keys + (u % L::kKeys) * L::TILE_BYTES, idesc_d, u > 0);
+            commit_by(leader, &k_empty[u % L::kKeys]);
         }
         if (ok && total > 0) commit_by(leader, acc_full);
         __syncwarp();
@@ -481,17 +496,25 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             tmem_ld32(dp_at, x[0]);
             tmem_ld32(dp_at + 32, x[1]);
             tmem_ld_wait();
-            uint32_t w[32];
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
                 const uint32_t *pair = &x[e >> 4][2 * (e & 15)];
-                float d0, d1;
-                unpack2(score_gradient<Lift<T>::kNeeded>(p[e], pack2(__uint_as_float(pair[0]), __uint_as_float(pair[1])), minus_delta, lift2), d0, d1);
-                if (masked) {
+                p[e] = score_gradient<Lift<T>::kNeeded>(p[e], pack2(__uint_as_float(pair[0]), __uint_as_float(pair[1])), minus_delta, lift2);
+            }
+            if (masked) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
                     const int j = j0 + 64 * half + 2 * e;
-                    d0 = j >= lo && j < hi ? d0 : 0.f;
-                    d1 = j + 1 >= lo && j + 1 < hi ? d1 : 0.f;
+                    float d0, d1;
+                    unpack2(p[e], d0, d1);
+                    p[e] = pack2(j >= lo && j < hi ? d0 : 0.f, j + 1 >= lo && j + 1 < hi ? d1 : 0.f);
                 }
+            }
+            uint32_t w[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+                float d0, d1;
+                unpack2(p[e], d0, d1);
                 w[e] = N::pack(d0, d1);
             }
             tmem_st32(dp_at, w);

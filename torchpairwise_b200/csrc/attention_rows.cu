@@ -1,7 +1,7 @@
 // What both gradient walks need of each query row, formed once: delta_i = dO_i . out_i - dlse_i, and the forward's lse_i, +inf for a
 // row that sees nothing (every probability is then exp(-inf) = 0), as powers of two for 32-bit walks.  The tensor-core walks add
 // rather than subtract: they get -delta_i and lift - lse_i.  Rows are padded to whole tiles of 128 as rows that see nothing.
-// Bound by HBM: reads dO and out once.  One warp per row.
+// Bound by HBM: reads dO and out once.
 //
 // Half precision also needs three maxima: the tensor-core walks round exp(s - lse) and ds = p (dO . v - delta) to the inputs' type, whose numbers end
 // at 65504 and lose digits below 2^-14.  |ds| <= p (|dO| (|v| + |out|) + |dlse|) <= p (2 max|dO| max|v| + max|dlse|), from which the walks take a power of two that
@@ -12,94 +12,139 @@ namespace tpw {
 namespace {
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Piece { T v[V]; };
-template <typename A> __device__ __forceinline__ A warp_sum(A x) {
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-    return x;
-}
 
-template <typename T, int V>
+// Rows in the order in which they lie in memory: (token, head) of a sequence.  LANES threads read one row V elements at a time, a warp
+// 32 / LANES rows side by side and kTurns times in a row, so that 2 * kTurns loads are in flight.
+constexpr int kTurns = 4;
+template <typename T, int V, int LANES>
 __global__ void __launch_bounds__(256) attention_rows_kernel(const AttnParams P, double units, double lift, double sign, unsigned *row_max) {
     typedef typename AttnAcc<T>::type A;
-    const int lane = threadIdx.x & 31;
-    const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (row >= P.B * P.Hq * P.Nqp) return;
-    const long long i = row % P.Nqp, bh = row / P.Nqp, h = bh % P.Hq, b = bh / P.Hq;
+    constexpr int ROWS = 8 * (32 / LANES) * kTurns;   // of a block
+    const long long per_batch = (P.Nqp * P.Hq + ROWS - 1) / ROWS, b = blockIdx.x / per_batch;
+    const long long base = (blockIdx.x % per_batch) * ROWS, i0 = base / P.Hq;
+    const int h0 = (int)(base % P.Hq), Hq = (int)P.Hq, D = (int)P.D;
+    const int part = threadIdx.x % LANES, group = threadIdx.x / LANES;
     A *lse = static_cast<A *>(P.row_lse), *delta = static_cast<A *>(P.row_delta);
-    if (i >= P.Nq) {
-        if (lane == 0) {
-            lse[row] = (A)(sign * INFINITY);
-            delta[row] = 0;
-        }
-        return;
-    }
-    const T *o = static_cast<const T *>(P.out) + ((b * P.Nq + i) * P.Hq + h) * P.D;
-    const T *g = static_cast<const T *>(P.dout) + b * P.do_s[0] + i * P.do_s[1] + h * P.do_s[2];
-    A dot = 0, sq = 0;
-    for (int d = lane * V; d < P.D; d += 32 * V) {
-        const Piece<T, V> x = *reinterpret_cast<const Piece<T, V> *>(o + d), y = *reinterpret_cast<const Piece<T, V> *>(g + d);
+    A dot[kTurns] = {}, sq[kTurns] = {};
+    auto place = [&](int t, long long &i, int &h) {
+        const int at = h0 + t * (256 / LANES) + group;
+        i = i0 + at / Hq;
+        h = at % Hq;
+    };
+    for (int d = part * V; d < D; d += LANES * V) {
+        Piece<T, V> x[kTurns] = {}, y[kTurns] = {};
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            dot += (A)x.v[e] * (A)y.v[e];
-            sq += (A)y.v[e] * (A)y.v[e];
+        for (int t = 0; t < kTurns; ++t) {
+            long long i;
+            int h;
+            place(t, i, h);
+            if (i < P.Nq) {
+                x[t] = *reinterpret_cast<const Piece<T, V> *>(static_cast<const T *>(P.out) + ((b * P.Nq + i) * P.Hq + h) * P.D + d);
+                y[t] = *reinterpret_cast<const Piece<T, V> *>(static_cast<const T *>(P.dout) + b * P.do_s[0] + i * P.do_s[1] + h * P.do_s[2] + d);
+            }
         }
+#pragma unroll
+        for (int t = 0; t < kTurns; ++t)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                dot[t] += (A)x[t].v[e] * (A)y[t].v[e];
+                if (sizeof(T) == 2) sq[t] += (A)y[t].v[e] * (A)y[t].v[e];
+            }
     }
-    dot = warp_sum(dot);
-    const A m = static_cast<const A *>(P.lse)[bh * P.Nq + i];
-    const bool sees = m != -(A)INFINITY;
-    const A more = P.dlse ? static_cast<const A *>(P.dlse)[bh * P.Nq + i] : (A)0;
-    if (lane == 0) {
-        lse[row] = sees ? m * (A)units + (A)lift : (A)(sign * INFINITY);
-        delta[row] = sees ? (A)sign * (dot - more) : (A)0;
+    unsigned top = 0, top_more = 0;
+#pragma unroll
+    for (int t = 0; t < kTurns; ++t) {
+#pragma unroll
+        for (int d = LANES / 2; d >= 1; d >>= 1) {
+            dot[t] += __shfl_xor_sync(0xffffffffu, dot[t], d);
+            if (sizeof(T) == 2) sq[t] += __shfl_xor_sync(0xffffffffu, sq[t], d);
+        }
+        long long i;
+        int h;
+        place(t, i, h);
+        if (part != 0 || i >= P.Nqp) continue;
+        const long long bh = b * P.Hq + h;
+        const A m = i < P.Nq ? static_cast<const A *>(P.lse)[bh * P.Nq + i] : -(A)INFINITY;
+        const bool sees = m != -(A)INFINITY;
+        const A more = sees && P.dlse ? static_cast<const A *>(P.dlse)[bh * P.Nq + i] : (A)0;
+        lse[bh * P.Nqp + i] = sees ? m * (A)units + (A)lift : (A)(sign * INFINITY);
+        delta[bh * P.Nqp + i] = sees ? (A)sign * (dot[t] - more) : (A)0;
+        if (row_max && sees) {
+            top = max(top, __float_as_uint(fabsf((float)sq[t])));
+            top_more = max(top_more, __float_as_uint(fabsf((float)more)));
+        }
     }
     if (row_max) {
-        sq = warp_sum(sq);
-        if (lane == 0 && sees) {
-            atomicMax(row_max, __float_as_uint(fabsf((float)sq)));
-            if (P.dlse) atomicMax(row_max + 2, __float_as_uint(fabsf((float)more)));
+        top = __reduce_max_sync(0xffffffffu, top);
+        top_more = __reduce_max_sync(0xffffffffu, top_more);
+        if ((threadIdx.x & 31) == 0) {
+            if (top) atomicMax(row_max, top);
+            if (top_more) atomicMax(row_max + 2, top_more);
         }
     }
 }
 
-template <int V>
+template <int V, int LANES>
 __global__ void __launch_bounds__(256) attention_value_norm_kernel(const AttnParams P, unsigned *row_max) {
-    const int lane = threadIdx.x & 31;
-    float top = 0.f;
-    for (long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); row < P.B * P.Nk * P.Hk; row += (long long)gridDim.x * 8) {
-        const long long h = row % P.Hk, bj = row / P.Hk, j = bj % P.Nk, b = bj / P.Nk;
-        if (P.key_lengths && j >= P.key_lengths[b]) continue;
-        const __half *v = static_cast<const __half *>(P.v) + b * P.v_s[0] + j * P.v_s[1] + h * P.v_s[2];
-        float sq = 0.f;
-        for (int d = lane * V; d < P.D; d += 32 * V) {
-            const Piece<__half, V> x = *reinterpret_cast<const Piece<__half, V> *>(v + d);
+    constexpr int ROWS = 8 * (32 / LANES) * kTurns;
+    const long long per_batch = (P.Nk * P.Hk + ROWS - 1) / ROWS, b = blockIdx.x / per_batch;
+    const long long base = (blockIdx.x % per_batch) * ROWS, j0 = base / P.Hk;
+    const int h0 = (int)(base % P.Hk), Hk = (int)P.Hk, D = (int)P.D, part = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    long long length = P.key_lengths ? P.key_lengths[b] : P.Nk;
+    length = length < P.Nk ? length : P.Nk;
+    if (j0 >= length) return;
+    float sq[kTurns] = {};
+    for (int d = part * V; d < D; d += LANES * V) {
+        Piece<__half, V> x[kTurns] = {};
 #pragma unroll
-            for (int e = 0; e < V; ++e) sq += (float)x.v[e] * (float)x.v[e];
+        for (int t = 0; t < kTurns; ++t) {
+            const int at = h0 + t * (256 / LANES) + group;
+            const long long j = j0 + at / Hk;
+            if (j < length) x[t] = *reinterpret_cast<const Piece<__half, V> *>(static_cast<const __half *>(P.v) + b * P.v_s[0] + j * P.v_s[1] + at % Hk * P.v_s[2] + d);
         }
-        sq = warp_sum(sq);
-        top = sq > top || sq != sq ? sq : top;
+#pragma unroll
+        for (int t = 0; t < kTurns; ++t)
+#pragma unroll
+            for (int e = 0; e < V; ++e) sq[t] += (float)x[t].v[e] * (float)x[t].v[e];
     }
-    if (lane == 0) atomicMax(row_max, __float_as_uint(fabsf(top)));
+    unsigned top = 0;
+#pragma unroll
+    for (int t = 0; t < kTurns; ++t) {
+#pragma unroll
+        for (int d = LANES / 2; d >= 1; d >>= 1) sq[t] += __shfl_xor_sync(0xffffffffu, sq[t], d);
+        top = max(top, __float_as_uint(fabsf(sq[t])));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0 && top) atomicMax(row_max, top);
 }
 
-template <typename T> int rows(AttnParams &P, double units, double lift, double sign, unsigned *row_max, cudaStream_t s) {
-    constexpr int W = sizeof(T) == 8 ? 2 : 4;
-    auto wide = [&](const void *p, const long long (&st)[3]) {
-        return reinterpret_cast<uintptr_t>(p) % (W * sizeof(T)) == 0 && st[0] % W == 0 && st[1] % W == 0 && st[2] % W == 0;
-    };
-    const long long dense[3] = {P.D, P.D, P.D};
-    const long long blocks = (P.B * P.Hq * P.Nqp + 7) / 8;
+template <typename T, int V, int LANES>
+int launch(const AttnParams &P, double units, double lift, double sign, unsigned *row_max, cudaStream_t s) {
+    constexpr int ROWS = 8 * (32 / LANES) * kTurns;
+    const long long blocks = (P.Nqp * P.Hq + ROWS - 1) / ROWS * P.B;
     TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
-    if (P.D % W == 0 && wide(P.out, dense) && wide(P.dout, P.do_s)) attention_rows_kernel<T, W><<<(unsigned)blocks, 256, 0, s>>>(P, units, lift, sign, row_max);
-    else attention_rows_kernel<T, 1><<<(unsigned)blocks, 256, 0, s>>>(P, units, lift, sign, row_max);
+    attention_rows_kernel<T, V, LANES><<<(unsigned)blocks, 256, 0, s>>>(P, units, lift, sign, row_max);
     TPW_LAUNCH_OK("attention_rows_kernel");
-    if (row_max && P.Nk > 0) {
-        const long long want = (P.B * P.Nk * P.Hk + 7) / 8, most = 16LL * sm_count();
-        const unsigned grid = (unsigned)(want < most ? want : most);
-        if (P.D % W == 0 && wide(P.v, P.v_s)) attention_value_norm_kernel<W><<<grid, 256, 0, s>>>(P, row_max + 1);
-        else attention_value_norm_kernel<1><<<grid, 256, 0, s>>>(P, row_max + 1);
-        TPW_LAUNCH_OK("attention_value_norm_kernel");
+    if constexpr (sizeof(T) == 2) {
+        const long long keys = (P.Nk * P.Hk + ROWS - 1) / ROWS * P.B;
+        if (row_max && keys > 0) {
+            TPW_CHECK_ARG(keys < (1LL << 31), "attention: more than 2^31 blocks of work");
+            attention_value_norm_kernel<V, LANES><<<(unsigned)keys, 256, 0, s>>>(P, row_max + 1);
+            TPW_LAUNCH_OK("attention_value_norm_kernel");
+        }
     }
     return TPW_OK;
+}
+
+template <typename T> int rows(const AttnParams &P, double units, double lift, double sign, unsigned *row_max, cudaStream_t s) {
+    constexpr int W = 16 / sizeof(T);   // elements of 16 bytes
+    auto wide = [&](const void *p, const long long (&st)[3]) { return aligned16(p) && st[0] % W == 0 && st[1] % W == 0 && st[2] % W == 0; };
+    const long long dense[3] = {P.D, P.D, P.D};
+    if (P.D % W != 0 || !wide(P.out, dense) || !wide(P.dout, P.do_s) || (row_max && !wide(P.v, P.v_s))) return launch<T, 1, 32>(P, units, lift, sign, row_max, s);
+    const long long pieces = P.D / W;
+    if (pieces <= 8) return launch<T, W, 8>(P, units, lift, sign, row_max, s);
+    if (pieces <= 16) return launch<T, W, 16>(P, units, lift, sign, row_max, s);
+    return launch<T, W, 32>(P, units, lift, sign, row_max, s);
 }
 
 } // namespace
