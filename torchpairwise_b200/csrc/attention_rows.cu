@@ -13,34 +13,35 @@ namespace {
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Piece { T v[V]; };
 
-// Rows in the order in which they lie in memory: (token, head) of a sequence.  LANES threads read one row V elements at a time, a warp
-// 32 / LANES rows side by side and kTurns times in a row, so that 2 * kTurns loads are in flight.
-constexpr int kTurns = 4;
+// A block takes consecutive tokens of one head.  LANES threads read one row V elements at a time, a warp 32 / LANES rows side by side and
+// kTurns times in a row, so that 2 * kTurns loads are in flight.
+constexpr int kTurns = 2;
 template <typename T, int V, int LANES>
-__global__ void __launch_bounds__(256) attention_rows_kernel(const AttnParams P, double units, double lift, double sign, unsigned *row_max) {
+__global__ void __launch_bounds__(256, sizeof(T) == 8 ? 4 : 6) attention_rows_kernel(const AttnParams P, double units, double lift, double sign, unsigned *row_max) {
     typedef typename AttnAcc<T>::type A;
     constexpr int ROWS = 8 * (32 / LANES) * kTurns;   // of a block
-    const long long per_batch = (P.Nqp * P.Hq + ROWS - 1) / ROWS, b = blockIdx.x / per_batch;
-    const long long base = (blockIdx.x % per_batch) * ROWS, i0 = base / P.Hq;
-    const int h0 = (int)(base % P.Hq), Hq = (int)P.Hq, D = (int)P.D;
-    const int part = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    const unsigned tiles = (unsigned)((P.Nqp + ROWS - 1) / ROWS), bh = blockIdx.x / tiles;
+    const int D = (int)P.D, h = (int)(bh % (unsigned)P.Hq), part = threadIdx.x % LANES;
+    const long long b = bh / (unsigned)P.Hq, i0 = (long long)(blockIdx.x % tiles) * ROWS + threadIdx.x / LANES;
+    const T *out = static_cast<const T *>(P.out) + (b * P.Nq * P.Hq + h) * P.D, *dout = static_cast<const T *>(P.dout) + b * P.do_s[0] + h * P.do_s[2];
     A *lse = static_cast<A *>(P.row_lse), *delta = static_cast<A *>(P.row_delta);
-    A dot[kTurns] = {}, sq[kTurns] = {};
-    auto place = [&](int t, long long &i, int &h) {
-        const int at = h0 + t * (256 / LANES) + group;
-        i = i0 + at / Hq;
-        h = at % Hq;
-    };
+    A dot[kTurns] = {}, sq[kTurns] = {}, m[kTurns], more[kTurns];
+#pragma unroll
+    for (int t = 0; t < kTurns; ++t) {   // on their way beside the rows
+        const long long i = i0 + t * (256 / LANES);
+        const bool own = part == 0 && i < P.Nq;
+        m[t] = own ? static_cast<const A *>(P.lse)[bh * P.Nq + i] : -(A)INFINITY;
+        more[t] = own && P.dlse ? static_cast<const A *>(P.dlse)[bh * P.Nq + i] : (A)0;
+    }
+#pragma unroll 1
     for (int d = part * V; d < D; d += LANES * V) {
         Piece<T, V> x[kTurns] = {}, y[kTurns] = {};
 #pragma unroll
         for (int t = 0; t < kTurns; ++t) {
-            long long i;
-            int h;
-            place(t, i, h);
+            const long long i = i0 + t * (256 / LANES);
             if (i < P.Nq) {
-                x[t] = *reinterpret_cast<const Piece<T, V> *>(static_cast<const T *>(P.out) + ((b * P.Nq + i) * P.Hq + h) * P.D + d);
-                y[t] = *reinterpret_cast<const Piece<T, V> *>(static_cast<const T *>(P.dout) + b * P.do_s[0] + i * P.do_s[1] + h * P.do_s[2] + d);
+                x[t] = *reinterpret_cast<const Piece<T, V> *>(out + i * P.Hq * P.D + d);
+                y[t] = *reinterpret_cast<const Piece<T, V> *>(dout + i * P.do_s[1] + d);
             }
         }
 #pragma unroll
@@ -59,19 +60,14 @@ __global__ void __launch_bounds__(256) attention_rows_kernel(const AttnParams P,
             dot[t] += __shfl_xor_sync(0xffffffffu, dot[t], d);
             if (sizeof(T) == 2) sq[t] += __shfl_xor_sync(0xffffffffu, sq[t], d);
         }
-        long long i;
-        int h;
-        place(t, i, h);
+        const long long i = i0 + t * (256 / LANES);
         if (part != 0 || i >= P.Nqp) continue;
-        const long long bh = b * P.Hq + h;
-        const A m = i < P.Nq ? static_cast<const A *>(P.lse)[bh * P.Nq + i] : -(A)INFINITY;
-        const bool sees = m != -(A)INFINITY;
-        const A more = sees && P.dlse ? static_cast<const A *>(P.dlse)[bh * P.Nq + i] : (A)0;
-        lse[bh * P.Nqp + i] = sees ? m * (A)units + (A)lift : (A)(sign * INFINITY);
-        delta[bh * P.Nqp + i] = sees ? (A)sign * (dot[t] - more) : (A)0;
+        const bool sees = m[t] != -(A)INFINITY;
+        lse[bh * P.Nqp + i] = sees ? m[t] * (A)units + (A)lift : (A)(sign * INFINITY);
+        delta[bh * P.Nqp + i] = sees ? (A)sign * (dot[t] - more[t]) : (A)0;
         if (row_max && sees) {
             top = max(top, __float_as_uint(fabsf((float)sq[t])));
-            top_more = max(top_more, __float_as_uint(fabsf((float)more)));
+            top_more = max(top_more, __float_as_uint(fabsf((float)more[t])));
         }
     }
     if (row_max) {
@@ -87,20 +83,19 @@ __global__ void __launch_bounds__(256) attention_rows_kernel(const AttnParams P,
 template <int V, int LANES>
 __global__ void __launch_bounds__(256) attention_value_norm_kernel(const AttnParams P, unsigned *row_max) {
     constexpr int ROWS = 8 * (32 / LANES) * kTurns;
-    const long long per_batch = (P.Nk * P.Hk + ROWS - 1) / ROWS, b = blockIdx.x / per_batch;
-    const long long base = (blockIdx.x % per_batch) * ROWS, j0 = base / P.Hk;
-    const int h0 = (int)(base % P.Hk), Hk = (int)P.Hk, D = (int)P.D, part = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    const unsigned tiles = (unsigned)((P.Nk + ROWS - 1) / ROWS), bh = blockIdx.x / tiles;
+    const int D = (int)P.D, h = (int)(bh % (unsigned)P.Hk), part = threadIdx.x % LANES;
+    const long long b = bh / (unsigned)P.Hk, j0 = (long long)(blockIdx.x % tiles) * ROWS + threadIdx.x / LANES;
+    const __half *v = static_cast<const __half *>(P.v) + b * P.v_s[0] + h * P.v_s[2];
     long long length = P.key_lengths ? P.key_lengths[b] : P.Nk;
     length = length < P.Nk ? length : P.Nk;
-    if (j0 >= length) return;
     float sq[kTurns] = {};
     for (int d = part * V; d < D; d += LANES * V) {
         Piece<__half, V> x[kTurns] = {};
 #pragma unroll
         for (int t = 0; t < kTurns; ++t) {
-            const int at = h0 + t * (256 / LANES) + group;
-            const long long j = j0 + at / Hk;
-            if (j < length) x[t] = *reinterpret_cast<const Piece<__half, V> *>(static_cast<const __half *>(P.v) + b * P.v_s[0] + j * P.v_s[1] + at % Hk * P.v_s[2] + d);
+            const long long j = j0 + t * (256 / LANES);
+            if (j < length) x[t] = *reinterpret_cast<const Piece<__half, V> *>(v + j * P.v_s[1] + d);
         }
 #pragma unroll
         for (int t = 0; t < kTurns; ++t)
@@ -121,12 +116,12 @@ __global__ void __launch_bounds__(256) attention_value_norm_kernel(const AttnPar
 template <typename T, int V, int LANES>
 int launch(const AttnParams &P, double units, double lift, double sign, unsigned *row_max, cudaStream_t s) {
     constexpr int ROWS = 8 * (32 / LANES) * kTurns;
-    const long long blocks = (P.Nqp * P.Hq + ROWS - 1) / ROWS * P.B;
+    const long long blocks = (P.Nqp + ROWS - 1) / ROWS * P.Hq * P.B;
     TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
     attention_rows_kernel<T, V, LANES><<<(unsigned)blocks, 256, 0, s>>>(P, units, lift, sign, row_max);
     TPW_LAUNCH_OK("attention_rows_kernel");
     if constexpr (sizeof(T) == 2) {
-        const long long keys = (P.Nk * P.Hk + ROWS - 1) / ROWS * P.B;
+        const long long keys = (P.Nk + ROWS - 1) / ROWS * P.Hk * P.B;
         if (row_max && keys > 0) {
             TPW_CHECK_ARG(keys < (1LL << 31), "attention: more than 2^31 blocks of work");
             attention_value_norm_kernel<V, LANES><<<(unsigned)keys, 256, 0, s>>>(P, row_max + 1);

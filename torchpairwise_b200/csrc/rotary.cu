@@ -23,111 +23,153 @@ struct RotaryParams {
     long long pos_stride[2];
     long long N, D, half, length, tokens;
     int heads_per_thread, head_groups, chunks;   // chunks per row: turned ones first, then copied ones
+    int small;                                   // fewer than 2^32 threads
     float sign;
 };
 
 template <typename T> struct Acc { typedef float type; };
 template <> struct Acc<double> { typedef double type; };
 
-template <typename T> __device__ __forceinline__ typename Acc<T>::type widen(T v) { return (typename Acc<T>::type)v; }
-template <typename T> __device__ __forceinline__ T narrow(typename Acc<T>::type v) { return (T)v; }
-
+// W elements as they lie in memory, and two neighbours of them widened and narrowed at a time
 template <typename T, int W> struct alignas(sizeof(T) * W) Chunk { T v[W]; };
+template <typename T> __device__ __forceinline__ void widen2(const T *p, typename Acc<T>::type &a, typename Acc<T>::type &b) {
+    a = p[0];
+    b = p[1];
+}
+template <> __device__ __forceinline__ void widen2<__nv_bfloat16>(const __nv_bfloat16 *p, float &a, float &b) {
+    const uint32_t w = *reinterpret_cast<const uint32_t *>(p);
+    a = __uint_as_float(w << 16);
+    b = __uint_as_float(w & 0xffff0000u);
+}
+template <> __device__ __forceinline__ void widen2<__half>(const __half *p, float &a, float &b) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(p));
+    a = f.x;
+    b = f.y;
+}
+template <typename T> __device__ __forceinline__ void narrow2(T *p, typename Acc<T>::type a, typename Acc<T>::type b) {
+    p[0] = a;
+    p[1] = b;
+}
+template <> __device__ __forceinline__ void narrow2<__nv_bfloat16>(__nv_bfloat16 *p, float a, float b) {
+    *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(a, b);
+}
+template <> __device__ __forceinline__ void narrow2<__half>(__half *p, float a, float b) { *reinterpret_cast<__half2 *>(p) = __floats2half2_rn(a, b); }
 
-// W elements per access (16 bytes, or one where a row or pointer is off that grid)
+// W elements per access (16 bytes, or one where a row or pointer is off that grid).  64 registers, so that 32 warps per SM keep
+// eight 16-byte loads each in flight: with 128 registers and half of the warps DRAM was 37 % busy.
 template <typename T, int W, bool INTER>
-__global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams P) {
+__global__ void __launch_bounds__(256, 4) rotary_kernel(const RotaryParams P) {
     typedef typename Acc<T>::type A;
     typedef Chunk<T, W> C;
     constexpr int PAIRS = INTER ? (W > 1 ? W / 2 : 1) : W;   // pairs per turned chunk
-    long long at = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const int chunk = (int)(at % P.chunks);
-    at /= P.chunks;
-    const int group = (int)(at % P.head_groups);
-    const long long token = at / P.head_groups;
+    unsigned chunk, group;
+    long long token;
+    if (P.small) {   // 32-bit divisions where they reach
+        const unsigned at = blockIdx.x * 256u + threadIdx.x, rest = at / (unsigned)P.chunks;
+        chunk = at - rest * P.chunks;
+        token = rest / (unsigned)P.head_groups;
+        group = rest - (unsigned)token * P.head_groups;
+    } else {
+        const long long at = (long long)blockIdx.x * 256 + threadIdx.x, rest = at / P.chunks;
+        chunk = (unsigned)(at - rest * P.chunks);
+        token = rest / P.head_groups;
+        group = (unsigned)(rest - token * P.head_groups);
+    }
     if (token >= P.tokens) return;
-    const long long b = token / P.N, n = token % P.N;
-    const int turned = (int)(P.half / PAIRS);
+    const long long b = P.small ? (unsigned)token / (unsigned)P.N : token / P.N, n = token - b * P.N;
+    const unsigned turned = (unsigned)(P.half / PAIRS);
     const bool turn = chunk < turned;
     // offsets of the one or two pieces of a row that this thread handles
-    long long o0, o1 = 0;
+    int o0, o1 = 0;
     bool two = false;
     if (turn) {
         if (INTER) {
-            o0 = (long long)chunk * (2 * PAIRS);
+            o0 = chunk * (2 * PAIRS);
             two = W == 1;
             o1 = o0 + 1;
         } else {
-            o0 = (long long)chunk * W;
-            o1 = P.half + o0;
+            o0 = chunk * W;
+            o1 = (int)P.half + o0;
             two = true;
         }
     } else {
-        o0 = 2 * P.half + (long long)(chunk - turned) * W;
+        o0 = 2 * (int)P.half + (chunk - turned) * W;
     }
     float c[PAIRS], s[PAIRS];
     if (turn) {
         const long long t = P.positions ? P.positions[b * P.pos_stride[0] + n * P.pos_stride[1]] : n;
         const bool inside = t >= 0 && t < P.length;
-        const float *pc = P.cos + (inside ? t : 0) * P.half + (long long)chunk * PAIRS;
-        const float *ps = P.sin + (inside ? t : 0) * P.half + (long long)chunk * PAIRS;
+        const float *pc = P.cos + (inside ? t : 0) * P.half + chunk * PAIRS;
+        const float *ps = P.sin + (inside ? t : 0) * P.half + chunk * PAIRS;
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) {
             c[i] = inside ? pc[i] : __int_as_float(0x7fffffff);
             s[i] = ps[i] * P.sign;
         }
     }
-    const long long h_end = P.H[0] + P.H[1];
-    long long h = (long long)group * P.heads_per_thread;
-    const long long h_stop = h + P.heads_per_thread < h_end ? h + P.heads_per_thread : h_end;
+    const int h_first = (int)P.H[0], h_end = h_first + (int)P.H[1];
+    int h = (int)(group * P.heads_per_thread);
+    const int h_stop = h + P.heads_per_thread < h_end ? h + P.heads_per_thread : h_end;
     auto work = [&](const C &x0, const C &x1, C &y0, C &y1) {
-        if (!turn) {
-            y0 = x0;
-        } else if (INTER && W > 1) {
+        if constexpr (W == 1) {
+            const A u = (A)x0.v[0], v = (A)x1.v[0];
+            y0.v[0] = (T)(u * (A)c[0] - v * (A)s[0]);
+            y1.v[0] = (T)(u * (A)s[0] + v * (A)c[0]);
+        } else if constexpr (INTER) {
 #pragma unroll
             for (int i = 0; i < PAIRS; ++i) {
-                const A u = widen(x0.v[(2 * i) % W]), v = widen(x0.v[(2 * i + 1) % W]);
-                y0.v[(2 * i) % W] = narrow<T>(u * (A)c[i] - v * (A)s[i]);
-                y0.v[(2 * i + 1) % W] = narrow<T>(u * (A)s[i] + v * (A)c[i]);
+                A u, v;
+                widen2<T>(&x0.v[2 * i], u, v);
+                narrow2<T>(&y0.v[2 * i], u * (A)c[i] - v * (A)s[i], u * (A)s[i] + v * (A)c[i]);
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < PAIRS; ++i) {
-                const A u = widen(x0.v[i]), v = widen(x1.v[i]);
-                y0.v[i] = narrow<T>(u * (A)c[i] - v * (A)s[i]);
-                y1.v[i] = narrow<T>(u * (A)s[i] + v * (A)c[i]);
+            for (int i = 0; i < PAIRS; i += 2) {
+                A u0, u1, v0, v1;
+                widen2<T>(&x0.v[i], u0, u1);
+                widen2<T>(&x1.v[i], v0, v1);
+                narrow2<T>(&y0.v[i], u0 * (A)c[i] - v0 * (A)s[i], u1 * (A)c[i + 1] - v1 * (A)s[i + 1]);
+                narrow2<T>(&y1.v[i], u0 * (A)s[i] + v0 * (A)c[i], u1 * (A)s[i + 1] + v1 * (A)c[i + 1]);
             }
         }
     };
-    auto from = [&](long long head) {
-        const int w = head >= P.H[0];
-        const long long hh = head - (w ? P.H[0] : 0);
-        return static_cast<const T *>(P.x[w]) + b * P.stride[w][0] + n * P.stride[w][1] + hh * P.stride[w][2];
-    };
-    auto to = [&](long long head) {
-        const int w = head >= P.H[0];
-        const long long hh = head - (w ? P.H[0] : 0);
-        return static_cast<T *>(P.out[w]) + (token * P.H[w] + hh) * P.D;
-    };
-    constexpr int U = 4;
-    for (; h < h_stop; h += U) {
-        C x0[U], x1[U];
+    const T *from[2];
+    T *to[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {   // head 0 of either tensor, counted in the heads of both
+        from[w] = static_cast<const T *>(P.x[w]) + b * P.stride[w][0] + n * P.stride[w][1] - (w ? h_first * P.stride[1][2] : 0);
+        to[w] = static_cast<T *>(P.out[w]) + (token * P.H[w] - (w ? h_first : 0)) * P.D;
+    }
+    // two heads at a time, the next two on their way meanwhile
+    constexpr int U = 2;
+    auto fetch = [&](int h, C (&x0)[U], C (&x1)[U]) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (h + u < h_stop) {
-                const T *p = from(h + u);
+                const T *p = h + u < h_first ? from[0] + (h + u) * P.stride[0][2] : from[1] + (h + u) * P.stride[1][2];
                 x0[u] = *reinterpret_cast<const C *>(p + o0);
                 if (two) x1[u] = *reinterpret_cast<const C *>(p + o1);
             }
+    };
+    C x0[U], x1[U];
+    fetch(h, x0, x1);
+    for (; h < h_stop; h += U) {
+        C z0[U], z1[U];
+        fetch(h + U, z0, z1);
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (h + u < h_stop) {
-                C y0, y1;
-                work(x0[u], x1[u], y0, y1);
-                T *p = to(h + u);
+                C y0 = x0[u], y1 = x1[u];
+                if (turn) work(x0[u], x1[u], y0, y1);
+                T *p = (h + u < h_first ? to[0] : to[1]) + (h + u) * P.D;
                 *reinterpret_cast<C *>(p + o0) = y0;
                 if (two) *reinterpret_cast<C *>(p + o1) = y1;
             }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            x0[u] = z0[u];
+            x1[u] = z1[u];
+        }
     }
 }
 
@@ -166,6 +208,7 @@ int launch(const tpw_rotary &a, RotaryParams &P, cudaStream_t s) {
     P.head_groups = (int)((heads + per - 1) / per);
     const long long threads = P.tokens * chunks * P.head_groups, blocks = (threads + 255) / 256;
     TPW_CHECK_ARG(blocks < (1LL << 31), "tpw_rotary_apply: more than 2^31 blocks of work");
+    P.small = blocks < (1LL << 24);
     if (wide) rotary_kernel<T, W, INTER><<<(unsigned)blocks, 256, 0, s>>>(P);
     else rotary_kernel<T, 1, INTER><<<(unsigned)blocks, 256, 0, s>>>(P);
     TPW_LAUNCH_OK("rotary_kernel");
