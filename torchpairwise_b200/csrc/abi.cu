@@ -86,6 +86,21 @@ static int encode_map_3d(CUtensorMap *map, const void *base, int elem_bytes,
                          uint64_t dim0, uint64_t dim1, uint64_t dim2,
                          uint32_t box0, uint32_t box1, bool swizzle128, CUtensorMapSwizzle swizzle, uint64_t pitch1 = 0, uint64_t pitch2 = 0);
 
+// The encoder is a driver call and needs a context bound to the calling thread.  A thread that
+// has only ever been handed tensors (an autograd worker, say) may not have one yet: binding the
+// runtime's current device does it.  Once per thread and device.
+static int bind_context() {
+    static thread_local int bound_device = -1;
+    int dev = 0;
+    TPW_CUDA_OK(cudaGetDevice(&dev));
+    if (bound_device != dev) {
+        TPW_CUDA_OK(cudaSetDevice(dev));
+        TPW_CUDA_OK(cudaFree(nullptr));
+        bound_device = dev;
+    }
+    return TPW_OK;
+}
+
 int make_tensor_map_3d(CUtensorMap *map, const void *base, int elem_bytes,
                        uint64_t dim0, uint64_t dim1, uint64_t dim2,
                        uint32_t box0, uint32_t box1, bool swizzle128) {
@@ -108,19 +123,7 @@ static int encode_map_3d(CUtensorMap *map, const void *base, int elem_bytes,
                          uint32_t box0, uint32_t box1, bool swizzle128, CUtensorMapSwizzle swizzle, uint64_t pitch1, uint64_t pitch2) {
     encode_tiled_fn encode = resolve_encode_tiled();
     if (!encode) return fail(TPW_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
-    // The encoder is a driver call and needs a context bound to the calling thread.  A thread that
-    // has only ever been handed tensors (an autograd worker, say) may not have one yet: binding the
-    // runtime's current device does it.  Once per thread and device.
-    {
-        static thread_local int bound_device = -1;
-        int dev = 0;
-        TPW_CUDA_OK(cudaGetDevice(&dev));
-        if (bound_device != dev) {
-            TPW_CUDA_OK(cudaSetDevice(dev));
-            TPW_CUDA_OK(cudaFree(nullptr));
-            bound_device = dev;
-        }
-    }
+    if (int e = bind_context()) return e;
     CUtensorMapDataType dt;
     switch (elem_bytes) {
         case 1: dt = CU_TENSOR_MAP_DATA_TYPE_UINT8; break;
@@ -146,17 +149,28 @@ static int encode_map_3d(CUtensorMap *map, const void *base, int elem_bytes,
     return TPW_OK;
 }
 
+int allow_shared_memory(const void *kernel, int bytes, std::atomic<unsigned long long> &done) {
+    int dev = 0;
+    TPW_CUDA_OK(cudaGetDevice(&dev));
+    const unsigned long long bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_acquire) & bit) return TPW_OK;
+    TPW_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_release);
+    return TPW_OK;
+}
+
 int make_tensor_map_heads(CUtensorMap *map, const void *base, uint64_t features, uint64_t tokens, uint64_t heads, uint64_t batch,
                           uint64_t token_pitch, uint64_t head_pitch, uint64_t batch_pitch, uint32_t box_tokens) {
-    CUtensorMap first;   // binds the context and resolves the encoder like every other map
-    int e = make_tensor_map_3d_pitched(&first, base, 2, features, tokens, heads, token_pitch, head_pitch, 64, box_tokens);
-    if (e != TPW_OK) return e;
-    if (batch_pitch % 16 != 0) return fail(TPW_ERR_INVALID, "tensor map: pitches are no multiples of 16 bytes");
+    encode_tiled_fn encode = resolve_encode_tiled();
+    if (!encode) return fail(TPW_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    if (int e = bind_context()) return e;
+    if (!aligned16(base)) return fail(TPW_ERR_INVALID, "tensor map: base address is not 16-byte aligned");
+    if (token_pitch % 16 != 0 || head_pitch % 16 != 0 || batch_pitch % 16 != 0) return fail(TPW_ERR_INVALID, "tensor map: pitches are no multiples of 16 bytes");
     cuuint64_t dims[4] = {features, tokens, heads, batch};
     cuuint64_t strides[3] = {token_pitch, head_pitch, batch_pitch};
     cuuint32_t box[4] = {64, box_tokens, 1, 1};
     cuuint32_t estr[4] = {1, 1, 1, 1};
-    CUresult r = resolve_encode_tiled()(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims, strides, box, estr,
+    CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims, strides, box, estr,
                                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(TPW_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);

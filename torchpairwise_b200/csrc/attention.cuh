@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 namespace tpw {
 
 struct AttnParams {
@@ -52,7 +54,13 @@ int attn_simple_backward(int dtype, const AttnParams &P, cudaStream_t s);
 long long attn_rows_bytes(int dtype, const AttnParams &P);
 int attn_rows(int dtype, AttnParams &P, void *scratch, bool tensor, cudaStream_t s);
 
-// abi.cu: 16-bit rows of [batch, tokens, heads, features] that lie the given numbers of bytes apart, as boxes of 64 features (128-byte
+// abi.cu: cudaFuncSetAttribute of a kernel's dynamic shared memory, once per device; `done` is the kernel's own word
+int allow_shared_memory(const void *kernel, int bytes, std::atomic<unsigned long long> &done);
+template <auto *KERNEL> int allow_shared_memory(int bytes) {
+    static std::atomic<unsigned long long> done{0};
+    return allow_shared_memory(reinterpret_cast<const void *>(KERNEL), bytes, done);
+}
+// 16-bit rows of [batch, tokens, heads, features] that lie the given numbers of bytes apart, as boxes of 64 features (128-byte
 // swizzle) by `box_tokens` tokens; what lies beyond the tensor reads as zero
 int make_tensor_map_heads(CUtensorMap *map, const void *base, uint64_t features, uint64_t tokens, uint64_t heads, uint64_t batch,
                           uint64_t token_pitch, uint64_t head_pitch, uint64_t batch_pitch, uint32_t box_tokens);

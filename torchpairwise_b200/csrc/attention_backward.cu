@@ -563,8 +563,8 @@ template <typename T, int BLOCKS> int launch(const AttnParams &P, cudaStream_t s
         F.tiles = (int)((P.Nk + TILE - 1) / TILE);
         const long long blocks = F.tiles * P.B * P.Hk;
         TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
-        auto kern = attention_dkv_kernel<T, BLOCKS>;
-        TPW_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::ALLOC));
+        constexpr auto *kern = &attention_dkv_kernel<T, BLOCKS>;
+        if (const int e = allow_shared_memory<kern>((int)L::ALLOC)) return e;
         kern<<<(unsigned)blocks, kTcThreads, L::ALLOC, s>>>(q, k, v, g, F);
         TPW_LAUNCH_OK("attention_dkv_kernel");
     }
@@ -572,8 +572,8 @@ template <typename T, int BLOCKS> int launch(const AttnParams &P, cudaStream_t s
         F.tiles = (int)((P.Nq + TILE - 1) / TILE);
         const long long blocks = F.tiles * P.B * P.Hq;
         TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
-        auto kern = attention_dq_kernel<T, BLOCKS>;
-        TPW_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::ALLOC));
+        constexpr auto *kern = &attention_dq_kernel<T, BLOCKS>;
+        if (const int e = allow_shared_memory<kern>((int)L::ALLOC)) return e;
         kern<<<(unsigned)blocks, kTcThreads, L::ALLOC, s>>>(q, k, v, g, F);
         TPW_LAUNCH_OK("attention_dq_kernel");
     }

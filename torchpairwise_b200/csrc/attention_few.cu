@@ -344,8 +344,8 @@ template <typename T, int BLOCKS, int MT> int launch(const FewParams &F, const C
     typedef FewSmem<BLOCKS> L;
     const long long blocks = F.a.B * F.a.Hk * F.splits;
     TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
-    auto kern = attention_few_kernel<T, BLOCKS, MT>;
-    TPW_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::ALLOC));
+    constexpr auto *kern = &attention_few_kernel<T, BLOCKS, MT>;
+    if (const int e = allow_shared_memory<kern>((int)L::ALLOC)) return e;
     kern<<<(unsigned)blocks, kFewThreads, L::ALLOC, s>>>(k, v, F);
     TPW_LAUNCH_OK("attention_few_kernel");
     return TPW_OK;

@@ -9,9 +9,11 @@
 // Bound: per pair of tiles 4 products of 128 x 128 x D, 2048 tensor-core clocks at D = 128, and 32768 exponentials, 2048 clocks of
 // the four special-function units: both pipes would be full at once.
 //
-// The reference m_i only moves when the maximum exceeds it by more than a factor 2^8 (the accumulators must then be read, scaled and written
-// back); until then probabilities up to 2^8 do no harm in fp32 sums.  Half precision additionally lifts them by 2^6: they
-// stay below 2^14, and lose digits only below 2^-20 of the row's largest.
+// The reference m_i is the first tile's maximum and moves only when a later score exceeds it by more than a factor 2^40 (the accumulators must
+// then be read, scaled and written back): probabilities above 1 do no harm in fp32 sums and bfloat16.  So a tile's probabilities do not
+// wait for its maximum, which is taken beside them; a tile that moves the reference forms them again.  Half precision ends at 2^16: there the
+// factor is 2^8, and all are lifted by 2^6, so that they lose digits only below 2^-20 of the row's largest.
+// A quarter of the exponentials is a polynomial on the FMA pipes, and O += P V starts when three quarters of P are there.
 #include "attention_tc.cuh"
 
 namespace tpw {
@@ -28,11 +30,10 @@ template <int BLOCKS> struct ForwardSmem {
     static constexpr uint32_t TILE_BYTES = BLOCKS * BLOCK_BYTES;
     static constexpr uint32_t OFF_RING = 2 * TILE_BYTES;
     static constexpr uint32_t OFF_BAR = OFF_RING + kSlots * TILE_BYTES;
-    static constexpr uint32_t OFF_TMEM = OFF_BAR + 8 * (2 * kSlots + 8);
+    static constexpr uint32_t OFF_TMEM = OFF_BAR + 8 * (2 * kSlots + 10);
     static constexpr uint32_t ALLOC = OFF_TMEM + 16 + 1024;
     static_assert(ALLOC <= 232448, "exceeds the dynamic shared memory of one CTA");
 };
-constexpr float kSlack = 8.f;
 
 template <typename T, int BLOCKS>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -44,7 +45,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *empty = full + L::kSlots, *q_full = empty + L::kSlots,
-             *s_full = q_full + 1, *p_full = s_full + 2, *o_full = p_full + 2, *drained = o_full + 2;
+             *s_full = q_full + 1, *p_most = s_full + 2, *p_full = p_most + 2, *o_full = p_full + 2, *drained = o_full + 2;
     uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(smem + L::OFF_TMEM);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_TMEM + 4);
 
@@ -72,7 +73,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         for (int i = 0; i < L::kSlots; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         mbar_init(q_full, 1);
         mbar_init(drained, 1);
-        for (int s = 0; s < 2; ++s) { mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&s_full[s], 1); mbar_init(&p_most[s], 4); mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
         *abort_flag = 0;
         mbar_init_fence();
         tma_prefetch_descriptor(&map_q);
@@ -156,9 +157,13 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             if (t + 1 < end && !(ok = arrived(u + 1))) break;
             for (int s = 0; s < 2 && ok; ++s) {
                 if (t_lo[s] <= t && t < t_hi[s]) {
-                    if (!(ok = warp_wait(&p_full[s], done[s] & 1, 5))) break;
+                    const uint32_t v_at = ring + (u % L::kSlots) * L::TILE_BYTES;
+                    if (!(ok = warp_wait(&p_most[s], done[s] & 1, 5))) break;
                     tc_fence_after();
-                    product_tokens(leader, tmem + (2 + s) * TILE, tmem + s * TILE, 32, ring + (u % L::kSlots) * L::TILE_BYTES, idesc_o, done[s] > 0);
+                    product_tokens<0, 6>(leader, tmem + (2 + s) * TILE, tmem + s * TILE, 32, v_at, idesc_o, done[s] > 0);
+                    if (!(ok = warp_wait(&p_full[s], done[s] & 1, 9))) break;
+                    tc_fence_after();
+                    product_tokens<6, 8>(leader, tmem + (2 + s) * TILE, tmem + s * TILE, 32, v_at, idesc_o, true);
                     commit_by(leader, &o_full[s]);
                     ++done[s];
                 }
@@ -198,17 +203,51 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         if (j < lo || j >= hi) x[g][e] = 0xff800000u;
                     }
             }
-            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            auto highest = [&]() {   // NaN for a score that is NaN or +inf: inf - inf makes the row NaN from there on
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < 32; e += 2)
+                for (int e = 0; e < 32; e += 2)
 #pragma unroll
-                for (int g = 0; g < 4; ++g) tops[g] = max3(tops[g], __uint_as_float(x[g][e]), __uint_as_float(x[g][e + 1]));
-            const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
-            const bool moves = m == -INFINITY ? top > -INFINITY : (top - m) * c > kSlack;
-            const bool scales = moves && m != -INFINITY;   // so far only zeros were added otherwise
-            if (__any_sync(0xffffffffu, scales)) {
+                    for (int g = 0; g < 4; ++g) tops[g] = max3_nan(tops[g], __uint_as_float(x[g][e]), __uint_as_float(x[g][e + 1]));
+                const float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
+                return top < INFINITY ? top : NAN;
+            };
+            f32x2 sum, shift2;
+            auto form = [&](int g) {   // 32 keys' probabilities
+                uint32_t p[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const f32x2 z = fma2(pack2(__uint_as_float(x[g][2 * e]), __uint_as_float(x[g][2 * e + 1])), pack2(c, c), shift2);
+                    const f32x2 y = e % 4 == 3 ? exp2_polynomial(z) : exp2_pair(z);
+                    sum = add2(sum, y);
+                    float y0, y1;
+                    unpack2(y, y0, y1);
+                    p[e] = N::pack(y0, y1);
+                }
+                tmem_st16(s_at + 16 * g, p);
+            };
+            auto hand_over = [&](uint64_t *bar) {
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar);
+            };
+            if (n == 0) m = highest();
+#pragma unroll 1
+            for (int pass = 0;; ++pass) {
+                const float shift = m == -INFINITY ? 0.f : N::kLift - m * c;
+                shift2 = pack2(shift, shift);
+                sum = pack2(0.f, 0.f);
+#pragma unroll
+                for (int g = 0; g < 3; ++g) form(g);
+                const float top = highest();
+                const bool moves = m == -INFINITY ? top != -INFINITY : !((top - m) * c <= N::kSlack);
+                if (pass > 0 || !__any_sync(0xffffffffu, moves)) break;
+                const bool scales = moves && m != -INFINITY;   // so far only zeros were added otherwise
                 const float by = scales ? exp2_fast((m - top) * c) : 1.f;
                 l *= by;
+                if (moves) m = top;
+                if (n == 0 || !__any_sync(0xffffffffu, scales)) continue;
                 if (!(ok = warp_wait(&o_full[s], (n - 1) & 1, 7))) break;
                 tc_fence_after();
                 for (int g = 0; g < 2 * BLOCKS; ++g) {
@@ -220,39 +259,21 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     tmem_st32(o_at + 32 * g, o);
                 }
             }
-            if (moves) m = top;
-            const float shift = m == -INFINITY ? 0.f : N::kLift - m * c;
-            const f32x2 c2 = pack2(c, c), shift2 = pack2(shift, shift);
-            f32x2 sum = pack2(0.f, 0.f);
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                uint32_t p[32];
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    const uint32_t *pair = &x[2 * g + (e >> 4)][2 * (e & 15)];
-                    const f32x2 z = fma2(pack2(__uint_as_float(pair[0]), __uint_as_float(pair[1])), c2, shift2);
-                    float z0, z1;
-                    unpack2(z, z0, z1);
-                    z0 = exp2_fast(z0);
-                    z1 = exp2_fast(z1);
-                    sum = add2(sum, pack2(z0, z1));
-                    p[e] = N::pack(z0, z1);
-                }
-                tmem_st32(s_at + 32 * g, p);
-            }
+            if (!ok) break;
+            // the first 96 keys' probabilities start the product while the last ones are formed
+            hand_over(&p_most[s]);
+            form(3);
+            hand_over(&p_full[s]);
             float s0, s1;
             unpack2(sum, s0, s1);
             l += s0 + s1;
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[s]);
         }
         if (ok && n > 0) {
             ok = warp_wait(&o_full[s], (n - 1) & 1, 8);
             tc_fence_after();
         }
         if (ok) {
+            if (m == -INFINITY) l = 0.f;   // nothing seen
             const float by = l == 0.f ? 0.f : 1.f / l;
             if (i < nq && P.lse)
                 static_cast<float *>(P.lse)[bh * P.Nq + i] = l == 0.f ? -INFINITY : (m * c - N::kLift + log2f(l)) * 0.69314718055994531f;
@@ -306,8 +327,8 @@ template <typename T, int BLOCKS> int launch(const AttnParams &P, cudaStream_t s
     if (e != TPW_OK) return e;
     const long long blocks = F.tiles * P.B * P.Hq;
     TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
-    auto kern = attention_forward_kernel<T, BLOCKS>;
-    TPW_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::ALLOC));
+    constexpr auto *kern = &attention_forward_kernel<T, BLOCKS>;
+    if (const int e = allow_shared_memory<kern>((int)L::ALLOC)) return e;
     kern<<<(unsigned)blocks, kTcThreads, L::ALLOC, s>>>(q, k, v, F);
     TPW_LAUNCH_OK("attention_forward_kernel");
     return TPW_OK;

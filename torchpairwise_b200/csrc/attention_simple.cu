@@ -352,13 +352,13 @@ __global__ void __launch_bounds__(256) attention_dq_simple_kernel(const AttnPara
     store_rows<T, A, RM, DP>(out, P.Hq * P.D, dq, by, row0, nq, D, ty, tx);
 }
 
-template <typename K>
-int run(K kern, const char *name, const AttnParams &P, long long rows, int tile_rows, long long heads, size_t smem, cudaStream_t s) {
+template <auto *KERNEL>
+int run(const char *name, const AttnParams &P, long long rows, int tile_rows, long long heads, size_t smem, cudaStream_t s) {
     const long long tiles = (rows + tile_rows - 1) / tile_rows, blocks = tiles * heads * P.B;
     TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
     if (blocks == 0) return TPW_OK;
-    TPW_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    kern<<<(unsigned)blocks, 256, smem, s>>>(P, (int)tiles);
+    if (const int e = allow_shared_memory<KERNEL>((int)smem)) return e;
+    KERNEL<<<(unsigned)blocks, 256, smem, s>>>(P, (int)tiles);
     TPW_LAUNCH_OK(name);
     return TPW_OK;
 }
@@ -367,17 +367,17 @@ template <typename T, int DP, int BM, int BN> int forward(const AttnParams &P, c
     typedef typename AttnAcc<T>::type A;
     constexpr size_t smem = sizeof(A) * ((BM + 2 * BN) * (DP + PAD) + BM * (BN + PAD));
     static_assert(smem <= 232448, "exceeds the dynamic shared memory of one CTA");
-    return run(attention_forward_simple_kernel<T, A, DP, BM, BN>, "attention_forward_simple_kernel", P, P.Nq, BM, P.Hq, smem, s);
+    return run<&attention_forward_simple_kernel<T, A, DP, BM, BN>>("attention_forward_simple_kernel", P, P.Nq, BM, P.Hq, smem, s);
 }
 template <typename T, int DP, int BK, int BQ> int backward(const AttnParams &P, cudaStream_t s) {
     typedef typename AttnAcc<T>::type A;
     constexpr size_t kv = sizeof(A) * (2 * (BK + BQ) * (DP + PAD) + 2 * BK * (BQ + PAD)), qs = sizeof(A) * (2 * (BK + BQ) * (DP + PAD) + BQ * (BK + PAD));
     static_assert(kv <= 232448 && qs <= 232448, "exceeds the dynamic shared memory of one CTA");
     if (P.dk) {
-        const int e = run(attention_dkv_simple_kernel<T, A, DP, BK, BQ>, "attention_dkv_simple_kernel", P, P.Nk, BK, P.Hk, kv, s);
+        const int e = run<&attention_dkv_simple_kernel<T, A, DP, BK, BQ>>("attention_dkv_simple_kernel", P, P.Nk, BK, P.Hk, kv, s);
         if (e != TPW_OK) return e;
     }
-    if (P.dq) return run(attention_dq_simple_kernel<T, A, DP, BQ, BK>, "attention_dq_simple_kernel", P, P.Nq, BQ, P.Hq, qs, s);
+    if (P.dq) return run<&attention_dq_simple_kernel<T, A, DP, BQ, BK>>("attention_dq_simple_kernel", P, P.Nq, BQ, P.Hq, qs, s);
     return TPW_OK;
 }
 

@@ -19,6 +19,7 @@ template <typename T> struct Narrow;
 template <> struct Narrow<__nv_bfloat16> {
     static constexpr uint32_t kFormat = 1;   // of the instruction descriptor
     static constexpr float kLift = 0.f;      // probabilities are formed times 2^kLift: bfloat16 has the exponents of float32
+    static constexpr float kSlack = 40.f;    // and may exceed 1 by 2^kSlack
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
         uint32_t r;
         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -28,6 +29,7 @@ template <> struct Narrow<__nv_bfloat16> {
 template <> struct Narrow<__half> {
     static constexpr uint32_t kFormat = 0;
     static constexpr float kLift = 6.f;      // and half precision loses digits below 2^-14: see attention_forward.cu
+    static constexpr float kSlack = 8.f;
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
         uint32_t r;
         asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -84,11 +86,13 @@ template <int BLOCKS> __device__ __forceinline__ void product_features(uint32_t 
     for (int k = 0; k < 4 * BLOCKS; ++k)
         if (k < steps) mma_ss(leader, d, a + feature_step(k), b + feature_step(k), idesc, k != 0);
 }
-// D (+)= P Y over 128 tokens; P in tensor memory, 16 tokens to 8 columns, its second half `gap` columns behind the first's start
+// D (+)= P Y over the tokens [16 FROM, 16 TO) of a tile; P in tensor memory, 16 tokens to 8 columns, its second half `gap` columns behind the
+// first's start
+template <int FROM = 0, int TO = TILE / 16>
 __device__ __forceinline__ void product_tokens(uint32_t leader, uint32_t d, uint32_t p, uint32_t gap, uint32_t y, uint32_t idesc, bool accumulate) {
     const uint64_t b = make_smem_desc_tokens(y);
 #pragma unroll
-    for (int k = 0; k < TILE / 16; ++k)
+    for (int k = FROM; k < TO; ++k)
         mma_ts(leader, d, p + (k < 4 ? 8 * k : gap + 8 * (k - 4)), b + (uint64_t)k * (2048 >> 4), idesc, accumulate || k != 0);
 }
 
@@ -125,6 +129,13 @@ __device__ __forceinline__ void tmem_st_16x128(uint32_t taddr, const uint32_t (&
         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint64_t *bar, int c0, int c1, int c2, int c3) {
@@ -150,19 +161,44 @@ template <int BLOCKS> __device__ __forceinline__ void clear_tokens(unsigned char
     __syncwarp();
 }
 
-// Registers per thread of a warpgroup.  A block of 384 threads is launched with 168 each, 64512: two warpgroups at 200 and one at 104.
+// Registers per thread of a warpgroup.  A block of 384 threads is launched with 168 each, 64512: two warpgroups at 208 and one at 88.
 constexpr int kTcThreads = 384;
-__device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 200;"); }
-__device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 104;"); }
+__device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
+__device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;"); }
 
 __device__ __forceinline__ float exp2_fast(float x) {   // 2 units of the last place; 0 below 2^-126
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
+// 2^z of a pair on the FMA pipes: 2^n 2^f with n the nearest whole number and f in [-1/2, 1/2], where the polynomial (relative minimax fit of
+// degree 4, by the exchange algorithm) is good to 2.6e-6.  Below 2^-126 it stays there: beside a row's largest term that is zero.
+// The special-function units make 16 exponentials a clock and SM, half of what the tensor cores could use; a share of them goes here.
+__device__ __forceinline__ f32x2 exp2_polynomial(f32x2 z) {
+    float z0, z1;
+    unpack2(z, z0, z1);
+    z = pack2(fmaxf(z0, -126.f), fmaxf(z1, -126.f));
+    const f32x2 magic = pack2(12582912.f, 12582912.f);   // 1.5 * 2^23: a sum with it ends in the nearest whole number
+    const f32x2 n = add2(z, magic), f = sub2(z, sub2(n, magic));
+    f32x2 p = pack2(0.009570102207362652f, 0.009570102207362652f);
+    p = fma2(p, f, pack2(0.05591785907745361f, 0.05591785907745361f));
+    p = fma2(p, f, pack2(0.240247443318367f, 0.240247443318367f));
+    p = fma2(p, f, pack2(0.6931217908859253f, 0.6931217908859253f));
+    p = fma2(p, f, pack2(0.9999992847442627f, 0.9999992847442627f));
+    float p0, p1, n0, n1;
+    unpack2(p, p0, p1);
+    unpack2(n, n0, n1);
+    return pack2(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23)), __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23)));
+}
+__device__ __forceinline__ f32x2 exp2_pair(f32x2 z) {
+    float z0, z1;
+    unpack2(z, z0, z1);
+    return pack2(exp2_fast(z0), exp2_fast(z1));
+}
+// NaN if any operand is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 
