@@ -41,15 +41,24 @@ template <> struct Lift<__half> {
     }
 };
 
-template <int BLOCKS> struct BackwardSmem {
-    static constexpr int kStages = BLOCKS == 2 ? 2 : 3;
+// Shared memory of either walk: the CTA's own two tiles, then rings of walked tiles, each with its full and empty barriers.
+template <int BLOCKS> struct KeysSmem {
+    static constexpr int kStages = BLOCKS == 2 ? 2 : 4;                        // of queries and of gradients
     static constexpr uint32_t TILE_BYTES = BLOCKS * BLOCK_BYTES;
-    static constexpr uint32_t OFF_RING = 2 * TILE_BYTES;                       // the CTA's own two tiles, then the walked tiles
-    static constexpr uint32_t OFF_ROWS = OFF_RING + kStages * 2 * TILE_BYTES;  // lse, delta of a query tile per stage
+    static constexpr uint32_t OFF_Q = 2 * TILE_BYTES, OFF_G = OFF_Q + kStages * TILE_BYTES;
+    static constexpr uint32_t OFF_ROWS = OFF_G + kStages * TILE_BYTES;         // lse, delta of a query tile per stage
     static constexpr uint32_t OFF_BAR = OFF_ROWS + kStages * 2 * TILE * 4;
-    static constexpr uint32_t OFF_TMEM = OFF_BAR + 8 * (4 * kStages + 10);
-    // queries walk: a V tile is free again once dP has read it, a K tile only after dQ
-    static constexpr int kKeys = BLOCKS == 2 ? 3 : 4, kValues = 2 * kStages - kKeys;
+    static constexpr uint32_t OFF_TMEM = OFF_BAR + 8 * (4 * kStages + 7);
+    static constexpr uint32_t ALLOC = OFF_TMEM + 16 + 1024;
+    static_assert(ALLOC <= 232448, "exceeds the dynamic shared memory of one CTA");
+};
+template <int BLOCKS> struct QueriesSmem {
+    // a V tile is free again once dP has read it, a K tile only after dQ
+    static constexpr int kKeys = BLOCKS == 2 ? 3 : 4, kValues = BLOCKS == 2 ? 2 : 3;
+    static constexpr uint32_t TILE_BYTES = BLOCKS * BLOCK_BYTES;
+    static constexpr uint32_t OFF_K = 2 * TILE_BYTES, OFF_V = OFF_K + kKeys * TILE_BYTES;
+    static constexpr uint32_t OFF_BAR = OFF_V + kValues * TILE_BYTES;
+    static constexpr uint32_t OFF_TMEM = OFF_BAR + 8 * (2 * (kKeys + kValues) + 8);
     static constexpr uint32_t ALLOC = OFF_TMEM + 16 + 1024;
     static_assert(ALLOC <= 232448, "exceeds the dynamic shared memory of one CTA");
 };
@@ -92,13 +101,13 @@ template <typename T, int BLOCKS>
 __global__ void __launch_bounds__(kTcThreads, 1)
 attention_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                      const __grid_constant__ CUtensorMap map_g, const BackwardParams F) {
-    typedef BackwardSmem<BLOCKS> L;
+    typedef KeysSmem<BLOCKS> L;
     typedef Narrow<T> N;
     const AttnParams &P = F.a;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *q_full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *g_full = q_full + L::kStages, *empty = g_full + L::kStages,
-             *kv_full = empty + L::kStages, *s_full = kv_full + 1, *dp_full = s_full + 1, *p_ready = dp_full + 1, *ds_ready = p_ready + 1,
+    uint64_t *q_full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *g_full = q_full + L::kStages, *q_empty = g_full + L::kStages,
+             *g_empty = q_empty + L::kStages, *kv_full = g_empty + L::kStages, *s_full = kv_full + 1, *dp_full = s_full + 1, *p_ready = dp_full + 1, *ds_ready = p_ready + 1,
              *acc_full = ds_ready + 1, *drained = acc_full + 1;
     uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(smem + L::OFF_TMEM);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_TMEM + 4);
@@ -115,7 +124,7 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     const int total = per_head * (int)P.group;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < L::kStages; ++i) { mbar_init(&q_full[i], 1); mbar_init(&g_full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < L::kStages; ++i) { mbar_init(&q_full[i], 1); mbar_init(&g_full[i], 1); mbar_init(&q_empty[i], 1); mbar_init(&g_empty[i], 1); }
         mbar_init(kv_full, 1);
         mbar_init(s_full, 1);
         mbar_init(dp_full, 1);
@@ -144,45 +153,40 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         if (!ok) give_up(site);
         return ok;
     };
-    const uint32_t k_at = smem_u32(smem), v_at = k_at + L::TILE_BYTES, ring = smem_u32(smem + L::OFF_RING);
-    const uint32_t rows_at = smem_u32(smem + L::OFF_ROWS);
+    const uint32_t k_at = smem_u32(smem), v_at = k_at + L::TILE_BYTES, q_ring = smem_u32(smem + L::OFF_Q), g_ring = smem_u32(smem + L::OFF_G),
+                   rows_at = smem_u32(smem + L::OFF_ROWS);
     const uint32_t S = tmem, DP = tmem + TILE, DV = tmem + 2 * TILE, DK = tmem + 3 * TILE;
 
     if (warp >= 8) registers_down();
     if (warp == 8) {
         if (lane == 0 && total > 0) {
-            uint32_t issued = 0;
+            uint32_t issued_q = 0, issued_g = 0;
             mbar_expect_tx(kv_full, 2 * L::TILE_BYTES);
             load_tokens<BLOCKS>(k_at, &map_k, kv_full, row0, hk, b);
             load_tokens<BLOCKS>(v_at, &map_v, kv_full, row0, hk, b);
-            for (int u = 0; u < total; ++u) {
+            auto load = [&](uint64_t *full, uint64_t *empty, uint32_t ring, const CUtensorMap *map, const void *terms, uint32_t terms_at, uint32_t u, uint32_t &issued) {
                 const uint32_t st = u % L::kStages;
                 if (u >= L::kStages && !wait_or_abort(&empty[st], parity_of_use(u, L::kStages) ^ 1, abort_flag)) {
                     give_up(1);
-                    break;
+                    return false;
                 }
                 const int h = hk * (int)P.group + u / per_head, i0 = (begin + u % per_head) * TILE;
-                const long long at = (b * P.Hq + h) * P.Nqp + i0;
-                const uint32_t q_at = ring + st * 2 * L::TILE_BYTES, rows = rows_at + st * 2 * TILE * 4;
-                mbar_expect_tx(&q_full[st], L::TILE_BYTES + TILE * 4);
-                load_tokens<BLOCKS>(q_at, &map_q, &q_full[st], i0, h, b);
-                bulk_load(rows, static_cast<const float *>(P.row_lse) + at, TILE * 4, &q_full[st]);
-                mbar_expect_tx(&g_full[st], L::TILE_BYTES + TILE * 4);
-                load_tokens<BLOCKS>(q_at + L::TILE_BYTES, &map_g, &g_full[st], i0, h, b);
-                bulk_load(rows + TILE * 4, static_cast<const float *>(P.row_delta) + at, TILE * 4, &g_full[st]);
+                mbar_expect_tx(&full[st], L::TILE_BYTES + TILE * 4);
+                load_tokens<BLOCKS>(ring + st * L::TILE_BYTES, map, &full[st], i0, h, b);
+                bulk_load(terms_at + st * 2 * TILE * 4, static_cast<const float *>(terms) + (b * P.Hq + h) * P.Nqp + i0, TILE * 4, &full[st]);
                 issued = u + 1;
-            }
-            for (uint32_t u = first_of_last_uses(issued, L::kStages); u < issued; ++u)
-                if (!wait_or_abort(&empty[u % L::kStages], parity_of_use(u, L::kStages), abort_flag)) {
-                    give_up(2);
+                return true;
+            };
+            // a gradient tile is free after dV, a query tile only after dK: the gradients are fetched first
+            for (int u = 0; u < total; ++u)
+                if (!load(g_full, g_empty, g_ring, &map_g, P.row_delta, rows_at + TILE * 4, u, issued_g) ||
+                    !load(q_full, q_empty, q_ring, &map_q, P.row_lse, rows_at, u, issued_q))
                     break;
-                }
+            if (!wait_for_releases(q_empty, issued_q, L::kStages, abort_flag) || !wait_for_releases(g_empty, issued_g, L::kStages, abort_flag)) give_up(2);
             if (*abort_flag) {   // what was issued arrives before the CTA ends
                 mbar_wait_bounded(kv_full, 0);
-                for (uint32_t u = first_of_last_uses(issued, L::kStages); u < issued; ++u) {
-                    mbar_wait_bounded(&q_full[u % L::kStages], parity_of_use(u, L::kStages));
-                    mbar_wait_bounded(&g_full[u % L::kStages], parity_of_use(u, L::kStages));
-                }
+                for (uint32_t u = first_of_last_uses(issued_q, L::kStages); u < issued_q; ++u) mbar_wait_bounded(&q_full[u % L::kStages], parity_of_use(u, L::kStages));
+                for (uint32_t u = first_of_last_uses(issued_g, L::kStages); u < issued_g; ++u) mbar_wait_bounded(&g_full[u % L::kStages], parity_of_use(u, L::kStages));
             }
         }
     } else if (warp == 9) {
@@ -191,26 +195,27 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         const uint32_t leader = elect_lane();
         bool ok = total == 0 || warp_wait(kv_full, 0, 3);
         // S^T or dP^T of use u, once its tile has arrived
-        auto first = [&](uint64_t *arrives, int u, uint32_t d, uint32_t own, uint32_t offset, uint64_t *done, int site) {
+        auto first = [&](uint64_t *arrives, int u, uint32_t d, uint32_t own, uint32_t ring, uint64_t *done, int site) {
             const uint32_t st = u % L::kStages;
             if (!warp_wait(&arrives[st], parity_of_use(u, L::kStages), site)) return false;
             tc_fence_after();
-            product_features<BLOCKS>(leader, d, own, ring + st * 2 * L::TILE_BYTES + offset, idesc_s, steps);
+            product_features<BLOCKS>(leader, d, own, ring + st * L::TILE_BYTES, idesc_s, steps);
             commit_by(leader, done);
             return true;
         };
-        if (total > 0 && ok) ok = first(q_full, 0, S, k_at, 0, s_full, 4) && first(g_full, 0, DP, v_at, L::TILE_BYTES, dp_full, 5);
+        if (total > 0 && ok) ok = first(q_full, 0, S, k_at, q_ring, s_full, 4) && first(g_full, 0, DP, v_at, g_ring, dp_full, 5);
         for (int u = 0; u < total && ok; ++u) {
-            const uint32_t q_at = ring + (u % L::kStages) * 2 * L::TILE_BYTES;
+            const uint32_t st = u % L::kStages;
             if (!(ok = warp_wait(p_ready, u & 1, 6))) break;
             tc_fence_after();
-            product_tokens(leader, DV, S, 64, q_at + L::TILE_BYTES, idesc_d, u > 0);
-            if (u + 1 < total && !(ok = first(q_full, u + 1, S, k_at, 0, s_full, 4))) break;
+            product_tokens(leader, DV, S, 64, g_ring + st * L::TILE_BYTES, idesc_d, u > 0);
+            commit_by(leader, &g_empty[st]);
+            if (u + 1 < total && !(ok = first(q_full, u + 1, S, k_at, q_ring, s_full, 4))) break;
             if (!(ok = warp_wait(ds_ready, u & 1, 7))) break;
             tc_fence_after();
-            product_tokens(leader, DK, DP, 64, q_at, idesc_d, u > 0);
-            commit_by(leader, &empty[u % L::kStages]);
-            if (u + 1 < total && !(ok = first(g_full, u + 1, DP, v_at, L::TILE_BYTES, dp_full, 5))) break;
+            product_tokens(leader, DK, DP, 64, q_ring + st * L::TILE_BYTES, idesc_d, u > 0);
+            commit_by(leader, &q_empty[st]);
+            if (u + 1 < total && !(ok = first(g_full, u + 1, DP, v_at, g_ring, dp_full, 5))) break;
         }
         if (ok && total > 0) commit_by(leader, acc_full);
         __syncwarp();
@@ -281,9 +286,8 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         const uint32_t *pair = &x[hh][4 * i + 2 * r];
-                        float z0, z1;
-                        unpack2(fma2(pack2(__uint_as_float(pair[0]), __uint_as_float(pair[1])), c2, minus_lse), z0, z1);
-                        p[hh][2 * i + r] = pack2(exp2_fast(z0), exp2_fast(z1));
+                        const f32x2 z = fma2(pack2(__uint_as_float(pair[0]), __uint_as_float(pair[1])), c2, minus_lse);
+                        p[hh][2 * i + r] = 2 * hh + r == 3 ? exp2_polynomial(z) : exp2_pair(z);
                     }
             }
             if (masked) hide(p, i0);
@@ -338,7 +342,7 @@ template <typename T, int BLOCKS>
 __global__ void __launch_bounds__(kTcThreads, 1)
 attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                     const __grid_constant__ CUtensorMap map_g, const BackwardParams F) {
-    typedef BackwardSmem<BLOCKS> L;
+    typedef QueriesSmem<BLOCKS> L;
     typedef Narrow<T> N;
     const AttnParams &P = F.a;
     extern __shared__ unsigned char smem_raw[];
@@ -391,7 +395,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         if (!ok) give_up(site);
         return ok;
     };
-    const uint32_t q_at = smem_u32(smem), g_at = q_at + L::TILE_BYTES, keys = smem_u32(smem + L::OFF_RING), values = keys + L::kKeys * L::TILE_BYTES;
+    const uint32_t q_at = smem_u32(smem), g_at = q_at + L::TILE_BYTES, keys = smem_u32(smem + L::OFF_K), values = smem_u32(smem + L::OFF_V);
     const uint32_t S = tmem, DP = tmem + TILE, DQ = tmem + 3 * TILE;
 
     if (warp >= 8) registers_down();
@@ -435,7 +439,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             if (!warp_wait(&k_full[sk], parity_of_use(u, L::kKeys), 4)) return false;
             tc_fence_after();
             const int beyond = see.length - (begin + u) * TILE;
-            if (beyond < TILE && (int)P.Nk > see.length) clear_tokens<BLOCKS>(smem + L::OFF_RING + sk * L::TILE_BYTES, beyond, lane);
+            if (beyond < TILE && (int)P.Nk > see.length) clear_tokens<BLOCKS>(smem + L::OFF_K + sk * L::TILE_BYTES, beyond, lane);
             product_features<BLOCKS>(leader, S, q_at, keys + sk * L::TILE_BYTES, idesc_s, steps);
             commit_by(leader, s_full);
             if (!warp_wait(&v_full[sv], parity_of_use(u, L::kValues), 10)) return false;
@@ -487,9 +491,8 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
                 const uint32_t *pair = &x[e >> 4][2 * (e & 15)];
-                float z0, z1;
-                unpack2(fma2(pack2(__uint_as_float(pair[0]), __uint_as_float(pair[1])), c2, minus_lse), z0, z1);
-                p[e] = pack2(exp2_fast(z0), exp2_fast(z1));
+                const f32x2 z = fma2(pack2(__uint_as_float(pair[0]), __uint_as_float(pair[1])), c2, minus_lse);
+                p[e] = e % 4 == 3 ? exp2_polynomial(z) : exp2_pair(z);
             }
             if (!(ok = warp_wait(&dp_full[u & 1], (u >> 1) & 1, 8))) break;
             tc_fence_after();
@@ -547,7 +550,6 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 }
 
 template <typename T, int BLOCKS> int launch(const AttnParams &P, cudaStream_t s) {
-    typedef BackwardSmem<BLOCKS> L;
     BackwardParams F = {};
     F.a = P;
     F.a.status = device_status_ptr();
@@ -564,8 +566,9 @@ template <typename T, int BLOCKS> int launch(const AttnParams &P, cudaStream_t s
         const long long blocks = F.tiles * P.B * P.Hk;
         TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
         constexpr auto *kern = &attention_dkv_kernel<T, BLOCKS>;
-        if (const int e = allow_shared_memory<kern>((int)L::ALLOC)) return e;
-        kern<<<(unsigned)blocks, kTcThreads, L::ALLOC, s>>>(q, k, v, g, F);
+        constexpr uint32_t smem = KeysSmem<BLOCKS>::ALLOC;
+        if (const int e = allow_shared_memory<kern>((int)smem)) return e;
+        kern<<<(unsigned)blocks, kTcThreads, smem, s>>>(q, k, v, g, F);
         TPW_LAUNCH_OK("attention_dkv_kernel");
     }
     if (P.dq) {
@@ -573,8 +576,9 @@ template <typename T, int BLOCKS> int launch(const AttnParams &P, cudaStream_t s
         const long long blocks = F.tiles * P.B * P.Hq;
         TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
         constexpr auto *kern = &attention_dq_kernel<T, BLOCKS>;
-        if (const int e = allow_shared_memory<kern>((int)L::ALLOC)) return e;
-        kern<<<(unsigned)blocks, kTcThreads, L::ALLOC, s>>>(q, k, v, g, F);
+        constexpr uint32_t smem = QueriesSmem<BLOCKS>::ALLOC;
+        if (const int e = allow_shared_memory<kern>((int)smem)) return e;
+        kern<<<(unsigned)blocks, kTcThreads, smem, s>>>(q, k, v, g, F);
         TPW_LAUNCH_OK("attention_dq_kernel");
     }
     return TPW_OK;

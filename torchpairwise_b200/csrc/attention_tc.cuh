@@ -171,13 +171,20 @@ __device__ __forceinline__ float exp2_fast(float x) {   // 2 units of the last p
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// NaN if any operand is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 // 2^z of a pair on the FMA pipes: 2^n 2^f with n the nearest whole number and f in [-1/2, 1/2], where the polynomial (relative minimax fit of
-// degree 4, by the exchange algorithm) is good to 2.6e-6.  Below 2^-126 it stays there: beside a row's largest term that is zero.
+// degree 4, by the exchange algorithm) is good to 2.6e-6.  Below 2^-126 it stays there: beside a row's largest term that is zero.  NaN
+// gives 2^128 - 2^104, infinity in 16 bits.
 // The special-function units make 16 exponentials a clock and SM, half of what the tensor cores could use; a share of them goes here.
 __device__ __forceinline__ f32x2 exp2_polynomial(f32x2 z) {
     float z0, z1;
     unpack2(z, z0, z1);
-    z = pack2(fmaxf(z0, -126.f), fmaxf(z1, -126.f));
+    z = pack2(max3_nan(z0, -126.f, -126.f), max3_nan(z1, -126.f, -126.f));
     const f32x2 magic = pack2(12582912.f, 12582912.f);   // 1.5 * 2^23: a sum with it ends in the nearest whole number
     const f32x2 n = add2(z, magic), f = sub2(z, sub2(n, magic));
     f32x2 p = pack2(0.009570102207362652f, 0.009570102207362652f);
@@ -195,12 +202,5 @@ __device__ __forceinline__ f32x2 exp2_pair(f32x2 z) {
     unpack2(z, z0, z1);
     return pack2(exp2_fast(z0), exp2_fast(z1));
 }
-// NaN if any operand is
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-
 } // namespace
 } // namespace tpw
