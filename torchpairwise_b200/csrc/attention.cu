@@ -27,6 +27,9 @@ int check(const tpw_attention *a, bool backward) {
 
 bool nothing(const tpw_attention &a) { return a.B == 0 || a.Nq == 0 || a.Hq == 0; }
 
+AttnSplits splits_of(int dtype, const AttnParams &P) {
+    return attn_few_fits(dtype, P) ? attn_few_splits(P) : attn_tc_fits(dtype, P) ? attn_tc_splits(P) : AttnSplits();
+}
 long long split_bytes(const AttnParams &P, const AttnSplits &splits) {
     return splits.count > 1 ? 4 * splits.count * P.B * P.Hq * P.Nq * (P.D + 1) : 0;
 }
@@ -41,7 +44,7 @@ int64_t tpw_attention_scratch_bytes(const tpw_attention *a) {
     if (tpw::check(a, false) != TPW_OK) return -1;
     if (tpw::nothing(*a)) return 0;
     const tpw::AttnParams P = tpw::attn_params(*a);
-    return tpw::attn_few_fits(a->dtype, P) ? tpw::split_bytes(P, tpw::attn_few_splits(P)) : 0;
+    return tpw::split_bytes(P, tpw::splits_of(a->dtype, P));
 }
 
 int tpw_attention_forward(const tpw_attention *a, void *scratch, int64_t scratch_bytes, tpw_stream_t stream) {
@@ -50,17 +53,16 @@ int tpw_attention_forward(const tpw_attention *a, void *scratch, int64_t scratch
     if (e != TPW_OK || tpw::nothing(*a)) return e;
     const tpw::AttnParams P = tpw::attn_params(*a);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (tpw::attn_few_fits(a->dtype, P)) {
-        tpw::AttnSplits splits = tpw::attn_few_splits(P);
+    if (tpw::attn_tc_fits(a->dtype, P)) {
+        tpw::AttnSplits splits = tpw::splits_of(a->dtype, P);
         const int64_t bytes = tpw::split_bytes(P, splits);
         TPW_CHECK_ARG(bytes == 0 || (scratch && tpw::aligned16(scratch) && scratch_bytes >= bytes),
                       "tpw_attention_forward: scratch of %lld bytes, 16-byte aligned, is needed", (long long)bytes);
         splits.out = static_cast<float *>(scratch);
         splits.lse = splits.out ? splits.out + splits.count * P.B * P.Hq * P.Nq * P.D : nullptr;
-        const int e = tpw::attn_few_forward(a->dtype, P, splits, s);
+        const int e = tpw::attn_few_fits(a->dtype, P) ? tpw::attn_few_forward(a->dtype, P, splits, s) : tpw::attn_tc_forward(a->dtype, P, splits, s);
         return e != TPW_OK || splits.count == 1 ? e : tpw::attn_join(a->dtype, P, splits, s);
     }
-    if (tpw::attn_tc_fits(a->dtype, P)) return tpw::attn_tc_forward(a->dtype, P, s);
     return tpw::attn_simple_forward(a->dtype, P, s);
 }
 

@@ -64,14 +64,16 @@ template <auto *KERNEL> int allow_shared_memory(int bytes) {
 // swizzle) by `box_tokens` tokens; what lies beyond the tensor reads as zero
 int make_tensor_map_heads(CUtensorMap *map, const void *base, uint64_t features, uint64_t tokens, uint64_t heads, uint64_t batch,
                           uint64_t token_pitch, uint64_t head_pitch, uint64_t batch_pitch, uint32_t box_tokens);
-// attention_forward.cu: 16-bit types on the tensor cores
-bool attn_tc_fits(int dtype, const AttnParams &P);
-int attn_tc_forward(int dtype, const AttnParams &P, cudaStream_t s);
-// attention_few.cu: few query rows, the keys cut into ranges that are joined afterwards
+// the keys cut into ranges whose parts are joined afterwards
 struct AttnSplits {
     int count = 1, keys = 0;             // ranges and keys of each
     float *out = nullptr, *lse = nullptr; // [count, B, Hq, Nq, D] outputs and [count, B, Hq, Nq] log-sums of the ranges
 };
+// attention_forward.cu: 16-bit types on the tensor cores
+bool attn_tc_fits(int dtype, const AttnParams &P);
+AttnSplits attn_tc_splits(const AttnParams &P);
+int attn_tc_forward(int dtype, const AttnParams &P, const AttnSplits &splits, cudaStream_t s);
+// attention_few.cu: few query rows
 bool attn_few_fits(int dtype, const AttnParams &P);
 AttnSplits attn_few_splits(const AttnParams &P);
 int attn_few_forward(int dtype, const AttnParams &P, const AttnSplits &splits, cudaStream_t s);

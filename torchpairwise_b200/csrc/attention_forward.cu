@@ -22,7 +22,9 @@ namespace {
 struct ForwardParams {
     AttnParams a;
     float scale_log2;
-    int tiles;          // of 256 queries
+    int tiles;                    // of 256 queries
+    int splits, tiles_per_split;  // ranges of key tiles
+    float *part_out, *part_lse;   // splits > 1
 };
 
 template <int BLOCKS> struct ForwardSmem {
@@ -50,10 +52,10 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_TMEM + 4);
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const long long heads = P.B * P.Hq;
+    const unsigned heads = (unsigned)(P.B * P.Hq), split = blockIdx.x % F.splits, item = blockIdx.x / F.splits;
     // a causal call's longest rows first, all heads of them together
-    const int tile = F.tiles - 1 - (int)(blockIdx.x / heads);
-    const long long bh = blockIdx.x % heads;
+    const int tile = F.tiles - 1 - (int)(item / heads);
+    const long long bh = item % heads;
     const int h = (int)(bh % P.Hq), b = (int)(bh / P.Hq), hk = h / (int)P.group;
     const Seen see(P, b);
     const int nq = (int)P.Nq, row0 = tile * 2 * TILE;
@@ -64,6 +66,11 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const int first = row0 + s * TILE, last = (first + TILE < nq ? first + TILE : nq) - 1;
         t_lo[s] = see.lo(first) / TILE;
         t_hi[s] = first < nq ? (see.hi(last) + TILE - 1) / TILE : 0;
+        if (F.splits > 1) {
+            const int from = split * F.tiles_per_split, to = from + F.tiles_per_split;
+            t_lo[s] = t_lo[s] > from ? t_lo[s] : from;
+            t_hi[s] = t_hi[s] < to ? t_hi[s] : to;
+        }
         if (t_hi[s] <= t_lo[s]) t_lo[s] = t_hi[s] = 0;
     }
     const bool some0 = t_hi[0] > 0, some1 = t_hi[1] > 0;
@@ -275,9 +282,13 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         if (ok) {
             if (m == -INFINITY) l = 0.f;   // nothing seen
             const float by = l == 0.f ? 0.f : 1.f / l;
-            if (i < nq && P.lse)
-                static_cast<float *>(P.lse)[bh * P.Nq + i] = l == 0.f ? -INFINITY : (m * c - N::kLift + log2f(l)) * 0.69314718055994531f;
+            const float lse = l == 0.f ? -INFINITY : (m * c - N::kLift + log2f(l)) * 0.69314718055994531f;
+            const long long flat = bh * P.Nq + i, all_rows = P.B * P.Hq * P.Nq;
+            if (i < nq && F.splits > 1) F.part_lse[split * all_rows + flat] = lse;
+            else if (i < nq && P.lse) static_cast<float *>(P.lse)[flat] = lse;
             T *out = static_cast<T *>(P.out) + ((b * P.Nq + i) * P.Hq + h) * P.D;
+            float *part = F.part_out + (split * all_rows + flat) * P.D;
+            const bool empty = n == 0 || l == 0.f;
 #pragma unroll 1
             for (int g = 0; g < 2 * BLOCKS; ++g) {
                 uint32_t o[32];
@@ -285,14 +296,25 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     tmem_ld32(o_at + 32 * g, o);
                     tmem_ld_wait();
                 }
+                if (F.splits > 1) {
+                    if (n == 0) break;   // nothing seen: the joining kernel does not look at it
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        float4 w;
+                        w.x = empty ? 0.f : __uint_as_float(o[e]) * by;
+                        w.y = empty ? 0.f : __uint_as_float(o[e + 1]) * by;
+                        w.z = empty ? 0.f : __uint_as_float(o[e + 2]) * by;
+                        w.w = empty ? 0.f : __uint_as_float(o[e + 3]) * by;
+                        if (i < nq && 32 * g + e < (int)P.D) *reinterpret_cast<float4 *>(part + 32 * g + e) = w;
+                    }
+                    continue;
+                }
 #pragma unroll
                 for (int e = 0; e < 32; e += 8) {
                     uint32_t w[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float a0 = n > 0 && l != 0.f ? __uint_as_float(o[e + 2 * k]) * by : 0.f, a1 = n > 0 && l != 0.f ? __uint_as_float(o[e + 2 * k + 1]) * by : 0.f;
-                        w[k] = N::pack(a0, a1);
-                    }
+                    for (int k = 0; k < 4; ++k)
+                        w[k] = empty ? 0u : N::pack(__uint_as_float(o[e + 2 * k]) * by, __uint_as_float(o[e + 2 * k + 1]) * by);
                     const int d = 32 * g + e;
                     if (i < nq && d < (int)P.D) *reinterpret_cast<uint4 *>(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
@@ -313,19 +335,23 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     }
 }
 
-template <typename T, int BLOCKS> int launch(const AttnParams &P, cudaStream_t s) {
+template <typename T, int BLOCKS> int launch(const AttnParams &P, const AttnSplits &splits, cudaStream_t s) {
     typedef ForwardSmem<BLOCKS> L;
     ForwardParams F = {};
     F.a = P;
     F.a.status = device_status_ptr();
     F.scale_log2 = (float)(P.scale * 1.4426950408889634074);
     F.tiles = (int)((P.Nq + 2 * TILE - 1) / (2 * TILE));
+    F.splits = splits.count;
+    F.tiles_per_split = splits.keys / TILE;
+    F.part_out = splits.out;
+    F.part_lse = splits.lse;
     CUtensorMap q, k, v;
     int e = make_tensor_map_heads(&q, P.q, P.D, P.Nq, P.Hq, P.B, 2 * P.q_s[1], 2 * P.q_s[2], 2 * P.q_s[0], TILE);
     if (e == TPW_OK) e = make_tensor_map_heads(&k, P.k, P.D, P.Nk, P.Hk, P.B, 2 * P.k_s[1], 2 * P.k_s[2], 2 * P.k_s[0], TILE);
     if (e == TPW_OK) e = make_tensor_map_heads(&v, P.v, P.D, P.Nk, P.Hk, P.B, 2 * P.v_s[1], 2 * P.v_s[2], 2 * P.v_s[0], TILE);
     if (e != TPW_OK) return e;
-    const long long blocks = F.tiles * P.B * P.Hq;
+    const long long blocks = F.tiles * P.B * P.Hq * F.splits;
     TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
     constexpr auto *kern = &attention_forward_kernel<T, BLOCKS>;
     if (const int e = allow_shared_memory<kern>((int)L::ALLOC)) return e;
@@ -348,9 +374,24 @@ bool attn_tc_fits(int dtype, const AttnParams &P) {
     return fits(P.q, P.q_s) && fits(P.k, P.k_s) && fits(P.v, P.v_s) && aligned16(P.out);
 }
 
-int attn_tc_forward(int dtype, const AttnParams &P, cudaStream_t s) {
-    if (dtype == TPW_F16) return P.D <= 64 ? launch<__half, 1>(P, s) : launch<__half, 2>(P, s);
-    return P.D <= 64 ? launch<__nv_bfloat16, 1>(P, s) : launch<__nv_bfloat16, 2>(P, s);
+// Ranges of keys for calls whose query tiles are fewer than two CTAs per SM: about three CTAs per SM, so that ragged sequences even
+// out, with at least four key tiles each, below which writing and joining the parts costs more than the keys.  bfloat16 [2, 256 x 16384, 32/8,
+// 128], lengths 16384 and 1638: 64 CTAs 260 us.
+AttnSplits attn_tc_splits(const AttnParams &P) {
+    AttnSplits r;
+    const long long blocks = (P.Nq + 2 * TILE - 1) / (2 * TILE) * P.B * P.Hq, sms = sm_count(), key_tiles = (P.Nk + TILE - 1) / TILE;
+    if (blocks >= 2 * sms || key_tiles < 8) return r;
+    long long want = (3 * sms + blocks / 2) / blocks;
+    if (want > key_tiles / 4) want = key_tiles / 4;
+    const long long per = (key_tiles + want - 1) / want;
+    r.keys = (int)(per * TILE);
+    r.count = (int)((key_tiles + per - 1) / per);
+    return r;
+}
+
+int attn_tc_forward(int dtype, const AttnParams &P, const AttnSplits &splits, cudaStream_t s) {
+    if (dtype == TPW_F16) return P.D <= 64 ? launch<__half, 1>(P, splits, s) : launch<__half, 2>(P, splits, s);
+    return P.D <= 64 ? launch<__nv_bfloat16, 1>(P, splits, s) : launch<__nv_bfloat16, 2>(P, splits, s);
 }
 
 } // namespace tpw
