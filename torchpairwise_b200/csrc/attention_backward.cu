@@ -22,7 +22,8 @@ namespace {
 struct BackwardParams {
     AttnParams a;
     float scale_log2, scale;
-    int tiles;
+    int q_tiles;
+    unsigned key_blocks;   // blocks of the keys walk, before those of the queries walk
 };
 
 // Half precision: probabilities are lifted by 2^12 and gradients of scores by another power of two (attention_rows.cu), both undone in
@@ -98,9 +99,8 @@ __device__ __forceinline__ void store_half(T *row, uint32_t acc, int half, float
 }
 
 template <typename T, int BLOCKS>
-__global__ void __launch_bounds__(kTcThreads, 1)
-attention_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                     const __grid_constant__ CUtensorMap map_g, const BackwardParams F) {
+__device__ __forceinline__ void keys_walk(const CUtensorMap &map_q, const CUtensorMap &map_k, const CUtensorMap &map_v, const CUtensorMap &map_g,
+                                   const BackwardParams &F, unsigned block) {
     typedef KeysSmem<BLOCKS> L;
     typedef Narrow<T> N;
     const AttnParams &P = F.a;
@@ -113,9 +113,9 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_TMEM + 4);
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const long long heads = P.B * P.Hk;
-    const int row0 = (int)(blockIdx.x / heads) * TILE;   // a causal call's first keys are seen by most queries
-    const long long bh = blockIdx.x % heads;
+    const unsigned heads = (unsigned)(P.B * P.Hk);
+    const int row0 = (int)(block / heads) * TILE;   // a causal call's first keys are seen by most queries
+    const long long bh = block % heads;
     const int hk = (int)(bh % P.Hk), b = (int)(bh / P.Hk);
     const Seen see(P, b);
     const int last = (row0 + TILE < see.length ? row0 + TILE : see.length) - 1;
@@ -339,9 +339,8 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
 }
 
 template <typename T, int BLOCKS>
-__global__ void __launch_bounds__(kTcThreads, 1)
-attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                    const __grid_constant__ CUtensorMap map_g, const BackwardParams F) {
+__device__ __forceinline__ void queries_walk(const CUtensorMap &map_q, const CUtensorMap &map_k, const CUtensorMap &map_v, const CUtensorMap &map_g,
+                                   const BackwardParams &F, unsigned block) {
     typedef QueriesSmem<BLOCKS> L;
     typedef Narrow<T> N;
     const AttnParams &P = F.a;
@@ -354,9 +353,9 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_TMEM + 4);
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const long long heads = P.B * P.Hq;
-    const int row0 = (F.tiles - 1 - (int)(blockIdx.x / heads)) * TILE;   // a causal call's longest rows first
-    const long long bh = blockIdx.x % heads;
+    const unsigned heads = (unsigned)(P.B * P.Hq);
+    const int row0 = (F.q_tiles - 1 - (int)(block / heads)) * TILE;   // a causal call's longest rows first
+    const long long bh = block % heads;
     const int h = (int)(bh % P.Hq), b = (int)(bh / P.Hq), hk = h / (int)P.group;
     const Seen see(P, b);
     const int nq = (int)P.Nq, last = (row0 + TILE < nq ? row0 + TILE : nq) - 1;
@@ -549,6 +548,16 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     }
 }
 
+// Both walks in one launch: the queries walk fills the SMs that the keys walk's last blocks leave, and a small problem is through in the time
+// of the longer one.
+template <typename T, int BLOCKS>
+__global__ void __launch_bounds__(kTcThreads, 1)
+attention_backward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                          const __grid_constant__ CUtensorMap map_g, const BackwardParams F) {
+    if (blockIdx.x < F.key_blocks) keys_walk<T, BLOCKS>(map_q, map_k, map_v, map_g, F, blockIdx.x);
+    else queries_walk<T, BLOCKS>(map_q, map_k, map_v, map_g, F, blockIdx.x - F.key_blocks);
+}
+
 template <typename T, int BLOCKS> int launch(const AttnParams &P, cudaStream_t s) {
     BackwardParams F = {};
     F.a = P;
@@ -561,26 +570,16 @@ template <typename T, int BLOCKS> int launch(const AttnParams &P, cudaStream_t s
     if (e == TPW_OK) e = make_tensor_map_heads(&v, P.v, P.D, P.Nk, P.Hk, P.B, 2 * P.v_s[1], 2 * P.v_s[2], 2 * P.v_s[0], TILE);
     if (e == TPW_OK) e = make_tensor_map_heads(&g, P.dout, P.D, P.Nq, P.Hq, P.B, 2 * P.do_s[1], 2 * P.do_s[2], 2 * P.do_s[0], TILE);
     if (e != TPW_OK) return e;
-    if (P.dk) {
-        F.tiles = (int)((P.Nk + TILE - 1) / TILE);
-        const long long blocks = F.tiles * P.B * P.Hk;
-        TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
-        constexpr auto *kern = &attention_dkv_kernel<T, BLOCKS>;
-        constexpr uint32_t smem = KeysSmem<BLOCKS>::ALLOC;
-        if (const int e = allow_shared_memory<kern>((int)smem)) return e;
-        kern<<<(unsigned)blocks, kTcThreads, smem, s>>>(q, k, v, g, F);
-        TPW_LAUNCH_OK("attention_dkv_kernel");
-    }
-    if (P.dq) {
-        F.tiles = (int)((P.Nq + TILE - 1) / TILE);
-        const long long blocks = F.tiles * P.B * P.Hq;
-        TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
-        constexpr auto *kern = &attention_dq_kernel<T, BLOCKS>;
-        constexpr uint32_t smem = QueriesSmem<BLOCKS>::ALLOC;
-        if (const int e = allow_shared_memory<kern>((int)smem)) return e;
-        kern<<<(unsigned)blocks, kTcThreads, smem, s>>>(q, k, v, g, F);
-        TPW_LAUNCH_OK("attention_dq_kernel");
-    }
+    F.q_tiles = (int)((P.Nq + TILE - 1) / TILE);
+    const long long keys = P.dk ? (P.Nk + TILE - 1) / TILE * P.B * P.Hk : 0, queries = P.dq ? F.q_tiles * P.B * P.Hq : 0;
+    TPW_CHECK_ARG(keys + queries < (1LL << 31), "attention: more than 2^31 blocks of work");
+    F.key_blocks = (unsigned)keys;
+    constexpr auto *kern = &attention_backward_kernel<T, BLOCKS>;
+    constexpr uint32_t smem = KeysSmem<BLOCKS>::ALLOC > QueriesSmem<BLOCKS>::ALLOC ? KeysSmem<BLOCKS>::ALLOC : QueriesSmem<BLOCKS>::ALLOC;
+    e = allow_shared_memory<kern>((int)smem);
+    if (e != TPW_OK) return e;
+    kern<<<(unsigned)(keys + queries), kTcThreads, smem, s>>>(q, k, v, g, F);
+    TPW_LAUNCH_OK("attention_backward_kernel");
     return TPW_OK;
 }
 

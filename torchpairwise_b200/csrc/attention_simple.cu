@@ -7,8 +7,10 @@
 // tile (dk, dv; all heads that share the key head one after the other, so their sum has a fixed order) and one over the keys per
 // query tile (dq); no atomics, the same bits each time.
 //
-// Bound by FP32 issue: 2 D lane-operations per pair forward, 7 D backward.  256 threads as 16 x 16; a thread holds a block
-// of rows and keys in registers.  All operand tiles lie row-major with 4 elements of padding, so that products that contract the
+// Bound by FP32 issue and by shared-memory reads: 2 D lane-operations per pair forward, 7 D backward; a 16-byte read takes four
+// wavefronts, whether lanes share addresses or not, so an 8 x 8 block of a thread reads 64 wavefronts per 64 clocks of FMAs, and a
+// 4 x 4 block twice as many.  16 x TX threads; up to 64 features TX = 8, whose blocks are 8 rows by 8 columns of what a product
+// writes.  All operand tiles lie row-major with 4 elements of padding, so that products that contract the
 // features read four features of a row at once (eight rows in eight bank groups) and products that contract tokens four features of
 // one token.
 #include "attention.cuh"
@@ -36,10 +38,11 @@ template <typename A> __device__ __forceinline__ A minus_infinity() { return -(A
 template <typename A> __device__ __forceinline__ A max_of(A a, A b) { return a > b ? a : b; }
 
 // Rows [row0, row0 + ROWS) of a [tokens, D] slice, widened, zero beyond `rows` and D.  `vec`: rows may be read four elements at a time.
-template <typename T, typename A, int ROWS, int DP>
+template <typename T, typename A, int ROWS, int DP, int THREADS>
 __device__ __forceinline__ void load_tile(A *dst, const T *src, long long stride, int row0, int rows, int D, bool vec) {
     constexpr int PER = DP / 4;
-    for (int c = threadIdx.x; c < ROWS * PER; c += 256) {
+#pragma unroll 4
+    for (int c = threadIdx.x; c < ROWS * PER; c += THREADS) {
         const int r = c / PER, d = (c % PER) * 4;
         Four<A> w = {};
         if (row0 + r < rows && d < D) {
@@ -59,8 +62,8 @@ __device__ __forceinline__ void load_tile(A *dst, const T *src, long long stride
     }
 }
 
-// acc[m][n] = X[ty * RM + m] . Y[tx + 16 n], contracting DP features
-template <typename A, int RM, int RN, int DP>
+// acc[m][n] = X[ty * RM + m] . Y[tx + TX n], contracting DP features
+template <typename A, int RM, int RN, int DP, int TX>
 __device__ __forceinline__ void product_nt(A (&acc)[RM][RN], const A *X, const A *Y, int ty, int tx) {
 #pragma unroll
     for (int m = 0; m < RM; ++m)
@@ -70,7 +73,7 @@ __device__ __forceinline__ void product_nt(A (&acc)[RM][RN], const A *X, const A
     for (int d = 0; d < DP; d += 4) {
         Four<A> y[RN];
 #pragma unroll
-        for (int n = 0; n < RN; ++n) y[n] = *reinterpret_cast<const Four<A> *>(Y + (tx + 16 * n) * (DP + PAD) + d);
+        for (int n = 0; n < RN; ++n) y[n] = *reinterpret_cast<const Four<A> *>(Y + (tx + TX * n) * (DP + PAD) + d);
 #pragma unroll
         for (int m = 0; m < RM; ++m) {
             const Four<A> x = *reinterpret_cast<const Four<A> *>(X + (ty * RM + m) * (DP + PAD) + d);
@@ -82,9 +85,9 @@ __device__ __forceinline__ void product_nt(A (&acc)[RM][RN], const A *X, const A
     }
 }
 
-// acc[m][4 c + e] += sum_j P[ty * RM + m][j] Y[j][64 c + 4 tx + e], contracting COLS tokens
-template <typename A, int RM, int COLS, int DP>
-__device__ __forceinline__ void product_nn(A (&acc)[RM][DP / 16], const A *P, const A *Y, int ty, int tx) {
+// acc[m][4 c + e] += sum_j P[ty * RM + m][j] Y[j][4 TX c + 4 tx + e], contracting COLS tokens
+template <typename A, int RM, int COLS, int DP, int TX>
+__device__ __forceinline__ void product_nn(A (&acc)[RM][DP / TX], const A *P, const A *Y, int ty, int tx) {
 #pragma unroll 1
     for (int j = 0; j < COLS; j += 4) {
         Four<A> p[RM];
@@ -93,8 +96,8 @@ __device__ __forceinline__ void product_nn(A (&acc)[RM][DP / 16], const A *P, co
 #pragma unroll
         for (int jj = 0; jj < 4; ++jj)
 #pragma unroll
-            for (int c = 0; c < DP / 64; ++c) {
-                const Four<A> y = *reinterpret_cast<const Four<A> *>(Y + (j + jj) * (DP + PAD) + 64 * c + 4 * tx);
+            for (int c = 0; c < DP / (4 * TX); ++c) {
+                const Four<A> y = *reinterpret_cast<const Four<A> *>(Y + (j + jj) * (DP + PAD) + 4 * TX * c + 4 * tx);
 #pragma unroll
                 for (int m = 0; m < RM; ++m)
 #pragma unroll
@@ -103,18 +106,18 @@ __device__ __forceinline__ void product_nn(A (&acc)[RM][DP / 16], const A *P, co
     }
 }
 
-template <typename T, typename A, int RM, int DP>
-__device__ __forceinline__ void store_rows(T *dst, long long row_stride, const A (&acc)[RM][DP / 16], const A (&factor)[RM], int row0, int rows, int D,
+template <typename T, typename A, int RM, int DP, int TX>
+__device__ __forceinline__ void store_rows(T *dst, long long row_stride, const A (&acc)[RM][DP / TX], const A (&factor)[RM], int row0, int rows, int D,
                                            int ty, int tx) {
 #pragma unroll
     for (int m = 0; m < RM; ++m) {
         const int r = row0 + ty * RM + m;
         if (r >= rows) continue;
 #pragma unroll
-        for (int c = 0; c < DP / 64; ++c)
+        for (int c = 0; c < DP / (4 * TX); ++c)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int d = 64 * c + 4 * tx + e;
+                const int d = 4 * TX * c + 4 * tx + e;
                 if (d < D) dst[(long long)r * row_stride + d] = (T)(acc[m][4 * c + e] * factor[m]);
             }
     }
@@ -124,12 +127,12 @@ template <typename T> __device__ __forceinline__ bool in_fours(const void *p, co
     return (reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T))) == 0 && s[0] % 4 == 0 && s[1] % 4 == 0 && s[2] % 4 == 0 && D % 4 == 0;
 }
 
-template <typename T, typename A, int DP, int BM, int BN>
-__global__ void __launch_bounds__(256) attention_forward_simple_kernel(const AttnParams P, int tiles) {
-    constexpr int RM = BM / 16, RN = BN / 16;
+template <typename T, typename A, int DP, int BM, int BN, int TX>
+__global__ void __launch_bounds__(16 * TX) attention_forward_simple_kernel(const AttnParams P, int tiles) {
+    constexpr int RM = BM / 16, RN = BN / TX, THREADS = 16 * TX;
     extern __shared__ __align__(32) unsigned char smem[];
     A *Q = reinterpret_cast<A *>(smem), *K = Q + BM * (DP + PAD), *V = K + BN * (DP + PAD), *S = V + BN * (DP + PAD);
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
     long long at = blockIdx.x;
     const int tile = (int)(P.causal ? tiles - 1 - at % tiles : at % tiles);   // the longest rows of a causal call first
     at /= tiles;
@@ -140,11 +143,11 @@ __global__ void __launch_bounds__(256) attention_forward_simple_kernel(const Att
     const T *k = static_cast<const T *>(P.k) + b * P.k_s[0] + hk * P.k_s[2];
     const T *v = static_cast<const T *>(P.v) + b * P.v_s[0] + hk * P.v_s[2];
     const bool kvec = in_fours<T>(P.k, P.k_s, P.D), vvec = in_fours<T>(P.v, P.v_s, P.D);
-    load_tile<T, A, BM, DP>(Q, q, P.q_s[1], row0, nq, D, in_fours<T>(P.q, P.q_s, P.D));
+    load_tile<T, A, BM, DP, THREADS>(Q, q, P.q_s[1], row0, nq, D, in_fours<T>(P.q, P.q_s, P.D));
     const A scale = scale_of<A>(P);
     const int last = row0 + BM < nq ? row0 + BM - 1 : nq - 1;
     const int j_lo = see.lo(row0) / BN * BN, j_hi = see.hi(last);
-    A m[RM], l[RM], O[RM][DP / 16];
+    A m[RM], l[RM], O[RM][DP / TX];
     int lo[RM], hi[RM];
 #pragma unroll
     for (int r = 0; r < RM; ++r) {
@@ -154,26 +157,26 @@ __global__ void __launch_bounds__(256) attention_forward_simple_kernel(const Att
         lo[r] = see.lo(i);
         hi[r] = i < nq ? see.hi(i) : 0;
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c) O[r][c] = 0;
+        for (int c = 0; c < DP / TX; ++c) O[r][c] = 0;
     }
     for (int j0 = j_lo; j0 < j_hi; j0 += BN) {
         __syncthreads();
-        load_tile<T, A, BN, DP>(K, k, P.k_s[1], j0, see.length, D, kvec);
-        load_tile<T, A, BN, DP>(V, v, P.v_s[1], j0, see.length, D, vvec);
+        load_tile<T, A, BN, DP, THREADS>(K, k, P.k_s[1], j0, see.length, D, kvec);
+        load_tile<T, A, BN, DP, THREADS>(V, v, P.v_s[1], j0, see.length, D, vvec);
         __syncthreads();
         A s[RM][RN];
-        product_nt<A, RM, RN, DP>(s, Q, K, ty, tx);
+        product_nt<A, RM, RN, DP, TX>(s, Q, K, ty, tx);
 #pragma unroll
         for (int r = 0; r < RM; ++r) {
             A top = minus_infinity<A>();
 #pragma unroll
             for (int n = 0; n < RN; ++n) {
-                const int j = j0 + tx + 16 * n;
+                const int j = j0 + tx + TX * n;
                 s[r][n] = j >= lo[r] && j < hi[r] ? s[r][n] * scale : minus_infinity<A>();
                 top = max_of(top, s[r][n]);
             }
 #pragma unroll
-            for (int d = 8; d >= 1; d >>= 1) top = max_of(top, __shfl_xor_sync(0xffffffffu, top, d));
+            for (int d = TX / 2; d >= 1; d >>= 1) top = max_of(top, __shfl_xor_sync(0xffffffffu, top, d));
             const A m_new = max_of(m[r], top);
             const A base = m_new == minus_infinity<A>() ? (A)0 : m_new;   // nothing seen so far: every power below is 0
             const A rescale = power(m[r] - base);
@@ -182,38 +185,38 @@ __global__ void __launch_bounds__(256) attention_forward_simple_kernel(const Att
             for (int n = 0; n < RN; ++n) {
                 const A p = power(s[r][n] - base);
                 sum += p;
-                S[(ty * RM + r) * (BN + PAD) + tx + 16 * n] = p;
+                S[(ty * RM + r) * (BN + PAD) + tx + TX * n] = p;
             }
             l[r] = l[r] * rescale + sum;
             m[r] = m_new;
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) O[r][c] *= rescale;
+            for (int c = 0; c < DP / TX; ++c) O[r][c] *= rescale;
         }
         __syncwarp();   // a row's probabilities are written and read by the same half warp
-        product_nn<A, RM, BN, DP>(O, S, V, ty, tx);
+        product_nn<A, RM, BN, DP, TX>(O, S, V, ty, tx);
     }
     A inv[RM];
 #pragma unroll
     for (int r = 0; r < RM; ++r) {
 #pragma unroll
-        for (int d = 8; d >= 1; d >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], d);
+        for (int d = TX / 2; d >= 1; d >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], d);
         inv[r] = l[r] == 0 ? (A)0 : 1 / l[r];
         const int i = row0 + ty * RM + r;
         if (P.lse && tx == 0 && i < nq)
             static_cast<A *>(P.lse)[(b * P.Hq + h) * P.Nq + i] = l[r] == 0 ? minus_infinity<A>() : natural(m[r]) + log_of(l[r]);
     }
     T *out = static_cast<T *>(P.out) + (b * P.Nq * P.Hq + h) * P.D;
-    store_rows<T, A, RM, DP>(out, P.Hq * P.D, O, inv, row0, nq, D, ty, tx);
+    store_rows<T, A, RM, DP, TX>(out, P.Hq * P.D, O, inv, row0, nq, D, ty, tx);
 }
 
 // dk, dv of BK keys: rows are keys, columns queries
-template <typename T, typename A, int DP, int BK, int BQ>
-__global__ void __launch_bounds__(256) attention_dkv_simple_kernel(const AttnParams P, int tiles) {
-    constexpr int RM = BK / 16, RN = BQ / 16;
+template <typename T, typename A, int DP, int BK, int BQ, int TX>
+__global__ void __launch_bounds__(16 * TX) attention_dkv_simple_kernel(const AttnParams P, int tiles) {
+    constexpr int RM = BK / 16, RN = BQ / TX, THREADS = 16 * TX;
     extern __shared__ __align__(32) unsigned char smem[];
     A *K = reinterpret_cast<A *>(smem), *V = K + BK * (DP + PAD), *Q = V + BK * (DP + PAD), *G = Q + BQ * (DP + PAD),
-      *S = G + BQ * (DP + PAD), *R = S + BK * (BQ + PAD);
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+      *S = G + BQ * (DP + PAD);
+    const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
     long long at = blockIdx.x;
     const int tile = (int)(at % tiles);
     at /= tiles;
@@ -222,11 +225,11 @@ __global__ void __launch_bounds__(256) attention_dkv_simple_kernel(const AttnPar
     const int row0 = tile * BK, nk = (int)P.Nk, nq = (int)P.Nq, D = (int)P.D;
     const T *k = static_cast<const T *>(P.k) + b * P.k_s[0] + hk * P.k_s[2];
     const T *v = static_cast<const T *>(P.v) + b * P.v_s[0] + hk * P.v_s[2];
-    load_tile<T, A, BK, DP>(K, k, P.k_s[1], row0, see.length, D, in_fours<T>(P.k, P.k_s, P.D));
-    load_tile<T, A, BK, DP>(V, v, P.v_s[1], row0, see.length, D, in_fours<T>(P.v, P.v_s, P.D));
+    load_tile<T, A, BK, DP, THREADS>(K, k, P.k_s[1], row0, see.length, D, in_fours<T>(P.k, P.k_s, P.D));
+    load_tile<T, A, BK, DP, THREADS>(V, v, P.v_s[1], row0, see.length, D, in_fours<T>(P.v, P.v_s, P.D));
     const bool qvec = in_fours<T>(P.q, P.q_s, P.D), gvec = in_fours<T>(P.dout, P.do_s, P.D);
     const A scale = scale_of<A>(P);
-    A dk[RM][DP / 16], dv[RM][DP / 16];
+    A dk[RM][DP / TX], dv[RM][DP / TX];
     int lo[RM], hi[RM];
 #pragma unroll
     for (int r = 0; r < RM; ++r) {
@@ -234,7 +237,7 @@ __global__ void __launch_bounds__(256) attention_dkv_simple_kernel(const AttnPar
         lo[r] = see.qlo(j);
         hi[r] = see.qhi(j);
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c) dk[r][c] = dv[r][c] = 0;
+        for (int c = 0; c < DP / TX; ++c) dk[r][c] = dv[r][c] = 0;
     }
     const int last = row0 + BK < see.length ? row0 + BK - 1 : see.length - 1;
     const int i_lo = see.qlo(row0) / BQ * BQ, i_hi = last < row0 ? 0 : see.qhi(last);
@@ -245,33 +248,35 @@ __global__ void __launch_bounds__(256) attention_dkv_simple_kernel(const AttnPar
         const A *delta = static_cast<const A *>(P.row_delta) + (b * P.Hq + h) * P.Nqp;
         for (int i0 = i_lo; i0 < i_hi; i0 += BQ) {
             __syncthreads();
-            load_tile<T, A, BQ, DP>(Q, q, P.q_s[1], i0, nq, D, qvec);
-            load_tile<T, A, BQ, DP>(G, g, P.do_s[1], i0, nq, D, gvec);
+            load_tile<T, A, BQ, DP, THREADS>(Q, q, P.q_s[1], i0, nq, D, qvec);
+            load_tile<T, A, BQ, DP, THREADS>(G, g, P.do_s[1], i0, nq, D, gvec);
             __syncthreads();
-            A s[RM][RN], p[RM][RN];
-            product_nt<A, RM, RN, DP>(s, K, Q, ty, tx);
+            A s[RM][RN];
+            product_nt<A, RM, RN, DP, TX>(s, K, Q, ty, tx);
 #pragma unroll
             for (int n = 0; n < RN; ++n) {
-                const int i = i0 + tx + 16 * n;
+                const int i = i0 + tx + TX * n;
                 const A row = i < nq ? lse[i] : (A)0;
 #pragma unroll
-                for (int r = 0; r < RM; ++r) {
-                    p[r][n] = i >= lo[r] && i < hi[r] ? power(s[r][n] * scale - row) : (A)0;
-                    S[(ty * RM + r) * (BQ + PAD) + tx + 16 * n] = p[r][n];
-                }
+                for (int r = 0; r < RM; ++r)
+                    S[(ty * RM + r) * (BQ + PAD) + tx + TX * n] = i >= lo[r] && i < hi[r] ? power(s[r][n] * scale - row) : (A)0;
             }
-            product_nt<A, RM, RN, DP>(s, V, G, ty, tx);
+            __syncwarp();   // a row's values are written and read by the same threads of one warp
+            product_nn<A, RM, BQ, DP, TX>(dv, S, G, ty, tx);
+            product_nt<A, RM, RN, DP, TX>(s, V, G, ty, tx);
+            __syncwarp();
 #pragma unroll
             for (int n = 0; n < RN; ++n) {
-                const int i = i0 + tx + 16 * n;
+                const int i = i0 + tx + TX * n;
                 const A mean = i < nq ? delta[i] : (A)0;
 #pragma unroll
-                for (int r = 0; r < RM; ++r)
-                    R[(ty * RM + r) * (BQ + PAD) + tx + 16 * n] = i >= lo[r] && i < hi[r] ? p[r][n] * (s[r][n] - mean) : (A)0;
+                for (int r = 0; r < RM; ++r) {   // ds in the place of p; 0 times what need not be finite
+                    A *at = &S[(ty * RM + r) * (BQ + PAD) + tx + TX * n];
+                    *at = i >= lo[r] && i < hi[r] ? *at * (s[r][n] - mean) : (A)0;
+                }
             }
             __syncwarp();
-            product_nn<A, RM, BQ, DP>(dv, S, G, ty, tx);
-            product_nn<A, RM, BQ, DP>(dk, R, Q, ty, tx);
+            product_nn<A, RM, BQ, DP, TX>(dk, S, Q, ty, tx);
         }
     }
     A one[RM], by[RM];
@@ -281,18 +286,18 @@ __global__ void __launch_bounds__(256) attention_dkv_simple_kernel(const AttnPar
         by[r] = (A)P.scale;
     }
     const long long to = (b * P.Nk * P.Hk + hk) * P.D;
-    store_rows<T, A, RM, DP>(static_cast<T *>(P.dk) + to, P.Hk * P.D, dk, by, row0, nk, D, ty, tx);
-    store_rows<T, A, RM, DP>(static_cast<T *>(P.dv) + to, P.Hk * P.D, dv, one, row0, nk, D, ty, tx);
+    store_rows<T, A, RM, DP, TX>(static_cast<T *>(P.dk) + to, P.Hk * P.D, dk, by, row0, nk, D, ty, tx);
+    store_rows<T, A, RM, DP, TX>(static_cast<T *>(P.dv) + to, P.Hk * P.D, dv, one, row0, nk, D, ty, tx);
 }
 
 // dq of BQ queries: rows are queries, columns keys
-template <typename T, typename A, int DP, int BQ, int BK>
-__global__ void __launch_bounds__(256) attention_dq_simple_kernel(const AttnParams P, int tiles) {
-    constexpr int RM = BQ / 16, RN = BK / 16;
+template <typename T, typename A, int DP, int BQ, int BK, int TX>
+__global__ void __launch_bounds__(16 * TX) attention_dq_simple_kernel(const AttnParams P, int tiles) {
+    constexpr int RM = BQ / 16, RN = BK / TX, THREADS = 16 * TX;
     extern __shared__ __align__(32) unsigned char smem[];
     A *Q = reinterpret_cast<A *>(smem), *G = Q + BQ * (DP + PAD), *K = G + BQ * (DP + PAD), *V = K + BK * (DP + PAD),
       *S = V + BK * (DP + PAD);
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
     long long at = blockIdx.x;
     const int tile = (int)(P.causal ? tiles - 1 - at % tiles : at % tiles);
     at /= tiles;
@@ -304,10 +309,10 @@ __global__ void __launch_bounds__(256) attention_dq_simple_kernel(const AttnPara
     const T *k = static_cast<const T *>(P.k) + b * P.k_s[0] + hk * P.k_s[2];
     const T *v = static_cast<const T *>(P.v) + b * P.v_s[0] + hk * P.v_s[2];
     const bool kvec = in_fours<T>(P.k, P.k_s, P.D), vvec = in_fours<T>(P.v, P.v_s, P.D);
-    load_tile<T, A, BQ, DP>(Q, q, P.q_s[1], row0, nq, D, in_fours<T>(P.q, P.q_s, P.D));
-    load_tile<T, A, BQ, DP>(G, g, P.do_s[1], row0, nq, D, in_fours<T>(P.dout, P.do_s, P.D));
+    load_tile<T, A, BQ, DP, THREADS>(Q, q, P.q_s[1], row0, nq, D, in_fours<T>(P.q, P.q_s, P.D));
+    load_tile<T, A, BQ, DP, THREADS>(G, g, P.do_s[1], row0, nq, D, in_fours<T>(P.dout, P.do_s, P.D));
     const A scale = scale_of<A>(P);
-    A dq[RM][DP / 16], row[RM], mean[RM], by[RM];
+    A dq[RM][DP / TX], row[RM], mean[RM], by[RM];
     int lo[RM], hi[RM];
 #pragma unroll
     for (int r = 0; r < RM; ++r) {
@@ -319,75 +324,80 @@ __global__ void __launch_bounds__(256) attention_dq_simple_kernel(const AttnPara
         mean[r] = i < nq ? static_cast<const A *>(P.row_delta)[from] : (A)0;
         by[r] = (A)P.scale;
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c) dq[r][c] = 0;
+        for (int c = 0; c < DP / TX; ++c) dq[r][c] = 0;
     }
     const int last = row0 + BQ < nq ? row0 + BQ - 1 : nq - 1;
     const int j_lo = see.lo(row0) / BK * BK, j_hi = see.hi(last);
     for (int j0 = j_lo; j0 < j_hi; j0 += BK) {
         __syncthreads();
-        load_tile<T, A, BK, DP>(K, k, P.k_s[1], j0, see.length, D, kvec);
-        load_tile<T, A, BK, DP>(V, v, P.v_s[1], j0, see.length, D, vvec);
+        load_tile<T, A, BK, DP, THREADS>(K, k, P.k_s[1], j0, see.length, D, kvec);
+        load_tile<T, A, BK, DP, THREADS>(V, v, P.v_s[1], j0, see.length, D, vvec);
         __syncthreads();
         A s[RM][RN], p[RM][RN];
-        product_nt<A, RM, RN, DP>(s, Q, K, ty, tx);
+        product_nt<A, RM, RN, DP, TX>(s, Q, K, ty, tx);
 #pragma unroll
         for (int r = 0; r < RM; ++r)
 #pragma unroll
             for (int n = 0; n < RN; ++n) {
-                const int j = j0 + tx + 16 * n;
+                const int j = j0 + tx + TX * n;
                 p[r][n] = j >= lo[r] && j < hi[r] ? power(s[r][n] * scale - row[r]) : (A)0;
             }
-        product_nt<A, RM, RN, DP>(s, G, V, ty, tx);
+        product_nt<A, RM, RN, DP, TX>(s, G, V, ty, tx);
 #pragma unroll
         for (int r = 0; r < RM; ++r)
 #pragma unroll
             for (int n = 0; n < RN; ++n) {
-                const int j = j0 + tx + 16 * n;
-                S[(ty * RM + r) * (BK + PAD) + tx + 16 * n] = j >= lo[r] && j < hi[r] ? p[r][n] * (s[r][n] - mean[r]) : (A)0;
+                const int j = j0 + tx + TX * n;
+                S[(ty * RM + r) * (BK + PAD) + tx + TX * n] = j >= lo[r] && j < hi[r] ? p[r][n] * (s[r][n] - mean[r]) : (A)0;
             }
         __syncwarp();
-        product_nn<A, RM, BK, DP>(dq, S, K, ty, tx);
+        product_nn<A, RM, BK, DP, TX>(dq, S, K, ty, tx);
     }
     T *out = static_cast<T *>(P.dq) + (b * P.Nq * P.Hq + h) * P.D;
-    store_rows<T, A, RM, DP>(out, P.Hq * P.D, dq, by, row0, nq, D, ty, tx);
+    store_rows<T, A, RM, DP, TX>(out, P.Hq * P.D, dq, by, row0, nq, D, ty, tx);
 }
 
 template <auto *KERNEL>
-int run(const char *name, const AttnParams &P, long long rows, int tile_rows, long long heads, size_t smem, cudaStream_t s) {
+int run(const char *name, const AttnParams &P, long long rows, int tile_rows, long long heads, int threads, size_t smem, cudaStream_t s) {
     const long long tiles = (rows + tile_rows - 1) / tile_rows, blocks = tiles * heads * P.B;
     TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
     if (blocks == 0) return TPW_OK;
     if (const int e = allow_shared_memory<KERNEL>((int)smem)) return e;
-    KERNEL<<<(unsigned)blocks, 256, smem, s>>>(P, (int)tiles);
+    KERNEL<<<(unsigned)blocks, threads, smem, s>>>(P, (int)tiles);
     TPW_LAUNCH_OK(name);
     return TPW_OK;
 }
 
-template <typename T, int DP, int BM, int BN> int forward(const AttnParams &P, cudaStream_t s) {
+template <typename T, int DP, int BM, int BN, int TX> int forward(const AttnParams &P, cudaStream_t s) {
     typedef typename AttnAcc<T>::type A;
     constexpr size_t smem = sizeof(A) * ((BM + 2 * BN) * (DP + PAD) + BM * (BN + PAD));
     static_assert(smem <= 232448, "exceeds the dynamic shared memory of one CTA");
-    return run<&attention_forward_simple_kernel<T, A, DP, BM, BN>>("attention_forward_simple_kernel", P, P.Nq, BM, P.Hq, smem, s);
+    return run<&attention_forward_simple_kernel<T, A, DP, BM, BN, TX>>("attention_forward_simple_kernel", P, P.Nq, BM, P.Hq, 16 * TX, smem, s);
 }
-template <typename T, int DP, int BK, int BQ> int backward(const AttnParams &P, cudaStream_t s) {
+// BR rows of the CTA's own, BC of the tiles it walks over
+template <typename T, int DP, int BR, int BC, int TX> int backward(const AttnParams &P, cudaStream_t s) {
     typedef typename AttnAcc<T>::type A;
-    constexpr size_t kv = sizeof(A) * (2 * (BK + BQ) * (DP + PAD) + 2 * BK * (BQ + PAD)), qs = sizeof(A) * (2 * (BK + BQ) * (DP + PAD) + BQ * (BK + PAD));
-    static_assert(kv <= 232448 && qs <= 232448, "exceeds the dynamic shared memory of one CTA");
+    constexpr size_t smem = sizeof(A) * (2 * (BR + BC) * (DP + PAD) + BR * (BC + PAD));
+    static_assert(smem <= 232448, "exceeds the dynamic shared memory of one CTA");
     if (P.dk) {
-        const int e = run<&attention_dkv_simple_kernel<T, A, DP, BK, BQ>>("attention_dkv_simple_kernel", P, P.Nk, BK, P.Hk, kv, s);
+        const int e = run<&attention_dkv_simple_kernel<T, A, DP, BR, BC, TX>>("attention_dkv_simple_kernel", P, P.Nk, BR, P.Hk, 16 * TX, smem, s);
         if (e != TPW_OK) return e;
     }
-    if (P.dq) return run<&attention_dq_simple_kernel<T, A, DP, BQ, BK>>("attention_dq_simple_kernel", P, P.Nq, BQ, P.Hq, qs, s);
+    if (P.dq) return run<&attention_dq_simple_kernel<T, A, DP, BR, BC, TX>>("attention_dq_simple_kernel", P, P.Nq, BR, P.Hq, 16 * TX, smem, s);
     return TPW_OK;
 }
 
 template <typename T> int forward_width(const AttnParams &P, cudaStream_t s) {
-    if constexpr (sizeof(T) == 8) return P.D <= 64 ? forward<T, 64, 32, 32>(P, s) : P.D <= 128 ? forward<T, 128, 32, 32>(P, s) : forward<T, 256, 32, 32>(P, s);
-    else return P.D <= 64 ? forward<T, 64, 128, 64>(P, s) : P.D <= 128 ? forward<T, 128, 128, 64>(P, s) : forward<T, 256, 64, 32>(P, s);
+    if constexpr (sizeof(T) == 8)
+        return P.D <= 64 ? forward<T, 64, 32, 32, 16>(P, s) : P.D <= 128 ? forward<T, 128, 32, 32, 16>(P, s) : forward<T, 256, 32, 32, 16>(P, s);
+    else
+        return P.D <= 64 ? forward<T, 64, 128, 64, 8>(P, s) : P.D <= 128 ? forward<T, 128, 128, 64, 16>(P, s) : forward<T, 256, 64, 32, 16>(P, s);
 }
 template <typename T> int backward_width(const AttnParams &P, cudaStream_t s) {
-    if constexpr (sizeof(T) == 8) return P.D <= 64 ? backward<T, 64, 32, 32>(P, s) : P.D <= 128 ? backward<T, 128, 32, 32>(P, s) : backward<T, 256, 16, 16>(P, s);
-    else return P.D <= 64 ? backward<T, 64, 64, 64>(P, s) : P.D <= 128 ? backward<T, 128, 64, 64>(P, s) : backward<T, 256, 32, 32>(P, s);
+    if constexpr (sizeof(T) == 8)
+        return P.D <= 64 ? backward<T, 64, 32, 32, 16>(P, s) : P.D <= 128 ? backward<T, 128, 32, 32, 16>(P, s) : backward<T, 256, 16, 16, 16>(P, s);
+    else
+        return P.D <= 64 ? backward<T, 64, 128, 32, 8>(P, s) : P.D <= 128 ? backward<T, 128, 64, 64, 16>(P, s) : backward<T, 256, 32, 32, 16>(P, s);
 }
 
 } // namespace

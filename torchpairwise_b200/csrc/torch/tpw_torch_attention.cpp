@@ -52,6 +52,13 @@ void same_kind(const char *name, const char *arg, const Tensor &t, const Tensor 
     TORCH_CHECK(t.scalar_type() == first.scalar_type(), name, ": ", arg, " has type ", t.scalar_type(), ", the first tensor ", first.scalar_type());
 }
 
+bool wants_node(std::initializer_list<const Tensor *> tensors) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor *t : tensors)
+        if (t->requires_grad()) return true;
+    return false;
+}
+
 // A view whose features lie side by side and whose strides the kernels can use as they are (views of a packed projection, transposed
 // batches); anything else is copied.  Broadcast dimensions and negative or odd strides of 16-bit rows count as anything else: the
 // tensor-core kernels fetch rows in pieces of 16 bytes.
@@ -70,11 +77,6 @@ void strides_of(const Tensor &x, int64_t (&s)[3]) {
     const int64_t dense[3] = {x.size(1) * x.size(2) * x.size(3), x.size(2) * x.size(3), x.size(3)};
     for (int d = 0; d < 3; ++d) s[d] = x.size(d) == 1 ? dense[d] : x.stride(d);
 }
-
-struct Shape {
-    bool unbatched;
-    Tensor q, k, v;   // [B, N, H, D], laid out
-};
 
 tpw_attention describe(const Tensor &q, const Tensor &k, const Tensor &v, const OptTensor &lengths, bool causal, int64_t window, double scale) {
     tpw_attention a = {};
@@ -97,33 +99,36 @@ Tensor scratch_for(int64_t bytes, const Tensor &like) {
     return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
 
+// out and lse, of the caller's rank
+variable_list attention_forward(const Tensor &q_, const Tensor &k_, const Tensor &v_, const OptTensor &lengths, bool causal, int64_t window, double scale) {
+    NvtxRange range("torchpairwise_b200::attention");
+    c10::cuda::CUDAGuard dg(q_.device());
+    const bool unbatched = q_.dim() == 3;
+    auto four = [&](const Tensor &t) { return laid_out(unbatched ? t.unsqueeze(0) : t); };
+    const Tensor q = four(q_), k = four(k_), v = four(v_);
+    tpw_attention a = describe(q, k, v, lengths, causal, window, scale);
+    Tensor out = at::empty(q.sizes(), q.options());
+    Tensor lse = at::empty({a.B, a.Hq, a.Nq}, q.options().dtype(a.dtype == TPW_F64 ? at::kDouble : at::kFloat));
+    a.out = out.mutable_data_ptr();
+    a.lse = lse.mutable_data_ptr();
+    Tensor scratch = scratch_for(tpw_attention_scratch_bytes(&a), q);
+    TPW_CALL(tpw_attention_forward(&a, scratch.defined() ? scratch.mutable_data_ptr() : nullptr, scratch.defined() ? scratch.numel() : 0, stream_of(q)));
+    if (unbatched) return {out.squeeze(0), lse.squeeze(0)};
+    return {out, lse};
+}
+
 struct AttentionFn : torch::autograd::Function<AttentionFn> {
-    static variable_list forward(AutogradContext *ctx, const Tensor &q_, const Tensor &k_, const Tensor &v_, const OptTensor &lengths, bool causal,
+    static variable_list forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const OptTensor &lengths, bool causal,
                                  int64_t window, double scale) {
         at::AutoDispatchBelowADInplaceOrView guard;
-        NvtxRange range("torchpairwise_b200::attention");
-        c10::cuda::CUDAGuard dg(q_.device());
-        const bool unbatched = q_.dim() == 3;
-        auto four = [&](const Tensor &t) { return laid_out(unbatched ? t.unsqueeze(0) : t); };
-        const Tensor q = four(q_), k = four(k_), v = four(v_);
-        tpw_attention a = describe(q, k, v, lengths, causal, window, scale);
-        Tensor out = at::empty(q.sizes(), q.options());
-        Tensor lse = at::empty({a.B, a.Hq, a.Nq}, q.options().dtype(a.dtype == TPW_F64 ? at::kDouble : at::kFloat));
-        a.out = out.mutable_data_ptr();
-        a.lse = lse.mutable_data_ptr();
-        Tensor scratch = scratch_for(tpw_attention_scratch_bytes(&a), q);
-        TPW_CALL(tpw_attention_forward(&a, scratch.defined() ? scratch.mutable_data_ptr() : nullptr, scratch.defined() ? scratch.numel() : 0, stream_of(q)));
-        if (unbatched) {
-            out = out.squeeze(0);
-            lse = lse.squeeze(0);
-        }
+        variable_list r = attention_forward(q, k, v, lengths, causal, window, scale);
         // the caller's own tensors are saved, so that a change in place before backward is an error
-        ctx->save_for_backward({q_, k_, v_, out, lse, lengths.has_value() ? *lengths : Tensor()});
+        ctx->save_for_backward({q, k, v, r[0], r[1], lengths.has_value() ? *lengths : Tensor()});
         ctx->saved_data["causal"] = causal;
         ctx->saved_data["window"] = window;
         ctx->saved_data["scale"] = scale;
         ctx->set_materialize_grads(false);
-        return {out, lse};
+        return r;
     }
     static variable_list backward(AutogradContext *ctx, variable_list go) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "attention: gradients of gradients are not provided");
@@ -193,55 +198,64 @@ std::tuple<Tensor, Tensor> attention(const Tensor &q, const Tensor &k, const Ten
         TORCH_CHECK(n.numel() == batch && n.dim() <= 1, "key_lengths must hold one length for each of the ", batch, " sequences. Got shape ", n.sizes());
         lengths = n.scalar_type() == at::kInt ? n.contiguous() : n.clamp(0, k.size(f - 2)).to(at::kInt).contiguous();
     }
+    if (!wants_node({&q, &k, &v})) {   // serving: no node, 2 us less
+        at::AutoDispatchBelowADInplaceOrView guard;
+        auto r = attention_forward(q, k, v, lengths, causal, window.value_or(0), c);
+        return {r[0], r[1]};
+    }
     auto r = AttentionFn::apply(q, k, v, lengths, causal, window.value_or(0), c);
     return {r[0], r[1]};
 }
 
 // ---- rotary positions ---------------------------------------------------------------------------------------------
+variable_list rotary_forward(const Tensor &q_, const OptTensor &k_, const Tensor &cos_, const Tensor &sin_, const OptTensor &positions, bool interleaved,
+                             bool inverse) {
+    NvtxRange range("torchpairwise_b200::rotary_embedding");
+    c10::cuda::CUDAGuard dg(q_.device());
+    const bool unbatched = q_.dim() == 3;
+    auto four = [&](const Tensor &t) {
+        Tensor x = unbatched ? t.unsqueeze(0) : t;
+        return x.is_neg() || (x.size(3) != 1 && x.stride(3) != 1) ? x.contiguous() : x;
+    };
+    const Tensor cos = cos_.contiguous(), sin = sin_.contiguous();
+    tpw_rotary a = {};
+    const Tensor x[2] = {four(q_), k_.has_value() ? four(*k_) : Tensor()};
+    variable_list out;
+    for (int w = 0; w < 2 && x[w].defined(); ++w) {
+        a.H[w] = x[w].size(2);
+        a.x[w] = x[w].const_data_ptr();
+        strides_of(x[w], a.stride[w]);
+        Tensor y = at::empty(x[w].sizes(), x[w].options());
+        a.out[w] = y.mutable_data_ptr();
+        out.push_back(unbatched ? y.squeeze(0) : y);
+    }
+    a.dtype = code_of("rotary_embedding", q_);
+    a.interleaved = interleaved;
+    a.inverse = inverse;
+    a.B = x[0].size(0); a.N = x[0].size(1); a.D = x[0].size(3);
+    a.half = cos.size(1);
+    a.length = cos.size(0);
+    a.cos = cos.const_data_ptr<float>();
+    a.sin = sin.const_data_ptr<float>();
+    if (positions.has_value()) {
+        const Tensor &p = *positions;
+        a.positions = p.const_data_ptr<int64_t>();
+        a.position_stride[0] = p.dim() == 2 && p.size(0) > 1 ? p.stride(0) : 0;
+        a.position_stride[1] = p.dim() >= 1 && p.size(-1) > 1 ? p.stride(-1) : 0;
+    }
+    TPW_CALL(tpw_rotary_apply(&a, stream_of(q_)));
+    return out;
+}
+
 struct RotaryFn : torch::autograd::Function<RotaryFn> {
-    static variable_list forward(AutogradContext *ctx, const Tensor &q_, const OptTensor &k_, const Tensor &cos_, const Tensor &sin_, const OptTensor &positions,
+    static variable_list forward(AutogradContext *ctx, const Tensor &q, const OptTensor &k, const Tensor &cos, const Tensor &sin, const OptTensor &positions,
                                  bool interleaved, bool inverse) {
         at::AutoDispatchBelowADInplaceOrView guard;
-        NvtxRange range("torchpairwise_b200::rotary_embedding");
-        c10::cuda::CUDAGuard dg(q_.device());
-        const bool unbatched = q_.dim() == 3;
-        auto four = [&](const Tensor &t) {
-            Tensor x = unbatched ? t.unsqueeze(0) : t;
-            return x.is_neg() || (x.size(3) != 1 && x.stride(3) != 1) ? x.contiguous() : x;
-        };
-        const Tensor cos = cos_.contiguous(), sin = sin_.contiguous();
-        tpw_rotary a = {};
-        const Tensor x[2] = {four(q_), k_.has_value() ? four(*k_) : Tensor()};
-        variable_list out;
-        for (int w = 0; w < 2 && x[w].defined(); ++w) {
-            a.H[w] = x[w].size(2);
-            a.x[w] = x[w].const_data_ptr();
-            strides_of(x[w], a.stride[w]);
-            for (int d = 0; d < 3; ++d)
-                if (x[w].size(d) != 1) a.stride[w][d] = x[w].stride(d);
-            Tensor y = at::empty(x[w].sizes(), x[w].options());
-            a.out[w] = y.mutable_data_ptr();
-            out.push_back(unbatched ? y.squeeze(0) : y);
-        }
-        a.dtype = code_of("rotary_embedding", q_);
-        a.interleaved = interleaved;
-        a.inverse = inverse;
-        a.B = x[0].size(0); a.N = x[0].size(1); a.D = x[0].size(3);
-        a.half = cos.size(1);
-        a.length = cos.size(0);
-        a.cos = cos.const_data_ptr<float>();
-        a.sin = sin.const_data_ptr<float>();
-        if (positions.has_value()) {
-            const Tensor &p = *positions;
-            a.positions = p.const_data_ptr<int64_t>();
-            a.position_stride[0] = p.dim() == 2 && p.size(0) > 1 ? p.stride(0) : 0;
-            a.position_stride[1] = p.dim() >= 1 && p.size(-1) > 1 ? p.stride(-1) : 0;
-        }
-        TPW_CALL(tpw_rotary_apply(&a, stream_of(q_)));
-        ctx->save_for_backward({cos_, sin_, positions.has_value() ? *positions : Tensor()});
+        variable_list out = rotary_forward(q, k, cos, sin, positions, interleaved, inverse);
+        ctx->save_for_backward({cos, sin, positions.has_value() ? *positions : Tensor()});
         ctx->saved_data["interleaved"] = interleaved;
         ctx->saved_data["inverse"] = inverse;
-        ctx->saved_data["pair"] = k_.has_value();
+        ctx->saved_data["pair"] = k.has_value();
         ctx->set_materialize_grads(false);
         return out;
     }
@@ -253,13 +267,18 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
         variable_list g(7);
         const bool first = go[0].defined() && ctx->needs_input_grad(0), second = pair && go[1].defined() && ctx->needs_input_grad(1);
         if (first) {
-            auto r = apply(go[0], second ? OptTensor(go[1]) : c10::nullopt, s[0], s[1], at_, inter, inverse);
+            auto r = turn(go[0], second ? OptTensor(go[1]) : c10::nullopt, s[0], s[1], at_, inter, inverse);
             g[0] = r[0];
             if (second) g[1] = r[1];
         } else if (second) {
-            g[1] = apply(go[1], c10::nullopt, s[0], s[1], at_, inter, inverse)[0];
+            g[1] = turn(go[1], c10::nullopt, s[0], s[1], at_, inter, inverse)[0];
         }
         return g;
+    }
+    static variable_list turn(const Tensor &q, const OptTensor &k, const Tensor &cos, const Tensor &sin, const OptTensor &positions, bool interleaved, bool inverse) {
+        if (wants_node({&q, k.has_value() ? &*k : &q})) return apply(q, k, cos, sin, positions, interleaved, inverse);
+        at::AutoDispatchBelowADInplaceOrView guard;
+        return rotary_forward(q, k, cos, sin, positions, interleaved, inverse);
     }
 };
 
@@ -295,7 +314,7 @@ variable_list rotary(const Tensor &q, const OptTensor &k, const Tensor &cos, con
     } else {
         TORCH_CHECK(cos.size(1) == 0 || cos.size(0) >= tokens, "rotary_embedding: ", tokens, " tokens, the tables end at ", cos.size(0));
     }
-    return RotaryFn::apply(q, k, cos, sin, at_, interleaved, false);
+    return RotaryFn::turn(q, k, cos, sin, at_, interleaved, false);
 }
 
 Tensor rotary_one(const Tensor &q, const Tensor &cos, const Tensor &sin, const OptTensor &positions, bool interleaved) {
