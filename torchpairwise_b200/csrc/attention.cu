@@ -28,7 +28,7 @@ int check(const tpw_attention *a, bool backward) {
 bool nothing(const tpw_attention &a) { return a.B == 0 || a.Nq == 0 || a.Hq == 0; }
 
 AttnSplits splits_of(int dtype, const AttnParams &P) {
-    return attn_few_fits(dtype, P) ? attn_few_splits(P) : attn_tc_fits(dtype, P) ? attn_tc_splits(P) : AttnSplits();
+    return attn_few_fits(dtype, P) ? attn_few_splits(P) : attn_tc_fits(dtype, P) ? attn_tc_splits(P) : attn_f32_fits(dtype, P) ? attn_f32_splits(P) : AttnSplits();
 }
 long long split_bytes(const AttnParams &P, const AttnSplits &splits) {
     return splits.count > 1 ? 4 * splits.count * P.B * P.Hq * P.Nq * (P.D + 1) : 0;
@@ -53,14 +53,15 @@ int tpw_attention_forward(const tpw_attention *a, void *scratch, int64_t scratch
     if (e != TPW_OK || tpw::nothing(*a)) return e;
     const tpw::AttnParams P = tpw::attn_params(*a);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (tpw::attn_tc_fits(a->dtype, P)) {
+    const bool f32 = tpw::attn_f32_fits(a->dtype, P);
+    if (f32 || tpw::attn_tc_fits(a->dtype, P)) {
         tpw::AttnSplits splits = tpw::splits_of(a->dtype, P);
         const int64_t bytes = tpw::split_bytes(P, splits);
         TPW_CHECK_ARG(bytes == 0 || (scratch && tpw::aligned16(scratch) && scratch_bytes >= bytes),
                       "tpw_attention_forward: scratch of %lld bytes, 16-byte aligned, is needed", (long long)bytes);
         splits.out = static_cast<float *>(scratch);
         splits.lse = splits.out ? splits.out + splits.count * P.B * P.Hq * P.Nq * P.D : nullptr;
-        const int e = tpw::attn_few_fits(a->dtype, P) ? tpw::attn_few_forward(a->dtype, P, splits, s) : tpw::attn_tc_forward(a->dtype, P, splits, s);
+        const int e = f32 ? tpw::attn_f32_forward(P, splits, s) : tpw::attn_few_fits(a->dtype, P) ? tpw::attn_few_forward(a->dtype, P, splits, s) : tpw::attn_tc_forward(a->dtype, P, splits, s);
         return e != TPW_OK || splits.count == 1 ? e : tpw::attn_join(a->dtype, P, splits, s);
     }
     return tpw::attn_simple_forward(a->dtype, P, s);
@@ -95,6 +96,7 @@ int tpw_attention_backward(const tpw_attention *a, void *scratch, int64_t scratc
     e = tpw::attn_rows(a->dtype, P, scratch, tensor, s);
     if (e != TPW_OK) return e;
     if (tensor) return tpw::attn_tc_backward(a->dtype, P, s);
+    if (tpw::attn_f32_backward_fits(a->dtype, P)) return tpw::attn_f32_backward(P, s);
     return tpw::attn_simple_backward(a->dtype, P, s);
 }
 

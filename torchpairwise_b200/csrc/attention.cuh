@@ -73,6 +73,12 @@ struct AttnSplits {
 bool attn_tc_fits(int dtype, const AttnParams &P);
 AttnSplits attn_tc_splits(const AttnParams &P);
 int attn_tc_forward(int dtype, const AttnParams &P, const AttnSplits &splits, cudaStream_t s);
+// attention_f32.cu: float32 on the tensor cores in three tf32 products
+bool attn_f32_fits(int dtype, const AttnParams &P);
+bool attn_f32_backward_fits(int dtype, const AttnParams &P);
+AttnSplits attn_f32_splits(const AttnParams &P);
+int attn_f32_forward(const AttnParams &P, const AttnSplits &splits, cudaStream_t s);
+int attn_f32_backward(const AttnParams &P, cudaStream_t s);
 // attention_few.cu: few query rows
 bool attn_few_fits(int dtype, const AttnParams &P);
 AttnSplits attn_few_splits(const AttnParams &P);

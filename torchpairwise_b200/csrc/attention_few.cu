@@ -348,7 +348,9 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams P,
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const int d = lane * 2 + 64 * k;
-        if (d < D) *reinterpret_cast<uint32_t *>(out + d) = Narrow<T>::pack(x[k] * inv, y[k] * inv);
+        if (d >= D) continue;
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float2 *>(out + d) = make_float2(x[k] * inv, y[k] * inv);
+        else *reinterpret_cast<uint32_t *>(out + d) = Narrow<T>::pack(x[k] * inv, y[k] * inv);
     }
     if (lane == 0 && P.lse) static_cast<float *>(P.lse)[row] = sum == 0.f ? -INFINITY : top + logf(sum);
 }
@@ -408,6 +410,7 @@ int attn_join(int dtype, const AttnParams &P, const AttnSplits &splits, cudaStre
     const long long blocks = (P.B * P.Hq * P.Nq + 7) / 8;
     TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
     if (dtype == TPW_F16) attention_join_kernel<__half><<<(unsigned)blocks, 256, 0, s>>>(P, splits.out, splits.lse, splits.count);
+    else if (dtype == TPW_F32) attention_join_kernel<float><<<(unsigned)blocks, 256, 0, s>>>(P, splits.out, splits.lse, splits.count);
     else attention_join_kernel<__nv_bfloat16><<<(unsigned)blocks, 256, 0, s>>>(P, splits.out, splits.lse, splits.count);
     TPW_LAUNCH_OK("attention_join_kernel");
     return TPW_OK;

@@ -8,17 +8,57 @@
 // brings ds to the top of the range.  A maximum does not depend on the order of its atomics.
 #include "attention.cuh"
 
+#include <type_traits>
+
 namespace tpw {
 namespace {
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Piece { T v[V]; };
 
+constexpr int kTurns = 2;
+// largest |v_j|^2 of the keys that are used
+template <int V, int LANES> __device__ __forceinline__ void value_norms(const AttnParams &P, unsigned block, unsigned *row_max) {
+    constexpr int ROWS = 8 * (32 / LANES) * kTurns;
+    const unsigned tiles = (unsigned)((P.Nk + ROWS - 1) / ROWS), bh = block / tiles;
+    const int D = (int)P.D, h = (int)(bh % (unsigned)P.Hk), part = threadIdx.x % LANES;
+    const long long b = bh / (unsigned)P.Hk, j0 = (long long)(block % tiles) * ROWS + threadIdx.x / LANES;
+    const __half *v = static_cast<const __half *>(P.v) + b * P.v_s[0] + h * P.v_s[2];
+    long long length = P.key_lengths ? P.key_lengths[b] : P.Nk;
+    length = length < P.Nk ? length : P.Nk;
+    float sq[kTurns] = {};
+    for (int d = part * V; d < D; d += LANES * V) {
+        Piece<__half, V> x[kTurns] = {};
+#pragma unroll
+        for (int t = 0; t < kTurns; ++t) {
+            const long long j = j0 + t * (256 / LANES);
+            if (j < length) x[t] = *reinterpret_cast<const Piece<__half, V> *>(v + j * P.v_s[1] + d);
+        }
+#pragma unroll
+        for (int t = 0; t < kTurns; ++t)
+#pragma unroll
+            for (int e = 0; e < V; ++e) sq[t] += (float)x[t].v[e] * (float)x[t].v[e];
+    }
+    unsigned top = 0;
+#pragma unroll
+    for (int t = 0; t < kTurns; ++t) {
+#pragma unroll
+        for (int d = LANES / 2; d >= 1; d >>= 1) sq[t] += __shfl_xor_sync(0xffffffffu, sq[t], d);
+        top = max(top, __float_as_uint(fabsf(sq[t])));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0 && top) atomicMax(row_max, top);
+}
+
 // A block takes consecutive tokens of one head.  LANES threads read one row V elements at a time, a warp 32 / LANES rows side by side and
 // kTurns times in a row, so that 2 * kTurns loads are in flight.
-constexpr int kTurns = 2;
 template <typename T, int V, int LANES>
-__global__ void __launch_bounds__(256, sizeof(T) == 8 ? 4 : 6) attention_rows_kernel(const AttnParams P, double units, double lift, double sign, unsigned *row_max) {
+__global__ void __launch_bounds__(256, sizeof(T) == 8 ? 4 : 6) attention_rows_kernel(const AttnParams P, double units, double lift, double sign, unsigned row_blocks, unsigned *row_max) {
     typedef typename AttnAcc<T>::type A;
+    if constexpr (std::is_same_v<T, __half>)
+        if (blockIdx.x >= row_blocks) {
+            value_norms<V, LANES>(P, blockIdx.x - row_blocks, row_max + 1);
+            return;
+        }
     constexpr int ROWS = 8 * (32 / LANES) * kTurns;   // of a block
     const unsigned tiles = (unsigned)((P.Nqp + ROWS - 1) / ROWS), bh = blockIdx.x / tiles;
     const int D = (int)P.D, h = (int)(bh % (unsigned)P.Hq), part = threadIdx.x % LANES;
@@ -80,54 +120,13 @@ __global__ void __launch_bounds__(256, sizeof(T) == 8 ? 4 : 6) attention_rows_ke
     }
 }
 
-template <int V, int LANES>
-__global__ void __launch_bounds__(256) attention_value_norm_kernel(const AttnParams P, unsigned *row_max) {
-    constexpr int ROWS = 8 * (32 / LANES) * kTurns;
-    const unsigned tiles = (unsigned)((P.Nk + ROWS - 1) / ROWS), bh = blockIdx.x / tiles;
-    const int D = (int)P.D, h = (int)(bh % (unsigned)P.Hk), part = threadIdx.x % LANES;
-    const long long b = bh / (unsigned)P.Hk, j0 = (long long)(blockIdx.x % tiles) * ROWS + threadIdx.x / LANES;
-    const __half *v = static_cast<const __half *>(P.v) + b * P.v_s[0] + h * P.v_s[2];
-    long long length = P.key_lengths ? P.key_lengths[b] : P.Nk;
-    length = length < P.Nk ? length : P.Nk;
-    float sq[kTurns] = {};
-    for (int d = part * V; d < D; d += LANES * V) {
-        Piece<__half, V> x[kTurns] = {};
-#pragma unroll
-        for (int t = 0; t < kTurns; ++t) {
-            const long long j = j0 + t * (256 / LANES);
-            if (j < length) x[t] = *reinterpret_cast<const Piece<__half, V> *>(v + j * P.v_s[1] + d);
-        }
-#pragma unroll
-        for (int t = 0; t < kTurns; ++t)
-#pragma unroll
-            for (int e = 0; e < V; ++e) sq[t] += (float)x[t].v[e] * (float)x[t].v[e];
-    }
-    unsigned top = 0;
-#pragma unroll
-    for (int t = 0; t < kTurns; ++t) {
-#pragma unroll
-        for (int d = LANES / 2; d >= 1; d >>= 1) sq[t] += __shfl_xor_sync(0xffffffffu, sq[t], d);
-        top = max(top, __float_as_uint(fabsf(sq[t])));
-    }
-    top = __reduce_max_sync(0xffffffffu, top);
-    if ((threadIdx.x & 31) == 0 && top) atomicMax(row_max, top);
-}
-
 template <typename T, int V, int LANES>
 int launch(const AttnParams &P, double units, double lift, double sign, unsigned *row_max, cudaStream_t s) {
     constexpr int ROWS = 8 * (32 / LANES) * kTurns;
-    const long long blocks = (P.Nqp + ROWS - 1) / ROWS * P.Hq * P.B;
-    TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
-    attention_rows_kernel<T, V, LANES><<<(unsigned)blocks, 256, 0, s>>>(P, units, lift, sign, row_max);
+    const long long blocks = (P.Nqp + ROWS - 1) / ROWS * P.Hq * P.B, values = row_max ? (P.Nk + ROWS - 1) / ROWS * P.Hk * P.B : 0;
+    TPW_CHECK_ARG(blocks + values < (1LL << 31), "attention: more than 2^31 blocks of work");
+    attention_rows_kernel<T, V, LANES><<<(unsigned)(blocks + values), 256, 0, s>>>(P, units, lift, sign, (unsigned)blocks, row_max);
     TPW_LAUNCH_OK("attention_rows_kernel");
-    if constexpr (sizeof(T) == 2) {
-        const long long keys = (P.Nk + ROWS - 1) / ROWS * P.Hk * P.B;
-        if (row_max && keys > 0) {
-            TPW_CHECK_ARG(keys < (1LL << 31), "attention: more than 2^31 blocks of work");
-            attention_value_norm_kernel<V, LANES><<<(unsigned)keys, 256, 0, s>>>(P, row_max + 1);
-            TPW_LAUNCH_OK("attention_value_norm_kernel");
-        }
-    }
     return TPW_OK;
 }
 

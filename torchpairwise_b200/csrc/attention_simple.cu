@@ -1,5 +1,5 @@
-// Attention and its gradients on the CUDA cores: every type, head width up to 256 and stride.  float32 and float64 always run
-// here; 16-bit types where the tensor-core kernels' layout rules are not met.
+// Attention and its gradients on the CUDA cores: every type, head width up to 256 and stride.  float64 always runs here; the other types where
+// the tensor-core kernels' rules on layout and width are not met.
 //
 // Forward: one pass over the keys with a running maximum m and sum l of every row; a tile's probabilities exp(s - m) are
 // multiplied into the output accumulators, which are scaled by exp(m_old - m_new) whenever the maximum moves.
@@ -375,16 +375,18 @@ template <typename T, int DP, int BM, int BN, int TX> int forward(const AttnPara
     return run<&attention_forward_simple_kernel<T, A, DP, BM, BN, TX>>("attention_forward_simple_kernel", P, P.Nq, BM, P.Hq, 16 * TX, smem, s);
 }
 // BR rows of the CTA's own, BC of the tiles it walks over
-template <typename T, int DP, int BR, int BC, int TX> int backward(const AttnParams &P, cudaStream_t s) {
-    typedef typename AttnAcc<T>::type A;
-    constexpr size_t smem = sizeof(A) * (2 * (BR + BC) * (DP + PAD) + BR * (BC + PAD));
+template <typename T, int DP, int BR, int BC, int TX> constexpr size_t backward_smem() {
+    constexpr size_t smem = sizeof(typename AttnAcc<T>::type) * (2 * (BR + BC) * (DP + PAD) + BR * (BC + PAD));
     static_assert(smem <= 232448, "exceeds the dynamic shared memory of one CTA");
-    if (P.dk) {
-        const int e = run<&attention_dkv_simple_kernel<T, A, DP, BR, BC, TX>>("attention_dkv_simple_kernel", P, P.Nk, BR, P.Hk, 16 * TX, smem, s);
-        if (e != TPW_OK) return e;
-    }
-    if (P.dq) return run<&attention_dq_simple_kernel<T, A, DP, BR, BC, TX>>("attention_dq_simple_kernel", P, P.Nq, BR, P.Hq, 16 * TX, smem, s);
-    return TPW_OK;
+    return smem;
+}
+template <typename T, int DP, int BR, int BC, int TX> int dkv(const AttnParams &P, cudaStream_t s) {
+    typedef typename AttnAcc<T>::type A;
+    return run<&attention_dkv_simple_kernel<T, A, DP, BR, BC, TX>>("attention_dkv_simple_kernel", P, P.Nk, BR, P.Hk, 16 * TX, backward_smem<T, DP, BR, BC, TX>(), s);
+}
+template <typename T, int DP, int BR, int BC, int TX> int dq(const AttnParams &P, cudaStream_t s) {
+    typedef typename AttnAcc<T>::type A;
+    return run<&attention_dq_simple_kernel<T, A, DP, BR, BC, TX>>("attention_dq_simple_kernel", P, P.Nq, BR, P.Hq, 16 * TX, backward_smem<T, DP, BR, BC, TX>(), s);
 }
 
 template <typename T> int forward_width(const AttnParams &P, cudaStream_t s) {
@@ -392,6 +394,10 @@ template <typename T> int forward_width(const AttnParams &P, cudaStream_t s) {
         return P.D <= 64 ? forward<T, 64, 32, 32, 16>(P, s) : P.D <= 128 ? forward<T, 128, 32, 32, 16>(P, s) : forward<T, 256, 32, 32, 16>(P, s);
     else
         return P.D <= 64 ? forward<T, 64, 128, 64, 8>(P, s) : P.D <= 128 ? forward<T, 128, 128, 64, 16>(P, s) : forward<T, 256, 64, 32, 16>(P, s);
+}
+template <typename T, int DP, int BR, int BC, int TX> int backward(const AttnParams &P, cudaStream_t s) {
+    const int e = P.dk ? dkv<T, DP, BR, BC, TX>(P, s) : TPW_OK;
+    return e != TPW_OK || !P.dq ? e : dq<T, DP, BR, BC, TX>(P, s);
 }
 template <typename T> int backward_width(const AttnParams &P, cudaStream_t s) {
     if constexpr (sizeof(T) == 8)
