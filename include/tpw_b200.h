@@ -594,7 +594,9 @@ TPW_API int tpw_widen(int bf16, const void *src, float *dst, int64_t n, tpw_stre
  * are never used, whatever they hold.  No counterpart in the reference.
  *
  * Scores, statistics and sums are held in 32 bits (64 for TPW_F64).  With 16-bit inputs the probabilities and the
- * gradients of the scores are rounded to the inputs' type before they enter a matrix product, as its operands must be.
+ * gradients of the scores are rounded to the inputs' type before they enter a matrix product, as its operands must be.  A
+ * gradient of a score is p_ij (grad_out_i . v_j - grad_out_i . out_i); with out_rest the second term is taken from out as it was before it
+ * was rounded, without it the rounding of out adds about a tenth to the error of grad_q and grad_k.
  */
 typedef struct tpw_attention {
     int32_t dtype;            /* TPW_F32, TPW_F64, TPW_F16, TPW_BF16 */
@@ -607,6 +609,7 @@ typedef struct tpw_attention {
     const int32_t *key_lengths; /* [B] on the device, clamped to [0, Nk]; NULL: Nk everywhere */
     void *out;                /* [B, Nq, Hq, D] dense */
     void *lse;                /* [B, Hq, Nq] dense, float (double for TPW_F64); NULL in the forward: not wanted */
+    void *out_rest;           /* 16-bit types, shaped like out: what rounding took from out, for a backward to come; NULL: not wanted */
     /* backward only; q .. lse as the forward had and left them */
     const void *grad_out;     /* [B, Nq, Hq, D] */
     int64_t grad_out_stride[3];

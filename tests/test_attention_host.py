@@ -26,7 +26,7 @@ def test_table_arguments():
 class _Attention(ctypes.Structure):
     _fields_ = [("dtype", ctypes.c_int32), ("causal", ctypes.c_int32), ("window", ctypes.c_int64), *((n, ctypes.c_int64) for n in ("B", "Nq", "Nk", "Hq", "Hk", "D")),
                 ("scale", ctypes.c_double), *((n, ctypes.c_void_p) for n in ("q", "k", "v")), *((n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride")),
-                ("key_lengths", ctypes.c_void_p), ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("grad_out", ctypes.c_void_p), ("grad_out_stride", ctypes.c_int64 * 3),
+                ("key_lengths", ctypes.c_void_p), ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("out_rest", ctypes.c_void_p), ("grad_out", ctypes.c_void_p), ("grad_out_stride", ctypes.c_int64 * 3),
                 ("grad_lse", ctypes.c_void_p), *((n, ctypes.c_void_p) for n in ("grad_q", "grad_k", "grad_v"))]
 
 

@@ -13,7 +13,7 @@ struct AttnParams {
     const void *q, *k, *v, *dout;
     long long q_s[3], k_s[3], v_s[3], do_s[3];   // batch, token, head
     const int *key_lengths;
-    void *out, *lse, *dq, *dk, *dv;
+    void *out, *lse, *rest, *dq, *dk, *dv;
     const void *dlse;
     long long B, Nq, Nk, Hq, Hk, D, group;       // group = Hq / Hk
     long long window;                            // 0: none
@@ -36,7 +36,7 @@ inline AttnParams attn_params(const tpw_attention &a) {
         P.do_s[i] = a.grad_out_stride[i];
     }
     P.key_lengths = a.key_lengths;
-    P.out = a.out; P.lse = a.lse; P.dq = a.grad_q; P.dk = a.grad_k; P.dv = a.grad_v;
+    P.out = a.out; P.lse = a.lse; P.rest = a.out_rest; P.dq = a.grad_q; P.dk = a.grad_k; P.dv = a.grad_v;
     P.dlse = a.grad_lse;
     P.B = a.B; P.Nq = a.Nq; P.Nk = a.Nk; P.Hq = a.Hq; P.Hk = a.Hk; P.D = a.D;
     P.group = a.Hk > 0 ? a.Hq / a.Hk : 1;
@@ -121,6 +121,9 @@ struct Seen {
         return j < length && h > 0 ? h : 0;
     }
 };
+
+// what rounding to T took from x
+template <typename T> __device__ __forceinline__ T rest_of(float x) { return (T)(x - (float)(T)x); }
 
 template <typename T> struct AttnAcc { typedef float type; };
 template <> struct AttnAcc<double> { typedef double type; };

@@ -288,7 +288,11 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                             y += by[w] * z.y;
                         }
                     if (F.splits > 1) *reinterpret_cast<float2 *>(F.part_out + (split * all_rows + flat) * D + d) = make_float2(x * inv, y * inv);
-                    else *reinterpret_cast<uint32_t *>(static_cast<T *>(P.out) + ((b * P.Nq + i) * P.Hq + h) * P.D + d) = N::pack(x * inv, y * inv);
+                    else {
+                        const long long to = ((b * P.Nq + i) * P.Hq + h) * P.D + d;
+                        *reinterpret_cast<uint32_t *>(static_cast<T *>(P.out) + to) = N::pack(x * inv, y * inv);
+                        if (P.rest) *reinterpret_cast<uint32_t *>(static_cast<T *>(P.rest) + to) = N::rest(x * inv, y * inv);
+                    }
                 }
             }
         }
@@ -343,14 +347,19 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams P,
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     const long long bh = row / P.Nq, i = row % P.Nq, h = bh % P.Hq, b = bh / P.Hq;
-    T *out = static_cast<T *>(P.out) + ((b * P.Nq + i) * P.Hq + h) * P.D;
+    const long long to = ((b * P.Nq + i) * P.Hq + h) * P.D;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const int d = lane * 2 + 64 * k;
         if (d >= D) continue;
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<float2 *>(out + d) = make_float2(x[k] * inv, y[k] * inv);
-        else *reinterpret_cast<uint32_t *>(out + d) = Narrow<T>::pack(x[k] * inv, y[k] * inv);
+        T *out = static_cast<T *>(P.out) + to + d;
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float2 *>(out) = make_float2(x[k] * inv, y[k] * inv);
+        } else {
+            *reinterpret_cast<uint32_t *>(out) = Narrow<T>::pack(x[k] * inv, y[k] * inv);
+            if (P.rest) *reinterpret_cast<uint32_t *>(static_cast<T *>(P.rest) + to + d) = Narrow<T>::rest(x[k] * inv, y[k] * inv);
+        }
     }
     if (lane == 0 && P.lse) static_cast<float *>(P.lse)[row] = sum == 0.f ? -INFINITY : top + logf(sum);
 }

@@ -311,12 +311,18 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 }
 #pragma unroll
                 for (int e = 0; e < 32; e += 8) {
-                    uint32_t w[4];
+                    uint32_t w[4], rest[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        w[k] = empty ? 0u : N::pack(__uint_as_float(o[e + 2 * k]) * by, __uint_as_float(o[e + 2 * k + 1]) * by);
+                    for (int k = 0; k < 4; ++k) {
+                        const float a0 = empty ? 0.f : __uint_as_float(o[e + 2 * k]) * by, a1 = empty ? 0.f : __uint_as_float(o[e + 2 * k + 1]) * by;
+                        w[k] = N::pack(a0, a1);
+                        rest[k] = N::rest(a0, a1);
+                    }
                     const int d = 32 * g + e;
-                    if (i < nq && d < (int)P.D) *reinterpret_cast<uint4 *>(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
+                    if (i < nq && d < (int)P.D) {
+                        *reinterpret_cast<uint4 *>(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
+                        if (P.rest) *reinterpret_cast<uint4 *>(static_cast<T *>(P.rest) + (out - static_cast<T *>(P.out)) + d) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+                    }
                 }
             }
         }
@@ -371,7 +377,7 @@ bool attn_tc_fits(int dtype, const AttnParams &P) {
             if (st[i] % 8 != 0 || st[i] <= 0 || st[i] >= (1LL << 38)) return false;
         return aligned16(p);
     };
-    return fits(P.q, P.q_s) && fits(P.k, P.k_s) && fits(P.v, P.v_s) && aligned16(P.out);
+    return fits(P.q, P.q_s) && fits(P.k, P.k_s) && fits(P.v, P.v_s) && aligned16(P.out) && aligned16(P.rest);
 }
 
 // Ranges of keys for calls whose query tiles are fewer than two CTAs per SM: about three CTAs per SM, so that ragged sequences even

@@ -1,4 +1,4 @@
-// What both gradient walks need of each query row, formed once: delta_i = dO_i . out_i - dlse_i, and the forward's lse_i, +inf for a
+// What both gradient walks need of each query row, formed once: delta_i = dO_i . out_i - dlse_i (out with what rounding took from it), and the forward's lse_i, +inf for a
 // row that sees nothing (every probability is then exp(-inf) = 0), as powers of two for 32-bit walks.  The tensor-core walks add
 // rather than subtract: they get -delta_i and lift - lse_i.  Rows are padded to whole tiles of 128 as rows that see nothing.
 // Bound by HBM: reads dO and out once.
@@ -52,7 +52,7 @@ template <int V, int LANES> __device__ __forceinline__ void value_norms(const At
 // A block takes consecutive tokens of one head.  LANES threads read one row V elements at a time, a warp 32 / LANES rows side by side and
 // kTurns times in a row, so that 2 * kTurns loads are in flight.
 template <typename T, int V, int LANES>
-__global__ void __launch_bounds__(256, sizeof(T) == 8 ? 4 : 6) attention_rows_kernel(const AttnParams P, double units, double lift, double sign, unsigned row_blocks, unsigned *row_max) {
+__global__ void __launch_bounds__(256, 4) attention_rows_kernel(const AttnParams P, double units, double lift, double sign, unsigned row_blocks, unsigned *row_max) {
     typedef typename AttnAcc<T>::type A;
     if constexpr (std::is_same_v<T, __half>)
         if (blockIdx.x >= row_blocks) {
@@ -60,10 +60,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 8 ? 4 : 6) attention_rows_ke
             return;
         }
     constexpr int ROWS = 8 * (32 / LANES) * kTurns;   // of a block
+    constexpr bool kHalf = std::is_same_v<T, __half>;
     const unsigned tiles = (unsigned)((P.Nqp + ROWS - 1) / ROWS), bh = blockIdx.x / tiles;
     const int D = (int)P.D, h = (int)(bh % (unsigned)P.Hq), part = threadIdx.x % LANES;
     const long long b = bh / (unsigned)P.Hq, i0 = (long long)(blockIdx.x % tiles) * ROWS + threadIdx.x / LANES;
     const T *out = static_cast<const T *>(P.out) + (b * P.Nq * P.Hq + h) * P.D, *dout = static_cast<const T *>(P.dout) + b * P.do_s[0] + h * P.do_s[2];
+    const T *rest = P.rest ? static_cast<const T *>(P.rest) + (b * P.Nq * P.Hq + h) * P.D : nullptr;
     A *lse = static_cast<A *>(P.row_lse), *delta = static_cast<A *>(P.row_delta);
     A dot[kTurns] = {}, sq[kTurns] = {}, m[kTurns], more[kTurns];
 #pragma unroll
@@ -75,21 +77,22 @@ __global__ void __launch_bounds__(256, sizeof(T) == 8 ? 4 : 6) attention_rows_ke
     }
 #pragma unroll 1
     for (int d = part * V; d < D; d += LANES * V) {
-        Piece<T, V> x[kTurns] = {}, y[kTurns] = {};
+        Piece<T, V> x[kTurns] = {}, y[kTurns] = {}, z[kTurns] = {};
 #pragma unroll
         for (int t = 0; t < kTurns; ++t) {
             const long long i = i0 + t * (256 / LANES);
             if (i < P.Nq) {
                 x[t] = *reinterpret_cast<const Piece<T, V> *>(out + i * P.Hq * P.D + d);
                 y[t] = *reinterpret_cast<const Piece<T, V> *>(dout + i * P.do_s[1] + d);
+                if (sizeof(T) == 2 && rest) z[t] = *reinterpret_cast<const Piece<T, V> *>(rest + i * P.Hq * P.D + d);
             }
         }
 #pragma unroll
         for (int t = 0; t < kTurns; ++t)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                dot[t] += (A)x[t].v[e] * (A)y[t].v[e];
-                if (sizeof(T) == 2) sq[t] += (A)y[t].v[e] * (A)y[t].v[e];
+                dot[t] += (sizeof(T) == 2 ? (A)x[t].v[e] + (A)z[t].v[e] : (A)x[t].v[e]) * (A)y[t].v[e];
+                if (kHalf) sq[t] += (A)y[t].v[e] * (A)y[t].v[e];
             }
     }
     unsigned top = 0, top_more = 0;
@@ -98,7 +101,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 8 ? 4 : 6) attention_rows_ke
 #pragma unroll
         for (int d = LANES / 2; d >= 1; d >>= 1) {
             dot[t] += __shfl_xor_sync(0xffffffffu, dot[t], d);
-            if (sizeof(T) == 2) sq[t] += __shfl_xor_sync(0xffffffffu, sq[t], d);
+            if (kHalf) sq[t] += __shfl_xor_sync(0xffffffffu, sq[t], d);
         }
         const long long i = i0 + t * (256 / LANES);
         if (part != 0 || i >= P.Nqp) continue;
@@ -134,7 +137,7 @@ template <typename T> int rows(const AttnParams &P, double units, double lift, d
     constexpr int W = 16 / sizeof(T);   // elements of 16 bytes
     auto wide = [&](const void *p, const long long (&st)[3]) { return aligned16(p) && st[0] % W == 0 && st[1] % W == 0 && st[2] % W == 0; };
     const long long dense[3] = {P.D, P.D, P.D};
-    if (P.D % W != 0 || !wide(P.out, dense) || !wide(P.dout, P.do_s) || (row_max && !wide(P.v, P.v_s))) return launch<T, 1, 32>(P, units, lift, sign, row_max, s);
+    if (P.D % W != 0 || !wide(P.out, dense) || !aligned16(P.rest) || !wide(P.dout, P.do_s) || (row_max && !wide(P.v, P.v_s))) return launch<T, 1, 32>(P, units, lift, sign, row_max, s);
     const long long pieces = P.D / W;
     if (pieces <= 8) return launch<T, W, 8>(P, units, lift, sign, row_max, s);
     if (pieces <= 16) return launch<T, W, 16>(P, units, lift, sign, row_max, s);

@@ -107,7 +107,7 @@ __device__ __forceinline__ void product_nn(A (&acc)[RM][DP / TX], const A *P, co
 }
 
 template <typename T, typename A, int RM, int DP, int TX>
-__device__ __forceinline__ void store_rows(T *dst, long long row_stride, const A (&acc)[RM][DP / TX], const A (&factor)[RM], int row0, int rows, int D,
+__device__ __forceinline__ void store_rows(T *dst, T *rest, long long row_stride, const A (&acc)[RM][DP / TX], const A (&factor)[RM], int row0, int rows, int D,
                                            int ty, int tx) {
 #pragma unroll
     for (int m = 0; m < RM; ++m) {
@@ -118,7 +118,10 @@ __device__ __forceinline__ void store_rows(T *dst, long long row_stride, const A
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int d = 4 * TX * c + 4 * tx + e;
-                if (d < D) dst[(long long)r * row_stride + d] = (T)(acc[m][4 * c + e] * factor[m]);
+                if (d >= D) continue;
+                dst[(long long)r * row_stride + d] = (T)(acc[m][4 * c + e] * factor[m]);
+                if constexpr (sizeof(T) == 2)
+                    if (rest) rest[(long long)r * row_stride + d] = rest_of<T>(acc[m][4 * c + e] * factor[m]);
             }
     }
 }
@@ -205,8 +208,8 @@ __global__ void __launch_bounds__(16 * TX) attention_forward_simple_kernel(const
         if (P.lse && tx == 0 && i < nq)
             static_cast<A *>(P.lse)[(b * P.Hq + h) * P.Nq + i] = l[r] == 0 ? minus_infinity<A>() : natural(m[r]) + log_of(l[r]);
     }
-    T *out = static_cast<T *>(P.out) + (b * P.Nq * P.Hq + h) * P.D;
-    store_rows<T, A, RM, DP, TX>(out, P.Hq * P.D, O, inv, row0, nq, D, ty, tx);
+    const long long to = (b * P.Nq * P.Hq + h) * P.D;
+    store_rows<T, A, RM, DP, TX>(static_cast<T *>(P.out) + to, P.rest ? static_cast<T *>(P.rest) + to : nullptr, P.Hq * P.D, O, inv, row0, nq, D, ty, tx);
 }
 
 // dk, dv of BK keys: rows are keys, columns queries
@@ -286,8 +289,8 @@ __global__ void __launch_bounds__(16 * TX) attention_dkv_simple_kernel(const Att
         by[r] = (A)P.scale;
     }
     const long long to = (b * P.Nk * P.Hk + hk) * P.D;
-    store_rows<T, A, RM, DP, TX>(static_cast<T *>(P.dk) + to, P.Hk * P.D, dk, by, row0, nk, D, ty, tx);
-    store_rows<T, A, RM, DP, TX>(static_cast<T *>(P.dv) + to, P.Hk * P.D, dv, one, row0, nk, D, ty, tx);
+    store_rows<T, A, RM, DP, TX>(static_cast<T *>(P.dk) + to, (T *)nullptr, P.Hk * P.D, dk, by, row0, nk, D, ty, tx);
+    store_rows<T, A, RM, DP, TX>(static_cast<T *>(P.dv) + to, (T *)nullptr, P.Hk * P.D, dv, one, row0, nk, D, ty, tx);
 }
 
 // dq of BQ queries: rows are queries, columns keys
@@ -354,7 +357,7 @@ __global__ void __launch_bounds__(16 * TX) attention_dq_simple_kernel(const Attn
         product_nn<A, RM, BK, DP, TX>(dq, S, K, ty, tx);
     }
     T *out = static_cast<T *>(P.dq) + (b * P.Nq * P.Hq + h) * P.D;
-    store_rows<T, A, RM, DP, TX>(out, P.Hq * P.D, dq, by, row0, nq, D, ty, tx);
+    store_rows<T, A, RM, DP, TX>(out, (T *)nullptr, P.Hq * P.D, dq, by, row0, nq, D, ty, tx);
 }
 
 template <auto *KERNEL>

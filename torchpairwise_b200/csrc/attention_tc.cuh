@@ -25,6 +25,10 @@ template <> struct Narrow<__nv_bfloat16> {
         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
         return r;
     }
+    static __device__ __forceinline__ uint32_t rest(float lo, float hi) {   // of what pack makes of them
+        const uint32_t w = pack(lo, hi);
+        return pack(lo - __uint_as_float(w << 16), hi - __uint_as_float(w & 0xffff0000u));
+    }
 };
 template <> struct Narrow<__half> {
     static constexpr uint32_t kFormat = 0;
@@ -34,6 +38,10 @@ template <> struct Narrow<__half> {
         uint32_t r;
         asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
         return r;
+    }
+    static __device__ __forceinline__ uint32_t rest(float lo, float hi) {
+        const float2 w = __half22float2(__floats2half2_rn(lo, hi));
+        return pack(lo - w.x, hi - w.y);
     }
 };
 

@@ -99,8 +99,9 @@ Tensor scratch_for(int64_t bytes, const Tensor &like) {
     return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
 
-// out and lse, of the caller's rank
-variable_list attention_forward(const Tensor &q_, const Tensor &k_, const Tensor &v_, const OptTensor &lengths, bool causal, int64_t window, double scale) {
+// out and lse, of the caller's rank; for a backward also the rest of out where it is rounded to 16 bits
+variable_list attention_forward(const Tensor &q_, const Tensor &k_, const Tensor &v_, const OptTensor &lengths, bool causal, int64_t window, double scale,
+                                Tensor *rest) {
     NvtxRange range("torchpairwise_b200::attention");
     c10::cuda::CUDAGuard dg(q_.device());
     const bool unbatched = q_.dim() == 3;
@@ -111,6 +112,10 @@ variable_list attention_forward(const Tensor &q_, const Tensor &k_, const Tensor
     Tensor lse = at::empty({a.B, a.Hq, a.Nq}, q.options().dtype(a.dtype == TPW_F64 ? at::kDouble : at::kFloat));
     a.out = out.mutable_data_ptr();
     a.lse = lse.mutable_data_ptr();
+    if (rest && q.element_size() == 2) {
+        *rest = at::empty(q.sizes(), q.options());
+        a.out_rest = rest->mutable_data_ptr();
+    }
     Tensor scratch = scratch_for(tpw_attention_scratch_bytes(&a), q);
     TPW_CALL(tpw_attention_forward(&a, scratch.defined() ? scratch.mutable_data_ptr() : nullptr, scratch.defined() ? scratch.numel() : 0, stream_of(q)));
     if (unbatched) return {out.squeeze(0), lse.squeeze(0)};
@@ -121,9 +126,10 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
     static variable_list forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const OptTensor &lengths, bool causal,
                                  int64_t window, double scale) {
         at::AutoDispatchBelowADInplaceOrView guard;
-        variable_list r = attention_forward(q, k, v, lengths, causal, window, scale);
+        Tensor rest;
+        variable_list r = attention_forward(q, k, v, lengths, causal, window, scale, &rest);
         // the caller's own tensors are saved, so that a change in place before backward is an error
-        ctx->save_for_backward({q, k, v, r[0], r[1], lengths.has_value() ? *lengths : Tensor()});
+        ctx->save_for_backward({q, k, v, r[0], r[1], lengths.has_value() ? *lengths : Tensor(), rest});
         ctx->saved_data["causal"] = causal;
         ctx->saved_data["window"] = window;
         ctx->saved_data["scale"] = scale;
@@ -145,6 +151,7 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
                                    ctx->saved_data["window"].toInt(), ctx->saved_data["scale"].toDouble());
         a.out = out.data_ptr();
         a.lse = lse.data_ptr();
+        a.out_rest = s[6].defined() ? s[6].data_ptr() : nullptr;
         a.grad_out = g.const_data_ptr();
         strides_of(g, a.grad_out_stride);
         Tensor gl, dq, dk, dv;
@@ -200,7 +207,7 @@ std::tuple<Tensor, Tensor> attention(const Tensor &q, const Tensor &k, const Ten
     }
     if (!wants_node({&q, &k, &v})) {   // serving: no node, 2 us less
         at::AutoDispatchBelowADInplaceOrView guard;
-        auto r = attention_forward(q, k, v, lengths, causal, window.value_or(0), c);
+        auto r = attention_forward(q, k, v, lengths, causal, window.value_or(0), c, nullptr);
         return {r[0], r[1]};
     }
     auto r = AttentionFn::apply(q, k, v, lengths, causal, window.value_or(0), c);
