@@ -78,24 +78,27 @@ __device__ __forceinline__ f32x2 score_gradient(f32x2 p, f32x2 dp, f32x2 minus_d
     return mul2(p, d);
 }
 
-// rows of an accumulator to global memory, this thread's half of the columns
+// A warp's 32 rows of an accumulator to global memory, this warpgroup's half of the columns, through shared memory that is no longer in use.
+// Rows from `keep` on are zero, rows from `valid` on are not there.
 template <typename T, int BLOCKS>
-__device__ __forceinline__ void store_half(T *row, uint32_t acc, int half, float by, bool keep, bool valid, int D) {
+__device__ __forceinline__ void store_half(T *rows, long long row_stride, uint32_t acc, unsigned char *smem, int warp, int lane, int half, float by, int keep, int valid, int D) {
+    const RowStage<4 * BLOCKS> stage = {reinterpret_cast<uint4 *>(smem) + warp * 128 * BLOCKS};
+    const int first = half * 32 * BLOCKS;
 #pragma unroll 1
     for (int g = 0; g < BLOCKS; ++g) {
-        const int col = half * 32 * BLOCKS + 32 * g;
         uint32_t o[32];
-        tmem_ld32(acc + col, o);
+        tmem_ld32(acc + first + 32 * g, o);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {
+        for (int k = 0; k < 4; ++k) {
             uint32_t w[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                w[k] = keep ? Narrow<T>::pack(__uint_as_float(o[e + 2 * k]) * by, __uint_as_float(o[e + 2 * k + 1]) * by) : 0u;
-            if (valid && col + e < D) *reinterpret_cast<uint4 *>(row + col + e) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int e = 0; e < 4; ++e)
+                w[e] = lane < keep ? Narrow<T>::pack(__uint_as_float(o[8 * k + 2 * e]) * by, __uint_as_float(o[8 * k + 2 * e + 1]) * by) : 0u;
+            stage.put(lane, 4 * g + k, w[0], w[1], w[2], w[3]);
         }
     }
+    stage.store(reinterpret_cast<unsigned char *>(rows + first), row_stride * 2, lane, valid, (D - first) / 8);
 }
 
 template <typename T, int BLOCKS>
@@ -317,12 +320,11 @@ __device__ __forceinline__ void keys_walk(const CUtensorMap &map_q, const CUtens
             tc_fence_after();
         }
         if (ok) {
-            const int j = row0 + (warp & 3) * 32 + lane;
-            const bool keep = total > 0 && j < see.length, valid = j < (int)P.Nk;
-            const long long to = ((b * P.Nk + j) * P.Hk + hk) * P.D;
+            const int row = row0 + (warp & 3) * 32, keep = total > 0 ? see.length - row : 0, valid = (int)P.Nk - row;
+            const long long to = ((b * P.Nk + row) * P.Hk + hk) * P.D;
             const float down = Lift<T>::kNeeded ? 0.000244140625f : 1.f;   // 2^-12
-            store_half<T, BLOCKS>(static_cast<T *>(P.dv) + to, DV + lanes, half, down, keep, valid, (int)P.D);
-            store_half<T, BLOCKS>(static_cast<T *>(P.dk) + to, DK + lanes, half, F.scale * down / lift, keep, valid, (int)P.D);
+            store_half<T, BLOCKS>(static_cast<T *>(P.dv) + to, P.Hk * P.D, DV + lanes, smem, warp, lane, half, down, keep, valid, (int)P.D);
+            store_half<T, BLOCKS>(static_cast<T *>(P.dk) + to, P.Hk * P.D, DK + lanes, smem, warp, lane, half, F.scale * down / lift, keep, valid, (int)P.D);
         }
     }
     tc_fence_before();
@@ -531,8 +533,9 @@ __device__ __forceinline__ void queries_walk(const CUtensorMap &map_q, const CUt
         }
         if (ok) {
             const float down = Lift<T>::kNeeded ? 0.000244140625f : 1.f;   // 2^-12
-            T *row = static_cast<T *>(P.dq) + ((b * P.Nq + i) * P.Hq + h) * P.D;
-            store_half<T, BLOCKS>(row, DQ + lanes, half, F.scale * down / lift, total > 0, i < nq, (int)P.D);
+            const int row = i - lane;
+            T *rows = static_cast<T *>(P.dq) + ((b * P.Nq + row) * P.Hq + h) * P.D;
+            store_half<T, BLOCKS>(rows, P.Hq * P.D, DQ + lanes, smem, warp, lane, half, F.scale * down / lift, total > 0 ? 32 : 0, nq - row, (int)P.D);
         }
     }
     tc_fence_before();

@@ -275,8 +275,8 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             unpack2(sum, s0, s1);
             l += s0 + s1;
         }
-        if (ok && n > 0) {
-            ok = warp_wait(&o_full[s], (n - 1) & 1, 8);
+        if (ok && uses > 0) {   // the last product; without one, this tile's rows of Q, which are stored through below
+            ok = n > 0 ? warp_wait(&o_full[s], (n - 1) & 1, 8) : warp_wait(q_full, 0, 10);
             tc_fence_after();
         }
         if (ok) {
@@ -286,18 +286,14 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const long long flat = bh * P.Nq + i, all_rows = P.B * P.Hq * P.Nq;
             if (i < nq && F.splits > 1) F.part_lse[split * all_rows + flat] = lse;
             else if (i < nq && P.lse) static_cast<float *>(P.lse)[flat] = lse;
-            T *out = static_cast<T *>(P.out) + ((b * P.Nq + i) * P.Hq + h) * P.D;
-            float *part = F.part_out + (split * all_rows + flat) * P.D;
             const bool empty = n == 0 || l == 0.f;
+            if (F.splits > 1) {   // nothing seen: the joining kernel does not look at it
+                float *part = F.part_out + (split * all_rows + flat) * P.D;
 #pragma unroll 1
-            for (int g = 0; g < 2 * BLOCKS; ++g) {
-                uint32_t o[32];
-                if (n > 0) {
+                for (int g = 0; g < 2 * BLOCKS && n > 0; ++g) {
+                    uint32_t o[32];
                     tmem_ld32(o_at + 32 * g, o);
                     tmem_ld_wait();
-                }
-                if (F.splits > 1) {
-                    if (n == 0) break;   // nothing seen: the joining kernel does not look at it
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
                         float4 w;
@@ -307,22 +303,30 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         w.w = empty ? 0.f : __uint_as_float(o[e + 3]) * by;
                         if (i < nq && 32 * g + e < (int)P.D) *reinterpret_cast<float4 *>(part + 32 * g + e) = w;
                     }
-                    continue;
                 }
+            } else {   // through this warp's rows of Q, which nobody reads any more
+                const RowStage<8 * BLOCKS> stage = {reinterpret_cast<uint4 *>(smem) + warp * 256 * BLOCKS};
+                const int row = i - lane, valid = nq - row, width = (int)P.D / 8;
+                const long long to = ((b * P.Nq + row) * P.Hq + h) * P.D, row_bytes = P.Hq * P.D * 2;
+#pragma unroll 1
+                for (int what = 0; what < (P.rest ? 2 : 1); ++what) {   // the result, and what rounding took from it
+#pragma unroll 1
+                    for (int g = 0; g < 2 * BLOCKS; ++g) {
+                        uint32_t o[32];
+                        if (n > 0) {
+                            tmem_ld32(o_at + 32 * g, o);
+                            tmem_ld_wait();
+                        }
+                        uint32_t w[16];
 #pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    uint32_t w[4], rest[4];
+                        for (int k = 0; k < 16; ++k) {
+                            const float a0 = empty ? 0.f : __uint_as_float(o[2 * k]) * by, a1 = empty ? 0.f : __uint_as_float(o[2 * k + 1]) * by;
+                            w[k] = what ? N::rest(a0, a1) : N::pack(a0, a1);
+                        }
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float a0 = empty ? 0.f : __uint_as_float(o[e + 2 * k]) * by, a1 = empty ? 0.f : __uint_as_float(o[e + 2 * k + 1]) * by;
-                        w[k] = N::pack(a0, a1);
-                        rest[k] = N::rest(a0, a1);
+                        for (int k = 0; k < 4; ++k) stage.put(lane, 4 * g + k, w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
                     }
-                    const int d = 32 * g + e;
-                    if (i < nq && d < (int)P.D) {
-                        *reinterpret_cast<uint4 *>(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
-                        if (P.rest) *reinterpret_cast<uint4 *>(static_cast<T *>(P.rest) + (out - static_cast<T *>(P.out)) + d) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
-                    }
+                    stage.store(reinterpret_cast<unsigned char *>(static_cast<T *>(what ? P.rest : P.out) + to), row_bytes, lane, valid, width);
                 }
             }
         }

@@ -174,6 +174,26 @@ constexpr int kTcThreads = 384;
 __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
 __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;"); }
 
+// 32 rows of a warp on their way to global memory: a lane has a row and puts it down in pieces of 16 bytes, the warp then stores whole
+// rows.  Straight from a row per lane every store would touch 32 half sectors.
+template <int PIECES> struct RowStage {
+    uint4 *at;   // the warp's own 32 * PIECES pieces of shared memory, no longer in use
+    static __device__ __forceinline__ int place(int row, int piece) {
+        return row * PIECES + (piece ^ (PIECES >= 8 ? row & 7 : (row * PIECES / 8) & (PIECES - 1)));
+    }
+    __device__ __forceinline__ void put(int lane, int piece, uint32_t a, uint32_t b, uint32_t c, uint32_t d) const { at[place(lane, piece)] = make_uint4(a, b, c, d); }
+    // rows below `valid`, pieces below `width`; row_bytes apart
+    __device__ __forceinline__ void store(unsigned char *to, long long row_bytes, int lane, int valid, int width) const {
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) {
+            const int row = (32 * k + lane) / PIECES, piece = lane % PIECES;
+            if (row < valid && piece < width) *reinterpret_cast<uint4 *>(to + row * row_bytes + piece * 16) = at[place(row, piece)];
+        }
+        __syncwarp();
+    }
+};
+
 __device__ __forceinline__ float exp2_fast(float x) {   // 2 units of the last place; 0 below 2^-126
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
