@@ -31,10 +31,42 @@ template <int BLOCKS> struct ForwardSmem {
     static constexpr int kSlots = BLOCKS == 2 ? 4 : 6;
     static constexpr uint32_t TILE_BYTES = BLOCKS * BLOCK_BYTES;
     static constexpr uint32_t OFF_RING = 2 * TILE_BYTES;
-    static constexpr uint32_t OFF_BAR = OFF_RING + kSlots * TILE_BYTES;
-    static constexpr uint32_t OFF_TMEM = OFF_BAR + 8 * (2 * kSlots + 10);
+    static constexpr uint32_t OFF_STAGE = OFF_RING + kSlots * TILE_BYTES;   // 4 KB a warp: 32 rows of 64 features
+    static constexpr uint32_t OFF_QUEUE = OFF_STAGE + 8 * 4096;
+    static constexpr uint32_t OFF_BAR = OFF_QUEUE + 32;
+    static constexpr uint32_t OFF_TMEM = OFF_BAR + 8 * (2 * kSlots + 17);
     static constexpr uint32_t ALLOC = OFF_TMEM + 16 + 1024;
     static_assert(ALLOC <= 232448, "exceeds the dynamic shared memory of one CTA");
+};
+
+// One block of the grid: 256 queries of a head, a range of keys, and the key tiles [lo, hi) that either query tile sees
+struct ForwardBlock {
+    Seen see;
+    int split, row0, h, b, hk, lo[2], hi[2], begin, end;
+    __device__ __forceinline__ ForwardBlock(const ForwardParams &F, unsigned block, unsigned heads, unsigned item, unsigned bh)
+        : see(F.a, bh / (unsigned)F.a.Hq), split((int)(block - item * F.splits)), row0((F.tiles - 1 - (int)(item / heads)) * 2 * TILE), h((int)(bh % (unsigned)F.a.Hq)),
+          b((int)(bh / (unsigned)F.a.Hq)), hk(h / (int)F.a.group) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int first = row0 + s * TILE, last = (first + TILE < see.nq ? first + TILE : see.nq) - 1;
+            lo[s] = see.lo(first) / TILE;
+            hi[s] = first < see.nq ? (see.hi(last) + TILE - 1) / TILE : 0;
+            if (F.splits > 1) {
+                const int from = split * F.tiles_per_split, to = from + F.tiles_per_split;
+                lo[s] = lo[s] > from ? lo[s] : from;
+                hi[s] = hi[s] < to ? hi[s] : to;
+            }
+            if (hi[s] <= lo[s]) lo[s] = hi[s] = 0;
+        }
+        const bool some0 = hi[0] > 0, some1 = hi[1] > 0;
+        begin = some0 && (!some1 || lo[0] < lo[1]) ? lo[0] : lo[1];
+        end = hi[0] > hi[1] ? hi[0] : hi[1];
+    }
+    // a causal call's longest rows first, all heads of them together
+    static __device__ __forceinline__ ForwardBlock of(const ForwardParams &F, unsigned block) {
+        const unsigned heads = (unsigned)(F.a.B * F.a.Hq), item = block / F.splits;
+        return ForwardBlock(F, block, heads, item, item % heads);
+    }
 };
 
 template <typename T, int BLOCKS>
@@ -46,41 +78,20 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const AttnParams &P = F.a;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *empty = full + L::kSlots, *q_full = empty + L::kSlots,
-             *s_full = q_full + 1, *p_most = s_full + 2, *p_full = p_most + 2, *o_full = p_full + 2, *drained = o_full + 2;
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *empty = full + L::kSlots, *q_full = empty + L::kSlots, *q_empty = q_full + 1,
+             *s_full = q_empty + 1, *p_most = s_full + 2, *p_full = p_most + 2, *o_full = p_full + 2, *o_empty = o_full + 2, *drained = o_empty + 2;
+    const BlockQueue queue = {drained + 1, drained + 3, smem_u32(smem + L::OFF_QUEUE)};
     uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(smem + L::OFF_TMEM);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_TMEM + 4);
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const unsigned heads = (unsigned)(P.B * P.Hq), split = blockIdx.x % F.splits, item = blockIdx.x / F.splits;
-    // a causal call's longest rows first, all heads of them together
-    const int tile = F.tiles - 1 - (int)(item / heads);
-    const long long bh = item % heads;
-    const int h = (int)(bh % P.Hq), b = (int)(bh / P.Hq), hk = h / (int)P.group;
-    const Seen see(P, b);
-    const int nq = (int)P.Nq, row0 = tile * 2 * TILE;
-    // key tiles [t_lo, t_hi) of each query tile, and of both
-    int t_lo[2], t_hi[2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        const int first = row0 + s * TILE, last = (first + TILE < nq ? first + TILE : nq) - 1;
-        t_lo[s] = see.lo(first) / TILE;
-        t_hi[s] = first < nq ? (see.hi(last) + TILE - 1) / TILE : 0;
-        if (F.splits > 1) {
-            const int from = split * F.tiles_per_split, to = from + F.tiles_per_split;
-            t_lo[s] = t_lo[s] > from ? t_lo[s] : from;
-            t_hi[s] = t_hi[s] < to ? t_hi[s] : to;
-        }
-        if (t_hi[s] <= t_lo[s]) t_lo[s] = t_hi[s] = 0;
-    }
-    const bool some0 = t_hi[0] > 0, some1 = t_hi[1] > 0;
-    const int begin = some0 && (!some1 || t_lo[0] < t_lo[1]) ? t_lo[0] : t_lo[1], end = t_hi[0] > t_hi[1] ? t_hi[0] : t_hi[1];
-
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kSlots; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
         mbar_init(drained, 1);
-        for (int s = 0; s < 2; ++s) { mbar_init(&s_full[s], 1); mbar_init(&p_most[s], 4); mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&s_full[s], 1); mbar_init(&p_most[s], 4); mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); mbar_init(&o_empty[s], 4); }
+        queue.init(10);   // the TMA lane, the MMA warp and eight warps of rows
         *abort_flag = 0;
         mbar_init_fence();
         tma_prefetch_descriptor(&map_q);
@@ -103,232 +114,268 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         return ok;
     };
     const uint32_t ring = smem_u32(smem + L::OFF_RING), q_at = smem_u32(smem);
-    const int uses = 2 * (end - begin);   // of the ring: K and V tiles in turn
+    unsigned block = blockIdx.x;
 
     if (warp >= 8) registers_down();
     if (warp == 8) {
-        if (lane == 0 && uses > 0) {
-            uint32_t issued = 0;
-            mbar_expect_tx(q_full, 2 * L::TILE_BYTES);
-            load_tokens<BLOCKS>(q_at, &map_q, q_full, row0, h, b);
-            load_tokens<BLOCKS>(q_at + L::TILE_BYTES, &map_q, q_full, row0 + TILE, h, b);
-            for (int u = 0; u < uses; ++u) {
-                const uint32_t slot = u % L::kSlots;
-                if (u >= L::kSlots && !wait_or_abort(&empty[slot], parity_of_use(u, L::kSlots) ^ 1, abort_flag)) {
-                    give_up(1);
-                    break;
+        if (lane == 0) {
+            // uses of the ring (K and V tiles in turn) and of the query tiles by all blocks so far
+            uint32_t used = 0, q_used = 0;
+            bool ok = true;
+            auto wait = [&](uint64_t *bar, uint32_t parity, int site) {
+                ok = wait_or_abort(bar, parity, abort_flag);
+                if (!ok) give_up(site);
+                return ok;
+            };
+            for (uint32_t n = 0; ok; ++n) {
+                const ForwardBlock W = ForwardBlock::of(F, block);
+                if (W.end > W.begin) {
+                    if (q_used > 0 && !wait(q_empty, (q_used & 1) ^ 1, 1)) break;
+                    mbar_expect_tx(q_full, 2 * L::TILE_BYTES);
+                    load_tokens<BLOCKS>(q_at, &map_q, q_full, W.row0, W.h, W.b);
+                    load_tokens<BLOCKS>(q_at + L::TILE_BYTES, &map_q, q_full, W.row0 + TILE, W.h, W.b);
+                    ++q_used;
                 }
-                mbar_expect_tx(&full[slot], L::TILE_BYTES);
-                load_tokens<BLOCKS>(ring + slot * L::TILE_BYTES, u & 1 ? &map_v : &map_k, &full[slot], (begin + u / 2) * TILE, hk, b);
-                issued = u + 1;
+                for (int u = 0; u < 2 * (W.end - W.begin); ++u, ++used) {
+                    const uint32_t slot = used % L::kSlots;
+                    if (used >= L::kSlots && !wait(&empty[slot], parity_of_use(used, L::kSlots) ^ 1, 1)) break;
+                    mbar_expect_tx(&full[slot], L::TILE_BYTES);
+                    load_tokens<BLOCKS>(ring + slot * L::TILE_BYTES, u & 1 ? &map_v : &map_k, &full[slot], (W.begin + u / 2) * TILE, W.hk, W.b);
+                }
+                auto waits = [&](uint64_t *bar, uint32_t parity) { return wait(bar, parity, 11); };
+                if (!ok || !queue.ask(n, waits) || !queue.next<false>(n, block, true, waits)) break;
             }
             // the commits that release the last uses have arrived before the CTA ends
-            for (uint32_t u = first_of_last_uses(issued, L::kSlots); u < issued; ++u)
-                if (!wait_or_abort(&empty[u % L::kSlots], parity_of_use(u, L::kSlots), abort_flag)) {
-                    give_up(2);
-                    break;
-                }
+            if (ok && (!wait_for_releases(empty, used, L::kSlots, abort_flag) || (q_used > 0 && !wait_or_abort(q_empty, (q_used & 1) ^ 1, abort_flag)))) give_up(2);
             if (*abort_flag) {   // what was issued arrives before the CTA ends
-                mbar_wait_bounded(q_full, 0);
-                for (uint32_t u = first_of_last_uses(issued, L::kSlots); u < issued; ++u) mbar_wait_bounded(&full[u % L::kSlots], parity_of_use(u, L::kSlots));
+                if (q_used > 0) mbar_wait_bounded(q_full, (q_used & 1) ^ 1);
+                for (uint32_t u = first_of_last_uses(used, L::kSlots); u < used; ++u) mbar_wait_bounded(&full[u % L::kSlots], parity_of_use(u, L::kSlots));
             }
         }
     } else if (warp == 9) {
         const int steps = (int)(P.D + 15) / 16;
         const uint32_t idesc_s = instruction(N::kFormat, TILE, false), idesc_o = instruction(N::kFormat, 16 * steps, true);
         const uint32_t leader = elect_lane();
-        int done[2] = {0, 0};
-        bool ok = uses == 0 || warp_wait(q_full, 0, 3);
-        auto arrived = [&](int u) {
+        uint32_t used = 0, q_used = 0, done[2] = {0, 0}, finished[2] = {0, 0};   // products and blocks of either tile
+        bool ok = true;
+        auto arrived = [&](uint32_t u) {
             if (!warp_wait(&full[u % L::kSlots], parity_of_use(u, L::kSlots), 4)) return false;
             tc_fence_after();
             return true;
         };
-        auto scores = [&](int s, int u) {
+        auto scores = [&](int s, uint32_t u) {
             product_features<BLOCKS>(leader, tmem + s * TILE, q_at + s * L::TILE_BYTES, ring + (u % L::kSlots) * L::TILE_BYTES, idesc_s, steps);
             commit_by(leader, &s_full[s]);
         };
-        auto release = [&](int u) {
-            commit_by(leader, &empty[u % L::kSlots]);
-        };
-        if (ok && uses > 0 && (ok = arrived(0))) {
-            for (int s = 0; s < 2; ++s)
-                if (t_lo[s] <= begin && begin < t_hi[s]) scores(s, 0);
-            release(0);
-        }
-        for (int t = begin; t < end && ok; ++t) {
-            const int u = 2 * (t - begin) + 1;   // of V; the next K is u + 1
-            if (!(ok = arrived(u))) break;
-            const int beyond = see.length - t * TILE;
-            if (beyond < TILE && (int)P.Nk > see.length) clear_tokens<BLOCKS>(smem + L::OFF_RING + (u % L::kSlots) * L::TILE_BYTES, beyond, lane);
-            if (t + 1 < end && !(ok = arrived(u + 1))) break;
-            for (int s = 0; s < 2 && ok; ++s) {
-                if (t_lo[s] <= t && t < t_hi[s]) {
-                    const uint32_t v_at = ring + (u % L::kSlots) * L::TILE_BYTES;
-                    if (!(ok = warp_wait(&p_most[s], done[s] & 1, 5))) break;
-                    tc_fence_after();
-                    product_tokens<0, 6>(leader, tmem + (2 + s) * TILE, tmem + s * TILE, 32, v_at, idesc_o, done[s] > 0);
-                    if (!(ok = warp_wait(&p_full[s], done[s] & 1, 9))) break;
-                    tc_fence_after();
-                    product_tokens<6, 8>(leader, tmem + (2 + s) * TILE, tmem + s * TILE, 32, v_at, idesc_o, true);
-                    commit_by(leader, &o_full[s]);
-                    ++done[s];
-                }
-                if (t_lo[s] <= t + 1 && t + 1 < t_hi[s]) scores(s, u + 1);
+        auto release = [&](uint32_t u) { commit_by(leader, &empty[u % L::kSlots]); };
+        for (uint32_t n = 0; ok; ++n) {
+            const ForwardBlock W = ForwardBlock::of(F, block);
+            if (W.end > W.begin) {
+                if (!(ok = warp_wait(q_full, q_used & 1, 3))) break;
+                ++q_used;
+                if (!(ok = arrived(used))) break;
+                for (int s = 0; s < 2; ++s)
+                    if (W.lo[s] <= W.begin && W.begin < W.hi[s]) scores(s, used);
+                release(used);
+                if (W.end == W.begin + 1) commit_by(leader, q_empty);
             }
-            release(u);
-            if (t + 1 < end) release(u + 1);
+            bool fresh[2] = {true, true};   // the output accumulators hold another block's sums
+            for (int t = W.begin; t < W.end && ok; ++t, used += 2) {
+                const uint32_t u = used + 1;   // of V; the next K is u + 1
+                if (!(ok = arrived(u))) break;
+                const int beyond = W.see.length - t * TILE;
+                if (beyond < TILE && (int)P.Nk > W.see.length) clear_tokens<BLOCKS>(smem + L::OFF_RING + (u % L::kSlots) * L::TILE_BYTES, beyond, lane);
+                if (t + 1 < W.end && !(ok = arrived(u + 1))) break;
+                for (int s = 0; s < 2 && ok; ++s) {
+                    if (W.lo[s] <= t && t < W.hi[s]) {
+                        const uint32_t v_at = ring + (u % L::kSlots) * L::TILE_BYTES;
+                        if (fresh[s] && finished[s] > 0 && !(ok = warp_wait(&o_empty[s], (finished[s] & 1) ^ 1, 12))) break;
+                        if (!(ok = warp_wait(&p_most[s], done[s] & 1, 5))) break;
+                        tc_fence_after();
+                        product_tokens<0, 6>(leader, tmem + (2 + s) * TILE, tmem + s * TILE, 32, v_at, idesc_o, !fresh[s]);
+                        if (!(ok = warp_wait(&p_full[s], done[s] & 1, 9))) break;
+                        tc_fence_after();
+                        product_tokens<6, 8>(leader, tmem + (2 + s) * TILE, tmem + s * TILE, 32, v_at, idesc_o, true);
+                        commit_by(leader, &o_full[s]);
+                        fresh[s] = false;
+                        ++done[s];
+                    }
+                    if (W.lo[s] <= t + 1 && t + 1 < W.hi[s]) scores(s, u + 1);
+                }
+                if (!ok) break;
+                release(u);
+                if (t + 1 < W.end) release(u + 1);
+                if (t + 2 == W.end) commit_by(leader, q_empty);
+            }
+            for (int s = 0; s < 2; ++s)
+                if (W.hi[s] > W.lo[s]) ++finished[s];
+            if (!ok || !queue.next<true>(n, block, lane == 0, [&](uint64_t *bar, uint32_t parity) { return ok = warp_wait(bar, parity, 11); })) break;
         }
         __syncwarp();
     } else if (warp < 8) {
         // ---- a query row per thread ----
         registers_up();
-        const int s = warp >> 2, i = row0 + s * TILE + (warp & 3) * 32 + lane;
+        const int s = warp >> 2;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + s * TILE, o_at = tmem + lanes + (2 + s) * TILE;
-        const int lo = see.lo(i), hi = i < nq ? see.hi(i) : 0;
-        // tiles in [from, to) are seen whole by every row of this tile
-        const int first = row0 + s * TILE, last = (first + TILE < nq ? first + TILE : nq) - 1;
-        const int all_lo = see.lo(last), all_hi = see.hi(first);
+        const RowStage<8> stage = {reinterpret_cast<uint4 *>(smem + L::OFF_STAGE) + warp * 256};
         const float c = F.scale_log2;
-        float m = -INFINITY, l = 0.f;
+        const long long all_rows = P.B * P.Hq * P.Nq;
+        uint32_t done = 0;   // scores of this tile by all blocks so far
         bool ok = true;
-        int n = 0;
-        for (int t = t_lo[s]; t < t_hi[s]; ++t, ++n) {
-            if (!(ok = warp_wait(&s_full[s], n & 1, 6))) break;
-            tc_fence_after();
-            uint32_t x[4][32];
-#pragma unroll
-            for (int g = 0; g < 4; ++g) tmem_ld32(s_at + 32 * g, x[g]);
-            tmem_ld_wait();
-            const int j0 = t * TILE;
-            if (j0 < all_lo || j0 + TILE > all_hi) {
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const int j = j0 + 32 * g + e;
-                        if (j < lo || j >= hi) x[g][e] = 0xff800000u;
-                    }
+        for (uint32_t turn = 0; ok; ++turn) {
+            int lo, hi, all_lo, all_hi, t_first, t_end;   // [lo, hi) of this row; [all_lo, all_hi) every row of the tile sees
+            {
+                const ForwardBlock W = ForwardBlock::of(F, block);
+                const int first = W.row0 + s * TILE, last = (first + TILE < W.see.nq ? first + TILE : W.see.nq) - 1, i = first + (warp & 3) * 32 + lane;
+                lo = W.see.lo(i);
+                hi = i < W.see.nq ? W.see.hi(i) : 0;
+                all_lo = W.see.lo(last);
+                all_hi = W.see.hi(first);
+                t_first = s ? W.lo[1] : W.lo[0];
+                t_end = s ? W.hi[1] : W.hi[0];
             }
-            auto highest = [&]() {   // NaN for a score that is NaN or +inf: inf - inf makes the row NaN from there on
-                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int e = 0; e < 32; e += 2)
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) tops[g] = max3_nan(tops[g], __uint_as_float(x[g][e]), __uint_as_float(x[g][e + 1]));
-                const float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
-                return top < INFINITY ? top : NAN;
-            };
-            f32x2 sum, shift2;
-            auto form = [&](int g) {   // 32 keys' probabilities
-                uint32_t p[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const f32x2 z = fma2(pack2(__uint_as_float(x[g][2 * e]), __uint_as_float(x[g][2 * e + 1])), pack2(c, c), shift2);
-                    const f32x2 y = e % 4 == 3 ? exp2_polynomial(z) : exp2_pair(z);
-                    sum = add2(sum, y);
-                    float y0, y1;
-                    unpack2(y, y0, y1);
-                    p[e] = N::pack(y0, y1);
-                }
-                tmem_st16(s_at + 16 * g, p);
-            };
-            auto hand_over = [&](uint64_t *bar) {
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar);
-            };
-            if (n == 0) m = highest();
+            float m = -INFINITY, l = 0.f;
+            int n = 0;
 #pragma unroll 1
-            for (int pass = 0;; ++pass) {
-                const float shift = m == -INFINITY ? 0.f : N::kLift - m * c;
-                shift2 = pack2(shift, shift);
-                sum = pack2(0.f, 0.f);
-#pragma unroll
-                for (int g = 0; g < 3; ++g) form(g);
-                const float top = highest();
-                const bool moves = m == -INFINITY ? top != -INFINITY : !((top - m) * c <= N::kSlack);
-                if (pass > 0 || !__any_sync(0xffffffffu, moves)) break;
-                const bool scales = moves && m != -INFINITY;   // so far only zeros were added otherwise
-                const float by = scales ? exp2_fast((m - top) * c) : 1.f;
-                l *= by;
-                if (moves) m = top;
-                if (n == 0 || !__any_sync(0xffffffffu, scales)) continue;
-                if (!(ok = warp_wait(&o_full[s], (n - 1) & 1, 7))) break;
+            for (int t = t_first; t < t_end; ++t, ++n, ++done) {
+                if (!(ok = warp_wait(&s_full[s], done & 1, 6))) break;
                 tc_fence_after();
-                for (int g = 0; g < 2 * BLOCKS; ++g) {
-                    uint32_t o[32];
-                    tmem_ld32(o_at + 32 * g, o);
-                    tmem_ld_wait();
+                uint32_t x[4][32];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * by);
-                    tmem_st32(o_at + 32 * g, o);
+                for (int g = 0; g < 4; ++g) tmem_ld32(s_at + 32 * g, x[g]);
+                tmem_ld_wait();
+                const int j0 = t * TILE;
+                if (j0 < all_lo || j0 + TILE > all_hi) {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const int j = j0 + 32 * g + e;
+                            if (j < lo || j >= hi) x[g][e] = 0xff800000u;
+                        }
                 }
+                auto highest = [&]() {   // NaN for a score that is NaN or +inf: inf - inf makes the row NaN from there on
+                    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2)
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) tops[g] = max3_nan(tops[g], __uint_as_float(x[g][e]), __uint_as_float(x[g][e + 1]));
+                    const float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
+                    return top < INFINITY ? top : NAN;
+                };
+                f32x2 sum, shift2;
+                auto form = [&](int g) {   // 32 keys' probabilities
+                    uint32_t p[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const f32x2 z = fma2(pack2(__uint_as_float(x[g][2 * e]), __uint_as_float(x[g][2 * e + 1])), pack2(c, c), shift2);
+                        const f32x2 y = e % 4 == 3 ? exp2_polynomial(z) : exp2_pair(z);
+                        sum = add2(sum, y);
+                        float y0, y1;
+                        unpack2(y, y0, y1);
+                        p[e] = N::pack(y0, y1);
+                    }
+                    tmem_st16(s_at + 16 * g, p);
+                };
+                auto hand_over = [&](uint64_t *bar) {
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar);
+                };
+                if (n == 0) m = highest();
+#pragma unroll 1
+                for (int pass = 0;; ++pass) {
+                    const float shift = m == -INFINITY ? 0.f : N::kLift - m * c;
+                    shift2 = pack2(shift, shift);
+                    sum = pack2(0.f, 0.f);
+#pragma unroll
+                    for (int g = 0; g < 3; ++g) form(g);
+                    const float top = highest();
+                    const bool moves = m == -INFINITY ? top != -INFINITY : !((top - m) * c <= N::kSlack);
+                    if (pass > 0 || !__any_sync(0xffffffffu, moves)) break;
+                    const bool scales = moves && m != -INFINITY;   // so far only zeros were added otherwise
+                    const float by = scales ? exp2_fast((m - top) * c) : 1.f;
+                    l *= by;
+                    if (moves) m = top;
+                    if (n == 0 || !__any_sync(0xffffffffu, scales)) continue;
+                    if (!(ok = warp_wait(&o_full[s], (done & 1) ^ 1, 7))) break;
+                    tc_fence_after();
+                    for (int g = 0; g < 2 * BLOCKS; ++g) {
+                        uint32_t o[32];
+                        tmem_ld32(o_at + 32 * g, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * by);
+                        tmem_st32(o_at + 32 * g, o);
+                    }
+                }
+                if (!ok) break;
+                // the first 96 keys' probabilities start the product while the last ones are formed
+                hand_over(&p_most[s]);
+                form(3);
+                hand_over(&p_full[s]);
+                float s0, s1;
+                unpack2(sum, s0, s1);
+                l += s0 + s1;
+            }
+            if (ok && n > 0) {
+                ok = warp_wait(&o_full[s], (done & 1) ^ 1, 8);
+                tc_fence_after();
             }
             if (!ok) break;
-            // the first 96 keys' probabilities start the product while the last ones are formed
-            hand_over(&p_most[s]);
-            form(3);
-            hand_over(&p_full[s]);
-            float s0, s1;
-            unpack2(sum, s0, s1);
-            l += s0 + s1;
-        }
-        if (ok && uses > 0) {   // the last product; without one, this tile's rows of Q, which are stored through below
-            ok = n > 0 ? warp_wait(&o_full[s], (n - 1) & 1, 8) : warp_wait(q_full, 0, 10);
-            tc_fence_after();
-        }
-        if (ok) {
+            const ForwardBlock W = ForwardBlock::of(F, block);
+            const int nq = W.see.nq, i = W.row0 + s * TILE + (warp & 3) * 32 + lane;
             if (m == -INFINITY) l = 0.f;   // nothing seen
             const float by = l == 0.f ? 0.f : 1.f / l;
             const float lse = l == 0.f ? -INFINITY : (m * c - N::kLift + log2f(l)) * 0.69314718055994531f;
-            const long long flat = bh * P.Nq + i, all_rows = P.B * P.Hq * P.Nq;
-            if (i < nq && F.splits > 1) F.part_lse[split * all_rows + flat] = lse;
+            const long long bh = W.b * P.Hq + W.h, flat = bh * P.Nq + i;
+            if (i < nq && F.splits > 1) F.part_lse[W.split * all_rows + flat] = lse;
             else if (i < nq && P.lse) static_cast<float *>(P.lse)[flat] = lse;
             const bool empty = n == 0 || l == 0.f;
-            if (F.splits > 1) {   // nothing seen: the joining kernel does not look at it
-                float *part = F.part_out + (split * all_rows + flat) * P.D;
+            const int row = i - lane, valid = nq - row;
+            const long long to = ((W.b * P.Nq + row) * P.Hq + W.h) * P.D, row_bytes = P.Hq * P.D * 2;
+            float *part = F.part_out + (W.split * all_rows + flat) * P.D;
 #pragma unroll 1
-                for (int g = 0; g < 2 * BLOCKS && n > 0; ++g) {
-                    uint32_t o[32];
-                    tmem_ld32(o_at + 32 * g, o);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        float4 w;
-                        w.x = empty ? 0.f : __uint_as_float(o[e]) * by;
-                        w.y = empty ? 0.f : __uint_as_float(o[e + 1]) * by;
-                        w.z = empty ? 0.f : __uint_as_float(o[e + 2]) * by;
-                        w.w = empty ? 0.f : __uint_as_float(o[e + 3]) * by;
-                        if (i < nq && 32 * g + e < (int)P.D) *reinterpret_cast<float4 *>(part + 32 * g + e) = w;
-                    }
+            for (int g = 0; g < BLOCKS; ++g) {   // 64 features at a time
+                uint32_t o[2][32];   // whatever lies there where nothing was seen
+                tmem_ld32(o_at + 64 * g, o[0]);
+                tmem_ld32(o_at + 64 * g + 32, o[1]);
+                tmem_ld_wait();
+                if (g == BLOCKS - 1 && n > 0) {   // the accumulators are read
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&o_empty[s]);
                 }
-            } else {   // through this warp's rows of Q, which nobody reads any more
-                const RowStage<8 * BLOCKS> stage = {reinterpret_cast<uint4 *>(smem) + warp * 256 * BLOCKS};
-                const int row = i - lane, valid = nq - row, width = (int)P.D / 8;
-                const long long to = ((b * P.Nq + row) * P.Hq + h) * P.D, row_bytes = P.Hq * P.D * 2;
+                if (F.splits > 1) {   // nothing seen: the joining kernel does not look at it
+#pragma unroll
+                    for (int e = 0; e < 64; e += 4) {
+                        float4 w;
+                        w.x = empty ? 0.f : __uint_as_float(o[e >> 5][e & 31]) * by;
+                        w.y = empty ? 0.f : __uint_as_float(o[e >> 5][(e & 31) + 1]) * by;
+                        w.z = empty ? 0.f : __uint_as_float(o[e >> 5][(e & 31) + 2]) * by;
+                        w.w = empty ? 0.f : __uint_as_float(o[e >> 5][(e & 31) + 3]) * by;
+                        if (n > 0 && i < nq && 64 * g + e < (int)P.D) *reinterpret_cast<float4 *>(part + 64 * g + e) = w;
+                    }
+                    continue;
+                }
 #pragma unroll 1
                 for (int what = 0; what < (P.rest ? 2 : 1); ++what) {   // the result, and what rounding took from it
-#pragma unroll 1
-                    for (int g = 0; g < 2 * BLOCKS; ++g) {
-                        uint32_t o[32];
-                        if (n > 0) {
-                            tmem_ld32(o_at + 32 * g, o);
-                            tmem_ld_wait();
-                        }
-                        uint32_t w[16];
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            const float a0 = empty ? 0.f : __uint_as_float(o[2 * k]) * by, a1 = empty ? 0.f : __uint_as_float(o[2 * k + 1]) * by;
-                            w[k] = what ? N::rest(a0, a1) : N::pack(a0, a1);
-                        }
+                    for (int k = 0; k < 8; ++k) {
+                        uint32_t w[4];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) stage.put(lane, 4 * g + k, w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t *pair = &o[k >> 2][8 * (k & 3) + 2 * e];
+                            const float a0 = empty ? 0.f : __uint_as_float(pair[0]) * by, a1 = empty ? 0.f : __uint_as_float(pair[1]) * by;
+                            w[e] = what ? N::rest(a0, a1) : N::pack(a0, a1);
+                        }
+                        stage.put(lane, k, w[0], w[1], w[2], w[3]);
                     }
-                    stage.store(reinterpret_cast<unsigned char *>(static_cast<T *>(what ? P.rest : P.out) + to), row_bytes, lane, valid, width);
+                    stage.store(reinterpret_cast<unsigned char *>(static_cast<T *>(what ? P.rest : P.out) + to + 64 * g), row_bytes, lane, valid, (int)P.D / 8 - 8 * g);
                 }
             }
+            if (!queue.next<true>(turn, block, lane == 0, [&](uint64_t *bar, uint32_t parity) { return ok = warp_wait(bar, parity, 11); })) break;
         }
     }
     tc_fence_before();

@@ -174,6 +174,58 @@ constexpr int kTcThreads = 384;
 __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
 __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;"); }
 
+// Persistent CTAs: a CTA that is done takes over a block of the grid that has not been launched yet (cluster launch control), instead of
+// ending and leaving the SM to set up the next one: launch, barriers, tensor memory and first loads are 7 us a block here.  The TMA lane
+// asks; the others learn the answer from a ring of two, and say when they have read it.
+struct BlockQueue {
+    uint64_t *answered, *read;   // [2] each
+    uint32_t response;           // shared-memory address of two times 16 bytes, 16-byte aligned
+    __device__ __forceinline__ void init(uint32_t readers) const {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&answered[i], 1);
+            mbar_init(&read[i], readers);
+        }
+    }
+    // The TMA lane, when it has issued the loads of its n-th block: asked for earlier, a block would wait behind a long one while other SMs
+    // run dry ([4, 1500 x 2111, 16, 64] with ragged lengths, asked for at a block's start: 105 us instead of 74).  False after a
+    // wait that gave up.
+    template <typename W> __device__ __forceinline__ bool ask(uint32_t n, W wait) const {
+        const uint32_t s = n & 1;
+        if (n >= 2 && !wait(&read[s], (n >> 1 & 1) ^ 1)) return false;
+        mbar_expect_tx(&answered[s], 16);
+        asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(response + 16 * s),
+                     "r"(smem_u32(&answered[s]))
+                     : "memory");
+        if (wait(&answered[s], n >> 1 & 1)) return true;
+        mbar_wait_bounded(&answered[s], n >> 1 & 1);   // it arrives before the CTA ends
+        return false;
+    }
+    __device__ __forceinline__ bool answer(uint32_t s, unsigned &block) const {
+        uint32_t got;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
+            "ld.shared.b128 r, [%2];\n\t"
+            "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t"
+            "mov.u32 %1, 0;\n\t"
+            "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, _, _, _}, r;\n\t}"
+            : "=r"(got), "=r"(block)
+            : "r"(response + 16 * s)
+            : "memory");
+        return got != 0;
+    }
+    // A reading warp (or lane): the n-th block after the first; false: there is none.  `one`: the lane that says it has read.
+    template <bool WARP, typename W> __device__ __forceinline__ bool next(uint32_t n, unsigned &block, bool one, W wait) const {
+        const uint32_t s = n & 1;
+        if (!wait(&answered[s], n >> 1 & 1)) return false;
+        const bool got = answer(s, block);
+        fence_proxy_async_smem();   // read before the next answer is written there
+        if (WARP) __syncwarp();
+        if (one) mbar_arrive(&read[s]);
+        return got;
+    }
+};
+
 // 32 rows of a warp on their way to global memory: a lane has a row and puts it down in pieces of 16 bytes, the warp then stores whole
 // rows.  Straight from a row per lane every store would touch 32 half sectors.
 template <int PIECES> struct RowStage {
