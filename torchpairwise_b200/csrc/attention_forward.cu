@@ -24,6 +24,7 @@ struct ForwardParams {
     float scale_log2;
     int tiles;                    // of 256 queries
     int splits, tiles_per_split;  // ranges of key tiles
+    Divider by_splits, by_heads, by_hq, by_group;   // splits, B * Hq, Hq, Hq / Hk
     float *part_out, *part_lse;   // splits > 1
 };
 
@@ -43,9 +44,11 @@ template <int BLOCKS> struct ForwardSmem {
 struct ForwardBlock {
     Seen see;
     int split, row0, h, b, hk, lo[2], hi[2], begin, end;
-    __device__ __forceinline__ ForwardBlock(const ForwardParams &F, unsigned block, unsigned heads, unsigned item, unsigned bh)
-        : see(F.a, bh / (unsigned)F.a.Hq), split((int)(block - item * F.splits)), row0((F.tiles - 1 - (int)(item / heads)) * 2 * TILE), h((int)(bh % (unsigned)F.a.Hq)),
-          b((int)(bh / (unsigned)F.a.Hq)), hk(h / (int)F.a.group) {
+    // a causal call's longest rows first, all heads of them together
+    __device__ __forceinline__ ForwardBlock(const ForwardParams &F, unsigned block) : ForwardBlock(F, block, block / F.by_splits) {}
+    __device__ __forceinline__ ForwardBlock(const ForwardParams &F, unsigned block, unsigned item) : ForwardBlock(F, block - item * F.splits, item / F.by_heads, item % F.by_heads) {}
+    __device__ __forceinline__ ForwardBlock(const ForwardParams &F, unsigned range, unsigned place, unsigned bh)
+        : see(F.a, bh / F.by_hq), split((int)range), row0((F.tiles - 1 - (int)place) * 2 * TILE), h((int)(bh % F.by_hq)), b((int)(bh / F.by_hq)), hk((int)((unsigned)h / F.by_group)) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const int first = row0 + s * TILE, last = (first + TILE < see.nq ? first + TILE : see.nq) - 1;
@@ -62,17 +65,13 @@ struct ForwardBlock {
         begin = some0 && (!some1 || lo[0] < lo[1]) ? lo[0] : lo[1];
         end = hi[0] > hi[1] ? hi[0] : hi[1];
     }
-    // a causal call's longest rows first, all heads of them together
-    static __device__ __forceinline__ ForwardBlock of(const ForwardParams &F, unsigned block) {
-        const unsigned heads = (unsigned)(F.a.B * F.a.Hq), item = block / F.splits;
-        return ForwardBlock(F, block, heads, item, item % heads);
-    }
 };
 
 template <typename T, int BLOCKS>
 __global__ void __launch_bounds__(kTcThreads, 1)
 attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                         const __grid_constant__ CUtensorMap map_v, const ForwardParams F) {
+                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_rest,
+                         const ForwardParams F) {
     typedef ForwardSmem<BLOCKS> L;
     typedef Narrow<T> N;
     const AttnParams &P = F.a;
@@ -128,7 +127,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 return ok;
             };
             for (uint32_t n = 0; ok; ++n) {
-                const ForwardBlock W = ForwardBlock::of(F, block);
+                const ForwardBlock W(F, block);
                 if (W.end > W.begin) {
                     if (q_used > 0 && !wait(q_empty, (q_used & 1) ^ 1, 1)) break;
                     mbar_expect_tx(q_full, 2 * L::TILE_BYTES);
@@ -169,7 +168,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         };
         auto release = [&](uint32_t u) { commit_by(leader, &empty[u % L::kSlots]); };
         for (uint32_t n = 0; ok; ++n) {
-            const ForwardBlock W = ForwardBlock::of(F, block);
+            const ForwardBlock W(F, block);
             if (W.end > W.begin) {
                 if (!(ok = warp_wait(q_full, q_used & 1, 3))) break;
                 ++q_used;
@@ -217,7 +216,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         registers_up();
         const int s = warp >> 2;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + s * TILE, o_at = tmem + lanes + (2 + s) * TILE;
-        const RowStage<8> stage = {reinterpret_cast<uint4 *>(smem + L::OFF_STAGE) + warp * 256};
+        const RowBlock rows = {smem + L::OFF_STAGE + warp * 4096};
         const float c = F.scale_log2;
         const long long all_rows = P.B * P.Hq * P.Nq;
         uint32_t done = 0;   // scores of this tile by all blocks so far
@@ -225,7 +224,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         for (uint32_t turn = 0; ok; ++turn) {
             int lo, hi, all_lo, all_hi, t_first, t_end;   // [lo, hi) of this row; [all_lo, all_hi) every row of the tile sees
             {
-                const ForwardBlock W = ForwardBlock::of(F, block);
+                const ForwardBlock W(F, block);
                 const int first = W.row0 + s * TILE, last = (first + TILE < W.see.nq ? first + TILE : W.see.nq) - 1, i = first + (warp & 3) * 32 + lane;
                 lo = W.see.lo(i);
                 hi = i < W.see.nq ? W.see.hi(i) : 0;
@@ -324,7 +323,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 tc_fence_after();
             }
             if (!ok) break;
-            const ForwardBlock W = ForwardBlock::of(F, block);
+            const ForwardBlock W(F, block);
             const int nq = W.see.nq, i = W.row0 + s * TILE + (warp & 3) * 32 + lane;
             if (m == -INFINITY) l = 0.f;   // nothing seen
             const float by = l == 0.f ? 0.f : 1.f / l;
@@ -333,8 +332,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             if (i < nq && F.splits > 1) F.part_lse[W.split * all_rows + flat] = lse;
             else if (i < nq && P.lse) static_cast<float *>(P.lse)[flat] = lse;
             const bool empty = n == 0 || l == 0.f;
-            const int row = i - lane, valid = nq - row;
-            const long long to = ((W.b * P.Nq + row) * P.Hq + W.h) * P.D, row_bytes = P.Hq * P.D * 2;
+            const int row = i - lane;
             float *part = F.part_out + (W.split * all_rows + flat) * P.D;
 #pragma unroll 1
             for (int g = 0; g < BLOCKS; ++g) {   // 64 features at a time
@@ -361,6 +359,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 }
 #pragma unroll 1
                 for (int what = 0; what < (P.rest ? 2 : 1); ++what) {   // the result, and what rounding took from it
+                    RowBlock::reuse(lane);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         uint32_t w[4];
@@ -370,13 +369,14 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                             const float a0 = empty ? 0.f : __uint_as_float(pair[0]) * by, a1 = empty ? 0.f : __uint_as_float(pair[1]) * by;
                             w[e] = what ? N::rest(a0, a1) : N::pack(a0, a1);
                         }
-                        stage.put(lane, k, w[0], w[1], w[2], w[3]);
+                        rows.put(lane, k, w[0], w[1], w[2], w[3]);
                     }
-                    stage.store(reinterpret_cast<unsigned char *>(static_cast<T *>(what ? P.rest : P.out) + to + 64 * g), row_bytes, lane, valid, (int)P.D / 8 - 8 * g);
+                    if (row < nq) rows.send(lane, what ? &map_rest : &map_out, 64 * g, row, W.h, W.b);
                 }
             }
             if (!queue.next<true>(turn, block, lane == 0, [&](uint64_t *bar, uint32_t parity) { return ok = warp_wait(bar, parity, 11); })) break;
         }
+        RowBlock::reuse(lane);   // the copy engine has read the last block before the CTA ends
     }
     tc_fence_before();
     __syncthreads();
@@ -403,16 +403,24 @@ template <typename T, int BLOCKS> int launch(const AttnParams &P, const AttnSpli
     F.tiles_per_split = splits.keys / TILE;
     F.part_out = splits.out;
     F.part_lse = splits.lse;
-    CUtensorMap q, k, v;
+    F.by_splits = divider(F.splits);
+    F.by_heads = divider(P.B * P.Hq);
+    F.by_hq = divider(P.Hq);
+    F.by_group = divider(P.group);
+    CUtensorMap q, k, v, out, rest;
     int e = make_tensor_map_heads(&q, P.q, P.D, P.Nq, P.Hq, P.B, 2 * P.q_s[1], 2 * P.q_s[2], 2 * P.q_s[0], TILE);
     if (e == TPW_OK) e = make_tensor_map_heads(&k, P.k, P.D, P.Nk, P.Hk, P.B, 2 * P.k_s[1], 2 * P.k_s[2], 2 * P.k_s[0], TILE);
     if (e == TPW_OK) e = make_tensor_map_heads(&v, P.v, P.D, P.Nk, P.Hk, P.B, 2 * P.v_s[1], 2 * P.v_s[2], 2 * P.v_s[0], TILE);
+    if (e == TPW_OK) e = make_tensor_map_heads(&out, P.out, P.D, P.Nq, P.Hq, P.B, 2 * P.Hq * P.D, 2 * P.D, 2 * P.Nq * P.Hq * P.D, 32);
+    if (e != TPW_OK) return e;
+    rest = out;
+    if (P.rest) e = make_tensor_map_heads(&rest, P.rest, P.D, P.Nq, P.Hq, P.B, 2 * P.Hq * P.D, 2 * P.D, 2 * P.Nq * P.Hq * P.D, 32);
     if (e != TPW_OK) return e;
     const long long blocks = F.tiles * P.B * P.Hq * F.splits;
     TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
     constexpr auto *kern = &attention_forward_kernel<T, BLOCKS>;
     if (const int e = allow_shared_memory<kern>((int)L::ALLOC)) return e;
-    kern<<<(unsigned)blocks, kTcThreads, L::ALLOC, s>>>(q, k, v, F);
+    kern<<<(unsigned)blocks, kTcThreads, L::ALLOC, s>>>(q, k, v, out, rest, F);
     TPW_LAUNCH_OK("attention_forward_kernel");
     return TPW_OK;
 }

@@ -246,6 +246,44 @@ template <int PIECES> struct RowStage {
     }
 };
 
+// 32 rows of 64 features on their way from a warp to global memory: a lane puts its row down in pieces of 16 bytes (128-byte swizzle), then the copy
+// engine takes the block, clipped to the tensor, while the warp goes on.  Plain stores held the warp up for 2 us a block when all
+// SMs wrote at once.  The 4 KB are 1024-byte aligned and the warp's own.
+struct RowBlock {
+    unsigned char *at;
+    __device__ __forceinline__ void put(int lane, int piece, uint32_t a, uint32_t b, uint32_t c, uint32_t d) const {
+        *reinterpret_cast<uint4 *>(at + swz128(lane, piece)) = make_uint4(a, b, c, d);
+    }
+    // before the next block is put down: the last one has been read
+    static __device__ __forceinline__ void reuse(int lane) {
+        if (lane == 0) tma_store_wait_read();
+        __syncwarp();
+    }
+    __device__ __forceinline__ void send(int lane, const CUtensorMap *map, int feature, int token, int head, int batch) const {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(reinterpret_cast<uint64_t>(map)),
+                         "r"(feature), "r"(token), "r"(head), "r"(batch), "r"(smem_u32(at))
+                         : "memory");
+            tma_store_commit();
+        }
+    }
+};
+
+// n / d for n < 2^31 by a multiplication; prepared on the host
+struct Divider {
+    uint32_t d, mul, shift;
+};
+inline Divider divider(long long d) {
+    Divider r = {(uint32_t)d, 0, 0};
+    while ((1ll << r.shift) < d) ++r.shift;
+    r.mul = (uint32_t)(((1ull << 32) * ((1ull << r.shift) - (uint64_t)d)) / (uint64_t)d + 1);
+    return r;
+}
+__device__ __forceinline__ uint32_t operator/(uint32_t n, const Divider &by) { return (__umulhi(n, by.mul) + n) >> by.shift; }
+__device__ __forceinline__ uint32_t operator%(uint32_t n, const Divider &by) { return n - (n / by) * by.d; }
+
 __device__ __forceinline__ float exp2_fast(float x) {   // 2 units of the last place; 0 below 2^-126
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
