@@ -380,10 +380,10 @@ template <typename T> int launch_width(const FewParams &F, const CUtensorMap &k,
 }
 
 // Keys of a range: so many that the ranges of full-length sequences make about four turns of two CTAs on every SM (ragged lengths and
-// windows leave ranges empty, which then cost nothing), at least 256, below which a CTA's start and the join cost more than its keys.
+// windows leave ranges empty, which then cost nothing), at least 512, whose 3 us are what the join and its launch cost.
 int keys_per_split(const AttnParams &P) {
     const long long want = P.B * P.Hk * P.Nk / (8LL * sm_count());
-    const long long keys = (want < 256 ? 256 : want) / STEP * STEP;
+    const long long keys = (want < 512 ? 512 : want) / STEP * STEP;
     return (int)(keys < P.Nk ? keys : (P.Nk + STEP - 1) / STEP * STEP);
 }
 

@@ -1,9 +1,9 @@
 // Rotary positions: each pair of features (a, b) of a row is turned by the angle of the row's position,
 // (a cos - b sin, a sin + b cos); the gradient is the turn back.
 //
-// Bound by HBM: every element is read and written once, 3 flops per element.  A thread holds the cosines and sines of one
-// 16-byte chunk of pairs in registers and walks over heads of its token with them, 4 at a time so that enough loads are in
-// flight, because loading them per head would move more bytes through L1 than the rows themselves.  Calls with too few rows to
+// Bound by HBM: every element is read and written once, 3 flops per element; bfloat16 [4, 4096, 40, 128] 64 us, 5.3 TB/s.  A thread holds the cosines and sines of one
+// 16-byte chunk of pairs in registers and walks over heads of its token with them, two at a time and the next two on their
+// way, because loading them per head would move more bytes through L1 than the rows themselves.  Calls with too few rows to
 // fill the GPU that way give each thread one head (latency instead of traffic is what counts there).
 #include "common.cuh"
 
@@ -23,7 +23,7 @@ struct RotaryParams {
     long long pos_stride[2];
     long long N, D, half, length, tokens;
     int heads_per_thread, head_groups, chunks;   // chunks per row: turned ones first, then copied ones
-    int small;                                   // fewer than 2^32 threads
+    int small, keep;                             // fewer than 2^32 threads; results of at most 64 MB
     float sign;
 };
 
@@ -32,6 +32,26 @@ template <> struct Acc<double> { typedef double type; };
 
 // W elements as they lie in memory, and two neighbours of them widened and narrowed at a time
 template <typename T, int W> struct alignas(sizeof(T) * W) Chunk { T v[W]; };
+// Every row is read and written once: past L1.  Results beyond what L2 holds are not kept there (bfloat16 [4, 4096, 40, 128] 67.4 -> 63.9 us);
+// smaller ones are what the next kernel reads.
+template <typename C> __device__ __forceinline__ C read_once(const void *p) {
+    if constexpr (sizeof(C) == 16) {
+        C c;
+        *reinterpret_cast<uint4 *>(&c) = __ldcs(static_cast<const uint4 *>(p));
+        return c;
+    } else {
+        return *static_cast<const C *>(p);
+    }
+}
+template <typename C> __device__ __forceinline__ void write_once(void *p, const C &c, bool keep) {
+    if constexpr (sizeof(C) == 16) {
+        if (!keep) {
+            __stcs(static_cast<uint4 *>(p), *reinterpret_cast<const uint4 *>(&c));
+            return;
+        }
+    }
+    *static_cast<C *>(p) = c;
+}
 template <typename T> __device__ __forceinline__ void widen2(const T *p, typename Acc<T>::type &a, typename Acc<T>::type &b) {
     a = p[0];
     b = p[1];
@@ -147,8 +167,8 @@ __global__ void __launch_bounds__(256, 4) rotary_kernel(const RotaryParams P) {
         for (int u = 0; u < U; ++u)
             if (h + u < h_stop) {
                 const T *p = h + u < h_first ? from[0] + (h + u) * P.stride[0][2] : from[1] + (h + u) * P.stride[1][2];
-                x0[u] = *reinterpret_cast<const C *>(p + o0);
-                if (two) x1[u] = *reinterpret_cast<const C *>(p + o1);
+                x0[u] = read_once<C>(p + o0);
+                if (two) x1[u] = read_once<C>(p + o1);
             }
     };
     C x0[U], x1[U];
@@ -162,8 +182,8 @@ __global__ void __launch_bounds__(256, 4) rotary_kernel(const RotaryParams P) {
                 C y0 = x0[u], y1 = x1[u];
                 if (turn) work(x0[u], x1[u], y0, y1);
                 T *p = (h + u < h_first ? to[0] : to[1]) + (h + u) * P.D;
-                *reinterpret_cast<C *>(p + o0) = y0;
-                if (two) *reinterpret_cast<C *>(p + o1) = y1;
+                write_once(p + o0, y0, P.keep);
+                if (two) write_once(p + o1, y1, P.keep);
             }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -200,8 +220,8 @@ int launch(const tpw_rotary &a, RotaryParams &P, cudaStream_t s) {
     const long long chunks = a.half / pairs + (a.D - 2 * a.half) / width;
     const long long heads = a.H[0] + a.H[1];
     P.chunks = (int)chunks;
-    // Heads per thread: as many of 4, 8 as leave the GPU at least eight blocks per SM.  bfloat16 [4, 4096, 40, 128]:
-    // DRAM-bound; a single new token of 8 sequences: 8 * 40 rows, one head per thread.
+    // Heads per thread: as many as leave the GPU at least eight blocks per SM.  More threads read the table more often (float32 [3, 1777, 24,
+    // 80], 32 turned, 8 heads 19.4 us, 2 heads 25.5); a new token of 8 sequences is 8 * 40 rows, one head per thread.
     long long per = 8;
     while (per > 1 && P.tokens * chunks * ((heads + per - 1) / per) < 8LL * 256 * sm_count()) per /= 2;
     P.heads_per_thread = (int)per;
@@ -209,6 +229,7 @@ int launch(const tpw_rotary &a, RotaryParams &P, cudaStream_t s) {
     const long long threads = P.tokens * chunks * P.head_groups, blocks = (threads + 255) / 256;
     TPW_CHECK_ARG(blocks < (1LL << 31), "tpw_rotary_apply: more than 2^31 blocks of work");
     P.small = blocks < (1LL << 24);
+    P.keep = P.tokens * heads * a.D * (long long)sizeof(T) <= (64LL << 20);
     if (wide) rotary_kernel<T, W, INTER><<<(unsigned)blocks, 256, 0, s>>>(P);
     else rotary_kernel<T, 1, INTER><<<(unsigned)blocks, 256, 0, s>>>(P);
     TPW_LAUNCH_OK("rotary_kernel");
