@@ -64,7 +64,7 @@ def assert_near(got, want, dtype, what, times=1.0):
     assert torch.equal(got[~fin], want[~fin]), what
     if not bool(fin.any()):
         return
-    g, w = got[fin], want[fin]
+    g, w = got[fin], want[fin].detach()
     norm, err = float(w.norm()), float((g - w).norm())
     tol = NORM_TOL[dtype] * times
     assert err <= tol * norm + 1e-300, f"{what}: relative error {err / max(norm, 1e-300):.3g} > {tol:.3g}"

@@ -227,3 +227,61 @@ def test_refusals():
     y.mul_(2)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_a_layer_trains_and_serves_what_it_trained(dtype):
+    """The example: packed projections, rotary positions, attention with gradients, and the same layer one token at a time."""
+    import importlib.util
+    from pathlib import Path
+    path = Path(__file__).resolve().parent.parent / "examples" / "attention_retrieval.py"
+    spec = importlib.util.spec_from_file_location("attention_retrieval", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    losses, apart = example.main(steps=6, sequences=32, dtype=dtype, report=lambda text: None)
+    assert all(math.isfinite(x) for x in losses)
+    # either side rounds probabilities and outputs a few times in the type: sixteen units for a sum of such terms
+    assert apart < 16 * torch.finfo(dtype).eps
+    assert tpw.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("d", [64, 128])
+def test_lengths_of_every_size_around_the_tiles(dtype, d):
+    """Each length from none to past two tiles of keys, against every number of queries that changes a kernel or fills a tile."""
+    g = torch.Generator().manual_seed(11)
+    sizes = [0, 1, 15, 16, 17, 63, 64, 65, 127, 128, 129, 255, 256, 257, 300]
+    k, v = (torch.randn(len(sizes), 300, 1, d, generator=g).to(dtype).cuda() for _ in range(2))
+    n = torch.tensor(sizes, dtype=torch.int32, device="cuda")
+    for nq in (1, 16, 17, 33, 129, 257):
+        q = torch.randn(len(sizes), nq, 2, d, generator=g).to(dtype).cuda()
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        for causal in (False, True):
+            out, lse = tpw.attention(*leaves, causal=causal, key_lengths=n, return_lse=True)
+            want = reference(q, k, v, causal=causal, lengths=sizes, grad=q)
+            assert_near(out, want[0], dtype, f"out {nq} {causal}")
+            assert_near(lse, want[1], torch.float64 if dtype == torch.float64 else torch.float32, f"lse {nq} {causal}")
+            # as above: the gradients of scores cancel where a row sees a key or two
+            few = [i for i, size in enumerate(sizes) if size < 3]
+            rest = [i for i, size in enumerate(sizes) if size >= 3]
+            for got, w, name in zip(torch.autograd.grad(out, leaves, q), want[2:], ("dq", "dk", "dv")):
+                assert_near(got[rest], w[rest], dtype, f"{name} {nq} {causal}", 2.0)
+                size = math.sqrt(w[few].numel()) * math.sqrt(d)
+                assert float((got[few].double() - w[few]).norm()) <= 2 * size * torch.finfo(dtype).eps, f"{name} {nq} {causal}"
+
+
+def test_many_blocks_of_every_kind_in_one_launch():
+    """More blocks than SMs, empty ones among them, so that CTAs take over blocks with and without keys."""
+    g = torch.Generator().manual_seed(12)
+    lengths = [0, 700, 128, 0, 1, 333, 256, 699]
+    q, k, v = (torch.randn(8, n, 12, 64, generator=g).bfloat16().cuda() for n in (600, 700, 700))
+    n = torch.tensor(lengths, device="cuda")
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    for mask in (dict(), dict(causal=True), dict(causal=True, window=130)):
+        out, lse = tpw.attention(*leaves, key_lengths=n, return_lse=True, **mask)
+        want = reference(q, k, v, lengths=lengths, grad=q, **mask)
+        assert_near(out, want[0], torch.bfloat16, "out")
+        assert_near(lse, want[1], torch.float32, "lse")
+        for got, w, name in zip(torch.autograd.grad(out, leaves, q), want[2:], ("dq", "dk", "dv")):
+            assert_near(got, w, torch.bfloat16, name, 2.0)
+    assert tpw.device_status() == 0

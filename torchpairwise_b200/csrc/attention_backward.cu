@@ -290,7 +290,7 @@ __device__ __forceinline__ void keys_walk(const CUtensorMap &map_q, const CUtens
                     for (int r = 0; r < 2; ++r) {
                         const uint32_t *pair = &x[hh][4 * i + 2 * r];
                         const f32x2 z = fma2(pack2(__uint_as_float(pair[0]), __uint_as_float(pair[1])), c2, minus_lse);
-                        p[hh][2 * i + r] = 2 * hh + r == 3 ? exp2_polynomial(z) : exp2_pair(z);
+                        p[hh][2 * i + r] = 2 * hh + r == 1 ? exp2_polynomial(z) : exp2_pair(z);
                     }
             }
             if (masked) hide(p, i0);
@@ -493,7 +493,7 @@ __device__ __forceinline__ void queries_walk(const CUtensorMap &map_q, const CUt
             for (int e = 0; e < 32; ++e) {
                 const uint32_t *pair = &x[e >> 4][2 * (e & 15)];
                 const f32x2 z = fma2(pack2(__uint_as_float(pair[0]), __uint_as_float(pair[1])), c2, minus_lse);
-                p[e] = e % 4 == 3 ? exp2_polynomial(z) : exp2_pair(z);
+                p[e] = e % 4 == 1 ? exp2_polynomial(z) : exp2_pair(z);
             }
             if (!(ok = warp_wait(&dp_full[u & 1], (u >> 1) & 1, 8))) break;
             tc_fence_after();

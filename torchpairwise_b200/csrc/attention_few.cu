@@ -299,13 +299,14 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     }
 }
 
-// out = sum_s w_s out_s, w_s = exp(lse_s - lse), lse = log sum_s exp(lse_s); one warp per row.  A lane holds the weight of every 32nd range;
-// the ranges' outputs are then fetched four at a time, none waiting for another (one after the other they took 8 us for 10 ranges of 512 rows).
-template <typename T>
+// out = sum_s w_s out_s, w_s = exp(lse_s - lse), lse = log sum_s exp(lse_s).  WARPS of a block's eight share a row: one, or all of them where the
+// ranges are many.  A lane holds the weight of every 32nd range; the ranges' outputs are fetched four at a time, none waiting for
+// another (one after the other they took 8 us for 10 ranges of 512 rows).  The order of the sums follows from the sizes alone.
+template <typename T, int WARPS>
 __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams P, const float *part_out, const float *part_lse, int splits) {
-    const int lane = threadIdx.x & 31, D = (int)P.D;
-    const long long rows = P.B * P.Hq * P.Nq, row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (row >= rows) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % WARPS, D = (int)P.D;
+    const long long rows = P.B * P.Hq * P.Nq, row = (long long)blockIdx.x * (8 / WARPS) + warp / WARPS;
+    if (row >= rows) return;   // the whole block, or whole rows
     const float log2e = 1.4426950408889634f;
     float top = -INFINITY;
     for (int s = lane; s < splits; s += 32) {
@@ -318,7 +319,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams P,
         top = x > top || x != x ? x : top;
     }
     float sum = 0.f, x[2] = {}, y[2] = {};
-    for (int s0 = 0; s0 < splits; s0 += 32) {
+    for (int s0 = 32 * share; s0 < splits; s0 += 32 * WARPS) {
         const float mine = s0 + lane < splits ? part_lse[(s0 + lane) * rows + row] : -INFINITY;
         const float w = mine == -INFINITY ? 0.f : exp2f((mine - top) * log2e);
         sum += w;
@@ -346,6 +347,23 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams P,
     }
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if constexpr (WARPS > 1) {
+        __shared__ float parts[WARPS][5][32];
+        const float mine[5] = {x[0], y[0], x[1], y[1], sum};
+#pragma unroll
+        for (int k = 0; k < 5; ++k) parts[share][k][lane] = mine[k];
+        __syncthreads();
+        if (share != 0) return;
+        x[0] = x[1] = y[0] = y[1] = sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            x[0] += parts[w][0][lane];
+            y[0] += parts[w][1][lane];
+            x[1] += parts[w][2][lane];
+            y[1] += parts[w][3][lane];
+            sum += parts[w][4][lane];
+        }
+    }
     const long long bh = row / P.Nq, i = row % P.Nq, h = bh % P.Hq, b = bh / P.Hq;
     const long long to = ((b * P.Nq + i) * P.Hq + h) * P.D;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -380,11 +398,13 @@ template <typename T> int launch_width(const FewParams &F, const CUtensorMap &k,
 }
 
 // Keys of a range: so many that the ranges of full-length sequences make about four turns of two CTAs on every SM (ragged lengths and
-// windows leave ranges empty, which then cost nothing), at least 512, whose 3 us are what the join and its launch cost.
+// windows leave ranges empty, which then cost nothing), at least 512, whose 3 us are what the join and its launch cost, and no more ranges of a
+// sequence than CTAs at a time.
 int keys_per_split(const AttnParams &P) {
-    const long long want = P.B * P.Hk * P.Nk / (8LL * sm_count());
-    const long long keys = (want < 512 ? 512 : want) / STEP * STEP;
-    return (int)(keys < P.Nk ? keys : (P.Nk + STEP - 1) / STEP * STEP);
+    const long long slots = 2LL * sm_count(), want = P.B * P.Hk * P.Nk / (4 * slots), least = (P.Nk + slots - 1) / slots;
+    const long long keys = want > least ? want : least, whole = (P.Nk + STEP - 1) / STEP * STEP;
+    const long long r = ((keys < 512 ? 512 : keys) + STEP - 1) / STEP * STEP;
+    return (int)(r < whole ? r : whole);
 }
 
 } // namespace
@@ -415,14 +435,16 @@ int attn_few_forward(int dtype, const AttnParams &P, const AttnSplits &splits, c
     return dtype == TPW_F16 ? launch_width<__half>(F, k, v, s) : launch_width<__nv_bfloat16>(F, k, v, s);
 }
 
-int attn_join(int dtype, const AttnParams &P, const AttnSplits &splits, cudaStream_t s) {
-    const long long blocks = (P.B * P.Hq * P.Nq + 7) / 8;
+template <typename T> static int join(const AttnParams &P, const AttnSplits &splits, cudaStream_t s) {
+    const long long rows = P.B * P.Hq * P.Nq, blocks = splits.count > 32 ? rows : (rows + 7) / 8;
     TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
-    if (dtype == TPW_F16) attention_join_kernel<__half><<<(unsigned)blocks, 256, 0, s>>>(P, splits.out, splits.lse, splits.count);
-    else if (dtype == TPW_F32) attention_join_kernel<float><<<(unsigned)blocks, 256, 0, s>>>(P, splits.out, splits.lse, splits.count);
-    else attention_join_kernel<__nv_bfloat16><<<(unsigned)blocks, 256, 0, s>>>(P, splits.out, splits.lse, splits.count);
+    if (splits.count > 32) attention_join_kernel<T, 8><<<(unsigned)blocks, 256, 0, s>>>(P, splits.out, splits.lse, splits.count);
+    else attention_join_kernel<T, 1><<<(unsigned)blocks, 256, 0, s>>>(P, splits.out, splits.lse, splits.count);
     TPW_LAUNCH_OK("attention_join_kernel");
     return TPW_OK;
+}
+int attn_join(int dtype, const AttnParams &P, const AttnSplits &splits, cudaStream_t s) {
+    return dtype == TPW_F16 ? join<__half>(P, splits, s) : dtype == TPW_F32 ? join<float>(P, splits, s) : join<__nv_bfloat16>(P, splits, s);
 }
 
 } // namespace tpw
