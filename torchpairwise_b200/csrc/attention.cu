@@ -33,6 +33,12 @@ AttnSplits splits_of(int dtype, const AttnParams &P) {
 long long split_bytes(const AttnParams &P, const AttnSplits &splits) {
     return splits.count > 1 ? 4 * splits.count * P.B * P.Hq * P.Nq * (P.D + 1) : 0;
 }
+long long forward_bytes(int dtype, const AttnParams &P) {
+    return attn_parts_fits(dtype, P) ? attn_parts_bytes(P, false) : split_bytes(P, splits_of(dtype, P));
+}
+long long backward_bytes(int dtype, const AttnParams &P) {
+    return attn_rows_bytes(dtype, P) + (attn_parts_backward_fits(dtype, P) ? attn_parts_bytes(P, true) : 0);
+}
 
 } // namespace
 } // namespace tpw
@@ -44,7 +50,7 @@ int64_t tpw_attention_scratch_bytes(const tpw_attention *a) {
     if (tpw::check(a, false) != TPW_OK) return -1;
     if (tpw::nothing(*a)) return 0;
     const tpw::AttnParams P = tpw::attn_params(*a);
-    return tpw::split_bytes(P, tpw::splits_of(a->dtype, P));
+    return tpw::forward_bytes(a->dtype, P);
 }
 
 int tpw_attention_forward(const tpw_attention *a, void *scratch, int64_t scratch_bytes, tpw_stream_t stream) {
@@ -55,10 +61,11 @@ int tpw_attention_forward(const tpw_attention *a, void *scratch, int64_t scratch
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool f32 = tpw::attn_f32_fits(a->dtype, P);
     if (f32 || tpw::attn_tc_fits(a->dtype, P)) {
-        tpw::AttnSplits splits = tpw::splits_of(a->dtype, P);
-        const int64_t bytes = tpw::split_bytes(P, splits);
+        const int64_t bytes = tpw::forward_bytes(a->dtype, P);
         TPW_CHECK_ARG(bytes == 0 || (scratch && tpw::aligned16(scratch) && scratch_bytes >= bytes),
                       "tpw_attention_forward: scratch of %lld bytes, 16-byte aligned, is needed", (long long)bytes);
+        if (tpw::attn_parts_fits(a->dtype, P)) return tpw::attn_parts_forward(P, scratch, s);
+        tpw::AttnSplits splits = tpw::splits_of(a->dtype, P);
         splits.out = static_cast<float *>(scratch);
         splits.lse = splits.out ? splits.out + splits.count * P.B * P.Hq * P.Nq * P.D : nullptr;
         const int e = f32 ? tpw::attn_f32_forward(P, splits, s) : tpw::attn_few_fits(a->dtype, P) ? tpw::attn_few_forward(a->dtype, P, splits, s) : tpw::attn_tc_forward(a->dtype, P, splits, s);
@@ -71,7 +78,7 @@ int64_t tpw_attention_backward_scratch_bytes(const tpw_attention *a) {
     tpw::clear_error();
     if (tpw::check(a, true) != TPW_OK) return -1;
     if (tpw::nothing(*a)) return 0;
-    return tpw::attn_rows_bytes(a->dtype, tpw::attn_params(*a));
+    return tpw::backward_bytes(a->dtype, tpw::attn_params(*a));
 }
 
 int tpw_attention_backward(const tpw_attention *a, void *scratch, int64_t scratch_bytes, tpw_stream_t stream) {
@@ -89,13 +96,14 @@ int tpw_attention_backward(const tpw_attention *a, void *scratch, int64_t scratc
         return TPW_OK;
     }
     tpw::AttnParams P = tpw::attn_params(*a);
-    TPW_CHECK_ARG(scratch && tpw::aligned16(scratch) && scratch_bytes >= tpw::attn_rows_bytes(a->dtype, P),
-                  "tpw_attention_backward: scratch of %lld bytes, 16-byte aligned, is needed", tpw::attn_rows_bytes(a->dtype, P));
+    const long long bytes = tpw::backward_bytes(a->dtype, P);
+    TPW_CHECK_ARG(scratch && tpw::aligned16(scratch) && scratch_bytes >= bytes, "tpw_attention_backward: scratch of %lld bytes, 16-byte aligned, is needed", bytes);
     if (!P.dq && !P.dk) return TPW_OK;
     const bool tensor = tpw::attn_tc_backward_fits(a->dtype, P);
     e = tpw::attn_rows(a->dtype, P, scratch, tensor, s);
     if (e != TPW_OK) return e;
     if (tensor) return tpw::attn_tc_backward(a->dtype, P, s);
+    if (tpw::attn_parts_backward_fits(a->dtype, P)) return tpw::attn_parts_backward(P, static_cast<unsigned char *>(scratch) + tpw::attn_rows_bytes(a->dtype, P), s);
     if (tpw::attn_f32_backward_fits(a->dtype, P)) return tpw::attn_f32_backward(P, s);
     return tpw::attn_simple_backward(a->dtype, P, s);
 }

@@ -79,6 +79,12 @@ bool attn_f32_backward_fits(int dtype, const AttnParams &P);
 AttnSplits attn_f32_splits(const AttnParams &P);
 int attn_f32_forward(const AttnParams &P, const AttnSplits &splits, cudaStream_t s);
 int attn_f32_backward(const AttnParams &P, cudaStream_t s);
+// attention_parts.cu: float32 up to 64 features on the 16-bit tensor cores, operands as sums of three bfloat16 numbers, which lie in scratch
+bool attn_parts_fits(int dtype, const AttnParams &P);
+bool attn_parts_backward_fits(int dtype, const AttnParams &P);
+long long attn_parts_bytes(const AttnParams &P, bool backward);
+int attn_parts_forward(const AttnParams &P, void *scratch, cudaStream_t s);
+int attn_parts_backward(const AttnParams &P, void *scratch, cudaStream_t s);
 // attention_few.cu: few query rows
 bool attn_few_fits(int dtype, const AttnParams &P);
 AttnSplits attn_few_splits(const AttnParams &P);
