@@ -72,59 +72,30 @@ __global__ void __launch_bounds__(256) attention_parts_kernel(const __grid_const
 }
 
 // ---- products of parts ----
-enum Keep { NONE, FILL, USE };   // of the left operand in the tensor cores' collector: it is read once for neighbouring MMAs that share it
-template <int KEEP> __device__ __forceinline__ void part_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-#define TPW_PART_SS(OP) \
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t" \
-                 "@q tcgen05.mma.cta_group::1.kind::f16" OP " [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader) : "memory")
-    if (KEEP == FILL) TPW_PART_SS(".collector::a::fill");
-    else if (KEEP == USE) TPW_PART_SS(".collector::a::lastuse");
-    else TPW_PART_SS("");
-#undef TPW_PART_SS
-}
-template <int KEEP> __device__ __forceinline__ void part_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-#define TPW_PART_TS(OP) \
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t" \
-                 "@q tcgen05.mma.cta_group::1.kind::f16" OP " [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader) : "memory")
-    if (KEEP == FILL) TPW_PART_TS(".collector::a::fill");
-    else if (KEEP == USE) TPW_PART_TS(".collector::a::lastuse");
-    else TPW_PART_TS("");
-#undef TPW_PART_TS
-}
+// the pairs of parts, small products first
+__device__ __forceinline__ constexpr int left_part(int i) { return i == 0 ? 2 : i == 2 || i == 3 ? 1 : 0; }
+__device__ __forceinline__ constexpr int right_part(int i) { return i == 1 ? 2 : i == 2 || i == 4 ? 1 : 0; }
 
-// D = X Y^T over 16 * steps features; X 128 tokens, Y 64
-__device__ __forceinline__ void parts_along_features(uint32_t leader, uint32_t d, uint32_t x, uint32_t y, uint32_t idesc, int steps) {
-    const uint64_t a0 = make_smem_desc(x), b0 = make_smem_desc(y);
-    auto a = [&](int part, int k) { return a0 + (uint64_t)(part * (OWN_PART >> 4)) + feature_step(k); };
-    auto b = [&](int part, int k) { return b0 + (uint64_t)(part * (WALK_PART >> 4)) + feature_step(k); };
+// D = X Y^T over 64 features (zeros beyond D); X 128 tokens, Y 64.  Fixed counts and addresses that are the same in every lane: the MMAs are
+// issued back to back (a count that depends on D: backward 196 -> 187 us at 64 features).
+__device__ __forceinline__ void parts_along_features(uint32_t leader, uint32_t d, uint32_t x, uint32_t y, uint32_t idesc) {
+    x = __shfl_sync(0xffffffffu, x, 0), y = __shfl_sync(0xffffffffu, y, 0), d = __shfl_sync(0xffffffffu, d, 0);
+    const uint64_t a = make_smem_desc(x), b = make_smem_desc(y);
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (k < steps) {
-            part_ss<NONE>(leader, d, a(2, k), b(0, k), idesc, k != 0);
-            part_ss<FILL>(leader, d, a(1, k), b(1, k), idesc, true);
-            part_ss<USE>(leader, d, a(1, k), b(0, k), idesc, true);
-            part_ss<FILL>(leader, d, a(0, k), b(2, k), idesc, true);
-            part_ss<USE>(leader, d, a(0, k), b(1, k), idesc, true);
-        }
+    for (int i = 0; i < 6; ++i)
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (k < steps) part_ss<NONE>(leader, d, a(0, k), b(0, k), idesc, true);
+        for (int k = 0; k < 4; ++k)
+            mma_ss(leader, d, a + left_part(i) * (OWN_PART >> 4) + feature_step(k), b + right_part(i) * (WALK_PART >> 4) + feature_step(k), idesc, i + k != 0);
 }
 // D = P Y over 64 tokens; P in tensor memory
 __device__ __forceinline__ void parts_along_tokens(uint32_t leader, uint32_t d, uint32_t p, uint32_t y, uint32_t idesc) {
-    const uint64_t b0 = make_smem_desc_tokens(y);
-    auto a = [&](int part, int k) { return p + part * PART_COLUMNS + 8 * k; };
-    auto b = [&](int part, int k) { return b0 + (uint64_t)(part * (WALK_PART >> 4)) + (uint64_t)k * (2048 >> 4); };
+    p = __shfl_sync(0xffffffffu, p, 0), y = __shfl_sync(0xffffffffu, y, 0), d = __shfl_sync(0xffffffffu, d, 0);
+    const uint64_t b = make_smem_desc_tokens(y);
 #pragma unroll
-    for (int k = 0; k < KEYS / 16; ++k) {
-        part_ts<NONE>(leader, d, a(2, k), b(0, k), idesc, k != 0);
-        part_ts<FILL>(leader, d, a(1, k), b(1, k), idesc, true);
-        part_ts<USE>(leader, d, a(1, k), b(0, k), idesc, true);
-        part_ts<FILL>(leader, d, a(0, k), b(2, k), idesc, true);
-        part_ts<USE>(leader, d, a(0, k), b(1, k), idesc, true);
-    }
+    for (int i = 0; i < 6; ++i)
 #pragma unroll
-    for (int k = 0; k < KEYS / 16; ++k) part_ts<NONE>(leader, d, a(0, k), b(0, k), idesc, true);
+        for (int k = 0; k < KEYS / 16; ++k)
+            mma_ts(leader, d, p + left_part(i) * PART_COLUMNS + 8 * k, b + right_part(i) * (WALK_PART >> 4) + k * (2048 >> 4), idesc, i + k != 0);
 }
 __device__ __forceinline__ uint32_t instruction_parts(uint32_t n, bool b_mn) { return instruction(Part::kFormat, n, b_mn); }
 
@@ -202,7 +173,7 @@ attention_forward_parts_kernel(const __grid_constant__ CUtensorMap map_q, const 
     const int h = (int)(bh % (unsigned)P.Hq), b = (int)(bh / (unsigned)P.Hq), hk = h / (int)P.group;
     const Seen see(P, b);
     const int nq = (int)P.Nq, last = (row0 + TILE < nq ? row0 + TILE : nq) - 1;
-    const int begin = see.lo(row0) / KEYS, end = (see.hi(last) + KEYS - 1) / KEYS, total = end > begin ? end - begin : 0;
+    const int begin = see.lo(row0) / KEYS, end = (see.hi(last) + KEYS - 1) / KEYS, total = __shfl_sync(0xffffffffu, end > begin ? end - begin : 0, 0);
 
     if (threadIdx.x == 0) {
         for (uint64_t *bar = q_full; bar <= drained; ++bar) mbar_init(bar, bar == s_read || bar == p_full ? 4 : 1);
@@ -254,14 +225,13 @@ attention_forward_parts_kernel(const __grid_constant__ CUtensorMap map_q, const 
             }
         }
     } else if (warp == 5) {
-        const int steps = (int)(P.D + 15) / 16;
-        const uint32_t idesc_s = instruction_parts(KEYS, false), idesc_o = instruction_parts(16 * steps, true);
+        const uint32_t idesc_s = instruction_parts(KEYS, false), idesc_o = instruction_parts(KEYS, true);
         const uint32_t leader = elect_lane();
         bool ok = total == 0 || warp_wait(q_full, 0, 3);
         auto scores = [&](int u) {
             if (!warp_wait(k_full, u & 1, 4)) return false;
             tc_fence_after();
-            parts_along_features(leader, S, q_at, k_at, idesc_s, steps);
+            parts_along_features(leader, S, q_at, k_at, idesc_s);
             commit_by(leader, s_full);
             commit_by(leader, k_empty);
             return true;
@@ -379,7 +349,7 @@ struct BackwardPartsSmem {
     static constexpr uint32_t OFF_X = 6 * OWN_PART, OFF_Y = OFF_X + kX * TILE_BYTES;
     static constexpr uint32_t OFF_ROWS = OFF_Y + kY * TILE_BYTES;   // keys walk: lse, delta of a query tile, with its Q
     static constexpr uint32_t OFF_BAR = OFF_ROWS + kX * 2 * KEYS * 4;
-    static constexpr uint32_t OFF_TMEM = OFF_BAR + 8 * 24;
+    static constexpr uint32_t OFF_TMEM = OFF_BAR + 8 * 26;
     static constexpr uint32_t ALLOC = OFF_TMEM + 16 + 1024;
     static_assert(ALLOC <= 232448, "exceeds the dynamic shared memory of one CTA");
 };
@@ -408,15 +378,24 @@ __device__ __forceinline__ void hide(float (&x)[KEYS], int first, int lo, int hi
 // Barriers of either walk.  A wait for a use of a barrier comes after the one before is known to be over: what both warpgroups pass or
 // arrive at, each at its own pace, has a barrier for the even tiles and one for the odd ones.
 struct BackwardBarriers {
-    uint64_t *own, *x_full, *x_empty, *y_full, *y_empty, *s_full, *s_read, *dp_full, *p_ready, *ds_ready, *sum_full, *sum_read, *all_full, *drained;
+    uint64_t *own, *x_full, *x_empty, *y_full, *y_empty, *s_full, *dp_full, *s_read, *p_ready, *ds_ready, *sum_full, *sum_read, *all_full, *drained;
     __device__ __forceinline__ explicit BackwardBarriers(uint64_t *at)
-        : own(at), x_full(at + 1), x_empty(at + 4), y_full(at + 7), y_empty(at + 9), s_full(at + 11), s_read(at + 13), dp_full(at + 15), p_ready(at + 16), ds_ready(at + 17),
-          sum_full(at + 19), sum_read(at + 21), all_full(at + 22), drained(at + 23) {}
-    __device__ __forceinline__ void init() const {
-        for (uint64_t *at = own; at <= drained; ++at) {
-            const bool rows = at == p_ready || at == ds_ready || at == ds_ready + 1 || at == sum_read;
-            mbar_init(at, at == s_read || at == s_read + 1 ? 8 : rows ? 4 : 1);
-        }
+        : own(at), x_full(at + 1), x_empty(at + 4), y_full(at + 7), y_empty(at + 9), s_full(at + 11), dp_full(at + 13), s_read(at + 15), p_ready(at + 17), ds_ready(at + 18),
+          sum_full(at + 20), sum_read(at + 22), all_full(at + 23), drained(at + 24) {}
+    template <bool OF_KEYS> __device__ __forceinline__ void init() const {
+        auto init = [](uint64_t *at, int n, int count) {
+            for (int i = 0; i < n; ++i) mbar_init(at + i, count);
+        };
+        init(own, 7, 1);                        // and x_full, x_empty
+        init(y_full, 2, 1);
+        init(y_empty, 2, OF_KEYS ? 2 : 1);      // keys walk: dP and dV read it
+        init(s_full, 4, 1);                     // and dp_full
+        init(s_read, 2, 8);
+        init(p_ready, 3, 4);                    // and ds_ready
+        init(sum_full, 2, 1);
+        init(sum_read, 1, 4);
+        init(all_full, 1, 2);
+        init(drained, 2, 1);
     }
 };
 
@@ -437,10 +416,10 @@ __device__ __forceinline__ void walk(const CUtensorMap &map_q, const CUtensorMap
     const Seen see(P, b);
     const int nq = (int)P.Nq, rows = OF_KEYS ? see.length : nq, last = (row0 + TILE < rows ? row0 + TILE : rows) - 1;
     const int first = last < row0 ? 0 : OF_KEYS ? see.qlo(row0) : see.lo(row0), end = last < row0 ? 0 : OF_KEYS ? see.qhi(last) : see.hi(last);
-    const int begin = first / KEYS, per_head = end > first ? (end + KEYS - 1) / KEYS - begin : 0, total = OF_KEYS ? per_head * (int)P.group : per_head;
+    const int begin = first / KEYS, per_head = end > first ? (end + KEYS - 1) / KEYS - begin : 0, total = __shfl_sync(0xffffffffu, OF_KEYS ? per_head * (int)P.group : per_head, 0);
 
     if (threadIdx.x == 0) {
-        bar.init();
+        bar.init<OF_KEYS>();
         *abort_flag = 0;
         mbar_init_fence();
         tma_prefetch_descriptor(&map_q);
@@ -503,9 +482,10 @@ __device__ __forceinline__ void walk(const CUtensorMap &map_q, const CUtensorMap
                 for (uint32_t u = first_of_last_uses(issued_y, L::kY); u < issued_y; ++u) mbar_wait_bounded(&bar.y_full[u % L::kY], parity_of_use(u, L::kY));
             }
         }
-    } else if (warp == 9) {
-        const int steps = (int)(P.D + 15) / 16;
-        const uint32_t idesc_s = instruction_parts(KEYS, false), idesc_d = instruction_parts(16 * steps, true);
+    } else if (warp == 9 || warp == 10) {
+        // Two warps issue, each the products of one chain: a wait and a commit cost the issuing warp 100 to 200 clocks, in which the other's MMAs
+        // run.
+        const uint32_t idesc_s = instruction_parts(KEYS, false), idesc_d = instruction_parts(KEYS, true);
         const uint32_t leader = elect_lane();
         bool ok = total == 0 || warp_wait(bar.own, 0, 3);
         auto arrived = [&](uint64_t *full, uint32_t u, uint32_t stages, int site) {
@@ -513,57 +493,56 @@ __device__ __forceinline__ void walk(const CUtensorMap &map_q, const CUtensorMap
             tc_fence_after();
             return true;
         };
-        if constexpr (OF_KEYS) {
-            auto scores = [&](int u) {
-                if (!arrived(bar.x_full, u, L::kX, 4)) return false;
-                parts_along_features(leader, S + (u & 1) * KEYS, own_x, ring_x + (u % L::kX) * L::TILE_BYTES, idesc_s, steps);
-                commit_by(leader, &bar.s_full[u & 1]);
-                return true;
-            };
-            auto products = [&](int u) {
-                if (!arrived(bar.y_full, u, L::kY, 5)) return false;
-                parts_along_features(leader, DP, own_y, ring_y + (u % L::kY) * L::TILE_BYTES, idesc_s, steps);
-                commit_by(leader, bar.dp_full);
-                return true;
-            };
-            if (total > 0 && ok) ok = scores(0) && products(0);
+        auto from_x = [&](int u) {   // scores
+            if (!arrived(bar.x_full, u, L::kX, 4)) return false;
+            parts_along_features(leader, S + (u & 1) * KEYS, own_x, ring_x + (u % L::kX) * L::TILE_BYTES, idesc_s);
+            commit_by(leader, &bar.s_full[u & 1]);
+            return true;
+        };
+        auto from_y = [&](int u) {   // dP
+            if (!arrived(bar.y_full, u, L::kY, 5)) return false;
+            parts_along_features(leader, DP + (OF_KEYS ? 0 : (u & 1) * KEYS), own_y, ring_y + (u % L::kY) * L::TILE_BYTES, idesc_s);
+            commit_by(leader, &bar.dp_full[OF_KEYS ? 0 : u & 1]);
+            commit_by(leader, &bar.y_empty[u % L::kY]);
+            return true;
+        };
+        auto sums = [&](uint32_t to, uint32_t parts, uint32_t tile, uint64_t *full, uint64_t *empty) {
+            tc_fence_after();
+            parts_along_tokens(leader, to, parts, tile, idesc_d);
+            commit_by(leader, full);
+            commit_by(leader, empty);
+        };
+        if (OF_KEYS && warp == 9) {   // S, dV
+            if (total > 0 && ok) ok = from_x(0);
             for (int u = 0; u < total && ok; ++u) {
                 if (u + 1 < total) {
                     if (u > 0 && !(ok = warp_wait(&bar.s_read[(u - 1) & 1], ((u - 1) >> 1) & 1, 6))) break;
-                    tc_fence_after();
-                    if (!(ok = scores(u + 1))) break;
+                    if (!(ok = from_x(u + 1))) break;
                 }
                 if (!(ok = warp_wait(bar.p_ready, u & 1, 7))) break;
-                tc_fence_after();
-                parts_along_tokens(leader, SUM, LEFT, ring_y + (u % L::kY) * L::TILE_BYTES, idesc_d);
-                commit_by(leader, &bar.sum_full[0]);
-                commit_by(leader, &bar.y_empty[u % L::kY]);
+                sums(SUM, LEFT, ring_y + (u % L::kY) * L::TILE_BYTES, &bar.sum_full[0], &bar.y_empty[u % L::kY]);
+            }
+        } else if (OF_KEYS) {   // dP, dK
+            if (total > 0 && ok) ok = from_y(0);
+            for (int u = 0; u < total && ok; ++u) {
                 if (!(ok = warp_wait(bar.ds_ready, u & 1, 8))) break;
                 tc_fence_after();
-                if (u + 1 < total && !(ok = products(u + 1))) break;
-                parts_along_tokens(leader, SUM + KEYS, RIGHT, ring_x + (u % L::kX) * L::TILE_BYTES, idesc_d);
-                commit_by(leader, &bar.sum_full[1]);
-                commit_by(leader, &bar.x_empty[u % L::kX]);
+                if (u + 1 < total && !(ok = from_y(u + 1))) break;
+                sums(SUM + KEYS, RIGHT, ring_x + (u % L::kX) * L::TILE_BYTES, &bar.sum_full[1], &bar.x_empty[u % L::kX]);
             }
-        } else {
-            auto both = [&](int u) {   // S and dP
-                if (!arrived(bar.x_full, u, L::kX, 4)) return false;
-                parts_along_features(leader, S + (u & 1) * KEYS, own_x, ring_x + (u % L::kX) * L::TILE_BYTES, idesc_s, steps);
-                if (!arrived(bar.y_full, u, L::kY, 5)) return false;
-                parts_along_features(leader, DP + (u & 1) * KEYS, own_y, ring_y + (u % L::kY) * L::TILE_BYTES, idesc_s, steps);
-                commit_by(leader, &bar.s_full[u & 1]);
-                commit_by(leader, &bar.y_empty[u % L::kY]);
-                return true;
-            };
-            if (total > 0 && ok) ok = both(0);
+        } else if (warp == 9) {   // S, dQ
+            if (total > 0 && ok) ok = from_x(0);
             for (int u = 0; u < total && ok; ++u) {
-                if (u + 1 < total && !(ok = both(u + 1))) break;   // tile u - 1's gradients are there, so its scores have been read
+                if (u + 1 < total && !(ok = from_x(u + 1))) break;   // tile u - 1's gradients are there, so its scores have been read
                 if (!(ok = warp_wait(&bar.ds_ready[u & 1], (u >> 1) & 1, 6))) break;
                 if (u > 0 && !(ok = warp_wait(bar.sum_read, (u & 1) ^ 1, 7))) break;
+                sums(SUM, u & 1 ? RIGHT : LEFT, ring_x + (u % L::kX) * L::TILE_BYTES, &bar.sum_full[u & 1], &bar.x_empty[u % L::kX]);
+            }
+        } else {   // dP
+            for (int u = 0; u < total && ok; ++u) {
+                if (u > 1 && !(ok = warp_wait(&bar.ds_ready[u & 1], ((u - 2) >> 1) & 1, 8))) break;
                 tc_fence_after();
-                parts_along_tokens(leader, SUM, u & 1 ? RIGHT : LEFT, ring_x + (u % L::kX) * L::TILE_BYTES, idesc_d);
-                commit_by(leader, &bar.sum_full[u & 1]);
-                commit_by(leader, &bar.x_empty[u % L::kX]);
+                ok = from_y(u);
             }
         }
         if (ok && total > 0) commit_by(leader, bar.all_full);
@@ -602,7 +581,7 @@ __device__ __forceinline__ void walk(const CUtensorMap &map_q, const CUtensorMap
                     unpack2(exp2_pair(fma2(pack2(p[e + 2], p[e + 3]), pack2(c, c), pack2(-t.z, -t.w))), p[e + 2], p[e + 3]);
                 }
                 if (group) {
-                    if (!(ok = warp_wait(bar.dp_full, u & 1, 11))) break;
+                    if (!(ok = warp_wait(&bar.dp_full[0], u & 1, 11))) break;
                     tc_fence_after();
 #pragma unroll
                     for (int g = 0; g < 2; ++g) {
@@ -649,7 +628,7 @@ __device__ __forceinline__ void walk(const CUtensorMap &map_q, const CUtensorMap
             const uint32_t parts_at = (group ? RIGHT : LEFT) + lanes;
             for (int u = group; u < total; u += 2) {
                 const int j0 = (begin + u) * KEYS;
-                if (!(ok = warp_wait(&bar.s_full[group], (u >> 1) & 1, 9))) break;
+                if (!(ok = warp_wait(&bar.s_full[group], (u >> 1) & 1, 9) && warp_wait(&bar.dp_full[group], (u >> 1) & 1, 11))) break;
                 tc_fence_after();
                 float p[KEYS];
                 take_row(S + group * KEYS + lanes, p);
@@ -700,12 +679,12 @@ __device__ __forceinline__ void walk(const CUtensorMap &map_q, const CUtensorMap
     }
     tc_fence_before();
     __syncthreads();
+    if ((warp == 9 || warp == 10) && *abort_flag) {   // the commits behind all MMAs were waited for, or one more of each issuing lane is waited for here
+        commit_by(elect_lane(), &bar.drained[warp - 9]);
+        mbar_wait_bounded(&bar.drained[warp - 9], 0);
+    }
+    __syncthreads();
     if (warp == 9) {
-        if (*abort_flag && lane == 0) {
-            tc_commit<false>(bar.drained);
-            mbar_wait_bounded(bar.drained, 0);
-        }
-        __syncwarp();
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
