@@ -24,7 +24,7 @@ typedef Narrow<__nv_bfloat16> Part;
 struct PartsParams {
     AttnParams a;
     float scale_log2, scale;
-    int tiles;             // of 128 queries
+    int tiles;             // of 256 queries forward, 128 backward
     unsigned key_blocks;   // backward: blocks of the keys walk, before those of the queries walk
 };
 
@@ -145,45 +145,61 @@ __device__ __forceinline__ void store_rows(float *to, long long row_stride, unsi
 }
 
 // ---- forward ----
-// A CTA has 128 queries, a row to a thread, and walks over key tiles; two CTAs to an SM, so that one's tensor-core work runs beside the other's
-// exponentials.  The next tile's scores are formed while this one's are worked on.
-constexpr int kForwardThreads = 192;
+// A CTA has two tiles of 128 queries, a row to a thread of either warpgroup, and a warp each that issues its MMAs; the key tiles come once for both,
+// through a ring.  While one tile's threads form probabilities the tensor cores work for the other, and the next scores are formed while these are worked on.
+// (A CTA per query tile, two to an SM, with room for one K and one V each, waited for them: 60 us where this takes 40, [4, 1024, 8, 64].)
 struct ForwardPartsSmem {
-    static constexpr uint32_t OFF_K = 3 * OWN_PART, OFF_V = OFF_K + 3 * WALK_PART;
-    static constexpr uint32_t OFF_BAR = OFF_V + 3 * WALK_PART;
-    static constexpr uint32_t OFF_TMEM = OFF_BAR + 8 * 10;
+    static constexpr int kSlots = 5;
+    static constexpr uint32_t TILE_BYTES = 3 * WALK_PART;
+    static constexpr uint32_t OFF_RING = 6 * OWN_PART;
+    static constexpr uint32_t OFF_BAR = OFF_RING + kSlots * TILE_BYTES;
+    static constexpr uint32_t OFF_TMEM = OFF_BAR + 8 * (2 * kSlots + 11);
     static constexpr uint32_t ALLOC = OFF_TMEM + 16 + 1024;
-    static_assert(2 * (ALLOC + 1024) <= 233472, "two CTAs to an SM");
+    static_assert(ALLOC <= 232448, "exceeds the dynamic shared memory of one CTA");
 };
 
-__global__ void __launch_bounds__(kForwardThreads, 2)
+__global__ void __launch_bounds__(kTcThreads, 1)
 attention_forward_parts_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PartsParams F) {
     typedef ForwardPartsSmem L;
     const AttnParams &P = F.a;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *q_full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *k_full = q_full + 1, *k_empty = k_full + 1, *v_full = k_empty + 1, *v_empty = v_full + 1,
-             *s_full = v_empty + 1, *s_read = s_full + 1, *p_full = s_read + 1, *o_full = p_full + 1, *drained = o_full + 1;
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *empty = full + L::kSlots, *q_full = empty + L::kSlots, *s_full = q_full + 1, *o_full = s_full + 2,
+             *s_read = o_full + 2, *p_full = s_read + 2, *drained = p_full + 2;   // two of each: the query tiles'
     uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(smem + L::OFF_TMEM);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_TMEM + 4);
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const unsigned heads = (unsigned)(P.B * P.Hq), bh = blockIdx.x % heads;
-    const int row0 = (F.tiles - 1 - (int)(blockIdx.x / heads)) * TILE;   // a causal call's longest rows first
+    const int row0 = (F.tiles - 1 - (int)(blockIdx.x / heads)) * 2 * TILE;   // a causal call's longest rows first
     const int h = (int)(bh % (unsigned)P.Hq), b = (int)(bh / (unsigned)P.Hq), hk = h / (int)P.group;
     const Seen see(P, b);
-    const int nq = (int)P.Nq, last = (row0 + TILE < nq ? row0 + TILE : nq) - 1;
-    const int begin = see.lo(row0) / KEYS, end = (see.hi(last) + KEYS - 1) / KEYS, total = __shfl_sync(0xffffffffu, end > begin ? end - begin : 0, 0);
+    const int nq = (int)P.Nq;
+    // key tiles [lo, hi) of query tile s, the same in every lane
+    auto range = [&](int s, int &lo, int &hi) {
+        const int first = row0 + s * TILE, last = (first + TILE < nq ? first + TILE : nq) - 1;
+        lo = see.lo(first) / KEYS;
+        hi = first < nq ? (see.hi(last) + KEYS - 1) / KEYS : 0;
+        if (hi <= lo) lo = hi = 0;
+        lo = __shfl_sync(0xffffffffu, lo, 0);
+        hi = __shfl_sync(0xffffffffu, hi, 0);
+    };
+    int lo0, hi0, lo1, hi1;
+    range(0, lo0, hi0);
+    range(1, lo1, hi1);
+    const int begin = hi0 > 0 && (hi1 == 0 || lo0 < lo1) ? lo0 : lo1, end = hi0 > hi1 ? hi0 : hi1, total = end - begin;
 
     if (threadIdx.x == 0) {
-        for (uint64_t *bar = q_full; bar <= drained; ++bar) mbar_init(bar, bar == s_read || bar == p_full ? 4 : 1);
+        for (int i = 0; i < L::kSlots; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 2); }
+        mbar_init(q_full, 1);
+        for (int s = 0; s < 2; ++s) { mbar_init(&s_full[s], 1); mbar_init(&o_full[s], 1); mbar_init(&s_read[s], 4); mbar_init(&p_full[s], 4); mbar_init(&drained[s], 1); }
         *abort_flag = 0;
         mbar_init_fence();
         tma_prefetch_descriptor(&map_q);
         tma_prefetch_descriptor(&map_k);
         tma_prefetch_descriptor(&map_v);
     }
-    if (warp == 5) tmem_alloc(tmem_ptr, 256);
+    if (warp == 9) tmem_alloc(tmem_ptr, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -197,72 +213,92 @@ attention_forward_parts_kernel(const __grid_constant__ CUtensorMap map_q, const 
         if (!ok) give_up(site);
         return ok;
     };
-    const uint32_t q_at = smem_u32(smem), k_at = smem_u32(smem + L::OFF_K), v_at = smem_u32(smem + L::OFF_V);
-    const uint32_t S = tmem, Pr = tmem + KEYS, O = Pr + 3 * PART_COLUMNS;
+    const uint32_t q_at = smem_u32(smem), ring = smem_u32(smem + L::OFF_RING);
+    // of query tile s: scores, the probabilities' parts, the sums of a key tile
+    auto at_of = [&](int s, uint32_t &S, uint32_t &Pr, uint32_t &O) {
+        S = tmem + s * 256;
+        Pr = S + KEYS;
+        O = Pr + 3 * PART_COLUMNS;
+    };
 
-    if (warp == 4) {
+    if (warp >= 8) registers_down();
+    if (warp == 8) {
         if (lane == 0 && total > 0) {
-            uint32_t issued_k = 0, issued_v = 0;
-            mbar_expect_tx(q_full, 3 * OWN_PART);
+            uint32_t used = 0;
+            mbar_expect_tx(q_full, 6 * OWN_PART);
             load_parts<TILE>(q_at, &map_q, q_full, row0, h, b, (int)P.B);
-            auto load = [&](uint64_t *full, uint64_t *empty, uint32_t to, const CUtensorMap *map, int u, uint32_t &issued) {
-                if (u > 0 && !wait_or_abort(empty, (u & 1) ^ 1, abort_flag)) {
+            load_parts<TILE>(q_at + 3 * OWN_PART, &map_q, q_full, row0 + TILE, h, b, (int)P.B);
+            for (uint32_t u = 0; u < 2u * total; ++u) {   // K and V in turn
+                const uint32_t slot = u % L::kSlots;
+                if (u >= L::kSlots && !wait_or_abort(&empty[slot], parity_of_use(u, L::kSlots) ^ 1, abort_flag)) {
                     give_up(1);
-                    return false;
+                    break;
                 }
-                mbar_expect_tx(full, 3 * WALK_PART);
-                load_parts<KEYS>(to, map, full, (begin + u) * KEYS, hk, b, (int)P.B);
-                issued = u + 1;
-                return true;
-            };
-            for (int u = 0; u < total; ++u)
-                if (!load(k_full, k_empty, k_at, &map_k, u, issued_k) || !load(v_full, v_empty, v_at, &map_v, u, issued_v)) break;
-            if (!wait_for_releases(k_empty, issued_k, 1, abort_flag) || !wait_for_releases(v_empty, issued_v, 1, abort_flag)) give_up(2);
+                mbar_expect_tx(&full[slot], L::TILE_BYTES);
+                load_parts<KEYS>(ring + slot * L::TILE_BYTES, u & 1 ? &map_v : &map_k, &full[slot], (begin + (int)(u / 2)) * KEYS, hk, b, (int)P.B);
+                used = u + 1;
+            }
+            if (!wait_for_releases(empty, used, L::kSlots, abort_flag)) give_up(2);
             if (*abort_flag) {   // what was issued arrives before the CTA ends
                 mbar_wait_bounded(q_full, 0);
-                if (issued_k > 0) mbar_wait_bounded(k_full, (issued_k & 1) ^ 1);
-                if (issued_v > 0) mbar_wait_bounded(v_full, (issued_v & 1) ^ 1);
+                for (uint32_t u = first_of_last_uses(used, L::kSlots); u < used; ++u) mbar_wait_bounded(&full[u % L::kSlots], parity_of_use(u, L::kSlots));
             }
         }
-    } else if (warp == 5) {
+    } else if (warp == 9 || warp == 10) {
+        const int s = warp - 9, lo = s ? lo1 : lo0, hi = s ? hi1 : hi0;
         const uint32_t idesc_s = instruction_parts(KEYS, false), idesc_o = instruction_parts(KEYS, true);
         const uint32_t leader = elect_lane();
+        uint32_t S, Pr, O, done = 0;
+        at_of(s, S, Pr, O);
         bool ok = total == 0 || warp_wait(q_full, 0, 3);
-        auto scores = [&](int u) {
-            if (!warp_wait(k_full, u & 1, 4)) return false;
+        auto mine = [&](int t) { return lo <= t && t < hi; };
+        auto scores = [&](int t) {
+            const uint32_t u = 2 * (t - begin), slot = u % L::kSlots;
+            if (!warp_wait(&full[slot], parity_of_use(u, L::kSlots), 4)) return false;
             tc_fence_after();
-            parts_along_features(leader, S, q_at, k_at, idesc_s);
-            commit_by(leader, s_full);
-            commit_by(leader, k_empty);
+            if (mine(t)) {
+                parts_along_features(leader, S, q_at + s * 3 * OWN_PART, ring + slot * L::TILE_BYTES, idesc_s);
+                commit_by(leader, &s_full[s]);
+            }
+            commit_by(leader, &empty[slot]);
             return true;
         };
-        if (total > 0 && ok) ok = scores(0);
-        for (int u = 0; u < total && ok; ++u) {
-            if (u + 1 < total) {
-                if (!(ok = warp_wait(s_read, u & 1, 5))) break;
+        if (total > 0 && ok) ok = scores(begin);
+        for (int t = begin; t < end && ok; ++t) {
+            if (t + 1 < end) {
+                if (mine(t) && mine(t + 1) && !(ok = warp_wait(&s_read[s], done & 1, 5))) break;
                 tc_fence_after();
-                if (!(ok = scores(u + 1))) break;
+                if (!(ok = scores(t + 1))) break;
             }
-            if (!(ok = warp_wait(v_full, u & 1, 6) && warp_wait(p_full, u & 1, 7))) break;
-            tc_fence_after();
-            parts_along_tokens(leader, O, Pr, v_at, idesc_o);
-            commit_by(leader, o_full);
-            commit_by(leader, v_empty);
+            const uint32_t u = 2 * (t - begin) + 1, slot = u % L::kSlots;
+            if (!(ok = warp_wait(&full[slot], parity_of_use(u, L::kSlots), 6))) break;
+            if (mine(t)) {
+                if (!(ok = warp_wait(&p_full[s], done & 1, 7))) break;
+                tc_fence_after();
+                parts_along_tokens(leader, O, Pr, ring + slot * L::TILE_BYTES, idesc_o);
+                commit_by(leader, &o_full[s]);
+                ++done;
+            }
+            commit_by(leader, &empty[slot]);
         }
         __syncwarp();
-    } else {
-        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-        const int i = row0 + warp * 32 + lane, lo = see.lo(i), hi = i < nq ? see.hi(i) : 0;
-        const int all_lo = see.lo(last), all_hi = row0 + TILE > nq ? 0 : see.hi(row0);   // seen by every row of the tile
+    } else if (warp < 8) {
+        registers_up();
+        const int s = warp >> 2, first = row0 + s * TILE, last = (first + TILE < nq ? first + TILE : nq) - 1, t_first = s ? lo1 : lo0, mine = (s ? hi1 : hi0) - t_first;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const int i = first + (warp & 3) * 32 + lane, lo = see.lo(i), hi = i < nq ? see.hi(i) : 0;
+        const int all_lo = see.lo(last), all_hi = see.hi(first);   // seen by every row of the tile; rows beyond Nq are not stored
         const float c = F.scale_log2;
+        uint32_t S, Pr, O;
+        at_of(s, S, Pr, O);
         float m = -INFINITY, l = 0.f;
         f32x2 acc[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) acc[e] = pack2(0.f, 0.f);
         bool ok = true;
-        for (int u = 0; u < total; ++u) {
-            const int j0 = (begin + u) * KEYS;
-            if (!(ok = warp_wait(s_full, u & 1, 8))) break;
+        for (int u = 0; u < mine; ++u) {
+            const int j0 = (t_first + u) * KEYS;
+            if (!(ok = warp_wait(&s_full[s], u & 1, 8))) break;
             tc_fence_after();
             float p[KEYS];
 #pragma unroll
@@ -275,7 +311,7 @@ attention_forward_parts_kernel(const __grid_constant__ CUtensorMap map_q, const 
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(s_read);
+            if (lane == 0) mbar_arrive(&s_read[s]);
             if (j0 < all_lo || j0 + KEYS > all_hi) {
 #pragma unroll
                 for (int e = 0; e < KEYS; ++e)
@@ -300,7 +336,7 @@ attention_forward_parts_kernel(const __grid_constant__ CUtensorMap map_q, const 
             unpack2(sum, s0, s1);
             l = l * by + (s0 + s1);
             if (u > 0) {   // the last tile's product is over
-                if (!(ok = warp_wait(o_full, (u & 1) ^ 1, 9))) break;
+                if (!(ok = warp_wait(&o_full[s], (u & 1) ^ 1, 9))) break;
                 tc_fence_after();
             }
             put_parts(Pr + lanes, p);
@@ -308,32 +344,34 @@ attention_forward_parts_kernel(const __grid_constant__ CUtensorMap map_q, const 
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full);
+            if (lane == 0) mbar_arrive(&p_full[s]);
 #pragma unroll
             for (int e = 0; e < 32; ++e) acc[e] = mul2(acc[e], pack2(by, by));
         }
-        if (ok && total > 0) {
-            ok = warp_wait(o_full, (total & 1) ^ 1, 10);
+        if (ok && mine > 0) {
+            ok = warp_wait(&o_full[s], (mine & 1) ^ 1, 10);
             tc_fence_after();
         }
         if (ok) {
-            if (total > 0) add_tile(acc, O + lanes);
+            if (mine > 0) add_tile(acc, O + lanes);
             const float lse = l == 0.f ? -INFINITY : (m * c + log2f(l)) * 0.69314718055994531f;
             if (i < nq && P.lse) static_cast<float *>(P.lse)[bh * P.Nq + i] = lse;
             const int row = i - lane;
-            store_rows(static_cast<float *>(P.out) + ((b * P.Nq + row) * P.Hq + h) * P.D, P.Hq * P.D, smem + warp * 8192, acc, l == 0.f ? 0.f : 1.f / l, l != 0.f, lane, nq - row, (int)P.D);
+            // through the tile's own queries, which no product reads any more
+            store_rows(static_cast<float *>(P.out) + ((b * P.Nq + row) * P.Hq + h) * P.D, P.Hq * P.D, smem + s * 3 * OWN_PART + (warp & 3) * 8192, acc, l == 0.f ? 0.f : 1.f / l,
+                       l != 0.f, lane, nq - row, (int)P.D);
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 5) {
-        if (*abort_flag && lane == 0) {   // the commits behind all MMAs were waited for, or one more is waited for here
-            tc_commit<false>(drained);
-            mbar_wait_bounded(drained, 0);
-        }
-        __syncwarp();
+    if ((warp == 9 || warp == 10) && *abort_flag) {   // the commits behind all MMAs were waited for, or one more of each issuing lane is waited for here
+        commit_by(elect_lane(), &drained[warp - 9]);
+        mbar_wait_bounded(&drained[warp - 9], 0);
+    }
+    __syncthreads();
+    if (warp == 9) {
         tc_fence_after();
-        tmem_dealloc(tmem, 256);
+        tmem_dealloc(tmem, 512);
     }
 }
 
@@ -750,12 +788,13 @@ long long attn_parts_bytes(const AttnParams &P, bool backward) {
 int attn_parts_forward(const AttnParams &P, void *scratch, cudaStream_t s) {
     CUtensorMap maps[4];
     if (const int e = make_parts(P, 3, scratch, maps, s)) return e;
-    const PartsParams F = parts_params(P);
+    PartsParams F = parts_params(P);
+    F.tiles = (int)((P.Nq + 2 * TILE - 1) / (2 * TILE));
     const long long blocks = F.tiles * P.B * P.Hq;
     TPW_CHECK_ARG(blocks < (1LL << 31), "attention: more than 2^31 blocks of work");
     constexpr auto *kern = &attention_forward_parts_kernel;
     if (const int e = allow_shared_memory<kern>((int)ForwardPartsSmem::ALLOC)) return e;
-    kern<<<(unsigned)blocks, kForwardThreads, ForwardPartsSmem::ALLOC, s>>>(maps[0], maps[1], maps[2], F);
+    kern<<<(unsigned)blocks, kTcThreads, ForwardPartsSmem::ALLOC, s>>>(maps[0], maps[1], maps[2], F);
     TPW_LAUNCH_OK("attention_forward_parts_kernel");
     return TPW_OK;
 }
