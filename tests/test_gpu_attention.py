@@ -285,3 +285,15 @@ def test_many_blocks_of_every_kind_in_one_launch():
         for got, w, name in zip(torch.autograd.grad(out, leaves, q), want[2:], ("dq", "dk", "dv")):
             assert_near(got, w, torch.bfloat16, name, 2.0)
     assert tpw.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_query_tiles_without_keys_beside_tiles_with_keys(dtype):
+    """A sequence shorter than its queries: the first 192 rows see nothing, and their zeros must not be mixed up with queries on their way in."""
+    g = torch.Generator().manual_seed(13)
+    q, k, v = (torch.randn(64, n, 4, 64, generator=g).to(dtype).cuda() for n in (256, 160, 160))
+    n = torch.full((64,), 64, dtype=torch.int32, device="cuda")
+    for _ in range(10):
+        out, lse = tpw.attention(q, k, v, causal=True, key_lengths=n, return_lse=True)
+        assert not out[:, :192].any() and bool((lse[:, :, :192] == -math.inf).all())
+        assert bool((out[:, 192:] != 0).any(-1).all())

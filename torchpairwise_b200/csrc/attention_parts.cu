@@ -351,6 +351,8 @@ attention_forward_parts_kernel(const __grid_constant__ CUtensorMap map_q, const 
         if (ok && mine > 0) {
             ok = warp_wait(&o_full[s], (mine & 1) ^ 1, 10);
             tc_fence_after();
+        } else if (ok && total > 0) {
+            ok = warp_wait(q_full, 0, 11);   // its queries are not on their way any more where the zeros go through
         }
         if (ok) {
             if (mine > 0) add_tile(acc, O + lanes);
