@@ -5,6 +5,7 @@
 // per 16 keys and warp.  The keys are cut into ranges so that all SMs read; a range is one CTA: a warp issues TMA into a ring of 64-key stages,
 // four warps take 16 keys of a stage each, with a running maximum, sum and output of their own that meet only at the end.  Ranges
 // write outputs and log-sums that attention_join_kernel weighs together (skipped when there is one range).
+// Measured bfloat16 [16, 1 x 16384, 32/8, 128], ragged lengths: 591 MB in 100 us, 5.9 TB/s, and 5 us for the join.
 #include "attention_tc.cuh"
 
 namespace tpw {

@@ -446,7 +446,7 @@ bool attn_tc_fits(int dtype, const AttnParams &P) {
 
 // Ranges of keys for calls whose query tiles are fewer than two CTAs per SM: about three CTAs per SM, so that ragged sequences even
 // out, with at least four key tiles each, below which writing and joining the parts costs more than the keys.  bfloat16 [2, 256 x 16384, 32/8,
-// 128], lengths 16384 and 1638: 64 CTAs 260 us.
+// 128], lengths 16384 and 1638: 64 CTAs without ranges 260 us, with them 92 and 13 for the join.
 AttnSplits attn_tc_splits(const AttnParams &P) {
     AttnSplits r;
     const long long blocks = (P.Nq + 2 * TILE - 1) / (2 * TILE) * P.B * P.Hq, sms = sm_count(), key_tiles = (P.Nk + TILE - 1) / TILE;
