@@ -297,3 +297,44 @@ def test_query_tiles_without_keys_beside_tiles_with_keys(dtype):
         out, lse = tpw.attention(q, k, v, causal=True, key_lengths=n, return_lse=True)
         assert not out[:, :192].any() and bool((lse[:, :, :192] == -math.inf).all())
         assert bool((out[:, 192:] != 0).any(-1).all())
+
+
+@pytest.mark.parametrize("d", [4, 12, 20, 44, 60, 64])
+@pytest.mark.parametrize("causal", [False, True])
+def test_float32_widths_and_magnitudes(d, causal):
+    """Widths that are no multiple of eight, views of a packed projection, and operands far from 1 whose products are not: float32 keeps all of its
+    digits at every exponent."""
+    g = torch.Generator().manual_seed(14)
+    packed = torch.randn(2, 300, 4 + 2 + 2, d, generator=g).cuda()
+    packed[:, :, :4] *= 2.0 ** 60
+    packed[:, :, 4:6] *= 2.0 ** -60
+    packed[:, :, 6:] *= 2.0 ** -30
+    q, k, v = packed[:, :, :4], packed[:, :, 4:6], packed[:, :, 6:]
+    go = torch.randn(2, 300, 4, d, generator=g).cuda() * 2.0 ** 20
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    lengths = [300, 211]
+    n = torch.tensor(lengths, device="cuda")
+    out, lse = tpw.attention(*leaves, causal=causal, key_lengths=n, return_lse=True)
+    want = reference(q, k, v, causal=causal, lengths=lengths, grad=go)
+    assert_near(out, want[0], torch.float32, f"out {d} {causal}")
+    assert_near(lse, want[1], torch.float32, f"lse {d} {causal}")
+    for got, w, name in zip(torch.autograd.grad(out, leaves, go), want[2:], ("dq", "dk", "dv")):
+        assert_near(got, w, torch.float32, f"{name} {d} {causal}", 2.0)
+    assert tpw.device_status() == 0
+
+
+def test_float32_keys_that_are_not_used_may_hold_anything():
+    g = torch.Generator().manual_seed(15)
+    q, k, v = (torch.randn(2, 256, 2, 64, generator=g).cuda() for _ in range(3))
+    n = torch.tensor([256, 130], device="cuda")
+    grads = []
+    for fill in (0.0, float("nan"), float("inf")):
+        kk, vv = k.clone(), v.clone()
+        kk[1, 130:], vv[1, 130:] = fill, fill
+        leaves = [t.requires_grad_() for t in (q.clone(), kk, vv)]
+        out = tpw.attention(*leaves, key_lengths=n)
+        grads.append((out.detach(), *torch.autograd.grad(out, leaves, q)))
+    for other in grads[1:]:
+        for a, b in zip(grads[0], other):
+            assert torch.equal(a, b)
+    assert not grads[0][2][1, 130:].any() and not grads[0][3][1, 130:].any()

@@ -776,9 +776,10 @@ PartsParams parts_params(const AttnParams &P) {
 
 } // namespace
 
-// Against the tf32 products, kernels' times, forward and backward: [4, 1024, 8, 64] 200 and 637 -> 69 and 229 us, [32, 128, 12, 64] 46 and 145 ->
-// 34 and 115.  Tiles of 128 rows: 64 tokens ([16, 64, 12, 64] 10 and 30 -> 13 and 39 us) leave them half empty, and forward the parts cost more than they
-// save up to [8, 77, 8, 64] (11.4 -> 12.6; backward 31 -> 21).  A forward call of few rows goes by ranges of keys (attn_f32_splits), which this kernel has not.
+// Against the tf32 products, all kernels of a call, forward and backward: [4, 1024, 8, 64] 200 and 637 -> 58 and 199 us, causal [1, 4096, 8, 64] 369 and 1263 ->
+// 161 and 339, [32, 128, 12, 64] 46 and 145 -> 41 and 101.  64 tokens ([16, 64, 12, 64] 10 and 30 -> 13 and 39 us) leave tiles of 128 rows half empty, and
+// forward the parts cost what they save at [8, 77, 8, 64] (11.4 -> 12.6; backward 31 -> 19).  A forward call of few rows goes by ranges of keys
+// (attn_f32_splits), which this kernel has not.
 static bool parts_fit(int dtype, const AttnParams &P, long long tokens) {
     const long long limit = 1LL << 34;   // numbers of 16-byte pieces stay below 2^31
     return P.D <= 64 && P.Nq >= tokens && P.Nk >= tokens && !tma_disabled() && P.B * P.Nq * P.Hq * row_features(P) < limit && P.B * P.Nk * P.Hk * row_features(P) < limit &&
