@@ -1,0 +1,78 @@
+"""The order that barriers give the 16-bit gradients' keys walk, from its source: a stage of shared memory is written anew only when every
+row warp has read what lies in it."""
+import re
+from pathlib import Path
+
+import pytest
+
+SOURCE = Path(__file__).resolve().parent.parent / "torchpairwise_b200" / "csrc" / "attention_backward.cu"
+
+
+def keys_walk():
+    text = SOURCE.read_text()
+    return text[text.index("void keys_walk("):text.index("void queries_walk(")]
+
+
+def section(text, first, last):
+    start = text.index(first)
+    return text[start:text.index(last, start)]
+
+
+def orders(text, tiles=12, stages=2):
+    """Edges a -> b, "a is over before b starts", of the walk as the source has it, and the ring that each row's term comes with."""
+    producer = section(text, "if (warp == 8) {", "} else if (warp == 9) {")
+    issuer = section(text, "for (int u = 0; u < total && ok; ++u) {", "if (ok && total > 0) commit_by(leader, acc_full);")
+    rows = section(text, "const float *rows = reinterpret_cast<const float *>(smem + L::OFF_ROWS", "hand_over(p, dp_at, ds_ready);")
+    # the ring that brings each term: the `load` that is given it, or is told (true) to bring both
+    calls = re.findall(r"load\((q|g)_full, ([^()]*)\)", producer)
+    ring = {term: next(name for name, rest in calls if f"P.row_{term}" in rest or " true," in rest) for term in ("lse", "delta")}
+    # what the issuing warp does in an iteration, in its order
+    steps = re.findall(r"warp_wait\((p_ready|ds_ready)|product_tokens\(leader, (DV|DK)|commit_by\(leader, &(q|g)_empty", issuer)
+    steps = [next(x for x in s if x) for s in steps]
+    released_after = {}   # ring -> the row warps' arrivals that its release comes after
+    waited = []
+    for s in steps:
+        if s in ("p_ready", "ds_ready"):
+            waited.append(s)
+        elif s in ("q", "g"):
+            released_after[s] = list(waited)
+    # where the row warps read the terms: before or after they say that P is there
+    read_before = {"lse": "p_ready" if rows.index("rows + 8 * i") < rows.index("p_ready") else "ds_ready",
+                   "delta": "p_ready" if rows.index("rows + TILE + 8 * i") < rows.index("hand_over(p, s_at, p_ready)") else "ds_ready"}
+    edges = {}
+
+    def edge(a, b):
+        edges.setdefault(a, set()).add(b)
+
+    for u in range(tiles):
+        for term in ("lse", "delta"):
+            edge(("read", term, u), (read_before[term], u))
+        for name in ("q", "g"):
+            for arrival in released_after[name]:
+                edge((arrival, u), ("empty", name, u))
+            edge(("empty", name, u), ("copy", name, u + stages))
+        edge(("p_ready", u), ("ds_ready", u))           # a row warp's own order
+        edge(("ds_ready", u), ("read", "lse", u + 1))
+    return edges, ring
+
+
+def reaches(edges, a, b):
+    todo, seen = [a], set()
+    while todo:
+        at = todo.pop()
+        if at == b:
+            return True
+        for x in edges.get(at, ()):
+            if x not in seen:
+                seen.add(x)
+                todo.append(x)
+    return False
+
+
+@pytest.mark.parametrize("stages", [2, 4])
+@pytest.mark.parametrize("term", ["lse", "delta"])
+def test_a_tile_s_row_terms_are_read_before_their_stage_is_written_anew(term, stages):
+    edges, ring = orders(keys_walk(), stages=stages)
+    for u in range(4):
+        assert reaches(edges, ("read", term, u), ("copy", ring[term], u + stages)), \
+            f"{term} of tile {u} may still be read when tile {u + stages} is copied over it (it comes with ring {ring[term]})"

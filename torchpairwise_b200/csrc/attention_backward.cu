@@ -171,24 +171,27 @@ __device__ __forceinline__ void keys_walk(const CUtensorMap &map_q, const CUtens
             mbar_expect_tx(kv_full, 2 * L::TILE_BYTES);
             load_tokens<BLOCKS>(k_at, &map_k, kv_full, row0, hk, b);
             load_tokens<BLOCKS>(v_at, &map_v, kv_full, row0, hk, b);
-            auto load = [&](uint64_t *full, uint64_t *empty, uint32_t ring, const CUtensorMap *map, const void *terms, uint32_t terms_at, uint32_t u, uint32_t &issued) {
+            auto load = [&](uint64_t *full, uint64_t *empty, uint32_t ring, const CUtensorMap *map, bool terms, uint32_t u, uint32_t &issued) {
                 const uint32_t st = u % L::kStages;
                 if (u >= L::kStages && !wait_or_abort(&empty[st], parity_of_use(u, L::kStages) ^ 1, abort_flag)) {
                     give_up(1);
                     return false;
                 }
                 const int h = hk * (int)P.group + u / per_head, i0 = (begin + u % per_head) * TILE;
-                mbar_expect_tx(&full[st], L::TILE_BYTES + TILE * 4);
+                mbar_expect_tx(&full[st], L::TILE_BYTES + (terms ? 2 * TILE * 4 : 0));
                 load_tokens<BLOCKS>(ring + st * L::TILE_BYTES, map, &full[st], i0, h, b);
-                bulk_load(terms_at + st * 2 * TILE * 4, static_cast<const float *>(terms) + (b * P.Hq + h) * P.Nqp + i0, TILE * 4, &full[st]);
+                if (terms) {
+                    const long long from = (b * P.Hq + h) * P.Nqp + i0;
+                    bulk_load(rows_at + st * 2 * TILE * 4, static_cast<const float *>(P.row_lse) + from, TILE * 4, &full[st]);
+                    bulk_load(rows_at + (2 * st + 1) * TILE * 4, static_cast<const float *>(P.row_delta) + from, TILE * 4, &full[st]);
+                }
                 issued = u + 1;
                 return true;
             };
-            // a gradient tile is free after dV, a query tile only after dK: the gradients are fetched first
+            // A gradient tile is free after dV, a query tile only after dK: the gradients are fetched first.  The row terms come with the queries: the
+            // row warps read delta until they arrive at ds_ready, for which dK waits and dV does not.
             for (int u = 0; u < total; ++u)
-                if (!load(g_full, g_empty, g_ring, &map_g, P.row_delta, rows_at + TILE * 4, u, issued_g) ||
-                    !load(q_full, q_empty, q_ring, &map_q, P.row_lse, rows_at, u, issued_q))
-                    break;
+                if (!load(g_full, g_empty, g_ring, &map_g, false, u, issued_g) || !load(q_full, q_empty, q_ring, &map_q, true, u, issued_q)) break;
             if (!wait_for_releases(q_empty, issued_q, L::kStages, abort_flag) || !wait_for_releases(g_empty, issued_g, L::kStages, abort_flag)) give_up(2);
             if (*abort_flag) {   // what was issued arrives before the CTA ends
                 mbar_wait_bounded(kv_full, 0);
@@ -299,7 +302,7 @@ __device__ __forceinline__ void keys_walk(const CUtensorMap &map_q, const CUtens
             }
             if (masked) hide(p, i0);
             hand_over(p, s_at, p_ready);
-            if (!(ok = warp_wait(dp_full, u & 1, 10) && warp_wait(&g_full[st], parity_of_use(u, L::kStages), 11))) break;
+            if (!(ok = warp_wait(dp_full, u & 1, 10))) break;
             tc_fence_after();
             tmem_ld_16x256(dp_at, x[0]);
             tmem_ld_16x256(dp_at + upper, x[1]);
