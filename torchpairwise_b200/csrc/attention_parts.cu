@@ -293,7 +293,7 @@ attention_forward_parts_kernel(const __grid_constant__ CUtensorMap map_q, const 
         const float c = F.scale_log2;
         uint32_t S, Pr, O;
         at_of(s, S, Pr, O);
-        float m = -INFINITY, l = 0.f;
+        float m = -INFINITY, l = 0.f, shift = 0.f;
         f32x2 acc[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) acc[e] = pack2(0.f, 0.f);
@@ -325,7 +325,11 @@ attention_forward_parts_kernel(const __grid_constant__ CUtensorMap map_q, const 
 #pragma unroll
                 for (int g = 0; g < 4; ++g) tops[g] = max3_nan(tops[g], p[e + 2 * g], p[e + 2 * g + 1]);
             const float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
-            const float shift = top == -INFINITY ? 0.f : -top * c, by = top == -INFINITY ? 1.f : exp2_fast(m * c + shift);
+            // Sums are relative to 2^-shift, so what they are scaled by is the quotient of two such powers: exactly 1 while the maximum stays.  (With m c formed
+            // anew in a fused multiply-add it was off by the rounding of top c in every tile, all to one side.)
+            const float before = shift;
+            shift = top == -INFINITY ? 0.f : __fmul_rn(-top, c);
+            const float by = m == -INFINITY ? 1.f : exp2_fast(shift - before);   // nothing seen before: sums are zero
             m = top;
             f32x2 sum = pack2(0.f, 0.f);
 #pragma unroll
@@ -358,7 +362,7 @@ attention_forward_parts_kernel(const __grid_constant__ CUtensorMap map_q, const 
         }
         if (ok) {
             if (mine > 0) add_tile(acc, O + lanes);
-            const float lse = l == 0.f ? -INFINITY : (m * c + log2f(l)) * 0.69314718055994531f;
+            const float lse = l == 0.f ? -INFINITY : (log2f(l) - shift) * 0.69314718055994531f;
             if (i < nq && P.lse) static_cast<float *>(P.lse)[bh * P.Nq + i] = lse;
             const int row = i - lane;
             // through the tile's own queries, which no product reads any more
