@@ -59,6 +59,13 @@ Tensor fresh(at::IntArrayRef sizes, const Tensor &like, at::ScalarType type) {
 }
 Tensor fresh(at::IntArrayRef sizes, const Tensor &like) { return fresh(sizes, like, like.scalar_type()); }
 
+// Forward-mode derivatives have no rule here.  A tensor that carries a tangent need not require a gradient, so without this the result would have
+// none and count as constant.
+void no_tangents(const char *name, std::initializer_list<const Tensor *> tensors) {
+    for (const Tensor *t : tensors)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), name, ": forward-mode derivatives are not provided");
+}
+
 bool wants_node(std::initializer_list<const Tensor *> tensors) {
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor *t : tensors)
@@ -145,6 +152,7 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list go) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "attention: gradients of gradients are not provided");
+        no_tangents("attention", {&go[0], &go[1]});
         NvtxRange range("torchpairwise_b200::attention_backward");
         auto s = ctx->get_saved_variables();
         const bool unbatched = s[0].dim() == 3;
@@ -212,6 +220,7 @@ std::tuple<Tensor, Tensor> attention(const Tensor &q, const Tensor &k, const Ten
         TORCH_CHECK(n.numel() == batch && n.dim() <= 1, "key_lengths must hold one length for each of the ", batch, " sequences. Got shape ", n.sizes());
         lengths = n.scalar_type() == at::kInt ? n.contiguous() : n.clamp(0, k.size(f - 2)).to(at::kInt).contiguous();
     }
+    no_tangents("attention", {&q, &k, &v});
     if (!wants_node({&q, &k, &v})) {   // serving: no node, 2 us less
         at::AutoDispatchBelowADInplaceOrView guard;
         auto r = attention_forward(q, k, v, lengths, causal, window.value_or(0), c, nullptr);
@@ -290,6 +299,7 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
         return g;
     }
     static variable_list turn(const Tensor &q, const OptTensor &k, const Tensor &cos, const Tensor &sin, const OptTensor &positions, bool interleaved, bool inverse) {
+        no_tangents("rotary_embedding", {&q, k.has_value() ? &*k : &q, &cos, &sin});
         if (wants_node({&q, k.has_value() ? &*k : &q})) return apply(q, k, cos, sin, positions, interleaved, inverse);
         at::AutoDispatchBelowADInplaceOrView guard;
         return rotary_forward(q, k, cos, sin, positions, interleaved, inverse);
