@@ -77,3 +77,14 @@ def test_the_body_of_a_custom_operator():
     assert torch.equal(got, want)
     for a, b in zip(torch.autograd.grad(got, leaves, g), torch.autograd.grad(want, leaves, g)):
         assert torch.equal(a, b)
+
+
+def test_frequencies_of_a_table_receive_no_gradient():
+    f = torch.ones(4, dtype=torch.float64, device="cuda", requires_grad=True)
+    table = torch.ops.torchpairwise_b200.rotary_table
+    with pytest.raises(RuntimeError, match="no gradient"):
+        table(f, 3)
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        table(forward_ad.make_dual(f.detach(), torch.ones(4, dtype=torch.float64, device="cuda")), 3)
+    with torch.no_grad():
+        assert torch.equal(table(f, 3)[0], table(f.detach(), 3)[0])

@@ -353,6 +353,8 @@ std::tuple<Tensor, Tensor> rotary_table(const Tensor &frequencies, int64_t lengt
     require_cuda(frequencies);
     TORCH_CHECK(frequencies.scalar_type() == at::kDouble && frequencies.dim() == 1, "rotary_table: frequencies must be a float64 vector");
     TORCH_CHECK(length >= 0, "rotary_table: negative length");
+    TORCH_CHECK(!(at::GradMode::is_enabled() && frequencies.requires_grad()), "rotary_table: the frequencies receive no gradient");
+    no_tangents("rotary_table", {&frequencies});
     c10::cuda::CUDAGuard dg(frequencies.device());
     const Tensor f = frequencies.contiguous();
     Tensor cos = at::empty({length, f.size(0)}, f.options().dtype(at::kFloat)), sin = at::empty_like(cos);
