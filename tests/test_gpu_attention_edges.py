@@ -27,3 +27,45 @@ def test_float32_weights_of_early_keys_do_not_drift(causal, keys, queries, heads
     for got, w, name in zip(torch.autograd.grad(out, leaves, go), want[2:], ("dq", "dk", "dv")):
         assert_near(got, w, torch.float32, name, 2.0)
     assert tpw.device_status() == 0
+
+
+@pytest.mark.parametrize("bad", [None, float("inf"), float("nan")])
+@pytest.mark.parametrize("heads", [(2, 2), (4, 2)])
+def test_half_precision_gradients_of_a_sequence_are_its_own(bad, heads):
+    """Sequences and heads whose gradients and values are 2^23 times another's, or not finite, change no bit of that other's gradients and cost it no
+    digits."""
+    g = torch.Generator().manual_seed(22)
+    hq, hk = heads
+    q, k, v, go = (torch.randn(2, 160, h, 64, generator=g) for h in (hq, hk, hk, hq))
+    small = -9 if bad is None else 5   # with 2^5 a gradient of a score is above half precision's 65504 unless it is scaled down
+    go[0] *= 2.0 ** 8
+    v[0] *= 2.0 ** 6
+    go[1] *= 2.0 ** small
+    go[1, :, :hq // 2] *= 2.0 ** 8     # heads of the same sequence are apart too
+    if bad is not None:
+        go[0] = bad
+    args = [t.half().cuda() for t in (q, k, v)]
+    go = go.half().cuda()
+    leaves = [t.requires_grad_() for t in args]
+    both = torch.autograd.grad(tpw.attention(*leaves), leaves, go)
+    alone = [t.detach()[1:].clone().requires_grad_() for t in args]
+    single = torch.autograd.grad(tpw.attention(*alone), alone, go[1:])
+    want = reference(*alone, grad=go[1:])
+    for got, other, w, name in zip(both, single, want[2:], ("dq", "dk", "dv")):
+        assert torch.equal(got[1:], other), name
+        half = w.shape[2] // 2
+        for part in (slice(0, half), slice(half, None)):
+            assert_near(got[1:, :, part], w[:, :, part], torch.float16, name, 2.0)
+
+
+def test_half_precision_query_heads_do_not_depend_on_one_another():
+    """An infinite gradient in one query head leaves the gradient of the queries of another alone, though they share keys."""
+    g = torch.Generator().manual_seed(23)
+    q, k, v, go = (torch.randn(1, 200, h, 64, generator=g).half().cuda() for h in (2, 1, 1, 2))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    go = go * 2.0 ** 6
+    bad = go.clone()
+    bad[:, 3, 1] = float("inf")
+    out = tpw.attention(*leaves)
+    a, b = (torch.autograd.grad(out, q, x, retain_graph=True)[0] for x in (go, bad))
+    assert torch.equal(a[:, :, 0], b[:, :, 0]) and bool(torch.isfinite(a).all())

@@ -22,7 +22,7 @@ struct AttnParams {
     // backward: rows of the pitch Nqp, [B, Hq, Nqp], of what a walk over the queries needs (attention_rows_kernel)
     void *row_lse, *row_delta;
     long long Nqp;
-    const unsigned *row_max;                     // 16-bit floats of half precision: largest |dO_i|^2 and |v_j|^2 as float bits
+    unsigned *row_max;                           // half precision on the tensor cores: largest |dO_i|^2, |dlse_i| and |v_j|^2 (attention_rows.cu)
     int *status;
 };
 

@@ -31,15 +31,21 @@ struct BackwardParams {
 };
 
 // Half precision: probabilities are lifted by 2^12 and gradients of scores by another power of two (attention_rows.cu), both undone in
-// the epilogue; the largest of either is then 2^12 and 2^15.
+// the epilogue; the largest of either is then 2^12 and 2^15.  factor: of the query heads [h, h + heads) of key head hk.
 template <typename T> struct Lift {
     static constexpr bool kNeeded = false;
-    static __device__ __forceinline__ float factor(const unsigned *) { return 1.f; }
+    static __device__ __forceinline__ float factor(const AttnParams &, int, int, int, int) { return 1.f; }
 };
 template <> struct Lift<__half> {
     static constexpr bool kNeeded = true;
-    static __device__ __forceinline__ float factor(const unsigned *row_max) {
-        const float most = 2.f * sqrtf(__uint_as_float(row_max[0])) * sqrtf(__uint_as_float(row_max[1])) + __uint_as_float(row_max[2]);
+    static __device__ __forceinline__ float factor(const AttnParams &P, int b, int h, int heads, int hk) {
+        const unsigned *rows = P.row_max + 2 * (b * P.Hq + h);
+        unsigned top = 0, more = 0;
+        for (int g = 0; g < heads; ++g) {
+            top = max(top, rows[2 * g]);
+            more = max(more, rows[2 * g + 1]);
+        }
+        const float most = 2.f * sqrtf(__uint_as_float(top)) * sqrtf(__uint_as_float(P.row_max[2 * P.B * P.Hq + b * P.Hk + hk])) + __uint_as_float(more);
         if (!(most > 0.f) || !(most < INFINITY)) return 1.f;
         const float e = floorf(3.f - log2f(most));
         return exp2f(e < -100.f ? -100.f : e > 100.f ? 100.f : e);
@@ -240,7 +246,7 @@ __device__ __forceinline__ void keys_walk(const CUtensorMap &map_q, const CUtens
         const uint32_t s_at = S + lanes + 64 * half, dp_at = DP + lanes + 64 * half;
         // query tiles from all_lo on, and below all_hi, are seen by every key of the tile; keys beyond the length are not stored
         const int all_lo = see.qlo(row0 + TILE - 1), all_hi = see.window ? row0 - see.off + see.window : 0x7fffffff;
-        const float c = F.scale_log2, lift = Lift<T>::factor(P.row_max);
+        const float c = F.scale_log2, lift = Lift<T>::factor(P, b, hk * (int)P.group, (int)P.group, hk);
         const f32x2 c2 = pack2(c, c), lift2 = pack2(lift, lift);
         // index 2 i + r of a half's 16 pairs: columns 8 i + 2 t and the next, row g + 8 r (and 16 in the upper half)
         auto hide = [&](f32x2 (&p)[2][16], int i0) {
@@ -478,7 +484,7 @@ __device__ __forceinline__ void queries_walk(const CUtensorMap &map_q, const CUt
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const int lo = see.lo(i), hi = i < nq ? see.hi(i) : 0;
         const int all_lo = see.lo(last), all_hi = see.hi(row0);   // seen by every query of the tile
-        const float c = F.scale_log2, lift = Lift<T>::factor(P.row_max);
+        const float c = F.scale_log2, lift = Lift<T>::factor(P, b, h, 1, hk);
         const float lse = static_cast<const float *>(P.row_lse)[bh * P.Nqp + i], delta = static_cast<const float *>(P.row_delta)[bh * P.Nqp + i];
         const f32x2 c2 = pack2(c, c), lift2 = pack2(lift, lift), minus_lse = pack2(lse, lse), minus_delta = pack2(delta, delta);
         bool ok = true;
