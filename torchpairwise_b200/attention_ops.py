@@ -15,14 +15,32 @@ from ._abi import LIB_PATH
 
 ATTENTION_OPS_LIBRARY = LIB_PATH.parent / "libtpw_b200_attention.so"
 
-if not ATTENTION_OPS_LIBRARY.exists():
-    raise ImportError(f"{ATTENTION_OPS_LIBRARY} is missing; run `python torchpairwise_b200/build.py`")
-torch.ops.load_library(str(ATTENTION_OPS_LIBRARY))
-_ops = torch.ops.torchpairwise_b200
-_attention, _rotary_one, _rotary_two, _table = _ops.attention.default, _ops.rotary_embedding.default, _ops.rotary_embedding.pair, _ops.rotary_table.default
+_attention = _rotary_one = _rotary_two = _table = None
+
+
+def _load() -> None:
+    global _attention, _rotary_one, _rotary_two, _table
+    if not ATTENTION_OPS_LIBRARY.exists():
+        raise ImportError(f"{ATTENTION_OPS_LIBRARY} is missing; run `python torchpairwise_b200/build.py`")
+    try:
+        torch.ops.load_library(str(ATTENTION_OPS_LIBRARY))
+    except OSError as e:
+        raise ImportError(f"{ATTENTION_OPS_LIBRARY} does not load with torch {torch.__version__}; run `python torchpairwise_b200/build.py`") from e
+    ops = torch.ops.torchpairwise_b200
+    _attention, _rotary_one, _rotary_two, _table = ops.attention.default, ops.rotary_embedding.default, ops.rotary_embedding.pair, ops.rotary_table.default
+
+
+# The distances need only the kernel library, so a tree without this one, or with one built against another torch, imports all the same: what is
+# missing is said by the functions that need it.
+try:
+    _load()
+except ImportError:
+    pass
 
 
 def _check(name: str, q: Tensor) -> None:
+    if _attention is None:
+        _load()
     if not q.is_cuda:
         raise RuntimeError(f"torchpairwise_b200 runs on CUDA tensors only (no CPU path); got a tensor on {q.device}")
     if torch._C._are_functorch_transforms_active():
@@ -108,4 +126,6 @@ def rotary_table(length: int, features: int, *, base: float = 10000.0, scaling: 
         freq = [f * (1.0 - t) + f / factor * t for f, t in zip(freq, blend)]
     elif scaling not in (None, "base"):
         raise ValueError(f"rotary_table: scaling must be None, 'linear', 'base' or 'bands'. Got {scaling!r}")
+    if _table is None:
+        _load()
     return _table(torch.tensor(freq, dtype=torch.float64, device=device), length, magnitude)
