@@ -69,7 +69,7 @@ def _obj_stale(src: Path, obj: Path) -> bool:
     if not obj.exists():
         return True
     t = obj.stat().st_mtime
-    return any(p.stat().st_mtime > t for p in [src, *_included(src)])
+    return any(p.stat().st_mtime > t for p in [src, *_included(src), Path(__file__)])   # this file has the compiler's flags
 
 
 def _compile_one(nvcc: str, src: Path, verbose: bool, force: bool) -> tuple[Path, str]:
