@@ -208,7 +208,7 @@ attention_forward_parts_kernel(const __grid_constant__ CUtensorMap map_q, const 
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
     auto give_up = [&](int site) {
         *abort_flag = 1;
-        if (P.status) atomicCAS(P.status, 0, (19 << 16) | site);
+        if (P.status) atomicCAS(P.status, 0, (22 << 16) | site);
     };
     auto warp_wait = [&](uint64_t *bar, uint32_t parity, int site) {
         const bool ok = __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag));
