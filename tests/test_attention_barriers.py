@@ -76,3 +76,17 @@ def test_a_tile_s_row_terms_are_read_before_their_stage_is_written_anew(term, st
     for u in range(4):
         assert reaches(edges, ("read", term, u), ("copy", ring[term], u + stages)), \
             f"{term} of tile {u} may still be read when tile {u + stages} is copied over it (it comes with ring {ring[term]})"
+
+
+@pytest.mark.parametrize("name", ["attention_forward.cu", "attention_backward.cu", "attention_parts.cu"])
+def test_what_is_drained_after_a_wait_that_gave_up_is_committed_by_the_lane_that_issued_it(name):
+    """A commit covers what its own thread issued.  The products are issued by the elected lane, so the commit behind which tensor memory is given back
+    must be the elected lane's too, whichever that is."""
+    text = (SOURCE.parent / name).read_text()
+    issued = re.findall(r"(?:product_features<BLOCKS>|product_tokens(?:<\d, \d>)?|parts_along_\w+)\((\w+),", text)
+    assert issued and set(issued) <= {"leader", "uint32_t"}, issued
+    assert re.search(r"leader = elect_lane\(\)", text)
+    drains = re.findall(r"if \([^;{}]*?\*abort_flag[^;{}]*?\) \{[^{}]*?drained[^{}]*?\}", text)
+    assert len(drains) == (1 if name == "attention_forward.cu" else 2)
+    for block in drains:
+        assert "commit_by(elect_lane()," in block and "tc_commit" not in block and "lane == 0" not in block, block

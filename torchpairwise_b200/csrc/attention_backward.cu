@@ -343,8 +343,8 @@ __device__ __forceinline__ void keys_walk(const CUtensorMap &map_q, const CUtens
     tc_fence_before();
     __syncthreads();
     if (warp == 9) {
-        if (*abort_flag && lane == 0) {   // the commits behind all MMAs were waited for, or one more is waited for here
-            tc_commit<false>(drained);
+        if (*abort_flag) {   // the commits behind all MMAs were waited for, or one more is waited for here
+            commit_by(elect_lane(), drained);   // of the lane that issued them
             mbar_wait_bounded(drained, 0);
         }
         __syncwarp();
@@ -554,8 +554,8 @@ __device__ __forceinline__ void queries_walk(const CUtensorMap &map_q, const CUt
     tc_fence_before();
     __syncthreads();
     if (warp == 9) {
-        if (*abort_flag && lane == 0) {
-            tc_commit<false>(drained);
+        if (*abort_flag) {
+            commit_by(elect_lane(), drained);   // of the lane that issued them
             mbar_wait_bounded(drained, 0);
         }
         __syncwarp();

@@ -387,8 +387,8 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     __syncthreads();
     if (warp == 9) {
         // all MMAs are over: the commits behind them were waited for, or, after a wait that gave up, one more is waited for here
-        if (*abort_flag && lane == 0) {
-            tc_commit<false>(drained);
+        if (*abort_flag) {
+            commit_by(elect_lane(), drained);   // of the lane that issued them
             mbar_wait_bounded(drained, 0);
         }
         __syncwarp();
