@@ -69,3 +69,34 @@ def test_half_precision_query_heads_do_not_depend_on_one_another():
     out = tpw.attention(*leaves)
     a, b = (torch.autograd.grad(out, q, x, retain_graph=True)[0] for x in (go, bad))
     assert torch.equal(a[:, :, 0], b[:, :, 0]) and bool(torch.isfinite(a).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("d", [33, 64, 128, 200])
+@pytest.mark.parametrize("queries", [8, 300])
+def test_rows_that_see_nothing_are_zero_whatever_others_see(dtype, d, queries):
+    """Half of the rows are before the first key, keys before the first window are seen by no row, and what stands beside either is not finite."""
+    g = torch.Generator().manual_seed(24)
+    q, k, v, go = (torch.randn(1, n, 2, d, generator=g).to(dtype).cuda() for n in (queries, 200, 200, queries))
+    seeing = queries // 2
+    n = torch.tensor([seeing], dtype=torch.int32, device="cuda")
+    empty = queries - seeing
+    for bad in (float("inf"), float("nan")):
+        for where in ("k", "v"):
+            kk, vv = k.clone(), v.clone()
+            (kk if where == "k" else vv)[:, 0] = bad
+            leaves = [t.detach().requires_grad_() for t in (q, kk, vv)]
+            out, lse = tpw.attention(*leaves, causal=True, key_lengths=n, return_lse=True)
+            dq, = torch.autograd.grad(out, leaves[0], go)
+            assert not out[:, :empty].any() and not dq[:, :empty].any() and bool((lse[:, :, :empty] == -float("inf")).all()), (bad, where)
+            assert bool(torch.isnan(out[:, empty:]).any() or torch.isinf(out[:, empty:]).any())
+        few = min(queries, 50)
+        unseen = 200 - few - 20 + 1   # keys that end before the first query's window of 20
+        for where in ("q", "go"):
+            qq, gg = q[:, :few].clone(), go[:, :few].clone()
+            (qq if where == "q" else gg)[:, 0] = bad
+            leaves = [t.detach().requires_grad_() for t in (qq, k, v)]
+            out = tpw.attention(*leaves, causal=True, window=20)
+            dk, dv = torch.autograd.grad(out, leaves[1:], gg)
+            assert not dk[:, :unseen].any() and not dv[:, :unseen].any(), (bad, where)
+    assert tpw.device_status() == 0

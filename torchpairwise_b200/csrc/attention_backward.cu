@@ -89,9 +89,10 @@ __device__ __forceinline__ f32x2 score_gradient(f32x2 p, f32x2 dp, f32x2 minus_d
 }
 
 // A warp's 32 rows of an accumulator to global memory, this warpgroup's half of the columns, through shared memory that is no longer in use.
-// Rows from `keep` on are zero, rows from `valid` on are not there.
+// A lane whose row is not to `keep` (nothing is seen from there, or nobody sees it) writes zeros, although its sums are 0 times what need not be
+// finite; rows from `valid` on are not there.
 template <typename T, int BLOCKS>
-__device__ __forceinline__ void store_half(T *rows, long long row_stride, uint32_t acc, unsigned char *smem, int warp, int lane, int half, float by, int keep, int valid, int D) {
+__device__ __forceinline__ void store_half(T *rows, long long row_stride, uint32_t acc, unsigned char *smem, int warp, int lane, int half, float by, bool keep, int valid, int D) {
     const RowStage<4 * BLOCKS> stage = {reinterpret_cast<uint4 *>(smem) + warp * 128 * BLOCKS};
     const int first = half * 32 * BLOCKS;
 #pragma unroll 1
@@ -104,7 +105,7 @@ __device__ __forceinline__ void store_half(T *rows, long long row_stride, uint32
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                w[e] = lane < keep ? Narrow<T>::pack(__uint_as_float(o[8 * k + 2 * e]) * by, __uint_as_float(o[8 * k + 2 * e + 1]) * by) : 0u;
+                w[e] = keep ? Narrow<T>::pack(__uint_as_float(o[8 * k + 2 * e]) * by, __uint_as_float(o[8 * k + 2 * e + 1]) * by) : 0u;
             stage.put(lane, 4 * g + k, w[0], w[1], w[2], w[3]);
         }
     }
@@ -333,7 +334,8 @@ __device__ __forceinline__ void keys_walk(const CUtensorMap &map_q, const CUtens
             tc_fence_after();
         }
         if (ok) {
-            const int row = row0 + (warp & 3) * 32, keep = total > 0 ? see.length - row : 0, valid = (int)P.Nk - row;
+            const int row = row0 + (warp & 3) * 32, j = row + lane, valid = (int)P.Nk - row;
+            const bool keep = total > 0 && see.qlo(j) < see.qhi(j);
             const long long to = ((b * P.Nk + row) * P.Hk + hk) * P.D;
             const float down = Lift<T>::kNeeded ? 0.000244140625f : 1.f;   // 2^-12
             store_half<T, BLOCKS>(static_cast<T *>(P.dv) + to, P.Hk * P.D, DV + lanes, smem, warp, lane, half, down, keep, valid, (int)P.D);
@@ -548,7 +550,7 @@ __device__ __forceinline__ void queries_walk(const CUtensorMap &map_q, const CUt
             const float down = Lift<T>::kNeeded ? 0.000244140625f : 1.f;   // 2^-12
             const int row = i - lane;
             T *rows = static_cast<T *>(P.dq) + ((b * P.Nq + row) * P.Hq + h) * P.D;
-            store_half<T, BLOCKS>(rows, P.Hq * P.D, DQ + lanes, smem, warp, lane, half, F.scale * down / lift, total > 0 ? 32 : 0, nq - row, (int)P.D);
+            store_half<T, BLOCKS>(rows, P.Hq * P.D, DQ + lanes, smem, warp, lane, half, F.scale * down / lift, total > 0 && lo < hi, nq - row, (int)P.D);
         }
     }
     tc_fence_before();

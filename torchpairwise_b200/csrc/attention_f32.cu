@@ -112,7 +112,7 @@ template <int N, int DP> __device__ __forceinline__ void along_tokens(float (&su
     }
 }
 
-// 16 rows from `row` on to a dense [tokens, D] slice, times by
+// 16 rows from `row` on to a dense [tokens, D] slice, times by; 0 is a row that sees nothing: zero, although its sums are 0 times what need not be finite
 template <int DP> __device__ __forceinline__ void store(float *dst, long long stride, const float (&acc)[DP / 8][4], const float (&by)[2], int row, int rows, int D, int g, int t) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -120,7 +120,8 @@ template <int DP> __device__ __forceinline__ void store(float *dst, long long st
         float *p = dst + (long long)(row + g + 8 * r) * stride + 2 * t;
 #pragma unroll
         for (int n = 0; n < DP / 8; ++n)
-            if (8 * n + 2 * t < D) *reinterpret_cast<float2 *>(p + 8 * n) = make_float2(acc[n][2 * r] * by[r], acc[n][2 * r + 1] * by[r]);
+            if (8 * n + 2 * t < D)
+                *reinterpret_cast<float2 *>(p + 8 * n) = by[r] == 0.f ? make_float2(0.f, 0.f) : make_float2(acc[n][2 * r] * by[r], acc[n][2 * r + 1] * by[r]);
     }
 }
 
@@ -328,11 +329,12 @@ __device__ __forceinline__ void walk(const F32Params &F, unsigned block) {
         if (STAGES == 1 && u + 1 < total) fetch_tile(u + 1);
     }
     fetch_wait<0>();
-    const float by[2] = {(float)P.scale, (float)P.scale};
+    const bool some[2] = {lo[0] < hi[0], lo[1] < hi[1]};
+    const float by[2] = {some[0] ? (float)P.scale : 0.f, some[1] ? (float)P.scale : 0.f}, as[2] = {some[0] ? 1.f : 0.f, some[1] ? 1.f : 0.f};
     if (KEYS) {
         const long long to = (b * P.Nk * P.Hk + hk) * P.D;
         store<DP>(static_cast<float *>(P.dk) + to, P.Hk * P.D, dx, by, row0 + 16 * warp, (int)P.Nk, D, g, t);
-        store<DP>(static_cast<float *>(P.dv) + to, P.Hk * P.D, reinterpret_cast<const float(&)[DP / 8][4]>(dw), one, row0 + 16 * warp, (int)P.Nk, D, g, t);
+        store<DP>(static_cast<float *>(P.dv) + to, P.Hk * P.D, reinterpret_cast<const float(&)[DP / 8][4]>(dw), as, row0 + 16 * warp, (int)P.Nk, D, g, t);
     } else {
         store<DP>(static_cast<float *>(P.dq) + (b * P.Nq * P.Hq + h0) * P.D, P.Hq * P.D, dx, by, row0 + 16 * warp, nq, D, g, t);
     }

@@ -665,7 +665,7 @@ __device__ __forceinline__ void walk(const CUtensorMap &map_q, const CUtensorMap
                 if (total > 0) add_tile(acc, sums_at);
                 const int row = i - lane;
                 float *to = static_cast<float *>(group ? P.dk : P.dv) + ((b * P.Nk + row) * P.Hk + hk) * P.D;
-                store_rows(to, P.Hk * P.D, smem + warp * 8192, acc, group ? F.scale : 1.f, total > 0 && i < see.length, lane, (int)P.Nk - row, (int)P.D);
+                store_rows(to, P.Hk * P.D, smem + warp * 8192, acc, group ? F.scale : 1.f, total > 0 && lo < see.qhi(i), lane, (int)P.Nk - row, (int)P.D);
             }
         } else {
             const int lo = see.lo(i), hi = i < nq ? see.hi(i) : 0;
@@ -719,7 +719,7 @@ __device__ __forceinline__ void walk(const CUtensorMap &map_q, const CUtensorMap
 #pragma unroll
                 for (int e = 0; e < 32; ++e) acc[e] = add2(acc[e], pack2(other[(2 * e) * TILE], other[(2 * e + 1) * TILE]));
                 const int row = i - lane;
-                store_rows(static_cast<float *>(P.dq) + ((b * P.Nq + row) * P.Hq + h0) * P.D, P.Hq * P.D, smem + warp * 8192, acc, F.scale, total > 0, lane, nq - row, (int)P.D);
+                store_rows(static_cast<float *>(P.dq) + ((b * P.Nq + row) * P.Hq + h0) * P.D, P.Hq * P.D, smem + warp * 8192, acc, F.scale, total > 0 && lo < hi, lane, nq - row, (int)P.D);
             }
         }
     }

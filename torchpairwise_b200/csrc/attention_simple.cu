@@ -106,6 +106,7 @@ __device__ __forceinline__ void product_nn(A (&acc)[RM][DP / TX], const A *P, co
     }
 }
 
+// A factor of 0 is a row that sees nothing: zero, although its sums are 0 times what need not be finite.
 template <typename T, typename A, int RM, int DP, int TX>
 __device__ __forceinline__ void store_rows(T *dst, T *rest, long long row_stride, const A (&acc)[RM][DP / TX], const A (&factor)[RM], int row0, int rows, int D,
                                            int ty, int tx) {
@@ -119,9 +120,10 @@ __device__ __forceinline__ void store_rows(T *dst, T *rest, long long row_stride
             for (int e = 0; e < 4; ++e) {
                 const int d = 4 * TX * c + 4 * tx + e;
                 if (d >= D) continue;
-                dst[(long long)r * row_stride + d] = (T)(acc[m][4 * c + e] * factor[m]);
+                const A x = factor[m] == 0 ? (A)0 : acc[m][4 * c + e] * factor[m];
+                dst[(long long)r * row_stride + d] = (T)x;
                 if constexpr (sizeof(T) == 2)
-                    if (rest) rest[(long long)r * row_stride + d] = rest_of<T>(acc[m][4 * c + e] * factor[m]);
+                    if (rest) rest[(long long)r * row_stride + d] = rest_of<T>(x);
             }
     }
 }
@@ -285,8 +287,8 @@ __global__ void __launch_bounds__(16 * TX) attention_dkv_simple_kernel(const Att
     A one[RM], by[RM];
 #pragma unroll
     for (int r = 0; r < RM; ++r) {
-        one[r] = 1;
-        by[r] = (A)P.scale;
+        one[r] = lo[r] < hi[r] ? (A)1 : (A)0;
+        by[r] = lo[r] < hi[r] ? (A)P.scale : (A)0;
     }
     const long long to = (b * P.Nk * P.Hk + hk) * P.D;
     store_rows<T, A, RM, DP, TX>(static_cast<T *>(P.dk) + to, (T *)nullptr, P.Hk * P.D, dk, by, row0, nk, D, ty, tx);
@@ -325,7 +327,7 @@ __global__ void __launch_bounds__(16 * TX) attention_dq_simple_kernel(const Attn
         const long long from = (b * P.Hq + h) * P.Nqp + i;
         row[r] = i < nq ? static_cast<const A *>(P.row_lse)[from] : (A)0;
         mean[r] = i < nq ? static_cast<const A *>(P.row_delta)[from] : (A)0;
-        by[r] = (A)P.scale;
+        by[r] = lo[r] < hi[r] ? (A)P.scale : (A)0;
 #pragma unroll
         for (int c = 0; c < DP / TX; ++c) dq[r][c] = 0;
     }
