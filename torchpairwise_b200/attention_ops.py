@@ -122,7 +122,8 @@ def rotary_table(length: int, features: int, *, base: float = 10000.0, scaling: 
         first = max(math.floor(index_of(fast_turns)), 0)
         last = min(math.ceil(index_of(slow_turns)), features - 1)
         span = max(last - first, 1e-3)
-        blend = [min(max((i - first) / span, 0.0), 1.0) for i in range(half)]
+        # a band that ends before the first pair holds none: every pair makes fewer than slow_turns turns
+        blend = [1.0 if last <= 0 else min(max((i - first) / span, 0.0), 1.0) for i in range(half)]
         freq = [f * (1.0 - t) + f / factor * t for f, t in zip(freq, blend)]
     elif scaling not in (None, "base"):
         raise ValueError(f"rotary_table: scaling must be None, 'linear', 'base' or 'bands'. Got {scaling!r}")
