@@ -15,6 +15,9 @@ int check(const tpw_attention *a, bool backward) {
     TPW_CHECK_ARG(a->window >= 0, "tpw_attention: negative window");
     TPW_CHECK_ARG(a->window == 0 || a->causal, "tpw_attention: a window needs causal attention");
     TPW_CHECK_ARG(a->scale > 0 && isfinite(a->scale), "tpw_attention: scale must be positive and finite");
+    // scores are powers of two in 32 bits but for double: a factor that is 0 or infinite there makes masked scores NaN
+    const float factor = static_cast<float>(a->scale * 1.4426950408889634074);
+    TPW_CHECK_ARG(a->dtype == TPW_F64 || (factor > 0.f && isfinite(factor)), "tpw_attention: scale %g is beyond the range of 32-bit scores", a->scale);
     const bool rows = a->B > 0 && a->Nq > 0 && a->Hq > 0, keys = a->B > 0 && a->Nk > 0 && a->Hk > 0;
     TPW_CHECK_ARG(!rows || (a->q && a->out), "tpw_attention: NULL pointer");
     TPW_CHECK_ARG(!keys || (a->k && a->v), "tpw_attention: NULL pointer");
