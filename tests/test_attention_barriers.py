@@ -90,3 +90,45 @@ def test_what_is_drained_after_a_wait_that_gave_up_is_committed_by_the_lane_that
     assert len(drains) == (1 if name == "attention_forward.cu" else 2)
     for block in drains:
         assert "commit_by(elect_lane()," in block and "tc_commit" not in block and "lane == 0" not in block, block
+
+
+def test_no_barrier_of_the_queries_walk_is_two_phases_ahead_of_a_waiting_warp():
+    """A wait by parity cannot tell a phase from the one two later.  So the phase that next completes on a barrier must depend on every warp having
+    passed its wait for the one before: of the barriers that tiles take in turn, from the order of both roles in the source."""
+    text = SOURCE.read_text()
+    text = text[text.index("void queries_walk("):text.index("// Both walks in one launch")]
+    issuer = section(text, "if (total > 0 && ok) ok = first(0);", "if (ok && total > 0) commit_by(leader, acc_full);")
+    first = section(text, "auto first = [&](int u) {", "return true;\n        };")
+    rows = section(text, "const bool masked = j0 < all_lo", "if (ok && total > 0) {\n            ok = warp_wait(acc_full")
+
+    def ops(code):
+        """(what, barrier, tile offset) in the order of the source."""
+        found = []
+        for m in re.finditer(r"warp_wait\(&?(\w+)|commit_by\(leader, &?(\w+)|mbar_arrive\(&?(\w+)|\bfirst\(u \+ 1\)", code):
+            wait, commit, arrive = m.groups()
+            found.append(("wait", wait, 0) if wait else ("arrive", commit or arrive, 0) if commit or arrive else ("first", None, 1))
+        return found
+
+    barriers = ("s_full", "s_read", "dp_full", "ds_ready")
+    # tiles take one barrier, or two in turn where the source picks it by the tile's last bit
+    count = {b: 2 if re.search(rf"&{b}\[u & 1\]", rows) else 1 for b in barriers}
+    assert all(("wait", b, 0) in ops(issuer) + ops(first) + ops(rows) for b in barriers)
+    edges, tiles = {}, 12
+
+    def chain(sequence):
+        for a, b in zip(sequence, sequence[1:]):
+            edges.setdefault(a, set()).add(b)
+
+    issued = [(w, b, 0) for w, b, _ in ops(first)]
+    for u in range(tiles):
+        for w, b, at in ops(issuer):
+            issued += [(x, y, u + 1) for x, y, _ in ops(first)] if w == "first" else [(w, b, u)]
+    chain(issued)
+    chain([(w, b, u) for u in range(tiles) for w, b, _ in ops(rows)])
+    for b in barriers:
+        for u in range(tiles):
+            edges.setdefault(("arrive", b, u), set()).add(("wait", b, u))
+    for b in barriers:
+        for u in range(4):
+            assert reaches(edges, ("wait", b, u), ("arrive", b, u + count[b])), \
+                f"{b}: tile {u + count[b]} may arrive before a warp has seen that tile {u} has"

@@ -69,7 +69,7 @@ template <int BLOCKS> struct QueriesSmem {
     static constexpr uint32_t TILE_BYTES = BLOCKS * BLOCK_BYTES;
     static constexpr uint32_t OFF_K = 2 * TILE_BYTES, OFF_V = OFF_K + kKeys * TILE_BYTES;
     static constexpr uint32_t OFF_BAR = OFF_V + kValues * TILE_BYTES;
-    static constexpr uint32_t OFF_TMEM = OFF_BAR + 8 * (2 * (kKeys + kValues) + 8);
+    static constexpr uint32_t OFF_TMEM = OFF_BAR + 8 * (2 * (kKeys + kValues) + 9);
     static constexpr uint32_t ALLOC = OFF_TMEM + 16 + 1024;
     static_assert(ALLOC <= 232448, "exceeds the dynamic shared memory of one CTA");
 };
@@ -365,7 +365,7 @@ __device__ __forceinline__ void queries_walk(const CUtensorMap &map_q, const CUt
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *k_full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *k_empty = k_full + L::kKeys, *v_full = k_empty + L::kKeys,
              *v_empty = v_full + L::kValues, *own_full = v_empty + L::kValues, *s_full = own_full + 1,
-             *s_read = s_full + 1, *dp_full = s_read + 1, *ds_ready = dp_full + 2, *acc_full = ds_ready + 1, *drained = acc_full + 1;
+             *s_read = s_full + 1, *dp_full = s_read + 1, *ds_ready = dp_full + 2, *acc_full = ds_ready + 2, *drained = acc_full + 1;
     uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(smem + L::OFF_TMEM);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_TMEM + 4);
 
@@ -387,7 +387,8 @@ __device__ __forceinline__ void queries_walk(const CUtensorMap &map_q, const CUt
         mbar_init(s_read, 8);
         mbar_init(&dp_full[0], 1);
         mbar_init(&dp_full[1], 1);
-        mbar_init(ds_ready, 8);
+        mbar_init(&ds_ready[0], 8);
+        mbar_init(&ds_ready[1], 8);
         mbar_init(acc_full, 1);
         mbar_init(drained, 1);
         *abort_flag = 0;
@@ -472,7 +473,9 @@ __device__ __forceinline__ void queries_walk(const CUtensorMap &map_q, const CUt
                 tc_fence_after();
                 if (!(ok = first(u + 1))) break;
             }
-            if (!(ok = warp_wait(ds_ready, u & 1, 6))) break;
+            // S and dP of the next tile are already under way, so its gradients may be ready before this warp has seen that this tile's are: a barrier
+            // each for even and odd tiles, or the wait would miss a phase and never end
+            if (!(ok = warp_wait(&ds_ready[u & 1], (u >> 1) & 1, 6))) break;
             tc_fence_after();
             product_tokens(leader, DQ, DP + (u & 1) * TILE, 64, keys + (u % L::kKeys) * L::TILE_BYTES, idesc_d, u > 0);
             commit_by(leader, &k_empty[u % L::kKeys]);
@@ -540,7 +543,7 @@ __device__ __forceinline__ void queries_walk(const CUtensorMap &map_q, const CUt
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(ds_ready);
+            if (lane == 0) mbar_arrive(&ds_ready[u & 1]);
         }
         if (ok && total > 0) {
             ok = warp_wait(acc_full, 0, 9);
