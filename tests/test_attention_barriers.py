@@ -132,3 +132,21 @@ def test_no_barrier_of_the_queries_walk_is_two_phases_ahead_of_a_waiting_warp():
         for u in range(4):
             assert reaches(edges, ("wait", b, u), ("arrive", b, u + count[b])), \
                 f"{b}: tile {u + count[b]} may arrive before a warp has seen that tile {u} has"
+
+
+def test_products_of_the_float32_walks_wait_for_the_tiles_they_read():
+    """Two warps issue the products of a walk.  Each tile that a product reads has arrived: its issuing warp waited for it, or for something that was made of it."""
+    text = (SOURCE.parent / "attention_parts.cu").read_text()
+    text = section(text, "if (OF_KEYS && warp == 9) {   // S, dV", "if (ok && total > 0) commit_by(leader, bar.all_full);")
+    branches = [text[:text.index("} else if (OF_KEYS) {")], text[text.index("} else if (OF_KEYS) {"):text.index("} else if (warp == 9) {")],
+                text[text.index("} else if (warp == 9) {"):text.index("} else {   // dP")]]
+    # The row warps of dK's gradients wait for the scores (ring x) and for dP, so x has arrived where they say that these are ready.  The row warps of dV's
+    # probabilities wait for the scores alone, which says nothing of ring y.
+    implied = {"p_ready": "", "ds_ready": "x"}
+    for branch, ring in zip(branches, ("y", "x", "x")):
+        loop = branch[branch.index("for (int u = 0;"):]
+        before = loop[:loop.index("sums(SUM")]
+        assert re.search(rf"ring_{ring} \+ \(u %", loop[loop.index("sums(SUM"):])
+        own = f"arrived(bar.{ring}_full, u," in before or f"from_{ring}(u)" in branch or f"from_{ring}(u + 1)" in branch
+        made = any(ring in implied[b] for b in re.findall(r"bar\.(p_ready|ds_ready)", before))
+        assert own or made, f"the products that read ring {ring} do not wait for it:\n{branch}"

@@ -566,6 +566,7 @@ __device__ __forceinline__ void walk(const CUtensorMap &map_q, const CUtensorMap
                     if (!(ok = from_x(u + 1))) break;
                 }
                 if (!(ok = warp_wait(bar.p_ready, u & 1, 7))) break;
+                if (!(ok = arrived(bar.y_full, u, L::kY, 12))) break;   // P is made of the scores: it says nothing of dO
                 sums(SUM, LEFT, ring_y + (u % L::kY) * L::TILE_BYTES, &bar.sum_full[0], &bar.y_empty[u % L::kY]);
             }
         } else if (OF_KEYS) {   // dP, dK
