@@ -100,3 +100,26 @@ def test_rows_that_see_nothing_are_zero_whatever_others_see(dtype, d, queries):
             dk, dv = torch.autograd.grad(out, leaves[1:], gg)
             assert not dk[:, :unseen].any() and not dv[:, :unseen].any(), (bad, where)
     assert tpw.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+def test_many_walks_of_random_lengths(dtype):
+    """What depends on which warp is first shows in one call of thousands: results of the same bits each time, and a clean status word."""
+    import random
+    rng = random.Random(31)
+    for _ in range(300):
+        hk = rng.choice([1, 2, 3])
+        hq, batch, d = hk * rng.choice([1, 2, 5]), rng.randint(1, 3), rng.choice([8, 40, 64, 72, 104, 128])
+        nq, nk = (rng.choice([rng.randint(1, 200), rng.randint(100, 900)]) for _ in range(2))
+        causal = rng.random() < 0.5
+        window = rng.choice([None, rng.randint(1, 300)]) if causal else None
+        n = torch.tensor([rng.randint(0, nk) for _ in range(batch)], dtype=torch.int32, device="cuda")
+        leaves = [torch.randn(batch, x, h, d, device="cuda", dtype=dtype).requires_grad_() for x, h in ((nq, hq), (nk, hk), (nk, hk))]
+        runs = []
+        for _ in range(4):
+            out = tpw.attention(*leaves, causal=causal, window=window, key_lengths=n)
+            runs.append([out, *torch.autograd.grad(out, leaves, leaves[0].detach())])
+        for other in runs[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+        assert all(bool(torch.isfinite(t).all()) for t in runs[0])
+    assert tpw.device_status() == 0
