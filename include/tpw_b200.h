@@ -593,7 +593,8 @@ TPW_API int tpw_widen(int bf16, const void *src, float *dst, int64_t n, tpw_stre
  * nothing has out = 0, lse = -inf and no gradient.  Query head h reads key head h / (Hq / Hk).  Keys and values from L on
  * are never used, whatever they hold.  No counterpart in the reference.
  *
- * Scores, statistics and sums are held in 32 bits (64 for TPW_F64).  With 16-bit inputs the probabilities and the
+ * Scores, statistics and sums are held in 32 bits (64 for TPW_F64).  Scores are to stay below 2^24 in magnitude: a probability is as good
+ * as its score.  Operands within the lengths are to be finite, float32 ones below 2^127.  With 16-bit inputs the probabilities and the
  * gradients of the scores are rounded to the inputs' type before they enter a matrix product, as its operands must be.  A
  * gradient of a score is p_ij (grad_out_i . v_j - grad_out_i . out_i); with out_rest the second term is taken from out as it was before it
  * was rounded, without it the rounding of out adds about a tenth to the error of grad_q and grad_k.
@@ -603,7 +604,7 @@ typedef struct tpw_attention {
     int32_t causal;
     int64_t window;           /* 0: none */
     int64_t B, Nq, Nk, Hq, Hk, D; /* Hq a multiple of Hk, 1 <= D <= 256 */
-    double scale;             /* positive, finite */
+    double scale;             /* positive, finite; but for TPW_F64 also as a float, times log2 e */
     const void *q, *k, *v;    /* [B, N, H, D]; strides of batch, token and head in elements, features side by side */
     int64_t q_stride[3], k_stride[3], v_stride[3];
     const int32_t *key_lengths; /* [B] on the device, clamped to [0, Nk]; NULL: Nk everywhere */

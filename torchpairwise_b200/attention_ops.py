@@ -62,7 +62,10 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False, window: 
     nothing is zero, and so are its gradients.  ``scale`` defaults to ``1 / sqrt(features)``.  ``return_lse`` also returns
     ``log(sum(exp(scores)))``, ``[batch, heads, queries]`` in float32 (float64 for float64), -inf for such a row; it is differentiable too.
 
-    Scores, statistics and sums are held in 32 bits (64 for float64); the gradients are summed in a fixed order.
+    Scores, statistics and sums are held in 32 bits (64 for float64); the gradients are summed in a fixed order.  A probability is as good as its
+    score, 2^-24 of the score's magnitude: scores are to stay below 2^24, beyond which neighbouring 32-bit numbers are more than a factor e apart.
+    Within a sequence's length operands are to be finite (float32: below 2^127); what is not makes the rows of its tile NaN, but for rows that
+    see nothing.  16-bit types run on the tensor cores where the features are a multiple of 8 up to 128, float32 where they are a multiple of 4 up to 128.
     """
     _check("attention", q)
     out, lse = _attention(q, k, v, causal, window, key_lengths, scale)
@@ -91,7 +94,7 @@ def rotary_table(length: int, features: int, *, base: float = 10000.0, scaling: 
 
     Pair i turns by ``base ** (-2 i / features)`` a position.  ``scaling`` stretches the context by ``factor``: "linear" divides
     every frequency; "base" raises the base to ``base * factor ** (features / (features - 2))``, which keeps the fastest pair and
-    divides the slowest by ``factor``; "bands" divides pairs that make fewer than ``slow_turns`` turns over ``original_length``
+    divides the slowest by ``factor``; "bands" (the interpolation by parts of the YaRN method) divides pairs that make fewer than ``slow_turns`` turns over ``original_length``
     positions, keeps those that make more than ``fast_turns`` and blends linearly in the pair's index between.  ``magnitude`` multiplies both tables.
     Angles are reduced in 64 bits, so long contexts lose nothing.
     """

@@ -73,7 +73,7 @@ struct AttnSplits {
 bool attn_tc_fits(int dtype, const AttnParams &P);
 AttnSplits attn_tc_splits(const AttnParams &P);
 int attn_tc_forward(int dtype, const AttnParams &P, const AttnSplits &splits, cudaStream_t s);
-// attention_f32.cu: float32 on the tensor cores in three tf32 products
+// attention_f32.cu: float32 up to 128 features on the tensor cores in three tf32 products
 bool attn_f32_fits(int dtype, const AttnParams &P);
 bool attn_f32_backward_fits(int dtype, const AttnParams &P);
 AttnSplits attn_f32_splits(const AttnParams &P);

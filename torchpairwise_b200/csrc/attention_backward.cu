@@ -15,8 +15,8 @@
 //
 // Two warpgroups share a tile's 128 rows: each has half of the columns, and writes its half of P or dS over the columns it read.
 //
-// Measured bfloat16 [2, 4096, 16/4, 128] 665 us = 1030 TFLOP/s on the five products that are asked for, 1450 on the seven; causal [1, 4096, 32/8, 128] the
-// tensor cores are busy 66 % of the time.  64 features 555 us.  Both walks in one launch; CTAs that take over further blocks, as in the
+// Measured with the row terms' kernel (attention_rows.cu), bfloat16 [2, 4096, 16/4, 128] 730 us = 940 TFLOP/s on the five products that are asked for, 1320 on the
+// seven; causal [1, 4096, 32/8, 128] the tensor cores are busy 66 % of the time.  [2, 4096, 16, 64] 575 us.  Both walks in one launch; CTAs that take over further blocks, as in the
 // forward, were slower (1520 -> 1575 us causal [1, 8192, 32/8, 128]): the accumulators leave no tensor memory to overlap two blocks in.
 #include "attention_tc.cuh"
 

@@ -1,5 +1,6 @@
-// Attention and its gradients in float32 up to 128 features, rows on 16-byte boundaries: what attention_parts.cu does not take, more than 64 features (whose
-// three parts of K, V and a tile of either side would not fit in shared memory), few tokens, and few rows against many keys.
+// Attention and its gradients in float32 up to 128 features, rows on 16-byte boundaries: what attention_parts.cu does not take, more than 64 features, few tokens,
+// and few rows against many keys.  (Above 64 features the three parts of a gradient walk's own two tiles alone are 192 KB and leave no room for walked ones.  The
+// forward's would fit, with a tile of queries at 96 KB and one tile each of 64 keys and values at 48; there is no such kernel.)
 //
 // Every product runs on the tensor cores with tf32 operands at float32 accuracy: x = h + l, h the nearest number of 11 digits, l the rest,
 // and x y = h h' + (h l' + l h') up to 2^-23.  The tensor cores add with truncation, so the large products are summed over at most 128

@@ -149,7 +149,7 @@ __device__ __forceinline__ void store_rows(float *to, long long row_stride, unsi
 // ---- forward ----
 // A CTA has two tiles of 128 queries, a row to a thread of either warpgroup, and a warp each that issues its MMAs; the key tiles come once for both,
 // through a ring.  While one tile's threads form probabilities the tensor cores work for the other, and the next scores are formed while these are worked on.
-// (A CTA per query tile, two to an SM, with room for one K and one V each, waited for them: 60 us where this takes 40, [4, 1024, 8, 64].)
+// (A CTA per query tile, two to an SM, with room for one K and one V each, waited for them: 60 us where this takes 48, [4, 1024, 8, 64].)
 struct ForwardPartsSmem {
     static constexpr int kSlots = 5;
     static constexpr uint32_t TILE_BYTES = 3 * WALK_PART;

@@ -76,7 +76,8 @@ template <> __device__ __forceinline__ void narrow2<__nv_bfloat16>(__nv_bfloat16
 template <> __device__ __forceinline__ void narrow2<__half>(__half *p, float a, float b) { *reinterpret_cast<__half2 *>(p) = __floats2half2_rn(a, b); }
 
 // W elements per access (16 bytes, or one where a row or pointer is off that grid).  64 registers, so that 32 warps per SM keep
-// eight 16-byte loads each in flight: with 128 registers and half of the warps DRAM was 37 % busy.
+// eight 16-byte loads each in flight: with 128 registers and half of the warps DRAM was 37 % busy.  In the half layout that is too few for the angles of
+// eight pairs beside four pieces on their way: 16-bit types store 88 bytes a thread to local memory and load 156 back (ptxas).
 template <typename T, int W, bool INTER>
 __global__ void __launch_bounds__(256, 4) rotary_kernel(const RotaryParams P) {
     typedef typename Acc<T>::type A;
