@@ -45,7 +45,8 @@ inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 
 int *device_status_ptr();
 
 // True when the environment variable TPW_DISABLE_TMA is set to a non-zero value: every kernel then
-// stages its tiles with guarded plain loads (a debugging aid; results are bit-identical).
+// stages its tiles with guarded plain loads (a debugging aid; results are bit-identical).  Attention takes
+// its kernels without TMA instead, whose results differ by their rounding.
 bool tma_disabled();
 
 // Number of SMs of the current device (cached per device).
