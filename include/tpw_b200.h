@@ -47,7 +47,7 @@ enum tpw_dtype {
     TPW_F64 = 1,
     TPW_I32 = 2, /* accepted by tpw_cmp_reduce_forward only */
     TPW_I64 = 3, /* accepted by tpw_cmp_reduce_forward only */
-    TPW_F16 = 4, /* accepted by the attention and rotary entry points only */
+    TPW_F16 = 4, /* accepted by the attention, rotary and cache entry points only */
     TPW_BF16 = 5 /* likewise */
 };
 
@@ -648,6 +648,66 @@ TPW_API int tpw_rotary_apply(const tpw_rotary *a, tpw_stream_t stream);
 /* cos, sin [length, half] = magnitude * cos, sin (t * frequency[i]), t < length; frequency in radians, [half] double on the device. */
 TPW_API int tpw_rotary_table(const double *frequency, double magnitude, float *cos, float *sin, int64_t length, int64_t half,
                              tpw_stream_t stream);
+
+/* ---- a cache of quantised keys and values, and attention over it ------------------------------------- */
+
+/*
+ * Keys and values of a token and head are cut into groups: of 32 features (groups = ceil(D / 32)), or the whole head (groups = 1).  Of a group
+ *   zero = the largest bfloat16 number that is not above its lowest value,
+ *   step = the smallest bfloat16 number, 2^-100 at least, of which 2^bits - 1 reach from the zero to its highest value,
+ *   code = the nearest whole number to (x - zero) / step, ties to even,
+ * and a code stands for zero + step * code, which is at most half a step from x.  A group with a value that is not finite, or 2^100 or
+ * more in magnitude, has NaN for its zero and step and reads as NaN.
+ *
+ * codes: [B, H, capacity, row bytes].  A row has W * 32 features, W = max(2, ceil(D / 32)); codes of those beyond D are 0.  Feature
+ * 32 w + 8 t + n of a key (n < 8, t < 4) is code (t W + w) 8 + n of its row, feature 32 w + 4 t + n of a value (n < 4, t < 8) is
+ * code (t W + w) 4 + n: what a lane of a tensor-core operand takes lies together.  Of two 4-bit codes in a byte the first is the lower.
+ * scales: [B, H, capacity, groups, 2] bfloat16, step and zero.
+ *
+ * A call's n tokens (or queries) are the last ones of their sequence: i stands at position lengths[b] - n + i.  There is no place for
+ * positions below 0 or from the capacity on: such a token is not stored and reads as zero, and is no key.
+ * No counterpart in the reference.
+ */
+typedef struct tpw_cache {
+    int32_t bits;             /* 4 or 8 */
+    int32_t groups;           /* 1 or ceil(D / 32) */
+    int64_t B, H, capacity, D; /* capacity a multiple of 64, 1 <= D <= 128 */
+    void *codes[2];           /* of keys and values; 16-byte aligned */
+    void *scales[2];          /* likewise */
+    const int32_t *lengths;   /* [B] on the device: how long each sequence is with the call's tokens */
+} tpw_cache;
+/* bytes of a row of codes; 0 where bits or D is not supported */
+TPW_API int64_t tpw_cache_row_bytes(int bits, int64_t D);
+
+typedef struct tpw_cache_rows {
+    int32_t dtype;            /* TPW_F32, TPW_F16, TPW_BF16 */
+    int32_t from_start;       /* read only: token i stands at position i, and reads as zero from lengths[b] on */
+    int64_t N;
+    void *x[2];               /* keys and values [B, N, H, D]: read by tpw_cache_write, written (dense) by tpw_cache_read */
+    int64_t stride[2][3];     /* write only: of batch, token and head in elements, features side by side */
+} tpw_cache_rows;
+TPW_API int tpw_cache_write(const tpw_cache *c, const tpw_cache_rows *rows, tpw_stream_t stream);
+/* zero + step * code in 32 bits, rounded once to the type */
+TPW_API int tpw_cache_read(const tpw_cache *c, const tpw_cache_rows *rows, tpw_stream_t stream);
+
+/*
+ * Attention as tpw_attention_forward defines it, with the keys and values that the cache stands for.  Scores, statistics and sums are held
+ * in 32 bits; with float32 queries nothing is rounded to fewer.
+ */
+typedef struct tpw_cache_attention_args {
+    int32_t dtype;            /* of q and out: TPW_F32, TPW_F16, TPW_BF16 */
+    int32_t causal;
+    int64_t window;           /* 0: none */
+    int64_t Nq, Hq;           /* Hq a multiple of the cache's heads */
+    double scale;             /* positive, finite, also as a float, times log2 e */
+    const void *q;            /* [B, Nq, Hq, D]; strides of batch, token and head in elements, features side by side */
+    int64_t q_stride[3];
+    void *out;                /* [B, Nq, Hq, D] dense */
+    float *lse;               /* [B, Hq, Nq] dense; NULL: not wanted */
+} tpw_cache_attention_args;
+/* Scratch (device memory, 16-byte aligned) that the call with these arguments wants; 0: none; -1: refused (tpw_last_error). */
+TPW_API int64_t tpw_cache_attention_scratch_bytes(const tpw_cache *c, const tpw_cache_attention_args *a);
+TPW_API int tpw_cache_attention(const tpw_cache *c, const tpw_cache_attention_args *a, void *scratch, int64_t scratch_bytes, tpw_stream_t stream);
 
 /* ---- measured issue peaks (roofline denominators for the CUDA-core kernels) -------------------- */
 

@@ -6,6 +6,7 @@ CUDA kernels behind the C ABI of ``include/tpw_b200.h``.  CUDA tensors only.
 """
 from ._abi import LIB_PATH, TpwError, device_status, lib, measure_issue_peak
 from .attention_ops import attention, rotary_embedding, rotary_table
+from .cache_ops import QuantizedCache, cache_attention, cache_read, cache_write, quantized_cache
 from .cpdist import cdist, pdist
 from .ops import (
     _directed_hausdorff,

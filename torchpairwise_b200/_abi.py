@@ -97,6 +97,11 @@ SIGNATURES = {
     "tpw_attention_backward": (_I, [_P, _P, _L, _P]),
     "tpw_rotary_apply": (_I, [_P, _P]),
     "tpw_rotary_table": (_I, [_P, _D, _P, _P, _L, _L, _P]),
+    "tpw_cache_row_bytes": (_L, [_I, _L]),
+    "tpw_cache_write": (_I, [_P, _P, _P]),
+    "tpw_cache_read": (_I, [_P, _P, _P]),
+    "tpw_cache_attention_scratch_bytes": (_L, [_P, _P]),
+    "tpw_cache_attention": (_I, [_P, _P, _P, _L, _P]),
     "tpw_measure_issue_peak": (_I, [_I, POINTER(c_double)]),
 }
 

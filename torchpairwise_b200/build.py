@@ -113,6 +113,9 @@ TORCH_LIB_PATH = LIB_DIR / "libtpw_b200_torch.so"
 # attention and rotary positions: a dispatcher namespace and library of their own
 ATTENTION_SRC = CSRC / "torch" / "tpw_torch_attention.cpp"
 ATTENTION_LIB_PATH = LIB_DIR / "libtpw_b200_attention.so"
+# the cache of quantised keys and values: the same namespace, a library of its own
+CACHE_SRC = CSRC / "torch" / "tpw_torch_cache.cpp"
+CACHE_LIB_PATH = LIB_DIR / "libtpw_b200_cache.so"
 
 
 def _build_host_layer(src: Path, lib: Path, force: bool) -> Path:
@@ -146,6 +149,7 @@ def build_torch_ops(force: bool = False) -> Path:
     against the installed torch, linked to ``libtpw_b200.so``; returns the path of ``libtpw_b200_torch.so``."""
     build_library()
     _build_host_layer(ATTENTION_SRC, ATTENTION_LIB_PATH, force)
+    _build_host_layer(CACHE_SRC, CACHE_LIB_PATH, force)
     return _build_host_layer(TORCH_SRC, TORCH_LIB_PATH, force)
 
 

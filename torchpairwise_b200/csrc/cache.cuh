@@ -1,0 +1,81 @@
+// What the kernels on a cache of quantised keys and values share: its layout (tpw_b200.h has the definition) and the arguments as a kernel
+// gets them.
+#pragma once
+#include "attention.cuh"
+
+namespace tpw {
+
+struct CacheParams {
+    unsigned char *codes[2];
+    uint32_t *scales[2];      // a group's step (low half) and zero as bfloat16
+    const int *lengths;
+    long long B, H, capacity;
+    int D, bits, groups, width, row_bytes;   // width: features of a row in storage / 32
+};
+
+inline int cache_width(long long D) { return D <= 64 ? 2 : (int)((D + 31) / 32); }
+inline CacheParams cache_params(const tpw_cache &c) {
+    CacheParams P = {};
+    for (int w = 0; w < 2; ++w) {
+        P.codes[w] = static_cast<unsigned char *>(c.codes[w]);
+        P.scales[w] = static_cast<uint32_t *>(c.scales[w]);
+    }
+    P.lengths = c.lengths;
+    P.B = c.B; P.H = c.H; P.capacity = c.capacity;
+    P.D = (int)c.D; P.bits = c.bits; P.groups = c.groups;
+    P.width = cache_width(c.D);
+    P.row_bytes = P.width * 4 * c.bits;
+    return P;
+}
+
+struct CacheAttnParams {
+    CacheParams c;
+    const void *q;
+    long long q_s[3];         // batch, token, head
+    void *out;
+    float *lse;
+    long long Nq, Hq, group, window;
+    int causal, dtype;
+    float scale_log2;
+    int *status;
+};
+
+// cache_rows.cu
+int cache_write(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s);
+int cache_read(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s);
+// cache_attention.cu
+long long cache_attention_bytes(const CacheAttnParams &P);
+int cache_attention(const CacheAttnParams &P, void *scratch, cudaStream_t s);
+
+#ifdef __CUDACC__
+namespace {
+
+__device__ __forceinline__ float step_of(uint32_t scales) { return __uint_as_float(scales << 16); }
+__device__ __forceinline__ float zero_of(uint32_t scales) { return __uint_as_float(scales & 0xffff0000u); }
+
+// The keys [lo, hi) that query i of sequence b sees.
+struct CacheSeen {
+    int length, off, window;   // keys that there are; position of query 0; window: 0 none
+    bool causal;
+    __device__ __forceinline__ CacheSeen(const CacheAttnParams &P, int b) {
+        int n = P.c.lengths[b];
+        const int cap = (int)P.c.capacity;
+        n = n < 0 ? 0 : n > (1 << 30) ? 1 << 30 : n;
+        length = n < cap ? n : cap;
+        off = n - (int)P.Nq;
+        causal = P.causal != 0;
+        window = (int)(P.window < cap ? P.window : 0);   // a window over all keys is none
+    }
+    __device__ __forceinline__ int hi(int i) const {
+        const int h = causal && i + off + 1 < length ? i + off + 1 : length;
+        return h > 0 ? h : 0;
+    }
+    __device__ __forceinline__ int lo(int i) const {
+        const int l = window ? i + off + 1 - window : 0;
+        return l > 0 ? l : 0;
+    }
+};
+
+} // namespace
+#endif
+} // namespace tpw

@@ -1,0 +1,242 @@
+// Tokens into a cache of quantised keys and values, and out of it.
+//
+// A lane has 8 neighbouring features of a row, 8 or 16 lanes the row; a group's lowest and highest value meet over 4 lanes (or all of the row).
+#include "cache.cuh"
+
+namespace tpw {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct RowsParams {
+    CacheParams c;
+    void *x[2];
+    long long stride[2][3];
+    long long N, rows;         // rows = B * H * N
+    int from_start, vector;    // vector: 16-byte pieces of a row
+};
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// n of 8 features as they lie in memory, widened
+template <typename T> __device__ __forceinline__ void load8(float (&x)[8], const T *p, int n, bool vector) {
+    if (vector) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = __ldcs(reinterpret_cast<const float4 *>(p)), b = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
+            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+            x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        } else {
+            const uint4 w = __ldcs(reinterpret_cast<const uint4 *>(p));
+            const T *v = reinterpret_cast<const T *>(&w);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = (float)v[k];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = (float)p[k < n ? k : 0];
+    }
+}
+template <typename T> __device__ __forceinline__ void store8(T *p, const float (&x)[8], int n, bool vector) {
+    if (vector) {
+        if constexpr (sizeof(T) == 4) {
+            __stcs(reinterpret_cast<float4 *>(p), make_float4(x[0], x[1], x[2], x[3]));
+            __stcs(reinterpret_cast<float4 *>(p) + 1, make_float4(x[4], x[5], x[6], x[7]));
+        } else {
+            alignas(16) T v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = (T)x[k];
+            __stcs(reinterpret_cast<uint4 *>(p), *reinterpret_cast<const uint4 *>(v));
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < n) p[k] = (T)x[k];
+    }
+}
+
+// a row of the call: token i of head h of sequence b at position `at`
+struct Row {
+    long long b, i, h, at;
+    bool stored;
+    __device__ __forceinline__ Row(const RowsParams &R, long long r) {
+        i = r % R.N;
+        const long long bh = r / R.N;
+        h = bh % R.c.H;
+        b = bh / R.c.H;
+        const long long n = R.c.lengths[b];
+        at = R.from_start ? i : n - R.N + i;
+        stored = at >= 0 && at < R.c.capacity && at < n;
+    }
+    __device__ __forceinline__ long long place(const RowsParams &R) const { return (b * R.c.H + h) * R.c.capacity + at; }
+};
+
+// where the 8 codes of lane l lie in a row: those of a key together, those of a value in two halves
+template <int BITS, int W> __device__ __forceinline__ int key_place(int l) { return ((l & 3) * W + (l >> 2)) * BITS; }
+template <int BITS, int W> __device__ __forceinline__ int value_place(int l, int half) { return ((2 * (l & 3) + half) * W + (l >> 2)) * (BITS / 2); }
+
+// 8 codes into words: 4 bits in one, 8 bits in two
+template <int BITS> __device__ __forceinline__ void pack8(uint32_t (&w)[2], const uint32_t (&code)[8]) {
+    w[0] = w[1] = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        if (BITS == 4) w[0] |= code[k] << (4 * k);
+        else w[k >> 2] |= code[k] << (8 * (k & 3));
+    }
+}
+
+template <typename T, int BITS, int W>
+__global__ void __launch_bounds__(kThreads) cache_write_kernel(const RowsParams R) {
+    constexpr int LANES = W == 2 ? 8 : 16;   // of a row; 4 * W of them have features
+    constexpr float MOST = BITS == 4 ? 15.f : 255.f;
+    const int which = blockIdx.y, l = threadIdx.x % LANES;
+    const long long r = (long long)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+    const Row row(R, r < R.rows ? r : R.rows - 1);
+    const bool live = r < R.rows && row.stored;
+    const int n = R.c.D - 8 * l;   // features of this lane that there are
+    float x[8];
+    float lo = INFINITY, hi = -INFINITY;
+    if (live && n > 0) {
+        load8(x, static_cast<const T *>(R.x[which]) + row.b * R.stride[which][0] + row.i * R.stride[which][1] + row.h * R.stride[which][2] + 8 * l, n, R.vector);
+        lo = hi = x[0];
+#pragma unroll
+        for (int k = 1; k < 8; ++k) {
+            lo = min_nan(lo, x[k]);
+            hi = max_nan(hi, x[k]);
+        }
+    }
+#pragma unroll
+    for (int d = 1; d < LANES; d <<= 1) {
+        if (d == 4 && R.c.groups > 1) break;
+        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+    }
+    if (!live || l >= 4 * W) return;
+    // zero: down to bfloat16
+    uint32_t zero_bits = __float_as_uint(lo);
+    if ((int)zero_bits < 0) zero_bits += 0xffffu;
+    zero_bits &= 0xffff0000u;
+    const float zero = __uint_as_float(zero_bits);
+    // step: the smallest bfloat16 number of which MOST (products of which are exact) reach the highest value.  The quotient's upper 16 bits are at most one
+    // number off.
+    const float range = __fsub_ru(hi, zero);
+    uint32_t step_bits = (__float_as_uint(range * (1.f / MOST)) + 0xffffu) & 0xffff0000u;
+    if (__uint_as_float(step_bits - 0x10000u) * MOST >= range) step_bits -= 0x10000u;
+    if (__uint_as_float(step_bits) * MOST < range) step_bits += 0x10000u;
+    const float least = 7.888609052210118e-31f;   // 2^-100
+    const bool fine = lo > -1.2676506002282294e30f && hi < 1.2676506002282294e30f;   // 2^100; NaN is not
+    float step = fmaxf(__uint_as_float(step_bits), least);
+    uint32_t code[8];
+    const float inv = 1.f / step, half = 0.5f * step;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float d = __fsub_rn(x[k], zero);
+        const float y = fmaf(d, inv, 12582912.f);   // 1.5 * 2^23: a sum with it ends in the nearest whole number
+        // the reciprocal's rounding can take that one off beside a middle: what is left says so, exactly
+        const float left = fmaf(y - 12582912.f, -step, d);
+        int c = __float_as_int(y) & 0x1ff;
+        if (fabsf(left) > half || (fabsf(left) == half && (c & 1))) c += left > 0.f ? 1 : -1;
+        code[k] = fine && k < n ? (uint32_t)c : 0u;
+    }
+    uint32_t w[2];
+    pack8<BITS>(w, code);
+    const long long place = row.place(R);
+    unsigned char *to = R.c.codes[which] + place * R.c.row_bytes;
+    if (which == 0) {
+        if (BITS == 4) *reinterpret_cast<uint32_t *>(to + key_place<BITS, W>(l)) = w[0];
+        else *reinterpret_cast<uint2 *>(to + key_place<BITS, W>(l)) = make_uint2(w[0], w[1]);
+    } else if (BITS == 4) {
+        *reinterpret_cast<uint16_t *>(to + value_place<BITS, W>(l, 0)) = (uint16_t)w[0];
+        *reinterpret_cast<uint16_t *>(to + value_place<BITS, W>(l, 1)) = (uint16_t)(w[0] >> 16);
+    } else {
+        *reinterpret_cast<uint32_t *>(to + value_place<BITS, W>(l, 0)) = w[0];
+        *reinterpret_cast<uint32_t *>(to + value_place<BITS, W>(l, 1)) = w[1];
+    }
+    const int group = R.c.groups > 1 ? l >> 2 : 0;
+    if (l == 4 * group && group < R.c.groups)
+        R.c.scales[which][place * R.c.groups + group] = fine ? __float_as_uint(step) >> 16 | zero_bits : 0x7fc07fc0u;
+}
+
+template <typename T, int BITS, int W>
+__global__ void __launch_bounds__(kThreads) cache_read_kernel(const RowsParams R) {
+    constexpr int LANES = 4 * W;
+    const int which = blockIdx.y;
+    const long long at = (long long)blockIdx.x * kThreads + threadIdx.x, r = at / LANES;
+    const int l = (int)(at % LANES), n = R.c.D - 8 * l;
+    if (r >= R.rows || n <= 0) return;
+    const Row row(R, r);
+    float x[8] = {};
+    if (row.stored) {
+        const long long place = row.place(R);
+        const unsigned char *from = R.c.codes[which] + place * R.c.row_bytes;
+        uint32_t w[2];
+        if (which == 0) {
+            w[0] = *reinterpret_cast<const uint32_t *>(from + key_place<BITS, W>(l));
+            if (BITS == 8) w[1] = *reinterpret_cast<const uint32_t *>(from + key_place<BITS, W>(l) + 4);
+        } else if (BITS == 4) {
+            w[0] = *reinterpret_cast<const uint16_t *>(from + value_place<BITS, W>(l, 0)) | (uint32_t)*reinterpret_cast<const uint16_t *>(from + value_place<BITS, W>(l, 1)) << 16;
+        } else {
+            w[0] = *reinterpret_cast<const uint32_t *>(from + value_place<BITS, W>(l, 0));
+            w[1] = *reinterpret_cast<const uint32_t *>(from + value_place<BITS, W>(l, 1));
+        }
+        const uint32_t scales = R.c.scales[which][place * R.c.groups + (R.c.groups > 1 ? l >> 2 : 0)];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t c = BITS == 4 ? w[0] >> (4 * k) & 15u : w[k >> 2] >> (8 * (k & 3)) & 255u;
+            // 2^23 + code, less 2^23: the conversion instruction is a quarter as fast
+            x[k] = fmaf(__uint_as_float(c | 0x4b000000u) - 8388608.f, step_of(scales), zero_of(scales));
+        }
+    }
+    store8(static_cast<T *>(R.x[which]) + ((row.b * R.N + row.i) * R.c.H + row.h) * R.c.D + 8 * l, x, n, R.vector);
+}
+
+template <typename T, int BITS, int W> int launch(const RowsParams &R, bool write, cudaStream_t s) {
+    const long long per = write ? kThreads / (W == 2 ? 8 : 16) : 0;
+    const long long blocks = write ? (R.rows + per - 1) / per : (R.rows * 4 * W + kThreads - 1) / kThreads;
+    TPW_CHECK_ARG(blocks < (1LL << 31), "tpw_cache: more than 2^31 blocks of work");
+    if (write) {
+        cache_write_kernel<T, BITS, W><<<dim3((unsigned)blocks, 2), kThreads, 0, s>>>(R);
+        TPW_LAUNCH_OK("cache_write_kernel");
+    } else {
+        cache_read_kernel<T, BITS, W><<<dim3((unsigned)blocks, 2), kThreads, 0, s>>>(R);
+        TPW_LAUNCH_OK("cache_read_kernel");
+    }
+    return TPW_OK;
+}
+template <typename T> int launch_width(const RowsParams &R, bool write, cudaStream_t s) {
+    if (R.c.bits == 4) return R.c.width == 2 ? launch<T, 4, 2>(R, write, s) : R.c.width == 3 ? launch<T, 4, 3>(R, write, s) : launch<T, 4, 4>(R, write, s);
+    return R.c.width == 2 ? launch<T, 8, 2>(R, write, s) : R.c.width == 3 ? launch<T, 8, 3>(R, write, s) : launch<T, 8, 4>(R, write, s);
+}
+int run(const CacheParams &P, const tpw_cache_rows &rows, bool write, cudaStream_t s) {
+    RowsParams R = {};
+    R.c = P;
+    R.N = rows.N;
+    R.rows = P.B * P.H * rows.N;
+    R.from_start = !write && rows.from_start;
+    const long long piece = rows.dtype == TPW_F32 ? 4 : 8;
+    R.vector = P.D % 8 == 0;
+    for (int w = 0; w < 2; ++w) {
+        R.x[w] = rows.x[w];
+        R.vector = R.vector && aligned16(rows.x[w]);
+        for (int k = 0; k < 3; ++k) {
+            R.stride[w][k] = rows.stride[w][k];
+            R.vector = R.vector && (!write || rows.stride[w][k] % piece == 0);
+        }
+    }
+    return rows.dtype == TPW_F32 ? launch_width<float>(R, write, s) : rows.dtype == TPW_F16 ? launch_width<__half>(R, write, s) : launch_width<__nv_bfloat16>(R, write, s);
+}
+
+} // namespace
+
+int cache_write(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s) { return run(P, rows, true, s); }
+int cache_read(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s) { return run(P, rows, false, s); }
+
+} // namespace tpw
