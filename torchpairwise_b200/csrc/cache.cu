@@ -101,6 +101,7 @@ int tpw_cache_attention(const tpw_cache *c, const tpw_cache_attention_args *a, v
     if (e != TPW_OK || c->B == 0 || a->Nq == 0 || a->Hq == 0) return e;
     tpw::CacheAttnParams P = tpw::attention_params(*c, *a);
     const int64_t bytes = tpw::cache_attention_bytes(P);
+    if (bytes < 0) return TPW_ERR_INVALID;
     TPW_CHECK_ARG(bytes == 0 || (scratch && tpw::aligned16(scratch) && scratch_bytes >= bytes), "tpw_cache_attention: scratch of %lld bytes, 16-byte aligned, is needed", (long long)bytes);
     P.status = tpw::device_status_ptr();
     return tpw::cache_attention(P, scratch, static_cast<cudaStream_t>(stream));

@@ -43,12 +43,12 @@ struct CacheAttnParams {
 // cache_rows.cu
 int cache_write(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s);
 int cache_read(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s);
-// cache_attention.cu
+// cache_attention.cu; -1: refused
 long long cache_attention_bytes(const CacheAttnParams &P);
 int cache_attention(const CacheAttnParams &P, void *scratch, cudaStream_t s);
-// cache_few_4.cu, cache_few_8.cu
-int cache_few_4(const CacheAttnParams &P, int rows, int row_blocks, int splits, cudaStream_t s);
-int cache_few_8(const CacheAttnParams &P, int rows, int row_blocks, int splits, cudaStream_t s);
+// cache_few_4.cu, cache_few_8.cu; with `bytes` they only say how much scratch the call wants
+int cache_few_4(const CacheAttnParams &P, void *scratch, long long *bytes, cudaStream_t s);
+int cache_few_8(const CacheAttnParams &P, void *scratch, long long *bytes, cudaStream_t s);
 
 #ifdef __CUDACC__
 namespace {

@@ -3,17 +3,20 @@
 // Bound by HBM (4-bit codes with their steps and zeros: 160 bytes for a key and value of 128 features), closely followed by the instructions that unpack
 // them.  So the codes go into the products as they are: as the low bits of half-precision numbers they are whole multiples of 2^-24,
 // exactly, and masks are all the unpacking there is.
-//   scores   K q^T, m16n8k16, 16 keys by 8 query rows: sum_g step_jg (sum_d c_jd q_d) + zero_jg (sum_d q_d).  A row of q is lifted by a
-//            power of two to half precision's upper end; the sums begin at minus half the code range times sum_d q_d, so that they stay small.
-//   output   V^T P^T, 16 features by 8 rows: the steps go into the probabilities, (p_j step_jg) c_jd, the zeros into a sum beside it.
+//   scores   K q^T, m16n8k16, 16 keys by 8 query rows: sum_g step_jg (sum_d c_jd q_d - M a_g) + (zero_jg + M step_jg) a_g, a_g = sum_d q_d over
+//            the group and M the middle code, so that sums stay small.  The second term is a product of its own, bfloat16: a word of the cache, step
+//            and zero, is the operand, with M a_g and a_g.  A row of q is lifted by a power of two to half precision's upper end.
+//   output   V^T P^T, 16 features by 8 rows: the steps go into the probabilities, (p_j step_jg) c_jd; one more product adds p_j zero_jg, of the same
+//            rounded p_j.  A warp turns its keys' steps and zeros into half precision once, scaled by a power of two that they share.
 // With keys along M a product has 8 rows of queries; rows along M would leave half of every product empty for up to 8 heads that share a key.
 //
 // Float32 queries: q and p step as two half-precision parts each, 22 bits; codes of values less half their range, and the products of 16 keys go
 // to sums in registers, because tensor-core sums truncate.
 //
-// A CTA is a warp that issues bulk copies into a ring of 128-key stages, and four warps with 32 keys of a stage each and a running reference, sum
-// and output of their own.  The CTAs of a cluster take equal shares of a sequence's keys, whatever its length, and join through
-// distributed shared memory: no second launch, the same order every time.
+// All stages of keys (64 or 128) of all sequences and heads form one line that the CTAs, three on an SM, take equal shares of, whatever the lengths: a
+// share ends and begins anywhere in a sequence.  What a CTA has of a head that others have parts of goes to scratch, and a second kernel, whose launch
+// overlaps this one, weighs the parts together in their order.  In a CTA four warps take 16 keys or 32 of a stage each, with a running reference, sum and
+// output of their own; bulk copies bring the stages into a ring, across the ends of heads.
 #pragma once
 #include "attention_tc.cuh"
 #include "cache.cuh"
@@ -21,32 +24,41 @@
 namespace tpw {
 namespace {
 
-constexpr int kCacheStage = 128;     // keys
-constexpr int kCacheWarps = 4;       // that compute
-constexpr int kCacheThreads = 32 * (kCacheWarps + 1);
-constexpr int kLift = 6;             // probabilities times steps are lifted by 2^6 beside 2^8 that they may exceed their reference by: below 2^16,
-constexpr float kSlack = 8.f;        // and normal half-precision numbers down to 2^-20 of it
+constexpr int kFewWarps = 4, kFewThreads = 128;
+constexpr float kFewLift = 6.f;      // probabilities are lifted by 2^6 beside the 2^8 that they may exceed their reference by: below 2^16, and
+constexpr float kFewSlack = 8.f;     // normal half-precision numbers down to 2^-20 of it
 
 struct CacheFewParams {
     CacheAttnParams a;
     int rows, row_blocks;            // group * Nq, and blocks of them
-    int splits;                      // CTAs of a cluster
+    int whole;                       // a CTA for each head and block of rows, no joining
+    int q_vector;                    // rows of queries in 16-byte pieces
+    float *part_out;                 // [CTA][2][rows of a block][features of a row in storage]: of a head begun by another CTA, of one that this CTA begins
+    float2 *part_stats;              // [CTA][2][rows of a block]: reference (a power of 2) and sum
 };
 
-// NG: groups of a row; W: features / 32; NT: blocks of 8 query rows; PARTS: half-precision parts of queries and probabilities
-template <int BITS, int W, int NG, int NT> struct CacheFewSmem {
-    static constexpr uint32_t ROW = W * 4 * BITS, CODES = kCacheStage * ROW, SCALES = kCacheStage * NG * 4, STAGE = 2 * (CODES + SCALES);
-    static constexpr int kStages = 106496 / STAGE < 6 ? 106496 / STAGE : 6;
-    static constexpr uint32_t RING = kStages * STAGE, DP = 32 * W, ROWS = 8 * NT;
-    // when the keys are done: the warps' shares and statistics, then the CTA's
-    static constexpr uint32_t OFF_STATS = kCacheWarps * ROWS * DP * 4, OFF_RESULT = OFF_STATS + kCacheWarps * ROWS * 8, OFF_RESULT_STATS = OFF_RESULT + ROWS * DP * 4,
-                              SHARES = OFF_RESULT_STATS + ROWS * 8;
-    static constexpr uint32_t OFF_BAR = RING > SHARES ? RING : SHARES, OFF_FLAG = OFF_BAR + 16 * kStages, ALLOC = OFF_FLAG + 16;
+template <int BITS, int W, int NG, int NT, int PARTS> struct CacheFew {
+    static constexpr int KEYS = BITS == 4 ? 128 : 64, SUB = KEYS / 64;   // of a stage; blocks of 16 keys to a warp
+    static constexpr uint32_t ROW = W * 4 * BITS, CODES = KEYS * ROW, SCALES = KEYS * NG * 4, STAGE = 2 * (CODES + SCALES), DP = 32 * W, ROWS = 8 * NT;
+    static constexpr int PER_SM = NT == 1 ? 3 : 2;
+    static constexpr uint32_t STATS = kFewWarps * 8 * 8, PREPARED = PARTS == 1 ? kFewWarps * SUB * NG * 64 : 0, QUERIES = PARTS * NT * W * 512, SUMS = NT * (W + 1) * 32;
+    static constexpr uint32_t ROOM = (NT == 1 ? 75776 : 112640) - STATS - PREPARED - QUERIES - SUMS - 192;
+    static constexpr int kStages = ROOM / STAGE < 8 ? ROOM / STAGE : 8;
+    static_assert(kStages >= 2, "a ring of two stages at least");
+    static_assert(kFewWarps * 8 * DP * 4 <= STAGE, "the warps' shares of 8 rows fit a stage");
+    static constexpr uint32_t OFF_STATS = kStages * STAGE, OFF_PREPARED = OFF_STATS + STATS, OFF_QUERIES = OFF_PREPARED + PREPARED, OFF_SUMS = OFF_QUERIES + QUERIES,
+                              OFF_BAR = OFF_SUMS + SUMS, OFF_FLAG = OFF_BAR + 16 * kStages, ALLOC = OFF_FLAG + 16;
 };
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_f16(float (&d)[4], const float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     uint32_t r;
@@ -55,18 +67,14 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 }
 __device__ __forceinline__ uint32_t half2_of(float lo, float hi) { return Narrow<__half>::pack(lo, hi); }
 __device__ __forceinline__ uint32_t half2_rest(float lo, float hi) { return Narrow<__half>::rest(lo, hi); }
+__device__ __forceinline__ uint32_t half2_times(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e < 1 ? 1 : e > 254 ? 254 : e) << 23); }   // 2^(e - 127)
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ float4 ld_cluster4(uint32_t at) {
-    float4 r;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w) : "r"(at) : "memory");
-    return r;
-}
-__device__ __forceinline__ float2 ld_cluster2(uint32_t at) {
-    float2 r;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(r.x), "=f"(r.y) : "r"(at) : "memory");
-    return r;
 }
 // N 32-bit words that lie together, in the widest pieces that their number allows
 template <int N> __device__ __forceinline__ void load_words(uint32_t (&w)[N], const unsigned char *p) {
@@ -88,11 +96,67 @@ template <int N> __device__ __forceinline__ void load_words(uint32_t (&w)[N], co
     }
 }
 
-// the n-th feature of a row of queries, in 32 bits
-__device__ __forceinline__ float query(const CacheAttnParams &P, long long row, int n) {
-    if (P.dtype == TPW_F32) return static_cast<const float *>(P.q)[row + n];
-    if (P.dtype == TPW_F16) return __half2float(static_cast<const __half *>(P.q)[row + n]);
-    return __bfloat162float(static_cast<const __nv_bfloat16 *>(P.q)[row + n]);
+// 8 features of a row of queries in 32 bits, `n` of which there are
+__device__ __forceinline__ void load_query(float (&x)[8], const CacheFewParams &F, long long at, int n) {
+    const CacheAttnParams &P = F.a;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = 0.f;
+    if (n <= 0) return;
+    if (P.dtype == TPW_F32) {
+        const float *p = static_cast<const float *>(P.q) + at;
+        if (F.q_vector) {
+            const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+            x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        } else
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k < n) x[k] = p[k];
+        return;
+    }
+    const uint16_t *p = static_cast<const uint16_t *>(P.q) + at;
+    alignas(16) uint16_t v[8] = {};
+    if (F.q_vector) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(p);
+    else
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < n) v[k] = p[k];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = P.dtype == TPW_F16 ? __half2float(__ushort_as_half(v[k])) : __uint_as_float((uint32_t)v[k] << 16);
+}
+// 4 features of a row of results, `n` of which there are
+__device__ __forceinline__ void store_out(const CacheAttnParams &P, long long at, const float (&x)[4], int n) {
+    if (n <= 0) return;
+    const bool vector = P.c.D % 4 == 0;
+    if (P.dtype == TPW_F32) {
+        float *p = static_cast<float *>(P.out) + at;
+        if (vector) *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+        else
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k < n) p[k] = x[k];
+        return;
+    }
+    uint16_t *p = static_cast<uint16_t *>(P.out) + at;
+    const uint32_t a = P.dtype == TPW_F16 ? half2_of(x[0], x[1]) : Narrow<__nv_bfloat16>::pack(x[0], x[1]);
+    const uint32_t b = P.dtype == TPW_F16 ? half2_of(x[2], x[3]) : Narrow<__nv_bfloat16>::pack(x[2], x[3]);
+    if (vector) *reinterpret_cast<uint2 *>(p) = make_uint2(a, b);
+    else {
+        const uint16_t e[4] = {(uint16_t)a, (uint16_t)(a >> 16), (uint16_t)b, (uint16_t)(b >> 16)};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k < n) p[k] = e[k];
+    }
+}
+
+// four features of row r from the weighed sums of values and of probabilities, which are lifted beside their reference
+__device__ __forceinline__ void finish(const CacheAttnParams &P, int b, int hk, int r, int d, float (&v)[4], float reference, float sum) {
+    const int nq = (int)P.Nq, i = r % nq, h = (int)(hk * P.group) + r / nq;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= inv;
+    if (d == 0 && P.lse) P.lse[(b * P.Hq + h) * P.Nq + i] = sum == 0.f ? -INFINITY : (reference - kFewLift + log2f(sum)) * 0.69314718055994531f;
+    store_out(P, ((b * P.Nq + i) * P.Hq + h) * P.c.D + d, v, P.c.D - d);
 }
 
 // Of 16 keys, the one in slot s of a product (a row of K, a column of P).  In this order the rows that lanes of a quarter warp read lie in different
@@ -101,172 +165,309 @@ __device__ __forceinline__ int key_of_slot(int s) {
     const int t = (s >> 1) & 3;
     return (s & 8) + ((s & 1) ? 4 + (t ^ 1) : t);
 }
+__device__ __forceinline__ int slot_of_key(int k) { return (k & 8) + ((k & 4) ? 2 * ((k & 3) ^ 1) + 1 : 2 * (k & 3)); }
+
+// The keys of a sequence that any row sees, and their stages
+template <int KEYS> struct Stages {
+    int first, end, begin, count;
+    __device__ __forceinline__ Stages(const CacheAttnParams &P, int b) {
+        const CacheSeen see(P, b);
+        first = see.lo(0);
+        end = see.hi((int)P.Nq - 1);
+        begin = first & ~63;
+        count = end > first ? (end - begin + KEYS - 1) / KEYS : 0;
+    }
+};
+// The line of all stages: sequences one after the other, a sequence's items (heads, and blocks of rows of each) one after the other, an item's
+// stages in order.  An item with stages stands on the line for kFewExtra more, which come first: what beginning and ending it costs.
+// Found by the whole CTA (128 threads): how long the line is, and the sequence that place `at` (or item `item` of sequence `of`) lies in.
+constexpr int kFewExtra = 1;
+struct Line {
+    unsigned total, before;   // places in all; in sequences before `b`
+    int b;
+    // the first place of a CTA's share
+    __device__ __forceinline__ unsigned start(unsigned share, unsigned shares) const { return total / shares * share + total % shares * share / shares; }
+};
+template <int KEYS> __device__ __forceinline__ Line line_of(const CacheFewParams &F, int share, int shares, int of, unsigned (&room)[kFewWarps + 2]) {
+    const CacheAttnParams &P = F.a;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = (int)P.c.B, per = (B + kFewThreads - 1) / kFewThreads;
+    const unsigned items = (unsigned)P.c.H * F.row_blocks;
+    const int b0 = tid * per < B ? tid * per : B, b1 = b0 + per < B ? b0 + per : B;
+    auto places = [&](int b) {
+        const int n = Stages<KEYS>(P, b).count;
+        return n > 0 ? (n + kFewExtra) * items : 0u;
+    };
+    unsigned mine = 0, last = 0;
+    for (int b = b0; b < b1; ++b) mine += last = places(b);
+    unsigned up = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const unsigned x = __shfl_up_sync(0xffffffffu, up, d);
+        if (lane >= d) up += x;
+    }
+    if (lane == 31) room[warp] = up;
+    __syncthreads();
+    Line r = {0, 0, 0};
+    unsigned before = up - mine;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) {
+        if (w < warp) before += room[w];
+        r.total += room[w];
+    }
+    const unsigned at = of < 0 ? r.start(share, shares) : 0;
+    if (of < 0 ? before <= at && at < before + mine : b0 <= of && of < b1)
+        for (int b = b0; b < b1; ++b) {
+            const unsigned n = per == 1 ? last : places(b);
+            if (of < 0 ? at < before + n : b == of) {
+                room[kFewWarps] = b;
+                room[kFewWarps + 1] = before;
+                break;
+            }
+            before += n;
+        }
+    __syncthreads();
+    r.b = (int)room[kFewWarps];
+    r.before = room[kFewWarps + 1];
+    return r;
+}
 
 template <int BITS, int W, int NG, int NT, int PARTS>
-__global__ void __launch_bounds__(kCacheThreads, 2) cache_few_kernel(const CacheFewParams F) {
-    typedef CacheFewSmem<BITS, W, NG, NT> L;
+__global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>::PER_SM) cache_few_kernel(const CacheFewParams F) {
+    typedef CacheFew<BITS, W, NG, NT, PARTS> L;
     const CacheAttnParams &P = F.a;
-    constexpr int DP = 32 * W, ROWS = 8 * NT;
-    constexpr bool CENTRED = PARTS == 2;
+    constexpr int DP = 32 * W, ROWS = 8 * NT, SUB = L::SUB, KEYS = L::KEYS;
+    constexpr bool WIDE = PARTS == 2;
     constexpr float MIDDLE = BITS == 4 ? 8.f : 128.f;
     extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ unsigned room[kFewWarps + 2];
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *empty = full + L::kStages;
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_FLAG);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int rank = (int)(blockIdx.x % F.splits);
-    const unsigned item = blockIdx.x / F.splits;
-    const int block = (int)(item % F.row_blocks), bh = (int)(item / F.row_blocks), hk = (int)(bh % P.c.H), b = (int)(bh / P.c.H);
-    const int nq = (int)P.Nq, row0 = block * ROWS;
-    const CacheSeen see(P, b);
-    // keys that any row sees, and this CTA's stages of them
-    const int first = see.lo(0), end = see.hi(nq - 1), begin = first & ~63;
-    const int all = end > first ? (end - begin + kCacheStage - 1) / kCacheStage : 0;
-    const int u0 = (int)((long long)all * rank / F.splits), u1 = (int)((long long)all * (rank + 1) / F.splits), stages = u1 - u0;
+    const int nq = (int)P.Nq, items = (int)P.c.H * F.row_blocks;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < L::kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], kCacheWarps); }
+        for (int i = 0; i < L::kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], kFewWarps); }
         *abort_flag = 0;
         mbar_init_fence();
     }
-    __syncthreads();
+    // this CTA's share: `total` stages from stage `stage` of item `item` of sequence b on
+    int b, item, stage, total;
+    if (F.whole) {
+        b = (int)(blockIdx.x / items);
+        item = (int)(blockIdx.x % items);
+        stage = 0;
+        total = Stages<KEYS>(P, b).count;
+        __syncthreads();
+    } else {
+        const Line line = line_of<KEYS>(F, (int)blockIdx.x, (int)gridDim.x, -1, room);
+        unsigned at = line.start(blockIdx.x, gridDim.x), to = line.start(blockIdx.x + 1, gridDim.x);
+        if (at == to) return;
+        b = line.b;
+        unsigned n = Stages<KEYS>(P, b).count, inside = (at - line.before) % (n + kFewExtra);
+        item = (int)((at - line.before) / (n + kFewExtra));
+        stage = inside > kFewExtra ? (int)inside - kFewExtra : 0;
+        // stages of the share: places that stand for one
+        total = 0;
+        for (int of = b, i = item; at < to;) {
+            const unsigned places = n + kFewExtra - inside < to - at ? n + kFewExtra - inside : to - at, extra = inside < kFewExtra ? kFewExtra - inside : 0;
+            total += places > extra ? (int)(places - extra) : 0;
+            at += places;
+            inside = 0;
+            if (at < to && ++i == items) {
+                i = 0;
+                do n = Stages<KEYS>(P, ++of).count;
+                while (n == 0);
+            }
+        }
+        if (total == 0) return;
+    }
     auto give_up = [&](int site) {
         *abort_flag = 1;
         if (P.status) atomicCAS(P.status, 0, (23 << 16) | site);
     };
 
-    float m[NT][2], l[NT][2], o[NT][2 * W][4], zeros[NT][NG][2];   // of rows 2 t, 2 t + 1 of every block: reference (a power of 2), sums
-    int top_step = 0;                                              // largest exponent of a step of a value so far, as in its bits
-    if (warp == kCacheWarps) {
-        if (lane == 0) {
-            uint32_t issued = 0;
-            const long long place0 = (long long)bh * P.c.capacity;
-            for (int u = 0; u < stages; ++u) {
-                const uint32_t st = u % L::kStages;
-                if (u >= L::kStages && !wait_or_abort(&empty[st], parity_of_use(u, L::kStages) ^ 1, abort_flag)) {
-                    give_up(1);
-                    break;
-                }
-                // capacity and the stage's first key are multiples of 64
-                const long long j = begin + (long long)(u0 + u) * kCacheStage;
-                const uint32_t n = (uint32_t)(P.c.capacity - j < kCacheStage ? P.c.capacity - j : kCacheStage), to = smem_u32(smem) + st * L::STAGE;
-                mbar_expect_tx(&full[st], n * 2 * (L::ROW + NG * 4));
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    bulk_load(to + w * L::CODES, P.c.codes[w] + (place0 + j) * L::ROW, n * L::ROW, &full[st]);
-                    bulk_load(to + 2 * L::CODES + w * L::SCALES, P.c.scales[w] + (place0 + j) * NG, n * NG * 4, &full[st]);
-                }
-                issued = u + 1;
+    // Lane 0 of warp 0 also issues the copies, as many stages ahead as the ring has room for.
+    int ahead_b = b, ahead_item = item, ahead_stage = stage, issued = 0;
+    bool ok = true;
+    auto fill = [&](int limit) {
+        limit = limit < total ? limit : total;
+        while (issued < limit && ok) {
+            const uint32_t st = issued % L::kStages;
+            if (issued >= L::kStages && !(ok = wait_or_abort(&empty[st], parity_of_use(issued, L::kStages) ^ 1, abort_flag))) {
+                give_up(1);
+                return;
             }
-            if (*abort_flag)   // what was issued arrives before the CTA ends
-                for (uint32_t u = first_of_last_uses(issued, L::kStages); u < issued; ++u) mbar_wait_bounded(&full[u % L::kStages], parity_of_use(u, L::kStages));
+            const Stages<KEYS> S(P, ahead_b);
+            // the capacity and a stage's first key are multiples of 64
+            const long long j = S.begin + ahead_stage * KEYS, place = ((long long)ahead_b * P.c.H + ahead_item / F.row_blocks) * P.c.capacity + j;
+            const uint32_t n = (uint32_t)(P.c.capacity - j < KEYS ? P.c.capacity - j : KEYS), to = smem_u32(smem) + st * L::STAGE;
+            mbar_expect_tx(&full[st], n * 2 * (L::ROW + NG * 4));
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                bulk_load(to + w * L::CODES, P.c.codes[w] + place * L::ROW, n * L::ROW, &full[st]);
+                bulk_load(to + 2 * L::CODES + w * L::SCALES, P.c.scales[w] + place * NG, n * NG * 4, &full[st]);
+            }
+            ++issued;
+            if (++ahead_stage == S.count) {
+                ahead_stage = 0;
+                if (++ahead_item == items) {
+                    ahead_item = 0;
+                    do ++ahead_b;
+                    while (issued < total && Stages<KEYS>(P, ahead_b).count == 0);
+                }
+            }
         }
-    } else {
-        // Queries as operands: row g of a block, features 32 w + 8 t + (0 .. 7), in the order in which masks leave the codes of a key.  Row r is
-        // query r % nq of head hk * group + r / nq.
-        uint32_t q[PARTS][NT][W][2][2];
-        float start[NT][NG][2], factor[NT][2];   // -MIDDLE 2^-24 sum_d q_d; scores of 2^: factor times the raw ones
-        int lo[NT][2], hi[NT][2];
-#pragma unroll
-        for (int x = 0; x < NT; ++x) {
-            const int r = row0 + 8 * x + g;
+    };
+    if (threadIdx.x == 0) fill(L::kStages);
+
+    float2 *stats = reinterpret_cast<float2 *>(smem + L::OFF_STATS);
+    uint32_t *queries = reinterpret_cast<uint32_t *>(smem + L::OFF_QUERIES);   // [part][block][w][lane][4]
+    float *query_sums = reinterpret_cast<float *>(smem + L::OFF_SUMS);         // [block][w and, last, the factor of scores][row]
+    // [block of 16 keys][step, zero][group][slot]
+    uint16_t *prepared = reinterpret_cast<uint16_t *>(smem + L::OFF_PREPARED) + warp * SUB * NG * 32;
+    const int slot0 = key_of_slot(g), value0 = t, value1 = 4 + (t ^ 1);   // and 8 more
+    int used = 0;
+
+    do {
+        const Stages<KEYS> S(P, b);
+        const CacheSeen see(P, b);
+        const int hk = item / F.row_blocks, row0 = item % F.row_blocks * ROWS, stage0 = stage;
+        const int stages = S.count - stage < total - used ? S.count - stage : total - used;
+        // Queries as operands, a warp making those of every fourth block of 32 features: row g of a block, features 32 w + 8 t + (0 .. 7), in the order
+        // in which masks leave the codes of a key.  Row r is query r % nq of head hk * group + r / nq.
+#pragma unroll 1
+        for (int unit = warp; unit < NT * W; unit += kFewWarps) {
+            const int x = unit / W, w = unit % W, r = row0 + 8 * x + g;
             const bool valid = r < F.rows;
-            const long long row = b * P.q_s[0] + (valid ? r % nq : 0) * P.q_s[1] + (hk * P.group + (valid ? r / nq : 0)) * P.q_s[2];
-            auto feature = [&](int d) { return valid && d < P.c.D ? query(P, row, d) : 0.f; };
-            float top = 0.f;
+            const int h = valid ? r / nq : 0;
+            const long long row = b * P.q_s[0] + (valid ? r - h * nq : 0) * P.q_s[1] + (hk * P.group + h) * P.q_s[2] + 8 * t;
+            float y[8] = {}, top = 0.f;
 #pragma unroll
-            for (int w = 0; w < W; ++w)
+            for (int v = 0; v < W; ++v) {
+                float z[8];
+                load_query(z, F, row + 32 * v, valid ? P.c.D - (32 * v + 8 * t) : 0);
 #pragma unroll
-                for (int n = 0; n < 8; ++n) top = fmaxf(top, fabsf(feature(32 * w + 8 * t + n)));
+                for (int n = 0; n < 8; ++n) {
+                    top = fmaxf(top, fabsf(z[n]));
+                    if (v == w) y[n] = z[n];
+                }
+            }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // into [2^14, 2^15)
             int lift = 14 + 127 - (int)(__float_as_uint(top) >> 23);
             lift = top == 0.f ? 0 : lift > 100 ? 100 : lift < -100 ? -100 : lift;
-            const float by = __uint_as_float((uint32_t)(127 + lift) << 23);
-            float sums[NG] = {};
+            const float by = power_of_two(127 + lift);
+            float sum = 0.f;
+            uint32_t parts[PARTS][4];
 #pragma unroll
-            for (int w = 0; w < W; ++w) {
-                float y[8];
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int n = 0; n < 8; ++n) {
-                    y[n] = feature(32 * w + 8 * t + n) * by;
-                    const float high = __half2float(__float2half_rn(y[n]));
-                    sums[NG > 1 ? w : 0] += PARTS == 1 ? high : high + __half2float(__float2half_rn(y[n] - high));
+                for (int e = 0; e < 2; ++e) {
+                    const int n = BITS == 4 ? 2 * k + e : 4 * k + e;
+                    const float s = BITS == 4 && e ? 0.0625f : 1.f, y0 = y[n] * by, y1 = y[n + (BITS == 4 ? 4 : 2)] * by;
+                    const float h0 = __half2float(__float2half_rn(y0)), h1 = __half2float(__float2half_rn(y1));
+                    parts[0][2 * k + e] = half2_of(h0 * s, h1 * s);
+                    sum += h0 + h1;
+                    if constexpr (WIDE) {
+                        const float r0 = __half2float(__float2half_rn(y0 - h0)), r1 = __half2float(__float2half_rn(y1 - h1));
+                        parts[1][2 * k + e] = half2_of(r0 * s, r1 * s);
+                        sum += r0 + r1;
+                    }
                 }
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
+            for (int part = 0; part < PARTS; ++part)
+                *reinterpret_cast<uint4 *>(queries + ((part * NT * W + unit) * 32 + lane) * 4) = make_uint4(parts[part][0], parts[part][1], parts[part][2], parts[part][3]);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if (t == 0) {
+                query_sums[(x * (W + 1) + w) * 8 + g] = sum * 5.9604644775390625e-8f;   // 2^-24, the unit of codes
+                if (w == 0) query_sums[(x * (W + 1) + W) * 8 + g] = fmaxf(P.scale_log2 * power_of_two(127 + 24 - lift), 1.17549435e-38f);
+            }
+        }
+        __syncthreads();
+        uint32_t q[PARTS][NT][W][2][2], qz[NT][PARTS][2];
+        float start[NT][NG][4], factor[NT][2];   // -M a_g; raw scores times the factor are powers of 2
+        int lo[NT][2], hi[NT][2];
+        float m[NT][2], l[NT][2], o[NT][2 * W][4], zeros[NT][NG][2], zero_sums[NT][4];   // rows 2 t, 2 t + 1 of every block: reference (a power of 2), sums
+        int top_scale = 1;                       // largest exponent of a step or zero of a value so far, as in its bits
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int n = BITS == 4 ? 2 * k + e : 4 * k + e;
-                        const float s = BITS == 4 && e ? 0.0625f : 1.f, y0 = y[n], y1 = y[n + (BITS == 4 ? 4 : 2)];
-                        q[0][x][w][k][e] = half2_of(y0 * s, y1 * s);
-                        if constexpr (PARTS == 2) {
-                            const float h0 = __half2float(__float2half_rn(y0)), h1 = __half2float(__float2half_rn(y1));
-                            q[1][x][w][k][e] = half2_of((y0 - h0) * s, (y1 - h1) * s);
-                        }
-                    }
+        for (int x = 0; x < NT; ++x) {
+            const float *sums = query_sums + x * (W + 1) * 8;
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(queries + ((part * NT * W + x * W + w) * 32 + lane) * 4);
+                    q[part][x][w][0][0] = v.x; q[part][x][w][0][1] = v.y;
+                    q[part][x][w][1][0] = v.z; q[part][x][w][1][1] = v.w;
+                }
+            float own = 0.f;   // a of row g, group t, in parts of 8 bits beside M times it
+            if (NG > 1) own = t < NG ? sums[t * 8 + g] : 0.f;
+            else if (t == 0)
+#pragma unroll
+                for (int w = 0; w < W; ++w) own += sums[w * 8 + g];
+#pragma unroll
+            for (int part = 0; part < 2 * PARTS; ++part) {
+                const uint32_t word = Narrow<__nv_bfloat16>::pack(own * MIDDLE, own);
+                qz[x][part / 2][part % 2] = word;
+                own -= __uint_as_float(word & 0xffff0000u);
             }
 #pragma unroll
-            for (int k = 0; k < NG; ++k) {
-                sums[k] += __shfl_xor_sync(0xffffffffu, sums[k], 1);
-                sums[k] += __shfl_xor_sync(0xffffffffu, sums[k], 2);
-            }
-            const float f = P.scale_log2 * __uint_as_float((uint32_t)(127 + 24 - lift) << 23);
+            for (int e = 0; e < 2; ++e) {
+                const int row = 2 * t + e, mine = row0 + 8 * x + row;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {   // of row 2 t + e, which lanes 4 (2 t + e) have
-                const int from = 4 * (2 * t + e), mine = row0 + 8 * x + 2 * t + e;
+                for (int k = 0; k < NG; ++k) {
+                    float a = 0.f;
+                    if (NG > 1) a = sums[k * 8 + row];
+                    else
 #pragma unroll
-                for (int k = 0; k < NG; ++k) start[x][k][e] = -MIDDLE * 5.9604644775390625e-8f * __shfl_sync(0xffffffffu, sums[k], from);
-                factor[x][e] = fmaxf(__shfl_sync(0xffffffffu, f, from), 1.17549435e-38f);
-                lo[x][e] = mine < F.rows ? see.lo(mine % nq) : 0;
-                hi[x][e] = mine < F.rows ? see.hi(mine % nq) : 1 << 30;
+                        for (int w = 0; w < W; ++w) a += sums[w * 8 + row];
+                    start[x][k][e] = start[x][k][2 + e] = -MIDDLE * a;
+                    zeros[x][k][e] = 0.f;
+                }
+                factor[x][e] = sums[W * 8 + row];
+                const int i = mine < F.rows ? mine % nq : 0;
+                lo[x][e] = mine < F.rows ? see.lo(i) : 0;
+                hi[x][e] = mine < F.rows ? see.hi(i) : 1 << 30;
                 m[x][e] = -INFINITY;
                 l[x][e] = 0.f;
-#pragma unroll
-                for (int k = 0; k < NG; ++k) zeros[x][k][e] = 0.f;
             }
 #pragma unroll
             for (int n = 0; n < 2 * W; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[x][n][e] = 0.f;
-        }
-        float step_by = 0.f;   // 2^kLift over the power of two in top_step
-        const int slot0 = key_of_slot(g), value0 = t, value1 = 4 + (t ^ 1);   // and 8 more
-        for (int u = 0; u < stages; ++u) {
-            const uint32_t st = u % L::kStages;
-            const bool ok = __all_sync(0xffffffffu, wait_or_abort(&full[st], parity_of_use(u, L::kStages), abort_flag));
-            if (!ok) {
-                give_up(2);
-                break;
-            }
-            const int j0 = begin + (u0 + u) * kCacheStage + 32 * warp;
-            if (j0 < end && j0 + 32 > first) {
-                const unsigned char *k_at = smem + st * L::STAGE + 32 * warp * L::ROW, *v_at = k_at + L::CODES;
-                const unsigned char *ks_at = smem + st * L::STAGE + 2 * L::CODES + 32 * warp * NG * 4, *vs_at = ks_at + L::SCALES;
-                float p[2][NT][4];
-                uint32_t vs[2][2][NG];   // [16 keys][slots g, g + 8][group]
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t kw[2][W * BITS / 4], ks[2][NG];
+            for (int e = 0; e < 4; ++e) zero_sums[x][e] = 0.f;
+        }
+        for (int u = 0; u < stages; ++u, ++used) {
+            const uint32_t st = used % L::kStages;
+            if (ok && !(ok = __all_sync(0xffffffffu, wait_or_abort(&full[st], parity_of_use(used, L::kStages), abort_flag)))) give_up(2);
+            const int j0 = S.begin + (stage0 + u) * KEYS + 16 * SUB * warp;
+            if (ok && j0 < S.end && j0 + 16 * SUB > S.first) {
+                const unsigned char *k_at = smem + st * L::STAGE + 16 * SUB * warp * L::ROW, *v_at = k_at + L::CODES;
+                const unsigned char *ks_at = smem + st * L::STAGE + 2 * L::CODES + 16 * SUB * warp * NG * 4, *vs_at = ks_at + L::SCALES;
+                float p[SUB][NT][4];
+#pragma unroll
+                for (int h = 0; h < SUB; ++h) {
+                    uint32_t kw[2][W * BITS / 4], ks[2][NG], kz[2];
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
                         const int key = 16 * h + 8 * s + slot0;
                         load_words(kw[s], k_at + key * L::ROW + t * (W * BITS));
                         load_words(ks[s], ks_at + key * NG * 4);
-                        load_words(vs[h][s], vs_at + key * NG * 4);
+                        kz[s] = t < NG ? reinterpret_cast<const uint32_t *>(ks_at)[key * NG + (t < NG ? t : 0)] : 0u;
                     }
 #pragma unroll
-                    for (int x = 0; x < NT; ++x)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) p[h][x][e] = 0.f;
+                    for (int x = 0; x < NT; ++x) {
+                        const float none[4] = {};
+                        mma_bf16(p[h][x], none, kz[0], kz[1], kz[0], kz[1], qz[x][0][0], qz[x][0][1]);
+                        if constexpr (WIDE) mma_bf16(p[h][x], p[h][x], kz[0], kz[1], kz[0], kz[1], qz[x][1][0], qz[x][1][1]);
+                    }
                     float acc[NT][4];
 #pragma unroll
                     for (int w = 0; w < W; ++w) {
-                        if (NG > 1 || w == 0)
-#pragma unroll
-                            for (int x = 0; x < NT; ++x)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) acc[x][e] = start[x][NG > 1 ? w : 0][e & 1];
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             uint32_t a[4];
@@ -285,18 +486,19 @@ __global__ void __launch_bounds__(kCacheThreads, 2) cache_few_kernel(const Cache
 #pragma unroll
                             for (int x = 0; x < NT; ++x)
 #pragma unroll
-                                for (int part = 0; part < PARTS; ++part) mma_f16(acc[x], a[0], a[1], a[2], a[3], q[part][x][w][k][0], q[part][x][w][k][1]);
+                                for (int part = 0; part < PARTS; ++part) {
+                                    const bool fresh = k == 0 && part == 0 && (NG > 1 || w == 0);
+                                    mma_f16(acc[x], fresh ? start[x][NG > 1 ? w : 0] : acc[x], a[0], a[1], a[2], a[3], q[part][x][w][k][0], q[part][x][w][k][1]);
+                                }
                         }
                         if (NG > 1 || w == W - 1)
 #pragma unroll
                             for (int s = 0; s < 2; ++s) {
-                                const uint32_t sc = ks[s][NG > 1 ? w : 0];
-                                const float step = step_of(sc), shift = fmaf(zero_of(sc), -1.f / MIDDLE, -step);
+                                const float step = step_of(ks[s][NG > 1 ? w : 0]);
 #pragma unroll
                                 for (int x = 0; x < NT; ++x)
 #pragma unroll
-                                    for (int e = 0; e < 2; ++e)
-                                        p[h][x][2 * s + e] = fmaf(shift, start[x][NG > 1 ? w : 0][e], fmaf(step, acc[x][2 * s + e], p[h][x][2 * s + e]));
+                                    for (int e = 0; e < 2; ++e) p[h][x][2 * s + e] = fmaf(step, acc[x][2 * s + e], p[h][x][2 * s + e]);
                             }
                     }
 #pragma unroll
@@ -304,15 +506,18 @@ __global__ void __launch_bounds__(kCacheThreads, 2) cache_few_kernel(const Cache
 #pragma unroll
                         for (int e = 0; e < 4; ++e) p[h][x][e] *= factor[x][e & 1];
                 }
+                // steps and zeros of values, a lane to a key
+                uint32_t vs[NG];
+                load_words(vs, vs_at + (lane % (16 * SUB)) * NG * 4);
                 // keys that some row does not see; steps and zeros of those that none sees need not be numbers
-                bool edge = j0 < first || j0 + 32 > end;
+                bool edge = j0 < S.first || j0 + 16 * SUB > S.end;
 #pragma unroll
                 for (int x = 0; x < NT; ++x)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) edge = edge || j0 < lo[x][e] || j0 + 32 > hi[x][e];
+                    for (int e = 0; e < 2; ++e) edge = edge || j0 < lo[x][e] || j0 + 16 * SUB > hi[x][e];
                 if (__any_sync(0xffffffffu, edge)) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                    for (int h = 0; h < SUB; ++h)
 #pragma unroll
                         for (int s = 0; s < 2; ++s) {
                             const int j = j0 + 16 * h + 8 * s + slot0;
@@ -320,69 +525,84 @@ __global__ void __launch_bounds__(kCacheThreads, 2) cache_few_kernel(const Cache
                             for (int x = 0; x < NT; ++x)
 #pragma unroll
                                 for (int e = 0; e < 2; ++e)
-                                    if (j < lo[x][e] || j >= hi[x][e] || j >= end) p[h][x][2 * s + e] = -INFINITY;
-#pragma unroll
-                            for (int k = 0; k < NG; ++k)
-                                if (j < first || j >= end) vs[h][s][k] = 0;
+                                    if (j < lo[x][e] || j >= hi[x][e] || j >= S.end) p[h][x][2 * s + e] = -INFINITY;
                         }
+                    const int j = j0 + lane % (16 * SUB);
+                    if (j < S.first || j >= S.end)
+#pragma unroll
+                        for (int k = 0; k < NG; ++k) vs[k] = 0;
                 }
-                // the reference moves, and sums are scaled, only where a score or a step has left it behind
-                int high_step = 0;
+                // the reference moves, and sums are scaled, only where a score, a step or a zero has left it behind
+                uint32_t high_scale = 0;
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int s = 0; s < 2; ++s)
-#pragma unroll
-                        for (int k = 0; k < NG; ++k) high_step = max(high_step, (int)(vs[h][s][k] & 0xffffu));
-                bool moves = high_step >> 7 > top_step;
+                for (int k = 0; k < NG; ++k) high_scale = max(high_scale, max(vs[k] << 16, vs[k] & 0x7fff0000u));
+                bool moves = (int)(high_scale >> 23) > top_scale;
                 float high[NT][2];
 #pragma unroll
                 for (int x = 0; x < NT; ++x)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        high[x][e] = fmaxf(fmaxf(p[0][x][e], p[0][x][2 + e]), fmaxf(p[1][x][e], p[1][x][2 + e]));
-                        moves = moves || high[x][e] > m[x][e] + kSlack;
+                        high[x][e] = fmaxf(p[0][x][e], p[0][x][2 + e]);
+                        if constexpr (SUB == 2) high[x][e] = fmaxf(high[x][e], fmaxf(p[1][x][e], p[1][x][2 + e]));
+                        moves = moves || high[x][e] > m[x][e] + kFewSlack;
                     }
                 if (__any_sync(0xffffffffu, moves)) {
-                    const int now = max(__reduce_max_sync(0xffffffffu, high_step >> 7), top_step);
-                    const float by_step = now > top_step && now - top_step < 127 ? __uint_as_float((uint32_t)(127 + top_step - now) << 23) : now > top_step ? 0.f : 1.f;
-                    top_step = now;
-                    step_by = __uint_as_float((uint32_t)(254 + kLift - (now > 7 ? now : 7)) << 23);
+                    const int now = max((int)(__reduce_max_sync(0xffffffffu, high_scale) >> 23), top_scale);
+                    const float by_scale = now - top_scale < 126 ? power_of_two(127 + top_scale - now) : 0.f;
+                    top_scale = now;
 #pragma unroll
-                    for (int x = 0; x < NT; ++x)
+                    for (int x = 0; x < NT; ++x) {
+                        float by[2];
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             float top = high[x][e];
 #pragma unroll
                             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
                             top = fmaxf(top, m[x][e]);
-                            const float by = top == m[x][e] ? 1.f : exp2_fast(m[x][e] - top);
+                            by[e] = top == m[x][e] ? 1.f : exp2_fast(m[x][e] - top);
                             m[x][e] = top;
-                            l[x][e] *= by;
+                            l[x][e] *= by[e];
 #pragma unroll
-                            for (int k = 0; k < NG; ++k) zeros[x][k][e] *= by;
-#pragma unroll
-                            for (int n = 0; n < 2 * W; ++n) {
-                                o[x][n][e] *= by * by_step;
-                                o[x][n][2 + e] *= by * by_step;
-                            }
+                            for (int k = 0; k < NG; ++k) zeros[x][k][e] *= by[e];
+                            by[e] *= by_scale;
                         }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            zero_sums[x][e] *= by[e & 1];
+#pragma unroll
+                            for (int n = 0; n < 2 * W; ++n) o[x][n][e] *= by[e & 1];
+                        }
+                    }
+                }
+                const float norm = power_of_two(253 - top_scale);   // steps and zeros below 1
+                if constexpr (!WIDE) {
+                    __syncwarp();   // the last ones are read
+                    if (lane < 16 * SUB) {
+                        uint16_t *to = prepared + (lane >> 4) * NG * 32 + slot_of_key(lane & 15);
+#pragma unroll
+                        for (int k = 0; k < NG; ++k) {
+                            const uint32_t both = half2_of(step_of(vs[k]) * norm, zero_of(vs[k]) * norm);
+                            to[16 * k] = (uint16_t)both;
+                            to[16 * (NG + k)] = (uint16_t)(both >> 16);
+                        }
+                    }
+                    __syncwarp();
                 }
 #pragma unroll
                 for (int x = 0; x < NT; ++x)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float shift = m[x][e] == -INFINITY ? 0.f : m[x][e];
+                        const float shift = m[x][e] == -INFINITY ? 0.f : kFewLift - m[x][e];
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
+                        for (int h = 0; h < SUB; ++h)
 #pragma unroll
                             for (int s = 0; s < 2; ++s) {
-                                p[h][x][2 * s + e] = exp2_fast(p[h][x][2 * s + e] - shift);
+                                p[h][x][2 * s + e] = exp2_fast(p[h][x][2 * s + e] + shift);
                                 l[x][e] += p[h][x][2 * s + e];
                             }
                     }
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < SUB; ++h) {
                     constexpr int UNITS = BITS == 4 ? 2 * W : 4 * W;   // bytes of a lane's codes of a value
                     uint32_t vw[4][(UNITS + 3) / 4];                   // of slots 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
@@ -394,21 +614,41 @@ __global__ void __launch_bounds__(kCacheThreads, 2) cache_few_kernel(const Cache
                             vw[s][1] = *reinterpret_cast<const uint16_t *>(at + 4);
                         }
                     }
-                    uint32_t y[PARTS][NT][2];
+                    // probabilities (times steps) as operands: slots 2 t, 2 t + 1 and 2 t + 8, 2 t + 9 of row g
+                    uint32_t y[PARTS][NT][2], pt[NT][2];
+                    const uint16_t *ready = prepared + h * NG * 32 + 2 * t;
+                    if constexpr (!WIDE) {
+                        const uint16_t *z = ready + 16 * (NG + (g < NG ? g : 0));
+                        const uint32_t z0 = g < NG ? *reinterpret_cast<const uint32_t *>(z) : 0u, z1 = g < NG ? *reinterpret_cast<const uint32_t *>(z + 8) : 0u;
+#pragma unroll
+                        for (int x = 0; x < NT; ++x) {
+#pragma unroll
+                            for (int s = 0; s < 2; ++s) pt[x][s] = transposed(half2_of(p[h][x][2 * s], p[h][x][2 * s + 1]));
+                            mma_f16(zero_sums[x], zero_sums[x], z0, 0u, z1, 0u, pt[x][0], pt[x][1]);
+                        }
+                    }
 #pragma unroll
                     for (int w = 0; w < W; ++w) {
                         if (NG > 1 || w == 0)
 #pragma unroll
                             for (int s = 0; s < 2; ++s) {
-                                const uint32_t sc = vs[h][s][NG > 1 ? w : 0];
-                                const float step = step_of(sc) * step_by, zero = CENTRED ? fmaf(step_of(sc), MIDDLE, zero_of(sc)) : zero_of(sc);
+                                if constexpr (!WIDE) {
+                                    const uint32_t step = *reinterpret_cast<const uint32_t *>(ready + 16 * (NG > 1 ? w : 0) + 8 * s);
 #pragma unroll
-                                for (int x = 0; x < NT; ++x) {
-                                    const float p0 = p[h][x][2 * s], p1 = p[h][x][2 * s + 1];
-                                    zeros[x][NG > 1 ? w : 0][0] = fmaf(p0, zero, zeros[x][NG > 1 ? w : 0][0]);
-                                    zeros[x][NG > 1 ? w : 0][1] = fmaf(p1, zero, zeros[x][NG > 1 ? w : 0][1]);
-                                    y[0][x][s] = transposed(half2_of(p0 * step, p1 * step));
-                                    if constexpr (PARTS == 2) y[1][x][s] = transposed(half2_rest(p0 * step, p1 * step));
+                                    for (int x = 0; x < NT; ++x) y[0][x][s] = half2_times(pt[x][s], step);
+                                } else {
+                                    const int key = 16 * h + 8 * s + slot0, j = j0 + key;
+                                    uint32_t sc = reinterpret_cast<const uint32_t *>(vs_at)[key * NG + (NG > 1 ? w : 0)];
+                                    if (j < S.first || j >= S.end) sc = 0;
+                                    const float step = step_of(sc) * norm, zero = fmaf(step_of(sc), MIDDLE, zero_of(sc));
+#pragma unroll
+                                    for (int x = 0; x < NT; ++x) {
+                                        const float p0 = p[h][x][2 * s], p1 = p[h][x][2 * s + 1];
+                                        zeros[x][NG > 1 ? w : 0][0] = fmaf(p0, zero, zeros[x][NG > 1 ? w : 0][0]);
+                                        zeros[x][NG > 1 ? w : 0][1] = fmaf(p1, zero, zeros[x][NG > 1 ? w : 0][1]);
+                                        y[0][x][s] = transposed(half2_of(p0 * step, p1 * step));
+                                        y[1][x][s] = transposed(half2_rest(p0 * step, p1 * step));
+                                    }
                                 }
                             }
 #pragma unroll
@@ -425,7 +665,7 @@ __global__ void __launch_bounds__(kCacheThreads, 2) cache_few_kernel(const Cache
                                     a[2 * s] = c & 0x00ff00ffu;
                                     a[2 * s + 1] = (c >> 8) & 0x00ff00ffu;
                                 }
-                                if constexpr (CENTRED)   // codes less the middle, as numbers
+                                if constexpr (WIDE)   // codes less the middle, as numbers
 #pragma unroll
                                     for (int e = 0; e < 2; ++e) {
                                         const uint32_t c = a[2 * s + e] | 0x64006400u;   // 1024 + code, for the upper 4 bits 1024 + 16 code
@@ -436,12 +676,12 @@ __global__ void __launch_bounds__(kCacheThreads, 2) cache_few_kernel(const Cache
                             }
 #pragma unroll
                             for (int x = 0; x < NT; ++x) {
-                                if constexpr (PARTS == 1) {
-                                    mma_f16(o[x][2 * w + k], a[0], a[1], a[2], a[3], y[0][x][0], y[0][x][1]);
+                                if constexpr (!WIDE) {
+                                    mma_f16(o[x][2 * w + k], o[x][2 * w + k], a[0], a[1], a[2], a[3], y[0][x][0], y[0][x][1]);
                                 } else {
                                     float sum[4] = {};
 #pragma unroll
-                                    for (int part = 0; part < PARTS; ++part) mma_f16(sum, a[0], a[1], a[2], a[3], y[part][x][0], y[part][x][1]);
+                                    for (int part = 0; part < PARTS; ++part) mma_f16(sum, sum, a[0], a[1], a[2], a[3], y[part][x][0], y[part][x][1]);
 #pragma unroll
                                     for (int e = 0; e < 4; ++e) o[x][2 * w + k][e] += sum[e];
                                 }
@@ -452,141 +692,196 @@ __global__ void __launch_bounds__(kCacheThreads, 2) cache_few_kernel(const Cache
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[st]);
+            // the last stage's room is where the warps' outputs meet: it is filled anew after that
+            if (threadIdx.x == 0 && u + 1 < stages) fill(used + L::kStages);
+            ok = __shfl_sync(0xffffffffu, ok, 0);
         }
-    }
-    __syncthreads();
-    // The warps' shares meet in the ring: [warp][row][feature] outputs, [warp][row] reference and sum
-    const bool failed = *abort_flag != 0;
-    float *share = reinterpret_cast<float *>(smem), *result = reinterpret_cast<float *>(smem + L::OFF_RESULT);
-    float2 *stats = reinterpret_cast<float2 *>(smem + L::OFF_STATS), *result_stats = reinterpret_cast<float2 *>(smem + L::OFF_RESULT_STATS);
-    if (warp < kCacheWarps) {
-        const int power = (top_step > 7 ? top_step : 7) - 127 - kLift + (CENTRED ? 0 : 24);
-        // as two factors: their exponents stay within 32 bits' range
-        const float unit = ldexpf(1.f, power / 2), unit2 = ldexpf(1.f, power - power / 2), upper = BITS == 4 && !CENTRED ? 0.0625f : 1.f;
+        // The warps' outputs meet, 8 rows at a time: [warp][row][feature] beside references and sums.  A thread weighs four features of a row together.
+        float *share = reinterpret_cast<float *>(smem + (used > 0 ? (used - 1) % L::kStages : 0) * L::STAGE);
+        const int power = top_scale + 1 - 127;
+        // two factors: either's exponent stays within 32 bits' range
+        const float unit = power_of_two(127 + power / 2), unit2 = power_of_two(127 + power - power / 2);
+        const float code = WIDE ? unit2 : unit2 * 16777216.f, code_upper = BITS == 4 && !WIDE ? code * 0.0625f : code;
+        const bool all = stages == S.count;
+        const long long part = ((long long)blockIdx.x * 2 + (stage0 == 0 ? 1 : 0)) * ROWS;
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
+        for (int x = 0; x < NT; ++x) {
+            __syncthreads();
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) {
                     l[x][e] += __shfl_xor_sync(0xffffffffu, l[x][e], d);
+                    if constexpr (WIDE)
 #pragma unroll
-                    for (int k = 0; k < NG; ++k) zeros[x][k][e] += __shfl_xor_sync(0xffffffffu, zeros[x][k][e], d);
+                        for (int k = 0; k < NG; ++k) zeros[x][k][e] += __shfl_xor_sync(0xffffffffu, zeros[x][k][e], d);
                 }
-                const int row = 8 * x + 2 * t + e;
-                if (g == 0) stats[warp * ROWS + row] = make_float2(m[x][e], l[x][e]);
+                if constexpr (!WIDE)   // row g of zero_sums is group g
+#pragma unroll
+                    for (int k = 0; k < NG; ++k) zeros[x][k][e] = __shfl_sync(0xffffffffu, zero_sums[x][e], 4 * k + t) * unit * unit2;
+                const int row = 2 * t + e;
+                if (row0 + 8 * x + row >= F.rows) continue;
+                if (g == 0) stats[warp * 8 + row] = make_float2(m[x][e], l[x][e]);
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
                     const float z = zeros[x][NG > 1 ? w : 0][e];
                     float4 v;
-                    v.x = fmaf(o[x][2 * w][e] * unit, unit2, z);
-                    v.y = fmaf(o[x][2 * w][2 + e] * unit, unit2 * upper, z);
-                    v.z = fmaf(o[x][2 * w + 1][e] * unit, unit2, z);
-                    v.w = fmaf(o[x][2 * w + 1][2 + e] * unit, unit2 * upper, z);
-                    *reinterpret_cast<float4 *>(share + (warp * ROWS + row) * DP + 32 * w + 4 * g) = v;
+                    v.x = fmaf(o[x][2 * w][e] * unit, code, z);
+                    v.y = fmaf(o[x][2 * w][2 + e] * unit, code_upper, z);
+                    v.z = fmaf(o[x][2 * w + 1][e] * unit, code, z);
+                    v.w = fmaf(o[x][2 * w + 1][2 + e] * unit, code_upper, z);
+                    *reinterpret_cast<float4 *>(share + (warp * 8 + row) * DP + 32 * w + 4 * g) = v;
                 }
             }
-    }
-    __syncthreads();
-    auto weight = [](float mine, float top) { return mine == -INFINITY ? 0.f : exp2_fast(mine - top); };   // NaN of a NaN
-    for (int at = threadIdx.x; at < ROWS * DP / 4; at += kCacheThreads) {
-        const int row = at / (DP / 4), d = at % (DP / 4) * 4;
-        float top = -INFINITY, sum = 0.f;
+            __syncthreads();
+            for (int at = threadIdx.x; at < 8 * DP / 4; at += kFewThreads) {
+                const int row = at / (DP / 4), d = at % (DP / 4) * 4, r = row0 + 8 * x + row;
+                if (r >= F.rows || !ok) break;
+                float2 s[kFewWarps];
+                float top = -INFINITY, sum = 0.f, v[4] = {};
 #pragma unroll
-        for (int w = 0; w < kCacheWarps; ++w) top = fmaxf(top, stats[w * ROWS + row].x);
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int w = 0; w < kFewWarps; ++w) {
+                    s[w] = stats[w * 8 + row];
+                    top = fmaxf(top, s[w].x);
+                }
 #pragma unroll
-        for (int w = 0; w < kCacheWarps; ++w) {
-            const float2 s = stats[w * ROWS + row];
-            if (s.y == 0.f) continue;   // saw nothing; what stands beside it need not be a number
-            const float by = s.x == -INFINITY ? s.y : weight(s.x, top);   // a sum with no reference is NaN
-            sum = fmaf(by, s.y, sum);
-            const float4 z = *reinterpret_cast<const float4 *>(share + (w * ROWS + row) * DP + d);
-            v.x = fmaf(by, z.x, v.x);
-            v.y = fmaf(by, z.y, v.y);
-            v.z = fmaf(by, z.z, v.z);
-            v.w = fmaf(by, z.w, v.w);
-        }
-        *reinterpret_cast<float4 *>(result + row * DP + d) = v;
-        if (d == 0) result_stats[row] = make_float2(top, sum);
-    }
-    if (F.splits > 1) cluster_sync();
-    else __syncthreads();
-    // the CTAs' results meet: a CTA finishes every splits-th row
-    for (int at = threadIdx.x; at < ROWS * DP / 4; at += kCacheThreads) {
-        const int row = at / (DP / 4), d = at % (DP / 4) * 4, r = row0 + row;
-        if (row % F.splits != rank || r >= F.rows || d >= P.c.D || failed) continue;
-        float top = -INFINITY, sum = 0.f;
-        for (int s = 0; s < F.splits; ++s) top = fmaxf(top, ld_cluster2(cluster_addr(result_stats + row, s)).x);
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < F.splits; ++s) {
-            const float2 z = ld_cluster2(cluster_addr(result_stats + row, s));
-            if (z.y == 0.f) continue;
-            const float by = z.x == -INFINITY ? z.y : weight(z.x, top);
-            sum = fmaf(by, z.y, sum);
-            const float4 y = ld_cluster4(cluster_addr(result + row * DP + d, s));
-            v.x = fmaf(by, y.x, v.x);
-            v.y = fmaf(by, y.y, v.y);
-            v.z = fmaf(by, y.z, v.z);
-            v.w = fmaf(by, y.w, v.w);
-        }
-        const int i = r % nq, h = (int)(hk * P.group) + r / nq, n = P.c.D - d;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const float out[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
-        const long long to = ((b * P.Nq + i) * P.Hq + h) * P.c.D + d;
-        if (d == 0 && P.lse) P.lse[(b * P.Hq + h) * P.Nq + i] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
-        if (P.dtype == TPW_F32) {
-            float *dst = static_cast<float *>(P.out) + to;
-            if (P.c.D % 4 == 0) *reinterpret_cast<float4 *>(dst) = make_float4(out[0], out[1], out[2], out[3]);
-            else
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (e < n) dst[e] = out[e];
-        } else {
-            const uint32_t a = P.dtype == TPW_F16 ? half2_of(out[0], out[1]) : Narrow<__nv_bfloat16>::pack(out[0], out[1]);
-            const uint32_t c = P.dtype == TPW_F16 ? half2_of(out[2], out[3]) : Narrow<__nv_bfloat16>::pack(out[2], out[3]);
-            uint16_t *dst = static_cast<uint16_t *>(P.out) + to;
-            if (P.c.D % 4 == 0) *reinterpret_cast<uint2 *>(dst) = make_uint2(a, c);
-            else {
-                const uint16_t e[4] = {(uint16_t)a, (uint16_t)(a >> 16), (uint16_t)c, (uint16_t)(c >> 16)};
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (k < n) dst[k] = e[k];
+                for (int w = 0; w < kFewWarps; ++w) {
+                    if (s[w].y == 0.f) continue;   // saw nothing; what stands beside it need not be a number
+                    const float by = s[w].x == -INFINITY ? s[w].y : exp2_fast(s[w].x - top);   // a sum with no reference is NaN
+                    const float4 z = *reinterpret_cast<const float4 *>(share + (w * 8 + row) * DP + d);
+                    sum = fmaf(by, s[w].y, sum);
+                    v[0] = fmaf(by, z.x, v[0]);
+                    v[1] = fmaf(by, z.y, v[1]);
+                    v[2] = fmaf(by, z.z, v[2]);
+                    v[3] = fmaf(by, z.w, v[3]);
+                }
+                if (all) finish(P, b, hk, r, d, v, top, sum);
+                else {
+                    if (d == 0) F.part_stats[part + 8 * x + row] = make_float2(top, sum);
+                    *reinterpret_cast<float4 *>(F.part_out + (part + 8 * x + row) * DP + d) = make_float4(v[0], v[1], v[2], v[3]);
+                }
             }
         }
-    }
-    if (F.splits > 1) cluster_sync();   // the others have read
+        __syncthreads();
+        if (threadIdx.x == 0 && used > 0) {
+            fence_proxy_async_smem();   // read and written by threads before copies write there
+            fill(used + L::kStages);
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        stage = 0;
+        if (++item == items) {
+            item = 0;
+            do ++b;
+            while (used < total && Stages<KEYS>(P, b).count == 0);
+        }
+    } while (used < total);
+    if (threadIdx.x == 0 && *abort_flag)   // what was issued arrives before the CTA ends
+        for (uint32_t u = first_of_last_uses(issued, L::kStages); u < (uint32_t)issued; ++u) mbar_wait_bounded(&full[u % L::kStages], parity_of_use(u, L::kStages));
 }
 
-template <int BITS, int W, int NG, int NT, int PARTS> int launch_few(const CacheFewParams &F, cudaStream_t s) {
-    typedef CacheFewSmem<BITS, W, NG, NT> L;
+// Items that several CTAs have parts of, and those that have no keys: a CTA to an item, a lane to four features of a row, four parts on their way at a time.
+template <int BITS, int W, int NG, int NT, int PARTS> __global__ void __launch_bounds__(kFewThreads) cache_join_kernel(const CacheFewParams F, int shares) {
+    typedef CacheFew<BITS, W, NG, NT, PARTS> L;
+    const CacheAttnParams &P = F.a;
+    constexpr int DP = 32 * W, ROWS = 8 * NT;
+    __shared__ unsigned room[kFewWarps + 2];
+    const int items = (int)P.c.H * F.row_blocks, of = (int)(blockIdx.x / items), item = (int)(blockIdx.x % items), hk = item / F.row_blocks, row0 = item % F.row_blocks * ROWS;
+    const int n = Stages<L::KEYS>(P, of).count;
+    const Line line = line_of<L::KEYS>(F, 0, shares, of, room);
+    const unsigned at = line.before + (unsigned)item * (n + kFewExtra) + kFewExtra;
+    // the CTA that has a place of the line; where places are fewer than CTAs some have none
+    auto owner = [&](unsigned place) { return (int)(((unsigned long long)(place + 1) * shares - 1) / line.total); };
+    auto none = [&](int c) { return line.start(c, shares) == line.start(c + 1, shares); };
+    const int first = n > 0 ? owner(at) : 0, last = n > 0 ? owner(at + n - 1) : -1;
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // of every CTA: what comes after this kernel comes after both
+    if (first == last) return;   // written already
+    for (int k = threadIdx.x; k < ROWS * DP / 4; k += kFewThreads) {
+        const int row = k / (DP / 4), d = k % (DP / 4) * 4, r = row0 + row;
+        if (r >= F.rows) break;
+        if (d >= P.c.D) continue;
+        float top = -INFINITY, sum = 0.f, v[4] = {};
+        for (int c0 = first; c0 <= last; c0 += 4) {
+            float2 s[4];
+            float4 z[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const bool has = c0 + u <= last && !none(c0 + u);
+                const long long place = ((long long)(c0 + u) * 2 + (c0 + u == first ? 1 : 0)) * ROWS + row;
+                s[u] = has ? F.part_stats[place] : make_float2(-INFINITY, 0.f);
+                z[u] = has ? *reinterpret_cast<const float4 *>(F.part_out + place * DP + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            float now = top;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) now = fmaxf(now, s[u].x);
+            const float old = now == top ? 1.f : exp2_fast(top - now);
+            sum *= old;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] *= old;
+            top = now;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (s[u].y == 0.f) continue;
+                const float by = s[u].x == -INFINITY ? s[u].y : exp2_fast(s[u].x - top);   // a sum with no reference is NaN
+                sum = fmaf(by, s[u].y, sum);
+                v[0] = fmaf(by, z[u].x, v[0]);
+                v[1] = fmaf(by, z[u].y, v[1]);
+                v[2] = fmaf(by, z[u].z, v[2]);
+                v[3] = fmaf(by, z[u].w, v[3]);
+            }
+        }
+        finish(P, of, hk, r, d, v, top, sum);
+    }
+}
+
+template <int BITS, int W, int NG, int NT, int PARTS> int launch_few(CacheFewParams F, void *scratch, long long *bytes, cudaStream_t s) {
+    typedef CacheFew<BITS, W, NG, NT, PARTS> L;
+    const CacheAttnParams &P = F.a;
+    F.row_blocks = (int)((F.rows + L::ROWS - 1) / L::ROWS);
+    const long long items = P.c.B * P.c.H * F.row_blocks, seen = P.window > 0 && P.window + P.Nq < P.c.capacity ? P.window + P.Nq : P.c.capacity;
+    const long long longest = (seen + L::KEYS - 1) / L::KEYS, slots = (long long)L::PER_SM * sm_count();
+    // A CTA for an item where none can have more than 512 keys, about what a second kernel costs.  Else shares of at least 256 keys.
+    F.whole = longest * L::KEYS <= 512;
+    const long long least = items * longest * L::KEYS / 256, ctas = F.whole ? items : least < slots ? least : slots;
+    if (bytes) {
+        *bytes = F.whole ? 0 : ctas * 2 * L::ROWS * (4 * L::DP + 8);
+        return TPW_OK;
+    }
+    TPW_CHECK_ARG(items * (longest + kFewExtra) < (1LL << 31), "tpw_cache_attention: more than 2^31 stages of work");
+    F.part_out = static_cast<float *>(scratch);
+    F.part_stats = reinterpret_cast<float2 *>(F.part_out + (F.whole ? 0 : ctas * 2 * L::ROWS * L::DP));
     constexpr auto *kern = &cache_few_kernel<BITS, W, NG, NT, PARTS>;
     if (const int e = allow_shared_memory<kern>((int)L::ALLOC)) return e;
-    const long long blocks = F.a.c.B * F.a.c.H * F.row_blocks * F.splits;
-    TPW_CHECK_ARG(blocks < (1LL << 31), "tpw_cache_attention: more than 2^31 blocks of work");
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)blocks);
-    config.blockDim = dim3(kCacheThreads);
-    config.dynamicSmemBytes = L::ALLOC;
-    config.stream = s;
-    cudaLaunchAttribute cluster = {};
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim = {(unsigned)F.splits, 1, 1};
-    config.attrs = &cluster;
-    config.numAttrs = F.splits > 1 ? 1 : 0;
-    TPW_CUDA_OK(cudaLaunchKernelEx(&config, kern, F));
+    kern<<<(unsigned)ctas, kFewThreads, L::ALLOC, s>>>(F);
     TPW_LAUNCH_OK("cache_few_kernel");
+    if (F.whole) return TPW_OK;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)items);
+    config.blockDim = dim3(kFewThreads);
+    config.stream = s;
+    cudaLaunchAttribute overlap = {};
+    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    overlap.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &overlap;
+    config.numAttrs = 1;
+    TPW_CUDA_OK(cudaLaunchKernelEx(&config, &cache_join_kernel<BITS, W, NG, NT, PARTS>, F, (int)ctas));
+    TPW_LAUNCH_OK("cache_join_kernel");
     return TPW_OK;
 }
-template <int BITS, int W, int NG> int launch_rows(const CacheFewParams &F, cudaStream_t s) {
-    if (F.a.dtype == TPW_F32) return launch_few<BITS, W, NG, 1, 2>(F, s);
-    return F.rows <= 8 ? launch_few<BITS, W, NG, 1, 1>(F, s) : launch_few<BITS, W, NG, 2, 1>(F, s);
+template <int BITS, int W, int NG> int launch_rows(const CacheFewParams &F, void *scratch, long long *bytes, cudaStream_t s) {
+    if (F.a.dtype == TPW_F32) return launch_few<BITS, W, NG, 1, 2>(F, scratch, bytes, s);
+    return F.rows <= 8 ? launch_few<BITS, W, NG, 1, 1>(F, scratch, bytes, s) : launch_few<BITS, W, NG, 2, 1>(F, scratch, bytes, s);
 }
-template <int BITS> int launch_width(const CacheFewParams &F, cudaStream_t s) {
-    const bool one = F.a.c.groups == 1;
-    if (F.a.c.width == 2) return one ? launch_rows<BITS, 2, 1>(F, s) : launch_rows<BITS, 2, 2>(F, s);
-    if (F.a.c.width == 3) return one ? launch_rows<BITS, 3, 1>(F, s) : launch_rows<BITS, 3, 3>(F, s);
-    return one ? launch_rows<BITS, 4, 1>(F, s) : launch_rows<BITS, 4, 4>(F, s);
+// with `bytes` only says how much scratch the call wants
+template <int BITS> int launch_width(const CacheAttnParams &P, void *scratch, long long *bytes, cudaStream_t s) {
+    CacheFewParams F = {};
+    F.a = P;
+    F.rows = (int)(P.group * P.Nq);
+    const long long piece = P.dtype == TPW_F32 ? 4 : 8;
+    F.q_vector = P.c.D % 8 == 0 && aligned16(P.q) && P.q_s[0] % piece == 0 && P.q_s[1] % piece == 0 && P.q_s[2] % piece == 0;
+    const bool one = P.c.groups == 1;
+    if (P.c.width == 2) return one ? launch_rows<BITS, 2, 1>(F, scratch, bytes, s) : launch_rows<BITS, 2, 2>(F, scratch, bytes, s);
+    if (P.c.width == 3) return one ? launch_rows<BITS, 3, 1>(F, scratch, bytes, s) : launch_rows<BITS, 3, 3>(F, scratch, bytes, s);
+    return one ? launch_rows<BITS, 4, 1>(F, scratch, bytes, s) : launch_rows<BITS, 4, 4>(F, scratch, bytes, s);
 }
 
 } // namespace

@@ -2,5 +2,5 @@
 #include "cache_few.cuh"
 
 namespace tpw {
-int cache_few_8(const CacheAttnParams &P, int rows, int row_blocks, int splits, cudaStream_t s) { return launch_width<8>({P, rows, row_blocks, splits}, s); }
+int cache_few_8(const CacheAttnParams &P, void *scratch, long long *bytes, cudaStream_t s) { return launch_width<8>(P, scratch, bytes, s); }
 } // namespace tpw
