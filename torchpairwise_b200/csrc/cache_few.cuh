@@ -32,6 +32,7 @@ struct CacheFewParams {
     CacheAttnParams a;
     int rows, row_blocks;            // group * Nq, and blocks of them
     int whole;                       // a CTA for each head and block of rows, no joining
+    Divider by_nq, by_blocks;
     int q_vector;                    // rows of queries in 16-byte pieces
     float *part_out;                 // [CTA][2][rows of a block][features of a row in storage]: of a head begun by another CTA, of one that this CTA begins
     float2 *part_stats;              // [CTA][2][rows of a block]: reference (a power of 2) and sum
@@ -50,15 +51,19 @@ template <int BITS, int W, int NG, int NT, int PARTS> struct CacheFew {
                               OFF_BAR = OFF_SUMS + SUMS, OFF_FLAG = OFF_BAR + 16 * kStages, ALLOC = OFF_FLAG + 16;
 };
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], const float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+// D += A B, and D = C + A B where C stays
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_from(float (&d)[4], const float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
-                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     uint32_t r;
@@ -150,8 +155,9 @@ __device__ __forceinline__ void store_out(const CacheAttnParams &P, long long at
 }
 
 // four features of row r from the weighed sums of values and of probabilities, which are lifted beside their reference
-__device__ __forceinline__ void finish(const CacheAttnParams &P, int b, int hk, int r, int d, float (&v)[4], float reference, float sum) {
-    const int nq = (int)P.Nq, i = r % nq, h = (int)(hk * P.group) + r / nq;
+__device__ __forceinline__ void finish(const CacheFewParams &F, int b, int hk, int r, int d, float (&v)[4], float reference, float sum) {
+    const CacheAttnParams &P = F.a;
+    const int over = (unsigned)r / F.by_nq, i = r - over * (int)P.Nq, h = (int)(hk * P.group) + over;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] *= inv;
@@ -181,7 +187,7 @@ template <int KEYS> struct Stages {
 // The line of all stages: sequences one after the other, a sequence's items (heads, and blocks of rows of each) one after the other, an item's
 // stages in order.  An item with stages stands on the line for kFewExtra more, which come first: what beginning and ending it costs.
 // Found by the whole CTA (128 threads): how long the line is, and the sequence that place `at` (or item `item` of sequence `of`) lies in.
-constexpr int kFewExtra = 1;
+constexpr int kFewExtra = 2;
 struct Line {
     unsigned total, before;   // places in all; in sequences before `b`
     int b;
@@ -287,44 +293,52 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
         if (P.status) atomicCAS(P.status, 0, (23 << 16) | site);
     };
 
-    // Lane 0 of warp 0 also issues the copies, as many stages ahead as the ring has room for.
-    int ahead_b = b, ahead_item = item, ahead_stage = stage, issued = 0;
+    // Warp 0 also issues the copies, as many stages ahead as the ring has room for: a lane each for the codes and scales of keys and values.
+    int ahead_b = b, ahead_item = item, ahead_left = 0, ahead_key = 0, issued = 0;
+    const uint32_t copy_bytes = lane & 2 ? NG * 4 : L::ROW, copy_to = smem_u32(smem) + (lane & 2 ? 2 * L::CODES + (lane & 1) * L::SCALES : (lane & 1) * L::CODES);
+    const unsigned char *copy_base = lane & 2 ? reinterpret_cast<const unsigned char *>(P.c.scales[lane & 1]) : P.c.codes[lane & 1], *copy_from = nullptr;
     bool ok = true;
+    auto ahead_of = [&](int skip) {   // the next item's stages but for the first `skip`
+        const Stages<KEYS> S(P, ahead_b);
+        ahead_left = S.count - skip;
+        ahead_key = S.begin + skip * KEYS;
+        copy_from = copy_base + (((long long)ahead_b * P.c.H + (unsigned)ahead_item / F.by_blocks) * P.c.capacity + ahead_key) * copy_bytes;
+    };
     auto fill = [&](int limit) {
         limit = limit < total ? limit : total;
         while (issued < limit && ok) {
             const uint32_t st = issued % L::kStages;
-            if (issued >= L::kStages && !(ok = wait_or_abort(&empty[st], parity_of_use(issued, L::kStages) ^ 1, abort_flag))) {
+            if (issued >= L::kStages && !(ok = __all_sync(0xffffffffu, wait_or_abort(&empty[st], parity_of_use(issued, L::kStages) ^ 1, abort_flag)))) {
                 give_up(1);
                 return;
             }
-            const Stages<KEYS> S(P, ahead_b);
             // the capacity and a stage's first key are multiples of 64
-            const long long j = S.begin + ahead_stage * KEYS, place = ((long long)ahead_b * P.c.H + ahead_item / F.row_blocks) * P.c.capacity + j;
-            const uint32_t n = (uint32_t)(P.c.capacity - j < KEYS ? P.c.capacity - j : KEYS), to = smem_u32(smem) + st * L::STAGE;
-            mbar_expect_tx(&full[st], n * 2 * (L::ROW + NG * 4));
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                bulk_load(to + w * L::CODES, P.c.codes[w] + place * L::ROW, n * L::ROW, &full[st]);
-                bulk_load(to + 2 * L::CODES + w * L::SCALES, P.c.scales[w] + place * NG, n * NG * 4, &full[st]);
-            }
+            const uint32_t n = (uint32_t)((int)P.c.capacity - ahead_key < KEYS ? (int)P.c.capacity - ahead_key : KEYS);
+            if (lane == 0) mbar_expect_tx(&full[st], n * 2 * (L::ROW + NG * 4));
+            __syncwarp();
+            if (lane < 4) bulk_load(copy_to + st * L::STAGE, copy_from, n * copy_bytes, &full[st]);
             ++issued;
-            if (++ahead_stage == S.count) {
-                ahead_stage = 0;
+            ahead_key += KEYS;
+            copy_from += KEYS * copy_bytes;
+            if (--ahead_left == 0 && issued < total) {
                 if (++ahead_item == items) {
                     ahead_item = 0;
                     do ++ahead_b;
-                    while (issued < total && Stages<KEYS>(P, ahead_b).count == 0);
+                    while (Stages<KEYS>(P, ahead_b).count == 0);
                 }
+                ahead_of(0);
             }
         }
     };
-    if (threadIdx.x == 0) fill(L::kStages);
+    if (warp == 0 && total > 0) {
+        ahead_of(stage);
+        fill(L::kStages);
+    }
 
     float2 *stats = reinterpret_cast<float2 *>(smem + L::OFF_STATS);
     uint32_t *queries = reinterpret_cast<uint32_t *>(smem + L::OFF_QUERIES);   // [part][block][w][lane][4]
     float *query_sums = reinterpret_cast<float *>(smem + L::OFF_SUMS);         // [block][w and, last, the factor of scores][row]
-    // [block of 16 keys][step, zero][group][slot]
+    // of every 16 keys: steps [pair of slots][group][slot of the pair], zeros [group][slot]
     uint16_t *prepared = reinterpret_cast<uint16_t *>(smem + L::OFF_PREPARED) + warp * SUB * NG * 32;
     const int slot0 = key_of_slot(g), value0 = t, value1 = 4 + (t ^ 1);   // and 8 more
     int used = 0;
@@ -332,7 +346,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
     do {
         const Stages<KEYS> S(P, b);
         const CacheSeen see(P, b);
-        const int hk = item / F.row_blocks, row0 = item % F.row_blocks * ROWS, stage0 = stage;
+        const int hk = (unsigned)item / F.by_blocks, row0 = (item - hk * F.row_blocks) * ROWS, stage0 = stage;
         const int stages = S.count - stage < total - used ? S.count - stage : total - used;
         // Queries as operands, a warp making those of every fourth block of 32 features: row g of a block, features 32 w + 8 t + (0 .. 7), in the order
         // in which masks leave the codes of a key.  Row r is query r % nq of head hk * group + r / nq.
@@ -340,7 +354,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
         for (int unit = warp; unit < NT * W; unit += kFewWarps) {
             const int x = unit / W, w = unit % W, r = row0 + 8 * x + g;
             const bool valid = r < F.rows;
-            const int h = valid ? r / nq : 0;
+            const int h = valid ? (unsigned)r / F.by_nq : 0;
             const long long row = b * P.q_s[0] + (valid ? r - h * nq : 0) * P.q_s[1] + (hk * P.group + h) * P.q_s[2] + 8 * t;
             float y[8] = {}, top = 0.f;
 #pragma unroll
@@ -389,7 +403,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
         __syncthreads();
         uint32_t q[PARTS][NT][W][2][2], qz[NT][PARTS][2];
         float start[NT][NG][4], factor[NT][2];   // -M a_g; raw scores times the factor are powers of 2
-        int lo[NT][2], hi[NT][2];
+        int lo[NT][2], hi[NT][2], all_lo = S.first, all_hi = S.end;   // keys that a row sees; that all rows do
         float m[NT][2], l[NT][2], o[NT][2 * W][4], zeros[NT][NG][2], zero_sums[NT][4];   // rows 2 t, 2 t + 1 of every block: reference (a power of 2), sums
         int top_scale = 1;                       // largest exponent of a step or zero of a value so far, as in its bits
 #pragma unroll
@@ -428,9 +442,11 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                     zeros[x][k][e] = 0.f;
                 }
                 factor[x][e] = sums[W * 8 + row];
-                const int i = mine < F.rows ? mine % nq : 0;
+                const int i = mine < F.rows ? (unsigned)mine % F.by_nq : 0;
                 lo[x][e] = mine < F.rows ? see.lo(i) : 0;
                 hi[x][e] = mine < F.rows ? see.hi(i) : 1 << 30;
+                all_lo = max(all_lo, lo[x][e]);
+                all_hi = min(all_hi, hi[x][e]);
                 m[x][e] = -INFINITY;
                 l[x][e] = 0.f;
             }
@@ -441,6 +457,8 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
 #pragma unroll
             for (int e = 0; e < 4; ++e) zero_sums[x][e] = 0.f;
         }
+        all_lo = __reduce_max_sync(0xffffffffu, all_lo);
+        all_hi = __reduce_min_sync(0xffffffffu, all_hi);
         for (int u = 0; u < stages; ++u, ++used) {
             const uint32_t st = used % L::kStages;
             if (ok && !(ok = __all_sync(0xffffffffu, wait_or_abort(&full[st], parity_of_use(used, L::kStages), abort_flag)))) give_up(2);
@@ -461,9 +479,10 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                     }
 #pragma unroll
                     for (int x = 0; x < NT; ++x) {
-                        const float none[4] = {};
-                        mma_bf16(p[h][x], none, kz[0], kz[1], kz[0], kz[1], qz[x][0][0], qz[x][0][1]);
-                        if constexpr (WIDE) mma_bf16(p[h][x], p[h][x], kz[0], kz[1], kz[0], kz[1], qz[x][1][0], qz[x][1][1]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) p[h][x][e] = 0.f;
+#pragma unroll
+                        for (int part = 0; part < PARTS; ++part) mma_bf16(p[h][x], kz[0], kz[1], kz[0], kz[1], qz[x][part][0], qz[x][part][1]);
                     }
                     float acc[NT][4];
 #pragma unroll
@@ -487,8 +506,9 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                             for (int x = 0; x < NT; ++x)
 #pragma unroll
                                 for (int part = 0; part < PARTS; ++part) {
-                                    const bool fresh = k == 0 && part == 0 && (NG > 1 || w == 0);
-                                    mma_f16(acc[x], fresh ? start[x][NG > 1 ? w : 0] : acc[x], a[0], a[1], a[2], a[3], q[part][x][w][k][0], q[part][x][w][k][1]);
+                                    if (k == 0 && part == 0 && (NG > 1 || w == 0))
+                                        mma_f16_from(acc[x], start[x][NG > 1 ? w : 0], a[0], a[1], a[2], a[3], q[part][x][w][k][0], q[part][x][w][k][1]);
+                                    else mma_f16(acc[x], a[0], a[1], a[2], a[3], q[part][x][w][k][0], q[part][x][w][k][1]);
                                 }
                         }
                         if (NG > 1 || w == W - 1)
@@ -501,21 +521,12 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                                     for (int e = 0; e < 2; ++e) p[h][x][2 * s + e] = fmaf(step, acc[x][2 * s + e], p[h][x][2 * s + e]);
                             }
                     }
-#pragma unroll
-                    for (int x = 0; x < NT; ++x)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) p[h][x][e] *= factor[x][e & 1];
                 }
                 // steps and zeros of values, a lane to a key
                 uint32_t vs[NG];
                 load_words(vs, vs_at + (lane % (16 * SUB)) * NG * 4);
                 // keys that some row does not see; steps and zeros of those that none sees need not be numbers
-                bool edge = j0 < S.first || j0 + 16 * SUB > S.end;
-#pragma unroll
-                for (int x = 0; x < NT; ++x)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) edge = edge || j0 < lo[x][e] || j0 + 16 * SUB > hi[x][e];
-                if (__any_sync(0xffffffffu, edge)) {
+                if (j0 < all_lo || j0 + 16 * SUB > all_hi) {
 #pragma unroll
                     for (int h = 0; h < SUB; ++h)
 #pragma unroll
@@ -535,7 +546,8 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                 // the reference moves, and sums are scaled, only where a score, a step or a zero has left it behind
                 uint32_t high_scale = 0;
 #pragma unroll
-                for (int k = 0; k < NG; ++k) high_scale = max(high_scale, max(vs[k] << 16, vs[k] & 0x7fff0000u));
+                for (int k = 0; k < NG; ++k) high_scale = __vmaxu2(high_scale, vs[k] & 0x7fffffffu);   // steps are not negative
+                high_scale = max(high_scale << 16, high_scale & 0xffff0000u);
                 bool moves = (int)(high_scale >> 23) > top_scale;
                 float high[NT][2];
 #pragma unroll
@@ -544,6 +556,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                     for (int e = 0; e < 2; ++e) {
                         high[x][e] = fmaxf(p[0][x][e], p[0][x][2 + e]);
                         if constexpr (SUB == 2) high[x][e] = fmaxf(high[x][e], fmaxf(p[1][x][e], p[1][x][2 + e]));
+                        high[x][e] *= factor[x][e];
                         moves = moves || high[x][e] > m[x][e] + kFewSlack;
                     }
                 if (__any_sync(0xffffffffu, moves)) {
@@ -578,12 +591,13 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                 if constexpr (!WIDE) {
                     __syncwarp();   // the last ones are read
                     if (lane < 16 * SUB) {
-                        uint16_t *to = prepared + (lane >> 4) * NG * 32 + slot_of_key(lane & 15);
+                        const int slot = slot_of_key(lane & 15);
+                        uint16_t *to = prepared + (lane >> 4) * NG * 32 + (slot >> 1) * 2 * NG + (slot & 1), *to_zero = prepared + (lane >> 4) * NG * 32 + 16 * NG + slot;
 #pragma unroll
                         for (int k = 0; k < NG; ++k) {
                             const uint32_t both = half2_of(step_of(vs[k]) * norm, zero_of(vs[k]) * norm);
-                            to[16 * k] = (uint16_t)both;
-                            to[16 * (NG + k)] = (uint16_t)(both >> 16);
+                            to[2 * k] = (uint16_t)both;
+                            to_zero[16 * k] = (uint16_t)(both >> 16);
                         }
                     }
                     __syncwarp();
@@ -597,7 +611,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                         for (int h = 0; h < SUB; ++h)
 #pragma unroll
                             for (int s = 0; s < 2; ++s) {
-                                p[h][x][2 * s + e] = exp2_fast(p[h][x][2 * s + e] + shift);
+                                p[h][x][2 * s + e] = exp2_fast(fmaf(p[h][x][2 * s + e], factor[x][e], shift));
                                 l[x][e] += p[h][x][2 * s + e];
                             }
                     }
@@ -616,15 +630,17 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                     }
                     // probabilities (times steps) as operands: slots 2 t, 2 t + 1 and 2 t + 8, 2 t + 9 of row g
                     uint32_t y[PARTS][NT][2], pt[NT][2];
-                    const uint16_t *ready = prepared + h * NG * 32 + 2 * t;
+                    uint32_t steps[2][NG];
                     if constexpr (!WIDE) {
-                        const uint16_t *z = ready + 16 * (NG + (g < NG ? g : 0));
+                        const uint16_t *ready = prepared + h * NG * 32, *z = ready + 16 * NG + 16 * (g < NG ? g : 0) + 2 * t;
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) load_words(steps[s], reinterpret_cast<const unsigned char *>(ready + (4 * s + t) * 2 * NG));
                         const uint32_t z0 = g < NG ? *reinterpret_cast<const uint32_t *>(z) : 0u, z1 = g < NG ? *reinterpret_cast<const uint32_t *>(z + 8) : 0u;
 #pragma unroll
                         for (int x = 0; x < NT; ++x) {
 #pragma unroll
                             for (int s = 0; s < 2; ++s) pt[x][s] = transposed(half2_of(p[h][x][2 * s], p[h][x][2 * s + 1]));
-                            mma_f16(zero_sums[x], zero_sums[x], z0, 0u, z1, 0u, pt[x][0], pt[x][1]);
+                            mma_f16(zero_sums[x], z0, 0u, z1, 0u, pt[x][0], pt[x][1]);
                         }
                     }
 #pragma unroll
@@ -633,9 +649,8 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
 #pragma unroll
                             for (int s = 0; s < 2; ++s) {
                                 if constexpr (!WIDE) {
-                                    const uint32_t step = *reinterpret_cast<const uint32_t *>(ready + 16 * (NG > 1 ? w : 0) + 8 * s);
 #pragma unroll
-                                    for (int x = 0; x < NT; ++x) y[0][x][s] = half2_times(pt[x][s], step);
+                                    for (int x = 0; x < NT; ++x) y[0][x][s] = half2_times(pt[x][s], steps[s][NG > 1 ? w : 0]);
                                 } else {
                                     const int key = 16 * h + 8 * s + slot0, j = j0 + key;
                                     uint32_t sc = reinterpret_cast<const uint32_t *>(vs_at)[key * NG + (NG > 1 ? w : 0)];
@@ -677,11 +692,11 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
 #pragma unroll
                             for (int x = 0; x < NT; ++x) {
                                 if constexpr (!WIDE) {
-                                    mma_f16(o[x][2 * w + k], o[x][2 * w + k], a[0], a[1], a[2], a[3], y[0][x][0], y[0][x][1]);
+                                    mma_f16(o[x][2 * w + k], a[0], a[1], a[2], a[3], y[0][x][0], y[0][x][1]);
                                 } else {
                                     float sum[4] = {};
 #pragma unroll
-                                    for (int part = 0; part < PARTS; ++part) mma_f16(sum, sum, a[0], a[1], a[2], a[3], y[part][x][0], y[part][x][1]);
+                                    for (int part = 0; part < PARTS; ++part) mma_f16(sum, a[0], a[1], a[2], a[3], y[part][x][0], y[part][x][1]);
 #pragma unroll
                                     for (int e = 0; e < 4; ++e) o[x][2 * w + k][e] += sum[e];
                                 }
@@ -693,8 +708,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[st]);
             // the last stage's room is where the warps' outputs meet: it is filled anew after that
-            if (threadIdx.x == 0 && u + 1 < stages) fill(used + L::kStages);
-            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if (warp == 0 && u + 1 < stages) fill(used + L::kStages);
         }
         // The warps' outputs meet, 8 rows at a time: [warp][row][feature] beside references and sums.  A thread weighs four features of a row together.
         float *share = reinterpret_cast<float *>(smem + (used > 0 ? (used - 1) % L::kStages : 0) * L::STAGE);
@@ -755,7 +769,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                     v[2] = fmaf(by, z.z, v[2]);
                     v[3] = fmaf(by, z.w, v[3]);
                 }
-                if (all) finish(P, b, hk, r, d, v, top, sum);
+                if (all) finish(F, b, hk, r, d, v, top, sum);
                 else {
                     if (d == 0) F.part_stats[part + 8 * x + row] = make_float2(top, sum);
                     *reinterpret_cast<float4 *>(F.part_out + (part + 8 * x + row) * DP + d) = make_float4(v[0], v[1], v[2], v[3]);
@@ -763,11 +777,10 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
             }
         }
         __syncthreads();
-        if (threadIdx.x == 0 && used > 0) {
+        if (warp == 0 && used > 0) {
             fence_proxy_async_smem();   // read and written by threads before copies write there
             fill(used + L::kStages);
         }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
         stage = 0;
         if (++item == items) {
             item = 0;
@@ -829,7 +842,7 @@ template <int BITS, int W, int NG, int NT, int PARTS> __global__ void __launch_b
                 v[3] = fmaf(by, z[u].w, v[3]);
             }
         }
-        finish(P, of, hk, r, d, v, top, sum);
+        finish(F, of, hk, r, d, v, top, sum);
     }
 }
 
@@ -837,6 +850,8 @@ template <int BITS, int W, int NG, int NT, int PARTS> int launch_few(CacheFewPar
     typedef CacheFew<BITS, W, NG, NT, PARTS> L;
     const CacheAttnParams &P = F.a;
     F.row_blocks = (int)((F.rows + L::ROWS - 1) / L::ROWS);
+    F.by_nq = divider(P.Nq);
+    F.by_blocks = divider(F.row_blocks);
     const long long items = P.c.B * P.c.H * F.row_blocks, seen = P.window > 0 && P.window + P.Nq < P.c.capacity ? P.window + P.Nq : P.c.capacity;
     const long long longest = (seen + L::KEYS - 1) / L::KEYS, slots = (long long)L::PER_SM * sm_count();
     // A CTA for an item where none can have more than 512 keys, about what a second kernel costs.  Else shares of at least 256 keys.
