@@ -187,7 +187,7 @@ template <int KEYS> struct Stages {
 // The line of all stages: sequences one after the other, a sequence's items (heads, and blocks of rows of each) one after the other, an item's
 // stages in order.  An item with stages stands on the line for kFewExtra more, which come first: what beginning and ending it costs.
 // Found by the whole CTA (128 threads): how long the line is, and the sequence that place `at` (or item `item` of sequence `of`) lies in.
-constexpr int kFewExtra = 2;
+constexpr int kFewExtra = 3;
 struct Line {
     unsigned total, before;   // places in all; in sequences before `b`
     int b;
@@ -330,9 +330,10 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
             }
         }
     };
+    // one stage for now: the queries are not to wait behind what all CTAs ask for
     if (warp == 0 && total > 0) {
         ahead_of(stage);
-        fill(L::kStages);
+        fill(1);
     }
 
     float2 *stats = reinterpret_cast<float2 *>(smem + L::OFF_STATS);
@@ -401,6 +402,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
             }
         }
         __syncthreads();
+        if (warp == 0 && used == 0) fill(L::kStages);
         uint32_t q[PARTS][NT][W][2][2], qz[NT][PARTS][2];
         float start[NT][NG][4], factor[NT][2];   // -M a_g; raw scores times the factor are powers of 2
         int lo[NT][2], hi[NT][2], all_lo = S.first, all_hi = S.end;   // keys that a row sees; that all rows do
