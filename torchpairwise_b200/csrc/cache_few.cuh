@@ -16,7 +16,7 @@
 // All stages of keys (64 or 128) of all sequences and heads form one line that the CTAs, three on an SM, take equal shares of, whatever the lengths: a
 // share ends and begins anywhere in a sequence.  What a CTA has of a head that others have parts of goes to scratch, and a second kernel, whose launch
 // overlaps this one, weighs the parts together in their order.  In a CTA four warps take 16 keys or 32 of a stage each, with a running reference, sum and
-// output of their own; bulk copies bring the stages into a ring, across the ends of heads.
+// output of their own, and a ring of their own that they fill by bulk copies, across the ends of heads.
 #pragma once
 #include "attention_tc.cuh"
 #include "cache.cuh"
@@ -39,16 +39,16 @@ struct CacheFewParams {
 };
 
 template <int BITS, int W, int NG, int NT, int PARTS> struct CacheFew {
-    static constexpr int KEYS = BITS == 4 ? 128 : 64, SUB = KEYS / 64;   // of a stage; blocks of 16 keys to a warp
-    static constexpr uint32_t ROW = W * 4 * BITS, CODES = KEYS * ROW, SCALES = KEYS * NG * 4, STAGE = 2 * (CODES + SCALES), DP = 32 * W, ROWS = 8 * NT;
+    static constexpr int KEYS = BITS == 4 ? 128 : 64, OWN = KEYS / kFewWarps, SUB = OWN / 16;   // of a stage; a warp's of them, and blocks of 16
+    static constexpr uint32_t ROW = W * 4 * BITS, CODES = OWN * ROW, SCALES = OWN * NG * 4, PIECE = 2 * (CODES + SCALES), DP = 32 * W, ROWS = 8 * NT;
     static constexpr int PER_SM = NT == 1 ? 3 : 2;
     static constexpr uint32_t STATS = kFewWarps * 8 * 8, PREPARED = PARTS == 1 ? kFewWarps * SUB * NG * 64 : 0, QUERIES = PARTS * NT * W * 512, SUMS = NT * (W + 1) * 32;
-    static constexpr uint32_t ROOM = (NT == 1 ? 75776 : 112640) - STATS - PREPARED - QUERIES - SUMS - 192;
-    static constexpr int kStages = ROOM / STAGE < 8 ? ROOM / STAGE : 8;
+    static constexpr uint32_t ROOM = (NT == 1 ? 75776 : 112640) - STATS - PREPARED - QUERIES - SUMS - 320;
+    static constexpr int kStages = ROOM / (kFewWarps * PIECE) < 8 ? ROOM / (kFewWarps * PIECE) : 8;
     static_assert(kStages >= 2, "a ring of two stages at least");
-    static_assert(kFewWarps * 8 * DP * 4 <= STAGE, "the warps' shares of 8 rows fit a stage");
-    static constexpr uint32_t OFF_STATS = kStages * STAGE, OFF_PREPARED = OFF_STATS + STATS, OFF_QUERIES = OFF_PREPARED + PREPARED, OFF_SUMS = OFF_QUERIES + QUERIES,
-                              OFF_BAR = OFF_SUMS + SUMS, OFF_FLAG = OFF_BAR + 16 * kStages, ALLOC = OFF_FLAG + 16;
+    static_assert(8 * DP * 4 <= PIECE, "a warp's 8 rows of results fit its piece of a stage");
+    static constexpr uint32_t RING = kStages * PIECE, OFF_STATS = kFewWarps * RING, OFF_PREPARED = OFF_STATS + STATS, OFF_QUERIES = OFF_PREPARED + PREPARED, OFF_SUMS = OFF_QUERIES + QUERIES,
+                              OFF_BAR = OFF_SUMS + SUMS, OFF_FLAG = OFF_BAR + 8 * kFewWarps * kStages, ALLOC = OFF_FLAG + 16;
 };
 
 // D += A B, and D = C + A B where C stays
@@ -60,6 +60,10 @@ __device__ __forceinline__ void mma_f16_from(float (&d)[4], const float (&c)[4],
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+__device__ __forceinline__ void mma_bf16_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -75,6 +79,11 @@ __device__ __forceinline__ uint32_t half2_rest(float lo, float hi) { return Narr
 __device__ __forceinline__ uint32_t half2_times(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e < 1 ? 1 : e > 254 ? 254 : e) << 23); }   // 2^(e - 127)
@@ -246,14 +255,15 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
     constexpr float MIDDLE = BITS == 4 ? 8.f : 128.f;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ unsigned room[kFewWarps + 2];
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *empty = full + L::kStages;
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_FLAG);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int nq = (int)P.Nq, items = (int)P.c.H * F.row_blocks;
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR) + warp * L::kStages;
+    unsigned char *ring = smem + warp * L::RING;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < L::kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], kFewWarps); }
+        for (int i = 0; i < kFewWarps * L::kStages; ++i) mbar_init(&full[i], 1);
         *abort_flag = 0;
         mbar_init_fence();
     }
@@ -293,30 +303,33 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
         if (P.status) atomicCAS(P.status, 0, (23 << 16) | site);
     };
 
-    // Warp 0 also issues the copies, as many stages ahead as the ring has room for: a lane each for the codes and scales of keys and values.
-    int ahead_b = b, ahead_item = item, ahead_left = 0, ahead_key = 0, issued = 0;
-    const uint32_t copy_bytes = lane & 2 ? NG * 4 : L::ROW, copy_to = smem_u32(smem) + (lane & 2 ? 2 * L::CODES + (lane & 1) * L::SCALES : (lane & 1) * L::CODES);
+    // A warp brings its own keys of every stage, as many stages ahead as its ring has room for: a lane each for the codes and scales of keys and values.
+    // It waits for no other warp.
+    int ahead_b = b, ahead_item = item, ahead_left = 0, ahead_key = 0, ahead_end = 0, issued = 0;
+    uint32_t issued_slot = 0, slot = 0, phase = 0;   // of the next stage to be issued; of the next to be used
+    const uint32_t copy_bytes = lane & 2 ? NG * 4 : L::ROW, copy_to = smem_u32(ring) + (lane & 2 ? 2 * L::CODES + (lane & 1) * L::SCALES : (lane & 1) * L::CODES);
     const unsigned char *copy_base = lane & 2 ? reinterpret_cast<const unsigned char *>(P.c.scales[lane & 1]) : P.c.codes[lane & 1], *copy_from = nullptr;
     bool ok = true;
     auto ahead_of = [&](int skip) {   // the next item's stages but for the first `skip`
         const Stages<KEYS> S(P, ahead_b);
         ahead_left = S.count - skip;
-        ahead_key = S.begin + skip * KEYS;
+        ahead_key = S.begin + skip * KEYS + warp * L::OWN;
+        ahead_end = S.end;
         copy_from = copy_base + (((long long)ahead_b * P.c.H + (unsigned)ahead_item / F.by_blocks) * P.c.capacity + ahead_key) * copy_bytes;
     };
     auto fill = [&](int limit) {
         limit = limit < total ? limit : total;
         while (issued < limit && ok) {
-            const uint32_t st = issued % L::kStages;
-            if (issued >= L::kStages && !(ok = __all_sync(0xffffffffu, wait_or_abort(&empty[st], parity_of_use(issued, L::kStages) ^ 1, abort_flag)))) {
-                give_up(1);
-                return;
+            const uint32_t st = issued_slot;
+            issued_slot = issued_slot + 1 == L::kStages ? 0 : issued_slot + 1;
+            // the capacity is a multiple of 64, so there are all of the warp's keys or none
+            const bool some = ahead_key < ahead_end;
+            if (lane == 0) {
+                if (some) mbar_expect_tx(&full[st], L::PIECE);
+                else mbar_arrive(&full[st]);
             }
-            // the capacity and a stage's first key are multiples of 64
-            const uint32_t n = (uint32_t)((int)P.c.capacity - ahead_key < KEYS ? (int)P.c.capacity - ahead_key : KEYS);
-            if (lane == 0) mbar_expect_tx(&full[st], n * 2 * (L::ROW + NG * 4));
             __syncwarp();
-            if (lane < 4) bulk_load(copy_to + st * L::STAGE, copy_from, n * copy_bytes, &full[st]);
+            if (some && lane < 4) bulk_load(copy_to + st * L::PIECE, copy_from, L::OWN * copy_bytes, &full[st]);
             ++issued;
             ahead_key += KEYS;
             copy_from += KEYS * copy_bytes;
@@ -331,7 +344,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
         }
     };
     // one stage for now: the queries are not to wait behind what all CTAs ask for
-    if (warp == 0 && total > 0) {
+    if (total > 0) {
         ahead_of(stage);
         fill(1);
     }
@@ -402,10 +415,15 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
             }
         }
         __syncthreads();
-        if (warp == 0 && used == 0) fill(L::kStages);
+        if (used == 0) fill(L::kStages);
         uint32_t q[PARTS][NT][W][2][2], qz[NT][PARTS][2];
-        float start[NT][NG][4], factor[NT][2];   // -M a_g; raw scores times the factor are powers of 2
-        int lo[NT][2], hi[NT][2], all_lo = S.first, all_hi = S.end;   // keys that a row sees; that all rows do
+        float start[NT][NG][4], factor[NT][2];   // -M a_g (WIDE); raw scores times the factor are powers of 2
+        int all_lo = S.first, all_hi = S.end;   // keys that all rows see
+        auto sees = [&](int x, int e, int &lo, int &hi) {   // those of a row
+            const int mine = row0 + 8 * x + 2 * t + e, i = mine < F.rows ? (unsigned)mine % F.by_nq : 0;
+            lo = mine < F.rows ? see.lo(i) : 0;
+            hi = mine < F.rows ? see.hi(i) : 1 << 30;
+        };
         float m[NT][2], l[NT][2], o[NT][2 * W][4], zeros[NT][NG][2], zero_sums[NT][4];   // rows 2 t, 2 t + 1 of every block: reference (a power of 2), sums
         int top_scale = 1;                       // largest exponent of a step or zero of a value so far, as in its bits
 #pragma unroll
@@ -426,13 +444,13 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                 for (int w = 0; w < W; ++w) own += sums[w * 8 + g];
 #pragma unroll
             for (int part = 0; part < 2 * PARTS; ++part) {
-                const uint32_t word = Narrow<__nv_bfloat16>::pack(own * MIDDLE, own);
+                const uint32_t word = Narrow<__nv_bfloat16>::pack(WIDE ? own * MIDDLE : 0.f, own);
                 qz[x][part / 2][part % 2] = word;
                 own -= __uint_as_float(word & 0xffff0000u);
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int row = 2 * t + e, mine = row0 + 8 * x + row;
+                const int row = 2 * t + e;
 #pragma unroll
                 for (int k = 0; k < NG; ++k) {
                     float a = 0.f;
@@ -440,15 +458,14 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                     else
 #pragma unroll
                         for (int w = 0; w < W; ++w) a += sums[w * 8 + row];
-                    start[x][k][e] = start[x][k][2 + e] = -MIDDLE * a;
+                    start[x][k][e] = start[x][k][2 + e] = WIDE ? -MIDDLE * a : 0.f;
                     zeros[x][k][e] = 0.f;
                 }
                 factor[x][e] = sums[W * 8 + row];
-                const int i = mine < F.rows ? (unsigned)mine % F.by_nq : 0;
-                lo[x][e] = mine < F.rows ? see.lo(i) : 0;
-                hi[x][e] = mine < F.rows ? see.hi(i) : 1 << 30;
-                all_lo = max(all_lo, lo[x][e]);
-                all_hi = min(all_hi, hi[x][e]);
+                int lo, hi;
+                sees(x, e, lo, hi);
+                all_lo = max(all_lo, lo);
+                all_hi = min(all_hi, hi);
                 m[x][e] = -INFINITY;
                 l[x][e] = 0.f;
             }
@@ -461,13 +478,17 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
         }
         all_lo = __reduce_max_sync(0xffffffffu, all_lo);
         all_hi = __reduce_min_sync(0xffffffffu, all_hi);
+        uint32_t st = slot;
         for (int u = 0; u < stages; ++u, ++used) {
-            const uint32_t st = used % L::kStages;
-            if (ok && !(ok = __all_sync(0xffffffffu, wait_or_abort(&full[st], parity_of_use(used, L::kStages), abort_flag)))) give_up(2);
-            const int j0 = S.begin + (stage0 + u) * KEYS + 16 * SUB * warp;
+            st = slot;
+            if (ok && !(ok = __all_sync(0xffffffffu, wait_or_abort(&full[st], phase, abort_flag)))) give_up(2);
+            if (++slot == L::kStages) {
+                slot = 0;
+                phase ^= 1;
+            }
+            const int j0 = S.begin + (stage0 + u) * KEYS + L::OWN * warp;
             if (ok && j0 < S.end && j0 + 16 * SUB > S.first) {
-                const unsigned char *k_at = smem + st * L::STAGE + 16 * SUB * warp * L::ROW, *v_at = k_at + L::CODES;
-                const unsigned char *ks_at = smem + st * L::STAGE + 2 * L::CODES + 16 * SUB * warp * NG * 4, *vs_at = ks_at + L::SCALES;
+                const unsigned char *k_at = ring + st * L::PIECE, *v_at = k_at + L::CODES, *ks_at = v_at + L::CODES, *vs_at = ks_at + L::SCALES;
                 float p[SUB][NT][4];
 #pragma unroll
                 for (int h = 0; h < SUB; ++h) {
@@ -482,9 +503,10 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
 #pragma unroll
                     for (int x = 0; x < NT; ++x) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) p[h][x][e] = 0.f;
-#pragma unroll
-                        for (int part = 0; part < PARTS; ++part) mma_bf16(p[h][x], kz[0], kz[1], kz[0], kz[1], qz[x][part][0], qz[x][part][1]);
+                        for (int part = 0; part < PARTS; ++part) {
+                            if (part == 0) mma_bf16_new(p[h][x], kz[0], kz[1], kz[0], kz[1], qz[x][part][0], qz[x][part][1]);
+                            else mma_bf16(p[h][x], kz[0], kz[1], kz[0], kz[1], qz[x][part][0], qz[x][part][1]);
+                        }
                     }
                     float acc[NT][4];
 #pragma unroll
@@ -530,15 +552,18 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                 // keys that some row does not see; steps and zeros of those that none sees need not be numbers
                 if (j0 < all_lo || j0 + 16 * SUB > all_hi) {
 #pragma unroll
-                    for (int h = 0; h < SUB; ++h)
+                    for (int x = 0; x < NT; ++x)
 #pragma unroll
-                        for (int s = 0; s < 2; ++s) {
-                            const int j = j0 + 16 * h + 8 * s + slot0;
+                        for (int e = 0; e < 2; ++e) {
+                            int lo, hi;
+                            sees(x, e, lo, hi);
 #pragma unroll
-                            for (int x = 0; x < NT; ++x)
+                            for (int h = 0; h < SUB; ++h)
 #pragma unroll
-                                for (int e = 0; e < 2; ++e)
-                                    if (j < lo[x][e] || j >= hi[x][e] || j >= S.end) p[h][x][2 * s + e] = -INFINITY;
+                                for (int s = 0; s < 2; ++s) {
+                                    const int j = j0 + 16 * h + 8 * s + slot0;
+                                    if (j < lo || j >= hi || j >= S.end) p[h][x][2 * s + e] = -INFINITY;
+                                }
                         }
                     const int j = j0 + lane % (16 * SUB);
                     if (j < S.first || j >= S.end)
@@ -548,7 +573,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                 // the reference moves, and sums are scaled, only where a score, a step or a zero has left it behind
                 uint32_t high_scale = 0;
 #pragma unroll
-                for (int k = 0; k < NG; ++k) high_scale = __vmaxu2(high_scale, vs[k] & 0x7fffffffu);   // steps are not negative
+                for (int k = 0; k < NG; ++k) high_scale = max_halves(high_scale, vs[k] & 0x7fffffffu);   // steps are not negative
                 high_scale = max(high_scale << 16, high_scale & 0xffff0000u);
                 bool moves = (int)(high_scale >> 23) > top_scale;
                 float high[NT][2];
@@ -708,12 +733,13 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                 }
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&empty[st]);
             // the last stage's room is where the warps' outputs meet: it is filled anew after that
-            if (warp == 0 && u + 1 < stages) fill(used + L::kStages);
+            if (u + 1 < stages) fill(used + 1 + L::kStages);
         }
-        // The warps' outputs meet, 8 rows at a time: [warp][row][feature] beside references and sums.  A thread weighs four features of a row together.
-        float *share = reinterpret_cast<float *>(smem + (used > 0 ? (used - 1) % L::kStages : 0) * L::STAGE);
+        // The warps' outputs meet, 8 rows at a time, each in the room of its last stage beside references and sums.  A thread weighs four features of a
+        // row together.
+        const uint32_t share_at = st * L::PIECE;
+        float *share = reinterpret_cast<float *>(ring + share_at);
         const int power = top_scale + 1 - 127;
         // two factors: either's exponent stays within 32 bits' range
         const float unit = power_of_two(127 + power / 2), unit2 = power_of_two(127 + power - power / 2);
@@ -722,7 +748,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
         const long long part = ((long long)blockIdx.x * 2 + (stage0 == 0 ? 1 : 0)) * ROWS;
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
-            __syncthreads();
+            if (x > 0) __syncthreads();
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
@@ -746,7 +772,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                     v.y = fmaf(o[x][2 * w][2 + e] * unit, code_upper, z);
                     v.z = fmaf(o[x][2 * w + 1][e] * unit, code, z);
                     v.w = fmaf(o[x][2 * w + 1][2 + e] * unit, code_upper, z);
-                    *reinterpret_cast<float4 *>(share + (warp * 8 + row) * DP + 32 * w + 4 * g) = v;
+                    *reinterpret_cast<float4 *>(share + row * DP + 32 * w + 4 * g) = v;
                 }
             }
             __syncthreads();
@@ -764,7 +790,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                 for (int w = 0; w < kFewWarps; ++w) {
                     if (s[w].y == 0.f) continue;   // saw nothing; what stands beside it need not be a number
                     const float by = s[w].x == -INFINITY ? s[w].y : exp2_fast(s[w].x - top);   // a sum with no reference is NaN
-                    const float4 z = *reinterpret_cast<const float4 *>(share + (w * 8 + row) * DP + d);
+                    const float4 z = *reinterpret_cast<const float4 *>(smem + w * L::RING + share_at + (row * DP + d) * 4);
                     sum = fmaf(by, s[w].y, sum);
                     v[0] = fmaf(by, z.x, v[0]);
                     v[1] = fmaf(by, z.y, v[1]);
@@ -779,10 +805,8 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
             }
         }
         __syncthreads();
-        if (warp == 0 && used > 0) {
-            fence_proxy_async_smem();   // read and written by threads before copies write there
-            fill(used + L::kStages);
-        }
+        fence_proxy_async_smem();   // read and written by threads before copies write there
+        fill(used + L::kStages);
         stage = 0;
         if (++item == items) {
             item = 0;
@@ -790,7 +814,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
             while (used < total && Stages<KEYS>(P, b).count == 0);
         }
     } while (used < total);
-    if (threadIdx.x == 0 && *abort_flag)   // what was issued arrives before the CTA ends
+    if (lane == 0 && *abort_flag)   // what was issued arrives before the CTA ends
         for (uint32_t u = first_of_last_uses(issued, L::kStages); u < (uint32_t)issued; ++u) mbar_wait_bounded(&full[u % L::kStages], parity_of_use(u, L::kStages));
 }
 
