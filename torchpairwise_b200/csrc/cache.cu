@@ -60,6 +60,7 @@ CacheAttnParams attention_params(const tpw_cache &c, const tpw_cache_attention_a
     P.window = a.window;
     P.causal = a.causal;
     P.dtype = a.dtype;
+    P.scale = a.scale;
     P.scale_log2 = (float)(a.scale * 1.4426950408889634074);
     return P;
 }
@@ -104,7 +105,7 @@ int tpw_cache_attention(const tpw_cache *c, const tpw_cache_attention_args *a, v
     if (bytes < 0) return TPW_ERR_INVALID;
     TPW_CHECK_ARG(bytes == 0 || (scratch && tpw::aligned16(scratch) && scratch_bytes >= bytes), "tpw_cache_attention: scratch of %lld bytes, 16-byte aligned, is needed", (long long)bytes);
     P.status = tpw::device_status_ptr();
-    return tpw::cache_attention(P, scratch, static_cast<cudaStream_t>(stream));
+    return tpw::cache_attention(P, scratch, scratch_bytes, static_cast<cudaStream_t>(stream));
 }
 
 } // extern "C"

@@ -36,6 +36,7 @@ struct CacheAttnParams {
     float *lse;
     long long Nq, Hq, group, window;
     int causal, dtype;
+    double scale;
     float scale_log2;
     int *status;
 };
@@ -43,9 +44,12 @@ struct CacheAttnParams {
 // cache_rows.cu
 int cache_write(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s);
 int cache_read(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s);
+// every sequence's keys and values, those before the last `last` (0: none) and their block of 128 tokens left out, at [batch, token, head] strides of x;
+// what is not stored or left out is not written
+int cache_expand(const CacheParams &P, int dtype, void *const (&x)[2], const int64_t (&stride)[3], long long last, cudaStream_t s);
 // cache_attention.cu; -1: refused
 long long cache_attention_bytes(const CacheAttnParams &P);
-int cache_attention(const CacheAttnParams &P, void *scratch, cudaStream_t s);
+int cache_attention(const CacheAttnParams &P, void *scratch, long long bytes, cudaStream_t s);
 // cache_few_4.cu, cache_few_8.cu; with `bytes` they only say how much scratch the call wants
 int cache_few_4(const CacheAttnParams &P, void *scratch, long long *bytes, cudaStream_t s);
 int cache_few_8(const CacheAttnParams &P, void *scratch, long long *bytes, cudaStream_t s);
@@ -61,11 +65,9 @@ struct CacheSeen {
     int length, off, window;   // keys that there are; position of query 0; window: 0 none
     bool causal;
     __device__ __forceinline__ CacheSeen(const CacheAttnParams &P, int b) {
-        int n = P.c.lengths[b];
-        const int cap = (int)P.c.capacity;
-        n = n < 0 ? 0 : n > (1 << 30) ? 1 << 30 : n;
-        length = n < cap ? n : cap;
-        off = n - (int)P.Nq;
+        const int n = P.c.lengths[b], cap = (int)P.c.capacity;
+        length = n < 0 ? 0 : n < cap ? n : cap;
+        off = length - (int)P.Nq;
         causal = P.causal != 0;
         window = (int)(P.window < cap ? P.window : 0);   // a window over all keys is none
     }

@@ -14,6 +14,8 @@ struct RowsParams {
     long long stride[2][3];
     long long N, rows;         // rows = B * H * N
     int from_start, vector;    // vector: 16-byte pieces of a row
+    int leave;                 // read: rows that are not stored are left as they were
+    long long last;            // read: and those before the last so many and their block of 128; 0: none are
 };
 
 __device__ __forceinline__ float min_nan(float a, float b) {
@@ -174,6 +176,10 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const RowsParams R
     if (r >= R.rows || n <= 0) return;
     const Row row(R, r);
     float x[8] = {};
+    if (R.leave) {
+        const long long end = R.c.lengths[row.b] < R.c.capacity ? R.c.lengths[row.b] : R.c.capacity;
+        if (!row.stored || (R.last > 0 && row.at < ((end - R.last) & ~127LL))) return;
+    }
     if (row.stored) {
         const long long place = row.place(R);
         const unsigned char *from = R.c.codes[which] + place * R.c.row_bytes;
@@ -195,7 +201,7 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const RowsParams R
             x[k] = fmaf(__uint_as_float(c | 0x4b000000u) - 8388608.f, step_of(scales), zero_of(scales));
         }
     }
-    store8(static_cast<T *>(R.x[which]) + ((row.b * R.N + row.i) * R.c.H + row.h) * R.c.D + 8 * l, x, n, R.vector);
+    store8(static_cast<T *>(R.x[which]) + row.b * R.stride[which][0] + row.i * R.stride[which][1] + row.h * R.stride[which][2] + 8 * l, x, n, R.vector);
 }
 
 template <typename T, int BITS, int W> int launch(const RowsParams &R, bool write, cudaStream_t s) {
@@ -215,28 +221,45 @@ template <typename T> int launch_width(const RowsParams &R, bool write, cudaStre
     if (R.c.bits == 4) return R.c.width == 2 ? launch<T, 4, 2>(R, write, s) : R.c.width == 3 ? launch<T, 4, 3>(R, write, s) : launch<T, 4, 4>(R, write, s);
     return R.c.width == 2 ? launch<T, 8, 2>(R, write, s) : R.c.width == 3 ? launch<T, 8, 3>(R, write, s) : launch<T, 8, 4>(R, write, s);
 }
-int run(const CacheParams &P, const tpw_cache_rows &rows, bool write, cudaStream_t s) {
+RowsParams params(const CacheParams &P, int dtype, long long N, void *const (&x)[2], const int64_t (&stride)[2][3]) {
     RowsParams R = {};
     R.c = P;
-    R.N = rows.N;
-    R.rows = P.B * P.H * rows.N;
-    R.from_start = !write && rows.from_start;
-    const long long piece = rows.dtype == TPW_F32 ? 4 : 8;
+    R.N = N;
+    R.rows = P.B * P.H * N;
+    const long long piece = dtype == TPW_F32 ? 4 : 8;
     R.vector = P.D % 8 == 0;
     for (int w = 0; w < 2; ++w) {
-        R.x[w] = rows.x[w];
-        R.vector = R.vector && aligned16(rows.x[w]);
+        R.x[w] = x[w];
+        R.vector = R.vector && aligned16(x[w]);
         for (int k = 0; k < 3; ++k) {
-            R.stride[w][k] = rows.stride[w][k];
-            R.vector = R.vector && (!write || rows.stride[w][k] % piece == 0);
+            R.stride[w][k] = stride[w][k];
+            R.vector = R.vector && stride[w][k] % piece == 0;
         }
     }
-    return rows.dtype == TPW_F32 ? launch_width<float>(R, write, s) : rows.dtype == TPW_F16 ? launch_width<__half>(R, write, s) : launch_width<__nv_bfloat16>(R, write, s);
+    return R;
+}
+int run(int dtype, const RowsParams &R, bool write, cudaStream_t s) {
+    return dtype == TPW_F32 ? launch_width<float>(R, write, s) : dtype == TPW_F16 ? launch_width<__half>(R, write, s) : launch_width<__nv_bfloat16>(R, write, s);
 }
 
 } // namespace
 
-int cache_write(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s) { return run(P, rows, true, s); }
-int cache_read(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s) { return run(P, rows, false, s); }
+int cache_write(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s) { return run(rows.dtype, params(P, rows.dtype, rows.N, rows.x, rows.stride), true, s); }
+
+int cache_read(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s) {
+    const int64_t dense[3] = {rows.N * P.H * P.D, P.H * P.D, P.D}, stride[2][3] = {{dense[0], dense[1], dense[2]}, {dense[0], dense[1], dense[2]}};
+    RowsParams R = params(P, rows.dtype, rows.N, rows.x, stride);
+    R.from_start = rows.from_start;
+    return run(rows.dtype, R, false, s);
+}
+
+int cache_expand(const CacheParams &P, int dtype, void *const (&x)[2], const int64_t (&stride)[3], long long last, cudaStream_t s) {
+    const int64_t both[2][3] = {{stride[0], stride[1], stride[2]}, {stride[0], stride[1], stride[2]}};
+    RowsParams R = params(P, dtype, P.capacity, x, both);
+    R.from_start = 1;
+    R.leave = 1;
+    R.last = last;
+    return run(dtype, R, false, s);
+}
 
 } // namespace tpw

@@ -54,6 +54,16 @@ Tensor fresh(at::IntArrayRef sizes, const Tensor &like, at::ScalarType type) {
 
 // A view whose features lie side by side, with strides that are read as they are; anything else is copied.
 Tensor laid_out(const Tensor &x) { return x.is_neg() || (x.size(3) != 1 && x.stride(3) != 1) ? x.contiguous() : x; }
+// Queries: many of them go through attention's tensor-core kernels, which fetch 16-bit rows in pieces of 16 bytes and take no broadcast dimensions
+Tensor laid_out_queries(const Tensor &x) {
+    bool fits = !x.is_neg() && (x.size(3) == 1 || x.stride(3) == 1);
+    for (int d = 0; d < 3; ++d) fits = fits && (x.size(d) == 1 || x.stride(d) > 0);
+    if (fits && x.element_size() == 2 && x.size(3) % 8 == 0) {
+        fits = reinterpret_cast<uintptr_t>(x.const_data_ptr()) % 16 == 0;
+        for (int d = 0; d < 3; ++d) fits = fits && (x.size(d) == 1 || x.stride(d) % 8 == 0);
+    }
+    return fits ? x : x.contiguous();
+}
 void strides_of(const Tensor &x, int64_t (&s)[3]) {
     // a dimension of one has no stride of its own: the one that a dense tensor would have
     const int64_t dense[3] = {x.size(1) * x.size(2) * x.size(3), x.size(2) * x.size(3), x.size(3)};
@@ -166,7 +176,7 @@ std::tuple<Tensor, Tensor> cache_attention(const Tensor &q_, const Tensor &k_cod
     a.scale = scale.value_or(1.0 / std::sqrt(static_cast<double>(features)));
     TORCH_CHECK(a.scale > 0 && std::isfinite(a.scale), "cache_attention: scale must be positive and finite. Got ", a.scale);
     no_gradient("cache_attention", q_);
-    const Tensor q = laid_out(q_);
+    const Tensor q = laid_out_queries(q_);
     a.q = q.const_data_ptr();
     strides_of(q, a.q_stride);
     a.causal = causal;
