@@ -17,7 +17,7 @@ int few(const CacheAttnParams &P, void *scratch, long long *bytes, cudaStream_t 
 struct Slices {
     long long row, sequence, step;   // bytes of a token and head, of a sequence's keys (or values); sequences at a time
     explicit Slices(const CacheAttnParams &P) {
-        row = P.c.D * (P.dtype == TPW_F32 ? 4 : 2);
+        row = P.c.D * 2;
         sequence = (P.c.capacity * P.c.H * row + 15) / 16 * 16;
         step = sequence > 0 ? kSlice / (2 * sequence) : P.c.B;
         step = step < 1 ? 1 : step < P.c.B ? step : P.c.B;
@@ -25,7 +25,7 @@ struct Slices {
     long long bytes() const { return 2 * sequence * step; }
 };
 tpw_attention slice(const CacheAttnParams &P, const Slices &S, void *scratch, long long first, long long count) {
-    const long long e = P.dtype == TPW_F32 ? 4 : 2;
+    const long long e = 2;   // bytes of a number
     tpw_attention a = {};
     a.dtype = P.dtype;
     a.causal = P.causal;
@@ -45,11 +45,13 @@ tpw_attention slice(const CacheAttnParams &P, const Slices &S, void *scratch, lo
     return a;
 }
 
+// Measured (bfloat16, 4 bits, [2, 16384, 8, 128] ragged): 192 rows 103 us as few and 132 as many, 256 rows 130 and 133, 512 rows 239 and 141; [8, 4096, 8, 128] the same; [1, 1000]
+// 31 and 25 at 192.  Float32 stays: [2, 8192, 8, 128] 512 rows 263 and 821 us, [2, 8192, 8, 64] 1024 rows 302 and 325.
 bool is_few(const CacheAttnParams &P) {
-    if (P.group * P.Nq <= 64) return true;
+    if (P.dtype == TPW_F32 || P.group * P.Nq <= 192) return true;
     const tpw_attention a = slice(P, Slices(P), reinterpret_cast<void *>(256), 0, 1);   // of the scratch only its alignment takes part
     const AttnParams A = attn_params(a);
-    return !attn_tc_fits(a.dtype, A) && !attn_f32_fits(a.dtype, A);   // attention's own kernels for odd widths are slower still
+    return !attn_tc_fits(a.dtype, A);   // attention's own kernels for odd widths are slower still
 }
 
 } // namespace

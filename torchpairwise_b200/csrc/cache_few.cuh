@@ -818,36 +818,38 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
         for (uint32_t u = first_of_last_uses(issued, L::kStages); u < (uint32_t)issued; ++u) mbar_wait_bounded(&full[u % L::kStages], parity_of_use(u, L::kStages));
 }
 
-// Items that several CTAs have parts of, and those that have no keys: a CTA to an item, a lane to four features of a row, four parts on their way at a time.
+// Items that several CTAs have parts of, and those that have no keys.  A lane has four features of a row, and four parts on their way at a time.  A CTA to an
+// item, a warp to a row; where items are few and their parts many (gridDim.y rows) a CTA to a row, whose warps share the parts.
 template <int BITS, int W, int NG, int NT, int PARTS> __global__ void __launch_bounds__(kFewThreads) cache_join_kernel(const CacheFewParams F, int shares) {
     typedef CacheFew<BITS, W, NG, NT, PARTS> L;
     const CacheAttnParams &P = F.a;
     constexpr int DP = 32 * W, ROWS = 8 * NT;
     __shared__ unsigned room[kFewWarps + 2];
+    __shared__ float met[kFewWarps][6][32];
     const int items = (int)P.c.H * F.row_blocks, of = (int)(blockIdx.x / items), item = (int)(blockIdx.x % items), hk = item / F.row_blocks, row0 = item % F.row_blocks * ROWS;
-    const int n = Stages<L::KEYS>(P, of).count;
+    const int n = Stages<L::KEYS>(P, of).count, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = 4 * lane;
     const Line line = line_of<L::KEYS>(F, 0, shares, of, room);
     const unsigned at = line.before + (unsigned)item * (n + kFewExtra) + kFewExtra;
     // the CTA that has a place of the line; where places are fewer than CTAs some have none
     auto owner = [&](unsigned place) { return (int)(((unsigned long long)(place + 1) * shares - 1) / line.total); };
-    auto none = [&](int c) { return line.start(c, shares) == line.start(c + 1, shares); };
+    auto none = [&](int c) { return line.total < (unsigned)shares && line.start(c, shares) == line.start(c + 1, shares); };
     const int first = n > 0 ? owner(at) : 0, last = n > 0 ? owner(at + n - 1) : -1;
     asm volatile("griddepcontrol.wait;" ::: "memory");   // of every CTA: what comes after this kernel comes after both
     if (first == last) return;   // written already
-    for (int k = threadIdx.x; k < ROWS * DP / 4; k += kFewThreads) {
-        const int row = k / (DP / 4), d = k % (DP / 4) * 4, r = row0 + row;
-        if (r >= F.rows) break;
-        if (d >= P.c.D) continue;
-        float top = -INFINITY, sum = 0.f, v[4] = {};
-        for (int c0 = first; c0 <= last; c0 += 4) {
+    // parts from, from + by, ... of a row: the highest reference, the weighed sums
+    auto gather = [&](int row, int from, int by, float &top, float &sum, float (&v)[4]) {
+        top = -INFINITY;
+        sum = v[0] = v[1] = v[2] = v[3] = 0.f;
+        for (int c0 = from; c0 <= last; c0 += 4 * by) {
             float2 s[4];
             float4 z[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const bool has = c0 + u <= last && !none(c0 + u);
-                const long long place = ((long long)(c0 + u) * 2 + (c0 + u == first ? 1 : 0)) * ROWS + row;
+                const int c = c0 + u * by;
+                const bool has = c <= last && !none(c);
+                const long long place = ((long long)c * 2 + (c == first ? 1 : 0)) * ROWS + row;
                 s[u] = has ? F.part_stats[place] : make_float2(-INFINITY, 0.f);
-                z[u] = has ? *reinterpret_cast<const float4 *>(F.part_out + place * DP + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+                z[u] = has && d < DP ? *reinterpret_cast<const float4 *>(F.part_out + place * DP + d) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
             float now = top;
 #pragma unroll
@@ -860,16 +862,45 @@ template <int BITS, int W, int NG, int NT, int PARTS> __global__ void __launch_b
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 if (s[u].y == 0.f) continue;
-                const float by = s[u].x == -INFINITY ? s[u].y : exp2_fast(s[u].x - top);   // a sum with no reference is NaN
-                sum = fmaf(by, s[u].y, sum);
-                v[0] = fmaf(by, z[u].x, v[0]);
-                v[1] = fmaf(by, z[u].y, v[1]);
-                v[2] = fmaf(by, z[u].z, v[2]);
-                v[3] = fmaf(by, z[u].w, v[3]);
+                const float w = s[u].x == -INFINITY ? s[u].y : exp2_fast(s[u].x - top);   // a sum with no reference is NaN
+                sum = fmaf(w, s[u].y, sum);
+                v[0] = fmaf(w, z[u].x, v[0]);
+                v[1] = fmaf(w, z[u].y, v[1]);
+                v[2] = fmaf(w, z[u].z, v[2]);
+                v[3] = fmaf(w, z[u].w, v[3]);
             }
         }
-        finish(F, of, hk, r, d, v, top, sum);
+    };
+    float top, sum, v[4];
+    if (gridDim.y == 1) {
+        for (int row = warp; row < ROWS && row0 + row < F.rows; row += kFewWarps) {
+            gather(row, first, 1, top, sum, v);
+            if (d < P.c.D) finish(F, of, hk, row0 + row, d, v, top, sum);
+        }
+        return;
     }
+    const int row = blockIdx.y;
+    if (row0 + row >= F.rows) return;
+    gather(row, first + warp, kFewWarps, top, sum, v);
+    const float mine[6] = {v[0], v[1], v[2], v[3], top, sum};
+#pragma unroll
+    for (int k = 0; k < 6; ++k) met[warp][k][lane] = mine[k];
+    __syncthreads();
+    if (warp > 0 || d >= P.c.D) return;
+    float all = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) all = fmaxf(all, met[w][4][lane]);
+    sum = v[0] = v[1] = v[2] = v[3] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) {
+        const float s = met[w][5][lane], t = met[w][4][lane];
+        if (s == 0.f) continue;
+        const float by = t == -INFINITY ? s : exp2_fast(t - all);
+        sum = fmaf(by, s, sum);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = fmaf(by, met[w][k][lane], v[k]);
+    }
+    finish(F, of, hk, row0 + row, d, v, all, sum);
 }
 
 template <int BITS, int W, int NG, int NT, int PARTS> int launch_few(CacheFewParams F, void *scratch, long long *bytes, cudaStream_t s) {
@@ -896,7 +927,7 @@ template <int BITS, int W, int NG, int NT, int PARTS> int launch_few(CacheFewPar
     TPW_LAUNCH_OK("cache_few_kernel");
     if (F.whole) return TPW_OK;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)items);
+    config.gridDim = dim3((unsigned)items, ctas > 4 * items ? (unsigned)(F.rows < (int)L::ROWS ? F.rows : L::ROWS) : 1);
     config.blockDim = dim3(kFewThreads);
     config.stream = s;
     cudaLaunchAttribute overlap = {};

@@ -6,16 +6,17 @@
 namespace tpw {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kTokens = 16;   // side by side in a block; a block takes kPasses times as many of a head, all on their way at once
+constexpr int kPasses = 4;
 
 struct RowsParams {
     CacheParams c;
     void *x[2];
     long long stride[2][3];
-    long long N, rows;         // rows = B * H * N
+    int N, tiles;              // tokens; blocks of tokens of a head
     int from_start, vector;    // vector: 16-byte pieces of a row
     int leave;                 // read: rows that are not stored are left as they were
-    long long last;            // read: and those before the last so many and their block of 128; 0: none are
+    int last;                  // read: and those before the last so many and their block of 128; 0: none are
 };
 
 __device__ __forceinline__ float min_nan(float a, float b) {
@@ -47,16 +48,24 @@ template <typename T> __device__ __forceinline__ void load8(float (&x)[8], const
         for (int k = 0; k < 8; ++k) x[k] = (float)p[k < n ? k : 0];
     }
 }
-template <typename T> __device__ __forceinline__ void store8(T *p, const float (&x)[8], int n, bool vector) {
+// `keep`: what is read next
+template <typename T> __device__ __forceinline__ void store8(T *p, const float (&x)[8], int n, bool vector, bool keep) {
     if (vector) {
         if constexpr (sizeof(T) == 4) {
-            __stcs(reinterpret_cast<float4 *>(p), make_float4(x[0], x[1], x[2], x[3]));
-            __stcs(reinterpret_cast<float4 *>(p) + 1, make_float4(x[4], x[5], x[6], x[7]));
+            const float4 a = make_float4(x[0], x[1], x[2], x[3]), b = make_float4(x[4], x[5], x[6], x[7]);
+            if (keep) {
+                reinterpret_cast<float4 *>(p)[0] = a;
+                reinterpret_cast<float4 *>(p)[1] = b;
+            } else {
+                __stcs(reinterpret_cast<float4 *>(p), a);
+                __stcs(reinterpret_cast<float4 *>(p) + 1, b);
+            }
         } else {
             alignas(16) T v[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = (T)x[k];
-            __stcs(reinterpret_cast<uint4 *>(p), *reinterpret_cast<const uint4 *>(v));
+            if (keep) *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(v);
+            else __stcs(reinterpret_cast<uint4 *>(p), *reinterpret_cast<const uint4 *>(v));
         }
     } else {
 #pragma unroll
@@ -65,20 +74,22 @@ template <typename T> __device__ __forceinline__ void store8(T *p, const float (
     }
 }
 
-// a row of the call: token i of head h of sequence b at position `at`
-struct Row {
-    long long b, i, h, at;
-    bool stored;
-    __device__ __forceinline__ Row(const RowsParams &R, long long r) {
-        i = r % R.N;
-        const long long bh = r / R.N;
-        h = bh % R.c.H;
-        b = bh / R.c.H;
-        const long long n = R.c.lengths[b];
-        at = R.from_start ? i : n - R.N + i;
-        stored = at >= 0 && at < R.c.capacity && at < n;
+// What a block works on: tokens i0, i0 + kTokens, ... of a head; token i stands at position i + shift, and positions [first, end) have a place.
+struct Block {
+    int b, h, i0, shift, end;
+    long long row0;   // of the cache
+    __device__ __forceinline__ Block(const RowsParams &R, int token) {
+        const unsigned bh = blockIdx.x / (unsigned)R.tiles;
+        h = (int)(bh % (unsigned)R.c.H);
+        b = (int)(bh / (unsigned)R.c.H);
+        i0 = (int)(blockIdx.x - bh * R.tiles) * kTokens * kPasses + token;
+        int n = R.c.lengths[b];
+        n = n < 0 ? 0 : n;
+        shift = R.from_start ? 0 : n - R.N;   // N < 2^30
+        end = n < (int)R.c.capacity ? n : (int)R.c.capacity;
+        row0 = (long long)bh * R.c.capacity;
     }
-    __device__ __forceinline__ long long place(const RowsParams &R) const { return (b * R.c.H + h) * R.c.capacity + at; }
+    __device__ __forceinline__ bool stored(int i) const { return i + shift >= 0 && i + shift < end; }
 };
 
 // where the 8 codes of lane l lie in a row: those of a key together, those of a value in two halves
@@ -96,123 +107,135 @@ template <int BITS> __device__ __forceinline__ void pack8(uint32_t (&w)[2], cons
 }
 
 template <typename T, int BITS, int W>
-__global__ void __launch_bounds__(kThreads) cache_write_kernel(const RowsParams R) {
+__global__ void __launch_bounds__(kTokens * (W == 2 ? 8 : 16)) cache_write_kernel(const RowsParams R) {
     constexpr int LANES = W == 2 ? 8 : 16;   // of a row; 4 * W of them have features
     constexpr float MOST = BITS == 4 ? 15.f : 255.f;
     const int which = blockIdx.y, l = threadIdx.x % LANES;
-    const long long r = (long long)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
-    const Row row(R, r < R.rows ? r : R.rows - 1);
-    const bool live = r < R.rows && row.stored;
+    const Block B(R, threadIdx.x / LANES);
     const int n = R.c.D - 8 * l;   // features of this lane that there are
-    float x[8];
-    float lo = INFINITY, hi = -INFINITY;
-    if (live && n > 0) {
-        load8(x, static_cast<const T *>(R.x[which]) + row.b * R.stride[which][0] + row.i * R.stride[which][1] + row.h * R.stride[which][2] + 8 * l, n, R.vector);
-        lo = hi = x[0];
+    const T *from = static_cast<const T *>(R.x[which]) + B.b * R.stride[which][0] + B.h * R.stride[which][2] + 8 * l;
+    float x[kPasses][8];
 #pragma unroll
-        for (int k = 1; k < 8; ++k) {
-            lo = min_nan(lo, x[k]);
-            hi = max_nan(hi, x[k]);
+    for (int u = 0; u < kPasses; ++u) {
+        const int i = B.i0 + u * kTokens;
+        if (i < R.N && B.stored(i) && n > 0) load8(x[u], from + i * R.stride[which][1], n, R.vector);
+        else x[u][0] = INFINITY;   // takes no part
+    }
+#pragma unroll
+    for (int u = 0; u < kPasses; ++u) {
+        const int i = B.i0 + u * kTokens;
+        const bool live = i < R.N && B.stored(i);
+        float lo = x[u][0], hi = live && n > 0 ? x[u][0] : -INFINITY;
+        if (live && n > 0)
+#pragma unroll
+            for (int k = 1; k < 8; ++k) {
+                lo = min_nan(lo, x[u][k]);
+                hi = max_nan(hi, x[u][k]);
+            }
+#pragma unroll
+        for (int d = 1; d < LANES; d <<= 1) {
+            if (d == 4 && R.c.groups > 1) break;
+            lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+            hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
         }
-    }
+        if (!live || l >= 4 * W) continue;
+        // zero: down to bfloat16
+        uint32_t zero_bits = __float_as_uint(lo);
+        if ((int)zero_bits < 0) zero_bits += 0xffffu;
+        zero_bits &= 0xffff0000u;
+        const float zero = __uint_as_float(zero_bits);
+        // step: the smallest bfloat16 number of which MOST (products of which are exact) reach the highest value.  The quotient's upper 16 bits are at
+        // most one number off.
+        const float range = __fsub_ru(hi, zero);
+        uint32_t step_bits = (__float_as_uint(range * (1.f / MOST)) + 0xffffu) & 0xffff0000u;
+        if (__uint_as_float(step_bits - 0x10000u) * MOST >= range) step_bits -= 0x10000u;
+        if (__uint_as_float(step_bits) * MOST < range) step_bits += 0x10000u;
+        const float least = 7.888609052210118e-31f;   // 2^-100
+        const bool fine = lo > -1.2676506002282294e30f && hi < 1.2676506002282294e30f;   // 2^100; NaN is not
+        const float step = fmaxf(__uint_as_float(step_bits), least), half = 0.5f * step;
+        float inv;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(step));
+        uint32_t code[8];
 #pragma unroll
-    for (int d = 1; d < LANES; d <<= 1) {
-        if (d == 4 && R.c.groups > 1) break;
-        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+        for (int k = 0; k < 8; ++k) {
+            const float d = __fsub_rn(x[u][k], zero);
+            const float y = fmaf(d, inv, 12582912.f);   // 1.5 * 2^23: a sum with it ends in the nearest whole number
+            // the reciprocal's rounding can take that one off beside a middle: what is left says so, exactly; half a step moves an odd code
+            const float left = fmaf(y - 12582912.f, -step, d);
+            int c = __float_as_int(y) & 0x1ff;
+            if (fabsf(left) > __int_as_float(__float_as_int(half) - (c & 1))) c += 1 | (__float_as_int(left) >> 31);
+            code[k] = fine && k < n ? (uint32_t)c : 0u;
+        }
+        uint32_t w[2];
+        pack8<BITS>(w, code);
+        const long long place = B.row0 + i + B.shift;
+        unsigned char *to = R.c.codes[which] + place * R.c.row_bytes;
+        if (which == 0) {
+            if (BITS == 4) *reinterpret_cast<uint32_t *>(to + key_place<BITS, W>(l)) = w[0];
+            else *reinterpret_cast<uint2 *>(to + key_place<BITS, W>(l)) = make_uint2(w[0], w[1]);
+        } else if (BITS == 4) {
+            *reinterpret_cast<uint16_t *>(to + value_place<BITS, W>(l, 0)) = (uint16_t)w[0];
+            *reinterpret_cast<uint16_t *>(to + value_place<BITS, W>(l, 1)) = (uint16_t)(w[0] >> 16);
+        } else {
+            *reinterpret_cast<uint32_t *>(to + value_place<BITS, W>(l, 0)) = w[0];
+            *reinterpret_cast<uint32_t *>(to + value_place<BITS, W>(l, 1)) = w[1];
+        }
+        const int group = R.c.groups > 1 ? l >> 2 : 0;
+        if (l == 4 * group && group < R.c.groups)
+            R.c.scales[which][place * R.c.groups + group] = fine ? __float_as_uint(step) >> 16 | zero_bits : 0x7fc07fc0u;
     }
-    if (!live || l >= 4 * W) return;
-    // zero: down to bfloat16
-    uint32_t zero_bits = __float_as_uint(lo);
-    if ((int)zero_bits < 0) zero_bits += 0xffffu;
-    zero_bits &= 0xffff0000u;
-    const float zero = __uint_as_float(zero_bits);
-    // step: the smallest bfloat16 number of which MOST (products of which are exact) reach the highest value.  The quotient's upper 16 bits are at most one
-    // number off.
-    const float range = __fsub_ru(hi, zero);
-    uint32_t step_bits = (__float_as_uint(range * (1.f / MOST)) + 0xffffu) & 0xffff0000u;
-    if (__uint_as_float(step_bits - 0x10000u) * MOST >= range) step_bits -= 0x10000u;
-    if (__uint_as_float(step_bits) * MOST < range) step_bits += 0x10000u;
-    const float least = 7.888609052210118e-31f;   // 2^-100
-    const bool fine = lo > -1.2676506002282294e30f && hi < 1.2676506002282294e30f;   // 2^100; NaN is not
-    float step = fmaxf(__uint_as_float(step_bits), least);
-    uint32_t code[8];
-    const float inv = 1.f / step, half = 0.5f * step;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const float d = __fsub_rn(x[k], zero);
-        const float y = fmaf(d, inv, 12582912.f);   // 1.5 * 2^23: a sum with it ends in the nearest whole number
-        // the reciprocal's rounding can take that one off beside a middle: what is left says so, exactly
-        const float left = fmaf(y - 12582912.f, -step, d);
-        int c = __float_as_int(y) & 0x1ff;
-        if (fabsf(left) > half || (fabsf(left) == half && (c & 1))) c += left > 0.f ? 1 : -1;
-        code[k] = fine && k < n ? (uint32_t)c : 0u;
-    }
-    uint32_t w[2];
-    pack8<BITS>(w, code);
-    const long long place = row.place(R);
-    unsigned char *to = R.c.codes[which] + place * R.c.row_bytes;
-    if (which == 0) {
-        if (BITS == 4) *reinterpret_cast<uint32_t *>(to + key_place<BITS, W>(l)) = w[0];
-        else *reinterpret_cast<uint2 *>(to + key_place<BITS, W>(l)) = make_uint2(w[0], w[1]);
-    } else if (BITS == 4) {
-        *reinterpret_cast<uint16_t *>(to + value_place<BITS, W>(l, 0)) = (uint16_t)w[0];
-        *reinterpret_cast<uint16_t *>(to + value_place<BITS, W>(l, 1)) = (uint16_t)(w[0] >> 16);
-    } else {
-        *reinterpret_cast<uint32_t *>(to + value_place<BITS, W>(l, 0)) = w[0];
-        *reinterpret_cast<uint32_t *>(to + value_place<BITS, W>(l, 1)) = w[1];
-    }
-    const int group = R.c.groups > 1 ? l >> 2 : 0;
-    if (l == 4 * group && group < R.c.groups)
-        R.c.scales[which][place * R.c.groups + group] = fine ? __float_as_uint(step) >> 16 | zero_bits : 0x7fc07fc0u;
 }
 
 template <typename T, int BITS, int W>
-__global__ void __launch_bounds__(kThreads) cache_read_kernel(const RowsParams R) {
+__global__ void __launch_bounds__(kTokens * 4 * W) cache_read_kernel(const RowsParams R) {
     constexpr int LANES = 4 * W;
-    const int which = blockIdx.y;
-    const long long at = (long long)blockIdx.x * kThreads + threadIdx.x, r = at / LANES;
-    const int l = (int)(at % LANES), n = R.c.D - 8 * l;
-    if (r >= R.rows || n <= 0) return;
-    const Row row(R, r);
-    float x[8] = {};
-    if (R.leave) {
-        const long long end = R.c.lengths[row.b] < R.c.capacity ? R.c.lengths[row.b] : R.c.capacity;
-        if (!row.stored || (R.last > 0 && row.at < ((end - R.last) & ~127LL))) return;
-    }
-    if (row.stored) {
-        const long long place = row.place(R);
+    const int which = blockIdx.y, l = threadIdx.x % LANES, n = R.c.D - 8 * l;
+    if (n <= 0) return;
+    const Block B(R, threadIdx.x / LANES);
+    const int first = R.last > 0 && B.end > R.last ? (B.end - R.last) & ~127 : 0;   // positions before it are left
+    uint32_t w[kPasses][2], scales[kPasses];
+#pragma unroll
+    for (int u = 0; u < kPasses; ++u) {
+        const int i = B.i0 + u * kTokens;
+        w[u][0] = w[u][1] = scales[u] = 0;
+        if (i >= R.N || !B.stored(i) || i + B.shift < first) continue;
+        const long long place = B.row0 + i + B.shift;
         const unsigned char *from = R.c.codes[which] + place * R.c.row_bytes;
-        uint32_t w[2];
         if (which == 0) {
-            w[0] = *reinterpret_cast<const uint32_t *>(from + key_place<BITS, W>(l));
-            if (BITS == 8) w[1] = *reinterpret_cast<const uint32_t *>(from + key_place<BITS, W>(l) + 4);
+            w[u][0] = __ldcs(reinterpret_cast<const uint32_t *>(from + key_place<BITS, W>(l)));
+            if (BITS == 8) w[u][1] = __ldcs(reinterpret_cast<const uint32_t *>(from + key_place<BITS, W>(l) + 4));
         } else if (BITS == 4) {
-            w[0] = *reinterpret_cast<const uint16_t *>(from + value_place<BITS, W>(l, 0)) | (uint32_t)*reinterpret_cast<const uint16_t *>(from + value_place<BITS, W>(l, 1)) << 16;
+            w[u][0] = __ldcs(reinterpret_cast<const uint16_t *>(from + value_place<BITS, W>(l, 0))) | (uint32_t)__ldcs(reinterpret_cast<const uint16_t *>(from + value_place<BITS, W>(l, 1))) << 16;
         } else {
-            w[0] = *reinterpret_cast<const uint32_t *>(from + value_place<BITS, W>(l, 0));
-            w[1] = *reinterpret_cast<const uint32_t *>(from + value_place<BITS, W>(l, 1));
+            w[u][0] = __ldcs(reinterpret_cast<const uint32_t *>(from + value_place<BITS, W>(l, 0)));
+            w[u][1] = __ldcs(reinterpret_cast<const uint32_t *>(from + value_place<BITS, W>(l, 1)));
         }
-        const uint32_t scales = R.c.scales[which][place * R.c.groups + (R.c.groups > 1 ? l >> 2 : 0)];
+        scales[u] = R.c.scales[which][place * R.c.groups + (R.c.groups > 1 ? l >> 2 : 0)];
+    }
+    T *to = static_cast<T *>(R.x[which]) + B.b * R.stride[which][0] + B.h * R.stride[which][2] + 8 * l;
+#pragma unroll
+    for (int u = 0; u < kPasses; ++u) {
+        const int i = B.i0 + u * kTokens;
+        if (i >= R.N || (R.leave && (!B.stored(i) || i + B.shift < first))) continue;
+        float x[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const uint32_t c = BITS == 4 ? w[0] >> (4 * k) & 15u : w[k >> 2] >> (8 * (k & 3)) & 255u;
+            const uint32_t c = BITS == 4 ? w[u][0] >> (4 * k) & 15u : w[u][k >> 2] >> (8 * (k & 3)) & 255u;
             // 2^23 + code, less 2^23: the conversion instruction is a quarter as fast
-            x[k] = fmaf(__uint_as_float(c | 0x4b000000u) - 8388608.f, step_of(scales), zero_of(scales));
+            x[k] = fmaf(__uint_as_float(c | 0x4b000000u) - 8388608.f, step_of(scales[u]), zero_of(scales[u]));
         }
+        store8(to + i * R.stride[which][1], x, n, R.vector, R.leave);
     }
-    store8(static_cast<T *>(R.x[which]) + row.b * R.stride[which][0] + row.i * R.stride[which][1] + row.h * R.stride[which][2] + 8 * l, x, n, R.vector);
 }
 
 template <typename T, int BITS, int W> int launch(const RowsParams &R, bool write, cudaStream_t s) {
-    const long long per = write ? kThreads / (W == 2 ? 8 : 16) : 0;
-    const long long blocks = write ? (R.rows + per - 1) / per : (R.rows * 4 * W + kThreads - 1) / kThreads;
+    const long long blocks = R.c.B * R.c.H * R.tiles;
     TPW_CHECK_ARG(blocks < (1LL << 31), "tpw_cache: more than 2^31 blocks of work");
     if (write) {
-        cache_write_kernel<T, BITS, W><<<dim3((unsigned)blocks, 2), kThreads, 0, s>>>(R);
+        cache_write_kernel<T, BITS, W><<<dim3((unsigned)blocks, 2), kTokens * (W == 2 ? 8 : 16), 0, s>>>(R);
         TPW_LAUNCH_OK("cache_write_kernel");
     } else {
-        cache_read_kernel<T, BITS, W><<<dim3((unsigned)blocks, 2), kThreads, 0, s>>>(R);
+        cache_read_kernel<T, BITS, W><<<dim3((unsigned)blocks, 2), kTokens * 4 * W, 0, s>>>(R);
         TPW_LAUNCH_OK("cache_read_kernel");
     }
     return TPW_OK;
@@ -224,8 +247,8 @@ template <typename T> int launch_width(const RowsParams &R, bool write, cudaStre
 RowsParams params(const CacheParams &P, int dtype, long long N, void *const (&x)[2], const int64_t (&stride)[2][3]) {
     RowsParams R = {};
     R.c = P;
-    R.N = N;
-    R.rows = P.B * P.H * N;
+    R.N = (int)N;
+    R.tiles = (int)((N + kTokens * kPasses - 1) / (kTokens * kPasses));
     const long long piece = dtype == TPW_F32 ? 4 : 8;
     R.vector = P.D % 8 == 0;
     for (int w = 0; w < 2; ++w) {
@@ -258,7 +281,7 @@ int cache_expand(const CacheParams &P, int dtype, void *const (&x)[2], const int
     RowsParams R = params(P, dtype, P.capacity, x, both);
     R.from_start = 1;
     R.leave = 1;
-    R.last = last;
+    R.last = (int)(last < P.capacity ? last : 0);
     return run(dtype, R, false, s);
 }
 
