@@ -19,14 +19,15 @@ struct RowsParams {
     int last;                  // read: and those before the last so many and their block of 128; 0: none are
 };
 
-__device__ __forceinline__ float min_nan(float a, float b) {
+// NaN if an operand is
+__device__ __forceinline__ float min_nan(float a, float b, float c) {
     float r;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 
@@ -96,13 +97,19 @@ struct Block {
 template <int BITS, int W> __device__ __forceinline__ int key_place(int l) { return ((l & 3) * W + (l >> 2)) * BITS; }
 template <int BITS, int W> __device__ __forceinline__ int value_place(int l, int half) { return ((2 * (l & 3) + half) * W + (l >> 2)) * (BITS / 2); }
 
-// 8 codes into words: 4 bits in one, 8 bits in two
-template <int BITS> __device__ __forceinline__ void pack8(uint32_t (&w)[2], const uint32_t (&code)[8]) {
-    w[0] = w[1] = 0;
+// 8 codes into words, 4 bits in one, 8 bits in two; `y` holds them above 1.5 * 2^23, whose bits add up to a constant
+template <int BITS> __device__ __forceinline__ void pack8(uint32_t (&w)[2], const float (&y)[8], int n) {
+    constexpr int PER = 32 / BITS;
+    constexpr uint32_t ONES = BITS == 4 ? 0x11111111u : 0x01010101u;
+    w[1] = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        if (BITS == 4) w[0] |= code[k] << (4 * k);
-        else w[k >> 2] |= code[k] << (8 * (k & 3));
+    for (int v = 0; v < 8 / PER; ++v) {
+        uint32_t x = 0;
+#pragma unroll
+        for (int k = PER - 1; k >= 0; --k) x = (x << BITS) + __float_as_uint(y[v * PER + k]);
+        x -= 0x4b400000u * ONES;
+        const int there = n - v * PER;
+        w[v] = there >= PER ? x : there <= 0 ? 0u : x & ((1u << (BITS * there)) - 1u);
     }
 }
 
@@ -128,15 +135,15 @@ __global__ void __launch_bounds__(kTokens * (W == 2 ? 8 : 16)) cache_write_kerne
         float lo = x[u][0], hi = live && n > 0 ? x[u][0] : -INFINITY;
         if (live && n > 0)
 #pragma unroll
-            for (int k = 1; k < 8; ++k) {
-                lo = min_nan(lo, x[u][k]);
-                hi = max_nan(hi, x[u][k]);
+            for (int k = 1; k < 8; k += 2) {
+                lo = min_nan(lo, x[u][k], x[u][k < 7 ? k + 1 : k]);
+                hi = max_nan(hi, x[u][k], x[u][k < 7 ? k + 1 : k]);
             }
 #pragma unroll
         for (int d = 1; d < LANES; d <<= 1) {
             if (d == 4 && R.c.groups > 1) break;
-            lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-            hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+            lo = min_nan(lo, lo, __shfl_xor_sync(0xffffffffu, lo, d));
+            hi = max_nan(hi, hi, __shfl_xor_sync(0xffffffffu, hi, d));
         }
         if (!live || l >= 4 * W) continue;
         // zero: down to bfloat16
@@ -152,24 +159,21 @@ __global__ void __launch_bounds__(kTokens * (W == 2 ? 8 : 16)) cache_write_kerne
         if (__uint_as_float(step_bits) * MOST < range) step_bits += 0x10000u;
         const float least = 7.888609052210118e-31f;   // 2^-100
         const bool fine = lo > -1.2676506002282294e30f && hi < 1.2676506002282294e30f;   // 2^100; NaN is not
-        const float step = fmaxf(__uint_as_float(step_bits), least), half = 0.5f * step;
+        const float step = fmaxf(__uint_as_float(step_bits), least);
         float inv;
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(step));
-        uint32_t code[8];
+        // The quotient, refined by what is left of it, exactly: a middle between two codes comes out as that.  A sum with 1.5 * 2^23 ends in the
+        // nearest whole number, ties to even.
+        float y[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const float d = __fsub_rn(x[u][k], zero);
-            const float y = fmaf(d, inv, 12582912.f);   // 1.5 * 2^23: a sum with it ends in the nearest whole number
-            // the reciprocal's rounding can take that one off beside a middle: what is left says so, exactly; half a step moves an odd code
-            const float left = fmaf(y - 12582912.f, -step, d);
-            int c = __float_as_int(y) & 0x1ff;
-            if (fabsf(left) > __int_as_float(__float_as_int(half) - (c & 1))) c += 1 | (__float_as_int(left) >> 31);
-            code[k] = fine && k < n ? (uint32_t)c : 0u;
+            const float d = __fsub_rn(x[u][k], zero), near = __fmul_rn(d, inv);
+            y[k] = __fadd_rn(fmaf(fmaf(-near, step, d), inv, near), 12582912.f);
         }
         uint32_t w[2];
-        pack8<BITS>(w, code);
+        pack8<BITS>(w, y, fine ? n : 0);
         const long long place = B.row0 + i + B.shift;
-        unsigned char *to = R.c.codes[which] + place * R.c.row_bytes;
+        unsigned char *to = R.c.codes[which] + place * (W * 4 * BITS);
         if (which == 0) {
             if (BITS == 4) *reinterpret_cast<uint32_t *>(to + key_place<BITS, W>(l)) = w[0];
             else *reinterpret_cast<uint2 *>(to + key_place<BITS, W>(l)) = make_uint2(w[0], w[1]);
@@ -200,7 +204,7 @@ __global__ void __launch_bounds__(kTokens * 4 * W) cache_read_kernel(const RowsP
         w[u][0] = w[u][1] = scales[u] = 0;
         if (i >= R.N || !B.stored(i) || i + B.shift < first) continue;
         const long long place = B.row0 + i + B.shift;
-        const unsigned char *from = R.c.codes[which] + place * R.c.row_bytes;
+        const unsigned char *from = R.c.codes[which] + place * (W * 4 * BITS);
         if (which == 0) {
             w[u][0] = __ldcs(reinterpret_cast<const uint32_t *>(from + key_place<BITS, W>(l)));
             if (BITS == 8) w[u][1] = __ldcs(reinterpret_cast<const uint32_t *>(from + key_place<BITS, W>(l) + 4));
@@ -220,9 +224,10 @@ __global__ void __launch_bounds__(kTokens * 4 * W) cache_read_kernel(const RowsP
         float x[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const uint32_t c = BITS == 4 ? w[u][0] >> (4 * k) & 15u : w[u][k >> 2] >> (8 * (k & 3)) & 255u;
-            // 2^23 + code, less 2^23: the conversion instruction is a quarter as fast
-            x[k] = fmaf(__uint_as_float(c | 0x4b000000u) - 8388608.f, step_of(scales[u]), zero_of(scales[u]));
+            // a byte to a code, then 2^23 + code less 2^23: the conversion instruction is a quarter as fast
+            const uint32_t bytes = BITS == 8 ? w[u][k >> 2] : (k & 1 ? w[u][0] >> 4 : w[u][0]) & 0x0f0f0f0fu;
+            const uint32_t c = __byte_perm(bytes, 0x4b000000u, 0x7440 + (BITS == 8 ? k & 3 : k >> 1));
+            x[k] = fmaf(__uint_as_float(c) - 8388608.f, step_of(scales[u]), zero_of(scales[u]));
         }
         store8(to + i * R.stride[which][1], x, n, R.vector, R.leave);
     }
