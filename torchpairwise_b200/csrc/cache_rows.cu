@@ -1,19 +1,18 @@
 // Tokens into a cache of quantised keys and values, and out of it.
-//
-// A lane has 8 neighbouring features of a row, 8 or 16 lanes the row; a group's lowest and highest value meet over 4 lanes (or all of the row).
+#include "attention_tc.cuh"
 #include "cache.cuh"
 
 namespace tpw {
 namespace {
 
-constexpr int kTokens = 16;   // side by side in a block; a block takes kPasses times as many of a head, all on their way at once
-constexpr int kPasses = 4;
+constexpr int kWriteTokens = 32, kReadTokens = 64, kReadSide = 16;   // of a block; read: side by side, the others in further passes
 
 struct RowsParams {
     CacheParams c;
     void *x[2];
     long long stride[2][3];
     int N, tiles;              // tokens; blocks of tokens of a head
+    Divider by_tiles, by_heads;
     int from_start, vector;    // vector: 16-byte pieces of a row
     int leave;                 // read: rows that are not stored are left as they were
     int last;                  // read: and those before the last so many and their block of 128; 0: none are
@@ -62,11 +61,9 @@ template <typename T> __device__ __forceinline__ void store8(T *p, const float (
                 __stcs(reinterpret_cast<float4 *>(p) + 1, b);
             }
         } else {
-            alignas(16) T v[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = (T)x[k];
-            if (keep) *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(v);
-            else __stcs(reinterpret_cast<uint4 *>(p), *reinterpret_cast<const uint4 *>(v));
+            const uint4 v = make_uint4(Narrow<T>::pack(x[0], x[1]), Narrow<T>::pack(x[2], x[3]), Narrow<T>::pack(x[4], x[5]), Narrow<T>::pack(x[6], x[7]));
+            if (keep) *reinterpret_cast<uint4 *>(p) = v;
+            else __stcs(reinterpret_cast<uint4 *>(p), v);
         }
     } else {
 #pragma unroll
@@ -75,15 +72,15 @@ template <typename T> __device__ __forceinline__ void store8(T *p, const float (
     }
 }
 
-// What a block works on: tokens i0, i0 + kTokens, ... of a head; token i stands at position i + shift, and positions [first, end) have a place.
-struct Block {
+// What a block works on: TOKENS tokens of a head, this thread's first being i0; token i stands at position i + shift, and positions [0, end) have a place.
+template <int TOKENS> struct Block {
     int b, h, i0, shift, end;
     long long row0;   // of the cache
     __device__ __forceinline__ Block(const RowsParams &R, int token) {
-        const unsigned bh = blockIdx.x / (unsigned)R.tiles;
-        h = (int)(bh % (unsigned)R.c.H);
-        b = (int)(bh / (unsigned)R.c.H);
-        i0 = (int)(blockIdx.x - bh * R.tiles) * kTokens * kPasses + token;
+        const unsigned bh = blockIdx.x / R.by_tiles;
+        b = (int)(bh / R.by_heads);
+        h = (int)bh - b * (int)R.c.H;
+        i0 = (int)(blockIdx.x - bh * R.tiles) * TOKENS + token;
         int n = R.c.lengths[b];
         n = n < 0 ? 0 : n;
         shift = R.from_start ? 0 : n - R.N;   // N < 2^30
@@ -113,123 +110,127 @@ template <int BITS> __device__ __forceinline__ void pack8(uint32_t (&w)[2], cons
     }
 }
 
+// A lane has 32 features of a token, so that what a group's step costs is paid once; 2 or 4 lanes a token.
 template <typename T, int BITS, int W>
-__global__ void __launch_bounds__(kTokens * (W == 2 ? 8 : 16)) cache_write_kernel(const RowsParams R) {
-    constexpr int LANES = W == 2 ? 8 : 16;   // of a row; 4 * W of them have features
+__global__ void __launch_bounds__(kWriteTokens * (W == 2 ? 2 : 4)) cache_write_kernel(const RowsParams R) {
+    constexpr int LANES = W == 2 ? 2 : 4;   // of a token; W of them have features
     constexpr float MOST = BITS == 4 ? 15.f : 255.f;
-    const int which = blockIdx.y, l = threadIdx.x % LANES;
-    const Block B(R, threadIdx.x / LANES);
-    const int n = R.c.D - 8 * l;   // features of this lane that there are
-    const T *from = static_cast<const T *>(R.x[which]) + B.b * R.stride[which][0] + B.h * R.stride[which][2] + 8 * l;
-    float x[kPasses][8];
+    const int which = blockIdx.y, w = threadIdx.x % LANES;
+    const Block<kWriteTokens> B(R, threadIdx.x / LANES);
+    const int n = R.c.D - 32 * w;   // features of this lane that there are
+    const bool stored = B.i0 < R.N && B.stored(B.i0), live = stored && n > 0;
+    const T *from = static_cast<const T *>(R.x[which]) + B.b * R.stride[which][0] + B.i0 * R.stride[which][1] + B.h * R.stride[which][2] + 32 * w;
+    float x[4][8];
 #pragma unroll
-    for (int u = 0; u < kPasses; ++u) {
-        const int i = B.i0 + u * kTokens;
-        if (i < R.N && B.stored(i) && n > 0) load8(x[u], from + i * R.stride[which][1], n, R.vector);
-        else x[u][0] = INFINITY;   // takes no part
-    }
+    for (int v = 0; v < 4; ++v)
+        if (live && 8 * v < n) load8(x[v], from + 8 * v, n - 8 * v, R.vector);
+    float lo = INFINITY, hi = -INFINITY;
+    if (live)
 #pragma unroll
-    for (int u = 0; u < kPasses; ++u) {
-        const int i = B.i0 + u * kTokens;
-        const bool live = i < R.N && B.stored(i);
-        float lo = x[u][0], hi = live && n > 0 ? x[u][0] : -INFINITY;
-        if (live && n > 0)
+        for (int v = 0; v < 4; ++v)
+            if (8 * v < n)
 #pragma unroll
-            for (int k = 1; k < 8; k += 2) {
-                lo = min_nan(lo, x[u][k], x[u][k < 7 ? k + 1 : k]);
-                hi = max_nan(hi, x[u][k], x[u][k < 7 ? k + 1 : k]);
-            }
+                for (int k = 0; k < 8; k += 2) {
+                    lo = min_nan(lo, x[v][k], x[v][k + 1]);
+                    hi = max_nan(hi, x[v][k], x[v][k + 1]);
+                }
+    if (R.c.groups == 1)
 #pragma unroll
         for (int d = 1; d < LANES; d <<= 1) {
-            if (d == 4 && R.c.groups > 1) break;
             lo = min_nan(lo, lo, __shfl_xor_sync(0xffffffffu, lo, d));
             hi = max_nan(hi, hi, __shfl_xor_sync(0xffffffffu, hi, d));
         }
-        if (!live || l >= 4 * W) continue;
-        // zero: down to bfloat16
-        uint32_t zero_bits = __float_as_uint(lo);
-        if ((int)zero_bits < 0) zero_bits += 0xffffu;
-        zero_bits &= 0xffff0000u;
-        const float zero = __uint_as_float(zero_bits);
-        // step: the smallest bfloat16 number of which MOST (products of which are exact) reach the highest value.  The quotient's upper 16 bits are at
-        // most one number off.
-        const float range = __fsub_ru(hi, zero);
-        uint32_t step_bits = (__float_as_uint(range * (1.f / MOST)) + 0xffffu) & 0xffff0000u;
-        if (__uint_as_float(step_bits - 0x10000u) * MOST >= range) step_bits -= 0x10000u;
-        if (__uint_as_float(step_bits) * MOST < range) step_bits += 0x10000u;
-        const float least = 7.888609052210118e-31f;   // 2^-100
-        const bool fine = lo > -1.2676506002282294e30f && hi < 1.2676506002282294e30f;   // 2^100; NaN is not
-        const float step = fmaxf(__uint_as_float(step_bits), least);
-        float inv;
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(step));
+    if (!stored || w >= W) return;
+    // zero: down to bfloat16
+    uint32_t zero_bits = __float_as_uint(lo);
+    if ((int)zero_bits < 0) zero_bits += 0xffffu;
+    zero_bits &= 0xffff0000u;
+    const float zero = __uint_as_float(zero_bits);
+    // step: the smallest bfloat16 number of which MOST (products of which are exact) reach the highest value.  The quotient's upper 16 bits are at
+    // most one number off.
+    const float range = __fsub_ru(hi, zero);
+    uint32_t step_bits = (__float_as_uint(range * (1.f / MOST)) + 0xffffu) & 0xffff0000u;
+    if (__uint_as_float(step_bits - 0x10000u) * MOST >= range) step_bits -= 0x10000u;
+    if (__uint_as_float(step_bits) * MOST < range) step_bits += 0x10000u;
+    const float least = 7.888609052210118e-31f;   // 2^-100
+    const bool fine = lo > -1.2676506002282294e30f && hi < 1.2676506002282294e30f;   // 2^100; NaN is not
+    const float step = fmaxf(__uint_as_float(step_bits), least);
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(step));
+    const long long place = B.row0 + B.i0 + B.shift;
+    unsigned char *to = R.c.codes[which] + place * (W * 4 * BITS);
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
         // The quotient, refined by what is left of it, exactly: a middle between two codes comes out as that.  A sum with 1.5 * 2^23 ends in the
         // nearest whole number, ties to even.
         float y[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const float d = __fsub_rn(x[u][k], zero), near = __fmul_rn(d, inv);
+            const float d = __fsub_rn(x[v][k], zero), near = __fmul_rn(d, inv);
             y[k] = __fadd_rn(fmaf(fmaf(-near, step, d), inv, near), 12582912.f);
         }
-        uint32_t w[2];
-        pack8<BITS>(w, y, fine ? n : 0);
-        const long long place = B.row0 + i + B.shift;
-        unsigned char *to = R.c.codes[which] + place * (W * 4 * BITS);
+        uint32_t code[2];
+        pack8<BITS>(code, y, live && fine ? n - 8 * v : 0);
+        const int l = 4 * w + v;
         if (which == 0) {
-            if (BITS == 4) *reinterpret_cast<uint32_t *>(to + key_place<BITS, W>(l)) = w[0];
-            else *reinterpret_cast<uint2 *>(to + key_place<BITS, W>(l)) = make_uint2(w[0], w[1]);
+            if (BITS == 4) *reinterpret_cast<uint32_t *>(to + key_place<BITS, W>(l)) = code[0];
+            else *reinterpret_cast<uint2 *>(to + key_place<BITS, W>(l)) = make_uint2(code[0], code[1]);
         } else if (BITS == 4) {
-            *reinterpret_cast<uint16_t *>(to + value_place<BITS, W>(l, 0)) = (uint16_t)w[0];
-            *reinterpret_cast<uint16_t *>(to + value_place<BITS, W>(l, 1)) = (uint16_t)(w[0] >> 16);
+            *reinterpret_cast<uint16_t *>(to + value_place<BITS, W>(l, 0)) = (uint16_t)code[0];
+            *reinterpret_cast<uint16_t *>(to + value_place<BITS, W>(l, 1)) = (uint16_t)(code[0] >> 16);
         } else {
-            *reinterpret_cast<uint32_t *>(to + value_place<BITS, W>(l, 0)) = w[0];
-            *reinterpret_cast<uint32_t *>(to + value_place<BITS, W>(l, 1)) = w[1];
+            *reinterpret_cast<uint32_t *>(to + value_place<BITS, W>(l, 0)) = code[0];
+            *reinterpret_cast<uint32_t *>(to + value_place<BITS, W>(l, 1)) = code[1];
         }
-        const int group = R.c.groups > 1 ? l >> 2 : 0;
-        if (l == 4 * group && group < R.c.groups)
-            R.c.scales[which][place * R.c.groups + group] = fine ? __float_as_uint(step) >> 16 | zero_bits : 0x7fc07fc0u;
     }
+    if (R.c.groups > 1 ? w < R.c.groups : w == 0) R.c.scales[which][place * R.c.groups + w] = fine ? __float_as_uint(step) >> 16 | zero_bits : 0x7fc07fc0u;
 }
 
 template <typename T, int BITS, int W>
-__global__ void __launch_bounds__(kTokens * 4 * W) cache_read_kernel(const RowsParams R) {
-    constexpr int LANES = 4 * W;
+__global__ void __launch_bounds__(kReadSide * 4 * W) cache_read_kernel(const RowsParams R) {
+    constexpr int LANES = 4 * W, PASSES = kReadTokens / kReadSide, ROW = W * 4 * BITS;
     const int which = blockIdx.y, l = threadIdx.x % LANES, n = R.c.D - 8 * l;
     if (n <= 0) return;
-    const Block B(R, threadIdx.x / LANES);
+    const Block<kReadTokens> B(R, threadIdx.x / LANES);
     const int first = R.last > 0 && B.end > R.last ? (B.end - R.last) & ~127 : 0;   // positions before it are left
-    uint32_t w[kPasses][2], scales[kPasses];
+    const long long place = B.row0 + B.i0 + B.shift;
+    const unsigned char *from = R.c.codes[which] + place * ROW;
+    const uint32_t *from_scales = R.c.scales[which] + place * R.c.groups + (R.c.groups > 1 ? l >> 2 : 0);
+    uint32_t w[PASSES][2], scales[PASSES];
+    bool there[PASSES];
 #pragma unroll
-    for (int u = 0; u < kPasses; ++u) {
-        const int i = B.i0 + u * kTokens;
+    for (int u = 0; u < PASSES; ++u) {
+        const int i = B.i0 + u * kReadSide;
         w[u][0] = w[u][1] = scales[u] = 0;
-        if (i >= R.N || !B.stored(i) || i + B.shift < first) continue;
-        const long long place = B.row0 + i + B.shift;
-        const unsigned char *from = R.c.codes[which] + place * (W * 4 * BITS);
+        there[u] = i < R.N && B.stored(i) && i + B.shift >= first;
+        if (!there[u]) continue;
+        const unsigned char *row = from + u * kReadSide * ROW;
         if (which == 0) {
-            w[u][0] = __ldcs(reinterpret_cast<const uint32_t *>(from + key_place<BITS, W>(l)));
-            if (BITS == 8) w[u][1] = __ldcs(reinterpret_cast<const uint32_t *>(from + key_place<BITS, W>(l) + 4));
+            w[u][0] = __ldcs(reinterpret_cast<const uint32_t *>(row + key_place<BITS, W>(l)));
+            if (BITS == 8) w[u][1] = __ldcs(reinterpret_cast<const uint32_t *>(row + key_place<BITS, W>(l) + 4));
         } else if (BITS == 4) {
-            w[u][0] = __ldcs(reinterpret_cast<const uint16_t *>(from + value_place<BITS, W>(l, 0))) | (uint32_t)__ldcs(reinterpret_cast<const uint16_t *>(from + value_place<BITS, W>(l, 1))) << 16;
+            w[u][0] = __ldcs(reinterpret_cast<const uint16_t *>(row + value_place<BITS, W>(l, 0))) | (uint32_t)__ldcs(reinterpret_cast<const uint16_t *>(row + value_place<BITS, W>(l, 1))) << 16;
         } else {
-            w[u][0] = __ldcs(reinterpret_cast<const uint32_t *>(from + value_place<BITS, W>(l, 0)));
-            w[u][1] = __ldcs(reinterpret_cast<const uint32_t *>(from + value_place<BITS, W>(l, 1)));
+            w[u][0] = __ldcs(reinterpret_cast<const uint32_t *>(row + value_place<BITS, W>(l, 0)));
+            w[u][1] = __ldcs(reinterpret_cast<const uint32_t *>(row + value_place<BITS, W>(l, 1)));
         }
-        scales[u] = R.c.scales[which][place * R.c.groups + (R.c.groups > 1 ? l >> 2 : 0)];
+        scales[u] = from_scales[u * kReadSide * R.c.groups];
     }
-    T *to = static_cast<T *>(R.x[which]) + B.b * R.stride[which][0] + B.h * R.stride[which][2] + 8 * l;
+    T *to = static_cast<T *>(R.x[which]) + B.b * R.stride[which][0] + B.i0 * R.stride[which][1] + B.h * R.stride[which][2] + 8 * l;
+    const long long further = kReadSide * R.stride[which][1];
 #pragma unroll
-    for (int u = 0; u < kPasses; ++u) {
-        const int i = B.i0 + u * kTokens;
-        if (i >= R.N || (R.leave && (!B.stored(i) || i + B.shift < first))) continue;
+    for (int u = 0; u < PASSES; ++u, to += further) {
+        if (R.leave ? !there[u] : B.i0 + u * kReadSide >= R.N) continue;
+        const float step = step_of(scales[u]), zero = zero_of(scales[u]);
+        const uint32_t even = w[u][0] & 0x0f0f0f0fu, odd = (w[u][0] >> 4) & 0x0f0f0f0fu;
         float x[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             // a byte to a code, then 2^23 + code less 2^23: the conversion instruction is a quarter as fast
-            const uint32_t bytes = BITS == 8 ? w[u][k >> 2] : (k & 1 ? w[u][0] >> 4 : w[u][0]) & 0x0f0f0f0fu;
-            const uint32_t c = __byte_perm(bytes, 0x4b000000u, 0x7440 + (BITS == 8 ? k & 3 : k >> 1));
-            x[k] = fmaf(__uint_as_float(c) - 8388608.f, step_of(scales[u]), zero_of(scales[u]));
+            const uint32_t c = __byte_perm(BITS == 8 ? w[u][k >> 2] : k & 1 ? odd : even, 0x4b000000u, 0x7440 + (BITS == 8 ? k & 3 : k >> 1));
+            x[k] = fmaf(__uint_as_float(c) - 8388608.f, step, zero);
         }
-        store8(to + i * R.stride[which][1], x, n, R.vector, R.leave);
+        store8(to, x, n, R.vector, R.leave);
     }
 }
 
@@ -237,10 +238,10 @@ template <typename T, int BITS, int W> int launch(const RowsParams &R, bool writ
     const long long blocks = R.c.B * R.c.H * R.tiles;
     TPW_CHECK_ARG(blocks < (1LL << 31), "tpw_cache: more than 2^31 blocks of work");
     if (write) {
-        cache_write_kernel<T, BITS, W><<<dim3((unsigned)blocks, 2), kTokens * (W == 2 ? 8 : 16), 0, s>>>(R);
+        cache_write_kernel<T, BITS, W><<<dim3((unsigned)blocks, 2), kWriteTokens * (W == 2 ? 2 : 4), 0, s>>>(R);
         TPW_LAUNCH_OK("cache_write_kernel");
     } else {
-        cache_read_kernel<T, BITS, W><<<dim3((unsigned)blocks, 2), kTokens * 4 * W, 0, s>>>(R);
+        cache_read_kernel<T, BITS, W><<<dim3((unsigned)blocks, 2), kReadSide * 4 * W, 0, s>>>(R);
         TPW_LAUNCH_OK("cache_read_kernel");
     }
     return TPW_OK;
@@ -249,11 +250,13 @@ template <typename T> int launch_width(const RowsParams &R, bool write, cudaStre
     if (R.c.bits == 4) return R.c.width == 2 ? launch<T, 4, 2>(R, write, s) : R.c.width == 3 ? launch<T, 4, 3>(R, write, s) : launch<T, 4, 4>(R, write, s);
     return R.c.width == 2 ? launch<T, 8, 2>(R, write, s) : R.c.width == 3 ? launch<T, 8, 3>(R, write, s) : launch<T, 8, 4>(R, write, s);
 }
-RowsParams params(const CacheParams &P, int dtype, long long N, void *const (&x)[2], const int64_t (&stride)[2][3]) {
+RowsParams params(const CacheParams &P, int dtype, long long N, int tokens, void *const (&x)[2], const int64_t (&stride)[2][3]) {
     RowsParams R = {};
     R.c = P;
     R.N = (int)N;
-    R.tiles = (int)((N + kTokens * kPasses - 1) / (kTokens * kPasses));
+    R.tiles = (int)((N + tokens - 1) / tokens);
+    R.by_tiles = divider(R.tiles);
+    R.by_heads = divider(P.H);
     const long long piece = dtype == TPW_F32 ? 4 : 8;
     R.vector = P.D % 8 == 0;
     for (int w = 0; w < 2; ++w) {
@@ -272,18 +275,18 @@ int run(int dtype, const RowsParams &R, bool write, cudaStream_t s) {
 
 } // namespace
 
-int cache_write(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s) { return run(rows.dtype, params(P, rows.dtype, rows.N, rows.x, rows.stride), true, s); }
+int cache_write(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s) { return run(rows.dtype, params(P, rows.dtype, rows.N, kWriteTokens, rows.x, rows.stride), true, s); }
 
 int cache_read(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s) {
     const int64_t dense[3] = {rows.N * P.H * P.D, P.H * P.D, P.D}, stride[2][3] = {{dense[0], dense[1], dense[2]}, {dense[0], dense[1], dense[2]}};
-    RowsParams R = params(P, rows.dtype, rows.N, rows.x, stride);
+    RowsParams R = params(P, rows.dtype, rows.N, kReadTokens, rows.x, stride);
     R.from_start = rows.from_start;
     return run(rows.dtype, R, false, s);
 }
 
 int cache_expand(const CacheParams &P, int dtype, void *const (&x)[2], const int64_t (&stride)[3], long long last, cudaStream_t s) {
     const int64_t both[2][3] = {{stride[0], stride[1], stride[2]}, {stride[0], stride[1], stride[2]}};
-    RowsParams R = params(P, dtype, P.capacity, x, both);
+    RowsParams R = params(P, dtype, P.capacity, kReadTokens, x, both);
     R.from_start = 1;
     R.leave = 1;
     R.last = (int)(last < P.capacity ? last : 0);
