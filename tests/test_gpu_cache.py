@@ -24,10 +24,10 @@ def check_stored(cache, k, v, group, where):
             c, s, z = (t[b, :, i:i + n] for t in want)
             gc, gs, gz = (t[b, :, at:at + n] for t in (code, step, zero))
             assert torch.equal(gs.nan_to_num(-1.0), s.nan_to_num(-1.0)) and torch.equal(gz.nan_to_num(-1e30), z.nan_to_num(-1e30))
-            # x - zero is rounded to 32 bits, 2^-24 of at most 255 steps: such a distance from a middle decides nothing
+            # 16-bit values: x - zero is rounded to 32 bits, 2^-24 of at most 255 steps: such a distance from a middle decides nothing
             x64 = x[b, i:i + n].transpose(0, 1).double()
             away = ((x64 - z) / s - torch.floor((x64 - z) / s) - 0.5).abs()
-            sure = (away > 255 * 2.0 ** -24) | ~torch.isfinite(s) | ((x64 - z).float().double() == x64 - z)
+            sure = (away > 255 * 2.0 ** -24) | ~torch.isfinite(s) | ((x64 - z).float().double() == x64 - z) | torch.tensor(x.dtype == torch.float32, device=x.device)
             assert torch.equal(gc[sure], c[sure]) and bool(((gc - c).abs() <= 1).all())
             fine = torch.isfinite(s)
             assert bool(((gz + gs * gc - x64).abs() <= gs / 2 * (1 + 2.0 ** -15))[fine].all())
@@ -83,6 +83,24 @@ def test_values_on_a_grid_middles_and_constants(bits, dtype):
         out = out[0, :, 0].cpu()
         assert torch.equal(out[[0, 1, 3, 4, 5]], rows[[0, 1, 3, 4, 5]])
         assert torch.equal(out[2], torch.cat((rows[2, :2], torch.round(rows[2, 2:]))))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_float32_values_beside_a_middle(bits):
+    """Values a unit of the last place to either side of middles between two codes, some of whose distances from the zero are no 32-bit numbers."""
+    most = 2 ** bits - 1
+    for zero, step in ((-3.75, 0.5), (-1.0, 2.0 ** -7 * 1.5), (-96.0, 0.75)):
+        middles = torch.tensor([zero + (c + 0.5) * step for c in range(min(most, 40))], dtype=torch.float64).float()
+        near = torch.stack((torch.nextafter(middles, torch.tensor(-math.inf)), middles, torch.nextafter(middles, torch.tensor(math.inf))), -1).flatten()[:60]
+        small = torch.tensor([1e-9, -1e-9])   # beside a middle at 0
+        x = torch.cat((torch.tensor([zero, zero + most * step]), small, near)).float()
+        x = torch.cat((x, x[:1].expand(64 - x.numel())))[None, None, None].cuda()
+        cache = tpw.quantized_cache(1, 64, 1, 64, bits=bits, group=None)
+        tpw.cache_write(cache, x, x, ints(1))
+        # (where 0 lies above the last code, as with 15 steps from -1, the step is another one, which the definition gives too)
+        want = [w[0, 0, 0] for w in quantised(x, bits, None)]
+        for got in unpacked(cache):
+            assert all(torch.equal(a[0, 0, 0], b) for a, b in zip(got, want))
 
 
 @pytest.mark.parametrize("bits", [4, 8])

@@ -167,7 +167,11 @@ __global__ void __launch_bounds__(kWriteTokens * (W == 2 ? 2 : 4)) cache_write_k
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const float d = __fsub_rn(x[v][k], zero), near = __fmul_rn(d, inv);
-            y[k] = __fadd_rn(fmaf(fmaf(-near, step, d), inv, near), 12582912.f);
+            const float quotient = fmaf(fmaf(-near, step, d), inv, near);
+            y[k] = __fadd_rn(quotient, 12582912.f);
+            // float32 values have digits that their distance from the zero has not: beside a middle, within four times what 255 can be off, 64 bits decide
+            if (sizeof(T) == 4 && fabsf(quotient - (y[k] - 12582912.f)) > 0.5f - 1.220703125e-4f)
+                y[k] = 12582912.f + (float)rint(((double)x[v][k] - (double)zero) / (double)step);
         }
         uint32_t code[2];
         pack8<BITS>(code, y, live && fine ? n - 8 * v : 0);
