@@ -44,9 +44,15 @@ struct CacheAttnParams {
 // cache_rows.cu
 int cache_write(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s);
 int cache_read(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s);
+// what cache_attention.cu does beside: the highest magnitudes of kRangeParts parts of every head, [2, B, H, kRangeParts]
+constexpr int kRangeParts = 16;
+int cache_ranges(const CacheParams &P, uint32_t *highest, cudaStream_t s);
 // every sequence's keys and values, those before the last `last` (0: none) and their block of 128 tokens left out, at [batch, token, head] strides of x;
-// what is not stored or left out is not written
-int cache_expand(const CacheParams &P, int dtype, void *const (&x)[2], const int64_t (&stride)[3], long long last, cudaStream_t s);
+// what is not stored or left out is not written.  With `highest` each head's are brought below 2^bring by a power of two.
+int cache_expand(const CacheParams &P, int dtype, void *const (&x)[2], const int64_t (&stride)[3], long long last, const uint32_t *highest, const int (&bring)[2], cudaStream_t s);
+// bfloat16 rows (strides of batch, token and head) to dense half precision ones and, `back`, the other way, times a head's highest power of two over 2^bring
+int cache_convert(bool back, const void *from, void *to, const int64_t (&stride)[3], const uint32_t *highest, int bring, long long B, long long N, long long Hq, long long H, long long D,
+                  cudaStream_t s);
 // cache_attention.cu; -1: refused
 long long cache_attention_bytes(const CacheAttnParams &P);
 int cache_attention(const CacheAttnParams &P, void *scratch, long long bytes, cudaStream_t s);

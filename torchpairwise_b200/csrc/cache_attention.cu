@@ -1,46 +1,67 @@
 // Attention over a cache of quantised keys and values: which kernels.
 //
 // Few query rows to a key head read the codes as they lie (cache_few.cuh).  Many make attention a matter of matrix products, and there each key tile is
-// read by many tiles of queries: keys and values are turned into the queries' type once, into scratch, and go through the kernels of
+// read by many tiles of queries: keys and values are turned into half precision once, into scratch, and go through the kernels of
 // attention.  Scratch is bounded: sequences go a few at a time, 128 MB of keys and values or one sequence, so that L2 holds most of what was just written.
+// Half precision also for bfloat16 queries: what codes stand for has more than bfloat16's 8 digits, and keys rounded to them made the results 2.4 times as
+// far off (chunk of 256 on 16384 keys: 0.0041 against 0.0017).  Its exponents do not reach, so each head's keys and values, and the queries and results
+// with them, are moved by a power of two.
 #include "cache.cuh"
 
 namespace tpw {
 namespace {
 
 constexpr long long kSlice = 128LL << 20;
+// half precision: a head's keys are brought below 2^8, its values below 2^14, so that their digits are normal numbers down to 2^-22 and 2^-28 of the
+// highest, and queries, multiplied by what their keys were divided by, overflow only where scores do
+constexpr int kKeys = 8, kValues = 14;
 
 int few(const CacheAttnParams &P, void *scratch, long long *bytes, cudaStream_t s) {
     return P.c.bits == 4 ? cache_few_4(P, scratch, bytes, s) : cache_few_8(P, scratch, bytes, s);
 }
 
+// Scratch of the many: keys and values of a slice; for bfloat16 also its heads' ranges, queries and results in half precision; then attention's own.
 struct Slices {
-    long long row, sequence, step;   // bytes of a token and head, of a sequence's keys (or values); sequences at a time
+    long long sequence, step, ranges, queries;   // bytes of a sequence's keys (or values); sequences at a time; bytes of the others
     explicit Slices(const CacheAttnParams &P) {
-        row = P.c.D * 2;
-        sequence = (P.c.capacity * P.c.H * row + 15) / 16 * 16;
+        auto round = [](long long bytes) { return (bytes + 255) / 256 * 256; };
+        sequence = round(P.c.capacity * P.c.H * P.c.D * 2);
         step = sequence > 0 ? kSlice / (2 * sequence) : P.c.B;
         step = step < 1 ? 1 : step < P.c.B ? step : P.c.B;
+        const bool wide = P.dtype == TPW_BF16;
+        ranges = wide ? round(step * P.c.H * 2 * kRangeParts * 4) : 0;
+        queries = wide ? round(step * P.Nq * P.Hq * P.c.D * 2) : 0;
     }
-    long long bytes() const { return 2 * sequence * step; }
+    long long bytes() const { return 2 * sequence * step + ranges + 2 * queries; }
+    unsigned char *values(void *scratch) const { return static_cast<unsigned char *>(scratch) + sequence * step; }
+    unsigned char *range(void *scratch) const { return static_cast<unsigned char *>(scratch) + 2 * sequence * step; }
+    unsigned char *query(void *scratch) const { return range(scratch) + ranges; }
+    unsigned char *result(void *scratch) const { return query(scratch) + queries; }
 };
 tpw_attention slice(const CacheAttnParams &P, const Slices &S, void *scratch, long long first, long long count) {
-    const long long e = 2;   // bytes of a number
     tpw_attention a = {};
-    a.dtype = P.dtype;
+    a.dtype = TPW_F16;
     a.causal = P.causal;
     a.window = P.window;
     a.B = count; a.Nq = P.Nq; a.Nk = P.c.capacity; a.Hq = P.Hq; a.Hk = P.c.H; a.D = P.c.D;
     a.scale = P.scale;
-    a.q = static_cast<const unsigned char *>(P.q) + first * P.q_s[0] * e;
     a.k = scratch;
-    a.v = static_cast<unsigned char *>(scratch) + S.sequence * S.step;
-    for (int i = 0; i < 3; ++i) a.q_stride[i] = P.q_s[i];
-    a.k_stride[0] = a.v_stride[0] = S.sequence / e;
+    a.v = S.values(scratch);
+    if (P.dtype == TPW_F16) {
+        a.q = static_cast<const unsigned char *>(P.q) + first * P.q_s[0] * 2;
+        for (int i = 0; i < 3; ++i) a.q_stride[i] = P.q_s[i];
+        a.out = static_cast<unsigned char *>(P.out) + first * P.Nq * P.Hq * P.c.D * 2;
+    } else {
+        a.q = S.query(scratch);
+        a.q_stride[0] = P.Nq * P.Hq * P.c.D;
+        a.q_stride[1] = P.Hq * P.c.D;
+        a.q_stride[2] = P.c.D;
+        a.out = S.result(scratch);
+    }
+    a.k_stride[0] = a.v_stride[0] = S.sequence / 2;
     a.k_stride[1] = a.v_stride[1] = P.c.D;
     a.k_stride[2] = a.v_stride[2] = P.c.capacity * P.c.D;
     a.key_lengths = P.c.lengths + first;
-    a.out = static_cast<unsigned char *>(P.out) + first * P.Nq * P.Hq * S.row;
     a.lse = P.lse ? P.lse + first * P.Hq * P.Nq : nullptr;
     return a;
 }
@@ -50,8 +71,8 @@ tpw_attention slice(const CacheAttnParams &P, const Slices &S, void *scratch, lo
 bool is_few(const CacheAttnParams &P) {
     if (P.dtype == TPW_F32 || P.group * P.Nq <= 192) return true;
     const tpw_attention a = slice(P, Slices(P), reinterpret_cast<void *>(256), 0, 1);   // of the scratch only its alignment takes part
-    const AttnParams A = attn_params(a);
-    return !attn_tc_fits(a.dtype, A);   // attention's own kernels for odd widths are slower still
+    const bool pieces = aligned16(P.q) && aligned16(P.out) && P.q_s[0] % 8 == 0 && P.q_s[1] % 8 == 0 && P.q_s[2] % 8 == 0;
+    return !pieces || !attn_tc_fits(a.dtype, attn_params(a));   // attention's own kernels for odd widths are slower still
 }
 
 } // namespace
@@ -78,9 +99,18 @@ int cache_attention(const CacheAttnParams &P, void *scratch, long long bytes, cu
             c.codes[w] += first * c.H * c.capacity * c.row_bytes;
             c.scales[w] += first * c.H * c.capacity * c.groups;
         }
-        int e = TPW_OK;
-        if (c.capacity > 0) e = cache_expand(c, P.dtype, {const_cast<void *>(a.k), const_cast<void *>(a.v)}, a.k_stride, P.window > 0 ? P.Nq - 1 + P.window : 0, s);
+        const bool wide = P.dtype == TPW_BF16;
+        uint32_t *highest = wide ? reinterpret_cast<uint32_t *>(S.range(scratch)) : nullptr;
+        int e = wide ? cache_ranges(c, highest, s) : TPW_OK;
+        if (e == TPW_OK) e = cache_expand(c, TPW_F16, {const_cast<void *>(a.k), const_cast<void *>(a.v)}, a.k_stride, P.window > 0 ? P.Nq - 1 + P.window : 0, highest, {kKeys, kValues}, s);
+        if (e == TPW_OK && wide) {
+            const int64_t stride[3] = {P.q_s[0], P.q_s[1], P.q_s[2]};
+            e = cache_convert(false, static_cast<const unsigned char *>(P.q) + first * P.q_s[0] * 2, const_cast<void *>(a.q), stride, highest, kKeys, count, P.Nq, P.Hq, P.c.H, P.c.D, s);
+        }
         if (e == TPW_OK) e = tpw_attention_forward(&a, static_cast<unsigned char *>(scratch) + S.bytes(), bytes - S.bytes(), s);
+        if (e == TPW_OK && wide)
+            e = cache_convert(true, a.out, static_cast<unsigned char *>(P.out) + first * P.Nq * P.Hq * P.c.D * 2, a.q_stride, highest + count * c.H * kRangeParts, kValues, count, P.Nq, P.Hq, P.c.H,
+                              P.c.D, s);
         if (e != TPW_OK) return e;
     }
     return TPW_OK;

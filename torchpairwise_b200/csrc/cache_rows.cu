@@ -16,6 +16,8 @@ struct RowsParams {
     int from_start, vector;    // vector: 16-byte pieces of a row
     int leave;                 // read: rows that are not stored are left as they were
     int last;                  // read: and those before the last so many and their block of 128; 0: none are
+    const uint32_t *highest;   // read: what cache_ranges found, or NULL; values are then brought below 2^bring[0] (keys), 2^bring[1]
+    int bring[2];
 };
 
 // NaN if an operand is
@@ -70,6 +72,66 @@ template <typename T> __device__ __forceinline__ void store8(T *p, const float (
         for (int k = 0; k < 8; ++k)
             if (k < n) p[k] = (T)x[k];
     }
+}
+
+// Many bfloat16 queries go through half precision, which has the digits but not the exponents (cache_attention.cu): each head's keys and values
+// are brought near a power of two.  `parts` has the highest magnitudes, as bits, of parts of a head; the factor is a power of two.
+__device__ __forceinline__ int exponent_of(const uint32_t *parts) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < kRangeParts; ++k) top = max(top, parts[k]);
+    return top == 0 ? 0 : (int)(top >> 23) - 126;   // the magnitudes are below 2 to this
+}
+__device__ __forceinline__ float bring_by(const uint32_t *parts, int to) {
+    const int e = to - exponent_of(parts) + 127;
+    return __uint_as_float((uint32_t)(e < 1 ? 1 : e > 254 ? 254 : e) << 23);
+}
+// the highest magnitude that the codes of a part of a head's keys (or values) can stand for; groups that are not numbers take no part
+__global__ void __launch_bounds__(256) cache_ranges_kernel(const CacheParams P, uint32_t *highest) {
+    const long long bh = blockIdx.y;
+    const int which = blockIdx.z, b = (int)(bh / P.H), cap = (int)P.capacity;
+    int n = P.lengths[b];
+    n = n < 0 ? 0 : n < cap ? n : cap;
+    const uint32_t *scales = P.scales[which] + bh * cap * P.groups;
+    const float most = P.bits == 4 ? 15.f : 255.f;
+    uint32_t top = 0;
+    for (int at = blockIdx.x * 256 + threadIdx.x; at < n * P.groups; at += kRangeParts * 256) {
+        const float zero = zero_of(scales[at]), end = fmaf(step_of(scales[at]), most, zero), high = fmaxf(fabsf(zero), fabsf(end));
+        if (fabsf(zero) <= high && high < 5.0706024009129176e30f) top = max(top, __float_as_uint(high));   // 2^102
+    }
+    __shared__ uint32_t tops[8];
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int w = 1; w < 8; ++w) top = max(top, tops[w]);
+        highest[(which * P.B * P.H + bh) * kRangeParts + blockIdx.x] = top;
+    }
+}
+// Rows of queries to half precision, times what their keys were divided by; rows of results back.  A thread has 8 features, a block 256 times that.
+struct ConvertParams {
+    const void *from;
+    void *to;
+    long long stride[3], pieces;   // of `from`; pieces of 8 features
+    const uint32_t *highest;
+    Divider by_d, by_heads, by_tokens, by_group;
+    int H;                         // key heads
+    int bring;
+};
+template <typename A, typename B> __global__ void __launch_bounds__(256) cache_convert_kernel(const ConvertParams C) {
+    const unsigned at = blockIdx.x * 256 + threadIdx.x;
+    if (at >= C.pieces) return;
+    const unsigned row = at / C.by_d, d = at - row * C.by_d.d, token = row / C.by_heads, h = row - token * C.by_heads.d, b = token / C.by_tokens, i = token - b * C.by_tokens.d;
+    const uint32_t *parts = C.highest + (b * C.H + h / C.by_group) * kRangeParts;
+    const int e = exponent_of(parts) - C.bring + 127;
+    const float by = __uint_as_float((uint32_t)(e < 1 ? 1 : e > 254 ? 254 : e) << 23);
+    const uint4 w = *reinterpret_cast<const uint4 *>(static_cast<const A *>(C.from) + b * C.stride[0] + i * C.stride[1] + h * C.stride[2] + 8 * d);
+    const A *v = reinterpret_cast<const A *>(&w);
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = (float)v[k] * by;
+    reinterpret_cast<uint4 *>(C.to)[at] = make_uint4(Narrow<B>::pack(x[0], x[1]), Narrow<B>::pack(x[2], x[3]), Narrow<B>::pack(x[4], x[5]), Narrow<B>::pack(x[6], x[7]));
 }
 
 // What a block works on: TOKENS tokens of a head, this thread's first being i0; token i stands at position i + shift, and positions [0, end) have a place.
@@ -222,10 +284,11 @@ __global__ void __launch_bounds__(kReadSide * 4 * W) cache_read_kernel(const Row
     }
     T *to = static_cast<T *>(R.x[which]) + B.b * R.stride[which][0] + B.i0 * R.stride[which][1] + B.h * R.stride[which][2] + 8 * l;
     const long long further = kReadSide * R.stride[which][1];
+    const float by = R.highest ? bring_by(R.highest + (which * R.c.B * R.c.H + B.b * R.c.H + B.h) * kRangeParts, R.bring[which]) : 1.f;
 #pragma unroll
     for (int u = 0; u < PASSES; ++u, to += further) {
         if (R.leave ? !there[u] : B.i0 + u * kReadSide >= R.N) continue;
-        const float step = step_of(scales[u]), zero = zero_of(scales[u]);
+        const float step = step_of(scales[u]) * by, zero = zero_of(scales[u]) * by;
         const uint32_t even = w[u][0] & 0x0f0f0f0fu, odd = (w[u][0] >> 4) & 0x0f0f0f0fu;
         float x[8];
 #pragma unroll
@@ -288,13 +351,44 @@ int cache_read(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s)
     return run(rows.dtype, R, false, s);
 }
 
-int cache_expand(const CacheParams &P, int dtype, void *const (&x)[2], const int64_t (&stride)[3], long long last, cudaStream_t s) {
+int cache_ranges(const CacheParams &P, uint32_t *highest, cudaStream_t s) {
+    TPW_CHECK_ARG(P.B * P.H < 65536, "tpw_cache_attention: more than 65535 heads of a slice");
+    cache_ranges_kernel<<<dim3(kRangeParts, (unsigned)(P.B * P.H), 2), 256, 0, s>>>(P, highest);
+    TPW_LAUNCH_OK("cache_ranges_kernel");
+    return TPW_OK;
+}
+
+int cache_expand(const CacheParams &P, int dtype, void *const (&x)[2], const int64_t (&stride)[3], long long last, const uint32_t *highest, const int (&bring)[2], cudaStream_t s) {
     const int64_t both[2][3] = {{stride[0], stride[1], stride[2]}, {stride[0], stride[1], stride[2]}};
     RowsParams R = params(P, dtype, P.capacity, kReadTokens, x, both);
     R.from_start = 1;
     R.leave = 1;
     R.last = (int)(last < P.capacity ? last : 0);
+    R.highest = highest;
+    for (int w = 0; w < 2; ++w) R.bring[w] = bring[w];
     return run(dtype, R, false, s);
+}
+
+int cache_convert(bool back, const void *from, void *to, const int64_t (&stride)[3], const uint32_t *highest, int bring, long long B, long long N, long long Hq, long long H, long long D,
+                  cudaStream_t s) {
+    ConvertParams C = {};
+    C.from = from;
+    C.to = to;
+    for (int k = 0; k < 3; ++k) C.stride[k] = stride[k];
+    C.pieces = B * N * Hq * (D / 8);
+    C.highest = highest;
+    C.by_d = divider(D / 8);
+    C.by_heads = divider(Hq);
+    C.by_tokens = divider(N);
+    C.by_group = divider(Hq / H);
+    C.H = (int)H;
+    C.bring = bring;
+    const long long blocks = (C.pieces + 255) / 256;
+    TPW_CHECK_ARG(C.pieces < (1LL << 31), "tpw_cache_attention: more than 2^34 numbers of queries of a slice");
+    if (back) cache_convert_kernel<__half, __nv_bfloat16><<<(unsigned)blocks, 256, 0, s>>>(C);
+    else cache_convert_kernel<__nv_bfloat16, __half><<<(unsigned)blocks, 256, 0, s>>>(C);
+    TPW_LAUNCH_OK("cache_convert_kernel");
+    return TPW_OK;
 }
 
 } // namespace tpw
