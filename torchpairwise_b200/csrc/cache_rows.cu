@@ -5,7 +5,7 @@
 namespace tpw {
 namespace {
 
-constexpr int kWriteTokens = 32, kReadTokens = 64, kReadSide = 16;   // of a block; read: side by side, the others in further passes
+constexpr int kWriteTokens = 32, kReadTokens = 64;   // of a block
 
 struct RowsParams {
     CacheParams c;
@@ -252,52 +252,64 @@ __global__ void __launch_bounds__(kWriteTokens * (W == 2 ? 2 : 4)) cache_write_k
     if (R.c.groups > 1 ? w < R.c.groups : w == 0) R.c.scales[which][place * R.c.groups + w] = fine ? __float_as_uint(step) >> 16 | zero_bits : 0x7fc07fc0u;
 }
 
+// A lane has what lies together in a row: features 8 l to 8 l + 7 of every group of 32, l < 4, which leave as pieces of 16 bytes, 64 side by side.
 template <typename T, int BITS, int W>
-__global__ void __launch_bounds__(kReadSide * 4 * W) cache_read_kernel(const RowsParams R) {
-    constexpr int LANES = 4 * W, PASSES = kReadTokens / kReadSide, ROW = W * 4 * BITS;
-    const int which = blockIdx.y, l = threadIdx.x % LANES, n = R.c.D - 8 * l;
-    if (n <= 0) return;
-    const Block<kReadTokens> B(R, threadIdx.x / LANES);
+__global__ void __launch_bounds__(4 * kReadTokens) cache_read_kernel(const RowsParams R) {
+    constexpr int WORDS = W * BITS / 4;
+    const int which = blockIdx.y, l = threadIdx.x & 3;
+    const Block<kReadTokens> B(R, threadIdx.x >> 2);
     const int first = R.last > 0 && B.end > R.last ? (B.end - R.last) & ~127 : 0;   // positions before it are left
-    const long long place = B.row0 + B.i0 + B.shift;
-    const unsigned char *from = R.c.codes[which] + place * ROW;
-    const uint32_t *from_scales = R.c.scales[which] + place * R.c.groups + (R.c.groups > 1 ? l >> 2 : 0);
-    uint32_t w[PASSES][2], scales[PASSES];
-    bool there[PASSES];
+    const bool there = B.i0 < R.N && B.stored(B.i0) && B.i0 + B.shift >= first;
+    if (R.leave ? !there : B.i0 >= R.N) return;
+    uint32_t w[WORDS] = {}, scales[W] = {};
+    if (there) {
+        const long long place = B.row0 + B.i0 + B.shift;
+        const unsigned char *row = R.c.codes[which] + place * (W * 4 * BITS) + l * (W * BITS);
+        if constexpr (WORDS % 4 == 0) {
 #pragma unroll
-    for (int u = 0; u < PASSES; ++u) {
-        const int i = B.i0 + u * kReadSide;
-        w[u][0] = w[u][1] = scales[u] = 0;
-        there[u] = i < R.N && B.stored(i) && i + B.shift >= first;
-        if (!there[u]) continue;
-        const unsigned char *row = from + u * kReadSide * ROW;
-        if (which == 0) {
-            w[u][0] = __ldcs(reinterpret_cast<const uint32_t *>(row + key_place<BITS, W>(l)));
-            if (BITS == 8) w[u][1] = __ldcs(reinterpret_cast<const uint32_t *>(row + key_place<BITS, W>(l) + 4));
-        } else if (BITS == 4) {
-            w[u][0] = __ldcs(reinterpret_cast<const uint16_t *>(row + value_place<BITS, W>(l, 0))) | (uint32_t)__ldcs(reinterpret_cast<const uint16_t *>(row + value_place<BITS, W>(l, 1))) << 16;
+            for (int k = 0; k < WORDS / 4; ++k) {
+                const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(row) + k);
+                w[4 * k] = v.x; w[4 * k + 1] = v.y; w[4 * k + 2] = v.z; w[4 * k + 3] = v.w;
+            }
+        } else if constexpr (WORDS % 2 == 0) {
+#pragma unroll
+            for (int k = 0; k < WORDS / 2; ++k) {
+                const uint2 v = __ldcs(reinterpret_cast<const uint2 *>(row) + k);
+                w[2 * k] = v.x; w[2 * k + 1] = v.y;
+            }
         } else {
-            w[u][0] = __ldcs(reinterpret_cast<const uint32_t *>(row + value_place<BITS, W>(l, 0)));
-            w[u][1] = __ldcs(reinterpret_cast<const uint32_t *>(row + value_place<BITS, W>(l, 1)));
-        }
-        scales[u] = from_scales[u * kReadSide * R.c.groups];
-    }
-    T *to = static_cast<T *>(R.x[which]) + B.b * R.stride[which][0] + B.i0 * R.stride[which][1] + B.h * R.stride[which][2] + 8 * l;
-    const long long further = kReadSide * R.stride[which][1];
-    const float by = R.highest ? bring_by(R.highest + (which * R.c.B * R.c.H + B.b * R.c.H + B.h) * kRangeParts, R.bring[which]) : 1.f;
 #pragma unroll
-    for (int u = 0; u < PASSES; ++u, to += further) {
-        if (R.leave ? !there[u] : B.i0 + u * kReadSide >= R.N) continue;
-        const float step = step_of(scales[u]) * by, zero = zero_of(scales[u]) * by;
-        const uint32_t even = w[u][0] & 0x0f0f0f0fu, odd = (w[u][0] >> 4) & 0x0f0f0f0fu;
+            for (int k = 0; k < WORDS; ++k) w[k] = __ldcs(reinterpret_cast<const uint32_t *>(row) + k);
+        }
+        const uint32_t *of = R.c.scales[which] + place * R.c.groups;
+#pragma unroll
+        for (int k = 0; k < W; ++k) scales[k] = R.c.groups == 1 ? of[0] : k < R.c.groups ? of[k] : 0u;
+    }
+    const float by = R.highest ? bring_by(R.highest + (which * R.c.B * R.c.H + B.b * R.c.H + B.h) * kRangeParts, R.bring[which]) : 1.f;
+    T *to = static_cast<T *>(R.x[which]) + B.b * R.stride[which][0] + B.i0 * R.stride[which][1] + B.h * R.stride[which][2] + 8 * l;
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+        const int n = R.c.D - 32 * k - 8 * l;
+        if (n <= 0) break;
+        // the 8 codes: a key's lie together, a value's in two runs of 4
+        uint32_t c[2];
+        if constexpr (BITS == 4) {
+            const uint32_t word = which == 0 ? w[k] : __byte_perm(w[k / 2], w[(W + k) / 2], (k % 2 ? 0x32 : 0x10) | ((W + k) % 2 ? 0x7600 : 0x5400));
+            c[0] = word & 0x0f0f0f0fu;
+            c[1] = (word >> 4) & 0x0f0f0f0fu;
+        } else {
+            c[0] = which == 0 ? w[2 * k] : w[k];
+            c[1] = which == 0 ? w[2 * k + 1] : w[W + k];
+        }
+        const float step = step_of(scales[k]) * by, zero = zero_of(scales[k]) * by;
         float x[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int e = 0; e < 8; ++e) {
             // a byte to a code, then 2^23 + code less 2^23: the conversion instruction is a quarter as fast
-            const uint32_t c = __byte_perm(BITS == 8 ? w[u][k >> 2] : k & 1 ? odd : even, 0x4b000000u, 0x7440 + (BITS == 8 ? k & 3 : k >> 1));
-            x[k] = fmaf(__uint_as_float(c) - 8388608.f, step, zero);
+            const uint32_t byte = BITS == 4 ? __byte_perm(c[e & 1], 0x4b000000u, 0x7440 + (e >> 1)) : __byte_perm(c[e >> 2], 0x4b000000u, 0x7440 + (e & 3));
+            x[e] = fmaf(__uint_as_float(byte) - 8388608.f, step, zero);
         }
-        store8(to, x, n, R.vector, R.leave);
+        store8(to + 32 * k, x, n, R.vector, R.leave);
     }
 }
 
@@ -308,7 +320,7 @@ template <typename T, int BITS, int W> int launch(const RowsParams &R, bool writ
         cache_write_kernel<T, BITS, W><<<dim3((unsigned)blocks, 2), kWriteTokens * (W == 2 ? 2 : 4), 0, s>>>(R);
         TPW_LAUNCH_OK("cache_write_kernel");
     } else {
-        cache_read_kernel<T, BITS, W><<<dim3((unsigned)blocks, 2), kReadSide * 4 * W, 0, s>>>(R);
+        cache_read_kernel<T, BITS, W><<<dim3((unsigned)blocks, 2), 4 * kReadTokens, 0, s>>>(R);
         TPW_LAUNCH_OK("cache_read_kernel");
     }
     return TPW_OK;
