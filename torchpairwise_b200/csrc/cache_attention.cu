@@ -81,9 +81,15 @@ long long cache_attention_bytes(const CacheAttnParams &P) {
     long long bytes = -1;
     if (is_few(P)) return few(P, nullptr, &bytes, nullptr), bytes;
     const Slices S(P);
-    const tpw_attention a = slice(P, S, reinterpret_cast<void *>(256), 0, S.step);
-    bytes = tpw_attention_scratch_bytes(&a);
-    return bytes < 0 ? bytes : S.bytes() + bytes;
+    // the last slice has fewer sequences, for which attention may cut the keys into more ranges
+    for (const long long count : {S.step, P.c.B % S.step}) {
+        if (count == 0) continue;
+        const tpw_attention a = slice(P, S, reinterpret_cast<void *>(256), 0, count);
+        const long long more = tpw_attention_scratch_bytes(&a);
+        if (more < 0) return more;
+        if (S.bytes() + more > bytes) bytes = S.bytes() + more;
+    }
+    return bytes;
 }
 
 int cache_attention(const CacheAttnParams &P, void *scratch, long long bytes, cudaStream_t s) {

@@ -192,6 +192,14 @@ template <int KEYS> struct Stages {
         begin = first & ~63;
         count = end > first ? (end - begin + KEYS - 1) / KEYS : 0;
     }
+    // of those, the keys that a block of rows sees: the stages stay, others are neither fetched nor looked at
+    __device__ __forceinline__ void narrow(const CacheFewParams &F, int b, int row0, int rows) {
+        const int nq = (int)F.a.Nq, last = (row0 + rows < F.rows ? row0 + rows : F.rows) - 1, i0 = row0 - (int)((unsigned)row0 / F.by_nq) * nq, i1 = i0 + last - row0;
+        if (i1 >= nq) return;   // rows of two heads
+        const CacheSeen see(F.a, b);
+        first = see.lo(i0);
+        end = see.hi(i1);
+    }
 };
 // The line of all stages: sequences one after the other, a sequence's items (heads, and blocks of rows of each) one after the other, an item's
 // stages in order.  An item with stages stands on the line for kFewExtra more, which come first: what beginning and ending it costs.
@@ -305,17 +313,20 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
 
     // A warp brings its own keys of every stage, as many stages ahead as its ring has room for: a lane each for the codes and scales of keys and values.
     // It waits for no other warp.
-    int ahead_b = b, ahead_item = item, ahead_left = 0, ahead_key = 0, ahead_end = 0, issued = 0;
+    int ahead_b = b, ahead_item = item, ahead_left = 0, ahead_key = 0, ahead_first = 0, ahead_end = 0, issued = 0;
     uint32_t issued_slot = 0, slot = 0, phase = 0;   // of the next stage to be issued; of the next to be used
     const uint32_t copy_bytes = lane & 2 ? NG * 4 : L::ROW, copy_to = smem_u32(ring) + (lane & 2 ? 2 * L::CODES + (lane & 1) * L::SCALES : (lane & 1) * L::CODES);
     const unsigned char *copy_base = lane & 2 ? reinterpret_cast<const unsigned char *>(P.c.scales[lane & 1]) : P.c.codes[lane & 1], *copy_from = nullptr;
     bool ok = true;
     auto ahead_of = [&](int skip) {   // the next item's stages but for the first `skip`
-        const Stages<KEYS> S(P, ahead_b);
+        const int head = (int)((unsigned)ahead_item / F.by_blocks);
+        Stages<KEYS> S(P, ahead_b);
         ahead_left = S.count - skip;
         ahead_key = S.begin + skip * KEYS + warp * L::OWN;
+        S.narrow(F, ahead_b, (ahead_item - head * F.row_blocks) * ROWS, ROWS);
+        ahead_first = S.first;
         ahead_end = S.end;
-        copy_from = copy_base + (((long long)ahead_b * P.c.H + (unsigned)ahead_item / F.by_blocks) * P.c.capacity + ahead_key) * copy_bytes;
+        copy_from = copy_base + (((long long)ahead_b * P.c.H + head) * P.c.capacity + ahead_key) * copy_bytes;
     };
     auto fill = [&](int limit) {
         limit = limit < total ? limit : total;
@@ -323,7 +334,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
             const uint32_t st = issued_slot;
             issued_slot = issued_slot + 1 == L::kStages ? 0 : issued_slot + 1;
             // the capacity is a multiple of 64, so there are all of the warp's keys or none
-            const bool some = ahead_key < ahead_end;
+            const bool some = ahead_key < ahead_end && ahead_key + L::OWN > ahead_first;
             if (lane == 0) {
                 if (some) mbar_expect_tx(&full[st], L::PIECE);
                 else mbar_arrive(&full[st]);
@@ -358,9 +369,10 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
     int used = 0;
 
     do {
-        const Stages<KEYS> S(P, b);
+        Stages<KEYS> S(P, b);
         const CacheSeen see(P, b);
         const int hk = (unsigned)item / F.by_blocks, row0 = (item - hk * F.row_blocks) * ROWS, stage0 = stage;
+        S.narrow(F, b, row0, ROWS);
         const int stages = S.count - stage < total - used ? S.count - stage : total - used;
         // Queries as operands, a warp making those of every fourth block of 32 features: row g of a block, features 32 w + 8 t + (0 .. 7), in the order
         // in which masks leave the codes of a key.  Row r is query r % nq of head hk * group + r / nq.
