@@ -16,7 +16,7 @@
 // All stages of keys (64 or 128) of all sequences and heads form one line that the CTAs, three on an SM, take equal shares of, whatever the lengths: a
 // share ends and begins anywhere in a sequence.  What a CTA has of a head that others have parts of goes to scratch, and a second kernel, whose launch
 // overlaps this one, weighs the parts together in their order.  In a CTA four warps take 16 keys or 32 of a stage each, with a running reference, sum and
-// output of their own, and a ring of their own that they fill by bulk copies, across the ends of heads.
+// output of their own; bulk copies bring the stages into a ring, across the ends of heads.
 #pragma once
 #include "attention_tc.cuh"
 #include "cache.cuh"
@@ -40,15 +40,15 @@ struct CacheFewParams {
 
 template <int BITS, int W, int NG, int NT, int PARTS> struct CacheFew {
     static constexpr int KEYS = BITS == 4 ? 128 : 64, OWN = KEYS / kFewWarps, SUB = OWN / 16;   // of a stage; a warp's of them, and blocks of 16
-    static constexpr uint32_t ROW = W * 4 * BITS, CODES = OWN * ROW, SCALES = OWN * NG * 4, PIECE = 2 * (CODES + SCALES), DP = 32 * W, ROWS = 8 * NT;
+    static constexpr uint32_t ROW = W * 4 * BITS, CODES = KEYS * ROW, SCALES = KEYS * NG * 4, STAGE = 2 * (CODES + SCALES), DP = 32 * W, ROWS = 8 * NT;
     static constexpr int PER_SM = NT == 1 ? 3 : 2;
     static constexpr uint32_t STATS = kFewWarps * 8 * 8, PREPARED = PARTS == 1 ? kFewWarps * SUB * NG * 64 : 0, QUERIES = PARTS * NT * W * 512, SUMS = NT * (W + 1) * 32;
     static constexpr uint32_t ROOM = (NT == 1 ? 75776 : 112640) - STATS - PREPARED - QUERIES - SUMS - 320;
-    static constexpr int kStages = ROOM / (kFewWarps * PIECE) < 8 ? ROOM / (kFewWarps * PIECE) : 8;
+    static constexpr int kStages = ROOM / STAGE < 8 ? ROOM / STAGE : 8;
     static_assert(kStages >= 2, "a ring of two stages at least");
-    static_assert(8 * DP * 4 <= PIECE, "a warp's 8 rows of results fit its piece of a stage");
-    static constexpr uint32_t RING = kStages * PIECE, OFF_STATS = kFewWarps * RING, OFF_PREPARED = OFF_STATS + STATS, OFF_QUERIES = OFF_PREPARED + PREPARED, OFF_SUMS = OFF_QUERIES + QUERIES,
-                              OFF_BAR = OFF_SUMS + SUMS, OFF_FLAG = OFF_BAR + 8 * kFewWarps * kStages, ALLOC = OFF_FLAG + 16;
+    static_assert(kFewWarps * 8 * DP * 4 <= STAGE, "the warps' 8 rows of results fit a stage");
+    static constexpr uint32_t OFF_STATS = kStages * STAGE, OFF_PREPARED = OFF_STATS + STATS, OFF_QUERIES = OFF_PREPARED + PREPARED, OFF_SUMS = OFF_QUERIES + QUERIES,
+                              OFF_BAR = OFF_SUMS + SUMS, OFF_FLAG = OFF_BAR + 16 * kStages, ALLOC = OFF_FLAG + 16;
 };
 
 // D += A B, and D = C + A B where C stays
@@ -266,12 +266,11 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_FLAG);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int nq = (int)P.Nq, items = (int)P.c.H * F.row_blocks;
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR) + warp * L::kStages;
-    unsigned char *ring = smem + warp * L::RING;
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *empty = full + L::kStages;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kFewWarps * L::kStages; ++i) mbar_init(&full[i], 1);
+        for (int i = 0; i < L::kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], kFewWarps); }
         *abort_flag = 0;
         mbar_init_fence();
     }
@@ -311,18 +310,17 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
         if (P.status) atomicCAS(P.status, 0, (23 << 16) | site);
     };
 
-    // A warp brings its own keys of every stage, as many stages ahead as its ring has room for: a lane each for the codes and scales of keys and values.
-    // It waits for no other warp.
+    // Warp 0 also issues the copies, as many stages ahead as the ring has room for: a lane each for the codes and scales of keys and values.
     int ahead_b = b, ahead_item = item, ahead_left = 0, ahead_key = 0, ahead_first = 0, ahead_end = 0, issued = 0;
-    uint32_t issued_slot = 0, slot = 0, phase = 0;   // of the next stage to be issued; of the next to be used
-    const uint32_t copy_bytes = lane & 2 ? NG * 4 : L::ROW, copy_to = smem_u32(ring) + (lane & 2 ? 2 * L::CODES + (lane & 1) * L::SCALES : (lane & 1) * L::CODES);
+    uint32_t issued_slot = 0, issued_phase = 1, slot = 0, phase = 0;   // of the next stage to be issued; of the next to be used
+    const uint32_t copy_bytes = lane & 2 ? NG * 4 : L::ROW, copy_to = smem_u32(smem) + (lane & 2 ? 2 * L::CODES + (lane & 1) * L::SCALES : (lane & 1) * L::CODES);
     const unsigned char *copy_base = lane & 2 ? reinterpret_cast<const unsigned char *>(P.c.scales[lane & 1]) : P.c.codes[lane & 1], *copy_from = nullptr;
     bool ok = true;
     auto ahead_of = [&](int skip) {   // the next item's stages but for the first `skip`
         const int head = (int)((unsigned)ahead_item / F.by_blocks);
         Stages<KEYS> S(P, ahead_b);
         ahead_left = S.count - skip;
-        ahead_key = S.begin + skip * KEYS + warp * L::OWN;
+        ahead_key = S.begin + skip * KEYS;
         S.narrow(F, ahead_b, (ahead_item - head * F.row_blocks) * ROWS, ROWS);
         ahead_first = S.first;
         ahead_end = S.end;
@@ -332,15 +330,23 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
         limit = limit < total ? limit : total;
         while (issued < limit && ok) {
             const uint32_t st = issued_slot;
-            issued_slot = issued_slot + 1 == L::kStages ? 0 : issued_slot + 1;
-            // the capacity is a multiple of 64, so there are all of the warp's keys or none
-            const bool some = ahead_key < ahead_end && ahead_key + L::OWN > ahead_first;
+            if (issued >= L::kStages && !(ok = __all_sync(0xffffffffu, wait_or_abort(&empty[st], issued_phase, abort_flag)))) {
+                give_up(1);
+                return;
+            }
+            if (++issued_slot == L::kStages) {
+                issued_slot = 0;
+                issued_phase ^= 1;
+            }
+            // the capacity and a stage's first key are multiples of 64
+            const bool some = ahead_key < ahead_end && ahead_key + KEYS > ahead_first;
+            const uint32_t n = (uint32_t)((int)P.c.capacity - ahead_key < KEYS ? (int)P.c.capacity - ahead_key : KEYS);
             if (lane == 0) {
-                if (some) mbar_expect_tx(&full[st], L::PIECE);
+                if (some) mbar_expect_tx(&full[st], n * 2 * (L::ROW + NG * 4));
                 else mbar_arrive(&full[st]);
             }
             __syncwarp();
-            if (some && lane < 4) bulk_load(copy_to + st * L::PIECE, copy_from, L::OWN * copy_bytes, &full[st]);
+            if (some && lane < 4) bulk_load(copy_to + st * L::STAGE, copy_from, n * copy_bytes, &full[st]);
             ++issued;
             ahead_key += KEYS;
             copy_from += KEYS * copy_bytes;
@@ -355,7 +361,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
         }
     };
     // one stage for now: the queries are not to wait behind what all CTAs ask for
-    if (total > 0) {
+    if (warp == 0 && total > 0) {
         ahead_of(stage);
         fill(1);
     }
@@ -427,7 +433,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
             }
         }
         __syncthreads();
-        if (used == 0) fill(L::kStages);
+        if (warp == 0 && used == 0) fill(L::kStages);
         uint32_t q[PARTS][NT][W][2][2], qz[NT][PARTS][2];
         float start[NT][NG][4], factor[NT][2];   // -M a_g (WIDE); raw scores times the factor are powers of 2
         int all_lo = S.first, all_hi = S.end;   // keys that all rows see
@@ -500,7 +506,8 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
             }
             const int j0 = S.begin + (stage0 + u) * KEYS + L::OWN * warp;
             if (ok && j0 < S.end && j0 + 16 * SUB > S.first) {
-                const unsigned char *k_at = ring + st * L::PIECE, *v_at = k_at + L::CODES, *ks_at = v_at + L::CODES, *vs_at = ks_at + L::SCALES;
+                const unsigned char *k_at = smem + st * L::STAGE + L::OWN * warp * L::ROW, *v_at = k_at + L::CODES;
+                const unsigned char *ks_at = smem + st * L::STAGE + 2 * L::CODES + L::OWN * warp * NG * 4, *vs_at = ks_at + L::SCALES;
                 float p[SUB][NT][4];
 #pragma unroll
                 for (int h = 0; h < SUB; ++h) {
@@ -745,13 +752,15 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                 }
             }
             __syncwarp();
-            // the last stage's room is where the warps' outputs meet: it is filled anew after that
-            if (u + 1 < stages) fill(used + 1 + L::kStages);
+            if (lane == 0) mbar_arrive(&empty[st]);
+            // A stage late, so that the other warps are done with what is filled anew.  The last stage's room is where the warps' outputs meet: it is
+            // filled after that.
+            if (warp == 0 && u + 1 < stages) fill(used + L::kStages);
         }
         // The warps' outputs meet, 8 rows at a time, each in the room of its last stage beside references and sums.  A thread weighs four features of a
         // row together.
-        const uint32_t share_at = st * L::PIECE;
-        float *share = reinterpret_cast<float *>(ring + share_at);
+        const uint32_t share_at = st * L::STAGE;
+        float *share = reinterpret_cast<float *>(smem + share_at + warp * 8 * DP * 4);
         const int power = top_scale + 1 - 127;
         // two factors: either's exponent stays within 32 bits' range
         const float unit = power_of_two(127 + power / 2), unit2 = power_of_two(127 + power - power / 2);
@@ -760,7 +769,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
         const long long part = ((long long)blockIdx.x * 2 + (stage0 == 0 ? 1 : 0)) * ROWS;
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
-            if (x > 0) __syncthreads();
+            __syncthreads();
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
@@ -802,7 +811,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                 for (int w = 0; w < kFewWarps; ++w) {
                     if (s[w].y == 0.f) continue;   // saw nothing; what stands beside it need not be a number
                     const float by = s[w].x == -INFINITY ? s[w].y : exp2_fast(s[w].x - top);   // a sum with no reference is NaN
-                    const float4 z = *reinterpret_cast<const float4 *>(smem + w * L::RING + share_at + (row * DP + d) * 4);
+                    const float4 z = *reinterpret_cast<const float4 *>(smem + share_at + ((w * 8 + row) * DP + d) * 4);
                     sum = fmaf(by, s[w].y, sum);
                     v[0] = fmaf(by, z.x, v[0]);
                     v[1] = fmaf(by, z.y, v[1]);
@@ -817,8 +826,10 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
             }
         }
         __syncthreads();
-        fence_proxy_async_smem();   // read and written by threads before copies write there
-        fill(used + L::kStages);
+        if (warp == 0) {
+            fence_proxy_async_smem();   // read and written by threads before copies write there
+            fill(used + L::kStages);
+        }
         stage = 0;
         if (++item == items) {
             item = 0;
@@ -826,7 +837,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
             while (used < total && Stages<KEYS>(P, b).count == 0);
         }
     } while (used < total);
-    if (lane == 0 && *abort_flag)   // what was issued arrives before the CTA ends
+    if (threadIdx.x == 0 && *abort_flag)   // what was issued arrives before the CTA ends
         for (uint32_t u = first_of_last_uses(issued, L::kStages); u < (uint32_t)issued; ++u) mbar_wait_bounded(&full[u % L::kStages], parity_of_use(u, L::kStages));
 }
 
