@@ -267,13 +267,14 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int nq = (int)P.Nq, items = (int)P.c.H * F.row_blocks;
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *empty = full + L::kStages;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], kFewWarps); }
         *abort_flag = 0;
         mbar_init_fence();
     }
+    // what came before has ended; the join may be set up meanwhile
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // this CTA's share: `total` stages from stage `stage` of item `item` of sequence b on
     int b, item, stage, total;
     if (F.whole) {
@@ -946,18 +947,22 @@ template <int BITS, int W, int NG, int NT, int PARTS> int launch_few(CacheFewPar
     F.part_stats = reinterpret_cast<float2 *>(F.part_out + (F.whole ? 0 : ctas * 2 * L::ROWS * L::DP));
     constexpr auto *kern = &cache_few_kernel<BITS, W, NG, NT, PARTS>;
     if (const int e = allow_shared_memory<kern>((int)L::ALLOC)) return e;
-    kern<<<(unsigned)ctas, kFewThreads, L::ALLOC, s>>>(F);
-    TPW_LAUNCH_OK("cache_few_kernel");
-    if (F.whole) return TPW_OK;
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)items, ctas > 4 * items ? (unsigned)(F.rows < (int)L::ROWS ? F.rows : L::ROWS) : 1);
-    config.blockDim = dim3(kFewThreads);
-    config.stream = s;
+    // Either kernel is launched while the one before it still runs, and waits for that one's end where it first reads what others write.
     cudaLaunchAttribute overlap = {};
     overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     overlap.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)ctas);
+    config.blockDim = dim3(kFewThreads);
+    config.dynamicSmemBytes = L::ALLOC;
+    config.stream = s;
     config.attrs = &overlap;
     config.numAttrs = 1;
+    TPW_CUDA_OK(cudaLaunchKernelEx(&config, kern, F));
+    TPW_LAUNCH_OK("cache_few_kernel");
+    if (F.whole) return TPW_OK;
+    config.gridDim = dim3((unsigned)items, ctas > 4 * items ? (unsigned)(F.rows < (int)L::ROWS ? F.rows : L::ROWS) : 1);
+    config.dynamicSmemBytes = 0;
     TPW_CUDA_OK(cudaLaunchKernelEx(&config, &cache_join_kernel<BITS, W, NG, NT, PARTS>, F, (int)ctas));
     TPW_LAUNCH_OK("cache_join_kernel");
     return TPW_OK;
