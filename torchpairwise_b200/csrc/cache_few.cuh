@@ -204,7 +204,7 @@ template <int KEYS> struct Stages {
 // The line of all stages: sequences one after the other, a sequence's items (heads, and blocks of rows of each) one after the other, an item's
 // stages in order.  An item with stages stands on the line for kFewExtra more, which come first: what beginning and ending it costs.
 // Found by the whole CTA (128 threads): how long the line is, and the sequence that place `at` (or item `item` of sequence `of`) lies in.
-constexpr int kFewExtra = 3;
+constexpr int kFewExtra = 4;
 struct Line {
     unsigned total, before;   // places in all; in sequences before `b`
     int b;
