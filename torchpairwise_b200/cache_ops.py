@@ -124,8 +124,13 @@ def cache_attention(q: Tensor, cache: QuantizedCache, key_lengths: Tensor, *, ca
 
     ``q`` is ``[batch, queries, heads, features]`` in float32, float16 or bfloat16, its heads a multiple of the cache's; ``key_lengths`` as
     in :func:`cache_write`, which comes first for new tokens: query i of a sequence with L keys stands at position ``L - queries + i``.
-    ``causal``, ``window``, ``scale``, ``return_lse`` and rows that see nothing are as in :func:`attention`.  What lies in the cache from a
-    sequence's length on is never used.  Not differentiable.
+    ``causal``, ``window``, ``scale``, ``return_lse`` and rows that see nothing are as in :func:`attention`; a length beyond the capacity counts
+    as the capacity.  What lies in the cache from a sequence's length on is never used.  Within it, what is not a number makes the rows of its
+    tile NaN.  Not differentiable.
+
+    Scores are to stay below 2^24 and results below 2^90 in magnitude, as are queries.  Scores, statistics and sums are held in 32 bits; with 16-bit queries
+    probabilities are rounded to half precision, and with more than 192 of them to a key head (their number times the heads that share
+    one) what the codes stand for is too, up to 65504 for float16, near a power of two of its head for bfloat16.  Float32 queries lose nothing.
     """
     _check("cache_attention", q)
     out, lse = _attend(q, *cache, key_lengths, causal, window, scale)
