@@ -142,6 +142,25 @@ def test_more_sequences_than_scratch_takes_at_once(dtype):
     assert_near(out[4:], attended(q[4:], alone, [7777], causal=True)[0], dtype, "out")
 
 
+@pytest.mark.parametrize("queries,heads,features", [(1, 3, 40), (100, 4, 64)])
+def test_very_many_short_sequences(queries, heads, features):
+    """More sequences and heads than one grid of the many-row path takes, most of them empty, and more sequences than threads that look for a place."""
+    batch = 30000
+    some = filled(3, 64, heads // 2 if queries > 1 else 3, features, 4, 32, seed=21)
+    pick = torch.arange(batch, device="cuda") % 3
+    cache = tpw.QuantizedCache(*(t[pick].contiguous() for t in some[:4]), features, 4)
+    n = torch.zeros(batch, dtype=torch.int32, device="cuda")
+    for b, length in ((0, 64), (17, 5), (9999, 33), (29999, 60)):
+        n[b] = length
+    q = torch.randn(3, queries, heads * 2 if queries > 1 else 3, features, generator=torch.Generator().manual_seed(22)).bfloat16().cuda()
+    out = tpw.cache_attention(q[pick].contiguous(), cache, n, causal=True)
+    for b in (0, 17, 9999, 29999):
+        alone = tpw.QuantizedCache(*(t[b:b + 1] for t in cache[:4]), features, 4)
+        assert_near(out[b:b + 1], attended(q[b % 3][None], alone, [int(n[b])], causal=True)[0], torch.bfloat16, b)
+    out[[0, 17, 9999, 29999]] = 0
+    assert not out.any()
+
+
 def test_offsets_beyond_32_bits():
     """5 GB of codes: the last sequence's rows lie past 2^32 bytes, and are those of a small cache."""
     small = filled(1, 1024, 8, 128, 8, 32, seed=14)

@@ -17,6 +17,7 @@ constexpr long long kSlice = 128LL << 20;
 constexpr int kKeys = 8, kValues = 14;
 
 int few(const CacheAttnParams &P, void *scratch, long long *bytes, cudaStream_t s) {
+    TPW_CHECK_ARG(P.group * P.Nq < (1LL << 30), "tpw_cache_attention: more than 2^30 query rows to a key head");
     return P.c.bits == 4 ? cache_few_4(P, scratch, bytes, s) : cache_few_8(P, scratch, bytes, s);
 }
 
@@ -26,11 +27,16 @@ struct Slices {
     explicit Slices(const CacheAttnParams &P) {
         auto round = [](long long bytes) { return (bytes + 255) / 256 * 256; };
         sequence = round(P.c.capacity * P.c.H * P.c.D * 2);
-        step = sequence > 0 ? kSlice / (2 * sequence) : P.c.B;
-        step = step < 1 ? 1 : step < P.c.B ? step : P.c.B;
+        // no more than the grid of cache_ranges takes, and no more queries than keys and values
+        const long long asked = P.Nq * P.Hq * P.c.D * 2;
+        step = P.c.B;
+        if (sequence > 0 && step > kSlice / (2 * sequence)) step = kSlice / (2 * sequence);
+        if (step > kSlice / asked) step = kSlice / asked;
+        if (step * P.c.H > 65535) step = 65535 / P.c.H;
+        if (step < 1) step = 1;
         const bool wide = P.dtype == TPW_BF16;
         ranges = wide ? round(step * P.c.H * 2 * kRangeParts * 4) : 0;
-        queries = wide ? round(step * P.Nq * P.Hq * P.c.D * 2) : 0;
+        queries = wide ? round(step * asked) : 0;
     }
     long long bytes() const { return 2 * sequence * step + ranges + 2 * queries; }
     unsigned char *values(void *scratch) const { return static_cast<unsigned char *>(scratch) + sequence * step; }
