@@ -10,9 +10,10 @@
 //            rounded p_j.  A warp turns its keys' steps and zeros into half precision once, scaled by a power of two that they share.
 // With keys along M a product has 8 rows of queries; rows along M would leave half of every product empty for up to 8 heads that share a key.
 //
-// Float32 queries: q and p step as two half-precision parts each, 22 bits.  Tensor-core sums truncate, so they are kept small: those of scores begin at
-// -M a_g, M the middle code, with zero_jg + M step_jg in the second term; codes of values are taken less M, and the products of 16 keys go to sums in registers.
-// (For 16-bit queries the beginnings would cost 16 registers of the 168 that three CTAs an SM leave: 51.3 -> 49.7 us without.)
+// Tensor-core sums truncate, so they are kept small: those of scores begin at -M a_g, M the middle code, with zero_jg + M step_jg in the second term.  (Not
+// for 4-bit groups of 32 and 16-bit queries: 32 codes below 16 add up to little, and the beginnings would cost 16 registers of the 168 that three CTAs an SM
+// leave, 51.3 -> 49.7 us without.)  Float32 queries: q and p step as two half-precision parts each, 22 bits; codes of values less M, and the products of 16 keys
+// go to sums in registers.
 //
 // All stages of keys (64 or 128) of all sequences and heads form one line that the CTAs, three on an SM, take equal shares of, whatever the lengths: a
 // share ends and begins anywhere in a sequence.  What a CTA has of a head that others have parts of goes to scratch, and a second kernel, whose launch
@@ -266,6 +267,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
     constexpr int DP = 32 * W, ROWS = 8 * NT, SUB = L::SUB, KEYS = L::KEYS;
     constexpr bool WIDE = PARTS == 2;
     constexpr float MIDDLE = BITS == 4 ? 8.f : 128.f;
+    constexpr bool SMALL = WIDE || NG == 1 || BITS == 8;   // sums of scores begin at -M a_g
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ unsigned room[kFewWarps + 2];
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_FLAG);
@@ -441,7 +443,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
         __syncthreads();
         if (warp == 0 && used == 0) fill(L::kStages);
         uint32_t q[PARTS][NT][W][2][2], qz[NT][PARTS][2];
-        float start[NT][NG][4], factor[NT][2];   // -M a_g (WIDE); raw scores times the factor are powers of 2
+        float start[NT][NG][4], factor[NT][2];   // -M a_g (SMALL); raw scores times the factor are powers of 2
         int all_lo = S.first, all_hi = S.end;   // keys that all rows see
         auto sees = [&](int x, int e, int &lo, int &hi) {   // those of a row
             const int mine = row0 + 8 * x + 2 * t + e, i = mine < F.rows ? (unsigned)mine % F.by_nq : 0;
@@ -468,7 +470,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                 for (int w = 0; w < W; ++w) own += sums[w * 8 + g];
 #pragma unroll
             for (int part = 0; part < 2 * PARTS; ++part) {
-                const uint32_t word = Narrow<__nv_bfloat16>::pack(WIDE ? own * MIDDLE : 0.f, own);
+                const uint32_t word = Narrow<__nv_bfloat16>::pack(SMALL ? own * MIDDLE : 0.f, own);
                 qz[x][part / 2][part % 2] = word;
                 own -= __uint_as_float(word & 0xffff0000u);
             }
@@ -482,7 +484,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                     else
 #pragma unroll
                         for (int w = 0; w < W; ++w) a += sums[w * 8 + row];
-                    start[x][k][e] = start[x][k][2 + e] = WIDE ? -MIDDLE * a : 0.f;
+                    start[x][k][e] = start[x][k][2 + e] = SMALL ? -MIDDLE * a : 0.f;
                     zeros[x][k][e] = 0.f;
                 }
                 factor[x][e] = sums[W * 8 + row];
