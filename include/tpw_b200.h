@@ -702,7 +702,7 @@ typedef struct tpw_cache_attention_args {
     double scale;             /* positive, finite, also as a float, times log2 e */
     const void *q;            /* [B, Nq, Hq, D]; strides of batch, token and head in elements, features side by side */
     int64_t q_stride[3];
-    void *out;                /* [B, Nq, Hq, D] dense */
+    void *out;                /* [B, Nq, Hq, D] dense, 16-byte aligned */
     float *lse;               /* [B, Hq, Nq] dense; NULL: not wanted */
 } tpw_cache_attention_args;
 /* Scratch (device memory, 16-byte aligned) that the call with these arguments wants; 0: none; -1: refused (tpw_last_error). */

@@ -95,7 +95,7 @@ def test_errors_of_the_entry_points_of_attention():
         refused, message = call(cache_of(**changes), attention())
         assert refused and text in message, (changes, message)
     for changes, text in ((dict(dtype=_abi.F64), b"dtype"), (dict(Hq=3), b"multiple"), (dict(window=4), b"causal"), (dict(window=-1), b"window"), (dict(scale=0.0), b"scale"),
-                          (dict(scale=1e-46), b"scale"), (dict(scale=2.4e38), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(Nq=-1), b"-1 queries"), (dict(q=None), b"NULL")):
+                          (dict(scale=1e-46), b"scale"), (dict(scale=2.4e38), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(Nq=-1), b"-1 queries"), (dict(q=None), b"NULL"), (dict(out=X + 8), b"aligned")):
         refused, message = call(cache_of(), attention(**changes))
         assert refused and text in message, (changes, message)
     assert lib.tpw_cache_attention_scratch_bytes(None, None) == -1

@@ -44,6 +44,7 @@ int check_attention(const tpw_cache *c, const tpw_cache_attention_args *a) {
     const float factor = static_cast<float>(a->scale * 1.4426950408889634074);
     TPW_CHECK_ARG(a->scale > 0 && isfinite(a->scale) && factor > 0.f && isfinite(factor), "tpw_cache_attention: scale %g: positive and finite, also in 32 bits, is needed", a->scale);
     TPW_CHECK_ARG((a->q && a->out) || c->B == 0 || a->Nq == 0 || a->Hq == 0, "tpw_cache_attention: NULL pointer");
+    TPW_CHECK_ARG(aligned16(a->out), "tpw_cache_attention: out must be 16-byte aligned");
     return TPW_OK;
 }
 
