@@ -1,0 +1,123 @@
+"""Attention over a quantised cache whose values differ in magnitude within a head: the small ones keep their digits beside the large ones."""
+import pytest
+import torch
+
+import torchpairwise_b200 as tpw
+from attention_cases import assert_near
+from cache_cases import attended
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+# The bounds are those of any other call, taken over the small values alone: a probability times a step is rounded once (float16's 2^-11, float32 in two
+# parts of them), the result once in its type, and neither depends on how large other groups, or tokens with no weight, are.
+
+
+def scene(ratio, queries, heads=4, key_heads=2, d=128, keys=300, bits=4, group=32):
+    g = torch.Generator().manual_seed(ratio + queries)
+    k, v = (torch.randn(2, keys, key_heads, d, generator=g).cuda() for _ in range(2))
+    q = 2 * torch.randn(2, queries, heads, d, generator=g).cuda()
+    n = torch.tensor([keys, keys - 37], dtype=torch.int32, device="cuda")
+    cache = tpw.quantized_cache(2, keys, key_heads, d, bits=bits, group=group)
+    return q, k, v, n, cache
+
+
+def stored(cache, k, v):
+    tpw.cache_write(cache, k, v, torch.full((k.shape[0],), k.shape[1], dtype=torch.int32, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("queries", [1, 5, 250])
+@pytest.mark.parametrize("ratio", [8, 14, 20])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_a_group_of_large_values_beside_small_ones(dtype, queries, ratio, bits):
+    q, k, v, n, cache = scene(ratio, queries, bits=bits)
+    v = v * 2.0 ** (-ratio // 2)
+    v[..., 32:64] *= 2.0 ** ratio
+    stored(cache, k, v)
+    q = q.to(dtype)
+    out = tpw.cache_attention(q, cache, n, causal=True)
+    want = attended(q, cache, n.tolist(), causal=True)[0]
+    small = torch.ones(128, dtype=torch.bool, device="cuda")
+    small[32:64] = False
+    assert_near(out[..., small], want[..., small], dtype, "small groups")
+    assert_near(out[..., ~small], want[..., ~small], dtype, "large group")
+    assert tpw.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("queries", [1, 5, 250])
+@pytest.mark.parametrize("ratio", [8, 14, 20])
+@pytest.mark.parametrize("bits,group", [(4, 32), (4, None), (8, None)])
+@pytest.mark.parametrize("place", [0, 130, 261])
+def test_a_large_token_that_nobody_attends_to(dtype, queries, ratio, bits, group, place):
+    """Its score is about 60 below the others', so that it takes e^-60 times the ratio of the result: nothing."""
+    q, k, v, n, cache = scene(ratio, queries, bits=bits, group=group)
+    q[..., 0] = 4.0
+    k[..., 0] = 0.0
+    k[:, place, :, 0] = -60 * 128 ** 0.5 / 4
+    v = v * 2.0 ** (-ratio // 2)
+    v[:, place] *= 2.0 ** ratio
+    stored(cache, k, v)
+    q = q.to(dtype)
+    out = tpw.cache_attention(q, cache, n)
+    want = attended(q, cache, n.tolist())[0]
+    assert_near(out, want, dtype, "out")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("queries", [1, 3])
+@pytest.mark.parametrize("ratio", [8, 20])
+@pytest.mark.parametrize("heads", [4, 32])
+def test_a_large_token_that_another_head_attends_to(dtype, queries, ratio, heads):
+    """Heads that share keys: the first looks at the large token alone, the others at all but that one, each in its own magnitude."""
+    q, k, v, n, cache = scene(ratio, queries, heads=heads, key_heads=2 if heads < 8 else 4)
+    group = heads // cache.k_codes.shape[1]
+    sees = (torch.arange(heads, device="cuda") % group == 0)[None, None, :]
+    q[..., 0] = torch.where(sees, 4.0, -4.0)
+    k[..., 0] = 0.0
+    k[:, 200, :, 0] = 60 * 128 ** 0.5 / 4
+    v = v * 2.0 ** (-ratio // 2)
+    v[:, 200] *= 2.0 ** ratio
+    stored(cache, k, v)
+    q = q.to(dtype)
+    out = tpw.cache_attention(q, cache, n)
+    want = attended(q, cache, n.tolist())[0]
+    first = sees[0, 0]
+    assert_near(out[:, :, ~first], want[:, :, ~first], dtype, "the others")
+    assert_near(out[:, :, first], want[:, :, first], dtype, "the first")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("queries", [1, 5])
+def test_large_tokens_that_lose_their_weight_on_the_way(dtype, queries):
+    """Scores climb by 8 from block to block while values fall by 2^6: what came first, large as it was, ends as nothing."""
+    q, k, v, n, cache = scene(1, queries, keys=640)
+    block = torch.arange(640, device="cuda") // 64
+    q[..., 0] = 4.0
+    k[..., 0] = (block * 8 * 128 ** 0.5 / 4)[None, :, None]
+    v = v * torch.exp2(10.0 - 2 * block)[None, :, None, None]
+    stored(cache, k, v)
+    q = q.to(dtype)
+    n = n.fill_(640)
+    out, lse = tpw.cache_attention(q, cache, n, return_lse=True)
+    want = attended(q, cache, [640, 640])
+    assert_near(out, want[0], dtype, "out")
+    assert_near(lse, want[1], torch.float32, "lse")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_constant_tokens_and_storage_that_was_never_written(dtype):
+    """Steps at the bottom (2^-100, all values of a token alike) and of zero, before and between others."""
+    q, k, v, n, cache = scene(2, 5, keys=512)
+    v[:, :130] = 3.0
+    v[:, 200:230] = -1.5
+    stored(cache, k, v)
+    for t in (cache.v_codes, cache.v_scales):
+        t[:, :, 64:100] = 0
+        t[:, :, 300:310] = 0
+    q = q.to(dtype)
+    out = tpw.cache_attention(q, cache, n)
+    assert_near(out, attended(q, cache, n.tolist())[0], dtype, "out")
+    n = n.fill_(130)
+    out = tpw.cache_attention(q, cache, n)
+    assert_near(out, attended(q, cache, n.tolist())[0], dtype, "constant values")

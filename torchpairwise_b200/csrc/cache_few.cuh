@@ -6,13 +6,17 @@
 //   scores   K q^T, m16n8k16, 16 keys by 8 query rows: sum_g step_jg (sum_d c_jd q_d) + zero_jg a_g, a_g = sum_d q_d over the group.  The second
 //            term is a product of its own, bfloat16: a word of the cache, step and zero, is the operand, beside 0 and a_g.  A row of q is
 //            lifted by a power of two to half precision's upper end.
-//   output   V^T P^T, 16 features by 8 rows: the steps go into the probabilities, (p_j step_jg) c_jd; one more product adds p_j zero_jg, of the same
-//            rounded p_j.  A warp turns its keys' steps and zeros into half precision once, scaled by a power of two that they share.
+//   output   V^T P^T, 16 features by 8 rows: the steps go into the probabilities, y_jg = p_j step_jg, formed in 32 bits and rounded to half precision
+//            once: sum_j y_jg (c_jd - M) + p_j (zero_jg + M step_jg), M the middle code, so that a rounding counts by how far a value is from its group's
+//            middle.  The second term stays in 32 bits; M sum_j y_jg comes from a product with ones.
+// Steps of one head may be any numbers from 2^-100 to 2^97, and half precision has 40 powers of two: a row of queries has a norm for every group,
+// a power of two that brings the largest y_jg that it met to [4, 8).  So what a row loses (2^-27 of its largest share) depends neither on other groups, nor on
+// other rows, nor on tokens that it gives no weight.  Norms move where references do, or where a step is far above those met.
 // With keys along M a product has 8 rows of queries; rows along M would leave half of every product empty for up to 8 heads that share a key.
 //
 // Tensor-core sums truncate, so they are kept small: those of scores begin at -M a_g, M the middle code, with zero_jg + M step_jg in the second term.  (Not
 // for 4-bit groups of 32 and 16-bit queries: 32 codes below 16 add up to little, and the beginnings would cost 16 registers of the 168 that three CTAs an SM
-// leave, 51.3 -> 49.7 us without.)  Float32 queries: q and p step as two half-precision parts each, 22 bits; codes of values less M, and the products of 16 keys
+// leave, 51.3 -> 49.7 us without.)  Float32 queries: q and y as two half-precision parts each, 22 bits; codes of values less M, and the products of 16 keys
 // go to sums in registers.
 //
 // All stages of keys (64 or 128) of all sequences and heads form one line that the CTAs, three on an SM, take equal shares of, whatever the lengths: a
@@ -20,18 +24,20 @@
 // overlaps this one, weighs the parts together in their order.  In a CTA four warps take 16 keys or 32 of a stage each, with a running reference, sum and
 // output of their own; bulk copies bring the stages into a ring, across the ends of heads.
 //
-// Measured bfloat16, 4 bits: [16, 1 x 16384, 32/8, 128] ragged, groups of 32, 185 MB in 46 us (4.0 TB/s), of which copies alone take 31 and the products without them 38;
-// [64, 1 x 4096, 32/8, 128], one group, 158 MB in 44 us.
+// Measured bfloat16, 4 bits: [16, 1 x 16384, 32/8, 128] ragged, groups of 32, 185 MB in 51 us (3.6 TB/s), of which copies alone take 31;
+// [64, 1 x 4096, 32/8, 128], one group, 158 MB in 45 us.  Norms by row and group cost 4 and 1 us of that against one power of two for all steps of a warp, which
+// leaves groups beside a loud one, and tokens beside a loud token, without digits: 1.5 us the look at them at the beginning of a head, the rest products in 32 bits.
 #pragma once
 #include "attention_tc.cuh"
 #include "cache.cuh"
+#include "packed_f32x2.cuh"
 
 namespace tpw {
 namespace {
 
 constexpr int kFewWarps = 4, kFewThreads = 128;
-constexpr float kFewLift = 6.f;      // probabilities are lifted by 2^6 beside the 2^8 that they may exceed their reference by: below 2^16, and
-constexpr float kFewSlack = 8.f;     // normal half-precision numbers down to 2^-20 of it
+constexpr int kFewSlack = 8;          // probabilities may exceed their reference by 2^8
+constexpr int kFewHighest = 110;      // norms go from 2^-110 to 2^110: p * norm * step never leaves the range of 32 bits on its way
 
 struct CacheFewParams {
     CacheAttnParams a;
@@ -47,12 +53,14 @@ template <int BITS, int W, int NG, int NT, int PARTS> struct CacheFew {
     static constexpr int KEYS = BITS == 4 ? 128 : 64, OWN = KEYS / kFewWarps, SUB = OWN / 16;   // of a stage; a warp's of them, and blocks of 16
     static constexpr uint32_t ROW = W * 4 * BITS, CODES = KEYS * ROW, SCALES = KEYS * NG * 4, STAGE = 2 * (CODES + SCALES), DP = 32 * W, ROWS = 8 * NT;
     static constexpr int PER_SM = NT == 1 ? 3 : 2;
-    static constexpr uint32_t STATS = kFewWarps * 8 * 8, PREPARED = PARTS == 1 ? kFewWarps * SUB * NG * 64 : 0, QUERIES = PARTS * NT * W * 512, SUMS = NT * (W + 1) * 32;
-    static constexpr uint32_t ROOM = (NT == 1 ? 75776 : 112640) - STATS - PREPARED - QUERIES - SUMS - 320;
+    static constexpr uint32_t NP = NG == 3 ? 4 : NG;   // words that a key's groups take
+    static constexpr uint32_t STATS = kFewWarps * 8 * 8, PREPARED = kFewWarps * SUB * 16 * NP * 8, NORMS = kFewWarps * NT * 8 * NP * 4,
+                              QUERIES = PARTS * NT * W * 512, SUMS = NT * (W + 1) * 32;
+    static constexpr uint32_t ROOM = (NT == 1 ? 75776 : 112640) - STATS - PREPARED - NORMS - QUERIES - SUMS - 320;
     static constexpr int kStages = ROOM / STAGE < 8 ? ROOM / STAGE : 8;
     static_assert(kStages >= 2, "a ring of two stages at least");
     static_assert(kFewWarps * 8 * DP * 4 <= STAGE, "the warps' 8 rows of results fit a stage");
-    static constexpr uint32_t OFF_STATS = kStages * STAGE, OFF_PREPARED = OFF_STATS + STATS, OFF_QUERIES = OFF_PREPARED + PREPARED, OFF_SUMS = OFF_QUERIES + QUERIES,
+    static constexpr uint32_t OFF_STATS = kStages * STAGE, OFF_PREPARED = OFF_STATS + STATS, OFF_NORMS = OFF_PREPARED + PREPARED, OFF_QUERIES = OFF_NORMS + NORMS, OFF_SUMS = OFF_QUERIES + QUERIES,
                               OFF_BAR = OFF_SUMS + SUMS, OFF_FLAG = OFF_BAR + 16 * kStages, ALLOC = OFF_FLAG + 16;
 };
 
@@ -81,11 +89,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 }
 __device__ __forceinline__ uint32_t half2_of(float lo, float hi) { return Narrow<__half>::pack(lo, hi); }
 __device__ __forceinline__ uint32_t half2_rest(float lo, float hi) { return Narrow<__half>::rest(lo, hi); }
-__device__ __forceinline__ uint32_t half2_times(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
 __device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -113,6 +116,23 @@ template <int N> __device__ __forceinline__ void load_words(uint32_t (&w)[N], co
 #pragma unroll
         for (int k = 0; k < N; ++k) w[k] = reinterpret_cast<const uint32_t *>(p)[k];
     }
+}
+
+// N floats, likewise
+template <uint32_t N> __device__ __forceinline__ void store_words(float *p, const float (&x)[N]) {
+    if constexpr (N == 4) *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    else if constexpr (N == 2) *reinterpret_cast<float2 *>(p) = make_float2(x[0], x[1]);
+    else p[0] = x[0];
+}
+// N pairs of floats
+template <int N> __device__ __forceinline__ void load_pairs(f32x2 (&x)[N], const float *p) {
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < N / 2; ++k) {
+            const ulonglong2 v = reinterpret_cast<const ulonglong2 *>(p)[k];
+            x[2 * k] = v.x; x[2 * k + 1] = v.y;
+        }
+    } else x[0] = *reinterpret_cast<const f32x2 *>(p);
 }
 
 // 8 features of a row of queries in 32 bits, `n` of which there are
@@ -168,14 +188,14 @@ __device__ __forceinline__ void store_out(const CacheAttnParams &P, long long at
     }
 }
 
-// four features of row r from the weighed sums of values and of probabilities, which are lifted beside their reference
+// four features of row r from the weighed sums of values and of probabilities
 __device__ __forceinline__ void finish(const CacheFewParams &F, int b, int hk, int r, int d, float (&v)[4], float reference, float sum) {
     const CacheAttnParams &P = F.a;
     const int over = (unsigned)r / F.by_nq, i = r - over * (int)P.Nq, h = (int)(hk * P.group) + over;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] *= inv;
-    if (d == 0 && P.lse) P.lse[(b * P.Hq + h) * P.Nq + i] = sum == 0.f ? -INFINITY : (reference - kFewLift + log2f(sum)) * 0.69314718055994531f;
+    if (d == 0 && P.lse) P.lse[(b * P.Hq + h) * P.Nq + i] = sum == 0.f ? -INFINITY : (reference + log2f(sum)) * 0.69314718055994531f;
     store_out(P, ((b * P.Nq + i) * P.Hq + h) * P.c.D + d, v, P.c.D - d);
 }
 
@@ -377,8 +397,10 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
     float2 *stats = reinterpret_cast<float2 *>(smem + L::OFF_STATS);
     uint32_t *queries = reinterpret_cast<uint32_t *>(smem + L::OFF_QUERIES);   // [part][block][w][lane][4]
     float *query_sums = reinterpret_cast<float *>(smem + L::OFF_SUMS);         // [block][w and, last, the factor of scores][row]
-    // of every 16 keys: steps [pair of slots][group][slot of the pair], zeros [group][slot]
-    uint16_t *prepared = reinterpret_cast<uint16_t *>(smem + L::OFF_PREPARED) + warp * SUB * NG * 32;
+    // a warp's own: of every 16 keys [slot][group] steps, then middles of values (zero + M step); of every row its norms
+    constexpr int NP = L::NP;
+    float *prepared = reinterpret_cast<float *>(smem + L::OFF_PREPARED) + warp * SUB * 32 * NP;
+    float *norms = reinterpret_cast<float *>(smem + L::OFF_NORMS) + warp * NT * 8 * NP;
     const int slot0 = key_of_slot(g), value0 = t, value1 = 4 + (t ^ 1);   // and 8 more
     int used = 0;
 
@@ -450,8 +472,10 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
             lo = mine < F.rows ? see.lo(i) : 0;
             hi = mine < F.rows ? see.hi(i) : 1 << 30;
         };
-        float m[NT][2], l[NT][2], o[NT][2 * W][4], zeros[NT][NG][2], zero_sums[NT][4];   // rows 2 t, 2 t + 1 of every block: reference (a power of 2), sums
-        int top_scale = 1;                       // largest exponent of a step or zero of a value so far, as in its bits
+        float m[NT][2], l[NT][2], o[NT][2 * W][4];   // rows 2 t, 2 t + 1 of every block: reference (a power of 2), sums
+        float ones[NT][4];                       // sums of y: of group g, rows 2 t, 2 t + 1
+        f32x2 middles[NT][NP];                   // sums of p (zero + M step) over this lane's keys: of a row two groups to a word, one after the other (one group: the two rows)
+        uint32_t limits[(NG + 1) / 2];           // the highest steps, as bits, that need no look at the norms; two groups in a word
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
             const float *sums = query_sums + x * (W + 1) * 8;
@@ -485,7 +509,6 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
 #pragma unroll
                         for (int w = 0; w < W; ++w) a += sums[w * 8 + row];
                     start[x][k][e] = start[x][k][2 + e] = SMALL ? -MIDDLE * a : 0.f;
-                    zeros[x][k][e] = 0.f;
                 }
                 factor[x][e] = sums[W * 8 + row];
                 int lo, hi;
@@ -500,8 +523,13 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[x][n][e] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) zero_sums[x][e] = 0.f;
+            for (int e = 0; e < 4; ++e) ones[x][e] = 0.f;
+#pragma unroll
+            for (int k = 0; k < NP; ++k) middles[x][k] = 0;
         }
+#pragma unroll
+        for (int k = 0; k < (NG + 1) / 2; ++k) limits[k] = 0xffffffffu;
+        for (int k = lane; k < NT * 8 * NP; k += 32) norms[k] = power_of_two(127 + kFewHighest);
         all_lo = __reduce_max_sync(0xffffffffu, all_lo);
         all_hi = __reduce_min_sync(0xffffffffu, all_hi);
         uint32_t st = slot;
@@ -597,12 +625,13 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
 #pragma unroll
                         for (int k = 0; k < NG; ++k) vs[k] = 0;
                 }
-                // the reference moves, and sums are scaled, only where a score, a step or a zero has left it behind
-                uint32_t high_scale = 0;
+                // References move, norms are looked at and sums are scaled, only where a score has left its reference behind or a step what norms allow
+                bool moves = false;
 #pragma unroll
-                for (int k = 0; k < NG; ++k) high_scale = max_halves(high_scale, vs[k] & 0x7fffffffu);   // steps are not negative
-                high_scale = max(high_scale << 16, high_scale & 0xffff0000u);
-                bool moves = (int)(high_scale >> 23) > top_scale;
+                for (int k = 0; k < (NG + 1) / 2; ++k) {
+                    const uint32_t steps = __byte_perm(vs[2 * k], 2 * k + 1 < NG ? vs[2 * k + 1 < NG ? 2 * k + 1 : 0] : 0u, 0x5410);
+                    moves = moves || max_halves(steps, limits[k]) != limits[k];
+                }
                 float high[NT][2];
 #pragma unroll
                 for (int x = 0; x < NT; ++x)
@@ -613,54 +642,39 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                         high[x][e] *= factor[x][e];
                         moves = moves || high[x][e] > m[x][e] + kFewSlack;
                     }
-                if (__any_sync(0xffffffffu, moves)) {
-                    const int now = max((int)(__reduce_max_sync(0xffffffffu, high_scale) >> 23), top_scale);
-                    const float by_scale = now - top_scale < 126 ? power_of_two(127 + top_scale - now) : 0.f;
-                    top_scale = now;
+                moves = __any_sync(0xffffffffu, moves);
+                float up[NT][2];   // of references
+                if (moves) {
 #pragma unroll
-                    for (int x = 0; x < NT; ++x) {
-                        float by[2];
+                    for (int x = 0; x < NT; ++x)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             float top = high[x][e];
 #pragma unroll
                             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
                             top = fmaxf(top, m[x][e]);
-                            by[e] = top == m[x][e] ? 1.f : exp2_fast(m[x][e] - top);
+                            up[x][e] = top == m[x][e] ? 0.f : top - m[x][e];
                             m[x][e] = top;
-                            l[x][e] *= by[e];
-#pragma unroll
-                            for (int k = 0; k < NG; ++k) zeros[x][k][e] *= by[e];
-                            by[e] *= by_scale;
+                            l[x][e] *= exp2_fast(-up[x][e]);
                         }
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            zero_sums[x][e] *= by[e & 1];
-#pragma unroll
-                            for (int n = 0; n < 2 * W; ++n) o[x][n][e] *= by[e & 1];
-                        }
-                    }
                 }
-                const float norm = power_of_two(253 - top_scale);   // steps and zeros below 1
-                if constexpr (!WIDE) {
-                    __syncwarp();   // the last ones are read
-                    if (lane < 16 * SUB) {
-                        const int slot = slot_of_key(lane & 15);
-                        uint16_t *to = prepared + (lane >> 4) * NG * 32 + (slot >> 1) * 2 * NG + (slot & 1), *to_zero = prepared + (lane >> 4) * NG * 32 + 16 * NG + slot;
+                __syncwarp();   // what the last keys left is read
+                if (lane < 16 * SUB) {
+                    float *to = prepared + ((lane >> 4) * 32 + slot_of_key(lane & 15)) * NP;
+                    alignas(16) float step[NP] = {}, middle[NP] = {};
 #pragma unroll
-                        for (int k = 0; k < NG; ++k) {
-                            const uint32_t both = half2_of(step_of(vs[k]) * norm, zero_of(vs[k]) * norm);
-                            to[2 * k] = (uint16_t)both;
-                            to_zero[16 * k] = (uint16_t)(both >> 16);
-                        }
+                    for (int k = 0; k < NG; ++k) {
+                        step[k] = step_of(vs[k]);
+                        middle[k] = fmaf(step[k], MIDDLE, zero_of(vs[k]));
                     }
-                    __syncwarp();
+                    store_words(to, step);
+                    store_words(to + 16 * NP, middle);
                 }
 #pragma unroll
                 for (int x = 0; x < NT; ++x)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float shift = m[x][e] == -INFINITY ? 0.f : kFewLift - m[x][e];
+                        const float shift = m[x][e] == -INFINITY ? 0.f : -m[x][e];
 #pragma unroll
                         for (int h = 0; h < SUB; ++h)
 #pragma unroll
@@ -669,6 +683,71 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                                 l[x][e] += p[h][x][2 * s + e];
                             }
                     }
+                __syncwarp();
+                if (moves) {
+                    uint32_t allowed[NG];
+#pragma unroll
+                    for (int k = 0; k < NG; ++k) allowed[k] = 0xffff;
+#pragma unroll
+                    for (int x = 0; x < NT; ++x) {
+                        float top[2][NG] = {}, *norm = norms + (8 * x + 2 * t) * NP;
+                        int was[2][NG];
+#pragma unroll
+                        for (int h = 0; h < SUB; ++h)
+#pragma unroll
+                            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                                for (int k = 0; k < NG; ++k) {
+                                    const float step = prepared[(h * 32 + g + 8 * s) * NP + k];
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e) top[e][k] = fmaxf(top[e][k], fabsf(p[h][x][2 * s + e] * step));
+                                }
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+#pragma unroll
+                            for (int k = 0; k < NG; ++k) was[e][k] = (int)(__float_as_uint(norm[e * NP + k]) >> 23) - 127;
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                                for (int k = 0; k < NG; ++k) top[e][k] = fmaxf(top[e][k], __shfl_xor_sync(0xffffffffu, top[e][k], d));
+                        __syncwarp();   // norms are read
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float by = exp2_fast(-up[x][e]);
+                            if constexpr (NP == 1) middles[x][0] = mul2(middles[x][0], e ? pack2(1.f, by) : pack2(by, 1.f));
+                            else {
+#pragma unroll
+                                for (int k = 0; k < NP / 2; ++k) middles[x][e * (NP / 2) + k] = mul2(middles[x][e * (NP / 2) + k], pack2(by, by));
+                            }
+#pragma unroll
+                            for (int k = 0; k < NG; ++k) {
+                                // up by what the reference went up; down so far that the largest y of these keys is below 8
+                                const int high = min(was[e][k] + (int)fminf(up[x][e], 1024.f), kFewHighest), now = max(min(high, 129 - (int)(__float_as_uint(top[e][k]) >> 23)), -kFewHighest);
+                                if (g == 0) norm[e * NP + k] = power_of_two(127 + now);
+                                // steps below 2^7 over the norm: y stays below 2^15
+                                if (m[x][e] > -INFINITY) allowed[k] = min(allowed[k], (uint32_t)((134 - now) << 7) - 1);
+                                const float scale = by * power_of_two(127 + now - was[e][k]);
+                                if (g == k) ones[x][e] *= scale;
+#pragma unroll
+                                for (int n = 0; n < 2 * W; ++n)
+                                    if (NG == 1 || n / 2 == k) {
+                                        o[x][n][e] *= scale;
+                                        o[x][n][2 + e] *= scale;
+                                    }
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < NG; ++k) allowed[k] = __reduce_min_sync(0xffffffffu, allowed[k]);
+#pragma unroll
+                    for (int k = 0; k < (NG + 1) / 2; ++k) limits[k] = allowed[2 * k] | (2 * k + 1 < NG ? allowed[2 * k + 1 < NG ? 2 * k + 1 : 0] : 0xffffu) << 16;
+                    __syncwarp();
+                }
+                f32x2 norm[NT][NP];   // laid out as the middles
+#pragma unroll
+                for (int x = 0; x < NT; ++x) load_pairs(norm[x], norms + (8 * x + 2 * t) * NP);
 #pragma unroll
                 for (int h = 0; h < SUB; ++h) {
                     constexpr int UNITS = BITS == 4 ? 2 * W : 4 * W;   // bytes of a lane's codes of a value
@@ -682,44 +761,55 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                             vw[s][1] = *reinterpret_cast<const uint16_t *>(at + 4);
                         }
                     }
-                    // probabilities (times steps) as operands: slots 2 t, 2 t + 1 and 2 t + 8, 2 t + 9 of row g
-                    uint32_t y[PARTS][NT][2], pt[NT][2];
-                    uint32_t steps[2][NG];
+                    // y as operands, slots 2 t, 2 t + 1 and 2 t + 8, 2 t + 9 of row g, of every group: rounded, and what that left
+                    uint32_t y[NG][PARTS][NT][2];
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        const float *steps = prepared + (h * 32 + g + 8 * s) * NP;
+                        auto narrow = [&](int k, int x, float y0, float y1) {
+                            y[k][0][x][s] = transposed(half2_of(y0, y1));
+                            if constexpr (WIDE) y[k][1][x][s] = transposed(half2_rest(y0, y1));
+                        };
+                        if constexpr (NP == 1) {
+                            const f32x2 step = pack2(steps[0], steps[0]), middle = pack2(steps[16], steps[16]);
+#pragma unroll
+                            for (int x = 0; x < NT; ++x) {
+                                const f32x2 both = pack2(p[h][x][2 * s], p[h][x][2 * s + 1]);
+                                middles[x][0] = fma2(both, middle, middles[x][0]);
+                                float y0, y1;
+                                unpack2(mul2(mul2(both, norm[x][0]), step), y0, y1);
+                                narrow(0, x, y0, y1);
+                            }
+                        } else {
+                            f32x2 step[NP / 2], middle[NP / 2];
+                            load_pairs(step, steps);
+                            load_pairs(middle, steps + 16 * NP);
+#pragma unroll
+                            for (int x = 0; x < NT; ++x) {
+                                const f32x2 p0 = pack2(p[h][x][2 * s], p[h][x][2 * s]), p1 = pack2(p[h][x][2 * s + 1], p[h][x][2 * s + 1]);
+#pragma unroll
+                                for (int k = 0; k < NP / 2; ++k) {
+                                    middles[x][k] = fma2(p0, middle[k], middles[x][k]);
+                                    middles[x][NP / 2 + k] = fma2(p1, middle[k], middles[x][NP / 2 + k]);
+                                    float a0, a1, b0, b1;
+                                    unpack2(mul2(mul2(p0, norm[x][k]), step[k]), a0, a1);
+                                    unpack2(mul2(mul2(p1, norm[x][NP / 2 + k]), step[k]), b0, b1);
+                                    narrow(2 * k, x, a0, b0);
+                                    if (2 * k + 1 < NG) narrow(2 * k + 1 < NG ? 2 * k + 1 : 0, x, a1, b1);
+                                }
+                            }
+                        }
+                    }
                     if constexpr (!WIDE) {
-                        const uint16_t *ready = prepared + h * NG * 32, *z = ready + 16 * NG + 16 * (g < NG ? g : 0) + 2 * t;
 #pragma unroll
-                        for (int s = 0; s < 2; ++s) load_words(steps[s], reinterpret_cast<const unsigned char *>(ready + (4 * s + t) * 2 * NG));
-                        const uint32_t z0 = g < NG ? *reinterpret_cast<const uint32_t *>(z) : 0u, z1 = g < NG ? *reinterpret_cast<const uint32_t *>(z + 8) : 0u;
+                        for (int k = 0; k < NG; ++k) {
+                            const uint32_t one = g == k ? 0x3c003c00u : 0u;   // 1 in row k
 #pragma unroll
-                        for (int x = 0; x < NT; ++x) {
-#pragma unroll
-                            for (int s = 0; s < 2; ++s) pt[x][s] = transposed(half2_of(p[h][x][2 * s], p[h][x][2 * s + 1]));
-                            mma_f16(zero_sums[x], z0, 0u, z1, 0u, pt[x][0], pt[x][1]);
+                            for (int x = 0; x < NT; ++x) mma_f16(ones[x], one, 0u, one, 0u, y[k][0][x][0], y[k][0][x][1]);
                         }
                     }
 #pragma unroll
                     for (int w = 0; w < W; ++w) {
-                        if (NG > 1 || w == 0)
-#pragma unroll
-                            for (int s = 0; s < 2; ++s) {
-                                if constexpr (!WIDE) {
-#pragma unroll
-                                    for (int x = 0; x < NT; ++x) y[0][x][s] = half2_times(pt[x][s], steps[s][NG > 1 ? w : 0]);
-                                } else {
-                                    const int key = 16 * h + 8 * s + slot0, j = j0 + key;
-                                    uint32_t sc = reinterpret_cast<const uint32_t *>(vs_at)[key * NG + (NG > 1 ? w : 0)];
-                                    if (j < S.first || j >= S.end) sc = 0;
-                                    const float step = step_of(sc) * norm, zero = fmaf(step_of(sc), MIDDLE, zero_of(sc));
-#pragma unroll
-                                    for (int x = 0; x < NT; ++x) {
-                                        const float p0 = p[h][x][2 * s], p1 = p[h][x][2 * s + 1];
-                                        zeros[x][NG > 1 ? w : 0][0] = fmaf(p0, zero, zeros[x][NG > 1 ? w : 0][0]);
-                                        zeros[x][NG > 1 ? w : 0][1] = fmaf(p1, zero, zeros[x][NG > 1 ? w : 0][1]);
-                                        y[0][x][s] = transposed(half2_of(p0 * step, p1 * step));
-                                        y[1][x][s] = transposed(half2_rest(p0 * step, p1 * step));
-                                    }
-                                }
-                            }
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {   // features 32 w + 4 g + 2 k and one more
                             uint32_t a[4];
@@ -746,11 +836,11 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
 #pragma unroll
                             for (int x = 0; x < NT; ++x) {
                                 if constexpr (!WIDE) {
-                                    mma_f16(o[x][2 * w + k], a[0], a[1], a[2], a[3], y[0][x][0], y[0][x][1]);
+                                    mma_f16(o[x][2 * w + k], a[0], a[1], a[2], a[3], y[NG > 1 ? w : 0][0][x][0], y[NG > 1 ? w : 0][0][x][1]);
                                 } else {
                                     float sum[4] = {};
 #pragma unroll
-                                    for (int part = 0; part < PARTS; ++part) mma_f16(sum, a[0], a[1], a[2], a[3], y[part][x][0], y[part][x][1]);
+                                    for (int part = 0; part < PARTS; ++part) mma_f16(sum, a[0], a[1], a[2], a[3], y[NG > 1 ? w : 0][part][x][0], y[NG > 1 ? w : 0][part][x][1]);
 #pragma unroll
                                     for (int e = 0; e < 4; ++e) o[x][2 * w + k][e] += sum[e];
                                 }
@@ -769,10 +859,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
         // row together.
         const uint32_t share_at = st * L::STAGE;
         float *share = reinterpret_cast<float *>(smem + share_at + warp * 8 * DP * 4);
-        const int power = top_scale + 1 - 127;
-        // two factors: either's exponent stays within 32 bits' range
-        const float unit = power_of_two(127 + power / 2), unit2 = power_of_two(127 + power - power / 2);
-        const float code = WIDE ? unit2 : unit2 * 16777216.f, code_upper = BITS == 4 && !WIDE ? code * 0.0625f : code;
+        constexpr float UNIT = WIDE ? 1.f : 16777216.f, UNIT_UPPER = BITS == 4 && !WIDE ? 1048576.f : UNIT;   // codes as half-precision numbers
         const bool all = stages == S.count;
         const long long part = ((long long)blockIdx.x * 2 + (stage0 == 0 ? 1 : 0)) * ROWS;
 #pragma unroll
@@ -781,26 +868,32 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
-                for (int d = 4; d < 32; d <<= 1) {
-                    l[x][e] += __shfl_xor_sync(0xffffffffu, l[x][e], d);
-                    if constexpr (WIDE)
+                for (int d = 4; d < 32; d <<= 1) l[x][e] += __shfl_xor_sync(0xffffffffu, l[x][e], d);
+                float back[NG], middle[NG];   // one over the norms; sums of p (zero + M step) less M sums of y
 #pragma unroll
-                        for (int k = 0; k < NG; ++k) zeros[x][k][e] += __shfl_xor_sync(0xffffffffu, zeros[x][k][e], d);
+                for (int k = 0; k < NG; ++k) {
+                    float lo, hi;
+                    unpack2(middles[x][NP == 1 ? 0 : e * (NP / 2) + k / 2], lo, hi);
+                    middle[k] = (NP == 1 ? e : k % 2) ? hi : lo;
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) middle[k] += __shfl_xor_sync(0xffffffffu, middle[k], d);
+                    back[k] = power_of_two(254 - (int)(__float_as_uint(norms[(8 * x + 2 * t + e) * NP + k]) >> 23));
                 }
-                if constexpr (!WIDE)   // row g of zero_sums is group g
+                if constexpr (!WIDE) {
 #pragma unroll
-                    for (int k = 0; k < NG; ++k) zeros[x][k][e] = __shfl_sync(0xffffffffu, zero_sums[x][e], 4 * k + t) * unit * unit2;
+                    for (int k = 0; k < NG; ++k) middle[k] = fmaf(__shfl_sync(0xffffffffu, ones[x][e], 4 * k + t) * -MIDDLE, back[k], middle[k]);
+                }
                 const int row = 2 * t + e;
                 if (row0 + 8 * x + row >= F.rows) continue;
                 if (g == 0) stats[warp * 8 + row] = make_float2(m[x][e], l[x][e]);
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
-                    const float z = zeros[x][NG > 1 ? w : 0][e];
+                    const float z = middle[NG > 1 ? w : 0], by = back[NG > 1 ? w : 0];
                     float4 v;
-                    v.x = fmaf(o[x][2 * w][e] * unit, code, z);
-                    v.y = fmaf(o[x][2 * w][2 + e] * unit, code_upper, z);
-                    v.z = fmaf(o[x][2 * w + 1][e] * unit, code, z);
-                    v.w = fmaf(o[x][2 * w + 1][2 + e] * unit, code_upper, z);
+                    v.x = fmaf(o[x][2 * w][e] * UNIT, by, z);
+                    v.y = fmaf(o[x][2 * w][2 + e] * UNIT_UPPER, by, z);
+                    v.z = fmaf(o[x][2 * w + 1][e] * UNIT, by, z);
+                    v.w = fmaf(o[x][2 * w + 1][2 + e] * UNIT_UPPER, by, z);
                     *reinterpret_cast<float4 *>(share + row * DP + 32 * w + 4 * g) = v;
                 }
             }
