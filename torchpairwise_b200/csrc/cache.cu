@@ -58,7 +58,7 @@ CacheAttnParams attention_params(const tpw_cache &c, const tpw_cache_attention_a
     P.Nq = a.Nq;
     P.Hq = a.Hq;
     P.group = a.Hq / c.H;
-    P.window = a.window;
+    P.window = a.window < c.capacity ? a.window : 0;   // a window over all keys is none: nothing is to be added to 2^63 - 1
     P.causal = a.causal;
     P.dtype = a.dtype;
     P.scale = a.scale;
