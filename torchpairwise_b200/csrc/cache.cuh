@@ -44,9 +44,10 @@ struct CacheAttnParams {
 // cache_rows.cu
 int cache_write(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s);
 int cache_read(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s);
-// what cache_attention.cu does beside: the highest magnitudes of kRangeParts parts of every head, [2, B, H, kRangeParts]
+// what cache_attention.cu does beside, for tokens from the block of 128 on that the last `last` (0: all) of a sequence begin in:
+// the highest magnitudes of kRangeParts parts of every head, [2, B, H, kRangeParts]
 constexpr int kRangeParts = 16;
-int cache_ranges(const CacheParams &P, uint32_t *highest, cudaStream_t s);
+int cache_ranges(const CacheParams &P, long long last, uint32_t *highest, cudaStream_t s);
 // every sequence's keys and values, those before the last `last` (0: none) and their block of 128 tokens left out, at [batch, token, head] strides of x;
 // what is not stored or left out is not written.  With `highest` each head's are brought below 2^bring by a power of two.
 int cache_expand(const CacheParams &P, int dtype, void *const (&x)[2], const int64_t (&stride)[3], long long last, const uint32_t *highest, const int (&bring)[2], cudaStream_t s);

@@ -113,8 +113,9 @@ int cache_attention(const CacheAttnParams &P, void *scratch, long long bytes, cu
         }
         const bool wide = P.dtype == TPW_BF16;
         uint32_t *highest = wide ? reinterpret_cast<uint32_t *>(S.range(scratch)) : nullptr;
-        int e = wide ? cache_ranges(c, highest, s) : TPW_OK;
-        if (e == TPW_OK) e = cache_expand(c, TPW_F16, {const_cast<void *>(a.k), const_cast<void *>(a.v)}, a.k_stride, P.window > 0 ? P.Nq - 1 + P.window : 0, highest, {kKeys, kValues}, s);
+        const long long last = P.window > 0 ? P.Nq - 1 + P.window : 0;   // what the first query sees, and the others on
+        int e = wide ? cache_ranges(c, last, highest, s) : TPW_OK;
+        if (e == TPW_OK) e = cache_expand(c, TPW_F16, {const_cast<void *>(a.k), const_cast<void *>(a.v)}, a.k_stride, last, highest, {kKeys, kValues}, s);
         if (e == TPW_OK && wide) {
             const int64_t stride[3] = {P.q_s[0], P.q_s[1], P.q_s[2]};
             e = cache_convert(false, static_cast<const unsigned char *>(P.q) + first * P.q_s[0] * 2, const_cast<void *>(a.q), stride, highest, kKeys, count, P.Nq, P.Hq, P.c.H, P.c.D, s);

@@ -90,16 +90,20 @@ __device__ __forceinline__ float bring_by(const uint32_t *parts, int to) {
     const int e = to - exponent_of(parts) + 127;
     return __uint_as_float((uint32_t)(e < 1 ? 1 : e > 254 ? 254 : e) << 23);
 }
-// the highest magnitude that the codes of a part of a head's keys (or values) can stand for; groups that are not numbers take no part
-__global__ void __launch_bounds__(256) cache_ranges_kernel(const CacheParams P, uint32_t *highest) {
+// The first position of a sequence of `end` stored tokens that counts where only the last `last` (0: all) do: that of their first block of 128
+__device__ __forceinline__ int first_of(int end, int last) { return last > 0 && end > last ? (end - last) & ~127 : 0; }
+// the highest magnitude that the codes of a part of a head's keys (or values), those before first_of left out, can stand for; groups that are not numbers take no part
+__global__ void __launch_bounds__(256) cache_ranges_kernel(const CacheParams P, int last, uint32_t *highest) {
     const long long bh = blockIdx.y;
     const int which = blockIdx.z, b = (int)(bh / P.H), cap = (int)P.capacity;
     int n = P.lengths[b];
     n = n < 0 ? 0 : n < cap ? n : cap;
-    const uint32_t *scales = P.scales[which] + bh * cap * P.groups;
+    const int first = first_of(n, last);
+    const uint32_t *scales = P.scales[which] + (bh * cap + first) * P.groups;
+    const long long count = (long long)(n - first) * P.groups;
     const float most = P.bits == 4 ? 15.f : 255.f;
     uint32_t top = 0;
-    for (int at = blockIdx.x * 256 + threadIdx.x; at < n * P.groups; at += kRangeParts * 256) {
+    for (long long at = blockIdx.x * 256 + threadIdx.x; at < count; at += kRangeParts * 256) {
         const float zero = zero_of(scales[at]), end = fmaf(step_of(scales[at]), most, zero), high = fmaxf(fabsf(zero), fabsf(end));
         if (fabsf(zero) <= high && high < 5.0706024009129176e30f) top = max(top, __float_as_uint(high));   // 2^102
     }
@@ -266,7 +270,7 @@ __global__ void __launch_bounds__(4 * kReadTokens) cache_read_kernel(const RowsP
     constexpr int WORDS = W * BITS / 4;
     const int which = blockIdx.y, l = threadIdx.x & 3;
     const Block<kReadTokens> B(R, threadIdx.x >> 2);
-    const int first = R.last > 0 && B.end > R.last ? (B.end - R.last) & ~127 : 0;   // positions before it are left
+    const int first = first_of(B.end, R.last);   // positions before it are left
     const bool there = B.i0 < R.N && B.stored(B.i0) && B.i0 + B.shift >= first;
     if (R.leave ? !there : B.i0 >= R.N) return;
     uint32_t w[WORDS] = {}, scales[W] = {};
@@ -371,9 +375,9 @@ int cache_read(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s)
     return run(rows.dtype, R, false, s);
 }
 
-int cache_ranges(const CacheParams &P, uint32_t *highest, cudaStream_t s) {
+int cache_ranges(const CacheParams &P, long long last, uint32_t *highest, cudaStream_t s) {
     TPW_CHECK_ARG(P.B * P.H < 65536, "tpw_cache_attention: more than 65535 heads of a slice");
-    cache_ranges_kernel<<<dim3(kRangeParts, (unsigned)(P.B * P.H), 2), 256, 0, s>>>(P, highest);
+    cache_ranges_kernel<<<dim3(kRangeParts, (unsigned)(P.B * P.H), 2), 256, 0, s>>>(P, (int)(last < P.capacity ? last : 0), highest);
     TPW_LAUNCH_OK("cache_ranges_kernel");
     return TPW_OK;
 }
