@@ -655,7 +655,7 @@ TPW_API int tpw_rotary_table(const double *frequency, double magnitude, float *c
  * Keys and values of a token and head are cut into groups: of 32 features (groups = ceil(D / 32)), or the whole head (groups = 1).  Of a group
  *   zero = the largest bfloat16 number that is not above its lowest value,
  *   step = the smallest bfloat16 number, 2^-100 at least, of which 2^bits - 1 reach from the zero to its highest value,
- *   code = the nearest whole number to (x - zero) / step, ties to even (16-bit values: x - zero as it is in 32 bits),
+ *   code = the nearest whole number to (x - zero) / step, ties to even (of float32 values: to the quotient in 64 bits),
  * and a code stands for zero + step * code, which is at most half a step from x.  A group with a value that is not finite, or 2^100 or
  * more in magnitude, has NaN for its zero and step and reads as NaN.
  *

@@ -1,13 +1,26 @@
 """Calls of the quantised cache that its documentation allows and that once went wrong: each against what it means."""
+from fractions import Fraction
+
 import pytest
 import torch
 
 import torchpairwise_b200 as tpw
 from attention_cases import assert_near
-from cache_cases import attended, filled
+from cache_cases import attended, filled, unpacked
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def below(x):
+    """The bfloat16 number before a positive one."""
+    return float((torch.tensor(x).bfloat16().view(torch.int16) - 1).view(torch.bfloat16))
+
+
+def above(x):
+    """The bfloat16 number after x."""
+    bits = torch.tensor(x).bfloat16().view(torch.int16)
+    return 2.0 ** -133 if x == 0 else float((bits + (1 if x > 0 else -1)).view(torch.bfloat16))
 
 
 def ints(*n):
@@ -46,3 +59,57 @@ def test_large_finite_numbers_that_no_query_sees(dtype, queries):
                 scales[b, :, part] = 2.0 ** 60
     got = tpw.cache_attention(q, tpw.QuantizedCache(*loud, 64, 4), n, causal=True, window=window, return_lse=True)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("group", [32, None])
+def test_16_bit_values_whose_distance_from_the_zero_has_many_digits(dtype, bits, group):
+    """Groups from a zero far below (or far above) the size of a value that lies on a middle but for it: the code is the nearest one in real arithmetic."""
+    most = 2 ** bits - 1
+    rows = []
+    for small in (2.0 ** -14, 2.0 ** -17, 2.0 ** -20, 2.0 ** -24, 2.0 ** -30, 2.0 ** -40, 2.0 ** -90):
+        for sign in (1, -1):
+            # from -small (or small) to most, steps of about 1: middles stand at (c + 1/2) steps
+            for step in (1.0, 1.0078125, 0.5, 4.0, 1.5):
+                row = [sign * small, step * most] + [(c + 0.5) * step for c in range(most if bits == 4 else 24)]
+                rows.append((row + [step] * 32)[:32])
+            # a zero that is large beside values near 0
+            for zero in (-1.0, -3.0, -7.0, -0.5):
+                step = 2.0 if bits == 4 else 0.125
+                rows.append(([zero, zero + most * step] + [sign * small * 2.0 ** -k for k in range(30)])[:32])
+    x = torch.tensor(rows, dtype=torch.float64).to(dtype)
+    assert torch.isfinite(x).all()
+    x = torch.cat((x, x.flip(0)), 1)[None, :, None].cuda()
+    n = x.shape[1]
+    cache = tpw.quantized_cache(1, n, 1, 64, bits=bits, group=group)
+    tpw.cache_write(cache, x, x, ints(n))
+    # 64 bits do not hold all of these differences either: rational numbers do
+    for code, step, zero in unpacked(cache):
+        for i in range(n):
+            for first in range(0, 64, group or 64):
+                part = [Fraction(v) for v in x[0, i, 0, first:first + (group or 64)].double().tolist()]
+                s, z = Fraction(float(step[0, 0, i, first])), Fraction(float(zero[0, 0, i, first]))
+                assert z <= min(part) and z + most * s >= max(part)
+                assert z + most * Fraction(below(float(s))) < max(part) and Fraction(above(float(z))) > min(part)   # the smallest and the largest that do
+                assert code[0, 0, i, first:first + len(part)].tolist() == [round((v - z) / s) for v in part]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("bits", [4, 8])
+def test_codes_of_16_bit_values_of_any_magnitude(dtype, bits):
+    g = torch.Generator().manual_seed(34)
+    top, most = 14 if dtype == torch.float16 else 90, 2 ** bits - 1
+    n = 4096
+    x = torch.randn(1, n, 2, 64, generator=g) * torch.exp2(torch.randint(-24 if dtype == torch.float16 else -90, top, (1, n, 2, 64), generator=g))
+    x = x.to(dtype).cuda()
+    cache = tpw.quantized_cache(1, n, 2, 64, bits=bits)
+    tpw.cache_write(cache, x, x, ints(n))
+    for code, step, zero in unpacked(cache):
+        real = x.transpose(1, 2).double()
+        for i, h, f in torch.randint(0, 64, (6000, 3), generator=g).tolist():
+            i, h, first = 64 * f + i, h % 2, f // 32 * 32
+            part = [Fraction(v) for v in real[0, h, i, first:first + 32].tolist()]
+            s, z = Fraction(float(step[0, h, i, first])), Fraction(float(zero[0, h, i, first]))
+            assert z <= min(part) and z + most * s >= max(part)
+            assert code[0, h, i, first:first + 32].tolist() == [round((v - z) / s) for v in part]

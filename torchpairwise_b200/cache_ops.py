@@ -50,7 +50,7 @@ class QuantizedCache(NamedTuple):
 
     A group of features (32, or the whole head) of a token has a zero, the largest bfloat16 number that is not above its lowest value, and
     a step, the smallest bfloat16 number (2^-100 at least) of which ``2**bits - 1`` reach from the zero to its highest value.  A value is
-    held as the nearest whole number of steps above the zero, ties to even, and reads as ``zero + step * code``, at most half a step off.
+    held as the nearest whole number of steps above the zero, ties to even (float32: nearest to the quotient in 64 bits), and reads as ``zero + step * code``, at most half a step off.
 
     ``k_codes`` and ``v_codes`` are uint8 ``[batch, heads, capacity, bytes of a row]``, ``k_scales`` and ``v_scales`` bfloat16
     ``[batch, heads, capacity, groups, 2]``, step and zero; all contiguous, the capacity a multiple of 64.  A row has ``W * 32``

@@ -2,7 +2,7 @@
 //
 // Bound by HBM on paper, by issue in fact: storing takes about 16 instructions a value.  What keeps them few: a lane has a group's 32 values, quotients are refined on the FMA
 // pipes (a test for middles on the logic pipe was 10 more), codes are added up above a constant instead of masked and shifted, and bytes become numbers by
-// permutation.  Measured bfloat16, 4 bits: 2 x 8192 tokens of 8 heads of 128, 67 MB stored and read back in 41 us; 4 x 16384 ragged read in 53 us, 5.9 TB/s.
+// permutation.  Measured bfloat16, 4 bits: 2 x 8192 tokens of 8 heads of 128, 67 MB stored and read back in 43 us; 4 x 16384 ragged read in 53 us, 5.9 TB/s.
 #include "attention_tc.cuh"
 #include "cache.cuh"
 
@@ -183,6 +183,12 @@ template <int BITS> __device__ __forceinline__ void pack8(uint32_t (&w)[2], cons
 // Apart, so that 32 rare divisions do not lie between the others' instructions ([3, 1777, 12, 80] stored and read: 35 -> 33 us)
 __device__ __noinline__ float code_in_64_bits(float x, float zero, float step) { return (float)rint(((double)x - (double)zero) / (double)step); }
 
+// x - zero rounded to odd: where 32 bits do not hold it, that neighbour whose last bit is set, so that it lies on the true side of any number of 23 bits or fewer
+__device__ __forceinline__ float distance(float x, float zero) {
+    const uint32_t below = __float_as_uint(__fsub_rz(x, zero)), above = __float_as_uint(__fsub_ru(x, zero));   // x is not below the zero
+    return __uint_as_float(below | ((below ^ above) & 1u));
+}
+
 // A lane has 32 features of a token, so that what a group's step costs is paid once; 2 or 4 lanes a token.
 template <typename T, int BITS, int W>
 __global__ void __launch_bounds__(kWriteTokens * (W == 2 ? 2 : 4)) cache_write_kernel(const RowsParams R) {
@@ -234,12 +240,14 @@ __global__ void __launch_bounds__(kWriteTokens * (W == 2 ? 2 : 4)) cache_write_k
     unsigned char *to = R.c.codes[which] + place * (W * 4 * BITS);
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
-        // The quotient, refined by what is left of it, exactly: a middle between two codes comes out as that.  A sum with 1.5 * 2^23 ends in the
-        // nearest whole number, ties to even.
+        // The quotient, refined by what is left of it, exactly: it is off by half a unit and 2^-45 of itself at most, and a middle between two codes comes out as
+        // that.  A sum with 1.5 * 2^23 ends in the nearest whole number, ties to even.  What 16-bit values lie on a middle but for lies too far down for 32 bits, but decides
+        // (1 less -2^-40): their distances are rounded to odd.  A middle times the step has 17 bits at most, a distance of 24 bits beside it differs by one of its last places, which
+        // is more than the quotient is off.  (A distance that is all ones lies beside a power of two; then the step is one too, and the quotient exact.)  2 x 8192 tokens: 41 -> 43 us.
         float y[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const float d = __fsub_rn(x[v][k], zero), near = __fmul_rn(d, inv);
+            const float d = sizeof(T) == 4 ? __fsub_rn(x[v][k], zero) : distance(x[v][k], zero), near = __fmul_rn(d, inv);
             const float quotient = fmaf(fmaf(-near, step, d), inv, near);
             y[k] = __fadd_rn(quotient, 12582912.f);
             // float32 values have digits that their distance from the zero has not: beside a middle 64 bits decide.  The distance and the quotient are
