@@ -244,19 +244,21 @@ __global__ void __launch_bounds__(kWriteTokens * (W == 2 ? 2 : 4)) cache_write_k
         // that.  A sum with 1.5 * 2^23 ends in the nearest whole number, ties to even.  What 16-bit values lie on a middle but for lies too far down for 32 bits, but decides
         // (1 less -2^-40): their distances are rounded to odd.  A middle times the step has 17 bits at most, a distance of 24 bits beside it differs by one of its last places, which
         // is more than the quotient is off.  (A distance that is all ones lies beside a power of two; then the step is one too, and the quotient exact.)  2 x 8192 tokens: 41 -> 43 us.
-        float y[8];
+        uint32_t code[2] = {0, 0};
+        if (live && 8 * v < n) {   // pieces beyond the head have no values
+            float y[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float d = sizeof(T) == 4 ? __fsub_rn(x[v][k], zero) : distance(x[v][k], zero), near = __fmul_rn(d, inv);
-            const float quotient = fmaf(fmaf(-near, step, d), inv, near);
-            y[k] = __fadd_rn(quotient, 12582912.f);
-            // float32 values have digits that their distance from the zero has not: beside a middle 64 bits decide.  The distance and the quotient are
-            // each off by 2^-24 and 2^-23 of at most MOST codes, 1.8e-7.
-            if (sizeof(T) == 4 && fabsf(quotient - (y[k] - 12582912.f)) > 0.5f - MOST * 2.4e-7f)
-                y[k] = 12582912.f + code_in_64_bits(x[v][k], zero, step);
+            for (int k = 0; k < 8; ++k) {
+                const float d = sizeof(T) == 4 ? __fsub_rn(x[v][k], zero) : distance(x[v][k], zero), near = __fmul_rn(d, inv);
+                const float quotient = fmaf(fmaf(-near, step, d), inv, near);
+                y[k] = __fadd_rn(quotient, 12582912.f);
+                // float32 values have digits that their distance from the zero has not: beside a middle 64 bits decide.  The distance and the quotient are
+                // each off by 2^-24 and 2^-23 of at most MOST codes, 1.8e-7.
+                if (sizeof(T) == 4 && fabsf(quotient - (y[k] - 12582912.f)) > 0.5f - MOST * 2.4e-7f)
+                    y[k] = 12582912.f + code_in_64_bits(x[v][k], zero, step);
+            }
+            pack8<BITS>(code, y, fine ? n - 8 * v : 0);
         }
-        uint32_t code[2];
-        pack8<BITS>(code, y, live && fine ? n - 8 * v : 0);
         const int l = 4 * w + v;
         if (which == 0) {
             if (BITS == 4) *reinterpret_cast<uint32_t *>(to + key_place<BITS, W>(l)) = code[0];
