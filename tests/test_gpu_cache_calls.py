@@ -113,3 +113,18 @@ def test_codes_of_16_bit_values_of_any_magnitude(dtype, bits):
             s, z = Fraction(float(step[0, h, i, first])), Fraction(float(zero[0, h, i, first]))
             assert z <= min(part) and z + most * s >= max(part)
             assert code[0, h, i, first:first + 32].tolist() == [round((v - z) / s) for v in part]
+
+
+def test_tensors_that_are_negated_when_they_are_read():
+    """torch._neg_view: a tensor whose sign waits in a flag, contiguous or not."""
+    g = torch.Generator().manual_seed(35)
+    k, v = (torch.randn(2, 9, 2, 64, generator=g).cuda() for _ in range(2))
+    n = ints(9, 20)
+    got, want = (tpw.quantized_cache(2, 64, 2, 64) for _ in range(2))
+    tpw.cache_write(want, -k, -v, n)
+    tpw.cache_write(got, torch._neg_view(k), torch._neg_view(v.transpose(1, 2).contiguous().transpose(1, 2)), n)
+    assert all(torch.equal(a, b) for a, b in zip(got[:4], want[:4]))
+    for queries in (1, 300):
+        q = torch.randn(2, queries, 4, 64, generator=g).half().cuda()
+        assert torch.equal(tpw.cache_attention(torch._neg_view(q), want, n), tpw.cache_attention(-q, want, n))
+    assert torch.equal(tpw.cache_read(want, torch._neg_view(-n))[0], tpw.cache_read(want, n)[0])

@@ -53,10 +53,14 @@ Tensor fresh(at::IntArrayRef sizes, const Tensor &like, at::ScalarType type) {
 }
 
 // A view whose features lie side by side, with strides that are read as they are; anything else is copied.
-Tensor laid_out(const Tensor &x) { return x.is_neg() || (x.size(3) != 1 && x.stride(3) != 1) ? x.contiguous() : x; }
+Tensor laid_out(const Tensor &x_) {
+    const Tensor x = x_.resolve_neg();
+    return x.size(3) != 1 && x.stride(3) != 1 ? x.contiguous() : x;
+}
 // Queries: many of them go through attention's tensor-core kernels, which fetch 16-bit rows in pieces of 16 bytes and take no broadcast dimensions
-Tensor laid_out_queries(const Tensor &x) {
-    bool fits = !x.is_neg() && (x.size(3) == 1 || x.stride(3) == 1);
+Tensor laid_out_queries(const Tensor &x_) {
+    const Tensor x = x_.resolve_neg();
+    bool fits = x.size(3) == 1 || x.stride(3) == 1;
     for (int d = 0; d < 3; ++d) fits = fits && (x.size(d) == 1 || x.stride(d) > 0);
     if (fits && x.element_size() == 2 && x.size(3) % 8 == 0) {
         fits = reinterpret_cast<uintptr_t>(x.const_data_ptr()) % 16 == 0;
@@ -101,7 +105,7 @@ struct Cache {
         TORCH_CHECK(key_lengths.scalar_type() == at::kInt || key_lengths.scalar_type() == at::kLong, "key_lengths must be int32 or int64, got ", key_lengths.scalar_type());
         TORCH_CHECK(key_lengths.dim() == 1 && key_lengths.size(0) == k_codes.size(0), "key_lengths must hold one length for each of the ", k_codes.size(0), " sequences. Got shape ",
                     key_lengths.sizes());
-        lengths = key_lengths.scalar_type() == at::kInt ? key_lengths.contiguous() : key_lengths.clamp(-1, int64_t(1) << 30).to(at::kInt).contiguous();
+        lengths = key_lengths.scalar_type() == at::kInt ? key_lengths.resolve_neg().contiguous() : key_lengths.clamp(-1, int64_t(1) << 30).to(at::kInt).contiguous();
         c.bits = (int32_t)bits;
         c.groups = (int32_t)k_scales.size(3);
         c.B = k_codes.size(0); c.H = k_codes.size(1); c.capacity = k_codes.size(2); c.D = features;
