@@ -128,3 +128,14 @@ def test_tensors_that_are_negated_when_they_are_read():
         q = torch.randn(2, queries, 4, 64, generator=g).half().cuda()
         assert torch.equal(tpw.cache_attention(torch._neg_view(q), want, n), tpw.cache_attention(-q, want, n))
     assert torch.equal(tpw.cache_read(want, torch._neg_view(-n))[0], tpw.cache_read(want, n)[0])
+
+
+def test_lengths_far_beyond_32_bits_with_very_many_tokens():
+    """Nearly 2^30 tokens (one row, repeated by its strides) of a sequence of 2^40: the last ones stand far beyond the capacity, none is stored."""
+    cache = tpw.quantized_cache(1, 64, 1, 8)
+    x = torch.ones(1, 1, 1, 8, device="cuda").expand(1, 2 ** 30 - 1, 1, 8)
+    for n in (torch.tensor([2 ** 40], device="cuda"), torch.tensor([2 ** 62], device="cuda"), ints(2 ** 31 - 1)):
+        tpw.cache_write(cache, x, x, n)
+        assert not any(bool(t.any()) for t in cache[:4])
+    tpw.cache_write(cache, x, x, torch.tensor([2 ** 30 - 1], device="cuda"))   # from position 0 on: the first 64 have a place
+    assert bool((tpw.cache_read(cache, ints(64), dtype=torch.float32)[0] == 1).all())

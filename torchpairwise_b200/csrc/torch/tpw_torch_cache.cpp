@@ -105,7 +105,7 @@ struct Cache {
         TORCH_CHECK(key_lengths.scalar_type() == at::kInt || key_lengths.scalar_type() == at::kLong, "key_lengths must be int32 or int64, got ", key_lengths.scalar_type());
         TORCH_CHECK(key_lengths.dim() == 1 && key_lengths.size(0) == k_codes.size(0), "key_lengths must hold one length for each of the ", k_codes.size(0), " sequences. Got shape ",
                     key_lengths.sizes());
-        lengths = key_lengths.scalar_type() == at::kInt ? key_lengths.resolve_neg().contiguous() : key_lengths.clamp(-1, int64_t(1) << 30).to(at::kInt).contiguous();
+        lengths = key_lengths.scalar_type() == at::kInt ? key_lengths.resolve_neg().contiguous() : key_lengths.clamp(-1, INT32_MAX).to(at::kInt).contiguous();
         c.bits = (int32_t)bits;
         c.groups = (int32_t)k_scales.size(3);
         c.B = k_codes.size(0); c.H = k_codes.size(1); c.capacity = k_codes.size(2); c.D = features;
