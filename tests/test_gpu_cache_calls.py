@@ -139,3 +139,20 @@ def test_lengths_far_beyond_32_bits_with_very_many_tokens():
         assert not any(bool(t.any()) for t in cache[:4])
     tpw.cache_write(cache, x, x, torch.tensor([2 ** 30 - 1], device="cuda"))   # from position 0 on: the first 64 have a place
     assert bool((tpw.cache_read(cache, ints(64), dtype=torch.float32)[0] == 1).all())
+
+
+def test_a_cache_that_wants_gradients_is_refused():
+    """Steps and zeros are 16-bit floating-point tensors: as parameters they would silently get none."""
+    cache = filled(1, 64, 1, 64, 4, 32, seed=36)
+    x, q, n = torch.zeros(1, 3, 1, 64, device="cuda"), torch.zeros(1, 1, 1, 64, device="cuda"), ints(3)
+    before = [t.clone() for t in cache[:4]]
+    for name in ("k_scales", "v_scales"):
+        wants = cache._replace(**{name: getattr(cache, name).requires_grad_()})
+        for call in (lambda: tpw.cache_read(wants, n), lambda: tpw.cache_attention(q, wants, n), lambda: tpw.cache_write(wants, x, x, n)):
+            with pytest.raises(RuntimeError, match="gradient"):
+                call()
+        with torch.no_grad():
+            tpw.cache_read(wants, n)
+            tpw.cache_attention(q, wants, n)
+        getattr(cache, name).requires_grad_(False)
+    assert all(torch.equal(a, b) for a, b in zip(cache[:4], before))

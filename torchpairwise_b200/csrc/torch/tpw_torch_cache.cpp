@@ -95,6 +95,7 @@ struct Cache {
             TORCH_CHECK(t->scalar_type() == at::kBFloat16 && t->dim() == 5 && t->size(0) == k_codes.size(0) && t->size(1) == k_codes.size(1) && t->size(2) == k_codes.size(2) &&
                             (t->size(3) == 1 || t->size(3) == groups) && t->size(4) == 2 && t->size(3) == k_scales.size(3),
                         name, ": scales must be bfloat16 [batch, heads, capacity, 1 or ", groups, ", 2], alike for keys and values. Got ", t->scalar_type(), " ", t->sizes());
+            no_gradient(name, *t);
         }
         const Tensor *all[4] = {&k_codes, &v_codes, &k_scales, &v_scales};
         for (int i = 0; i < 4; ++i) {
