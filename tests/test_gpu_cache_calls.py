@@ -156,3 +156,21 @@ def test_a_cache_that_wants_gradients_is_refused():
             tpw.cache_attention(q, wants, n)
         getattr(cache, name).requires_grad_(False)
     assert all(torch.equal(a, b) for a, b in zip(cache[:4], before))
+
+
+def test_a_cache_of_inference_mode():
+    """Made under torch.inference_mode: written, read and attended to there; outside it is read, and a write is refused before it happens."""
+    x, q, n = torch.ones(1, 3, 1, 64, device="cuda"), torch.ones(1, 1, 1, 64, device="cuda"), ints(3)
+    with torch.inference_mode():
+        cache = tpw.quantized_cache(1, 64, 1, 64)
+        tpw.cache_write(cache, x, x, n)
+        inside = tpw.cache_attention(q, cache, n)
+    assert torch.equal(tpw.cache_attention(q, cache, n), inside) and bool((tpw.cache_read(cache, n)[1][:, :3] == 1).all())
+    with torch.no_grad(), pytest.raises(RuntimeError, match="inference"):
+        tpw.cache_write(cache, 2 * x, 2 * x, n)
+    assert bool((tpw.cache_read(cache, n)[1][:, :3] == 1).all())
+    # an ordinary cache may be written there
+    cache = tpw.quantized_cache(1, 64, 1, 64)
+    with torch.inference_mode():
+        tpw.cache_write(cache, x, x, n)
+    assert torch.equal(tpw.cache_attention(q, cache, n), inside)

@@ -140,8 +140,9 @@ void cache_write(const Tensor &k_codes, const Tensor &v_codes, const Tensor &k_s
         strides_of(x[w], a.stride[w]);
     }
     a.N = k.size(1);
-    TPW_CALL(tpw_cache_write(&cache.c, &a, stream_of(k_codes)));
+    // refuses tensors of inference mode outside of it: before anything is written
     for (const Tensor *t : {&k_codes, &v_codes, &k_scales, &v_scales}) t->unsafeGetTensorImpl()->bump_version();
+    TPW_CALL(tpw_cache_write(&cache.c, &a, stream_of(k_codes)));
 }
 
 std::tuple<Tensor, Tensor> cache_read(const Tensor &k_codes, const Tensor &v_codes, const Tensor &k_scales, const Tensor &v_scales, int64_t features, int64_t bits,
