@@ -121,3 +121,19 @@ def test_constant_tokens_and_storage_that_was_never_written(dtype):
     n = n.fill_(130)
     out = tpw.cache_attention(q, cache, n)
     assert_near(out, attended(q, cache, n.tolist())[0], dtype, "constant values")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("queries", [1, 4, 20])
+@pytest.mark.parametrize("bits,group", [(4, 32), (4, None), (8, 32)])
+def test_keys_far_from_zero_and_queries_whose_groups_cancel(dtype, queries, bits, group):
+    """Scores are held in 32 bits, the sums of a group's queries that meet its zero among them: terms of about 50 * 32 that cancel, of which four truncations
+    leave 2^-22, 3e-5 of a score after its scale; log-sums are about 40, so that 2^-19 of them (8e-5) is twice that."""
+    q, k, v, n, cache = scene(3, queries, bits=bits, group=group)
+    q = q / 2
+    q[..., :32] += 1
+    q[..., 32:64] -= 1
+    stored(cache, k + 50, v)
+    q = q.to(dtype)
+    lse = tpw.cache_attention(q, cache, n, return_lse=True)[1]
+    assert_near(lse, attended(q, cache, n.tolist())[1], torch.float32, "lse", times=0.25)

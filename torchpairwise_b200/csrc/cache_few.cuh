@@ -4,8 +4,9 @@
 // them.  So the codes go into the products as they are: as the low bits of half-precision numbers they are whole multiples of 2^-24,
 // exactly, and masks are all the unpacking there is.
 //   scores   K q^T, m16n8k16, 16 keys by 8 query rows: sum_g step_jg (sum_d c_jd q_d) + zero_jg a_g, a_g = sum_d q_d over the group.  The second
-//            term is a product of its own, bfloat16: a word of the cache, step and zero, is the operand, beside 0 and a_g.  A row of q is
-//            lifted by a power of two to half precision's upper end.
+//            term is a product of its own, bfloat16: words of the cache, step and zero, are the operand, beside 0 (or M a_g, below) and a_g in four parts,
+//            32 bits (two parts left 2^-17 of every term: log-sums of keys far from zero were off by 1e-5).  A row of q is lifted by a power of two to half
+//            precision's upper end.
 //   output   V^T P^T, 16 features by 8 rows: the steps go into the probabilities, y_jg = p_j step_jg, formed in 32 bits and rounded to half precision
 //            once: sum_j y_jg (c_jd - M) + p_j (zero_jg + M step_jg), M the middle code, so that a rounding counts by how far a value is from its group's
 //            middle.  The second term stays in 32 bits; M sum_j y_jg comes from a product with ones.
@@ -288,6 +289,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
     constexpr bool WIDE = PARTS == 2;
     constexpr float MIDDLE = BITS == 4 ? 8.f : 128.f;
     constexpr bool SMALL = WIDE || NG == 1 || BITS == 8;   // sums of scores begin at -M a_g
+    constexpr int ZEROS = NG > 2 && SMALL ? 2 : 1;                 // products that zeros take
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ unsigned room[kFewWarps + 2];
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_FLAG);
@@ -464,7 +466,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
         }
         __syncthreads();
         if (warp == 0 && used == 0) fill(L::kStages);
-        uint32_t q[PARTS][NT][W][2][2], qz[NT][PARTS][2];
+        uint32_t q[PARTS][NT][W][2][2], qz[NT][ZEROS][2];
         float start[NT][NG][4], factor[NT][2];   // -M a_g (SMALL); raw scores times the factor are powers of 2
         int all_lo = S.first, all_hi = S.end;   // keys that all rows see
         auto sees = [&](int x, int e, int &lo, int &hi) {   // those of a row
@@ -487,16 +489,34 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                     q[part][x][w][0][0] = v.x; q[part][x][w][0][1] = v.y;
                     q[part][x][w][1][0] = v.z; q[part][x][w][1][1] = v.w;
                 }
-            float own = 0.f;   // a of row g, group t, in parts of 8 bits beside M times it
-            if (NG > 1) own = t < NG ? sums[t * 8 + g] : 0.f;
-            else if (t == 0)
+            // a of row g in four bfloat16 parts, beside M times it, as the K of a product has room for them: four lanes' pairs, twice.  One group: a part to a
+            // lane.  Two: a group and part to a lane, twice.  More: a group to a lane, and two parts in a word where M is not wanted, else two products.
+            float own = 0.f, a[4];
+            if (NG > 1) own = (t & (NG == 2 ? 1 : 3)) < NG ? sums[(NG == 2 ? t & 1 : t) * 8 + g] : 0.f;
+            else
 #pragma unroll
                 for (int w = 0; w < W; ++w) own += sums[w * 8 + g];
 #pragma unroll
-            for (int part = 0; part < 2 * PARTS; ++part) {
-                const uint32_t word = Narrow<__nv_bfloat16>::pack(SMALL ? own * MIDDLE : 0.f, own);
-                qz[x][part / 2][part % 2] = word;
-                own -= __uint_as_float(word & 0xffff0000u);
+            for (int part = 0; part < 4; ++part) {
+                a[part] = __uint_as_float(Narrow<__nv_bfloat16>::pack(0.f, own) & 0xffff0000u);
+                own -= a[part];
+            }
+            auto word = [&](float part) { return Narrow<__nv_bfloat16>::pack(SMALL ? part * MIDDLE : 0.f, part); };
+            if constexpr (NG == 1) {
+                qz[x][0][0] = word(t == 0 ? a[0] : t == 1 ? a[1] : t == 2 ? a[2] : a[3]);
+                qz[x][0][1] = 0;
+            } else if constexpr (NG == 2) {
+                qz[x][0][0] = word(t < 2 ? a[0] : a[1]);
+                qz[x][0][1] = word(t < 2 ? a[2] : a[3]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    if constexpr (ZEROS == 1) qz[x][0][k] = Narrow<__nv_bfloat16>::pack(a[2 * k], a[2 * k + 1]);
+                    else {
+                        qz[x][k][0] = word(a[2 * k]);
+                        qz[x][k][1] = word(a[2 * k + 1]);
+                    }
+                }
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -553,15 +573,14 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                         const int key = 16 * h + 8 * s + slot0;
                         load_words(kw[s], k_at + key * L::ROW + t * (W * BITS));
                         load_words(ks[s], ks_at + key * NG * 4);
-                        kz[s] = t < NG ? reinterpret_cast<const uint32_t *>(ks_at)[key * NG + (t < NG ? t : 0)] : 0u;
+                        kz[s] = reinterpret_cast<const uint32_t *>(ks_at)[key * NG + (NG == 1 ? 0 : NG == 2 ? t & 1 : t < NG ? t : 0)];
+                        if (NG == 3 && t == 3) kz[s] = 0;
+                        if (NG > 2 && ZEROS == 1) kz[s] = __byte_perm(kz[s], kz[s], 0x3232);   // the zero twice
                     }
 #pragma unroll
                     for (int x = 0; x < NT; ++x) {
-#pragma unroll
-                        for (int part = 0; part < PARTS; ++part) {
-                            if (part == 0) mma_bf16_new(p[h][x], kz[0], kz[1], kz[0], kz[1], qz[x][part][0], qz[x][part][1]);
-                            else mma_bf16(p[h][x], kz[0], kz[1], kz[0], kz[1], qz[x][part][0], qz[x][part][1]);
-                        }
+                        mma_bf16_new(p[h][x], kz[0], kz[1], kz[0], kz[1], qz[x][0][0], qz[x][0][1]);
+                        if constexpr (ZEROS == 2) mma_bf16(p[h][x], kz[0], kz[1], kz[0], kz[1], qz[x][1][0], qz[x][1][1]);
                     }
                     float acc[NT][4];
 #pragma unroll
