@@ -137,3 +137,18 @@ def test_keys_far_from_zero_and_queries_whose_groups_cancel(dtype, queries, bits
     q = q.to(dtype)
     lse = tpw.cache_attention(q, cache, n, return_lse=True)[1]
     assert_near(lse, attended(q, cache, n.tolist())[1], torch.float32, "lse", times=0.25)
+
+
+@pytest.mark.parametrize("queries", [1, 7, 100])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("group", [32, None])
+def test_float32_scores_of_some_size_keep_their_digits(queries, bits, group):
+    """Scores up to about 30, of which float32 sums leave some 2^-24 a term: 128 of them, about 1 each, 2^-20 of a probability; the bound is 8 times that."""
+    q, k, v, n, cache = scene(4, queries, bits=bits, group=group)
+    loud = 1 + 4 * (torch.rand(128, generator=torch.Generator().manual_seed(5)) < 0.06).cuda()
+    stored(cache, k * loud, v)
+    q = 2 * q
+    out, lse = tpw.cache_attention(q, cache, n, causal=True, return_lse=True)
+    want = attended(q, cache, n.tolist(), causal=True)
+    assert_near(out, want[0], torch.float32, "out")
+    assert_near(lse, want[1], torch.float32, "lse", times=0.125)

@@ -15,10 +15,11 @@
 // other rows, nor on tokens that it gives no weight.  Norms move where references do, or where a step is far above those met.
 // With keys along M a product has 8 rows of queries; rows along M would leave half of every product empty for up to 8 heads that share a key.
 //
-// Tensor-core sums truncate, so they are kept small: those of scores begin at -M a_g, M the middle code, with zero_jg + M step_jg in the second term.  (Not
+// Tensor-core sums truncate, so they are kept small: those of scores are of codes less M, or begin at -M a_g, with zero_jg + M step_jg in the second term.  (Not
 // for 4-bit groups of 32 and 16-bit queries: 32 codes below 16 add up to little, and the beginnings would cost 16 registers of the 168 that three CTAs an SM
-// leave, 51.3 -> 49.7 us without.)  Float32 queries: q and y as two half-precision parts each, 22 bits; codes of values less M, and the products of 16 keys
-// go to sums in registers.
+// leave, 51.3 -> 49.7 us without.)  Float32 queries: q and y as two half-precision parts each, what those leave is below 2^-23;
+// codes less M as numbers, since the products of 4-bit codes below 2^-20 are lined up as if they were 2^-14 and lose 6 digits (errors of results 6e-6 -> 6e-7, no time), and the
+// products of 16 keys with values go to sums in registers.
 //
 // All stages of keys (64 or 128) of all sequences and heads form one line that the CTAs, three on an SM, take equal shares of, whatever the lengths: a
 // share ends and begins anywhere in a sequence.  What a CTA has of a head that others have parts of goes to scratch, and a second kernel, whose launch
@@ -134,6 +135,15 @@ template <int N> __device__ __forceinline__ void load_pairs(f32x2 (&x)[N], const
             x[2 * k] = v.x; x[2 * k + 1] = v.y;
         }
     } else x[0] = *reinterpret_cast<const f32x2 *>(p);
+}
+
+// Two codes that masks left in halves as numbers, less the middle; `upper`: 16 times the codes of 4 bits
+template <int BITS> __device__ __forceinline__ uint32_t numbers_of(uint32_t codes, bool upper) {
+    constexpr float MIDDLE = BITS == 4 ? 8.f : 128.f;
+    const uint32_t c = codes | 0x64006400u;   // 1024 and that
+    const __half2 v = *reinterpret_cast<const __half2 *>(&c);
+    const __half2 r = BITS == 4 && upper ? __hfma2(v, __float2half2_rn(0.0625f), __float2half2_rn(-64.f - MIDDLE)) : __hsub2(v, __float2half2_rn(1024.f + MIDDLE));
+    return *reinterpret_cast<const uint32_t *>(&r);
 }
 
 // 8 features of a row of queries in 32 bits, `n` of which there are
@@ -288,7 +298,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
     constexpr int DP = 32 * W, ROWS = 8 * NT, SUB = L::SUB, KEYS = L::KEYS;
     constexpr bool WIDE = PARTS == 2;
     constexpr float MIDDLE = BITS == 4 ? 8.f : 128.f;
-    constexpr bool SMALL = WIDE || NG == 1 || BITS == 8;   // sums of scores begin at -M a_g
+    constexpr bool SMALL = WIDE || NG == 1 || BITS == 8;   // sums of scores are less M a_g
     constexpr int ZEROS = NG > 2 && SMALL ? 2 : 1;                 // products that zeros take
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ unsigned room[kFewWarps + 2];
@@ -444,7 +454,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int n = BITS == 4 ? 2 * k + e : 4 * k + e;
-                    const float s = BITS == 4 && e ? 0.0625f : 1.f, y0 = y[n] * by, y1 = y[n + (BITS == 4 ? 4 : 2)] * by;
+                    const float s = BITS == 4 && e && !WIDE ? 0.0625f : 1.f, y0 = y[n] * by, y1 = y[n + (BITS == 4 ? 4 : 2)] * by;
                     const float h0 = __half2float(__float2half_rn(y0)), h1 = __half2float(__float2half_rn(y1));
                     parts[0][2 * k + e] = half2_of(h0 * s, h1 * s);
                     sum += h0 + h1;
@@ -460,14 +470,14 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             if (t == 0) {
-                query_sums[(x * (W + 1) + w) * 8 + g] = sum * 5.9604644775390625e-8f;   // 2^-24, the unit of codes
-                if (w == 0) query_sums[(x * (W + 1) + W) * 8 + g] = fmaxf(P.scale_log2 * power_of_two(127 + 24 - lift), 1.17549435e-38f);
+                query_sums[(x * (W + 1) + w) * 8 + g] = WIDE ? sum : sum * 5.9604644775390625e-8f;   // 2^-24, the unit of codes
+                if (w == 0) query_sums[(x * (W + 1) + W) * 8 + g] = fmaxf(P.scale_log2 * power_of_two(127 + (WIDE ? 0 : 24) - lift), 1.17549435e-38f);
             }
         }
         __syncthreads();
         if (warp == 0 && used == 0) fill(L::kStages);
         uint32_t q[PARTS][NT][W][2][2], qz[NT][ZEROS][2];
-        float start[NT][NG][4], factor[NT][2];   // -M a_g (SMALL); raw scores times the factor are powers of 2
+        float start[NT][NG][4], factor[NT][2];   // -M a_g (SMALL, where codes are not less M already); raw scores times the factor are powers of 2
         int all_lo = S.first, all_hi = S.end;   // keys that all rows see
         auto sees = [&](int x, int e, int &lo, int &hi) {   // those of a row
             const int mine = row0 + 8 * x + 2 * t + e, i = mine < F.rows ? (unsigned)mine % F.by_nq : 0;
@@ -528,7 +538,7 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                     else
 #pragma unroll
                         for (int w = 0; w < W; ++w) a += sums[w * 8 + row];
-                    start[x][k][e] = start[x][k][2 + e] = SMALL ? -MIDDLE * a : 0.f;
+                    start[x][k][e] = start[x][k][2 + e] = SMALL && !WIDE ? -MIDDLE * a : 0.f;
                 }
                 factor[x][e] = sums[W * 8 + row];
                 int lo, hi;
@@ -598,6 +608,10 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                                     const uint32_t c = kw[s][2 * w + k];
                                     a[s] = c & 0x00ff00ffu;
                                     a[2 + s] = (c >> 8) & 0x00ff00ffu;
+                                }
+                                if constexpr (WIDE) {
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e) a[2 * e + s] = numbers_of<BITS>(a[2 * e + s], e);
                                 }
                             }
 #pragma unroll
@@ -843,14 +857,10 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                                     a[2 * s] = c & 0x00ff00ffu;
                                     a[2 * s + 1] = (c >> 8) & 0x00ff00ffu;
                                 }
-                                if constexpr (WIDE)   // codes less the middle, as numbers
+                                if constexpr (WIDE) {
 #pragma unroll
-                                    for (int e = 0; e < 2; ++e) {
-                                        const uint32_t c = a[2 * s + e] | 0x64006400u;   // 1024 + code, for the upper 4 bits 1024 + 16 code
-                                        const __half2 v = *reinterpret_cast<const __half2 *>(&c);
-                                        const __half2 r = BITS == 4 && e ? __hfma2(v, __float2half2_rn(0.0625f), __float2half2_rn(-64.f - MIDDLE)) : __hsub2(v, __float2half2_rn(1024.f + MIDDLE));
-                                        a[2 * s + e] = *reinterpret_cast<const uint32_t *>(&r);
-                                    }
+                                    for (int e = 0; e < 2; ++e) a[2 * s + e] = numbers_of<BITS>(a[2 * s + e], e);
+                                }
                             }
 #pragma unroll
                             for (int x = 0; x < NT; ++x) {
