@@ -152,3 +152,23 @@ def test_float32_scores_of_some_size_keep_their_digits(queries, bits, group):
     want = attended(q, cache, n.tolist(), causal=True)
     assert_near(out, want[0], torch.float32, "out")
     assert_near(lse, want[1], torch.float32, "lse", times=0.125)
+
+
+@pytest.mark.parametrize("bits,group,d", [(4, 32, 128), (4, None, 64), (8, 32, 64), (8, None, 128)])
+def test_long_caches_that_are_attended_to_evenly(bits, group, d):
+    """Results of tens of thousands of about equal terms are hundreds of times smaller than those: the bound of any other float16 call holds for them."""
+    batch, keys, heads = 16, 65536, 8
+    g = torch.Generator(device="cuda").manual_seed(6)
+    cache = tpw.quantized_cache(batch, keys, heads, d, bits=bits, group=group)
+    n = torch.full((batch,), keys, dtype=torch.int32, device="cuda")
+    for b in range(batch):
+        one = tpw.QuantizedCache(*(t[b:b + 1] for t in cache[:4]), d, bits)
+        k, v = (torch.randn(1, keys, heads, d, generator=g, device="cuda") for _ in range(2))
+        tpw.cache_write(one, k, v, n[:1])
+    q = (0.2 * torch.randn(batch, 1, 2 * heads, d, generator=g, device="cuda")).half()
+    out, lse = tpw.cache_attention(q, cache, n, return_lse=True)
+    k, v = (x[0].double() for x in tpw.cache_read(one, n[:1], dtype=torch.float32))
+    for h in range(2 * heads):
+        s = k[:, h // 2] @ q[-1, 0, h].double() * d ** -0.5
+        assert_near(out[-1, 0, h], torch.softmax(s, 0) @ v[:, h // 2], torch.float16, "out")
+        assert_near(lse[-1, h], torch.logsumexp(s, 0, keepdim=True), torch.float32, "lse")

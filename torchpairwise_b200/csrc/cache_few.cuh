@@ -9,7 +9,8 @@
 //            precision's upper end.
 //   output   V^T P^T, 16 features by 8 rows: the steps go into the probabilities, y_jg = p_j step_jg, formed in 32 bits and rounded to half precision
 //            once: sum_j y_jg (c_jd - M) + p_j (zero_jg + M step_jg), M the middle code, so that a rounding counts by how far a value is from its group's
-//            middle.  The second term stays in 32 bits; M sum_j y_jg comes from a product with ones.
+//            middle.  The second term stays in 32 bits; M sum_j y_jg comes from a product with ones, and is taken off every second stage: tensor cores cut sums
+//            off at 24 digits, which over 65536 keys attended to evenly cost 12 times a float16 rounding (35 times in 8 bits; 51.7 -> 52.6 us with it).
 // Steps of one head may be any numbers from 2^-100 to 2^97, and half precision has 40 powers of two: a row of queries has a norm for every group,
 // a power of two that brings the largest y_jg that it met to [4, 8).  So what a row loses (2^-27 of its largest share) depends neither on other groups, nor on
 // other rows, nor on tokens that it gives no weight.  Norms move where references do, or where a step is far above those met.
@@ -876,6 +877,27 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                             }
                         }
                     }
+                }
+            }
+            // M sums of y leave the outputs every second stage, before sums that grow by M with every key have lost what even attention leaves of their differences
+            if constexpr (!WIDE) {
+                if (u % 2) {
+#pragma unroll
+                    for (int x = 0; x < NT; ++x)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                            for (int k = 0; k < NG; ++k) {
+                                const float less = __shfl_sync(0xffffffffu, ones[x][e], 4 * k + t) * (MIDDLE * -5.9604644775390625e-8f);   // 2^-24, as codes
+#pragma unroll
+                                for (int n = 0; n < 2 * W; ++n)
+                                    if (NG == 1 || n / 2 == k) {
+                                        o[x][n][e] += less;
+                                        o[x][n][2 + e] += BITS == 4 ? 16.f * less : less;
+                                    }
+                            }
+                            ones[x][e] = 0.f;
+                        }
                 }
             }
             __syncwarp();
