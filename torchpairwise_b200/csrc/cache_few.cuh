@@ -1120,9 +1120,10 @@ template <int BITS, int W, int NG, int NT, int PARTS> int launch_few(CacheFewPar
 }
 template <int BITS, int W, int NG> int launch_rows(const CacheFewParams &F, void *scratch, long long *bytes, cudaStream_t s) {
     if (F.a.dtype == TPW_F32) return launch_few<BITS, W, NG, 1, 2>(F, scratch, bytes, s);
-    // 8 rows at a time take less than 16 where 16 would leave half of their last block empty: [8, 12345, 8, 128] through a window of 4096, 20 rows 36 us and 39, 32 rows 43 and 42
-    const int blocks = (F.rows + 7) / 8;
-    return blocks == 1 || blocks == 3 ? launch_few<BITS, W, NG, 1, 1>(F, scratch, bytes, s) : launch_few<BITS, W, NG, 2, 1>(F, scratch, bytes, s);
+    // 16 rows at a time unpack the codes half as often, by 8 warps an SM instead of 12, and pay for a last block that is half empty.  Measured 8 / 16 at a time, bfloat16, us:
+    // [8, 12345, 8, 128] through a window of 4096, 4 bits, groups of 32, 16 rows 30.7 / 30.2, 40 rows 55 / 65, 80 rows 97 / 96, 128 rows 147 / 140; one group 26 / 24, 46 / 51, 79 / 74,
+    // 119 / 107; [2, 16384, 8, 128] 22 / 25, 37 / 41, 63 / 64, 91 / 92; [4, 8000, 8, 64] in 8 bits 19 / 17, 35 / 38, 59 / 53, 87 / 77; [1, 1000, 8, 128] 12 / 18, 13 / 18, 16 / 21, 18 / 22.
+    return F.rows <= 80 ? launch_few<BITS, W, NG, 1, 1>(F, scratch, bytes, s) : launch_few<BITS, W, NG, 2, 1>(F, scratch, bytes, s);
 }
 // with `bytes` only says how much scratch the call wants
 template <int BITS> int launch_width(const CacheAttnParams &P, void *scratch, long long *bytes, cudaStream_t s) {
