@@ -174,3 +174,40 @@ def test_a_cache_of_inference_mode():
     with torch.inference_mode():
         tpw.cache_write(cache, x, x, n)
     assert torch.equal(tpw.cache_attention(q, cache, n), inside)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("queries,heads,d", [(10, 8, 128), (9, 18, 64), (41, 4, 96), (48, 8, 128), (12, 32, 64), (60, 12, 40), (100, 8, 20), (70, 8, 33)])
+@pytest.mark.parametrize("bits,group", [(4, 32), (8, None)])
+def test_log_sums_of_rows_that_go_straight_to_the_codes(dtype, queries, heads, d, bits, group):
+    """20 to 400 rows to a key head: up to 192 of them, and all of odd widths, have scores in 32 bits, whatever the type of the queries."""
+    cache = filled(2, 700, 2, d, bits, group, seed=37)
+    q = torch.randn(2, queries, heads, d, generator=torch.Generator().manual_seed(38)).to(dtype).cuda()
+    out, lse = tpw.cache_attention(q, cache, ints(700, 333), causal=True, return_lse=True)
+    want = attended(q, cache, [700, 333], causal=True)
+    assert_near(out, want[0], dtype, "out")
+    assert_near(lse, want[1], torch.float32, "lse")
+
+
+@pytest.mark.parametrize("queries,heads", [(193, 2), (100, 4), (600, 2)])
+@pytest.mark.parametrize("bits,group", [(4, 32), (8, None)])
+def test_log_sums_of_many_bfloat16_rows(queries, heads, bits, group):
+    """More rows go through half precision: codes' values and queries are rounded to it, and log-sums are as good as its rounding."""
+    cache = filled(2, 700, 1, 64, bits, group, seed=39)
+    q = torch.randn(2, queries, heads, 64, generator=torch.Generator().manual_seed(40)).bfloat16().cuda()
+    out, lse = tpw.cache_attention(q, cache, ints(700, 333), causal=True, return_lse=True)
+    want = attended(q, cache, [700, 333], causal=True)
+    assert_near(out, want[0], torch.bfloat16, "out")
+    assert_near(lse, want[1], torch.float16, "lse")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("options", [dict(causal=True), dict(), dict(causal=True, window=70)], ids=str)
+def test_many_rows_with_lengths_beyond_the_capacity_and_below_zero(dtype, options):
+    cache = filled(3, 512, 1, 64, 4, 32, seed=41)
+    q = torch.randn(3, 300, 2, 64, generator=torch.Generator().manual_seed(42)).to(dtype).cuda()
+    want = tpw.cache_attention(q, cache, ints(512, 0, 77), return_lse=True, **options)
+    assert_near(want[0], attended(q, cache, [512, 0, 77], **options)[0], dtype, "out")
+    for n in (ints(1000, -5, 77), ints(2 ** 31 - 1, -2 ** 31, 77), torch.tensor([2 ** 40, -(2 ** 40), 77], device="cuda")):
+        got = tpw.cache_attention(q, cache, n, return_lse=True, **options)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
