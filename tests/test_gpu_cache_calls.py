@@ -211,3 +211,15 @@ def test_many_rows_with_lengths_beyond_the_capacity_and_below_zero(dtype, option
     for n in (ints(1000, -5, 77), ints(2 ** 31 - 1, -2 ** 31, 77), torch.tensor([2 ** 40, -(2 ** 40), 77], device="cuda")):
         got = tpw.cache_attention(q, cache, n, return_lse=True, **options)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+def test_more_key_heads_than_a_grid_has_rows(dtype):
+    some = filled(1, 64, 7, 8, 4, 32, seed=43)
+    heads = 70000
+    pick = torch.arange(heads, device="cuda") % 7
+    cache = tpw.QuantizedCache(*(t[:, pick].contiguous() for t in some[:4]), 8, 4)
+    q = torch.randn(1, 193, 7, 8, generator=torch.Generator().manual_seed(44)).to(dtype).cuda()
+    out = tpw.cache_attention(q[:, :, pick].contiguous(), cache, ints(60), causal=True)
+    want = tpw.cache_attention(q, some, ints(60), causal=True)
+    assert torch.equal(out, want[:, :, pick])

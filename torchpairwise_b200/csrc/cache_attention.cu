@@ -27,12 +27,11 @@ struct Slices {
     explicit Slices(const CacheAttnParams &P) {
         auto round = [](long long bytes) { return (bytes + 255) / 256 * 256; };
         sequence = round(P.c.capacity * P.c.H * P.c.D * 2);
-        // no more than the grid of cache_ranges takes, and no more queries than keys and values
+        // no more queries than keys and values
         const long long asked = P.Nq * P.Hq * P.c.D * 2;
         step = P.c.B;
         if (sequence > 0 && step > kSlice / (2 * sequence)) step = kSlice / (2 * sequence);
         if (step > kSlice / asked) step = kSlice / asked;
-        if (step * P.c.H > 65535) step = 65535 / P.c.H;
         if (step < 1) step = 1;
         const bool wide = P.dtype == TPW_BF16;
         ranges = wide ? round(step * P.c.H * 2 * kRangeParts * 4) : 0;

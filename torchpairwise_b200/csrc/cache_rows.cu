@@ -94,17 +94,17 @@ __device__ __forceinline__ float bring_by(const uint32_t *parts, int to) {
 __device__ __forceinline__ int first_of(int end, int last) { return last > 0 && end > last ? (end - last) & ~127 : 0; }
 // the highest magnitude that the codes of a part of a head's keys (or values), those before first_of left out, can stand for; groups that are not numbers take no part
 __global__ void __launch_bounds__(256) cache_ranges_kernel(const CacheParams P, int last, uint32_t *highest) {
-    const long long bh = blockIdx.y;
-    const int which = blockIdx.z, b = (int)(bh / P.H), cap = (int)P.capacity;
+    const long long bh = blockIdx.x;
+    const int part = blockIdx.y, which = blockIdx.z, b = (int)(bh / P.H), cap = (int)P.capacity;
     int n = P.lengths[b];
     n = n < 0 ? 0 : n < cap ? n : cap;
     const int first = first_of(n, last);
-    const uint32_t *scales = P.scales[which] + (bh * cap + first) * P.groups;
-    const long long count = (long long)(n - first) * P.groups;
+    const unsigned count = (unsigned)(n - first) * P.groups, start = part * 256 + threadIdx.x;   // below 2^32: 2^30 - 64 places, 4 groups
+    const uint32_t *scales = P.scales[which] + (bh * cap + first) * P.groups + start;
     const float most = P.bits == 4 ? 15.f : 255.f;
     uint32_t top = 0;
-    for (long long at = blockIdx.x * 256 + threadIdx.x; at < count; at += kRangeParts * 256) {
-        const float zero = zero_of(scales[at]), end = fmaf(step_of(scales[at]), most, zero), high = fmaxf(fabsf(zero), fabsf(end));
+    for (unsigned left = start < count ? (count - start - 1) / (kRangeParts * 256) + 1 : 0; left > 0; --left, scales += kRangeParts * 256) {
+        const float zero = zero_of(*scales), end = fmaf(step_of(*scales), most, zero), high = fmaxf(fabsf(zero), fabsf(end));
         if (fabsf(zero) <= high && high < 5.0706024009129176e30f) top = max(top, __float_as_uint(high));   // 2^102
     }
     __shared__ uint32_t tops[8];
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(256) cache_ranges_kernel(const CacheParams P, 
     if (threadIdx.x == 0) {
 #pragma unroll
         for (int w = 1; w < 8; ++w) top = max(top, tops[w]);
-        highest[(which * P.B * P.H + bh) * kRangeParts + blockIdx.x] = top;
+        highest[(which * P.B * P.H + bh) * kRangeParts + part] = top;
     }
 }
 // Rows of queries to half precision, times what their keys were divided by; rows of results back.  A thread has 8 features, a block 256 times that.
@@ -386,8 +386,8 @@ int cache_read(const CacheParams &P, const tpw_cache_rows &rows, cudaStream_t s)
 }
 
 int cache_ranges(const CacheParams &P, long long last, uint32_t *highest, cudaStream_t s) {
-    TPW_CHECK_ARG(P.B * P.H < 65536, "tpw_cache_attention: more than 65535 heads of a slice");
-    cache_ranges_kernel<<<dim3(kRangeParts, (unsigned)(P.B * P.H), 2), 256, 0, s>>>(P, (int)(last < P.capacity ? last : 0), highest);
+    TPW_CHECK_ARG(P.B * P.H < (1LL << 31), "tpw_cache_attention: more than 2^31 heads of a slice");
+    cache_ranges_kernel<<<dim3((unsigned)(P.B * P.H), kRangeParts, 2), 256, 0, s>>>(P, (int)(last < P.capacity ? last : 0), highest);
     TPW_LAUNCH_OK("cache_ranges_kernel");
     return TPW_OK;
 }
