@@ -172,3 +172,32 @@ def test_long_caches_that_are_attended_to_evenly(bits, group, d):
         s = k[:, h // 2] @ q[-1, 0, h].double() * d ** -0.5
         assert_near(out[-1, 0, h], torch.softmax(s, 0) @ v[:, h // 2], torch.float16, "out")
         assert_near(lse[-1, h], torch.logsumexp(s, 0, keepdim=True), torch.float32, "lse")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("queries", [1, 5, 40])
+@pytest.mark.parametrize("weight,size", [(6, -6), (10, -9), (20, -12), (10, None), (40, -14), (80, -30)])
+@pytest.mark.parametrize("options", [dict(), dict(causal=True), dict(causal=True, window=333)], ids=str)
+def test_a_first_token_that_takes_the_weight_and_has_small_values(dtype, queries, weight, size, options):
+    """Scores of the first token, and of one in the middle, lie far above the others', its values far below: what the rest adds keeps its digits."""
+    q, k, v, n, cache = scene(7, queries, keys=640)
+    q = q / 2
+    q[..., 0] = 4.0
+    q[:, :, 1:, 0] = 1.0   # and not for every head
+    k[..., 0] = 0.0
+    k[:, [0, 401], :, 0] = weight * 128 ** 0.5 / 4
+    v[:, [0, 401]] *= 0.0 if size is None else 2.0 ** size
+    stored(cache, k, v)
+    q = q.to(dtype)
+    n = torch.tensor([640, 517], dtype=torch.int32, device="cuda")
+    out, lse = tpw.cache_attention(q, cache, n, return_lse=True, **options)
+    want = attended(q, cache, n.tolist(), **options)
+    # The large tokens' scores S have one term of about S among 128, which a sum in 32 bits cuts off by up to 2^-23 S in each of the dozen steps that follow: between two such
+    # tokens (float32 results follow their ratio, 16-bit ones are coarser) that may be 24 * 2^-23 S, or 2^-18.4 S; S / 4 of the type's 2^-17, 2^-19 S, allow two thirds of it.
+    times = 1 + weight / 4 if dtype == torch.float32 else 1
+    for h in range(4):
+        if dtype == torch.float16 and float(want[0][:, :, h].abs().max()) < 2.0 ** -14:   # below which its numbers lie 2^-24 apart
+            assert bool(((out[:, :, h] - want[0][:, :, h]).abs() <= 2.0 ** -25 + 2.0 ** -10 * want[0][:, :, h].abs().max()).all())
+        else:
+            assert_near(out[:, :, h], want[0][:, :, h], dtype, "out", times=times)
+    assert_near(lse, want[1], torch.float32, "lse")

@@ -660,11 +660,11 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                         for (int k = 0; k < NG; ++k) vs[k] = 0;
                 }
                 // References move, norms are looked at and sums are scaled, only where a score has left its reference behind or a step what norms allow
-                bool moves = false;
+                bool loud = false, moves = false;
 #pragma unroll
                 for (int k = 0; k < (NG + 1) / 2; ++k) {
                     const uint32_t steps = __byte_perm(vs[2 * k], 2 * k + 1 < NG ? vs[2 * k + 1 < NG ? 2 * k + 1 : 0] : 0u, 0x5410);
-                    moves = moves || max_halves(steps, limits[k]) != limits[k];
+                    loud = loud || max_halves(steps, limits[k]) != limits[k];
                 }
                 float high[NT][2];
 #pragma unroll
@@ -676,9 +676,10 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                         high[x][e] *= factor[x][e];
                         moves = moves || high[x][e] > m[x][e] + kFewSlack;
                     }
-                moves = __any_sync(0xffffffffu, moves);
+                moves = __any_sync(0xffffffffu, moves || loud);
                 float up[NT][2];   // of references
                 if (moves) {
+                    loud = __any_sync(0xffffffffu, loud);
 #pragma unroll
                     for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -686,9 +687,18 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                             float top = high[x][e];
 #pragma unroll
                             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                            top = fmaxf(top, m[x][e]);
-                            up[x][e] = top == m[x][e] ? 0.f : top - m[x][e];
-                            m[x][e] = top;
+                            float now = fmaxf(top, m[x][e]);
+                            // Steps are large beside what norms allow, which reckon with scores like the highest.  Where one token takes the weight and has small
+                            // values all others would be: the reference comes down to these keys' scores, so far that the sum of probabilities stays below about 2^24.
+                            if (loud) {   // (of the whole warp: so are the exchanges)
+                                float sum = l[x][e];
+#pragma unroll
+                                for (int d = 4; d < 32; d <<= 1) sum = fmaxf(sum, __shfl_xor_sync(0xffffffffu, sum, d));
+                                const int room = 24 + 127 - (int)(__float_as_uint(sum) >> 23);
+                                if (top > -INFINITY) now = fmaxf(top, m[x][e] - (room < 0 ? 0.f : room > 24 ? 24.f : (float)room));
+                            }
+                            up[x][e] = now == m[x][e] ? 0.f : now - m[x][e];
+                            m[x][e] = now;
                             l[x][e] *= exp2_fast(-up[x][e]);
                         }
                 }
@@ -757,8 +767,8 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                             }
 #pragma unroll
                             for (int k = 0; k < NG; ++k) {
-                                // up by what the reference went up; down so far that the largest y of these keys is below 8
-                                const int high = min(was[e][k] + (int)fminf(up[x][e], 1024.f), kFewHighest), now = max(min(high, 129 - (int)(__float_as_uint(top[e][k]) >> 23)), -kFewHighest);
+                                // up or down with the reference; down so far that the largest y of these keys is below 8
+                                const int high = min(was[e][k] + (int)floorf(fminf(up[x][e], 1024.f)), kFewHighest), now = max(min(high, 129 - (int)(__float_as_uint(top[e][k]) >> 23)), -kFewHighest);
                                 if (g == 0) norm[e * NP + k] = power_of_two(127 + now);
                                 // steps below 2^7 over the norm: y stays below 2^15
                                 if (m[x][e] > -INFINITY) allowed[k] = min(allowed[k], (uint32_t)((134 - now) << 7) - 1);
