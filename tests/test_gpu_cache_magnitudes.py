@@ -4,7 +4,7 @@ import torch
 
 import torchpairwise_b200 as tpw
 from attention_cases import assert_near
-from cache_cases import attended
+from cache_cases import attended, values
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -201,3 +201,22 @@ def test_a_first_token_that_takes_the_weight_and_has_small_values(dtype, queries
         else:
             assert_near(out[:, :, h], want[0][:, :, h], dtype, "out", times=times)
     assert_near(lse, want[1], torch.float32, "lse")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("queries", [1, 30])
+def test_scores_near_the_top(dtype, queries):
+    """Scores of millions, where 32 bits hold them to a unit: finite results, of the keys that have the highest."""
+    q, k, v, n, cache = scene(8, queries, keys=640)
+    k[..., 0] = 0.0
+    k[:, 100::7, :, 0] = 3000.0   # all the same: kept exactly, as the highest of their groups
+    k[:, 100::7, :, 1:] = 0.0
+    v = v * torch.exp2(torch.randint(-6, 7, v.shape[:2], generator=torch.Generator().manual_seed(9)).float()).cuda()[..., None, None]
+    stored(cache, k, v)
+    q[..., 0] = 40000.0 if dtype == torch.float16 else 60000.0
+    q = q.to(dtype)
+    out = tpw.cache_attention(q, cache, n)
+    for b, length in enumerate(n.tolist()):
+        want = values(cache)[1][b, 100:length:7].mean(0)   # [heads, features]
+        for h in range(4):
+            assert_near(out[b, :, h], want[h // 2].expand(queries, -1), dtype, "out")

@@ -770,8 +770,8 @@ __global__ void __launch_bounds__(kFewThreads, CacheFew<BITS, W, NG, NT, PARTS>:
                                 // up or down with the reference; down so far that the largest y of these keys is below 8
                                 const int high = min(was[e][k] + (int)floorf(fminf(up[x][e], 1024.f)), kFewHighest), now = max(min(high, 129 - (int)(__float_as_uint(top[e][k]) >> 23)), -kFewHighest);
                                 if (g == 0) norm[e * NP + k] = power_of_two(127 + now);
-                                // steps below 2^7 over the norm: y stays below 2^15
-                                if (m[x][e] > -INFINITY) allowed[k] = min(allowed[k], (uint32_t)((134 - now) << 7) - 1);
+                                // steps below 2^6 over the norm: y stays below 2^14, and twice that where scores near 2^24 are a unit off
+                                if (m[x][e] > -INFINITY) allowed[k] = min(allowed[k], (uint32_t)((133 - now) << 7) - 1);
                                 const float scale = by * power_of_two(127 + now - was[e][k]);
                                 if (g == k) ones[x][e] *= scale;
 #pragma unroll
