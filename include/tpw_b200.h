@@ -692,7 +692,8 @@ TPW_API int tpw_cache_read(const tpw_cache *c, const tpw_cache_rows *rows, tpw_s
 
 /*
  * Attention as tpw_attention_forward defines it, with the keys and values that the cache stands for.  Scores, statistics and sums are held
- * in 32 bits; with float32 queries nothing is rounded to fewer.
+ * in 32 bits, operands of products in fewer: a probability times the step of a value in half precision (float32 queries: in two such parts, as queries are); with more than 192 rows of
+ * 16-bit queries to a key head probabilities and what codes stand for in half precision (float16: up to 65504; bfloat16: under a power of two of the head).
  */
 typedef struct tpw_cache_attention_args {
     int32_t dtype;            /* of q and out: TPW_F32, TPW_F16, TPW_BF16 */

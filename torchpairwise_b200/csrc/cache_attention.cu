@@ -2,7 +2,8 @@
 //
 // Few query rows to a key head read the codes as they lie (cache_few.cuh).  Many make attention a matter of matrix products, and there each key tile is
 // read by many tiles of queries: keys and values are turned into half precision once, into scratch, and go through the kernels of
-// attention.  Scratch is bounded: sequences go a few at a time, 128 MB of keys and values or one sequence, so that L2 holds most of what was just written.
+// attention.  Sequences go a few at a time, 128 MB of keys and values or one sequence, so that L2 holds most of what was just written; for bfloat16 there are
+// queries and results of as many beside them.  Both scratch and the grids that fill it follow the capacity, not the lengths: short sequences in a large capacity pay for it.
 // Half precision also for bfloat16 queries: what codes stand for has more than bfloat16's 8 digits, and keys rounded to them made the results 2.4 times as
 // far off (chunk of 256 on 16384 keys: 0.0041 against 0.0017).  Its exponents do not reach, so each head's keys and values, and the queries and results
 // with them, are moved by a power of two.
@@ -71,8 +72,10 @@ tpw_attention slice(const CacheAttnParams &P, const Slices &S, void *scratch, lo
     return a;
 }
 
-// Measured (bfloat16, 4 bits, [2, 16384, 8, 128] ragged): 192 rows 103 us as few and 132 as many, 256 rows 130 and 133, 512 rows 239 and 141; [8, 4096, 8, 128] the same; [1, 1000]
-// 31 and 25 at 192.  Float32 stays: [2, 8192, 8, 128] 512 rows 263 and 821 us, [2, 8192, 8, 64] 1024 rows 302 and 325.
+// Measured (bfloat16, us, as few and as many): [2, 16384, 8, 128] ragged, 4 bits, 192 rows 124 / 117, 224 rows 139 / 117, 256 rows 156 / 118; [4, 8000, 8, 64] in 8 bits 192 rows 108 / 105, 224 rows
+// 123 / 105; [1, 1000, 8, 128] 224 rows 29 / 35; [8, 12345, 8, 128] through a window of 4096, 224 rows 229 / 333 (the capacity counts), 256 rows 257 / 336.
+// Float32 stays: 512 rows [2, 8192, 8, 128] 263 us, 821 through attention's float32 kernels; where the times meet, 1024 rows [2, 8192, 8, 64] 302 and 325, was the last
+// measurement, so that for prompts of thousands of rows the few-row kernel, whose time grows with them, is the slower one.
 bool is_few(const CacheAttnParams &P) {
     if (P.dtype == TPW_F32 || P.group * P.Nq <= 192) return true;
     const tpw_attention a = slice(P, Slices(P), reinterpret_cast<void *>(256), 0, 1);   // of the scratch only its alignment takes part

@@ -27,8 +27,8 @@
 // overlaps this one, weighs the parts together in their order.  In a CTA four warps take 16 keys or 32 of a stage each, with a running reference, sum and
 // output of their own; bulk copies bring the stages into a ring, across the ends of heads.
 //
-// Measured bfloat16, 4 bits: [16, 1 x 16384, 32/8, 128] ragged, groups of 32, 185 MB in 51 us (3.6 TB/s), of which copies alone take 31;
-// [64, 1 x 4096, 32/8, 128], one group, 158 MB in 45 us.  Norms by row and group cost 4 and 1 us of that against one power of two for all steps of a warp, which
+// Measured bfloat16, 4 bits: [16, 1 x 16384, 32/8, 128] ragged, groups of 32, 185 MB in 52 us (3.6 TB/s), of which copies alone take 31;
+// [64, 1 x 4096, 32/8, 128], one group, 158 MB in 46 us.  Norms by row and group cost 4 and 1 us of that against one power of two for all steps of a warp, which
 // leaves groups beside a loud one, and tokens beside a loud token, without digits: 1.5 us the look at them at the beginning of a head, the rest products in 32 bits.
 #pragma once
 #include "attention_tc.cuh"

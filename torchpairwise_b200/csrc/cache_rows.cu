@@ -1,6 +1,7 @@
 // Tokens into a cache of quantised keys and values, and out of it.
 //
-// Bound by HBM on paper, by issue in fact: storing takes about 16 instructions a value.  What keeps them few: a lane has a group's 32 values, quotients are refined on the FMA
+// Bound by HBM on paper.  Storing waits for its loads first (5.5 warps of those that wait, 28 % of DRAM: a block asks for its sequence's length before its values, has one token a lane, and
+// ends), and takes about 21 instructions a value, 64 % of the issue slots.  What keeps them few: a lane has a group's 32 values, quotients are refined on the FMA
 // pipes (a test for middles on the logic pipe was 10 more), codes are added up above a constant instead of masked and shifted, and bytes become numbers by
 // permutation.  Measured bfloat16, 4 bits: 2 x 8192 tokens of 8 heads of 128, 67 MB stored and read back in 43 us; 4 x 16384 ragged read in 53 us, 5.9 TB/s.
 #include "attention_tc.cuh"
