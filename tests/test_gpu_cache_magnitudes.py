@@ -220,3 +220,20 @@ def test_scores_near_the_top(dtype, queries):
         want = values(cache)[1][b, 100:length:7].mean(0)   # [heads, features]
         for h in range(4):
             assert_near(out[b, :, h], want[h // 2].expand(queries, -1), dtype, "out")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("queries", [1, 5, 250])
+@pytest.mark.parametrize("bits,group", [(4, 32), (4, None), (8, 32), (8, None)])
+def test_values_that_are_zero_stay_zero(dtype, queries, bits, group):
+    """Groups of zeros have a step all the same (2^-100): what is all zeros gives zeros, to the last bit."""
+    q, k, v, n, cache = scene(9, queries, bits=bits, group=group)
+    stored(cache, k, torch.zeros_like(v))
+    q = q.to(dtype)
+    assert not tpw.cache_attention(q, cache, n, causal=True).any()
+    if group:
+        v[..., 32:64] = 0
+        stored(cache, k, v)
+        out = tpw.cache_attention(q, cache, n, causal=True)
+        assert not out[..., 32:64].any()
+        assert_near(out, attended(q, cache, n.tolist(), causal=True)[0], dtype, "out")

@@ -128,7 +128,7 @@ def cache_attention(q: Tensor, cache: QuantizedCache, key_lengths: Tensor, *, ca
     as the capacity.  What lies in the cache from a sequence's length on is never used.  Within it, what is not a number makes the rows of its
     tile NaN.  Not differentiable.
 
-    Scores are to stay below 2^24 and results below 2^90 in magnitude, as are queries.  Scores, statistics and sums are held in 32 bits, and a query to 2^-39 of
+    Scores are to stay below 2^24 and results below 2^90 in magnitude, as are queries; results below 2^-104 may be given as zero.  Scores, statistics and sums are held in 32 bits, and a query to 2^-39 of
     the highest magnitude of its row.  Operands of products have fewer: with 16-bit queries a probability times the step of a value is rounded to half precision
     (2^-12 of it, 2^-27 of the largest that its row met in the group), with float32 queries it and the query are two such parts (2^-23).  With more than 192 16-bit queries to
     a key head (their number times the heads that share one; widths that are multiples of 8) the probabilities and what the codes stand for are rounded to half precision: up to 65504 for float16; for

@@ -206,7 +206,11 @@ __device__ __forceinline__ void finish(const CacheFewParams &F, int b, int hk, i
     const int over = (unsigned)r / F.by_nq, i = r - over * (int)P.Nq, h = (int)(hk * P.group) + over;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] *= inv;
+    for (int e = 0; e < 4; ++e) {
+        v[e] *= inv;
+        // A group of zeros has a step all the same, 2^-100, and M steps do not go without a rest, up to 2^-12 of them: below 2^-104 there is nothing else
+        if (fabsf(v[e]) < 4.930380657631324e-32f) v[e] = 0.f;
+    }
     if (d == 0 && P.lse) P.lse[(b * P.Hq + h) * P.Nq + i] = sum == 0.f ? -INFINITY : (reference + log2f(sum)) * 0.69314718055994531f;
     store_out(P, ((b * P.Nq + i) * P.Hq + h) * P.c.D + d, v, P.c.D - d);
 }
